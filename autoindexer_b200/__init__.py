@@ -19,9 +19,12 @@ from .meta import CompiledLayout, RowLayouts, compile_layout
 from .positions import (BlockType, PositionBlock, PositionBlockList, blocks_from_concat, cursor_stream,
                         document_blocks, positions_from_operations)
 from .decode import decode_attention
+from .head_norm import qk_norm_rope
 from .index_head import compute_index_losses_b200
+from .paged import paged_append, shared_prefix_attention
 from .prefill import plain_causal_attn_b200, prefill_attention_interface, prefill_layout
-from .rope import SectionedRope, default_inv_freq
+from .rope import SectionedRope, default_inv_freq, rope_table
+from .verify import verify_draft
 
 __all__ = [
     "B200_ATTN_KEY",
@@ -48,4 +51,9 @@ __all__ = [
     "prefill_layout",
     "SectionedRope",
     "default_inv_freq",
+    "rope_table",
+    "qk_norm_rope",
+    "paged_append",
+    "shared_prefix_attention",
+    "verify_draft",
 ]

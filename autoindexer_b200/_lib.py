@@ -31,7 +31,8 @@ LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "_ai_attn.so
 
 DTYPE_BF16, DTYPE_F16, DTYPE_F32 = 0, 1, 2
 # AiProfKind, in order.
-PROF_KINDS = ("prerot", "fwd", "fwd_fill", "delta", "dq", "dkdv", "bwd_fill", "simt", "decode")
+PROF_KINDS = ("prerot", "fwd", "fwd_fill", "delta", "dq", "dkdv", "bwd_fill", "simt", "decode", "head_norm",
+              "append", "prefix", "verify")
 ABI_VERSION = 9
 BWD_DQ, BWD_DKDV = 1, 2
 
@@ -60,6 +61,14 @@ EXPORTED_SYMBOLS = (
     "ai_index_bwd",
     "ai_index_rows_sizes",
     "ai_index_rows",
+    "ai_head_norm_fwd",
+    "ai_head_norm_bwd_workspace",
+    "ai_head_norm_bwd",
+    "ai_paged_append",
+    "ai_prefix_attn_workspace",
+    "ai_prefix_attn",
+    "ai_verify_draft_workspace",
+    "ai_verify_draft",
 )
 
 _i32p = ctypes.POINTER(ctypes.c_int32)
@@ -274,6 +283,136 @@ class AiPrepTables(ctypes.Structure):
     ]
 
 
+class AiPositions(ctypes.Structure):
+    _fields_ = [
+        ("ptr", ctypes.c_void_p),
+        ("stride_b", ctypes.c_int64),
+        ("is_int64", ctypes.c_int32),
+    ]
+
+
+class AiHeadNormArgs(ctypes.Structure):
+    _fields_ = [
+        ("batch", ctypes.c_int32),
+        ("seq_len", ctypes.c_int32),
+        ("num_q_heads", ctypes.c_int32),
+        ("num_kv_heads", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("weight_dtype", ctypes.c_int32),
+        ("eps", ctypes.c_float),
+        ("q", AiTensor4),
+        ("k", AiTensor4),
+        ("q_out", AiTensor4),
+        ("k_out", AiTensor4),
+        ("q_weight", ctypes.c_void_p),
+        ("k_weight", ctypes.c_void_p),
+        ("rope_cos", ctypes.c_void_p),
+        ("rope_sin", ctypes.c_void_p),
+        ("n_pos", ctypes.c_int32),
+        ("pos", AiPositions),
+        ("status", ctypes.c_void_p),
+    ]
+
+
+class AiHeadNormBwdArgs(ctypes.Structure):
+    _fields_ = [
+        ("fwd", AiHeadNormArgs),
+        ("dq_out", AiTensor4),
+        ("dk_out", AiTensor4),
+        ("dq", AiTensor4),
+        ("dk", AiTensor4),
+        ("dq_weight", ctypes.c_void_p),
+        ("dk_weight", ctypes.c_void_p),
+        ("workspace", ctypes.c_void_p),
+        ("workspace_bytes", ctypes.c_size_t),
+    ]
+
+
+class AiPagedAppendArgs(ctypes.Structure):
+    _fields_ = [
+        ("batch", ctypes.c_int32),
+        ("seq_len", ctypes.c_int32),
+        ("num_kv_heads", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("weight_dtype", ctypes.c_int32),
+        ("eps", ctypes.c_float),
+        ("k", AiTensor4),
+        ("v", AiTensor4),
+        ("k_pages", AiTensor4),
+        ("v_pages", AiTensor4),
+        ("n_pages", ctypes.c_int32),
+        ("page_size", ctypes.c_int32),
+        ("page_table", ctypes.c_void_p),
+        ("page_table_stride", ctypes.c_int64),
+        ("max_pages", ctypes.c_int32),
+        ("lens", ctypes.c_void_p),
+        ("new_lens", ctypes.c_void_p),
+        ("k_weight", ctypes.c_void_p),
+        ("rope_cos", ctypes.c_void_p),
+        ("rope_sin", ctypes.c_void_p),
+        ("n_pos", ctypes.c_int32),
+        ("pos", AiPositions),
+        ("status", ctypes.c_void_p),
+    ]
+
+
+class AiPrefixAttnArgs(ctypes.Structure):
+    _fields_ = [
+        ("batch", ctypes.c_int32),
+        ("seq_len", ctypes.c_int32),
+        ("num_q_heads", ctypes.c_int32),
+        ("num_kv_heads", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("scale", ctypes.c_float),
+        ("q", AiTensor4),
+        ("out", AiTensor4),
+        ("lse", ctypes.c_void_p),
+        ("k_pages", AiTensor4),
+        ("v_pages", AiTensor4),
+        ("n_pages", ctypes.c_int32),
+        ("page_size", ctypes.c_int32),
+        ("prefix_pages", ctypes.c_void_p),
+        ("prefix_len", ctypes.c_int32),
+        ("page_table", ctypes.c_void_p),
+        ("page_table_stride", ctypes.c_int64),
+        ("max_pages", ctypes.c_int32),
+        ("lens", ctypes.c_void_p),
+        ("query_lens", ctypes.c_void_p),
+        ("status", ctypes.c_void_p),
+        ("workspace", ctypes.c_void_p),
+        ("workspace_bytes", ctypes.c_size_t),
+    ]
+
+
+class AiVerifyArgs(ctypes.Structure):
+    _fields_ = [
+        ("batch", ctypes.c_int32),
+        ("n_draft", ctypes.c_int32),
+        ("vocab", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("target", ctypes.c_void_p),
+        ("target_stride_b", ctypes.c_int64),
+        ("target_stride_t", ctypes.c_int64),
+        ("draft", ctypes.c_void_p),
+        ("draft_stride_b", ctypes.c_int64),
+        ("draft_stride_t", ctypes.c_int64),
+        ("tokens", ctypes.c_void_p),
+        ("uniforms", ctypes.c_void_p),
+        ("noise", ctypes.c_void_p),
+        ("temperature", ctypes.c_void_p),
+        ("draft_lens", ctypes.c_void_p),
+        ("accepted", ctypes.c_void_p),
+        ("out_tokens", ctypes.c_void_p),
+        ("logprobs", ctypes.c_void_p),
+        ("status", ctypes.c_void_p),
+        ("workspace", ctypes.c_void_p),
+        ("workspace_bytes", ctypes.c_size_t),
+    ]
+
+
 _lock = threading.Lock()
 _lib = None
 
@@ -327,6 +466,18 @@ def _bind(handle):
     handle.ai_index_rows_sizes.argtypes = [P(AiPrepList), vp, P(i32), P(i64), vp]
     handle.ai_index_rows.restype = ctypes.c_int
     handle.ai_index_rows.argtypes = [P(AiPrepList), vp, i64, P(AiIndexRowsOut)]
+    for name, args in (("ai_head_norm_fwd", AiHeadNormArgs), ("ai_head_norm_bwd", AiHeadNormBwdArgs),
+                       ("ai_paged_append", AiPagedAppendArgs), ("ai_prefix_attn", AiPrefixAttnArgs),
+                       ("ai_verify_draft", AiVerifyArgs)):
+        fn = getattr(handle, name)
+        fn.restype = ctypes.c_int
+        fn.argtypes = [P(args), vp]
+    for name, args in (("ai_head_norm_bwd_workspace", AiHeadNormBwdArgs),
+                       ("ai_prefix_attn_workspace", AiPrefixAttnArgs),
+                       ("ai_verify_draft_workspace", AiVerifyArgs)):
+        fn = getattr(handle, name)
+        fn.restype = ctypes.c_int
+        fn.argtypes = [P(args), P(ctypes.c_size_t)]
     return handle
 
 

@@ -1,0 +1,137 @@
+// New keys and values into the paged cache (declared in include/ai_attn.h):
+// keys normalised and rotated on the way, values copied, straight from the
+// projections' layout to each token's slot.
+//
+// A row of D elements sits in D / 16 lanes (ai_head_row.cuh); a warp takes a
+// few heads of one token, K rows and V rows alike, so the token's page and
+// its angles are looked up once per item.  HBM-bound (each row moves in and
+// out once); with one token per sequence it is a launch latency.
+
+#include <cuda_runtime.h>
+
+#include <cstring>
+
+#include "ai_head_row.cuh"
+#include "ai_kernels.h"
+
+namespace ai {
+namespace append {
+
+using namespace headrow;
+
+constexpr int kWarps = 4;
+constexpr int kThreads = 32 * kWarps;
+
+template <typename T, int D, bool kVec>
+__global__ void __launch_bounds__(kThreads) append_kernel(const AiPagedAppendArgs a, const int per, const int chunks,
+                                                          const int64_t items) {
+  constexpr int kLanes = D / 16, kRows = 32 / kLanes;
+  const int lane = threadIdx.x % 32, sub = lane / kLanes, l = lane % kLanes;
+  const int64_t it = (int64_t)blockIdx.x * kWarps + threadIdx.x / 32;
+  if (it >= items) return;
+  const int64_t tok = it / chunks, b = tok / a.seq_len;
+  const int t = (int)(tok % a.seq_len);
+  if (t >= (a.new_lens ? min(__ldg(a.new_lens + b), a.seq_len) : a.seq_len)) return;
+  const int64_t n = (int64_t)__ldg(a.lens + b) + t;
+  int page = -1;
+  if (n >= 0 && n / a.page_size < a.max_pages) page = __ldg(a.page_table + b * a.page_table_stride + n / a.page_size);
+  if (page < 0 || page >= a.n_pages) {
+    report(a.status, AI_ERR_DEV_BOUNDS);
+    return;
+  }
+  const int64_t slot = n % a.page_size;
+  const int h0 = (int)(it % chunks) * per, h1 = min(a.num_kv_heads, h0 + per);
+  const T* k = static_cast<const T*>(a.k.ptr) + b * a.k.stride_b + t * a.k.stride_t + 8 * l;
+  const T* v = static_cast<const T*>(a.v.ptr) + b * a.v.stride_b + t * a.v.stride_t + 8 * l;
+  T* ko = static_cast<T*>(a.k_pages.ptr) + page * a.k_pages.stride_b + slot * a.k_pages.stride_t + 8 * l;
+  T* vo = static_cast<T*>(a.v_pages.ptr) + page * a.v_pages.stride_b + slot * a.v_pages.stride_t + 8 * l;
+  float wlo[8], whi[8], cs[8], sn[8];
+  int64_t row = 0;
+  if (a.rope_cos) row = table_row(a.pos, b, t, a.n_pos, a.status);
+  load_angles(a.rope_cos, a.rope_sin, row, D / 2, l, cs, sn);
+  load_weight<T>(a.k_weight, a.weight_dtype == AI_DTYPE_F32, D, l, wlo, whi);
+  for (int hb = h0; hb < h1; hb += kRows) {
+    const int64_t h = min(hb + sub, h1 - 1);  // (rows past the last head repeat it, unstored)
+    const Raw8<T> klo = load8<T, kVec>(k + h * a.k.stride_h), khi = load8<T, kVec>(k + h * a.k.stride_h + D / 2);
+    const Raw8<T> vlo = load8<T, kVec>(v + h * a.v.stride_h), vhi = load8<T, kVec>(v + h * a.v.stride_h + D / 2);
+    float flo[8], fhi[8];
+    unpack(klo, flo);
+    unpack(khi, fhi);
+    if (a.k_weight) {
+      const float r = inv_rms<D>(flo, fhi, a.eps);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) flo[i] *= r * wlo[i], fhi[i] *= r * whi[i];
+    }
+    rotate(flo, fhi, cs, sn);
+    if (hb + sub < h1) {
+      store8<T, kVec>(ko + h * a.k_pages.stride_h, pack<T>(flo));
+      store8<T, kVec>(ko + h * a.k_pages.stride_h + D / 2, pack<T>(fhi));
+      store8<T, kVec>(vo + h * a.v_pages.stride_h, vlo);
+      store8<T, kVec>(vo + h * a.v_pages.stride_h + D / 2, vhi);
+    }
+  }
+}
+
+int check(const AiPagedAppendArgs* a) {
+  if (!a) return AI_ERR_NULL;
+  if (a->batch <= 0 || a->seq_len <= 0 || a->num_kv_heads <= 0 || a->n_pages <= 0 || a->page_size <= 0 ||
+      a->max_pages <= 0)
+    return AI_ERR_SHAPE;
+  if (a->head_dim != 32 && a->head_dim != 64 && a->head_dim != 128) return AI_ERR_HEAD_DIM;
+  if (a->dtype != AI_DTYPE_BF16 && a->dtype != AI_DTYPE_F16 && a->dtype != AI_DTYPE_F32) return AI_ERR_DTYPE;
+  if (a->weight_dtype != a->dtype && a->weight_dtype != AI_DTYPE_F32) return AI_ERR_DTYPE;
+  for (const AiTensor4* t : {&a->k, &a->v, &a->k_pages, &a->v_pages}) {
+    if (!t->ptr) return AI_ERR_NULL;
+    if (t->stride_b < 0 || t->stride_h < 0 || t->stride_t < 0) return AI_ERR_STRIDE;
+  }
+  if (!a->page_table || !a->lens) return AI_ERR_NULL;
+  if (a->page_table_stride < 0) return AI_ERR_STRIDE;
+  if ((a->rope_cos != nullptr) != (a->rope_sin != nullptr)) return AI_ERR_NULL;
+  if (a->rope_cos) {
+    if (!a->pos.ptr) return AI_ERR_NULL;
+    if (a->n_pos <= 0) return AI_ERR_SHAPE;
+    if (a->pos.stride_b < 0) return AI_ERR_STRIDE;
+    if ((reinterpret_cast<uintptr_t>(a->rope_cos) | reinterpret_cast<uintptr_t>(a->rope_sin)) & 15)
+      return AI_ERR_ALIGN;
+  }
+  return AI_OK;
+}
+
+template <typename T, int D>
+int launch(const AiPagedAppendArgs& a, cudaStream_t st) {
+  // One row group per item while that gives every SM at most a few warps;
+  // then a token's heads stay together.
+  constexpr int kRows = 32 / (D / 16);
+  const int64_t tokens = (int64_t)a.batch * a.seq_len;
+  const int per = tokens <= 4096 ? (kRows < a.num_kv_heads ? kRows : a.num_kv_heads) : a.num_kv_heads;
+  const int chunks = (a.num_kv_heads + per - 1) / per;
+  const int64_t items = tokens * chunks, blocks = (items + kWarps - 1) / kWarps;
+  if (blocks > 0x7fffffff) return AI_ERR_SHAPE;
+  const bool vec = rows_aligned(a.k, a.dtype) && rows_aligned(a.v, a.dtype) && rows_aligned(a.k_pages, a.dtype) &&
+                   rows_aligned(a.v_pages, a.dtype);
+  ProfScope ps(AI_PROF_APPEND, st);
+  if (vec)
+    append_kernel<T, D, true><<<(unsigned)blocks, kThreads, 0, st>>>(a, per, chunks, items);
+  else
+    append_kernel<T, D, false><<<(unsigned)blocks, kThreads, 0, st>>>(a, per, chunks, items);
+  return cudaGetLastError() == cudaSuccess ? AI_OK : AI_ERR_LAUNCH;
+}
+
+template <typename T>
+int dispatch(const AiPagedAppendArgs& a, cudaStream_t st) {
+  if (a.head_dim == 128) return launch<T, 128>(a, st);
+  if (a.head_dim == 64) return launch<T, 64>(a, st);
+  return launch<T, 32>(a, st);
+}
+
+}  // namespace append
+}  // namespace ai
+
+extern "C" int ai_paged_append(const AiPagedAppendArgs* args, void* stream) {
+  const int rc = ai::append::check(args);
+  if (rc != AI_OK) return rc;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (args->dtype == AI_DTYPE_BF16) return ai::append::dispatch<__nv_bfloat16>(*args, st);
+  if (args->dtype == AI_DTYPE_F16) return ai::append::dispatch<__half>(*args, st);
+  return ai::append::dispatch<float>(*args, st);
+}

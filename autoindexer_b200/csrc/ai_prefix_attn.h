@@ -1,0 +1,41 @@
+// Shared by the kernels of the shared-prefix attention.
+#pragma once
+
+#include <stdint.h>
+
+#include "../../include/ai_attn.h"
+#include "ai_common.cuh"
+
+namespace ai {
+namespace prefix {
+
+// Own keys of a sequence (clamped to what its page table can hold) and its
+// real query tokens.
+struct Lens {
+  int keys, n;
+};
+
+__device__ __forceinline__ Lens seq_lens(const AiPrefixAttnArgs& a, int64_t b) {
+  Lens r;
+  r.keys = __ldg(a.lens + b);
+  r.n = a.query_lens ? __ldg(a.query_lens + b) : a.seq_len;
+  if (r.keys < 0 || r.keys > a.max_pages * a.page_size || r.n < 0 || r.n > a.seq_len) {
+    report(a.status, AI_ERR_DEV_BOUNDS);
+    r.keys = max(0, min(r.keys, a.max_pages * a.page_size));
+    r.n = max(0, min(r.n, a.seq_len));
+  }
+  return r;
+}
+
+// Page i of a table; a page outside the pool is reported and read as page 0.
+__device__ __forceinline__ int page_of(const AiPrefixAttnArgs& a, const int32_t* table, int64_t i) {
+  const int p = __ldg(table + i);
+  if (p < 0 || p >= a.n_pages) {
+    report(a.status, AI_ERR_DEV_BOUNDS);
+    return 0;
+  }
+  return p;
+}
+
+}  // namespace prefix
+}  // namespace ai

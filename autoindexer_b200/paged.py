@@ -1,0 +1,166 @@
+"""The paged key / value cache: appending to it and attending over it.
+
+Keys and values live in pools of pages ``(n_pages, Hkv, page_size, D)``; a
+sequence's tokens are the slots of the pages its row of ``page_table`` lists,
+and a batch may share a prefix whose pages are listed once.  All lengths and
+tables are device tensors, nothing synchronises, and the calls can be captured
+in a CUDA graph (the page tables' width and ``prefix_len`` fix the launch).
+
+Keys are stored as the scores use them: ``paged_append`` normalises and
+rotates them on the way in.
+"""
+
+from __future__ import annotations
+
+from typing import Optional, Tuple
+
+import torch
+from torch import Tensor
+
+from . import _call, _lib
+from .attention import status_word
+
+__all__ = ["paged_append", "shared_prefix_attention"]
+
+
+def _pools(k_pages: Tensor, v_pages: Tensor, heads: int, head_dim: int, dtype, device) -> None:
+    if k_pages.dim() != 4 or k_pages.shape != v_pages.shape or k_pages.shape[1] != heads or k_pages.shape[3] != head_dim:
+        raise ValueError(f"k_pages and v_pages must be (n_pages, {heads}, page_size, {head_dim}), got "
+                         f"{tuple(k_pages.shape)} and {tuple(v_pages.shape)}")
+    for name, p in (("k_pages", k_pages), ("v_pages", v_pages)):
+        if p.dtype != dtype:
+            raise TypeError(f"{name} is {p.dtype}, the call's tensors {dtype}")
+        if p.stride(3) != 1:
+            raise ValueError(f"{name} must have a contiguous last dimension")
+        if p.numel() == 0:
+            raise ValueError(f"{name} is empty")
+        _call.on_device(name, p, device)
+
+
+def _table(page_table: Tensor, batch: int, device) -> Tensor:
+    if page_table.dim() != 2:
+        raise ValueError(f"page_table must be ({batch}, max_pages), got {tuple(page_table.shape)}")
+    return _call.ints("page_table", page_table, (batch, page_table.shape[1]), device)
+
+
+def paged_append(key: Tensor, value: Tensor, k_pages: Tensor, v_pages: Tensor, page_table: Tensor, lens: Tensor,
+                 rope: Optional[Tuple[Tensor, Tensor]] = None, positions: Optional[Tensor] = None,
+                 new_lens: Optional[Tensor] = None, key_weight: Optional[Tensor] = None, eps: float = 1e-6) -> None:
+    """Writes new tokens into the cache, in place.
+
+    ``key`` and ``value`` ``(B, Hkv, T, D)``: token ``t < new_lens[b]`` (all
+    ``T`` without it) becomes sequence ``b``'s token ``lens[b] + t``, in slot
+    ``n % page_size`` of page ``page_table[b, n // page_size]``.  ``lens``
+    ``(B,)`` int32 counts the tokens a sequence holds already and is not
+    changed.  ``key_weight`` (``(D,)``) normalises each key row as
+    ``qk_norm_rope`` does, ``rope`` / ``positions`` rotate it (as there).
+    ``page_table`` ``(B, max_pages)`` int32; a token whose page lies outside
+    it or outside the pool is dropped and sets the status word.  CUDA tensors
+    of one dtype (bfloat16, float16, float32), head_dim 32, 64 or 128, any
+    page size, any strides with the last dimension contiguous.  Two tokens
+    given the same slot race; no gradient flows through the cache."""
+    device = _call.cuda_device("key", key)
+    if key.dim() != 4 or key.shape != value.shape:
+        raise ValueError(f"key and value must be (B, Hkv, T, D), got {tuple(key.shape)} and {tuple(value.shape)}")
+    B, H, T, D = key.shape
+    if key.numel() == 0:
+        raise ValueError("key and value must not be empty")
+    if D not in (32, 64, 128):
+        raise ValueError(f"head_dim must be 32, 64 or 128, got {D}")
+    if value.dtype != key.dtype:
+        raise TypeError(f"value is {value.dtype}, key {key.dtype}")
+    _call.on_device("value", value, device)
+    _pools(k_pages, v_pages, H, D, key.dtype, device)
+    page_table = _table(page_table, B, device)
+    if page_table.shape[1] == 0:
+        raise ValueError("page_table has no columns")
+    lens = _call.ints("lens", lens, (B,), device)
+    w = _call.head_weight("key_weight", key_weight, key)
+    k, v = _call.dense_d(key), _call.dense_d(value)
+    a = _lib.AiPagedAppendArgs()
+    a.batch, a.num_kv_heads, a.seq_len, a.head_dim = B, H, T, D
+    a.dtype = _call.dtype_code(key, "key")
+    a.weight_dtype = a.dtype if w is None else _call.dtype_code(w, "key_weight")
+    a.eps = float(eps)
+    a.k, a.v, a.k_pages, a.v_pages = _call.t4(k), _call.t4(v), _call.t4(k_pages), _call.t4(v_pages)
+    a.n_pages, a.page_size = k_pages.shape[0], k_pages.shape[2]
+    a.page_table, a.page_table_stride, a.max_pages = page_table.data_ptr(), page_table.stride(0), page_table.shape[1]
+    a.lens = lens.data_ptr()
+    if new_lens is not None:
+        new_lens = _call.ints("new_lens", new_lens, (B,), device)
+        a.new_lens = new_lens.data_ptr()
+    if w is not None:
+        a.k_weight = w.data_ptr()
+    keep = _call.fill_rope(a, rope, positions, B, T, D, device)
+    a.status = status_word(device).data_ptr()
+    _call.launch(_lib.lib().ai_paged_append, a, device, "ai_paged_append")
+    del keep
+
+
+def shared_prefix_attention(query: Tensor, k_pages: Tensor, v_pages: Tensor, prefix_pages: Optional[Tensor],
+                            prefix_len: int, page_table: Tensor, lens: Tensor, scaling: Optional[float] = None,
+                            query_lens: Optional[Tensor] = None, return_lse: bool = False):
+    """Attention of a batch over its shared prefix and each sequence's own tokens.
+
+    ``query`` ``(B, Hq, T, D)`` (normalised and rotated): query token ``t <
+    query_lens[b]`` (all ``T`` without it) sees the ``prefix_len`` keys of
+    ``prefix_pages`` (int32) and the first ``lens[b] - query_lens[b] + t + 1``
+    keys of the pages in row ``b`` of ``page_table``, so ``lens`` ``(B,)``
+    int32 counts the new tokens, already appended.  Returns ``(B, T, Hq, D)``
+    (and the float32 log-sum-exp ``(B, Hq, T)`` with ``return_lse``); a padding
+    token, or one without a key, gives zeros and ``-inf``.  ``scaling``
+    defaults to ``D ** -0.5``.  With ``prefix_len`` 0 it is plain paged
+    decoding.
+
+    CUDA tensors of one dtype, head_dim 32, 64 or 128, any page size, any
+    strides with the last dimension contiguous.  The keys that some query of
+    the sequence sees must hold finite values; the slots past them may hold
+    anything.  A length or page out of range is clamped and sets the status
+    word."""
+    device = _call.cuda_device("query", query)
+    if query.dim() != 4 or query.numel() == 0:
+        raise ValueError(f"query must be (B, Hq, T, D) and not empty, got {tuple(query.shape)}")
+    B, Hq, T, D = query.shape
+    if D not in (32, 64, 128):
+        raise ValueError(f"head_dim must be 32, 64 or 128, got {D}")
+    heads = k_pages.shape[1] if k_pages.dim() == 4 else 0
+    if heads == 0 or Hq % heads != 0:
+        raise ValueError(f"num_q_heads {Hq} is not a multiple of num_kv_heads {heads}")
+    _pools(k_pages, v_pages, heads, D, query.dtype, device)
+    S = k_pages.shape[2]
+    page_table = _table(page_table, B, device)
+    lens = _call.ints("lens", lens, (B,), device)
+    prefix_len = int(prefix_len)
+    if prefix_len < 0:
+        raise ValueError(f"prefix_len {prefix_len} is negative")
+    q = _call.dense_d(query)
+    out = torch.empty((B, T, Hq, D), dtype=query.dtype, device=device)
+    a = _lib.AiPrefixAttnArgs()
+    a.batch, a.num_q_heads, a.seq_len, a.head_dim = B, Hq, T, D
+    a.num_kv_heads = heads
+    a.dtype = _call.dtype_code(query, "query")
+    a.scale = float(scaling) if scaling is not None else D ** -0.5
+    a.q, a.k_pages, a.v_pages = _call.t4(q), _call.t4(k_pages), _call.t4(v_pages)
+    a.out = _lib.AiTensor4(out.data_ptr(), T * Hq * D, D, Hq * D)
+    a.n_pages, a.page_size = k_pages.shape[0], S
+    if prefix_len:
+        if prefix_pages is None or prefix_pages.dim() != 1 or prefix_pages.shape[0] * S < prefix_len:
+            raise ValueError(f"prefix_pages must list the pages of {prefix_len} keys ({S} a page)")
+        prefix_pages = _call.ints("prefix_pages", prefix_pages, tuple(prefix_pages.shape), device)
+        a.prefix_pages = prefix_pages.data_ptr()
+    a.prefix_len = prefix_len
+    a.page_table, a.page_table_stride, a.max_pages = page_table.data_ptr(), page_table.stride(0), page_table.shape[1]
+    a.lens = lens.data_ptr()
+    if query_lens is not None:
+        query_lens = _call.ints("query_lens", query_lens, (B,), device)
+        a.query_lens = query_lens.data_ptr()
+    lse = None
+    if return_lse:
+        lse = torch.empty((B, Hq, T), dtype=torch.float32, device=device)
+        a.lse = lse.data_ptr()
+    a.status = status_word(device).data_ptr()
+    lib = _lib.lib()
+    ws = _call.workspace(lib.ai_prefix_attn_workspace, a, device, "ai_prefix_attn_workspace")
+    _call.launch(lib.ai_prefix_attn, a, device, "ai_prefix_attn")
+    del ws
+    return (out, lse) if return_lse else out

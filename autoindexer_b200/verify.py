@@ -1,0 +1,94 @@
+"""Verification of drafted tokens against the target model's probabilities.
+
+A drafter proposes a few tokens per sequence, the target model scores them in
+one forward, and ``verify_draft`` keeps the longest prefix that leaves the
+target's distribution unchanged, plus one token sampled where it stopped.
+Random numbers are inputs, so a step can be repeated exactly.
+"""
+
+from __future__ import annotations
+
+from typing import Optional, Tuple
+
+import torch
+from torch import Tensor
+
+from . import _call, _lib
+from .attention import status_word
+
+__all__ = ["verify_draft"]
+
+MAX_DRAFT = 64
+
+
+def verify_draft(target_logits: Tensor, draft_tokens: Tensor, uniforms: Tensor, noise: Tensor,
+                 draft_logits: Optional[Tensor] = None, draft_lens: Optional[Tensor] = None,
+                 temperature: Optional[Tensor] = None) -> Tuple[Tensor, Tensor, Tensor]:
+    """Accepts drafted tokens and samples the next one, per sequence.
+
+    ``target_logits`` ``(B, L + 1, V)``: row ``i`` scores the token after the
+    first ``i`` drafted ones; ``draft_tokens`` ``(B, L)`` int64;
+    ``draft_logits`` ``(B, L, V)`` the logits they were sampled from (``None``:
+    proposed with certainty, as by a lookup); ``draft_lens`` ``(B,)`` int32 how
+    many are real; ``temperature`` ``(B,)`` float32 divides both (``None``: 1;
+    0 decodes greedily).  ``uniforms`` ``(B, L)`` float32 in ``[0, 1)`` decide
+    acceptance: ``u * q(x) < p(x)``; ``noise`` ``(B, V)`` float32 exponential
+    variates (> 0) choose the next token: the largest ``r / noise`` with ``r``
+    the residual ``max(p - q, 0)`` after a refusal, else ``p``; equal values
+    go to the lowest index.
+
+    Returns ``(accepted (B,) int32, tokens (B, L + 1) int64, logprobs (B, L +
+    1) float32)``: the accepted tokens and the next one, then -1, and each
+    one's log-probability under the target (0 past them, and in greedy rows).
+
+    Logits are CUDA bfloat16, float16 or float32, finite or ``-inf``, with a
+    contiguous vocabulary; up to 64 drafted tokens.  A token outside the
+    vocabulary is refused and sets the status word."""
+    device = _call.cuda_device("target_logits", target_logits)
+    if target_logits.dim() != 3 or target_logits.numel() == 0:
+        raise ValueError(f"target_logits must be (B, L + 1, V) and not empty, got {tuple(target_logits.shape)}")
+    B, rows, V = target_logits.shape
+    L = rows - 1
+    if L > MAX_DRAFT:
+        raise ValueError(f"at most {MAX_DRAFT} drafted tokens, got {L}")
+    if draft_tokens.dtype != torch.int64:
+        raise TypeError(f"draft_tokens must be int64, got {draft_tokens.dtype}")
+    if tuple(draft_tokens.shape) != (B, L):
+        raise ValueError(f"draft_tokens must have shape {(B, L)}, got {tuple(draft_tokens.shape)}")
+    _call.on_device("draft_tokens", draft_tokens, device)
+    draft_tokens = draft_tokens.contiguous()
+    uniforms = _call.floats("uniforms", uniforms, (B, L), device)
+    noise = _call.floats("noise", noise, (B, V), device)
+    target = _call.dense_d(target_logits)
+    a = _lib.AiVerifyArgs()
+    a.batch, a.n_draft, a.vocab = B, L, V
+    a.dtype = _call.dtype_code(target, "target_logits")
+    a.target = target.data_ptr()
+    a.target_stride_b, a.target_stride_t = target.stride(0), target.stride(1)
+    if draft_logits is not None:
+        if tuple(draft_logits.shape) != (B, L, V):
+            raise ValueError(f"draft_logits must have shape {(B, L, V)}, got {tuple(draft_logits.shape)}")
+        if draft_logits.dtype != target.dtype:
+            raise TypeError(f"draft_logits is {draft_logits.dtype}, target_logits {target.dtype}")
+        _call.on_device("draft_logits", draft_logits, device)
+        draft_logits = _call.dense_d(draft_logits)
+        if L:
+            a.draft = draft_logits.data_ptr()
+            a.draft_stride_b, a.draft_stride_t = draft_logits.stride(0), draft_logits.stride(1)
+    if draft_lens is not None:
+        draft_lens = _call.ints("draft_lens", draft_lens, (B,), device)
+        a.draft_lens = draft_lens.data_ptr()
+    if temperature is not None:
+        temperature = _call.floats("temperature", temperature, (B,), device)
+        a.temperature = temperature.data_ptr()
+    accepted = torch.empty(B, dtype=torch.int32, device=device)
+    tokens = torch.empty((B, rows), dtype=torch.int64, device=device)
+    logprobs = torch.empty((B, rows), dtype=torch.float32, device=device)
+    a.tokens, a.uniforms, a.noise = draft_tokens.data_ptr(), uniforms.data_ptr(), noise.data_ptr()
+    a.accepted, a.out_tokens, a.logprobs = accepted.data_ptr(), tokens.data_ptr(), logprobs.data_ptr()
+    a.status = status_word(device).data_ptr()
+    lib = _lib.lib()
+    ws = _call.workspace(lib.ai_verify_draft_workspace, a, device, "ai_verify_draft_workspace")
+    _call.launch(lib.ai_verify_draft, a, device, "ai_verify_draft")
+    del ws
+    return accepted, tokens, logprobs

@@ -448,6 +448,168 @@ int ai_index_rows_sizes(const AiPrepList* list, const int32_t* block_type, int32
                         int64_t* edits);
 int ai_index_rows(const AiPrepList* list, const int32_t* block_type, int64_t editable_start, AiIndexRowsOut* out);
 
+/* ------------------------------------------------------------------------
+ * Operators around the attention kernels: per-head norms with the position
+ * rotation, the paged K/V cache, attention of a batch that shares a prefix,
+ * and the verification of drafted tokens.
+ *
+ * Position ids are rows of the rotary table (rope_cos / rope_sin, fp32
+ * [n_pos][D/2], rotate-half pairing: dims k and k + D/2 share slot k).  An id
+ * outside the table is AI_ERR_DEV_BOUNDS in the status word and takes row 0.
+ * ------------------------------------------------------------------------ */
+
+/* Position ids of (row b, token t): ptr[b * stride_b + t]. */
+typedef struct AiPositions {
+  const void* ptr;            /* int32 or int64 */
+  int64_t stride_b;           /* elements; 0: one row shared by the batch */
+  int32_t is_int64;
+} AiPositions;
+
+/* out = R(pos) (w * x / sqrt(mean(x^2) + eps)) for every head row of q and k,
+ * one launch.  A NULL weight leaves that tensor unnormalised, NULL tables
+ * leave both unrotated; k.ptr NULL (num_kv_heads 0) is q alone.  Sums, the
+ * norm and the rotation are fp32, rounded once to the output's type. */
+typedef struct AiHeadNormArgs {
+  int32_t batch;
+  int32_t seq_len;
+  int32_t num_q_heads;
+  int32_t num_kv_heads;       /* 0: no k */
+  int32_t head_dim;           /* 32, 64 or 128 */
+  int32_t dtype;              /* AiDtype of q, k and the outputs */
+  int32_t weight_dtype;       /* dtype, or AI_DTYPE_F32 */
+  float eps;
+  AiTensor4 q, k;             /* (B, Hq, T, D), (B, Hkv, T, D) */
+  AiTensor4 q_out, k_out;
+  const void* q_weight;       /* [D] or NULL */
+  const void* k_weight;
+  const float* rope_cos;      /* [n_pos][D/2], or NULL */
+  const float* rope_sin;
+  int32_t n_pos;
+  AiPositions pos;
+  int32_t* status;
+} AiHeadNormArgs;
+
+/* Gradients of q_out and k_out (dq_out, dk_out) to dq, dk and, for the
+ * weights that are not NULL, dq_weight / dk_weight (weight_dtype, [D]).
+ * fwd.q_out and fwd.k_out are not read.  The weight gradients are summed over
+ * the rows in a fixed order (no atomics). */
+typedef struct AiHeadNormBwdArgs {
+  AiHeadNormArgs fwd;
+  AiTensor4 dq_out, dk_out;
+  AiTensor4 dq, dk;
+  void* dq_weight;
+  void* dk_weight;
+  void* workspace;            /* ai_head_norm_bwd_workspace bytes, 16-B aligned */
+  size_t workspace_bytes;
+} AiHeadNormBwdArgs;
+
+int ai_head_norm_fwd(const AiHeadNormArgs* args, void* stream);
+int ai_head_norm_bwd_workspace(const AiHeadNormBwdArgs* args, size_t* bytes);
+int ai_head_norm_bwd(const AiHeadNormBwdArgs* args, void* stream);
+
+/* New keys and values into a paged cache: token t < new_lens[b] of sequence b
+ * becomes its token n = lens[b] + t, stored in slot n % page_size of page
+ * page_table[b][n / page_size].  Keys are normalised (k_weight not NULL) and
+ * rotated (tables not NULL) on the way, values copied.  A token whose page
+ * is outside the table or the pool is skipped with AI_ERR_DEV_BOUNDS. */
+typedef struct AiPagedAppendArgs {
+  int32_t batch;
+  int32_t seq_len;            /* T: new tokens given per sequence */
+  int32_t num_kv_heads;
+  int32_t head_dim;           /* 32, 64 or 128 */
+  int32_t dtype;
+  int32_t weight_dtype;
+  float eps;
+  AiTensor4 k, v;             /* (B, Hkv, T, D) */
+  AiTensor4 k_pages, v_pages; /* (n_pages, Hkv, page_size, D) */
+  int32_t n_pages;
+  int32_t page_size;
+  const int32_t* page_table;  /* [B][max_pages] */
+  int64_t page_table_stride;
+  int32_t max_pages;
+  const int32_t* lens;        /* [B]: tokens each sequence holds already */
+  const int32_t* new_lens;    /* [B], or NULL: T for every sequence */
+  const void* k_weight;
+  const float* rope_cos;
+  const float* rope_sin;
+  int32_t n_pos;
+  AiPositions pos;
+  int32_t* status;
+} AiPagedAppendArgs;
+
+int ai_paged_append(const AiPagedAppendArgs* args, void* stream);
+
+/* Attention over a paged cache of a batch whose sequences share a prefix.
+ * Query token t < n_b = query_lens[b] of sequence b sees the prefix_len keys
+ * of prefix_pages and the first lens[b] - n_b + t + 1 keys of its own pages
+ * (lens counts the new tokens).  Padding tokens (t >= n_b) and tokens without
+ * a key give 0 (lse -inf).  K and V hold the keys as the scores use them
+ * (already rotated).  The prefix's K and V are read once per 128 query rows
+ * of a KV head over the whole batch, not once per sequence. */
+typedef struct AiPrefixAttnArgs {
+  int32_t batch;
+  int32_t seq_len;            /* T: query tokens per sequence */
+  int32_t num_q_heads;
+  int32_t num_kv_heads;
+  int32_t head_dim;           /* 32, 64 or 128 */
+  int32_t dtype;
+  float scale;
+  AiTensor4 q;                /* (B, Hq, T, D) */
+  AiTensor4 out;              /* (B, Hq, T, D) view */
+  float* lse;                 /* (B, Hq, T) natural log, or NULL */
+  AiTensor4 k_pages, v_pages; /* (n_pages, Hkv, page_size, D) */
+  int32_t n_pages;
+  int32_t page_size;
+  const int32_t* prefix_pages; /* [ceil(prefix_len / page_size)] */
+  int32_t prefix_len;
+  const int32_t* page_table;  /* [B][max_pages] */
+  int64_t page_table_stride;
+  int32_t max_pages;
+  const int32_t* lens;        /* [B]: own tokens of each sequence, the new ones included */
+  const int32_t* query_lens;  /* [B], or NULL: T for every sequence */
+  int32_t* status;
+  void* workspace;            /* ai_prefix_attn_workspace bytes, 256-B aligned */
+  size_t workspace_bytes;
+} AiPrefixAttnArgs;
+
+int ai_prefix_attn_workspace(const AiPrefixAttnArgs* args, size_t* bytes);
+int ai_prefix_attn(const AiPrefixAttnArgs* args, void* stream);
+
+/* Verification of drafted tokens.  With tau_b = temperature[b] (NULL: 1),
+ * p_i = softmax(target[b, i] / tau_b) and q_i = softmax(draft[b, i] / tau_b)
+ * (draft NULL: q_i is one-hot at the drafted token), drafted token x_i is
+ * accepted iff uniforms[b, i] * q_i(x_i) < p_i(x_i), up to the first refusal
+ * a (n_b = draft_lens[b] if there is none).  The next token is
+ * argmax_v r(v) / noise[b, v] with r = max(p_a - q_a, 0) after a refusal and
+ * r = p_a after none (noise: exponential variates, so the token is a sample
+ * of r); where r is zero everywhere, r = p_a.  tau_b = 0 decodes greedily:
+ * p_i is one-hot at the largest logit.  Equal values go to the lowest index.
+ * Logits are finite or -inf. */
+typedef struct AiVerifyArgs {
+  int32_t batch;
+  int32_t n_draft;            /* L: drafted tokens given per sequence, 0 .. 64 */
+  int32_t vocab;
+  int32_t dtype;              /* AiDtype of the logits */
+  const void* target;         /* (B, L + 1, V), v contiguous */
+  int64_t target_stride_b, target_stride_t;
+  const void* draft;          /* (B, L, V), or NULL */
+  int64_t draft_stride_b, draft_stride_t;
+  const int64_t* tokens;      /* [B][L] */
+  const float* uniforms;      /* [B][L], in [0, 1) */
+  const float* noise;         /* [B][V], > 0 */
+  const float* temperature;   /* [B], or NULL */
+  const int32_t* draft_lens;  /* [B], or NULL: L for every sequence */
+  int32_t* accepted;          /* [B]: a */
+  int64_t* out_tokens;        /* [B][L + 1]: x_0 .. x_{a-1}, the next token, then -1 */
+  float* logprobs;            /* [B][L + 1]: log p_i of each token of out_tokens, 0 past them */
+  int32_t* status;
+  void* workspace;            /* ai_verify_draft_workspace bytes, 256-B aligned */
+  size_t workspace_bytes;
+} AiVerifyArgs;
+
+int ai_verify_draft_workspace(const AiVerifyArgs* args, size_t* bytes);
+int ai_verify_draft(const AiVerifyArgs* args, void* stream);
+
 /* Synchronises the stream, copies the device status word to *host_out and
  * resets it to AI_OK.  For tests and debugging; not needed on the hot path. */
 int ai_attn_read_status(int32_t* dev_status, void* stream, int32_t* host_out);
@@ -483,7 +645,11 @@ typedef enum AiProfKind {
   AI_PROF_BWD_FILL = 6, /* backward rows no block owns */
   AI_PROF_SIMT = 7,     /* fp32 / fp16 / other head_dim path */
   AI_PROF_DECODE = 8,   /* decode step (split-K + combine) */
-  AI_PROF_KINDS = 9
+  AI_PROF_HEAD_NORM = 9, /* per-head norms with the rotation, forward and backward */
+  AI_PROF_APPEND = 10,  /* paged cache append */
+  AI_PROF_PREFIX = 11,  /* shared-prefix attention (split + combine) */
+  AI_PROF_VERIFY = 12,  /* draft verification */
+  AI_PROF_KINDS = 13
 } AiProfKind;
 int ai_attn_profile_enable(int on);
 int ai_attn_profile_read(float* ms_by_kind, int32_t* launches_by_kind);
