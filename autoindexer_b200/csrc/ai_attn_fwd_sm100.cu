@@ -1240,19 +1240,23 @@ bool strides_ok(const AiTensor4& t) {
 
 }  // namespace sm100
 
-// 4-D map over a (B, H, T, 128) bf16 tensor; box = 64 dims x box_rows rows,
-// 128-byte swizzle, zero fill past T.
-bool sm100_make_map(CUtensorMap* map, const AiTensor4& t, int B, int H, int T, int box_rows) {
+// 4-D map over a (B, H, T, head_dim) bf16 or fp16 tensor; box = 64 dims x
+// box_rows rows, 128-byte swizzle, zero fill past T.
+bool sm100_make_map_of(CUtensorMap* map, const AiTensor4& t, int B, int H, int T, int box_rows, int head_dim, int dtype) {
   auto enc = sm100::get_encode();
   if (!enc) return false;
-  cuuint64_t dims[4] = {(cuuint64_t)sm100::D, (cuuint64_t)T, (cuuint64_t)H, (cuuint64_t)B};
+  cuuint64_t dims[4] = {(cuuint64_t)head_dim, (cuuint64_t)T, (cuuint64_t)H, (cuuint64_t)B};
   cuuint64_t strides[3] = {(cuuint64_t)t.stride_t * 2, (cuuint64_t)t.stride_h * 2, (cuuint64_t)t.stride_b * 2};
   cuuint32_t box[4] = {64, (cuuint32_t)box_rows, 1, 1};
   cuuint32_t estr[4] = {1, 1, 1, 1};
-  CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, t.ptr, dims, strides, box, estr,
-                   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  CUresult r = enc(map, dtype == AI_DTYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4,
+                   t.ptr, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS;
+}
+
+bool sm100_make_map(CUtensorMap* map, const AiTensor4& t, int B, int H, int T, int box_rows) {
+  return sm100_make_map_of(map, t, B, H, T, box_rows, sm100::D, AI_DTYPE_BF16);
 }
 
 bool sm100_fwd_supported(int dtype, int head_dim) { return dtype == AI_DTYPE_BF16 && head_dim == sm100::D; }

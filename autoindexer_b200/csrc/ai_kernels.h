@@ -57,6 +57,8 @@ int sm100_bwd(const AiAttnBwdArgs& a, float* delta, void* rot, bool rot_ready, f
               int parts, cudaStream_t st, cudaError_t* cuda_err);
 // TMA map over a (B, H, T, 128) bf16 tensor, box 64 x box_rows, 128-byte swizzle.
 bool sm100_make_map(CUtensorMap* map, const AiTensor4& t, int B, int H, int T, int box_rows);
+// The same over (B, H, T, head_dim) bf16 or fp16, head_dim 64 or 128.
+bool sm100_make_map_of(CUtensorMap* map, const AiTensor4& t, int B, int H, int T, int box_rows, int head_dim, int dtype);
 
 // Once-rotated Q and K copies (bf16, head_dim 128) for the tensor-core kernels:
 // bytes of scratch they need (q_bytes: offset of the K copy), and the launch

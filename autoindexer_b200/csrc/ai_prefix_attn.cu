@@ -135,7 +135,7 @@ extern "C" int ai_prefix_attn_workspace(const AiPrefixAttnArgs* args, size_t* by
   const int rc = ai::prefix::check(args);
   if (rc != AI_OK) return rc;
   if (!bytes) return AI_ERR_NULL;
-  *bytes = 0;
+  *bytes = ai::prefix::sm100_fits(*args) ? ai::prefix::sm100_workspace(*args) : 0;
   return AI_OK;
 }
 
@@ -143,6 +143,7 @@ extern "C" int ai_prefix_attn(const AiPrefixAttnArgs* args, void* stream) {
   const int rc = ai::prefix::check(args);
   if (rc != AI_OK) return rc;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (ai::prefix::sm100_fits(*args)) return ai::prefix::sm100_launch(*args, st);
   if (args->dtype == AI_DTYPE_BF16) return ai::prefix::simt_launch<__nv_bfloat16>(*args, st);
   if (args->dtype == AI_DTYPE_F16) return ai::prefix::simt_launch<__half>(*args, st);
   return ai::prefix::simt_launch<float>(*args, st);

@@ -1,6 +1,7 @@
 // Shared by the kernels of the shared-prefix attention.
 #pragma once
 
+#include <cuda_runtime.h>
 #include <stdint.h>
 
 #include "../../include/ai_attn.h"
@@ -8,6 +9,12 @@
 
 namespace ai {
 namespace prefix {
+
+// The tensor-core kernels (ai_prefix_attn_sm100.cu): whether they take the
+// call, the scratch they need, and the launch.
+bool sm100_fits(const AiPrefixAttnArgs& a);
+size_t sm100_workspace(const AiPrefixAttnArgs& a);
+int sm100_launch(const AiPrefixAttnArgs& a, cudaStream_t st);
 
 // Own keys of a sequence (clamped to what its page table can hold) and its
 // real query tokens.
