@@ -1,28 +1,27 @@
 // Shared-prefix attention on the tensor cores: bf16 / fp16, head_dim 64 or
 // 128, page sizes that are powers of two from 16.
 //
-// Work is key tiles of 64 keys.  A unit is 128 query rows of one KV head with
-// one key list: either 128 of the B T G rows that share the prefix (G query
-// heads per KV head), or the rows of one sequence with its own keys.  The
-// tiles of all units stand in one line, the prefix's units first, and every
-// CTA takes an equal stretch of it, whatever the lengths are (they are read on
-// the device); a stretch crosses units, and the rows of a unit cut by a
-// stretch's end leave partial results (O / l in fp32 and the log2-sum) that
-// the combine launch joins with the other key list's.
+// Every query row attends over two key lists, the prefix's and its own
+// sequence's.  The rows that share a list (of one KV head) are a unit: the
+// B T G rows over the batch for the prefix (G query heads per KV head), the
+// T G rows of a sequence for its own keys.  A unit's keys are cut into tiles;
+// the tiles of all units stand in one line, and every worker takes an equal
+// stretch of it, whatever the lengths are (they are read on the device).  A
+// stretch crosses units, and the rows of a unit that a worker touched leave
+// partial results (O / l in fp32 and the log2-sum), which the combine launch
+// joins with the other list's.
 //
-// Per CTA (192 threads, two CTAs per SM, whose phases fill each other's
-// gaps): four softmax warps (a thread per row), a TMA warp streaming K and V
-// pages into a ring of tiles, an MMA warp.
-//   S = Q K^T    tcgen05, M = 128 rows, N = 64 keys, two S buffers in TMEM
-//   P = 2^(S - m) written over S as the 16-bit A operand of O += P V
-//   O             fp32 in TMEM, rescaled only when a row's maximum grows by
-//                 more than 2^8 (P then stays below 2^8 and sums in fp32)
-// The MMA warp issues S of tile g + 1 before P V of tile g, so the scores of
-// the next tile are ready when the softmax returns.
-//
-// Few rows per KV head: HBM-bound, each K / V byte is read once and most of
-// the 128 rows are empty (their warps skip the softmax).  Many rows:
-// tensor-bound, 4 D 128 64 FLOP per 32 KB (D = 128) tile pair.
+// Two kernels, by the rows that meet each key:
+//   tile kernel   many rows, long lists: 128 rows x 64 keys a step on
+//                 tcgen05 (worker: a CTA);
+//   warp kernel   few rows, short lists: 16 rows x 32 keys a step on
+//                 mma.sync, K and V by TMA (worker: one to four warps).
+//                 HBM-bound with few rows; a worker has no barrier of the CTA
+//                 in its loop and a short list costs a few loads, where the
+//                 tile kernel pays a chain of TMA, MMA and TMEM latencies per
+//                 unit (measured: 4.8 us per unit of one 64-key tile).
+// They run one after the other by programmatic dependent launch, so that the
+// second fills the SMs the first leaves.
 
 #include <cuda.h>
 #include <cuda_bf16.h>
@@ -65,71 +64,163 @@ struct Smem {
 };
 static_assert(2 * (Smem<128>::SCAN + 4 * (kMaxBatch + 1) + 1024 + 1024) <= 228 * 1024, "two CTAs per SM");
 
+constexpr int kWarpRows = 64;   // most rows of a sequence on the warp kernel
+constexpr int kWarpKeys = 32;   // keys of its tile
+constexpr int kShortPrefix = 6;  // positions of a prefix per worker of the warp kernel, at most
+// What starting a unit costs, in tiles of its kernel (chosen by the spread of
+// the CTAs' times over prefixes and sequences of 1 to 32768 keys).
+constexpr int kStartTile = 4, kStartWarp = 2;
+
+// One kernel's line of tiles.  Starting a unit costs about as much as `start`
+// tiles (its rows in, its partial results out), so `start` idle positions
+// stand before its tiles.
+struct Line {
+  int workers;
+  int least;          // positions a worker takes at least
+  int start;
+  int units_prefix;   // prefix units on this line, each of tiles_prefix tiles
+  int tiles_prefix;
+  int per_seq;        // units per sequence on this line (0: own keys are not on it)
+  int rows_prefix;    // rows of a prefix slot
+  int rows_own;       // rows of an own slot
+  int64_t base_prefix, base_own;  // first row of each region; slot (unit + worker) follows
+};
+
 // What the host knows of the work.
 struct Plan {
   int group;        // G: query heads per KV head
   int rows_seq;     // T G
   int rows_all;     // B T G
-  int tiles_prefix; // key tiles of the prefix
-  int rt, tt;       // row tiles of all rows / of one sequence
-  int units_prefix; // Hkv rt (0 without a prefix)
-  int part_rows;    // rows kept of a sequence's unit: min(128, T G)
-  float* part_o;    // prefix slots [units_prefix + ctas][128][D], then own slots [B tt Hkv + ctas][part_rows][D]
-  float* part_lse;  // the same rows
-  int* scan;        // [B + 1] own tiles before each sequence
-  int64_t own_base; // rows of the prefix slots
+  int rt, tt;       // tile kernel: row tiles of all rows / of one sequence
+  int split;        // warps of a warp-kernel worker
+  bool prefix_warp, own_warp;  // which kernel has the list
+  Line tile, warp;
+  float* part_o;    // [rows][D]
+  float* part_lse;  // [rows]
+  int* scan;        // [B + 1] positions before each sequence's own units, per unit
 };
 
-// A CTA's stretch within one unit.
-struct Seg {
-  int unit;        // prefix unit, or unit of the sequences (b tt + row tile) Hkv + hk
-  int b;           // -1: the prefix
-  int hk, row0, rows;
-  int j0, n;       // key tiles [j0, j0 + n)
-  int keys;        // keys of the list
+// Positions of a line whose sequences have `own` positions per unit (the host
+// has checked that they fit in an int).
+__device__ __forceinline__ int line_total(const Line& l, int own) {
+  return l.units_prefix * (l.start + l.tiles_prefix) + own * l.per_seq;
+}
+
+// The line's stretches: n workers have work, none less than `least` positions
+// unless the line is shorter; the first `more` take one position more.
+struct Split {
+  int n, len, more;
+  __device__ __forceinline__ int begin(int w) const { return w * len + min(w, more); }
+  __device__ __forceinline__ int worker(int x) const {
+    const int head = more * (len + 1);
+    return x < head ? x / (len + 1) : more + (x - head) / len;
+  }
 };
 
-__device__ __forceinline__ Seg locate(const AiPrefixAttnArgs& a, const Plan& p, const int* scan, int w, int w1) {
-  Seg s;
-  const int before = p.units_prefix * p.tiles_prefix;
-  if (w < before) {
-    s.unit = w / p.tiles_prefix;
-    s.b = -1;
-    s.hk = s.unit / p.rt;
-    s.row0 = (s.unit % p.rt) * BM;
-    s.rows = min(BM, p.rows_all - s.row0);
-    s.j0 = w % p.tiles_prefix;
-    s.n = min(p.tiles_prefix - s.j0, w1 - w);
-    s.keys = a.prefix_len;
-    return s;
+__device__ __forceinline__ Split split_line(const Line& l, int total) {
+  Split s{0, 1, 0};
+  if (total > 0) {
+    s.n = min(l.workers, (total + l.least - 1) / l.least);
+    s.len = total / s.n;
+    s.more = total - s.len * s.n;
   }
-  const int per = p.tt * a.num_kv_heads, x = w - before;
-  int lo = 0, hi = a.batch - 1;  // the last sequence with scan * per <= x that has tiles
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) / 2;
-    if (scan[mid] * per <= x)
-      lo = mid;
-    else
-      hi = mid - 1;
-  }
-  const int tiles = scan[lo + 1] - scan[lo], rem = x - scan[lo] * per, v = rem / tiles;
-  s.b = lo;
-  s.unit = lo * per + v;
-  s.hk = v % a.num_kv_heads;
-  s.row0 = (v / a.num_kv_heads) * BM;
-  s.rows = min(BM, p.rows_seq - s.row0);
-  s.j0 = rem % tiles;
-  s.n = min(tiles - s.j0, w1 - w);
-  s.keys = seq_lens(a, lo).keys;
   return s;
 }
 
-// First tile of CTA `cta` of the `ctas` that have work (at most one per tile,
-// so that no stretch is empty).
-__device__ __forceinline__ int stretch(int64_t total, int cta, int ctas) { return (int)(total * cta / ctas); }
+// scan[b] = positions before sequence b on the line of its own keys, for one
+// unit per sequence (one warp; tiles of `keys` keys).
+__device__ __forceinline__ void scan_own(const AiPrefixAttnArgs& a, int keys, int start, int* scan) {
+  const int lane = threadIdx.x % 32;
+  int base = 0;
+  for (int b0 = 0; b0 < a.batch; b0 += 32) {
+    const int b = b0 + lane;
+    int v = b < a.batch ? (seq_lens(a, b).keys + keys - 1) / keys : 0;
+    if (v > 0) v += start;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int u = __shfl_up_sync(0xffffffffu, v, o);
+      if (lane >= o) v += u;
+    }
+    if (b < a.batch) scan[b + 1] = base + v;
+    base += __shfl_sync(0xffffffffu, v, 31);
+  }
+  if (lane == 0) scan[0] = 0;
+}
 
-// The CTA whose stretch holds tile w.
-__device__ __forceinline__ int cta_of(int64_t w, int64_t total, int ctas) { return (int)(((w + 1) * ctas - 1) / total); }
+// A worker's stretch within one unit.
+struct Seg {
+  int unit;        // of its region
+  int b;           // sequence, -1: the prefix
+  int sub;         // unit within the sequence, or within the prefix
+  int j0, n;       // tiles [j0, j0 + n) of the unit
+  int keys;        // keys of the list
+};
+
+// The stretch [w, w1) within the unit at position w; `w` moves to its end.
+// (n may be 0: idle positions only.)
+__device__ __forceinline__ Seg locate(const AiPrefixAttnArgs& a, const Line& l, const int* scan, int& w, int w1) {
+  Seg s;
+  const int per = l.start + l.tiles_prefix, before = l.units_prefix * per;
+  int at, size;  // position within the unit, and its positions
+  if (w < before) {
+    s.unit = s.sub = w / per;
+    s.b = -1;
+    at = w - s.unit * per;
+    size = per;
+    s.keys = a.prefix_len;
+  } else {
+    const int x = w - before;
+    int lo = 0, hi = a.batch - 1;  // the last sequence that begins at or before x (it has tiles)
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) / 2;
+      if (scan[mid] * l.per_seq <= x)
+        lo = mid;
+      else
+        hi = mid - 1;
+    }
+    size = scan[lo + 1] - scan[lo];
+    const int rem = x - scan[lo] * l.per_seq;
+    s.b = lo;
+    s.sub = rem / size;
+    s.unit = lo * l.per_seq + s.sub;
+    at = rem - s.sub * size;
+    s.keys = seq_lens(a, lo).keys;
+  }
+  const int end = min(size, at + (w1 - w));
+  s.j0 = max(0, at - l.start);
+  s.n = max(0, end - l.start - s.j0);
+  w += end - at;
+  return s;
+}
+
+// The next stretch with tiles from position w on (n = 0: there is none).
+__device__ __forceinline__ Seg next_seg(const AiPrefixAttnArgs& a, const Line& l, const int* scan, int& w, int w1) {
+  Seg s{};
+  while (w < w1 && s.n == 0) s = locate(a, l, scan, w, w1);
+  return s;
+}
+
+// Query row `i` of a unit's rows: i counts (t, query head of the group) in a
+// sequence, and the sequences before it for the prefix.
+struct Row {
+  int b, t, g;
+};
+
+__device__ __forceinline__ Row row_of(const Plan& p, int b, int i) {
+  Row r;
+  r.b = b < 0 ? i / p.rows_seq : b;
+  const int rem = b < 0 ? i - r.b * p.rows_seq : i;
+  r.t = rem / p.group;
+  r.g = rem - r.t * p.group;
+  return r;
+}
+
+// Keys of the list that row r sees; -1 for a padding token.
+__device__ __forceinline__ int visible(const AiPrefixAttnArgs& a, const Row& r, bool prefix, int keys) {
+  const Lens len = seq_lens(a, r.b);
+  if (r.t >= len.n) return -1;
+  return prefix ? keys : max(0, keys - len.n + r.t + 1);
+}
 
 template <typename T> struct Pair;
 template <> struct Pair<__nv_bfloat16> {
@@ -155,10 +246,12 @@ __host__ __device__ constexpr uint32_t idesc(uint32_t fmt, int M, int N, bool b_
 
 template <typename T, int D>
 __global__ void __launch_bounds__(kThreads, 2)
-    split_kernel(const AiPrefixAttnArgs a, const Plan p, const __grid_constant__ CUtensorMap tm_k,
+    tile_kernel(const AiPrefixAttnArgs a, const Plan p, const __grid_constant__ CUtensorMap tm_k,
                  const __grid_constant__ CUtensorMap tm_v, const bool q_vec) {
   using L = Smem<D>;
   constexpr int CB = D / 64;
+  // (the warp kernel reads nothing this one writes)
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   extern __shared__ uint8_t smem_raw[];
   uint8_t* sm = tile::align1024(smem_raw);
   const uint32_t sbase = ptx::smem_u32(sm);
@@ -179,32 +272,25 @@ __global__ void __launch_bounds__(kThreads, 2)
     ptx::tmem_alloc(sbase + L::TMEM_SLOT, kTmemCols);
     ptx::tmem_relinquish();
   }
-  // Own key tiles before each sequence (warp 0, 32 sequences at a time).
   if (warp == 0) {
-    int base = 0;
-    for (int b0 = 0; b0 < a.batch; b0 += 32) {
-      const int b = b0 + lane;
-      int v = b < a.batch ? (seq_lens(a, b).keys + BN - 1) / BN : 0;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int u = __shfl_up_sync(0xffffffffu, v, o);
-        if (lane >= o) v += u;
-      }
-      if (b < a.batch) scan[b + 1] = base + v;
-      base += __shfl_sync(0xffffffffu, v, 31);
-    }
-    if (lane == 0) scan[0] = 0;
+    if (p.tile.per_seq)
+      scan_own(a, BN, p.tile.start, scan);
+    else if (lane == 0)
+      scan[0] = scan[a.batch] = 0;
   }
   ptx::tc_fence_before();
   __syncthreads();
   ptx::tc_fence_after();
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(sm + L::TMEM_SLOT);
-  const int64_t total = (int64_t)p.units_prefix * p.tiles_prefix + (int64_t)scan[a.batch] * p.tt * a.num_kv_heads;
-  const int ctas = (int)min((int64_t)gridDim.x, total);
-  const bool busy = (int)blockIdx.x < ctas;
-  const int w0 = busy ? stretch(total, blockIdx.x, ctas) : 0, w1 = busy ? stretch(total, blockIdx.x + 1, ctas) : 0;
-  if (blockIdx.x == 0)
+  const Split line = split_line(p.tile, line_total(p.tile, scan[a.batch]));
+  const bool busy = (int)blockIdx.x < line.n;
+  const int w0 = busy ? line.begin(blockIdx.x) : 0, w1 = busy ? line.begin(blockIdx.x + 1) : 0;
+  if (blockIdx.x == 0 && p.tile.per_seq)
     for (int b = tid; b <= a.batch; b += kThreads) p.scan[b] = scan[b];
+  // KV head and rows of a segment.
+  auto head = [&](const Seg& s) { return s.b < 0 ? s.sub / p.rt : s.sub % a.num_kv_heads; };
+  auto first_row = [&](const Seg& s) { return (s.b < 0 ? s.sub % p.rt : s.sub / a.num_kv_heads) * BM; };
+  auto rows = [&](const Seg& s, int row0) { return min(BM, (s.b < 0 ? p.rows_all : p.rows_seq) - row0); };
 
   // Bounded wait of a whole warp: true in every lane or false in every lane
   // (a warp leaves its loops together).
@@ -224,49 +310,56 @@ __global__ void __launch_bounds__(kThreads, 2)
     const int r = tid;
     const uint32_t lane_base = (uint32_t)(warp * 32) << 16;
     const float sl2 = a.scale * kLog2e;
-    int g = 0;
-    bool ok = true;
-    for (int w = w0; w < w1 && ok;) {
-      const Seg s = locate(a, p, scan, w, w1);
-      w += s.n;
-      // Q rows (the last S of the segment before has been waited for, so no
-      // MMA reads Q any more): 16-byte chunks, neighbouring threads along a row.
-      for (int x = tid; x < BM * (D / 8); x += 128) {
-        const int row = x / (D / 8), c = x % (D / 8);
-        uint4 v = make_uint4(0, 0, 0, 0);
-        if (row < s.rows) {
-          const int all = s.row0 + row, b = s.b < 0 ? all / p.rows_seq : s.b;
-          const int rem = s.b < 0 ? all % p.rows_seq : all, t = rem / p.group, h = s.hk * p.group + rem % p.group;
-          const T* q = static_cast<const T*>(a.q.ptr) + b * a.q.stride_b + h * a.q.stride_h + t * a.q.stride_t + 8 * c;
+    // The rows of a segment: the thread's visible keys of its list, and Q into
+    // shared memory (once no MMA reads the Q before it).  A row of Q is
+    // D / 8 16-byte chunks; neighbouring threads take a row's chunks and keep
+    // up to eight rows' loads in flight.  Rows without a query are neither
+    // loaded, masked nor stored: their TMEM lanes reach no other row.
+    int limit = 0, least = 0;
+    bool valid = false, active = false;
+    auto load_rows = [&](const Seg& s) {
+      constexpr int kPer = 128 / (D / 8), kFly = 8;  // rows a step, steps in flight
+      const int c = tid % (D / 8), hk = head(s), row0 = first_row(s), n_rows = rows(s, row0);
+      for (int r0 = tid / (D / 8); r0 - tid / (D / 8) < n_rows; r0 += kPer * kFly) {
+        uint4 v[kFly];
+#pragma unroll
+        for (int i = 0; i < kFly; ++i) {
+          const int row = r0 + i * kPer;
+          if (row >= n_rows) continue;
+          const Row x = row_of(p, s.b, row0 + row);
+          const T* q = static_cast<const T*>(a.q.ptr) + x.b * a.q.stride_b + (hk * p.group + x.g) * a.q.stride_h +
+                       x.t * a.q.stride_t + 8 * c;
           if (q_vec) {
-            v = __ldg(reinterpret_cast<const uint4*>(q));
+            v[i] = __ldg(reinterpret_cast<const uint4*>(q));
           } else {
             T e[8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) e[i] = q[i];
-            memcpy(&v, e, 16);
+            for (int k = 0; k < 8; ++k) e[k] = q[k];
+            memcpy(&v[i], e, 16);
           }
         }
-        *reinterpret_cast<uint4*>(sm + L::Q + tile::chunk_off<BM>(row, c)) = v;
+#pragma unroll
+        for (int i = 0; i < kFly; ++i) {
+          const int row = r0 + i * kPer;
+          if (row < n_rows) *reinterpret_cast<uint4*>(sm + L::Q + tile::chunk_off<BM>(row, c)) = v[i];
+        }
       }
       ptx::fence_proxy_async_smem();
       ptx::mbar_arrive(bar(L::Q_READY));
-      // The row's visible keys of this list.  Rows without a query are not
-      // masked and not stored (their TMEM lanes reach no other row).
-      int limit = 0x7fffffff;
-      bool valid = false;
-      if (r < s.rows) {
-        const int all = s.row0 + r, b = s.b < 0 ? all / p.rows_seq : s.b;
-        const int t = (s.b < 0 ? all % p.rows_seq : all) / p.group;
-        const Lens len = seq_lens(a, b);
-        valid = t < len.n;
-        if (valid) limit = s.b < 0 ? s.keys : max(0, s.keys - len.n + t + 1);
-      }
-      const bool active = __any_sync(0xffffffffu, valid);
-      int least = limit;
+      const int seen = r < n_rows ? visible(a, row_of(p, s.b, row0 + r), s.b < 0, s.keys) : -1;
+      valid = seen >= 0;
+      limit = valid ? seen : 0x7fffffff;
+      active = __any_sync(0xffffffffu, valid);
+      least = limit;
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) least = min(least, __shfl_xor_sync(0xffffffffu, least, o));
-
+    };
+    int g = 0;
+    bool ok = true;
+    int w = w0;
+    Seg s = next_seg(a, p.tile, scan, w, w1);
+    if (s.n > 0) load_rows(s);
+    while (s.n > 0) {
       float m = -CUDART_INF_F, l = 0.f;
       for (int j = 0; j < s.n; ++j, ++g) {
         const int k0 = (s.j0 + j) * BN, x = g & 1;
@@ -357,19 +450,26 @@ __global__ void __launch_bounds__(kThreads, 2)
         ptx::mbar_arrive(bar(L::P_READY + x));
       }
       if (!ok) break;
+      // The last S of this segment is done: the next segment's rows come in
+      // while its last P V runs.
+      const Seg cur = s;
+      const bool cur_valid = valid, cur_active = active;
+      s = next_seg(a, p.tile, scan, w, w1);
+      if (s.n > 0) load_rows(s);
       // The rows' partial results.
       if (!(ok = wait(L::O_DONE + ((g - 1) & 1), ((g - 1) >> 1) & 1))) break;
       ptx::tc_fence_after();
-      if (active) {
-        const int64_t row = s.b < 0 ? (int64_t)(s.unit + (int)blockIdx.x) * BM + r
-                                    : p.own_base + (int64_t)(s.unit + (int)blockIdx.x) * p.part_rows + r;
+      if (cur_active) {
+        const int64_t slot = cur.unit + (int)blockIdx.x;
+        const int64_t row = (cur.b < 0 ? p.tile.base_prefix + slot * p.tile.rows_prefix
+                                       : p.tile.base_own + slot * p.tile.rows_own) + r;
         const float inv = l > 0.f ? 1.f / l : 0.f;
 #pragma unroll
         for (int c = 0; c < D / 32; ++c) {
           uint32_t o[32];
           ptx::tmem_ld32(tmem + lane_base + C_O + 32 * c, o);
           ptx::tmem_wait_ld();
-          if (valid) {
+          if (cur_valid) {
 #pragma unroll
             for (int i = 0; i < 32; i += 8) {
               uint32_t v8[8];
@@ -379,7 +479,7 @@ __global__ void __launch_bounds__(kThreads, 2)
             }
           }
         }
-        if (valid) p.part_lse[row] = l > 0.f ? m + log2f(l) : -CUDART_INF_F;
+        if (cur_valid) p.part_lse[row] = l > 0.f ? m + log2f(l) : -CUDART_INF_F;
       }
       ptx::tc_fence_before();
     }
@@ -394,9 +494,9 @@ __global__ void __launch_bounds__(kThreads, 2)
     int item = 0;
     bool ok = true;
     for (int w = w0; w < w1 && ok;) {
-      const Seg s = locate(a, p, scan, w, w1);
-      w += s.n;
+      const Seg s = next_seg(a, p.tile, scan, w, w1);
       const int32_t* table = s.b < 0 ? a.prefix_pages : a.page_table + s.b * a.page_table_stride;
+      const int hk = head(s);
       for (int j = 0; j < s.n && ok; ++j) {
         const int k0 = (s.j0 + j) * BN;
         const int pieces = (min(BN, s.keys - k0) + box - 1) / box;  // pages past the list are not read
@@ -413,7 +513,7 @@ __global__ void __launch_bounds__(kThreads, 2)
           __syncwarp();
           if (mine)
             ptx::tma_load_4d(sbase + L::RING + slot * L::kTile + cb * (BN * 128) + piece * box * 128,
-                             kv ? &tm_v : &tm_k, bar(L::FULL + slot), 64 * cb, at, s.hk, page);
+                             kv ? &tm_v : &tm_k, bar(L::FULL + slot), 64 * cb, at, hk, page);
         }
       }
     }
@@ -444,8 +544,8 @@ __global__ void __launch_bounds__(kThreads, 2)
     int g = 0, seg = 0;
     bool ok = true;
     for (int w = w0; w < w1 && ok; ++seg) {
-      const Seg s = locate(a, p, scan, w, w1);
-      w += s.n;
+      const Seg s = next_seg(a, p.tile, scan, w, w1);
+      if (s.n == 0) break;
       if (!wait(L::Q_READY, seg & 1)) break;
       ptx::tc_fence_after();
       ok = issue_s(g) && (s.n < 2 || issue_s(g + 1));
@@ -477,61 +577,435 @@ __global__ void __launch_bounds__(kThreads, 2)
   }
 }
 
-// A warp per (sequence, query token, query head): joins the partial results
-// of the row's prefix and own stretches, in stretch order.
+// ---------------------------------------------------------------- warp kernel
+template <typename T>
+__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if constexpr (Pair<T>::kFmt == 1)
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// Four 8 x 8 matrices of 16-bit elements, a row address from each lane.
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ void ldsm4_t(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+
+// A worker is `split` warps, each with 16 of the unit's rows, that share a
+// ring of tiles (K and V of 32 keys, 128-byte swizzle).  The CTA's last warp
+// fills the rings by TMA, a lane per worker, running ahead across units; no
+// barrier of the CTA is in the loop.  A warp's step: S = Q K^T and O += P V as
+// 16 x 8 x 16 MMAs, Q's fragments and O in registers, K and V by ldmatrix.
+// With a few warps per scheduler the step is bound by its own chain of
+// instructions, so loads and look-ups are kept out of it.
+namespace warpk {
+constexpr int kMaxThreads = 384;
+__host__ __device__ constexpr int workers(int split) { return split == 4 ? 2 : split == 2 ? 5 : 6; }  // per CTA (one per SM)
+template <int D>
+struct Ring {
+  static constexpr uint32_t kHalf = kWarpKeys * 128;  // 64 dims of a tile's keys
+  static constexpr uint32_t kTile = (D / 64) * kHalf;
+  // 192 KB in flight per SM, shared by its workers.
+  __host__ __device__ static constexpr int stages(int split) { return 192 * 1024 / (workers(split) * 2 * (int)kTile); }
+  static size_t bytes(int split, int batch) {
+    return workers(split) * stages(split) * (2 * kTile + 16) + 8 + 4 * ((size_t)batch + 1) + 1024;
+  }
+};
+}  // namespace warpk
+
 template <typename T, int D>
-__global__ void __launch_bounds__(256) combine_kernel(const AiPrefixAttnArgs a, const Plan p, const int grid) {
+__global__ void __launch_bounds__(warpk::kMaxThreads, 1)
+    warp_kernel(const AiPrefixAttnArgs a, const Plan p, const int split, const __grid_constant__ CUtensorMap tm_k,
+                const __grid_constant__ CUtensorMap tm_v, const bool q_vec) {
+  using R = warpk::Ring<D>;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  constexpr int KS = D / 16, NB = D / 8;  // k steps of Q K^T, 8-dim blocks of O
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* sm = tile::align1024(smem_raw);
+  const uint32_t sbase = ptx::smem_u32(sm);
+  const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, r = lane / 4, c = lane % 4;
+  const int n_local = warpk::workers(split), n_warps = n_local * split;
+  // (lane i of the loading warp serves the CTA's worker i)
+  const int local = warp < n_warps ? warp / split : min(lane, n_local - 1);
+  const int stages = R::stages(split);
+  const uint32_t bars = sbase + n_local * stages * 2 * R::kTile;
+  volatile int* s_abort = reinterpret_cast<volatile int*>(sm + n_local * stages * (2 * R::kTile + 16));
+  int* scan = const_cast<int*>(s_abort) + 2;
+  auto full = [&](int st) { return bars + 16u * (uint32_t)(local * stages + st); };
+  auto empty = [&](int st) { return full(st) + 8; };
+  if (tid == 0) {
+    for (int i = 0; i < n_local * stages; ++i) {
+      ptx::mbar_init(bars + 16u * i, 1);
+      ptx::mbar_init(bars + 16u * i + 8, split);
+    }
+    *s_abort = 0;
+    ptx::fence_mbar_init();
+    ptx::prefetch_tmap(&tm_k);
+    ptx::prefetch_tmap(&tm_v);
+  }
+  if (warp == 0) {
+    if (p.warp.per_seq)
+      scan_own(a, kWarpKeys, p.warp.start, scan);
+    else if (lane == 0)
+      scan[0] = scan[a.batch] = 0;
+  }
+  __syncthreads();
+  if (blockIdx.x == 0 && p.warp.per_seq)
+    for (int b = tid; b <= a.batch; b += blockDim.x) p.scan[b] = scan[b];
+  const Split line = split_line(p.warp, line_total(p.warp, scan[a.batch]));
+  const int worker = blockIdx.x * n_local + local;
+  const bool busy = worker < line.n;
+  const int w0 = busy ? line.begin(worker) : 0, w1 = busy ? line.begin(worker + 1) : 0;
+  const float sl2 = a.scale * kLog2e;
+  const uint32_t ring = sbase + local * stages * 2 * R::kTile;
+
+  auto wait = [&](uint32_t bar, uint32_t parity) -> bool {
+    if (__all_sync(0xffffffffu, ptx::mbar_try_wait(bar, parity))) return true;
+    bool ok = !*s_abort;
+    if (ok && !ptx::mbar_wait(bar, parity, kWait)) {
+      report(a.status, AI_ERR_DEV_TIMEOUT);
+      *s_abort = 1;
+      ok = false;
+    }
+    return __all_sync(0xffffffffu, ok);
+  };
+
+  if (warp == n_warps) {
+    // ------------------------------------------------------------ loads
+    // Every lane walks its worker's stretch; a stage that is still in use is
+    // looked at again in the next round, after the other lanes' turns.
+    constexpr int CB = D / 64;
+    const int box = min(a.page_size, kWarpKeys), page_bits = 31 - __clz(a.page_size);
+    int w = w0, st = 0, turn = 0, j = 0;
+    Seg s{};
+    const int32_t* table = nullptr;
+    int hk = 0;
+    bool live = lane < n_local;
+    auto advance = [&]() {
+      s = next_seg(a, p.warp, scan, w, w1);
+      j = 0;
+      live = s.n > 0;
+      table = s.b < 0 ? a.prefix_pages : a.page_table + s.b * a.page_table_stride;
+      hk = s.sub % a.num_kv_heads;
+    };
+    if (live) advance();
+    long long last = clock64();
+    while (__any_sync(0xffffffffu, live)) {
+      bool moved = false;
+      if (live && (turn == 0 || ptx::mbar_test_wait(empty(st), (turn - 1) & 1))) {
+        const int k0 = (s.j0 + j) * kWarpKeys;
+        // (pages past the list are not read)
+        const int pieces = box == kWarpKeys ? 1 : (min(kWarpKeys, s.keys - k0) + box - 1) / box;
+        const uint32_t dst = ring + st * 2 * R::kTile;
+        ptx::mbar_arrive_expect_tx(full(st), (uint32_t)(pieces * box * D * 4));
+        for (int piece = 0; piece < pieces; ++piece) {
+          const int key = k0 + piece * box, at = key & (a.page_size - 1);
+          const int page = page_of(a, table, key >> page_bits);
+#pragma unroll
+          for (int cb = 0; cb < CB; ++cb) {
+            const uint32_t to = dst + cb * R::kHalf + piece * box * 128;
+            ptx::tma_load_4d(to, &tm_k, full(st), 64 * cb, at, hk, page);
+            ptx::tma_load_4d(to + R::kTile, &tm_v, full(st), 64 * cb, at, hk, page);
+          }
+        }
+        moved = true;
+        if (++st == stages) st = 0, ++turn;
+        if (++j == s.n) advance();
+      }
+      if (__any_sync(0xffffffffu, moved)) {
+        last = clock64();
+      } else if (__any_sync(0xffffffffu, *s_abort || clock64() - last > kWait)) {
+        if (!*s_abort) report(a.status, AI_ERR_DEV_TIMEOUT);
+        *s_abort = 1;
+        break;
+      }
+    }
+    // After a wait that gave up: the loads in flight land before the CTA ends.
+    if (*s_abort && lane < n_local)
+      for (int i = 0; i < stages; ++i) {
+        const int turns = turn + (i < st);  // loads of stage i
+        if (turns > 0) ptx::mbar_wait(full(i), (turns - 1) & 1, kWait);
+      }
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    return;
+  }
+
+  // Lane's place in an 8 x 8 matrix set (K by rows, V transposed): row and
+  // swizzled chunk offsets, for every second chunk of a 128-byte row.
+  const int mat = lane / 8, in = lane % 8;
+  const uint32_t k_row = ((mat >> 1) * 8 + in) * 128, v_row = ((mat & 1) * 8 + in) * 128;
+  uint32_t k_off[4], v_off[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    k_off[i] = k_row + (((2 * i + (mat & 1)) ^ in) << 4);
+    v_off[i] = v_row + (((2 * i + (mat >> 1)) ^ in) << 4);
+  }
+  int st = 0;
+  uint32_t turn = 0;  // parity of the stage's current load
+  bool ok = true;
+  for (int w = w0; w < w1 && ok;) {
+    const Seg s = next_seg(a, p.warp, scan, w, w1);
+    if (s.n == 0) break;
+    // (units go by groups of 16 split rows, then by KV head)
+    const int group = s.sub / a.num_kv_heads, hk = s.sub - group * a.num_kv_heads;
+    const int in_unit = (warp % split) * 16, row0 = group * 16 * split + in_unit;
+    const int n_rows = (s.b < 0 ? p.rows_all : p.rows_seq) - row0;  // of this warp, when positive
+    const bool any = n_rows > 0;
+    // Q's fragments of rows r and r + 8 (zero past the unit's rows), and the
+    // keys that those rows see.
+    uint32_t q[KS][4];
+    int seen[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int i = r + 8 * h;
+      const bool has = i < n_rows;
+      const Row x = row_of(p, s.b, has ? row0 + i : 0);
+      const T* src = static_cast<const T*>(a.q.ptr) + x.b * a.q.stride_b + (hk * p.group + x.g) * a.q.stride_h +
+                     x.t * a.q.stride_t + 2 * c;
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          uint32_t v;
+          if (q_vec) {
+            v = __ldg(reinterpret_cast<const uint32_t*>(src + 16 * ks + 8 * e));
+          } else {
+            const T pair[2] = {src[16 * ks + 8 * e], src[16 * ks + 8 * e + 1]};
+            memcpy(&v, pair, 4);
+          }
+          q[ks][h + 2 * e] = has ? v : 0u;
+        }
+      seen[h] = has ? visible(a, x, s.b < 0, s.keys) : -1;
+    }
+    // Tiles that end by `least` are seen whole (rows without a query see
+    // whatever there is and are not stored).
+    int least = min(seen[0] < 0 ? 0x7fffffff : seen[0], seen[1] < 0 ? 0x7fffffff : seen[1]);
+#pragma unroll
+    for (int d = 4; d < 32; d <<= 1) least = min(least, __shfl_xor_sync(0xffffffffu, least, d));
+    float o[NB][4];
+#pragma unroll
+    for (int i = 0; i < NB; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[i][e] = 0.f;
+    float m[2] = {-CUDART_INF_F, -CUDART_INF_F}, l[2] = {0.f, 0.f};
+
+    for (int j = s.j0; j < s.j0 + s.n; ++j) {
+      const int k0 = j * kWarpKeys;
+      const uint32_t kt = ring + st * 2 * R::kTile, vt = kt + R::kTile;
+      if (!(ok = wait(full(st), turn))) break;
+      if (any) {
+        float sc[4][4];
+#pragma unroll
+        for (int nt = 0; nt < 4; ++nt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) sc[nt][e] = 0.f;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            uint32_t k4[4];  // keys 16 half + 0..7 and 8..15, dims 16 ks + 0..7 and 8..15
+            ldsm4(k4, kt + k_off[ks & 3] + (ks >> 2) * R::kHalf + half * 2048);
+            mma16816<T>(sc[2 * half], q[ks], k4[0], k4[1]);
+            mma16816<T>(sc[2 * half + 1], q[ks], k4[2], k4[3]);
+          }
+        // Softmax of rows r (h = 0) and r + 8 (h = 1): the lane's keys are
+        // 8 nt + 2 c + {0, 1}.
+        float base[2], alpha[2] = {1.f, 1.f};
+        bool rescale = false;
+        if (k0 + kWarpKeys > least) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int lim = seen[h] - k0 - 2 * c;
+#pragma unroll
+            for (int nt = 0; nt < 4; ++nt)
+#pragma unroll
+              for (int e = 0; e < 2; ++e)
+                if (8 * nt + e >= lim) sc[nt][2 * h + e] = -CUDART_INF_F;
+          }
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          float mx = fmaxf(sc[0][2 * h], sc[0][2 * h + 1]);
+#pragma unroll
+          for (int nt = 1; nt < 4; ++nt) mx = ptx::fmax3(mx, sc[nt][2 * h], sc[nt][2 * h + 1]);
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2)) * sl2;
+          // (O is rescaled only when the maximum grows by more than 2^8)
+          if (mx > m[h] + 8.f) {
+            if (m[h] != -CUDART_INF_F) {
+              alpha[h] = ptx::ex2(m[h] - mx);
+              rescale = true;
+            }
+            m[h] = mx;
+          }
+          base[h] = m[h] == -CUDART_INF_F ? 0.f : m[h];
+        }
+        if (__any_sync(0xffffffffu, rescale)) {
+          l[0] *= alpha[0], l[1] *= alpha[1];
+#pragma unroll
+          for (int i = 0; i < NB; ++i) {
+            o[i][0] *= alpha[0], o[i][1] *= alpha[0];
+            o[i][2] *= alpha[1], o[i][3] *= alpha[1];
+          }
+        }
+        uint32_t pa[2][4];  // P's fragments of keys 0..15 and 16..31
+#pragma unroll
+        for (int nt = 0; nt < 4; ++nt)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const float p0 = ptx::ex2(fmaf(sc[nt][2 * h], sl2, -base[h]));
+            const float p1 = ptx::ex2(fmaf(sc[nt][2 * h + 1], sl2, -base[h]));
+            l[h] += p0 + p1;
+            pa[nt >> 1][(nt & 1) * 2 + h] = Pair<T>::pack(p0, p1);
+          }
+        const bool ragged = k0 + kWarpKeys > s.keys;
+#pragma unroll
+        for (int kk = 0; kk < 2; ++kk) {
+          // Slots past the list hold anything, NaN included, and meet P = 0:
+          // their values are cleared.
+          uint32_t keep[2] = {0xffffffffu, 0xffffffffu};
+          if (ragged) {
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const int left = s.keys - (k0 + 16 * kk + 8 * e + 2 * c);
+              keep[e] = left >= 2 ? 0xffffffffu : left == 1 ? 0xffffu : 0u;
+            }
+          }
+#pragma unroll
+          for (int i = 0; i < NB; i += 2) {
+            uint32_t v4[4];  // keys 16 kk + 0..7 and 8..15 of dims 8 i + 0..7, then of 8 (i + 1) + 0..7
+            ldsm4_t(v4, vt + v_off[(i >> 1) & 3] + (i >> 3) * R::kHalf + kk * 2048);
+            if (ragged) v4[0] &= keep[0], v4[1] &= keep[1], v4[2] &= keep[0], v4[3] &= keep[1];
+            mma16816<T>(o[i], pa[kk], v4[0], v4[1]);
+            mma16816<T>(o[i + 1], pa[kk], v4[2], v4[3]);
+          }
+        }
+      }
+      __syncwarp();
+      if (lane == 0) ptx::mbar_arrive(empty(st));
+      if (++st == stages) st = 0, turn ^= 1;
+    }
+    if (!ok) break;
+    // Partial rows: the lane's dims 8 i + 2 c + {0, 1} of rows r and r + 8.
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      float sum = l[h];
+      sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+      sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+      if (seen[h] < 0) continue;
+      const int64_t slot = s.unit + worker;
+      const int64_t row = (s.b < 0 ? p.warp.base_prefix + slot * p.warp.rows_prefix
+                                   : p.warp.base_own + slot * p.warp.rows_own) + in_unit + r + 8 * h;
+      const float inv = sum > 0.f ? 1.f / sum : 0.f;
+#pragma unroll
+      for (int i = 0; i < NB; ++i)
+        *reinterpret_cast<float2*>(p.part_o + row * D + 8 * i + 2 * c) = make_float2(o[i][2 * h] * inv, o[i][2 * h + 1] * inv);
+      if (c == 0) p.part_lse[row] = sum > 0.f ? m[h] + log2f(sum) : -CUDART_INF_F;
+    }
+  }
+  // The combine launch waits for this one; it must not end before the tile kernel's.
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+
+// ---------------------------------------------------------------- combine
+// `wide` warps per (sequence, query token, query head) join the partial
+// results of the row's prefix and own stretches: each takes every wide-th of
+// them, and the first adds up the warps' sums in order.
+template <typename T, int D>
+__global__ void __launch_bounds__(256) combine_kernel(const AiPrefixAttnArgs a, const Plan p, const int wide) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
   constexpr int E = D / 32;
-  const int b = blockIdx.y, lane = threadIdx.x % 32, item = blockIdx.x * 8 + threadIdx.x / 32;
-  if (item >= a.seq_len * a.num_q_heads) return;
-  const int t = item / a.num_q_heads, h = item % a.num_q_heads, hk = h / p.group;
+  __shared__ float s_acc[8][D + 2];
+  const int b = blockIdx.y, lane = threadIdx.x % 32, warp = threadIdx.x / 32, part = warp % wide;
+  const int item = blockIdx.x * (8 / wide) + warp / wide;
+  const bool has = item < a.seq_len * a.num_q_heads;
+  const int t = has ? item / a.num_q_heads : 0, h = has ? item % a.num_q_heads : 0, hk = h / p.group;
   const int rem = t * p.group + h % p.group;
   float M = -CUDART_INF_F, sum = 0.f, acc[E];
 #pragma unroll
   for (int e = 0; e < E; ++e) acc[e] = 0.f;
-  if (t < seq_lens(a, b).n) {
-    const int64_t before = (int64_t)p.units_prefix * p.tiles_prefix;
-    const int per = p.tt * a.num_kv_heads, s0 = p.scan[b], tiles = p.scan[b + 1] - s0;
-    const int64_t total = before + (int64_t)p.scan[a.batch] * per;
-    const int ctas = (int)min((int64_t)grid, total);
-    const int all = b * p.rows_seq + rem, up = hk * p.rt + all / BM;
-    const int own = (rem / BM) * a.num_kv_heads + hk;
-    int64_t row[2] = {0, 0}, step[2] = {BM, p.part_rows};
+  if (has && t < seq_lens(a, b).n) {
+    // (without room for own keys neither kernel has written the scan)
+    const bool own = a.max_pages > 0;
+    const int s0 = own ? p.scan[b] : 0, size = own ? p.scan[b + 1] - s0 : 0, own_all = own ? p.scan[a.batch] : 0;
+    int64_t row[2] = {0, 0}, step[2] = {0, 0};
     int n[2] = {0, 0};
-    if (p.units_prefix > 0) {
-      const int64_t w = (int64_t)up * p.tiles_prefix;
-      const int c = cta_of(w, total, ctas);
-      n[0] = cta_of(w + p.tiles_prefix - 1, total, ctas) - c + 1;
-      row[0] = (int64_t)(up + c) * BM + all % BM;
+    if (a.prefix_len > 0) {
+      const Line& l = p.prefix_warp ? p.warp : p.tile;
+      const int all = b * p.rows_seq + rem;
+      const int group_rows = p.prefix_warp ? 16 * p.split : BM;
+      const int unit = p.prefix_warp ? (all / group_rows) * a.num_kv_heads + hk : hk * p.rt + all / BM;
+      const Split line = split_line(l, line_total(l, own_all));
+      const int x = unit * (l.start + l.tiles_prefix) + l.start, first = line.worker(x);
+      n[0] = line.worker(x + l.tiles_prefix - 1) - first + 1;
+      step[0] = l.rows_prefix;
+      row[0] = l.base_prefix + (unit + first) * step[0] + all % group_rows;
     }
-    if (tiles > 0) {
-      const int64_t w = before + (int64_t)s0 * per + (int64_t)own * tiles;
-      const int c = cta_of(w, total, ctas);
-      n[1] = cta_of(w + tiles - 1, total, ctas) - c + 1;
-      row[1] = p.own_base + (int64_t)(b * per + own + c) * p.part_rows + rem % BM;
+    if (size > 0) {
+      const Line& l = p.own_warp ? p.warp : p.tile;
+      // (a sequence is one group of the warp kernel)
+      const int sub = p.own_warp ? hk : rem / BM * a.num_kv_heads + hk, unit = b * l.per_seq + sub;
+      const Split line = split_line(l, line_total(l, own_all));
+      const int x = l.units_prefix * (l.start + l.tiles_prefix) + s0 * l.per_seq + sub * size + l.start;
+      const int first = line.worker(x);
+      n[1] = line.worker(x + size - l.start - 1) - first + 1;
+      step[1] = l.rows_own;
+      row[1] = l.base_own + (unit + first) * step[1] + rem % BM;
     }
+    const int all_n = n[0] + n[1];
+    auto row_at = [&](int i) { return i < n[0] ? row[0] + i * step[0] : row[1] + (i - n[0]) * step[1]; };
+    for (int i = lane; i < all_n; i += 32) M = fmaxf(M, p.part_lse[row_at(i)]);
 #pragma unroll
-    for (int k = 0; k < 2; ++k)
-      for (int i = 0; i < n[k]; ++i) M = fmaxf(M, p.part_lse[row[k] + i * step[k]]);
+    for (int d = 16; d > 0; d >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, d));
     if (M != -CUDART_INF_F) {
-#pragma unroll
-      for (int k = 0; k < 2; ++k)
+      for (int i0 = part; i0 < all_n; i0 += 32 * wide) {
+        const int mine = i0 + lane * wide;
+        const float my_wgt = mine < all_n ? exp2f(p.part_lse[row_at(mine)] - M) : 0.f;
+        const int cnt = min(32, (all_n - i0 + wide - 1) / wide);
 #pragma unroll 4
-        for (int i = 0; i < n[k]; ++i) {
-          const int64_t rr = row[k] + i * step[k];
-          const float wgt = exp2f(p.part_lse[rr] - M);
+        for (int k = 0; k < cnt; ++k) {
+          const float wgt = __shfl_sync(0xffffffffu, my_wgt, k);
+          const float* src = p.part_o + row_at(i0 + k * wide) * D + E * lane;
           float o[E];
           if constexpr (E == 4)
-            *reinterpret_cast<float4*>(o) = *reinterpret_cast<const float4*>(p.part_o + rr * D + E * lane);
+            *reinterpret_cast<float4*>(o) = *reinterpret_cast<const float4*>(src);
           else
-            *reinterpret_cast<float2*>(o) = *reinterpret_cast<const float2*>(p.part_o + rr * D + E * lane);
+            *reinterpret_cast<float2*>(o) = *reinterpret_cast<const float2*>(src);
           sum += wgt;
 #pragma unroll
           for (int e = 0; e < E; ++e) acc[e] = fmaf(wgt, o[e], acc[e]);
         }
+      }
     }
   }
+  if (wide > 1) {
+    if (part > 0) {
+#pragma unroll
+      for (int e = 0; e < E; ++e) s_acc[warp][E * lane + e] = acc[e];
+      if (lane == 0) s_acc[warp][D] = sum;
+    }
+    __syncthreads();
+    if (part > 0) return;
+    for (int k = 1; k < wide; ++k) {
+      sum += s_acc[warp + k][D];
+#pragma unroll
+      for (int e = 0; e < E; ++e) acc[e] += s_acc[warp + k][E * lane + e];
+    }
+  }
+  if (!has) return;
   T* o = static_cast<T*>(a.out.ptr) + b * a.out.stride_b + h * a.out.stride_h + t * a.out.stride_t + E * lane;
 #pragma unroll
   for (int e = 0; e < E; ++e) o[e] = from_f32<T>(sum > 0.f ? acc[e] / sum : 0.f);
@@ -540,62 +1014,134 @@ __global__ void __launch_bounds__(256) combine_kernel(const AiPrefixAttnArgs a, 
         sum > 0.f ? (M + log2f(sum)) * kLn2 : -CUDART_INF_F;
 }
 
+// ---------------------------------------------------------------- host
 int sm_count() {
   int dev = 0, sms = 148;
   if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
   return sms;
 }
 
-// The launch's shape and the workspace's layout; false when the sizes do not fit.
-bool make_plan(const AiPrefixAttnArgs& a, Plan* p, int* ctas, size_t* bytes) {
-  const int64_t G = a.num_q_heads / a.num_kv_heads, rows = G * a.seq_len, all = rows * a.batch;
-  const int64_t tiles = ((int64_t)a.prefix_len + BN - 1) / BN, rt = (all + BM - 1) / BM, tt = (rows + BM - 1) / BM;
-  const int64_t most_own = ((int64_t)a.max_pages * a.page_size + BN - 1) / BN;
-  const int64_t units = tiles > 0 ? rt * a.num_kv_heads : 0, units_own = a.batch * tt * a.num_kv_heads;
-  const int64_t most = units * tiles + units_own * most_own;
-  if (all > 0x7fffffff || most > 0x7fffffff || units_own > 0x7fffffff) return false;
-  const int64_t slots = 2 * (int64_t)sm_count();
-  *ctas = (int)(most < 1 ? 1 : most < slots ? most : slots);
+// Warps of a warp-kernel worker for units of `rows` rows.
+int warp_split(int64_t rows) { return rows <= 16 ? 1 : rows <= 32 ? 2 : 4; }
+
+// The launches' shape and the workspace's layout; false when the sizes do not fit.
+bool make_plan(const AiPrefixAttnArgs& a, Plan* p, size_t* bytes) {
+  *p = Plan{};
+  const int64_t G = a.num_q_heads / a.num_kv_heads, rows = G * a.seq_len, all = rows * a.batch, H = a.num_kv_heads;
+  const int64_t capacity = (int64_t)a.max_pages * a.page_size;
+  if (all > 0x7fffffff || a.batch * ((rows + BM - 1) / BM) * H > 0x7fffffff) return false;
   p->group = (int)G;
   p->rows_seq = (int)rows;
   p->rows_all = (int)all;
-  p->tiles_prefix = (int)tiles;
-  p->rt = (int)rt;
-  p->tt = (int)tt;
-  p->units_prefix = (int)units;
-  p->part_rows = (int)(rows < BM ? rows : BM);
-  p->own_base = units > 0 ? (units + *ctas) * BM : 0;
-  const int64_t n = p->own_base + (units_own + *ctas) * p->part_rows;
+  p->rt = (int)((all + BM - 1) / BM);
+  p->tt = (int)((rows + BM - 1) / BM);
+  p->own_warp = rows <= kWarpRows;
+  p->split = warp_split(rows);
+  const int sms = sm_count(), workers = sms * warpk::workers(p->split);
+  // A prefix goes with the sequences' own keys to the warp kernel, in groups
+  // of rows that read it again each, while that gives a worker few positions
+  // (a launch of the tile kernel costs as much).
+  const int64_t group_rows = 16 * p->split, groups = (all + group_rows - 1) / group_rows;
+  p->prefix_warp = p->own_warp && groups * H * (kStartWarp + (a.prefix_len + kWarpKeys - 1) / kWarpKeys) <=
+                                      (int64_t)kShortPrefix * workers;
+  int64_t at = 0;  // rows of the partial results so far
+  auto line = [&](Line& l, bool prefix, bool own, int keys, int64_t units, int64_t per_seq, int64_t rows_prefix,
+                  int64_t rows_own, int64_t workers, int start, int least) {
+    const int64_t tiles = ((int64_t)a.prefix_len + keys - 1) / keys;
+    l.tiles_prefix = (int)tiles;
+    l.units_prefix = prefix && tiles > 0 ? (int)units : 0;
+    l.per_seq = own ? (int)per_seq : 0;
+    const int64_t most_own = (capacity + keys - 1) / keys;
+    const int64_t most = l.units_prefix * (start + tiles) +
+                         a.batch * (int64_t)l.per_seq * (most_own > 0 ? start + most_own : 0);
+    if (most > 0x7fffffff) return false;
+    const int64_t want = (most + least - 1) / least;
+    l.workers = (int)(want < workers ? want : workers);
+    l.least = least;
+    l.start = start;
+    l.rows_prefix = (int)rows_prefix;
+    l.rows_own = (int)rows_own;
+    if (l.units_prefix > 0) {
+      l.base_prefix = at;
+      at += (l.units_prefix + l.workers) * rows_prefix;
+    }
+    if (l.per_seq > 0) {
+      l.base_own = at;
+      at += (a.batch * (int64_t)l.per_seq + l.workers) * rows_own;
+    }
+    return true;
+  };
+  if (!line(p->tile, !p->prefix_warp, !p->own_warp, BN, p->rt * H, p->tt * H, BM, rows < BM ? rows : BM, 2 * sms,
+            kStartTile, kStartTile + 1))
+    return false;
+  if (!line(p->warp, p->prefix_warp, p->own_warp, kWarpKeys, groups * H, H, all < group_rows ? all : group_rows, rows,
+            workers, kStartWarp, 2))
+    return false;
   char* ws = static_cast<char*>(a.workspace);
-  size_t at = 0;
+  size_t off = 0;
   auto take = [&](size_t want) {
-    char* q = ws + at;
-    at += (want + 255) & ~size_t(255);
+    char* q = ws + off;
+    off += (want + 255) & ~size_t(255);
     return q;
   };
-  p->part_o = reinterpret_cast<float*>(take((size_t)n * a.head_dim * 4));
-  p->part_lse = reinterpret_cast<float*>(take((size_t)n * 4));
+  p->part_o = reinterpret_cast<float*>(take((size_t)at * a.head_dim * 4));
+  p->part_lse = reinterpret_cast<float*>(take((size_t)at * 4));
   p->scan = reinterpret_cast<int*>(take(((size_t)a.batch + 1) * 4));
-  *bytes = at;
+  *bytes = off;
   return true;
 }
 
 template <typename T, int D>
-int launch_t(const AiPrefixAttnArgs& a, const Plan& p, int ctas, const CUtensorMap& tk, const CUtensorMap& tv,
-             cudaStream_t st) {
-  const size_t smem = Smem<D>::bytes(a.batch);
-  if (cudaFuncSetAttribute(split_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
-    return AI_ERR_LAUNCH;
+int launch_t(const AiPrefixAttnArgs& a, const Plan& p, cudaStream_t st) {
   const bool q_vec = (reinterpret_cast<uintptr_t>(a.q.ptr) & 15) == 0 &&
                      ((a.q.stride_b | a.q.stride_h | a.q.stride_t) & 7) == 0;
   ProfScope ps(AI_PROF_PREFIX, st);
-  split_kernel<T, D><<<ctas, kThreads, smem, st>>>(a, p, tk, tv, q_vec);
-  if (cudaGetLastError() != cudaSuccess) return AI_ERR_LAUNCH;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)((a.seq_len * a.num_q_heads + 7) / 8), a.batch);
-  cfg.blockDim = dim3(256);
   cfg.stream = st;
-  if (cudaLaunchKernelEx(&cfg, combine_kernel<T, D>, a, p, ctas) != cudaSuccess) return AI_ERR_LAUNCH;
+  cfg.attrs = attr;
+  cfg.numAttrs = 0;  // the first launch follows whatever ran before in full
+  CUtensorMap tk, tv;
+  auto maps = [&](int keys) {
+    const int box = a.page_size < keys ? a.page_size : keys;
+    return sm100_make_map_of(&tk, a.k_pages, a.n_pages, a.num_kv_heads, a.page_size, box, D, a.dtype) &&
+           sm100_make_map_of(&tv, a.v_pages, a.n_pages, a.num_kv_heads, a.page_size, box, D, a.dtype);
+  };
+  auto smem_of = [&](auto kernel, size_t bytes) {
+    cfg.dynamicSmemBytes = bytes;
+    return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) == cudaSuccess;
+  };
+  if (p.tile.workers > 0) {
+    if (!maps(BN)) return AI_ERR_TMA;
+    if (!smem_of(tile_kernel<T, D>, Smem<D>::bytes(a.batch))) return AI_ERR_LAUNCH;
+    cfg.gridDim = dim3(p.tile.workers);
+    cfg.blockDim = dim3(kThreads);
+    if (cudaLaunchKernelEx(&cfg, tile_kernel<T, D>, a, p, tk, tv, q_vec) != cudaSuccess) return AI_ERR_LAUNCH;
+    cfg.numAttrs = 1;
+  }
+  if (p.warp.workers > 0) {
+    const int split = p.split, per = warpk::workers(split);
+    if (!maps(kWarpKeys)) return AI_ERR_TMA;
+    if (!smem_of(warp_kernel<T, D>, warpk::Ring<D>::bytes(split, a.batch))) return AI_ERR_LAUNCH;
+    cfg.gridDim = dim3((p.warp.workers + per - 1) / per);
+    cfg.blockDim = dim3(32 * (split * per + 1));
+    if (cudaLaunchKernelEx(&cfg, warp_kernel<T, D>, a, p, split, tk, tv, q_vec) != cudaSuccess) return AI_ERR_LAUNCH;
+    cfg.numAttrs = 1;
+  }
+  // Warps per row: one for every four partial results, while the rows leave
+  // the GPU's warps idle.
+  const Line& lp = p.prefix_warp ? p.warp : p.tile;
+  const int64_t rows = (int64_t)a.batch * a.seq_len * a.num_q_heads;
+  const int parts = lp.units_prefix > 0 ? lp.workers / lp.units_prefix : 1;
+  int wide = 1;
+  while (wide < 8 && 4 * wide < parts && 2 * wide * rows <= 32 * (int64_t)sm_count()) wide *= 2;
+  const int per = 8 / wide;
+  cfg.gridDim = dim3((unsigned)((a.seq_len * a.num_q_heads + per - 1) / per), a.batch);
+  cfg.blockDim = dim3(256);
+  cfg.dynamicSmemBytes = 0;
+  if (cudaLaunchKernelEx(&cfg, combine_kernel<T, D>, a, p, wide) != cudaSuccess) return AI_ERR_LAUNCH;
   return cudaGetLastError() == cudaSuccess ? AI_OK : AI_ERR_LAUNCH;
 }
 
@@ -612,36 +1158,26 @@ bool sm100_fits(const AiPrefixAttnArgs& a) {
     if (t->stride_b <= 0 || t->stride_h <= 0 || t->stride_t <= 0) return false;
   }
   tc::Plan p;
-  int ctas;
   size_t bytes;
-  return tc::make_plan(a, &p, &ctas, &bytes);
+  return tc::make_plan(a, &p, &bytes);
 }
 
 size_t sm100_workspace(const AiPrefixAttnArgs& a) {
   tc::Plan p;
-  int ctas;
   size_t bytes = 0;
-  tc::make_plan(a, &p, &ctas, &bytes);
+  tc::make_plan(a, &p, &bytes);
   return bytes;
 }
 
 int sm100_launch(const AiPrefixAttnArgs& a, cudaStream_t st) {
   tc::Plan p;
-  int ctas;
   size_t bytes;
-  if (!tc::make_plan(a, &p, &ctas, &bytes)) return AI_ERR_SHAPE;
+  if (!tc::make_plan(a, &p, &bytes)) return AI_ERR_SHAPE;
   if (!a.workspace || a.workspace_bytes < bytes) return AI_ERR_WORKSPACE;
   if (reinterpret_cast<uintptr_t>(a.workspace) & 255) return AI_ERR_ALIGN;
-  const int box = a.page_size < tc::BN ? a.page_size : tc::BN;
-  CUtensorMap tk, tv;
-  if (!sm100_make_map_of(&tk, a.k_pages, a.n_pages, a.num_kv_heads, a.page_size, box, a.head_dim, a.dtype) ||
-      !sm100_make_map_of(&tv, a.v_pages, a.n_pages, a.num_kv_heads, a.page_size, box, a.head_dim, a.dtype))
-    return AI_ERR_TMA;
   if (a.dtype == AI_DTYPE_BF16)
-    return a.head_dim == 128 ? tc::launch_t<__nv_bfloat16, 128>(a, p, ctas, tk, tv, st)
-                             : tc::launch_t<__nv_bfloat16, 64>(a, p, ctas, tk, tv, st);
-  return a.head_dim == 128 ? tc::launch_t<__half, 128>(a, p, ctas, tk, tv, st)
-                           : tc::launch_t<__half, 64>(a, p, ctas, tk, tv, st);
+    return a.head_dim == 128 ? tc::launch_t<__nv_bfloat16, 128>(a, p, st) : tc::launch_t<__nv_bfloat16, 64>(a, p, st);
+  return a.head_dim == 128 ? tc::launch_t<__half, 128>(a, p, st) : tc::launch_t<__half, 64>(a, p, st);
 }
 
 }  // namespace prefix
