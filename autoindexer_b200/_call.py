@@ -1,4 +1,8 @@
-"""Argument checks and the launch shared by the operator wrappers."""
+"""Argument checks and the launch shared by the operator wrappers.
+
+A decode step calls several small operators, so these stay short: devices are
+compared as indices, and a struct is filled with one constructor call where it
+can be."""
 
 from __future__ import annotations
 
@@ -9,8 +13,25 @@ import torch
 from torch import Tensor
 
 from . import _lib
+from .attention import status_word
 
 _DTYPES = {torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_F16, torch.float32: _lib.DTYPE_F32}
+_status_ptrs = {}  # device index -> address of its status word (status_word keeps the tensor)
+
+
+def _stream_of(index: int) -> int:
+    return torch.cuda.current_stream(index).cuda_stream
+
+
+# (torch's own lookup without the Stream object around it, where there is one)
+raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", _stream_of)
+
+
+def status_ptr(index: int) -> int:
+    ptr = _status_ptrs.get(index)
+    if ptr is None:
+        ptr = _status_ptrs[index] = status_word(torch.device("cuda", index)).data_ptr()
+    return ptr
 
 
 def dtype_code(x: Tensor, name: str) -> int:
@@ -25,86 +46,89 @@ def dense_d(x: Tensor) -> Tensor:
 
 
 def t4(x: Tensor) -> "_lib.AiTensor4":
-    s = x.stride()
-    return _lib.AiTensor4(x.data_ptr(), s[0], s[1], s[2])
+    return _lib.AiTensor4(x.data_ptr(), *x.stride()[:3])
 
 
-def on_device(name: str, x: Tensor, device: torch.device) -> None:
-    if x.device != device:
-        raise RuntimeError(f"{name} is on {x.device}, expected {device}")
+def on_device(name: str, x: Tensor, index: int) -> None:
+    if x.get_device() != index:
+        raise RuntimeError(f"{name} is on {x.device}, expected cuda:{index}")
 
 
-def cuda_device(name: str, x: Tensor) -> torch.device:
+def cuda_index(name: str, x: Tensor) -> int:
     if not x.is_cuda:
         raise RuntimeError(f"autoindexer_b200 operators run on CUDA tensors only ({name} is on {x.device})")
-    return x.device
+    return x.get_device()
 
 
-def ints(name: str, x: Tensor, shape: Tuple[int, ...], device: torch.device) -> Tensor:
-    """An int32 tensor of ``shape`` on ``device`` with its last dimension contiguous."""
-    if x.dtype != torch.int32:
-        raise TypeError(f"{name} must be int32, got {x.dtype}")
-    if tuple(x.shape) != shape:
+def _typed(name: str, x: Tensor, dtype, shape: Tuple[int, ...], index: int) -> None:
+    if x.dtype is not dtype:
+        raise TypeError(f"{name} must be {dtype}, got {x.dtype}")
+    if x.shape != shape:
         raise ValueError(f"{name} must have shape {shape}, got {tuple(x.shape)}")
-    on_device(name, x, device)
+    if x.get_device() != index:
+        on_device(name, x, index)
+
+
+def ints(name: str, x: Tensor, shape: Tuple[int, ...], index: int) -> Tensor:
+    """An int32 tensor of ``shape`` on the device with its last dimension contiguous."""
+    _typed(name, x, torch.int32, shape, index)
     return x if x.stride(-1) == 1 else x.contiguous()
 
 
-def floats(name: str, x: Tensor, shape: Tuple[int, ...], device: torch.device) -> Tensor:
-    """A contiguous float32 tensor of ``shape`` on ``device``."""
-    if x.dtype != torch.float32:
-        raise TypeError(f"{name} must be float32, got {x.dtype}")
-    if tuple(x.shape) != shape:
-        raise ValueError(f"{name} must have shape {shape}, got {tuple(x.shape)}")
-    on_device(name, x, device)
+def floats(name: str, x: Tensor, shape: Tuple[int, ...], index: int) -> Tensor:
+    """A contiguous float32 tensor of ``shape`` on the device."""
+    _typed(name, x, torch.float32, shape, index)
     return x.contiguous()
 
 
-def fill_rope(a, rope, positions: Optional[Tensor], batch: int, seq_len: int, head_dim: int, device):
+def fill_rope(a, rope, positions: Optional[Tensor], batch: int, seq_len: int, head_dim: int, index: int):
     """Sets the rotary table and the position ids of ``a``; returns the
-    tensors to keep alive until the launch."""
+    tensors to keep alive until the launch (cos, sin, positions)."""
     if rope is None:
         if positions is not None:
             raise ValueError("positions without a rope table")
-        return None
+        return None, None, None
     if positions is None:
         raise ValueError("a rope table needs positions")
     cos, sin = rope
-    shape = (cos.shape[0], head_dim // 2)
-    cos, sin = floats("rope cos", cos, shape, device), floats("rope sin", sin, shape, device)
-    if shape[0] == 0:
+    n = cos.shape[0]
+    shape = (n, head_dim // 2)
+    cos, sin = floats("rope cos", cos, shape, index), floats("rope sin", sin, shape, index)
+    if n == 0:
         raise ValueError("the rope table is empty")
-    if positions.dtype not in (torch.int64, torch.int32):
+    is_int64 = positions.dtype is torch.int64
+    if not is_int64 and positions.dtype is not torch.int32:
         raise TypeError(f"positions must be int64 or int32, got {positions.dtype}")
-    rows = 1 if positions.dim() == 1 else positions.shape[0]
-    if positions.dim() > 2 or positions.shape[-1] != seq_len or rows not in (1, batch):
-        raise ValueError(f"positions must be ({seq_len},) or ({batch}, {seq_len}), got {tuple(positions.shape)}")
-    on_device("positions", positions, device)
+    dims = positions.shape
+    rows = 1 if len(dims) == 1 else dims[0] if dims else 0
+    if len(dims) > 2 or rows not in (1, batch) or dims[-1] != seq_len:
+        raise ValueError(f"positions must be ({seq_len},) or ({batch}, {seq_len}), got {tuple(dims)}")
+    on_device("positions", positions, index)
     if positions.stride(-1) != 1:
         positions = positions.contiguous()
-    a.rope_cos, a.rope_sin, a.n_pos = cos.data_ptr(), sin.data_ptr(), shape[0]
-    a.pos.ptr = positions.data_ptr()
-    a.pos.stride_b = positions.stride(0) if rows > 1 else 0
-    a.pos.is_int64 = positions.dtype == torch.int64
+    a.rope_cos, a.rope_sin, a.n_pos = cos.data_ptr(), sin.data_ptr(), n
+    a.pos = _lib.AiPositions(positions.data_ptr(), positions.stride(0) if rows > 1 else 0, is_int64)
     return cos, sin, positions
 
 
-def head_weight(name: str, w: Optional[Tensor], x: Tensor) -> Optional[Tensor]:
+def head_weight(name: str, w: Optional[Tensor], x: Tensor, index: int) -> Optional[Tensor]:
     """A norm weight ``(D,)`` of ``x``'s dtype or float32."""
     if w is None:
         return None
-    if tuple(w.shape) != (x.shape[-1],):
+    if w.shape != x.shape[-1:]:
         raise ValueError(f"{name} must have shape ({x.shape[-1]},), got {tuple(w.shape)}")
-    if w.dtype not in (x.dtype, torch.float32):
+    if w.dtype is not x.dtype and w.dtype is not torch.float32:
         raise TypeError(f"{name} must be {x.dtype} or float32, got {w.dtype}")
-    on_device(name, w, x.device)
+    on_device(name, w, index)
     return w.contiguous()
 
 
 def workspace(query, args, device: torch.device, what: str) -> Optional[Tensor]:
     """Allocates what the library asks for and sets it in ``args``."""
     n = ctypes.c_size_t(0)
-    _lib.check(query(ctypes.byref(args), ctypes.byref(n)), what)
+    code = query(args, n)
+    if code:
+        _lib.check(code, what)
     if not n.value:
         return None
     ws = torch.empty(n.value, dtype=torch.uint8, device=device)
@@ -112,10 +136,11 @@ def workspace(query, args, device: torch.device, what: str) -> Optional[Tensor]:
     return ws
 
 
-def launch(fn, args, device: torch.device, what: str) -> None:
+def launch(fn, args, index: int, what: str) -> None:
     """Runs one library call on the device's current stream."""
-    if device.index == torch.cuda.current_device():
-        _lib.check(fn(ctypes.byref(args), torch.cuda.current_stream(device).cuda_stream), what)
-        return
-    with torch.cuda.device(device):
-        _lib.check(fn(ctypes.byref(args), torch.cuda.current_stream(device).cuda_stream), what)
+    if index != torch.cuda.current_device():
+        with torch.cuda.device(index):
+            return launch(fn, args, index, what)
+    code = fn(args, raw_stream(index))
+    if code:
+        _lib.check(code, what)

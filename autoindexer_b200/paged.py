@@ -18,29 +18,29 @@ import torch
 from torch import Tensor
 
 from . import _call, _lib
-from .attention import status_word
 
 __all__ = ["paged_append", "shared_prefix_attention"]
 
 
-def _pools(k_pages: Tensor, v_pages: Tensor, heads: int, head_dim: int, dtype, device) -> None:
-    if k_pages.dim() != 4 or k_pages.shape != v_pages.shape or k_pages.shape[1] != heads or k_pages.shape[3] != head_dim:
+def _pools(k_pages: Tensor, v_pages: Tensor, heads: int, head_dim: int, dtype, index: int) -> None:
+    s = k_pages.shape
+    if len(s) != 4 or s != v_pages.shape or s[1] != heads or s[3] != head_dim:
         raise ValueError(f"k_pages and v_pages must be (n_pages, {heads}, page_size, {head_dim}), got "
                          f"{tuple(k_pages.shape)} and {tuple(v_pages.shape)}")
+    if s[0] == 0 or s[2] == 0:
+        raise ValueError("k_pages and v_pages are empty")
     for name, p in (("k_pages", k_pages), ("v_pages", v_pages)):
-        if p.dtype != dtype:
+        if p.dtype is not dtype:
             raise TypeError(f"{name} is {p.dtype}, the call's tensors {dtype}")
         if p.stride(3) != 1:
             raise ValueError(f"{name} must have a contiguous last dimension")
-        if p.numel() == 0:
-            raise ValueError(f"{name} is empty")
-        _call.on_device(name, p, device)
+        _call.on_device(name, p, index)
 
 
-def _table(page_table: Tensor, batch: int, device) -> Tensor:
+def _table(page_table: Tensor, batch: int, index: int) -> Tensor:
     if page_table.dim() != 2:
         raise ValueError(f"page_table must be ({batch}, max_pages), got {tuple(page_table.shape)}")
-    return _call.ints("page_table", page_table, (batch, page_table.shape[1]), device)
+    return _call.ints("page_table", page_table, (batch, page_table.shape[1]), index)
 
 
 def paged_append(key: Tensor, value: Tensor, k_pages: Tensor, v_pages: Tensor, page_table: Tensor, lens: Tensor,
@@ -59,7 +59,7 @@ def paged_append(key: Tensor, value: Tensor, k_pages: Tensor, v_pages: Tensor, p
     of one dtype (bfloat16, float16, float32), head_dim 32, 64 or 128, any
     page size, any strides with the last dimension contiguous.  Two tokens
     given the same slot race; no gradient flows through the cache."""
-    device = _call.cuda_device("key", key)
+    index = _call.cuda_index("key", key)
     if key.dim() != 4 or key.shape != value.shape:
         raise ValueError(f"key and value must be (B, Hkv, T, D), got {tuple(key.shape)} and {tuple(value.shape)}")
     B, H, T, D = key.shape
@@ -69,13 +69,13 @@ def paged_append(key: Tensor, value: Tensor, k_pages: Tensor, v_pages: Tensor, p
         raise ValueError(f"head_dim must be 32, 64 or 128, got {D}")
     if value.dtype != key.dtype:
         raise TypeError(f"value is {value.dtype}, key {key.dtype}")
-    _call.on_device("value", value, device)
-    _pools(k_pages, v_pages, H, D, key.dtype, device)
-    page_table = _table(page_table, B, device)
+    _call.on_device("value", value, index)
+    _pools(k_pages, v_pages, H, D, key.dtype, index)
+    page_table = _table(page_table, B, index)
     if page_table.shape[1] == 0:
         raise ValueError("page_table has no columns")
-    lens = _call.ints("lens", lens, (B,), device)
-    w = _call.head_weight("key_weight", key_weight, key)
+    lens = _call.ints("lens", lens, (B,), index)
+    w = _call.head_weight("key_weight", key_weight, key, index)
     k, v = _call.dense_d(key), _call.dense_d(value)
     a = _lib.AiPagedAppendArgs()
     a.batch, a.num_kv_heads, a.seq_len, a.head_dim = B, H, T, D
@@ -87,13 +87,13 @@ def paged_append(key: Tensor, value: Tensor, k_pages: Tensor, v_pages: Tensor, p
     a.page_table, a.page_table_stride, a.max_pages = page_table.data_ptr(), page_table.stride(0), page_table.shape[1]
     a.lens = lens.data_ptr()
     if new_lens is not None:
-        new_lens = _call.ints("new_lens", new_lens, (B,), device)
+        new_lens = _call.ints("new_lens", new_lens, (B,), index)
         a.new_lens = new_lens.data_ptr()
     if w is not None:
         a.k_weight = w.data_ptr()
-    keep = _call.fill_rope(a, rope, positions, B, T, D, device)
-    a.status = status_word(device).data_ptr()
-    _call.launch(_lib.lib().ai_paged_append, a, device, "ai_paged_append")
+    keep = _call.fill_rope(a, rope, positions, B, T, D, index)
+    a.status = _call.status_ptr(index)
+    _call.launch(_lib.lib().ai_paged_append, a, index, "ai_paged_append")
     del keep
 
 
@@ -117,7 +117,7 @@ def shared_prefix_attention(query: Tensor, k_pages: Tensor, v_pages: Tensor, pre
     the sequence sees must hold finite values; the slots past them may hold
     anything.  A length or page out of range is clamped and sets the status
     word."""
-    device = _call.cuda_device("query", query)
+    index = _call.cuda_index("query", query)
     if query.dim() != 4 or query.numel() == 0:
         raise ValueError(f"query must be (B, Hq, T, D) and not empty, got {tuple(query.shape)}")
     B, Hq, T, D = query.shape
@@ -126,14 +126,20 @@ def shared_prefix_attention(query: Tensor, k_pages: Tensor, v_pages: Tensor, pre
     heads = k_pages.shape[1] if k_pages.dim() == 4 else 0
     if heads == 0 or Hq % heads != 0:
         raise ValueError(f"num_q_heads {Hq} is not a multiple of num_kv_heads {heads}")
-    _pools(k_pages, v_pages, heads, D, query.dtype, device)
+    _pools(k_pages, v_pages, heads, D, query.dtype, index)
     S = k_pages.shape[2]
-    page_table = _table(page_table, B, device)
-    lens = _call.ints("lens", lens, (B,), device)
+    page_table = _table(page_table, B, index)
+    lens = _call.ints("lens", lens, (B,), index)
     prefix_len = int(prefix_len)
     if prefix_len < 0:
         raise ValueError(f"prefix_len {prefix_len} is negative")
+    device = query.device
     q = _call.dense_d(query)
+    st = q.stride()
+    if q.data_ptr() % 16 or (st[0] | st[1] | st[2]) * q.element_size() % 16:
+        q = q.contiguous()  # the kernels read 16-byte pieces of its rows
+        if q.data_ptr() % 16:
+            q = q.clone()
     out = torch.empty((B, T, Hq, D), dtype=query.dtype, device=device)
     a = _lib.AiPrefixAttnArgs()
     a.batch, a.num_q_heads, a.seq_len, a.head_dim = B, Hq, T, D
@@ -146,21 +152,21 @@ def shared_prefix_attention(query: Tensor, k_pages: Tensor, v_pages: Tensor, pre
     if prefix_len:
         if prefix_pages is None or prefix_pages.dim() != 1 or prefix_pages.shape[0] * S < prefix_len:
             raise ValueError(f"prefix_pages must list the pages of {prefix_len} keys ({S} a page)")
-        prefix_pages = _call.ints("prefix_pages", prefix_pages, tuple(prefix_pages.shape), device)
+        prefix_pages = _call.ints("prefix_pages", prefix_pages, tuple(prefix_pages.shape), index)
         a.prefix_pages = prefix_pages.data_ptr()
     a.prefix_len = prefix_len
     a.page_table, a.page_table_stride, a.max_pages = page_table.data_ptr(), page_table.stride(0), page_table.shape[1]
     a.lens = lens.data_ptr()
     if query_lens is not None:
-        query_lens = _call.ints("query_lens", query_lens, (B,), device)
+        query_lens = _call.ints("query_lens", query_lens, (B,), index)
         a.query_lens = query_lens.data_ptr()
     lse = None
     if return_lse:
         lse = torch.empty((B, Hq, T), dtype=torch.float32, device=device)
         a.lse = lse.data_ptr()
-    a.status = status_word(device).data_ptr()
+    a.status = _call.status_ptr(index)
     lib = _lib.lib()
     ws = _call.workspace(lib.ai_prefix_attn_workspace, a, device, "ai_prefix_attn_workspace")
-    _call.launch(lib.ai_prefix_attn, a, device, "ai_prefix_attn")
+    _call.launch(lib.ai_prefix_attn, a, index, "ai_prefix_attn")
     del ws
     return (out, lse) if return_lse else out

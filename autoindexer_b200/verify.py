@@ -14,7 +14,6 @@ import torch
 from torch import Tensor
 
 from . import _call, _lib
-from .attention import status_word
 
 __all__ = ["verify_draft"]
 
@@ -44,7 +43,7 @@ def verify_draft(target_logits: Tensor, draft_tokens: Tensor, uniforms: Tensor, 
     Logits are CUDA bfloat16, float16 or float32, finite or ``-inf``, with a
     contiguous vocabulary; up to 64 drafted tokens.  A token outside the
     vocabulary is refused and sets the status word."""
-    device = _call.cuda_device("target_logits", target_logits)
+    index, device = _call.cuda_index("target_logits", target_logits), target_logits.device
     if target_logits.dim() != 3 or target_logits.numel() == 0:
         raise ValueError(f"target_logits must be (B, L + 1, V) and not empty, got {tuple(target_logits.shape)}")
     B, rows, V = target_logits.shape
@@ -55,10 +54,10 @@ def verify_draft(target_logits: Tensor, draft_tokens: Tensor, uniforms: Tensor, 
         raise TypeError(f"draft_tokens must be int64, got {draft_tokens.dtype}")
     if tuple(draft_tokens.shape) != (B, L):
         raise ValueError(f"draft_tokens must have shape {(B, L)}, got {tuple(draft_tokens.shape)}")
-    _call.on_device("draft_tokens", draft_tokens, device)
+    _call.on_device("draft_tokens", draft_tokens, index)
     draft_tokens = draft_tokens.contiguous()
-    uniforms = _call.floats("uniforms", uniforms, (B, L), device)
-    noise = _call.floats("noise", noise, (B, V), device)
+    uniforms = _call.floats("uniforms", uniforms, (B, L), index)
+    noise = _call.floats("noise", noise, (B, V), index)
     target = _call.dense_d(target_logits)
     a = _lib.AiVerifyArgs()
     a.batch, a.n_draft, a.vocab = B, L, V
@@ -70,25 +69,25 @@ def verify_draft(target_logits: Tensor, draft_tokens: Tensor, uniforms: Tensor, 
             raise ValueError(f"draft_logits must have shape {(B, L, V)}, got {tuple(draft_logits.shape)}")
         if draft_logits.dtype != target.dtype:
             raise TypeError(f"draft_logits is {draft_logits.dtype}, target_logits {target.dtype}")
-        _call.on_device("draft_logits", draft_logits, device)
+        _call.on_device("draft_logits", draft_logits, index)
         draft_logits = _call.dense_d(draft_logits)
         if L:
             a.draft = draft_logits.data_ptr()
             a.draft_stride_b, a.draft_stride_t = draft_logits.stride(0), draft_logits.stride(1)
     if draft_lens is not None:
-        draft_lens = _call.ints("draft_lens", draft_lens, (B,), device)
+        draft_lens = _call.ints("draft_lens", draft_lens, (B,), index)
         a.draft_lens = draft_lens.data_ptr()
     if temperature is not None:
-        temperature = _call.floats("temperature", temperature, (B,), device)
+        temperature = _call.floats("temperature", temperature, (B,), index)
         a.temperature = temperature.data_ptr()
     accepted = torch.empty(B, dtype=torch.int32, device=device)
     tokens = torch.empty((B, rows), dtype=torch.int64, device=device)
     logprobs = torch.empty((B, rows), dtype=torch.float32, device=device)
     a.tokens, a.uniforms, a.noise = draft_tokens.data_ptr(), uniforms.data_ptr(), noise.data_ptr()
     a.accepted, a.out_tokens, a.logprobs = accepted.data_ptr(), tokens.data_ptr(), logprobs.data_ptr()
-    a.status = status_word(device).data_ptr()
+    a.status = _call.status_ptr(index)
     lib = _lib.lib()
     ws = _call.workspace(lib.ai_verify_draft_workspace, a, device, "ai_verify_draft_workspace")
-    _call.launch(lib.ai_verify_draft, a, device, "ai_verify_draft")
+    _call.launch(lib.ai_verify_draft, a, index, "ai_verify_draft")
     del ws
     return accepted, tokens, logprobs
