@@ -40,29 +40,35 @@ namespace prefix {
 namespace tc {
 
 constexpr int BM = 128, BN = 64;
-constexpr int kThreads = 192;
-constexpr int kMaxBatch = 2048;  // the tile scan of the sequences sits in shared memory
-constexpr uint32_t kTmemCols = 256;
-constexpr uint32_t C_S = 0;    // two S buffers of 64 columns (P over their first 32)
-constexpr uint32_t C_O = 128;  // D columns
+constexpr int kMaxBatch = 2048;  // the scan of the sequences sits in shared memory
 constexpr long long kWait = 1000000000LL;
 
-template <int D>
+// Threads of a tile-kernel CTA with NT row tiles: a softmax warpgroup each, a
+// TMA and an MMA warp.
+__host__ __device__ constexpr int tile_threads(int NT) { return 128 * NT + 64; }
+
+template <int D, int NT>
 struct Smem {
   static constexpr uint32_t kTile = BN * D * 2;    // one K or V tile: D / 64 column blocks of 64 rows x 128 bytes
-  static constexpr uint32_t kQBlock = BM * 128;    // one column block of Q
-  static constexpr int kSlots = D == 128 ? 4 : 8;  // ring of tiles, K and V alternating (64 KB)
+  static constexpr uint32_t kQBlock = BM * 128;    // one column block of a Q tile
+  static constexpr uint32_t kQ = BM * D * 2;
+  static constexpr int kSlots = NT * (D == 128 ? 4 : 8);  // ring of tiles, K and V alternating (64 KB per row tile)
   static constexpr uint32_t Q = 0;
-  static constexpr uint32_t RING = Q + BM * D * 2;
+  static constexpr uint32_t RING = Q + NT * kQ;
   static constexpr uint32_t BARS = RING + kSlots * kTile;
-  static constexpr int FULL = 0, EMPTY = kSlots, S_FULL = 2 * kSlots, P_READY = S_FULL + 2, O_DONE = P_READY + 2,
-                       Q_READY = O_DONE + 2, FINAL = Q_READY + 1, N_BARS = FINAL + 1;
+  // (two of each per row tile, for the two S buffers)
+  static constexpr int FULL = 0, EMPTY = kSlots, S_FULL = 2 * kSlots, P_READY = S_FULL + 2 * NT,
+                       O_DONE = P_READY + 2 * NT, Q_READY = O_DONE + 2 * NT, FINAL = Q_READY + NT, N_BARS = FINAL + 1;
   static constexpr uint32_t TMEM_SLOT = BARS + 8 * N_BARS;
   static constexpr uint32_t ABORT = TMEM_SLOT + 4;
   static constexpr uint32_t SCAN = ABORT + 4;  // int [B + 1]
   static size_t bytes(int batch) { return SCAN + 4 * ((size_t)batch + 1) + 1024; }
+  // TMEM: two S buffers of 64 columns per row tile (P over their first 32), then O of D columns each.
+  static constexpr uint32_t kTmemCols = 256 * NT;
+  static constexpr uint32_t C_S = 0, C_O = 128 * NT;
 };
-static_assert(2 * (Smem<128>::SCAN + 4 * (kMaxBatch + 1) + 1024 + 1024) <= 228 * 1024, "two CTAs per SM");
+static_assert(2 * (Smem<128, 1>::SCAN + 4 * (kMaxBatch + 1) + 1024 + 1024) <= 228 * 1024, "two CTAs per SM");
+static_assert(Smem<128, 2>::SCAN + 4 * (kMaxBatch + 1) + 1024 <= 227 * 1024, "one CTA per SM");
 
 constexpr int kWarpRows = 64;   // most rows of a sequence on the warp kernel
 constexpr int kWarpKeys = 32;   // keys of its tile
@@ -81,8 +87,8 @@ struct Line {
   int units_prefix;   // prefix units on this line, each of tiles_prefix tiles
   int tiles_prefix;
   int per_seq;        // units per sequence on this line (0: own keys are not on it)
-  int rows_prefix;    // rows of a prefix slot
-  int rows_own;       // rows of an own slot
+  int rows_prefix;    // rows of a prefix unit (and of its slots)
+  int rows_own;       // rows of a sequence's unit
   int64_t base_prefix, base_own;  // first row of each region; slot (unit + worker) follows
 };
 
@@ -91,7 +97,8 @@ struct Plan {
   int group;        // G: query heads per KV head
   int rows_seq;     // T G
   int rows_all;     // B T G
-  int rt, tt;       // tile kernel: row tiles of all rows / of one sequence
+  int nt;           // row tiles of a tile-kernel CTA
+  int rt;           // units of a KV head's rows of the prefix, on the tile kernel
   int split;        // warps of a warp-kernel worker
   bool prefix_warp, own_warp;  // which kernel has the list
   Line tile, warp;
@@ -244,12 +251,16 @@ __host__ __device__ constexpr uint32_t idesc(uint32_t fmt, int M, int N, bool b_
          ((uint32_t)(M >> 4) << 24);
 }
 
-template <typename T, int D>
-__global__ void __launch_bounds__(kThreads, 2)
+// NT = 1: up to 128 rows a unit, two CTAs per SM whose phases fill each
+// other's gaps; NT = 2: up to 256, halved over two row tiles that share every
+// K and V tile (each is read from L2 once, not twice), one CTA per SM.
+template <typename T, int D, int NT>
+__global__ void __launch_bounds__(tile_threads(NT), NT == 1 ? 2 : 1)
     tile_kernel(const AiPrefixAttnArgs a, const Plan p, const __grid_constant__ CUtensorMap tm_k,
-                 const __grid_constant__ CUtensorMap tm_v, const bool q_vec) {
-  using L = Smem<D>;
-  constexpr int CB = D / 64;
+                const __grid_constant__ CUtensorMap tm_v) {
+  using L = Smem<D, NT>;
+  constexpr int CB = D / 64, kTma = 4 * NT, kMma = kTma + 1;
+  constexpr uint32_t C_S = L::C_S, C_O = L::C_O;
   // (the warp kernel reads nothing this one writes)
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   extern __shared__ uint8_t smem_raw[];
@@ -262,14 +273,14 @@ __global__ void __launch_bounds__(kThreads, 2)
 
   if (tid == 0) {
     for (int i = 0; i < L::N_BARS; ++i) {
-      const bool wide = i == L::P_READY || i == L::P_READY + 1 || i == L::Q_READY;
+      const bool wide = (i >= L::P_READY && i < L::O_DONE) || (i >= L::Q_READY && i < L::FINAL);
       ptx::mbar_init(bar(i), wide ? 128 : 1);
     }
     *s_abort = 0;
     ptx::fence_mbar_init();
   }
-  if (warp == 5) {
-    ptx::tmem_alloc(sbase + L::TMEM_SLOT, kTmemCols);
+  if (warp == kMma) {
+    ptx::tmem_alloc(sbase + L::TMEM_SLOT, L::kTmemCols);
     ptx::tmem_relinquish();
   }
   if (warp == 0) {
@@ -286,11 +297,8 @@ __global__ void __launch_bounds__(kThreads, 2)
   const bool busy = (int)blockIdx.x < line.n;
   const int w0 = busy ? line.begin(blockIdx.x) : 0, w1 = busy ? line.begin(blockIdx.x + 1) : 0;
   if (blockIdx.x == 0 && p.tile.per_seq)
-    for (int b = tid; b <= a.batch; b += kThreads) p.scan[b] = scan[b];
-  // KV head and rows of a segment.
+    for (int b = tid; b <= a.batch; b += tile_threads(NT)) p.scan[b] = scan[b];
   auto head = [&](const Seg& s) { return s.b < 0 ? s.sub / p.rt : s.sub % a.num_kv_heads; };
-  auto first_row = [&](const Seg& s) { return (s.b < 0 ? s.sub % p.rt : s.sub / a.num_kv_heads) * BM; };
-  auto rows = [&](const Seg& s, int row0) { return min(BM, (s.b < 0 ? p.rows_all : p.rows_seq) - row0); };
 
   // Bounded wait of a whole warp: true in every lane or false in every lane
   // (a warp leaves its loops together).
@@ -305,10 +313,12 @@ __global__ void __launch_bounds__(kThreads, 2)
     return __all_sync(0xffffffffu, ok);
   };
 
-  if (warp < 4) {
+  if (warp < kTma) {
     // ------------------------------------------------------------ softmax
-    const int r = tid;
-    const uint32_t lane_base = (uint32_t)(warp * 32) << 16;
+    const int wg = warp / 4, r = tid % 128;  // row tile, row of it
+    const uint32_t lane_base = (uint32_t)((warp % 4) * 32) << 16;
+    const uint32_t c_o = tmem + lane_base + C_O + (uint32_t)(wg * D);
+    const int S_FULL = L::S_FULL + 2 * wg, P_READY = L::P_READY + 2 * wg, O_DONE = L::O_DONE + 2 * wg;
     const float sl2 = a.scale * kLog2e;
     // The rows of a segment: the thread's visible keys of its list, and Q into
     // shared memory (once no MMA reads the Q before it).  A row of Q is
@@ -317,42 +327,41 @@ __global__ void __launch_bounds__(kThreads, 2)
     // loaded, masked nor stored: their TMEM lanes reach no other row.
     int limit = 0, least = 0;
     bool valid = false, active = false;
+    int in_unit = 0;  // the thread's row of the unit
     auto load_rows = [&](const Seg& s) {
       constexpr int kPer = 128 / (D / 8), kFly = 8;  // rows a step, steps in flight
-      const int c = tid % (D / 8), hk = head(s), row0 = first_row(s), n_rows = rows(s, row0);
-      for (int r0 = tid / (D / 8); r0 - tid / (D / 8) < n_rows; r0 += kPer * kFly) {
+      const bool pre = s.b < 0;
+      const int per = pre ? p.tile.rows_prefix : p.tile.rows_own, half = (per + NT - 1) / NT, hk = head(s);
+      const int row0 = (pre ? s.sub % p.rt : s.sub / a.num_kv_heads) * per + wg * half;
+      const int n_rows = min(min(half, per - wg * half), (pre ? p.rows_all : p.rows_seq) - row0);
+      const int c = r % (D / 8);
+      uint8_t* q_sm = sm + L::Q + wg * L::kQ;
+      for (int r0 = r / (D / 8); r0 - r / (D / 8) < n_rows; r0 += kPer * kFly) {
         uint4 v[kFly];
 #pragma unroll
         for (int i = 0; i < kFly; ++i) {
           const int row = r0 + i * kPer;
           if (row >= n_rows) continue;
           const Row x = row_of(p, s.b, row0 + row);
-          const T* q = static_cast<const T*>(a.q.ptr) + x.b * a.q.stride_b + (hk * p.group + x.g) * a.q.stride_h +
-                       x.t * a.q.stride_t + 8 * c;
-          if (q_vec) {
-            v[i] = __ldg(reinterpret_cast<const uint4*>(q));
-          } else {
-            T e[8];
-#pragma unroll
-            for (int k = 0; k < 8; ++k) e[k] = q[k];
-            memcpy(&v[i], e, 16);
-          }
+          v[i] = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(a.q.ptr) + x.b * a.q.stride_b +
+                                                      (hk * p.group + x.g) * a.q.stride_h + x.t * a.q.stride_t + 8 * c));
         }
 #pragma unroll
         for (int i = 0; i < kFly; ++i) {
           const int row = r0 + i * kPer;
-          if (row < n_rows) *reinterpret_cast<uint4*>(sm + L::Q + tile::chunk_off<BM>(row, c)) = v[i];
+          if (row < n_rows) *reinterpret_cast<uint4*>(q_sm + tile::chunk_off<BM>(row, c)) = v[i];
         }
       }
       ptx::fence_proxy_async_smem();
-      ptx::mbar_arrive(bar(L::Q_READY));
-      const int seen = r < n_rows ? visible(a, row_of(p, s.b, row0 + r), s.b < 0, s.keys) : -1;
+      ptx::mbar_arrive(bar(L::Q_READY + wg));
+      const int seen = r < n_rows ? visible(a, row_of(p, s.b, row0 + r), pre, s.keys) : -1;
       valid = seen >= 0;
       limit = valid ? seen : 0x7fffffff;
       active = __any_sync(0xffffffffu, valid);
       least = limit;
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) least = min(least, __shfl_xor_sync(0xffffffffu, least, o));
+      in_unit = wg * half + r;
     };
     int g = 0;
     bool ok = true;
@@ -363,8 +372,8 @@ __global__ void __launch_bounds__(kThreads, 2)
       float m = -CUDART_INF_F, l = 0.f;
       for (int j = 0; j < s.n; ++j, ++g) {
         const int k0 = (s.j0 + j) * BN, x = g & 1;
-        const uint32_t c_s = tmem + lane_base + C_S + 64u * (uint32_t)x;
-        if (!(ok = wait(L::S_FULL + x, (g >> 1) & 1))) break;
+        const uint32_t c_s = tmem + lane_base + C_S + (uint32_t)(wg * 128 + x * 64);
+        if (!(ok = wait(S_FULL + x, (g >> 1) & 1))) break;
         ptx::tc_fence_after();
         if (active) {
           uint32_t s0[32], s1[32];
@@ -397,16 +406,16 @@ __global__ void __launch_bounds__(kThreads, 2)
           }
           if (__any_sync(0xffffffffu, rescale)) {
             // O holds the tiles before this one once their last P V is done.
-            if (!(ok = wait(L::O_DONE + (x ^ 1), ((g - 1) >> 1) & 1))) break;
+            if (!(ok = wait(O_DONE + (x ^ 1), ((g - 1) >> 1) & 1))) break;
             ptx::tc_fence_after();
 #pragma unroll
             for (int c = 0; c < D / 16; ++c) {
               uint32_t o[16];
-              ptx::tmem_ld16(tmem + lane_base + C_O + 16 * c, o);
+              ptx::tmem_ld16(c_o + 16 * c, o);
               ptx::tmem_wait_ld();
 #pragma unroll
               for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
-              ptx::tmem_st16(tmem + lane_base + C_O + 16 * c, o);
+              ptx::tmem_st16(c_o + 16 * c, o);
             }
             l *= alpha;
           }
@@ -434,9 +443,10 @@ __global__ void __launch_bounds__(kThreads, 2)
           ptx::tmem_wait_st();
         }
         ptx::tc_fence_before();
-        if (k0 + BN > s.keys) {
+        if (wg == 0 && k0 + BN > s.keys) {
           // Slots past the list hold anything, NaN included, and meet P = 0:
-          // clear their V rows.
+          // clear their V rows (before the first row tile's P V, which the
+          // second's follows).
           const int item = 2 * g + 1;
           if (!(ok = wait(L::FULL + item % L::kSlots, (item / L::kSlots) & 1))) break;
           uint8_t* v = sm + L::RING + (item % L::kSlots) * L::kTile;
@@ -447,27 +457,28 @@ __global__ void __launch_bounds__(kThreads, 2)
           }
           ptx::fence_proxy_async_smem();
         }
-        ptx::mbar_arrive(bar(L::P_READY + x));
+        ptx::mbar_arrive(bar(P_READY + x));
       }
       if (!ok) break;
       // The last S of this segment is done: the next segment's rows come in
       // while its last P V runs.
       const Seg cur = s;
       const bool cur_valid = valid, cur_active = active;
+      const int cur_row = in_unit;
       s = next_seg(a, p.tile, scan, w, w1);
       if (s.n > 0) load_rows(s);
       // The rows' partial results.
-      if (!(ok = wait(L::O_DONE + ((g - 1) & 1), ((g - 1) >> 1) & 1))) break;
+      if (!(ok = wait(O_DONE + ((g - 1) & 1), ((g - 1) >> 1) & 1))) break;
       ptx::tc_fence_after();
       if (cur_active) {
         const int64_t slot = cur.unit + (int)blockIdx.x;
         const int64_t row = (cur.b < 0 ? p.tile.base_prefix + slot * p.tile.rows_prefix
-                                       : p.tile.base_own + slot * p.tile.rows_own) + r;
+                                       : p.tile.base_own + slot * p.tile.rows_own) + cur_row;
         const float inv = l > 0.f ? 1.f / l : 0.f;
 #pragma unroll
         for (int c = 0; c < D / 32; ++c) {
           uint32_t o[32];
-          ptx::tmem_ld32(tmem + lane_base + C_O + 32 * c, o);
+          ptx::tmem_ld32(c_o + 32 * c, o);
           ptx::tmem_wait_ld();
           if (cur_valid) {
 #pragma unroll
@@ -483,7 +494,7 @@ __global__ void __launch_bounds__(kThreads, 2)
       }
       ptx::tc_fence_before();
     }
-  } else if (warp == 4) {
+  } else if (warp == kTma) {
     // ------------------------------------------------------------ TMA
     if (lane == 0) {
       ptx::prefetch_tmap(&tm_k);
@@ -528,39 +539,54 @@ __global__ void __launch_bounds__(kThreads, 2)
     const uint64_t d_k = ptx::sdesc_sw128(sbase + L::RING, 16, 1024);
     const uint64_t d_v = ptx::sdesc_sw128(sbase + L::RING, BN * 128, 1024);
     constexpr uint64_t kT = L::kTile >> 4;
-    auto issue_s = [&](int g) -> bool {
-      const int item = 2 * g, slot = item % L::kSlots;
-      if (!wait(L::FULL + slot, (item / L::kSlots) & 1)) return false;
+    auto wait_k = [&](int g) -> bool {
+      const int item = 2 * g;
+      if (!wait(L::FULL + item % L::kSlots, (item / L::kSlots) & 1)) return false;
       ptx::tc_fence_after();
+      return true;
+    };
+    // S of row tile t and tile g (after the last one its K slot is free).
+    auto issue_s = [&](int t, int g) {
+      const int slot = (2 * g) % L::kSlots;
 #pragma unroll
       for (int kk = 0; kk < D / 16; ++kk)
-        ptx::mma_ss_w(tmem + C_S + 64u * (uint32_t)(g & 1),
-                      d_q + (uint64_t)(((kk >> 2) * L::kQBlock + (kk & 3) * 32) >> 4),
+        ptx::mma_ss_w(tmem + C_S + (uint32_t)(t * 128 + (g & 1) * 64),
+                      d_q + (uint64_t)((t * L::kQ + (kk >> 2) * L::kQBlock + (kk & 3) * 32) >> 4),
                       d_k + kT * (uint64_t)slot + (uint64_t)(((kk >> 2) * (BN * 128) + (kk & 3) * 32) >> 4), i_qk, kk > 0);
-      ptx::mma_commit_w(bar(L::S_FULL + (g & 1)));
-      ptx::mma_commit_w(bar(L::EMPTY + slot));
-      return true;
+      ptx::mma_commit_w(bar(L::S_FULL + 2 * t + (g & 1)));
+      if (t == NT - 1) ptx::mma_commit_w(bar(L::EMPTY + slot));
     };
     int g = 0, seg = 0;
     bool ok = true;
     for (int w = w0; w < w1 && ok; ++seg) {
       const Seg s = next_seg(a, p.tile, scan, w, w1);
       if (s.n == 0) break;
-      if (!wait(L::Q_READY, seg & 1)) break;
-      ptx::tc_fence_after();
-      ok = issue_s(g) && (s.n < 2 || issue_s(g + 1));
+      for (int t = 0; t < NT && ok; ++t) ok = wait(L::Q_READY + t, seg & 1);
+      for (int j = 0; j < 2 && j < s.n && ok; ++j) {
+        if (!(ok = wait_k(g + j))) break;
+#pragma unroll
+        for (int t = 0; t < NT; ++t) issue_s(t, g + j);
+      }
       for (int j = 0; j < s.n && ok; ++j) {
         const int gj = g + j, item = 2 * gj + 1, slot = item % L::kSlots;
-        ok = wait(L::P_READY + (gj & 1), (gj >> 1) & 1) && wait(L::FULL + slot, (item / L::kSlots) & 1);
-        if (!ok) break;
-        ptx::tc_fence_after();
+        const bool more = j + 2 < s.n;
 #pragma unroll
-        for (int kk = 0; kk < BN / 16; ++kk)
-          ptx::mma_ts_w(tmem + C_O, tmem + C_S + 64u * (uint32_t)(gj & 1) + 8u * (uint32_t)kk,
-                        d_v + kT * (uint64_t)slot + (uint64_t)((kk * 2048) >> 4), i_pv, (j > 0 || kk > 0) ? 1u : 0u);
-        ptx::mma_commit_w(bar(L::O_DONE + (gj & 1)));
-        ptx::mma_commit_w(bar(L::EMPTY + slot));
-        if (j + 2 < s.n) ok = issue_s(gj + 2);
+        for (int t = 0; t < NT; ++t) {
+          ok = wait(L::P_READY + 2 * t + (gj & 1), (gj >> 1) & 1) &&
+               (t > 0 || wait(L::FULL + slot, (item / L::kSlots) & 1));
+          if (!ok) break;
+          ptx::tc_fence_after();
+#pragma unroll
+          for (int kk = 0; kk < BN / 16; ++kk)
+            ptx::mma_ts_w(tmem + C_O + (uint32_t)(t * D), tmem + C_S + (uint32_t)(t * 128 + (gj & 1) * 64 + 8 * kk),
+                          d_v + kT * (uint64_t)slot + (uint64_t)((kk * 2048) >> 4), i_pv, (j > 0 || kk > 0) ? 1u : 0u);
+          ptx::mma_commit_w(bar(L::O_DONE + 2 * t + (gj & 1)));
+          if (t == NT - 1) ptx::mma_commit_w(bar(L::EMPTY + slot));
+          if (more) {
+            if (t == 0 && !(ok = wait_k(gj + 2))) break;
+            issue_s(t, gj + 2);
+          }
+        }
       }
       g += s.n;
     }
@@ -571,9 +597,9 @@ __global__ void __launch_bounds__(kThreads, 2)
 
   ptx::tc_fence_before();
   __syncthreads();
-  if (warp == 5) {
+  if (warp == kMma) {
     ptx::tc_fence_after();
-    ptx::tmem_dealloc(tmem, kTmemCols);
+    ptx::tmem_dealloc(tmem, L::kTmemCols);
   }
 }
 
@@ -629,7 +655,7 @@ struct Ring {
 template <typename T, int D>
 __global__ void __launch_bounds__(warpk::kMaxThreads, 1)
     warp_kernel(const AiPrefixAttnArgs a, const Plan p, const int split, const __grid_constant__ CUtensorMap tm_k,
-                const __grid_constant__ CUtensorMap tm_v, const bool q_vec) {
+                const __grid_constant__ CUtensorMap tm_v) {
   using R = warpk::Ring<D>;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   constexpr int KS = D / 16, NB = D / 8;  // k steps of Q K^T, 8-dim blocks of O
@@ -759,9 +785,9 @@ __global__ void __launch_bounds__(warpk::kMaxThreads, 1)
   for (int w = w0; w < w1 && ok;) {
     const Seg s = next_seg(a, p.warp, scan, w, w1);
     if (s.n == 0) break;
-    // (units go by groups of 16 split rows, then by KV head)
+    // (units go by groups of rows, then by KV head)
     const int group = s.sub / a.num_kv_heads, hk = s.sub - group * a.num_kv_heads;
-    const int in_unit = (warp % split) * 16, row0 = group * 16 * split + in_unit;
+    const int in_unit = (warp % split) * 16, row0 = group * (s.b < 0 ? p.warp.rows_prefix : 0) + in_unit;
     const int n_rows = (s.b < 0 ? p.rows_all : p.rows_seq) - row0;  // of this warp, when positive
     const bool any = n_rows > 0;
     // Q's fragments of rows r and r + 8 (zero past the unit's rows), and the
@@ -779,13 +805,7 @@ __global__ void __launch_bounds__(warpk::kMaxThreads, 1)
       for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          uint32_t v;
-          if (q_vec) {
-            v = __ldg(reinterpret_cast<const uint32_t*>(src + 16 * ks + 8 * e));
-          } else {
-            const T pair[2] = {src[16 * ks + 8 * e], src[16 * ks + 8 * e + 1]};
-            memcpy(&v, pair, 4);
-          }
+          const uint32_t v = __ldg(reinterpret_cast<const uint32_t*>(src + 16 * ks + 8 * e));
           q[ks][h + 2 * e] = has ? v : 0u;
         }
       seen[h] = has ? visible(a, x, s.b < 0, s.keys) : -1;
@@ -946,24 +966,22 @@ __global__ void __launch_bounds__(256) combine_kernel(const AiPrefixAttnArgs a, 
     if (a.prefix_len > 0) {
       const Line& l = p.prefix_warp ? p.warp : p.tile;
       const int all = b * p.rows_seq + rem;
-      const int group_rows = p.prefix_warp ? 16 * p.split : BM;
-      const int unit = p.prefix_warp ? (all / group_rows) * a.num_kv_heads + hk : hk * p.rt + all / BM;
+      const int grp = all / l.rows_prefix, unit = p.prefix_warp ? grp * a.num_kv_heads + hk : hk * p.rt + grp;
       const Split line = split_line(l, line_total(l, own_all));
       const int x = unit * (l.start + l.tiles_prefix) + l.start, first = line.worker(x);
       n[0] = line.worker(x + l.tiles_prefix - 1) - first + 1;
       step[0] = l.rows_prefix;
-      row[0] = l.base_prefix + (unit + first) * step[0] + all % group_rows;
+      row[0] = l.base_prefix + (unit + first) * step[0] + all - grp * l.rows_prefix;
     }
     if (size > 0) {
       const Line& l = p.own_warp ? p.warp : p.tile;
-      // (a sequence is one group of the warp kernel)
-      const int sub = p.own_warp ? hk : rem / BM * a.num_kv_heads + hk, unit = b * l.per_seq + sub;
+      const int grp = rem / l.rows_own, sub = grp * a.num_kv_heads + hk, unit = b * l.per_seq + sub;
       const Split line = split_line(l, line_total(l, own_all));
       const int x = l.units_prefix * (l.start + l.tiles_prefix) + s0 * l.per_seq + sub * size + l.start;
       const int first = line.worker(x);
       n[1] = line.worker(x + size - l.start - 1) - first + 1;
       step[1] = l.rows_own;
-      row[1] = l.base_own + (unit + first) * step[1] + rem % BM;
+      row[1] = l.base_own + (unit + first) * step[1] + rem - grp * l.rows_own;
     }
     const int all_n = n[0] + n[1];
     auto row_at = [&](int i) { return i < n[0] ? row[0] + i * step[0] : row[1] + (i - n[0]) * step[1]; };
@@ -1029,12 +1047,10 @@ bool make_plan(const AiPrefixAttnArgs& a, Plan* p, size_t* bytes) {
   *p = Plan{};
   const int64_t G = a.num_q_heads / a.num_kv_heads, rows = G * a.seq_len, all = rows * a.batch, H = a.num_kv_heads;
   const int64_t capacity = (int64_t)a.max_pages * a.page_size;
-  if (all > 0x7fffffff || a.batch * ((rows + BM - 1) / BM) * H > 0x7fffffff) return false;
+  if (all > 0x7fffffff || a.batch * rows * H > 0x7fffffff) return false;
   p->group = (int)G;
   p->rows_seq = (int)rows;
   p->rows_all = (int)all;
-  p->rt = (int)((all + BM - 1) / BM);
-  p->tt = (int)((rows + BM - 1) / BM);
   p->own_warp = rows <= kWarpRows;
   p->split = warp_split(rows);
   const int sms = sm_count(), workers = sms * warpk::workers(p->split);
@@ -1071,8 +1087,12 @@ bool make_plan(const AiPrefixAttnArgs& a, Plan* p, size_t* bytes) {
     }
     return true;
   };
-  if (!line(p->tile, !p->prefix_warp, !p->own_warp, BN, p->rt * H, p->tt * H, BM, rows < BM ? rows : BM, 2 * sms,
-            kStartTile, kStartTile + 1))
+  // Rows go evenly over as few units as hold them.
+  p->nt = (a.prefix_len > 0 ? all : rows) > BM ? 2 : 1;
+  const int64_t most_unit = BM * p->nt, rt = (all + most_unit - 1) / most_unit, tt = (rows + most_unit - 1) / most_unit;
+  p->rt = (int)rt;
+  if (!line(p->tile, !p->prefix_warp, !p->own_warp, BN, rt * H, tt * H, (all + rt - 1) / rt, (rows + tt - 1) / tt,
+            p->nt == 1 ? 2 * sms : sms, kStartTile, kStartTile + 1))
     return false;
   if (!line(p->warp, p->prefix_warp, p->own_warp, kWarpKeys, groups * H, H, all < group_rows ? all : group_rows, rows,
             workers, kStartWarp, 2))
@@ -1093,8 +1113,6 @@ bool make_plan(const AiPrefixAttnArgs& a, Plan* p, size_t* bytes) {
 
 template <typename T, int D>
 int launch_t(const AiPrefixAttnArgs& a, const Plan& p, cudaStream_t st) {
-  const bool q_vec = (reinterpret_cast<uintptr_t>(a.q.ptr) & 15) == 0 &&
-                     ((a.q.stride_b | a.q.stride_h | a.q.stride_t) & 7) == 0;
   ProfScope ps(AI_PROF_PREFIX, st);
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -1115,10 +1133,13 @@ int launch_t(const AiPrefixAttnArgs& a, const Plan& p, cudaStream_t st) {
   };
   if (p.tile.workers > 0) {
     if (!maps(BN)) return AI_ERR_TMA;
-    if (!smem_of(tile_kernel<T, D>, Smem<D>::bytes(a.batch))) return AI_ERR_LAUNCH;
     cfg.gridDim = dim3(p.tile.workers);
-    cfg.blockDim = dim3(kThreads);
-    if (cudaLaunchKernelEx(&cfg, tile_kernel<T, D>, a, p, tk, tv, q_vec) != cudaSuccess) return AI_ERR_LAUNCH;
+    cfg.blockDim = dim3(tile_threads(p.nt));
+    const bool ok = p.nt == 1 ? smem_of(tile_kernel<T, D, 1>, Smem<D, 1>::bytes(a.batch)) &&
+                                    cudaLaunchKernelEx(&cfg, tile_kernel<T, D, 1>, a, p, tk, tv) == cudaSuccess
+                              : smem_of(tile_kernel<T, D, 2>, Smem<D, 2>::bytes(a.batch)) &&
+                                    cudaLaunchKernelEx(&cfg, tile_kernel<T, D, 2>, a, p, tk, tv) == cudaSuccess;
+    if (!ok) return AI_ERR_LAUNCH;
     cfg.numAttrs = 1;
   }
   if (p.warp.workers > 0) {
@@ -1127,7 +1148,7 @@ int launch_t(const AiPrefixAttnArgs& a, const Plan& p, cudaStream_t st) {
     if (!smem_of(warp_kernel<T, D>, warpk::Ring<D>::bytes(split, a.batch))) return AI_ERR_LAUNCH;
     cfg.gridDim = dim3((p.warp.workers + per - 1) / per);
     cfg.blockDim = dim3(32 * (split * per + 1));
-    if (cudaLaunchKernelEx(&cfg, warp_kernel<T, D>, a, p, split, tk, tv, q_vec) != cudaSuccess) return AI_ERR_LAUNCH;
+    if (cudaLaunchKernelEx(&cfg, warp_kernel<T, D>, a, p, split, tk, tv) != cudaSuccess) return AI_ERR_LAUNCH;
     cfg.numAttrs = 1;
   }
   // Warps per row: one for every four partial results, while the rows leave
@@ -1152,9 +1173,10 @@ bool sm100_fits(const AiPrefixAttnArgs& a) {
   if (a.head_dim != 64 && a.head_dim != 128) return false;
   if (a.page_size < 16 || (a.page_size & (a.page_size - 1)) || a.batch > tc::kMaxBatch) return false;
   if (!(a.scale > 0.f)) return false;  // the row maximum is taken before the scale
-  for (const AiTensor4* t : {&a.k_pages, &a.v_pages}) {
-    // what a tensor map asks for
+  for (const AiTensor4* t : {&a.q, &a.k_pages, &a.v_pages}) {
+    // 16-byte rows: what a tensor map and the loads of Q ask for
     if ((reinterpret_cast<uintptr_t>(t->ptr) & 15) || ((t->stride_b | t->stride_h | t->stride_t) & 7)) return false;
+    if (t == &a.q) continue;
     if (t->stride_b <= 0 || t->stride_h <= 0 || t->stride_t <= 0) return false;
   }
   tc::Plan p;
