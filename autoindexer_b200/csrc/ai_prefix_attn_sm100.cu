@@ -40,8 +40,25 @@ namespace prefix {
 namespace tc {
 
 constexpr int BM = 128, BN = 64;
-constexpr int kMaxBatch = 2048;  // the scan of the sequences sits in shared memory
+constexpr int kMaxBatch = 1024;  // two scans of the sequences sit in shared memory
 constexpr long long kWait = 1000000000LL;
+
+// One kernel's line of tiles.  Starting a unit costs about as much as `start`
+// tiles (its rows in, its partial results out), so `start` idle positions
+// stand before its tiles.
+struct Line {
+  int workers;
+  int least;          // positions a worker takes at least
+  int start;
+  int units_prefix;   // prefix units on this line, each of tiles_prefix tiles: (KV head, group of rows)
+  int groups;         // groups of rows a KV head has
+  int rows_prefix;    // rows of a prefix unit
+  int slot_prefix;    // rows of its slots (the most a unit can have)
+  int tiles_prefix;
+  int per_seq;        // units per sequence on this line (0: own keys are not on it)
+  int rows_own;       // rows of a sequence's unit
+  int64_t base_prefix, base_own;  // first row of each region; slot (unit + worker) follows
+};
 
 // Threads of a tile-kernel CTA with NT row tiles: a softmax warpgroup each, a
 // TMA and an MMA warp.
@@ -59,53 +76,52 @@ struct Smem {
   // (two of each per row tile, for the two S buffers)
   static constexpr int FULL = 0, EMPTY = kSlots, S_FULL = 2 * kSlots, P_READY = S_FULL + 2 * NT,
                        O_DONE = P_READY + 2 * NT, Q_READY = O_DONE + 2 * NT, FINAL = Q_READY + NT, N_BARS = FINAL + 1;
-  static constexpr uint32_t TMEM_SLOT = BARS + 8 * N_BARS;
+  static constexpr uint32_t LINE = BARS + 8 * N_BARS;  // the line with the rows that there are
+  static constexpr uint32_t TMEM_SLOT = LINE + sizeof(Line);
   static constexpr uint32_t ABORT = TMEM_SLOT + 4;
-  static constexpr uint32_t SCAN = ABORT + 4;  // int [B + 1]
-  static size_t bytes(int batch) { return SCAN + 4 * ((size_t)batch + 1) + 1024; }
+  static constexpr uint32_t SCAN = ABORT + 4;  // int [2][B + 1]
+  static size_t bytes(int batch) { return SCAN + 8 * ((size_t)batch + 1) + 1024; }
   // TMEM: two S buffers of 64 columns per row tile (P over their first 32), then O of D columns each.
   static constexpr uint32_t kTmemCols = 256 * NT;
   static constexpr uint32_t C_S = 0, C_O = 128 * NT;
 };
-static_assert(2 * (Smem<128, 1>::SCAN + 4 * (kMaxBatch + 1) + 1024 + 1024) <= 228 * 1024, "two CTAs per SM");
-static_assert(Smem<128, 2>::SCAN + 4 * (kMaxBatch + 1) + 1024 <= 227 * 1024, "one CTA per SM");
+static_assert(2 * (Smem<128, 1>::SCAN + 8 * (kMaxBatch + 1) + 1024 + 1024) <= 228 * 1024, "two CTAs per SM");
+static_assert(Smem<128, 2>::SCAN + 8 * (kMaxBatch + 1) + 1024 <= 227 * 1024, "one CTA per SM");
 
 constexpr int kWarpRows = 64;   // most rows of a sequence on the warp kernel
 constexpr int kWarpKeys = 32;   // keys of its tile
 constexpr int kShortPrefix = 6;  // positions of a prefix per worker of the warp kernel, at most
+constexpr int kFewOwn = 6;       // positions of own keys per worker of the tile kernel, at most
 // What starting a unit costs, in tiles of its kernel (chosen by the spread of
 // the CTAs' times over prefixes and sequences of 1 to 32768 keys).
 constexpr int kStartTile = 4, kStartWarp = 2;
-
-// One kernel's line of tiles.  Starting a unit costs about as much as `start`
-// tiles (its rows in, its partial results out), so `start` idle positions
-// stand before its tiles.
-struct Line {
-  int workers;
-  int least;          // positions a worker takes at least
-  int start;
-  int units_prefix;   // prefix units on this line, each of tiles_prefix tiles
-  int tiles_prefix;
-  int per_seq;        // units per sequence on this line (0: own keys are not on it)
-  int rows_prefix;    // rows of a prefix unit (and of its slots)
-  int rows_own;       // rows of a sequence's unit
-  int64_t base_prefix, base_own;  // first row of each region; slot (unit + worker) follows
-};
 
 // What the host knows of the work.
 struct Plan {
   int group;        // G: query heads per KV head
   int rows_seq;     // T G
-  int rows_all;     // B T G
   int nt;           // row tiles of a tile-kernel CTA
-  int rt;           // units of a KV head's rows of the prefix, on the tile kernel
   int split;        // warps of a warp-kernel worker
   bool prefix_warp, own_warp;  // which kernel has the list
   Line tile, warp;
   float* part_o;    // [rows][D]
   float* part_lse;  // [rows]
   int* scan;        // [B + 1] positions before each sequence's own units, per unit
+  int* tokens;      // [B + 1] real query tokens before each sequence
 };
+
+// The line with the rows that there are: the prefix's units have the real
+// query tokens' rows, evenly over as few groups as hold them (the host knows
+// only that slot_prefix is the most a unit can have).
+__device__ __forceinline__ Line live_line(const AiPrefixAttnArgs& a, const Line& l, int rows) {
+  Line r = l;
+  if (l.units_prefix > 0) {
+    r.groups = (rows + l.slot_prefix - 1) / l.slot_prefix;
+    r.units_prefix = r.groups * a.num_kv_heads;
+    r.rows_prefix = r.groups > 0 ? (rows + r.groups - 1) / r.groups : 0;
+  }
+  return r;
+}
 
 // Positions of a line whose sequences have `own` positions per unit (the host
 // has checked that they fit in an int).
@@ -135,23 +151,42 @@ __device__ __forceinline__ Split split_line(const Line& l, int total) {
 }
 
 // scan[b] = positions before sequence b on the line of its own keys, for one
-// unit per sequence (one warp; tiles of `keys` keys).
-__device__ __forceinline__ void scan_own(const AiPrefixAttnArgs& a, int keys, int start, int* scan) {
+// unit per sequence (zeros if the line has none); tokens[b] = real query
+// tokens before it.  One warp; tiles of `keys` keys.
+__device__ __forceinline__ void scan_seqs(const AiPrefixAttnArgs& a, const Line& l, int keys, int* scan, int* tokens) {
   const int lane = threadIdx.x % 32;
-  int base = 0;
+  int base = 0, base_t = 0;
   for (int b0 = 0; b0 < a.batch; b0 += 32) {
     const int b = b0 + lane;
-    int v = b < a.batch ? (seq_lens(a, b).keys + keys - 1) / keys : 0;
-    if (v > 0) v += start;
+    int v = 0, n = 0;
+    if (b < a.batch) {
+      const Lens len = seq_lens(a, b);
+      n = len.n;
+      if (l.per_seq > 0 && len.keys > 0) v = l.start + (len.keys + keys - 1) / keys;
+    }
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const int u = __shfl_up_sync(0xffffffffu, v, o);
-      if (lane >= o) v += u;
+      const int u = __shfl_up_sync(0xffffffffu, v, o), x = __shfl_up_sync(0xffffffffu, n, o);
+      if (lane >= o) v += u, n += x;
     }
-    if (b < a.batch) scan[b + 1] = base + v;
+    if (b < a.batch) scan[b + 1] = base + v, tokens[b + 1] = base_t + n;
     base += __shfl_sync(0xffffffffu, v, 31);
+    base_t += __shfl_sync(0xffffffffu, n, 31);
   }
-  if (lane == 0) scan[0] = 0;
+  if (lane == 0) scan[0] = tokens[0] = 0;
+}
+
+// The last sequence b with scan[b] * per <= x.
+__device__ __forceinline__ int find_seq(const int* scan, int batch, int per, int x) {
+  int lo = 0, hi = batch - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) / 2;
+    if (scan[mid] * per <= x)
+      lo = mid;
+    else
+      hi = mid - 1;
+  }
+  return lo;
 }
 
 // A worker's stretch within one unit.
@@ -177,14 +212,7 @@ __device__ __forceinline__ Seg locate(const AiPrefixAttnArgs& a, const Line& l, 
     s.keys = a.prefix_len;
   } else {
     const int x = w - before;
-    int lo = 0, hi = a.batch - 1;  // the last sequence that begins at or before x (it has tiles)
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) / 2;
-      if (scan[mid] * l.per_seq <= x)
-        lo = mid;
-      else
-        hi = mid - 1;
-    }
+    const int lo = find_seq(scan, a.batch, l.per_seq, x);  // (it has tiles)
     size = scan[lo + 1] - scan[lo];
     const int rem = x - scan[lo] * l.per_seq;
     s.b = lo;
@@ -207,18 +235,22 @@ __device__ __forceinline__ Seg next_seg(const AiPrefixAttnArgs& a, const Line& l
   return s;
 }
 
-// Query row `i` of a unit's rows: i counts (t, query head of the group) in a
-// sequence, and the sequences before it for the prefix.
+// Query row `i` of a list's rows: i counts (t, query head of the group) of a
+// sequence, and the real tokens of the sequences before it for the prefix.
 struct Row {
   int b, t, g;
 };
 
-__device__ __forceinline__ Row row_of(const Plan& p, int b, int i) {
+__device__ __forceinline__ Row row_of(const AiPrefixAttnArgs& a, const Plan& p, const int* tokens, int b, int i) {
   Row r;
-  r.b = b < 0 ? i / p.rows_seq : b;
-  const int rem = b < 0 ? i - r.b * p.rows_seq : i;
-  r.t = rem / p.group;
-  r.g = rem - r.t * p.group;
+  r.t = i / p.group;
+  r.g = i - r.t * p.group;
+  r.b = b;
+  if (b < 0) {
+    r.b = r.t / a.seq_len;  // right where every sequence has all its tokens
+    if (tokens[r.b] > r.t || tokens[r.b + 1] <= r.t) r.b = find_seq(tokens, a.batch, 1, r.t);
+    r.t -= tokens[r.b];
+  }
   return r;
 }
 
@@ -269,6 +301,7 @@ __global__ void __launch_bounds__(tile_threads(NT), NT == 1 ? 2 : 1)
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
   volatile int* s_abort = reinterpret_cast<volatile int*>(sm + L::ABORT);
   int* scan = reinterpret_cast<int*>(sm + L::SCAN);
+  int* tokens = scan + a.batch + 1;
   auto bar = [&](int i) { return sbase + L::BARS + 8u * (uint32_t)i; };
 
   if (tid == 0) {
@@ -284,21 +317,25 @@ __global__ void __launch_bounds__(tile_threads(NT), NT == 1 ? 2 : 1)
     ptx::tmem_relinquish();
   }
   if (warp == 0) {
-    if (p.tile.per_seq)
-      scan_own(a, BN, p.tile.start, scan);
-    else if (lane == 0)
-      scan[0] = scan[a.batch] = 0;
+    scan_seqs(a, p.tile, BN, scan, tokens);
+    __syncwarp();
+    if (lane == 0) *reinterpret_cast<Line*>(sm + L::LINE) = live_line(a, p.tile, tokens[a.batch] * p.group);
   }
   ptx::tc_fence_before();
   __syncthreads();
   ptx::tc_fence_after();
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(sm + L::TMEM_SLOT);
-  const Split line = split_line(p.tile, line_total(p.tile, scan[a.batch]));
+  const int all_rows = tokens[a.batch] * p.group;
+  const Line& ln = *reinterpret_cast<const Line*>(sm + L::LINE);
+  const Split line = split_line(ln, line_total(ln, scan[a.batch]));
   const bool busy = (int)blockIdx.x < line.n;
   const int w0 = busy ? line.begin(blockIdx.x) : 0, w1 = busy ? line.begin(blockIdx.x + 1) : 0;
-  if (blockIdx.x == 0 && p.tile.per_seq)
-    for (int b = tid; b <= a.batch; b += tile_threads(NT)) p.scan[b] = scan[b];
-  auto head = [&](const Seg& s) { return s.b < 0 ? s.sub / p.rt : s.sub % a.num_kv_heads; };
+  if (blockIdx.x == 0)
+    for (int b = tid; b <= a.batch; b += tile_threads(NT)) {
+      if (ln.per_seq > 0) p.scan[b] = scan[b];
+      p.tokens[b] = tokens[b];
+    }
+  auto head = [&](const Seg& s) { return s.b < 0 ? s.sub / ln.groups : s.sub % a.num_kv_heads; };
 
   // Bounded wait of a whole warp: true in every lane or false in every lane
   // (a warp leaves its loops together).
@@ -321,40 +358,46 @@ __global__ void __launch_bounds__(tile_threads(NT), NT == 1 ? 2 : 1)
     const int S_FULL = L::S_FULL + 2 * wg, P_READY = L::P_READY + 2 * wg, O_DONE = L::O_DONE + 2 * wg;
     const float sl2 = a.scale * kLog2e;
     // The rows of a segment: the thread's visible keys of its list, and Q into
-    // shared memory (once no MMA reads the Q before it).  A row of Q is
-    // D / 8 16-byte chunks; neighbouring threads take a row's chunks and keep
-    // up to eight rows' loads in flight.  Rows without a query are neither
-    // loaded, masked nor stored: their TMEM lanes reach no other row.
+    // shared memory (once no MMA reads the Q before it).  A thread finds its
+    // row; a warp then loads its 32 rows, D / 8 lanes a row, eight loads in
+    // flight.  Rows without a query are neither loaded, masked nor stored:
+    // their TMEM lanes reach no other row.
     int limit = 0, least = 0;
     bool valid = false, active = false;
     int in_unit = 0;  // the thread's row of the unit
     auto load_rows = [&](const Seg& s) {
-      constexpr int kPer = 128 / (D / 8), kFly = 8;  // rows a step, steps in flight
+      constexpr int kLanes = D / 8, kPer = 32 / kLanes, kFly = 8;  // lanes a row, rows a load, loads in flight
       const bool pre = s.b < 0;
-      const int per = pre ? p.tile.rows_prefix : p.tile.rows_own, half = (per + NT - 1) / NT, hk = head(s);
-      const int row0 = (pre ? s.sub % p.rt : s.sub / a.num_kv_heads) * per + wg * half;
-      const int n_rows = min(min(half, per - wg * half), (pre ? p.rows_all : p.rows_seq) - row0);
-      const int c = r % (D / 8);
+      const int per = pre ? ln.rows_prefix : ln.rows_own, half = (per + NT - 1) / NT, hk = head(s);
+      const int row0 = (pre ? s.sub % ln.groups : s.sub / a.num_kv_heads) * per + wg * half;
+      const int n_rows = min(min(half, per - wg * half), (pre ? all_rows : p.rows_seq) - row0);
+      int seen = -1;
+      unsigned long long src = 0;
+      if (r < n_rows) {
+        const Row x = row_of(a, p, tokens, s.b, row0 + r);
+        src = reinterpret_cast<unsigned long long>(static_cast<const T*>(a.q.ptr) + x.b * a.q.stride_b +
+                                                   (hk * p.group + x.g) * a.q.stride_h + x.t * a.q.stride_t);
+        seen = visible(a, x, pre, s.keys);
+      }
       uint8_t* q_sm = sm + L::Q + wg * L::kQ;
-      for (int r0 = r / (D / 8); r0 - r / (D / 8) < n_rows; r0 += kPer * kFly) {
+      const int base = (warp % 4) * 32;
+#pragma unroll
+      for (int i0 = 0; i0 < 32; i0 += kPer * kFly) {
+        if (base + i0 >= n_rows) break;
         uint4 v[kFly];
 #pragma unroll
         for (int i = 0; i < kFly; ++i) {
-          const int row = r0 + i * kPer;
-          if (row >= n_rows) continue;
-          const Row x = row_of(p, s.b, row0 + row);
-          v[i] = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(a.q.ptr) + x.b * a.q.stride_b +
-                                                      (hk * p.group + x.g) * a.q.stride_h + x.t * a.q.stride_t + 8 * c));
+          const unsigned long long at = __shfl_sync(0xffffffffu, src, i0 + i * kPer + lane / kLanes);
+          if (at) v[i] = __ldg(reinterpret_cast<const uint4*>(at) + lane % kLanes);
         }
 #pragma unroll
         for (int i = 0; i < kFly; ++i) {
-          const int row = r0 + i * kPer;
-          if (row < n_rows) *reinterpret_cast<uint4*>(q_sm + tile::chunk_off<BM>(row, c)) = v[i];
+          const int row = base + i0 + i * kPer + lane / kLanes;
+          if (row < n_rows) *reinterpret_cast<uint4*>(q_sm + tile::chunk_off<BM>(row, lane % kLanes)) = v[i];
         }
       }
       ptx::fence_proxy_async_smem();
       ptx::mbar_arrive(bar(L::Q_READY + wg));
-      const int seen = r < n_rows ? visible(a, row_of(p, s.b, row0 + r), pre, s.keys) : -1;
       valid = seen >= 0;
       limit = valid ? seen : 0x7fffffff;
       active = __any_sync(0xffffffffu, valid);
@@ -366,7 +409,7 @@ __global__ void __launch_bounds__(tile_threads(NT), NT == 1 ? 2 : 1)
     int g = 0;
     bool ok = true;
     int w = w0;
-    Seg s = next_seg(a, p.tile, scan, w, w1);
+    Seg s = next_seg(a, ln, scan, w, w1);
     if (s.n > 0) load_rows(s);
     while (s.n > 0) {
       float m = -CUDART_INF_F, l = 0.f;
@@ -465,15 +508,15 @@ __global__ void __launch_bounds__(tile_threads(NT), NT == 1 ? 2 : 1)
       const Seg cur = s;
       const bool cur_valid = valid, cur_active = active;
       const int cur_row = in_unit;
-      s = next_seg(a, p.tile, scan, w, w1);
+      s = next_seg(a, ln, scan, w, w1);
       if (s.n > 0) load_rows(s);
       // The rows' partial results.
       if (!(ok = wait(O_DONE + ((g - 1) & 1), ((g - 1) >> 1) & 1))) break;
       ptx::tc_fence_after();
       if (cur_active) {
         const int64_t slot = cur.unit + (int)blockIdx.x;
-        const int64_t row = (cur.b < 0 ? p.tile.base_prefix + slot * p.tile.rows_prefix
-                                       : p.tile.base_own + slot * p.tile.rows_own) + cur_row;
+        const int64_t row = (cur.b < 0 ? ln.base_prefix + slot * ln.slot_prefix
+                                       : ln.base_own + slot * ln.rows_own) + cur_row;
         const float inv = l > 0.f ? 1.f / l : 0.f;
 #pragma unroll
         for (int c = 0; c < D / 32; ++c) {
@@ -505,7 +548,7 @@ __global__ void __launch_bounds__(tile_threads(NT), NT == 1 ? 2 : 1)
     int item = 0;
     bool ok = true;
     for (int w = w0; w < w1 && ok;) {
-      const Seg s = next_seg(a, p.tile, scan, w, w1);
+      const Seg s = next_seg(a, ln, scan, w, w1);
       const int32_t* table = s.b < 0 ? a.prefix_pages : a.page_table + s.b * a.page_table_stride;
       const int hk = head(s);
       for (int j = 0; j < s.n && ok; ++j) {
@@ -559,7 +602,7 @@ __global__ void __launch_bounds__(tile_threads(NT), NT == 1 ? 2 : 1)
     int g = 0, seg = 0;
     bool ok = true;
     for (int w = w0; w < w1 && ok; ++seg) {
-      const Seg s = next_seg(a, p.tile, scan, w, w1);
+      const Seg s = next_seg(a, ln, scan, w, w1);
       if (s.n == 0) break;
       for (int t = 0; t < NT && ok; ++t) ok = wait(L::Q_READY + t, seg & 1);
       for (int j = 0; j < 2 && j < s.n && ok; ++j) {
@@ -647,7 +690,7 @@ struct Ring {
   // 192 KB in flight per SM, shared by its workers.
   __host__ __device__ static constexpr int stages(int split) { return 192 * 1024 / (workers(split) * 2 * (int)kTile); }
   static size_t bytes(int split, int batch) {
-    return workers(split) * stages(split) * (2 * kTile + 16) + 8 + 4 * ((size_t)batch + 1) + 1024;
+    return workers(split) * stages(split) * (2 * kTile + 16) + sizeof(Line) + 8 + 8 * ((size_t)batch + 1) + 1024;
   }
 };
 }  // namespace warpk
@@ -668,8 +711,10 @@ __global__ void __launch_bounds__(warpk::kMaxThreads, 1)
   const int local = warp < n_warps ? warp / split : min(lane, n_local - 1);
   const int stages = R::stages(split);
   const uint32_t bars = sbase + n_local * stages * 2 * R::kTile;
-  volatile int* s_abort = reinterpret_cast<volatile int*>(sm + n_local * stages * (2 * R::kTile + 16));
+  Line* s_line = reinterpret_cast<Line*>(sm + n_local * stages * (2 * R::kTile + 16));
+  volatile int* s_abort = reinterpret_cast<volatile int*>(s_line + 1);
   int* scan = const_cast<int*>(s_abort) + 2;
+  int* tokens = scan + a.batch + 1;
   auto full = [&](int st) { return bars + 16u * (uint32_t)(local * stages + st); };
   auto empty = [&](int st) { return full(st) + 8; };
   if (tid == 0) {
@@ -683,15 +728,19 @@ __global__ void __launch_bounds__(warpk::kMaxThreads, 1)
     ptx::prefetch_tmap(&tm_v);
   }
   if (warp == 0) {
-    if (p.warp.per_seq)
-      scan_own(a, kWarpKeys, p.warp.start, scan);
-    else if (lane == 0)
-      scan[0] = scan[a.batch] = 0;
+    scan_seqs(a, p.warp, kWarpKeys, scan, tokens);
+    __syncwarp();
+    if (lane == 0) *s_line = live_line(a, p.warp, tokens[a.batch] * p.group);
   }
   __syncthreads();
-  if (blockIdx.x == 0 && p.warp.per_seq)
-    for (int b = tid; b <= a.batch; b += blockDim.x) p.scan[b] = scan[b];
-  const Split line = split_line(p.warp, line_total(p.warp, scan[a.batch]));
+  const int all_rows = tokens[a.batch] * p.group;
+  const Line& ln = *s_line;
+  if (blockIdx.x == 0)
+    for (int b = tid; b <= a.batch; b += blockDim.x) {
+      p.scan[b] = scan[b];
+      if (ln.units_prefix > 0) p.tokens[b] = tokens[b];
+    }
+  const Split line = split_line(ln, line_total(ln, scan[a.batch]));
   const int worker = blockIdx.x * n_local + local;
   const bool busy = worker < line.n;
   const int w0 = busy ? line.begin(worker) : 0, w1 = busy ? line.begin(worker + 1) : 0;
@@ -721,11 +770,11 @@ __global__ void __launch_bounds__(warpk::kMaxThreads, 1)
     int hk = 0;
     bool live = lane < n_local;
     auto advance = [&]() {
-      s = next_seg(a, p.warp, scan, w, w1);
+      s = next_seg(a, ln, scan, w, w1);
       j = 0;
       live = s.n > 0;
       table = s.b < 0 ? a.prefix_pages : a.page_table + s.b * a.page_table_stride;
-      hk = s.sub % a.num_kv_heads;
+      hk = s.b < 0 ? s.sub / ln.groups : s.sub;
     };
     if (live) advance();
     long long last = clock64();
@@ -783,12 +832,12 @@ __global__ void __launch_bounds__(warpk::kMaxThreads, 1)
   uint32_t turn = 0;  // parity of the stage's current load
   bool ok = true;
   for (int w = w0; w < w1 && ok;) {
-    const Seg s = next_seg(a, p.warp, scan, w, w1);
+    const Seg s = next_seg(a, ln, scan, w, w1);
     if (s.n == 0) break;
-    // (units go by groups of rows, then by KV head)
-    const int group = s.sub / a.num_kv_heads, hk = s.sub - group * a.num_kv_heads;
-    const int in_unit = (warp % split) * 16, row0 = group * (s.b < 0 ? p.warp.rows_prefix : 0) + in_unit;
-    const int n_rows = (s.b < 0 ? p.rows_all : p.rows_seq) - row0;  // of this warp, when positive
+    const bool pre = s.b < 0;
+    const int hk = pre ? s.sub / ln.groups : s.sub, in_unit = (warp % split) * 16;
+    const int unit0 = pre ? (s.sub - hk * ln.groups) * ln.rows_prefix : 0, row0 = unit0 + in_unit;
+    const int n_rows = min((pre ? all_rows : p.rows_seq) - unit0, pre ? ln.rows_prefix : p.rows_seq) - in_unit;  // of this warp, when positive
     const bool any = n_rows > 0;
     // Q's fragments of rows r and r + 8 (zero past the unit's rows), and the
     // keys that those rows see.
@@ -798,7 +847,7 @@ __global__ void __launch_bounds__(warpk::kMaxThreads, 1)
     for (int h = 0; h < 2; ++h) {
       const int i = r + 8 * h;
       const bool has = i < n_rows;
-      const Row x = row_of(p, s.b, has ? row0 + i : 0);
+      const Row x = row_of(a, p, tokens, s.b, has ? row0 + i : 0);
       const T* src = static_cast<const T*>(a.q.ptr) + x.b * a.q.stride_b + (hk * p.group + x.g) * a.q.stride_h +
                      x.t * a.q.stride_t + 2 * c;
 #pragma unroll
@@ -927,8 +976,8 @@ __global__ void __launch_bounds__(warpk::kMaxThreads, 1)
       sum += __shfl_xor_sync(0xffffffffu, sum, 2);
       if (seen[h] < 0) continue;
       const int64_t slot = s.unit + worker;
-      const int64_t row = (s.b < 0 ? p.warp.base_prefix + slot * p.warp.rows_prefix
-                                   : p.warp.base_own + slot * p.warp.rows_own) + in_unit + r + 8 * h;
+      const int64_t row = (s.b < 0 ? ln.base_prefix + slot * ln.slot_prefix
+                                   : ln.base_own + slot * ln.rows_own) + in_unit + r + 8 * h;
       const float inv = sum > 0.f ? 1.f / sum : 0.f;
 #pragma unroll
       for (int i = 0; i < NB; ++i)
@@ -959,22 +1008,22 @@ __global__ void __launch_bounds__(256) combine_kernel(const AiPrefixAttnArgs a, 
   for (int e = 0; e < E; ++e) acc[e] = 0.f;
   if (has && t < seq_lens(a, b).n) {
     // (without room for own keys neither kernel has written the scan)
-    const bool own = a.max_pages > 0;
+    const bool own = a.max_pages > 0, pre = a.prefix_len > 0;
     const int s0 = own ? p.scan[b] : 0, size = own ? p.scan[b + 1] - s0 : 0, own_all = own ? p.scan[a.batch] : 0;
+    const int all_rows = pre ? p.tokens[a.batch] * p.group : 0;
     int64_t row[2] = {0, 0}, step[2] = {0, 0};
     int n[2] = {0, 0};
-    if (a.prefix_len > 0) {
-      const Line& l = p.prefix_warp ? p.warp : p.tile;
-      const int all = b * p.rows_seq + rem;
-      const int grp = all / l.rows_prefix, unit = p.prefix_warp ? grp * a.num_kv_heads + hk : hk * p.rt + grp;
+    if (pre) {
+      const Line l = live_line(a, p.prefix_warp ? p.warp : p.tile, all_rows);
+      const int all = p.tokens[b] * p.group + rem, grp = all / l.rows_prefix, unit = hk * l.groups + grp;
       const Split line = split_line(l, line_total(l, own_all));
       const int x = unit * (l.start + l.tiles_prefix) + l.start, first = line.worker(x);
       n[0] = line.worker(x + l.tiles_prefix - 1) - first + 1;
-      step[0] = l.rows_prefix;
+      step[0] = l.slot_prefix;
       row[0] = l.base_prefix + (unit + first) * step[0] + all - grp * l.rows_prefix;
     }
     if (size > 0) {
-      const Line& l = p.own_warp ? p.warp : p.tile;
+      const Line l = live_line(a, p.own_warp ? p.warp : p.tile, all_rows);
       const int grp = rem / l.rows_own, sub = grp * a.num_kv_heads + hk, unit = b * l.per_seq + sub;
       const Split line = split_line(l, line_total(l, own_all));
       const int x = l.units_prefix * (l.start + l.tiles_prefix) + s0 * l.per_seq + sub * size + l.start;
@@ -1050,7 +1099,6 @@ bool make_plan(const AiPrefixAttnArgs& a, Plan* p, size_t* bytes) {
   if (all > 0x7fffffff || a.batch * rows * H > 0x7fffffff) return false;
   p->group = (int)G;
   p->rows_seq = (int)rows;
-  p->rows_all = (int)all;
   p->own_warp = rows <= kWarpRows;
   p->split = warp_split(rows);
   const int sms = sm_count(), workers = sms * warpk::workers(p->split);
@@ -1061,11 +1109,13 @@ bool make_plan(const AiPrefixAttnArgs& a, Plan* p, size_t* bytes) {
   p->prefix_warp = p->own_warp && groups * H * (kStartWarp + (a.prefix_len + kWarpKeys - 1) / kWarpKeys) <=
                                       (int64_t)kShortPrefix * workers;
   int64_t at = 0;  // rows of the partial results so far
-  auto line = [&](Line& l, bool prefix, bool own, int keys, int64_t units, int64_t per_seq, int64_t rows_prefix,
-                  int64_t rows_own, int64_t workers, int start, int least) {
+  // (most: rows of a prefix unit at most; own: rows and units of a sequence)
+  auto line = [&](Line& l, bool prefix, bool own, int keys, int64_t most_unit, int64_t per_seq, int64_t rows_own,
+                  int64_t workers, int start, int least) {
     const int64_t tiles = ((int64_t)a.prefix_len + keys - 1) / keys;
     l.tiles_prefix = (int)tiles;
-    l.units_prefix = prefix && tiles > 0 ? (int)units : 0;
+    l.slot_prefix = (int)(all < most_unit ? all : most_unit);
+    l.units_prefix = prefix && tiles > 0 ? (int)((all + most_unit - 1) / most_unit * H) : 0;
     l.per_seq = own ? (int)per_seq : 0;
     const int64_t most_own = (capacity + keys - 1) / keys;
     const int64_t most = l.units_prefix * (start + tiles) +
@@ -1075,11 +1125,10 @@ bool make_plan(const AiPrefixAttnArgs& a, Plan* p, size_t* bytes) {
     l.workers = (int)(want < workers ? want : workers);
     l.least = least;
     l.start = start;
-    l.rows_prefix = (int)rows_prefix;
     l.rows_own = (int)rows_own;
     if (l.units_prefix > 0) {
       l.base_prefix = at;
-      at += (l.units_prefix + l.workers) * rows_prefix;
+      at += (int64_t)(l.units_prefix + l.workers) * l.slot_prefix;
     }
     if (l.per_seq > 0) {
       l.base_own = at;
@@ -1087,16 +1136,17 @@ bool make_plan(const AiPrefixAttnArgs& a, Plan* p, size_t* bytes) {
     }
     return true;
   };
-  // Rows go evenly over as few units as hold them.
   p->nt = (a.prefix_len > 0 ? all : rows) > BM ? 2 : 1;
-  const int64_t most_unit = BM * p->nt, rt = (all + most_unit - 1) / most_unit, tt = (rows + most_unit - 1) / most_unit;
-  p->rt = (int)rt;
-  if (!line(p->tile, !p->prefix_warp, !p->own_warp, BN, rt * H, tt * H, (all + rt - 1) / rt, (rows + tt - 1) / tt,
+  const int64_t most_unit = BM * p->nt, tt = (rows + most_unit - 1) / most_unit;
+  // Own keys join the tile kernel's line when there is room for few of them
+  // and the kernel runs anyway: a launch less.
+  if (!p->prefix_warp && a.batch * H * tt * (kStartTile + (capacity + BN - 1) / BN) <=
+                             (int64_t)kFewOwn * (p->nt == 1 ? 2 * sms : sms))
+    p->own_warp = false;
+  if (!line(p->tile, !p->prefix_warp, !p->own_warp, BN, most_unit, tt * H, (rows + tt - 1) / tt,
             p->nt == 1 ? 2 * sms : sms, kStartTile, kStartTile + 1))
     return false;
-  if (!line(p->warp, p->prefix_warp, p->own_warp, kWarpKeys, groups * H, H, all < group_rows ? all : group_rows, rows,
-            workers, kStartWarp, 2))
-    return false;
+  if (!line(p->warp, p->prefix_warp, p->own_warp, kWarpKeys, group_rows, H, rows, workers, kStartWarp, 2)) return false;
   char* ws = static_cast<char*>(a.workspace);
   size_t off = 0;
   auto take = [&](size_t want) {
@@ -1107,6 +1157,7 @@ bool make_plan(const AiPrefixAttnArgs& a, Plan* p, size_t* bytes) {
   p->part_o = reinterpret_cast<float*>(take((size_t)at * a.head_dim * 4));
   p->part_lse = reinterpret_cast<float*>(take((size_t)at * 4));
   p->scan = reinterpret_cast<int*>(take(((size_t)a.batch + 1) * 4));
+  p->tokens = reinterpret_cast<int*>(take(((size_t)a.batch + 1) * 4));
   *bytes = off;
   return true;
 }
