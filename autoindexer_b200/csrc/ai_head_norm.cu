@@ -28,7 +28,7 @@ using namespace headrow;
 
 constexpr int kWarps = 8;
 constexpr int kThreads = 32 * kWarps;
-constexpr int kUnroll = 4;     // row groups a forward warp has in flight
+constexpr int kUnroll = 2;     // row groups a forward warp has in flight
 constexpr int kUnrollBwd = 2;  // (x and dout each)
 
 // How one tensor's rows are cut: `chunks` items per token, `per` heads each.
@@ -36,20 +36,32 @@ struct Cut {
   int heads, per, chunks;
 };
 
+struct Item {
+  uint32_t b, t, chunk;
+};
+
+// (the launch keeps the item count within 32 bits: a 64-bit division costs
+// more than a row)
+__device__ __forceinline__ Item item_of(uint32_t it, const Cut& c, int seq_len) {
+  const uint32_t tok = it / (uint32_t)c.chunks, b = tok / (uint32_t)seq_len;
+  return {b, tok - b * (uint32_t)seq_len, it - tok * (uint32_t)c.chunks};
+}
+
 template <typename T, int D, bool kVec>
-__global__ void __launch_bounds__(kThreads) fwd_kernel(const AiHeadNormArgs a, const Cut cq, const Cut ck,
-                                                       const int64_t items_q, const int64_t items) {
+__global__ void __launch_bounds__(kThreads, 3) fwd_kernel(const AiHeadNormArgs a, const Cut cq, const Cut ck,
+                                                       const uint32_t items_q, const uint32_t items) {
   constexpr int kLanes = D / 16, kRows = 32 / kLanes;
   const int lane = threadIdx.x % 32, sub = lane / kLanes, l = lane % kLanes;
-  int64_t it = (int64_t)blockIdx.x * kWarps + threadIdx.x / 32;
+  uint32_t it = blockIdx.x * kWarps + threadIdx.x / 32;
   if (it >= items) return;
   const bool is_k = it >= items_q;
   if (is_k) it -= items_q;
   const Cut c = is_k ? ck : cq;
   const AiTensor4 src = is_k ? a.k : a.q, dst = is_k ? a.k_out : a.q_out;
   const void* weight = is_k ? a.k_weight : a.q_weight;
-  const int64_t tok = it / c.chunks, b = tok / a.seq_len, t = tok % a.seq_len;
-  const int h0 = (int)(it % c.chunks) * c.per, h1 = min(c.heads, h0 + c.per);
+  const Item i0 = item_of(it, c, a.seq_len);
+  const int64_t b = i0.b, t = i0.t;
+  const int h0 = i0.chunk * c.per, h1 = min(c.heads, h0 + c.per);
   const T* x = static_cast<const T*>(src.ptr) + b * src.stride_b + t * src.stride_t + 8 * l;
   T* y = static_cast<T*>(dst.ptr) + b * dst.stride_b + t * dst.stride_t + 8 * l;
   float wlo[8], whi[8], cs[8], sn[8];
@@ -92,14 +104,14 @@ __global__ void __launch_bounds__(kThreads) fwd_kernel(const AiHeadNormArgs a, c
 // weight and one gradient of it.
 template <typename T, int D, bool kVec>
 __global__ void __launch_bounds__(kThreads) bwd_kernel(const AiHeadNormBwdArgs g, const Cut cq, const Cut ck,
-                                                       const int blocks_q, const int64_t tokens,
+                                                       const int blocks_q, const uint32_t tokens,
                                                        float* __restrict__ part) {
   constexpr int kLanes = D / 16, kRows = 32 / kLanes;
   const AiHeadNormArgs& a = g.fwd;
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, sub = lane / kLanes, l = lane % kLanes;
   const bool is_k = (int)blockIdx.x >= blocks_q;
-  const int64_t block = is_k ? blockIdx.x - blocks_q : blockIdx.x;
-  const int64_t n_warps = (int64_t)(is_k ? gridDim.x - blocks_q : blocks_q) * kWarps;
+  const uint32_t block = is_k ? blockIdx.x - blocks_q : blockIdx.x;
+  const uint32_t n_warps = (is_k ? gridDim.x - blocks_q : blocks_q) * kWarps;
   const Cut c = is_k ? ck : cq;
   const AiTensor4 xt = is_k ? a.k : a.q, gt = is_k ? g.dk_out : g.dq_out, dt = is_k ? g.dk : g.dq;
   const void* weight = is_k ? a.k_weight : a.q_weight;
@@ -108,9 +120,10 @@ __global__ void __launch_bounds__(kThreads) bwd_kernel(const AiHeadNormBwdArgs g
 #pragma unroll
   for (int i = 0; i < 8; ++i) dwlo[i] = dwhi[i] = 0.f;
 
-  for (int64_t it = block * kWarps + warp; it < tokens * c.chunks; it += n_warps) {
-    const int64_t tok = it / c.chunks, b = tok / a.seq_len, t = tok % a.seq_len;
-    const int h0 = (int)(it % c.chunks) * c.per, h1 = min(c.heads, h0 + c.per);
+  for (uint32_t it = block * kWarps + warp; it < tokens * (uint32_t)c.chunks; it += n_warps) {
+    const Item i0 = item_of(it, c, a.seq_len);
+    const int64_t b = i0.b, t = i0.t;
+    const int h0 = i0.chunk * c.per, h1 = min(c.heads, h0 + c.per);
     const T* x = static_cast<const T*>(xt.ptr) + b * xt.stride_b + t * xt.stride_t + 8 * l;
     const T* go = static_cast<const T*>(gt.ptr) + b * gt.stride_b + t * gt.stride_t + 8 * l;
     T* dx = static_cast<T*>(dt.ptr) + b * dt.stride_b + t * dt.stride_t + 8 * l;
@@ -307,14 +320,14 @@ int launch_fwd(const AiHeadNormArgs& a, cudaStream_t st) {
   const Cut ck = cut(a.num_kv_heads > 0 ? a.num_kv_heads : 1, tokens, D, kUnroll);
   const int64_t items_q = tokens * cq.chunks, items = items_q + (a.num_kv_heads > 0 ? tokens * ck.chunks : 0);
   const int64_t blocks = (items + kWarps - 1) / kWarps;
-  if (blocks > 0x7fffffff) return AI_ERR_SHAPE;
+  if (items > 0x7fffffff) return AI_ERR_SHAPE;
   bool vec = rows_aligned(a.q, a.dtype) && rows_aligned(a.q_out, a.dtype);
   if (a.num_kv_heads > 0) vec = vec && rows_aligned(a.k, a.dtype) && rows_aligned(a.k_out, a.dtype);
   ProfScope ps(AI_PROF_HEAD_NORM, st);
   if (vec)
-    fwd_kernel<T, D, true><<<(unsigned)blocks, kThreads, 0, st>>>(a, cq, ck, items_q, items);
+    fwd_kernel<T, D, true><<<(unsigned)blocks, kThreads, 0, st>>>(a, cq, ck, (uint32_t)items_q, (uint32_t)items);
   else
-    fwd_kernel<T, D, false><<<(unsigned)blocks, kThreads, 0, st>>>(a, cq, ck, items_q, items);
+    fwd_kernel<T, D, false><<<(unsigned)blocks, kThreads, 0, st>>>(a, cq, ck, (uint32_t)items_q, (uint32_t)items);
   return cudaGetLastError() == cudaSuccess ? AI_OK : AI_ERR_LAUNCH;
 }
 
@@ -323,6 +336,8 @@ int launch_bwd(const AiHeadNormBwdArgs& g, cudaStream_t st) {
   const AiHeadNormArgs& a = g.fwd;
   const BwdPlan p = plan_bwd(a);
   const int64_t tokens = (int64_t)a.batch * a.seq_len;
+  // (a warp's next item may lie one round past the last)
+  if ((tokens * p.q.chunks > tokens * p.k.chunks ? tokens * p.q.chunks : tokens * p.k.chunks) > 0x7fffffff) return AI_ERR_SHAPE;
   float* part = static_cast<float*>(g.workspace);
   bool vec = rows_aligned(a.q, a.dtype) && rows_aligned(g.dq_out, a.dtype) && rows_aligned(g.dq, a.dtype);
   if (a.num_kv_heads > 0)
@@ -330,9 +345,9 @@ int launch_bwd(const AiHeadNormBwdArgs& g, cudaStream_t st) {
   {
     ProfScope ps(AI_PROF_HEAD_NORM, st);
     if (vec)
-      bwd_kernel<T, D, true><<<p.blocks, kThreads, 0, st>>>(g, p.q, p.k, p.blocks_q, tokens, part);
+      bwd_kernel<T, D, true><<<p.blocks, kThreads, 0, st>>>(g, p.q, p.k, p.blocks_q, (uint32_t)tokens, part);
     else
-      bwd_kernel<T, D, false><<<p.blocks, kThreads, 0, st>>>(g, p.q, p.k, p.blocks_q, tokens, part);
+      bwd_kernel<T, D, false><<<p.blocks, kThreads, 0, st>>>(g, p.q, p.k, p.blocks_q, (uint32_t)tokens, part);
     if (cudaGetLastError() != cudaSuccess) return AI_ERR_LAUNCH;
   }
   if (a.q_weight || (a.num_kv_heads > 0 && a.k_weight)) {

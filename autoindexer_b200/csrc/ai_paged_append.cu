@@ -24,23 +24,26 @@ constexpr int kThreads = 32 * kWarps;
 
 template <typename T, int D, bool kVec>
 __global__ void __launch_bounds__(kThreads) append_kernel(const AiPagedAppendArgs a, const int per, const int chunks,
-                                                          const int64_t items) {
+                                                          const uint32_t items) {
   constexpr int kLanes = D / 16, kRows = 32 / kLanes;
   const int lane = threadIdx.x % 32, sub = lane / kLanes, l = lane % kLanes;
-  const int64_t it = (int64_t)blockIdx.x * kWarps + threadIdx.x / 32;
+  const uint32_t it = blockIdx.x * kWarps + threadIdx.x / 32;
   if (it >= items) return;
-  const int64_t tok = it / chunks, b = tok / a.seq_len;
-  const int t = (int)(tok % a.seq_len);
+  // (32-bit divisions: the launch keeps the item count within them)
+  const uint32_t tok = it / (uint32_t)chunks, seq = tok / (uint32_t)a.seq_len;
+  const int64_t b = seq;
+  const int t = (int)(tok - seq * (uint32_t)a.seq_len);
   if (t >= (a.new_lens ? min(__ldg(a.new_lens + b), a.seq_len) : a.seq_len)) return;
   const int64_t n = (int64_t)__ldg(a.lens + b) + t;
   int page = -1;
-  if (n >= 0 && n / a.page_size < a.max_pages) page = __ldg(a.page_table + b * a.page_table_stride + n / a.page_size);
+  const int col = n >= 0 && n <= 0x7fffffff ? (int)n / a.page_size : -1;
+  if (col >= 0 && col < a.max_pages) page = __ldg(a.page_table + b * a.page_table_stride + col);
   if (page < 0 || page >= a.n_pages) {
     report(a.status, AI_ERR_DEV_BOUNDS);
     return;
   }
-  const int64_t slot = n % a.page_size;
-  const int h0 = (int)(it % chunks) * per, h1 = min(a.num_kv_heads, h0 + per);
+  const int64_t slot = (int)n - col * a.page_size;
+  const int h0 = (int)(it - tok * (uint32_t)chunks) * per, h1 = min(a.num_kv_heads, h0 + per);
   const T* k = static_cast<const T*>(a.k.ptr) + b * a.k.stride_b + t * a.k.stride_t + 8 * l;
   const T* v = static_cast<const T*>(a.v.ptr) + b * a.v.stride_b + t * a.v.stride_t + 8 * l;
   T* ko = static_cast<T*>(a.k_pages.ptr) + page * a.k_pages.stride_b + slot * a.k_pages.stride_t + 8 * l;
@@ -106,14 +109,14 @@ int launch(const AiPagedAppendArgs& a, cudaStream_t st) {
   const int per = tokens <= 4096 ? (kRows < a.num_kv_heads ? kRows : a.num_kv_heads) : a.num_kv_heads;
   const int chunks = (a.num_kv_heads + per - 1) / per;
   const int64_t items = tokens * chunks, blocks = (items + kWarps - 1) / kWarps;
-  if (blocks > 0x7fffffff) return AI_ERR_SHAPE;
+  if (items > 0x7fffffff) return AI_ERR_SHAPE;
   const bool vec = rows_aligned(a.k, a.dtype) && rows_aligned(a.v, a.dtype) && rows_aligned(a.k_pages, a.dtype) &&
                    rows_aligned(a.v_pages, a.dtype);
   ProfScope ps(AI_PROF_APPEND, st);
   if (vec)
-    append_kernel<T, D, true><<<(unsigned)blocks, kThreads, 0, st>>>(a, per, chunks, items);
+    append_kernel<T, D, true><<<(unsigned)blocks, kThreads, 0, st>>>(a, per, chunks, (uint32_t)items);
   else
-    append_kernel<T, D, false><<<(unsigned)blocks, kThreads, 0, st>>>(a, per, chunks, items);
+    append_kernel<T, D, false><<<(unsigned)blocks, kThreads, 0, st>>>(a, per, chunks, (uint32_t)items);
   return cudaGetLastError() == cudaSuccess ? AI_OK : AI_ERR_LAUNCH;
 }
 
