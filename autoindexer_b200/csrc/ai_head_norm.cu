@@ -30,6 +30,8 @@ constexpr int kWarps = 8;
 constexpr int kThreads = 32 * kWarps;
 constexpr int kUnroll = 2;     // row groups a forward warp has in flight
 constexpr int kUnrollBwd = 2;  // (x and dout each)
+constexpr int kCtasPerSm = 2;  // of the backward
+constexpr int kStart = 1;      // what a token costs beside its row groups, in row groups
 
 // How one tensor's rows are cut: `chunks` items per token, `per` heads each.
 struct Cut {
@@ -64,7 +66,7 @@ __global__ void __launch_bounds__(kThreads, 3) fwd_kernel(const AiHeadNormArgs a
   const int h0 = i0.chunk * c.per, h1 = min(c.heads, h0 + c.per);
   const T* x = static_cast<const T*>(src.ptr) + b * src.stride_b + t * src.stride_t + 8 * l;
   T* y = static_cast<T*>(dst.ptr) + b * dst.stride_b + t * dst.stride_t + 8 * l;
-  float wlo[8], whi[8], cs[8], sn[8];
+  F8 wlo, whi, cs, sn;
   int64_t row = 0;
   if (a.rope_cos) row = table_row(a.pos, b, t, a.n_pos, a.status);
   load_angles(a.rope_cos, a.rope_sin, row, D / 2, l, cs, sn);
@@ -81,15 +83,8 @@ __global__ void __launch_bounds__(kThreads, 3) fwd_kernel(const AiHeadNormArgs a
     }
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) {
-      float flo[8], fhi[8];
-      unpack(lo[u], flo);
-      unpack(hi[u], fhi);
-      if (weight) {
-        const float r = inv_rms<D>(flo, fhi, a.eps);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) flo[i] *= r * wlo[i], fhi[i] *= r * whi[i];
-      }
-      rotate(flo, fhi, cs, sn);
+      F8 flo = unpack(lo[u]), fhi = unpack(hi[u]);
+      norm_rotate<D>(flo, fhi, weight != nullptr, wlo, whi, cs, sn, a.eps);
       const int hh = h + u * kRows + sub;
       if (hh < h1) {
         T* p = y + (int64_t)hh * dst.stride_h;
@@ -103,7 +98,7 @@ __global__ void __launch_bounds__(kThreads, 3) fwd_kernel(const AiHeadNormArgs a
 // CTAs [0, blocks_q) walk q's items, the others k's, so that a warp has one
 // weight and one gradient of it.
 template <typename T, int D, bool kVec>
-__global__ void __launch_bounds__(kThreads) bwd_kernel(const AiHeadNormBwdArgs g, const Cut cq, const Cut ck,
+__global__ void __launch_bounds__(kThreads, kCtasPerSm) bwd_kernel(const AiHeadNormBwdArgs g, const Cut cq, const Cut ck,
                                                        const int blocks_q, const uint32_t tokens,
                                                        float* __restrict__ part) {
   constexpr int kLanes = D / 16, kRows = 32 / kLanes;
@@ -115,10 +110,8 @@ __global__ void __launch_bounds__(kThreads) bwd_kernel(const AiHeadNormBwdArgs g
   const Cut c = is_k ? ck : cq;
   const AiTensor4 xt = is_k ? a.k : a.q, gt = is_k ? g.dk_out : g.dq_out, dt = is_k ? g.dk : g.dq;
   const void* weight = is_k ? a.k_weight : a.q_weight;
-  float wlo[8], whi[8], dwlo[8], dwhi[8];
+  F8 wlo, whi, dwlo = fill8(0.f), dwhi = fill8(0.f);
   load_weight<T>(weight, a.weight_dtype == AI_DTYPE_F32, D, l, wlo, whi);
-#pragma unroll
-  for (int i = 0; i < 8; ++i) dwlo[i] = dwhi[i] = 0.f;
 
   for (uint32_t it = block * kWarps + warp; it < tokens * (uint32_t)c.chunks; it += n_warps) {
     const Item i0 = item_of(it, c, a.seq_len);
@@ -127,12 +120,10 @@ __global__ void __launch_bounds__(kThreads) bwd_kernel(const AiHeadNormBwdArgs g
     const T* x = static_cast<const T*>(xt.ptr) + b * xt.stride_b + t * xt.stride_t + 8 * l;
     const T* go = static_cast<const T*>(gt.ptr) + b * gt.stride_b + t * gt.stride_t + 8 * l;
     T* dx = static_cast<T*>(dt.ptr) + b * dt.stride_b + t * dt.stride_t + 8 * l;
-    float cs[8], sn[8];
+    F8 cs, sn;
     int64_t row = 0;
     if (a.rope_cos) row = table_row(a.pos, b, t, a.n_pos, a.status);
     load_angles(a.rope_cos, a.rope_sin, row, D / 2, l, cs, sn);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) sn[i] = -sn[i];  // the transposed rotation
     for (int h = h0; h < h1; h += kUnrollBwd * kRows) {
       Raw8<T> xlo[kUnrollBwd], xhi[kUnrollBwd], glo[kUnrollBwd], ghi[kUnrollBwd];
 #pragma unroll
@@ -148,32 +139,29 @@ __global__ void __launch_bounds__(kThreads) bwd_kernel(const AiHeadNormBwdArgs g
 #pragma unroll
       for (int u = 0; u < kUnrollBwd; ++u) {
         const int hh = h + u * kRows + sub;
-        float flo[8], fhi[8];
-        unpack(glo[u], flo);
-        unpack(ghi[u], fhi);
-        rotate(flo, fhi, cs, sn);
+        F8 flo = unpack(glo[u]), fhi = unpack(ghi[u]);
+        rotate<true>(flo, fhi, cs, sn);
         if (weight) {
-          float nlo[8], nhi[8];
-          unpack(xlo[u], nlo);
-          unpack(xhi[u], nhi);
-          const float r = inv_rms<D>(nlo, nhi, a.eps);
-          const float keep = hh < h1 ? 1.f : 0.f;  // a repeated row adds nothing to dw
-          float dot = 0.f;
+          // With F = r R^T dout and U = F w: dw += F x, mean(u n) = sum(U x) / D
+          // and dx = U - x r^2 mean(u n).
+          const F8 x0 = unpack(xlo[u]), x1 = unpack(xhi[u]);
+          const float r = inv_rms<D>(x0, x1, a.eps);
+          scale8(flo, r);
+          scale8(fhi, r);
+          if (hh < h1) {  // a repeated row adds nothing to dw
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            nlo[i] *= r, nhi[i] *= r;
-            if (keep != 0.f) {
-              dwlo[i] = fmaf(flo[i], nlo[i], dwlo[i]);
-              dwhi[i] = fmaf(fhi[i], nhi[i], dwhi[i]);
+            for (int i = 0; i < 4; ++i) {
+              dwlo.v[i] = __ffma2_rn(flo.v[i], x0.v[i], dwlo.v[i]);
+              dwhi.v[i] = __ffma2_rn(fhi.v[i], x1.v[i], dwhi.v[i]);
             }
-            flo[i] *= wlo[i], fhi[i] *= whi[i];
-            dot = fmaf(flo[i], nlo[i], fmaf(fhi[i], nhi[i], dot));
           }
-          dot = row_sum<kLanes>(dot) * (1.f / D);
+          mul8(flo, wlo);
+          mul8(fhi, whi);
+          const float m = -r * r * (row_sum<kLanes>(dot8(flo, x0, fhi, x1)) * (1.f / D));
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            flo[i] = r * (flo[i] - nlo[i] * dot);
-            fhi[i] = r * (fhi[i] - nhi[i] * dot);
+          for (int i = 0; i < 4; ++i) {
+            flo.v[i] = __ffma2_rn(x0.v[i], make_float2(m, m), flo.v[i]);
+            fhi.v[i] = __ffma2_rn(x1.v[i], make_float2(m, m), fhi.v[i]);
           }
         }
         if (hh < h1) {
@@ -186,18 +174,18 @@ __global__ void __launch_bounds__(kThreads) bwd_kernel(const AiHeadNormBwdArgs g
   }
 
   // The CTA's row of dw: lanes of equal dims, then the warps in order.
-  __shared__ float s_dw[kWarps][D];
+  __shared__ __align__(8) float s_dw[kWarps][D];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
+  for (int i = 0; i < 4; ++i) {
 #pragma unroll
     for (int o = kLanes; o < 32; o <<= 1) {
-      dwlo[i] += __shfl_xor_sync(0xffffffffu, dwlo[i], o);
-      dwhi[i] += __shfl_xor_sync(0xffffffffu, dwhi[i], o);
+      dwlo.v[i].x += __shfl_xor_sync(0xffffffffu, dwlo.v[i].x, o), dwlo.v[i].y += __shfl_xor_sync(0xffffffffu, dwlo.v[i].y, o);
+      dwhi.v[i].x += __shfl_xor_sync(0xffffffffu, dwhi.v[i].x, o), dwhi.v[i].y += __shfl_xor_sync(0xffffffffu, dwhi.v[i].y, o);
     }
-  }
-  if (sub == 0) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) s_dw[warp][8 * l + i] = dwlo[i], s_dw[warp][D / 2 + 8 * l + i] = dwhi[i];
+    if (sub == 0) {
+      *reinterpret_cast<float2*>(&s_dw[warp][8 * l + 2 * i]) = dwlo.v[i];
+      *reinterpret_cast<float2*>(&s_dw[warp][D / 2 + 8 * l + 2 * i]) = dwhi.v[i];
+    }
   }
   __syncthreads();
   if (threadIdx.x < D) {
@@ -295,21 +283,24 @@ struct BwdPlan {
   int blocks_q, blocks;
 };
 
-// CTAs in proportion to the heads, at most four per SM.
+// CTAs in proportion to what a token's heads cost, all resident at once.
 BwdPlan plan_bwd(const AiHeadNormArgs& a) {
   BwdPlan p;
   const int64_t tokens = (int64_t)a.batch * a.seq_len;
   p.q = cut(a.num_q_heads, tokens, a.head_dim, kUnrollBwd);
   p.k = cut(a.num_kv_heads > 0 ? a.num_kv_heads : 1, tokens, a.head_dim, kUnrollBwd);
-  const int64_t most = 4 * (int64_t)sm_count();
-  auto blocks = [&](const Cut& c) {
+  const int64_t most = kCtasPerSm * (int64_t)sm_count();
+  const int rows = 32 / (a.head_dim / 16);
+  auto cost = [&](const Cut& c) { return (c.heads + rows - 1) / rows + kStart * c.chunks; };  // of a token
+  const int64_t cq = cost(p.q), ck = a.num_kv_heads > 0 ? cost(p.k) : 0;
+  auto blocks = [&](const Cut& c, int64_t share) {
     const int64_t need = (tokens * c.chunks + kWarps - 1) / kWarps;
-    int64_t share = most * c.heads / (a.num_q_heads + a.num_kv_heads);
     if (share < 1) share = 1;
     return (int)(need < share ? need : share);
   };
-  p.blocks_q = blocks(p.q);
-  p.blocks = p.blocks_q + (a.num_kv_heads > 0 ? blocks(p.k) : 0);
+  int64_t share_k = (most * ck + (cq + ck) / 2) / (cq + ck);
+  p.blocks_q = blocks(p.q, most - share_k);
+  p.blocks = p.blocks_q + (ck > 0 ? blocks(p.k, share_k) : 0);
   return p;
 }
 

@@ -23,7 +23,7 @@ constexpr int kWarps = 4;
 constexpr int kThreads = 32 * kWarps;
 
 template <typename T, int D, bool kVec>
-__global__ void __launch_bounds__(kThreads) append_kernel(const AiPagedAppendArgs a, const int per, const int chunks,
+__global__ void __launch_bounds__(kThreads, 8) append_kernel(const AiPagedAppendArgs a, const int per, const int chunks,
                                                           const uint32_t items) {
   constexpr int kLanes = D / 16, kRows = 32 / kLanes;
   const int lane = threadIdx.x % 32, sub = lane / kLanes, l = lane % kLanes;
@@ -48,7 +48,7 @@ __global__ void __launch_bounds__(kThreads) append_kernel(const AiPagedAppendArg
   const T* v = static_cast<const T*>(a.v.ptr) + b * a.v.stride_b + t * a.v.stride_t + 8 * l;
   T* ko = static_cast<T*>(a.k_pages.ptr) + page * a.k_pages.stride_b + slot * a.k_pages.stride_t + 8 * l;
   T* vo = static_cast<T*>(a.v_pages.ptr) + page * a.v_pages.stride_b + slot * a.v_pages.stride_t + 8 * l;
-  float wlo[8], whi[8], cs[8], sn[8];
+  F8 wlo, whi, cs, sn;
   int64_t row = 0;
   if (a.rope_cos) row = table_row(a.pos, b, t, a.n_pos, a.status);
   load_angles(a.rope_cos, a.rope_sin, row, D / 2, l, cs, sn);
@@ -57,15 +57,8 @@ __global__ void __launch_bounds__(kThreads) append_kernel(const AiPagedAppendArg
     const int64_t h = min(hb + sub, h1 - 1);  // (rows past the last head repeat it, unstored)
     const Raw8<T> klo = load8<T, kVec>(k + h * a.k.stride_h), khi = load8<T, kVec>(k + h * a.k.stride_h + D / 2);
     const Raw8<T> vlo = load8<T, kVec>(v + h * a.v.stride_h), vhi = load8<T, kVec>(v + h * a.v.stride_h + D / 2);
-    float flo[8], fhi[8];
-    unpack(klo, flo);
-    unpack(khi, fhi);
-    if (a.k_weight) {
-      const float r = inv_rms<D>(flo, fhi, a.eps);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) flo[i] *= r * wlo[i], fhi[i] *= r * whi[i];
-    }
-    rotate(flo, fhi, cs, sn);
+    F8 flo = unpack(klo), fhi = unpack(khi);
+    norm_rotate<D>(flo, fhi, a.k_weight != nullptr, wlo, whi, cs, sn, a.eps);
     if (hb + sub < h1) {
       store8<T, kVec>(ko + h * a.k_pages.stride_h, pack<T>(flo));
       store8<T, kVec>(ko + h * a.k_pages.stride_h + D / 2, pack<T>(fhi));
