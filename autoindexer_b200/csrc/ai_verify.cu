@@ -348,13 +348,33 @@ __device__ __forceinline__ unsigned long long best_of(float best, int at_, unsig
 template <typename T>
 __global__ void __launch_bounds__(kThreads) pick_kernel(const AiVerifyArgs a, const Ws w, const int slice,
                                                         const bool vec) {
-  asm volatile("griddepcontrol.wait;" ::: "memory");
   const int b = blockIdx.y, tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
   const int n = drafted(a, b), rows = n_rows(a);
   const float tau = tau_of(a, b), c = slope(tau);
   __shared__ Stat st[2 * kMaxDraft + 1];
   __shared__ int s_refused[kMaxDraft + 1];
   __shared__ unsigned long long s_key[kWarps];
+  // What the stats pass has no part in is read while it runs: the drafted
+  // tokens with their logits and uniforms (thread i: token i), and the slice's
+  // noise on its way to L2.
+  const int v0 = blockIdx.x * slice, v1 = min(a.vocab, v0 + slice);
+  long long tok = -1;
+  float u = 0.f, x_p = 0.f, x_q = 0.f;
+  if (tid < n) {
+    tok = a.tokens[(int64_t)b * a.n_draft + tid];
+    u = __ldg(a.uniforms + (int64_t)b * a.n_draft + tid);
+    if (tok < 0 || tok >= a.vocab) {
+      report(a.status, AI_ERR_DEV_BOUNDS);
+      tok = -1;
+    } else {
+      x_p = at(row_ptr<T>(a, b, tid), tok);
+      if (a.draft) x_q = at(row_ptr<T>(a, b, a.n_draft + 1 + tid), tok);
+    }
+  }
+  if (tau > 0.f)
+    for (int v = v0 + 32 * tid; v < v1; v += 32 * kThreads)
+      asm volatile("prefetch.global.L2 [%0];" ::"l"(a.noise + (int64_t)b * a.vocab + v));
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   for (int r = warp; r < rows; r += kWarps) {
     if (!needed(a, r, n)) continue;
     const Stat* p = w.stat + ((int64_t)b * rows + r) * w.splits;
@@ -364,25 +384,21 @@ __global__ void __launch_bounds__(kThreads) pick_kernel(const AiVerifyArgs a, co
     if (lane == 0) st[r] = s;
   }
   __syncthreads();
-  for (int i = tid; i < n; i += kThreads) {
-    const long long tok = a.tokens[(int64_t)b * a.n_draft + i];
-    bool ok;
-    if (tok < 0 || tok >= a.vocab) {
-      report(a.status, AI_ERR_DEV_BOUNDS);
-      ok = false;
-    } else if (!(tau > 0.f)) {
-      ok = tok == st[i].at;
-    } else {
-      const Stat& sp = st[i];
-      const float p = sp.s > 0.f ? weight(at(row_ptr<T>(a, b, i), tok), c, sp.o) / sp.s : 0.f;
+  if (tid < n) {  // (kMaxDraft is below a CTA's threads)
+    bool ok = false;
+    if (tok >= 0 && !(tau > 0.f)) {
+      ok = tok == st[tid].at;
+    } else if (tok >= 0) {
+      const Stat& sp = st[tid];
+      const float p = sp.s > 0.f ? weight(x_p, c, sp.o) / sp.s : 0.f;
       float q = 1.f;
       if (a.draft) {
-        const Stat& sq = st[a.n_draft + 1 + i];
-        q = sq.s > 0.f ? weight(at(row_ptr<T>(a, b, a.n_draft + 1 + i), tok), c, sq.o) / sq.s : 0.f;
+        const Stat& sq = st[a.n_draft + 1 + tid];
+        q = sq.s > 0.f ? weight(x_q, c, sq.o) / sq.s : 0.f;
       }
-      ok = __ldg(a.uniforms + (int64_t)b * a.n_draft + i) * q < p;
+      ok = u * q < p;
     }
-    s_refused[i] = !ok;
+    s_refused[tid] = !ok;
   }
   __syncthreads();
   int stop = 0;
@@ -403,10 +419,9 @@ __global__ void __launch_bounds__(kThreads) pick_kernel(const AiVerifyArgs a, co
       d.oq = sq.o == -CUDART_INF_F ? 0.f : sq.o;
       d.iq = sq.s > 0.f ? 1.f / sq.s : 0.f;
     } else if (stop < n) {
-      const long long tok = a.tokens[(int64_t)b * a.n_draft + stop];
-      if (tok >= 0 && tok < a.vocab) d.drop = (int)tok;
+      const long long refused = a.tokens[(int64_t)b * a.n_draft + stop];
+      if (refused >= 0 && refused < a.vocab) d.drop = (int)refused;
     }
-    const int v0 = blockIdx.x * slice, v1 = min(a.vocab, v0 + slice);
     float best = 0.f;
     int best_at = 0;
     if (vec)
