@@ -1,8 +1,10 @@
 """Argument checks and the launch shared by the operator wrappers.
 
-A decode step calls several small operators, so these stay short: devices are
-compared as indices, and a struct is filled with one constructor call where it
-can be."""
+A decode step calls several small operators, and a model calls them with the
+same few signatures over and over.  A wrapper therefore keeps, per signature
+(shapes, strides, types, devices and options of the arguments), the checked
+argument struct without its pointers; a call with a known signature copies it
+and sets the pointers."""
 
 from __future__ import annotations
 
@@ -34,6 +36,27 @@ def status_ptr(index: int) -> int:
     return ptr
 
 
+def sig(x: Optional[Tensor]):
+    """What of a tensor the checks and the argument struct go by."""
+    return None if x is None else (x.shape, x.stride(), x.dtype, x.get_device())
+
+
+class Plans(dict):
+    """Checked argument structs by signature, at most a few hundred."""
+
+    def keep(self, key, given, used, args) -> None:
+        """Keeps ``args`` unless a tensor had to be copied for it."""
+        if all(x is y for x, y in zip(given, used)):
+            if len(self) >= 512:
+                self.clear()
+            self[key] = args
+
+
+def copy(args):
+    """A struct of one call's own."""
+    return type(args).from_buffer_copy(args)
+
+
 def dtype_code(x: Tensor, name: str) -> int:
     code = _DTYPES.get(x.dtype)
     if code is None:
@@ -47,6 +70,10 @@ def dense_d(x: Tensor) -> Tensor:
 
 def t4(x: Tensor) -> "_lib.AiTensor4":
     return _lib.AiTensor4(x.data_ptr(), *x.stride()[:3])
+
+
+def strides4(x: Tensor) -> "_lib.AiTensor4":
+    return _lib.AiTensor4(None, *x.stride()[:3])
 
 
 def on_device(name: str, x: Tensor, index: int) -> None:
@@ -81,9 +108,10 @@ def floats(name: str, x: Tensor, shape: Tuple[int, ...], index: int) -> Tensor:
     return x.contiguous()
 
 
-def fill_rope(a, rope, positions: Optional[Tensor], batch: int, seq_len: int, head_dim: int, index: int):
-    """Sets the rotary table and the position ids of ``a``; returns the
-    tensors to keep alive until the launch (cos, sin, positions)."""
+def check_rope(a, rope, positions: Optional[Tensor], batch: int, seq_len: int, head_dim: int, index: int):
+    """Sets what ``a`` says of the rotary table and the position ids; returns
+    (cos, sin, positions) as the kernels read them, whose pointers
+    ``point_rope`` sets."""
     if rope is None:
         if positions is not None:
             raise ValueError("positions without a rope table")
@@ -106,9 +134,14 @@ def fill_rope(a, rope, positions: Optional[Tensor], batch: int, seq_len: int, he
     on_device("positions", positions, index)
     if positions.stride(-1) != 1:
         positions = positions.contiguous()
-    a.rope_cos, a.rope_sin, a.n_pos = cos.data_ptr(), sin.data_ptr(), n
-    a.pos = _lib.AiPositions(positions.data_ptr(), positions.stride(0) if rows > 1 else 0, is_int64)
+    a.n_pos = n
+    a.pos = _lib.AiPositions(None, positions.stride(0) if rows > 1 else 0, is_int64)
     return cos, sin, positions
+
+
+def point_rope(a, cos: Optional[Tensor], sin: Optional[Tensor], positions: Optional[Tensor]) -> None:
+    if cos is not None:
+        a.rope_cos, a.rope_sin, a.pos.ptr = cos.data_ptr(), sin.data_ptr(), positions.data_ptr()
 
 
 def head_weight(name: str, w: Optional[Tensor], x: Tensor, index: int) -> Optional[Tensor]:

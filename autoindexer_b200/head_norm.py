@@ -21,36 +21,72 @@ from . import _call, _lib
 __all__ = ["qk_norm_rope"]
 
 
-def _args(q, k, wq, wk, rope, positions, eps, index):
-    """The call's arguments without its outputs, and the (cos, sin,
-    positions) tensors they point to."""
+_PLANS = _call.Plans()
+
+
+def _plan(query, key, q_weight, k_weight, cos, sin, positions, eps):
+    """Checks the arguments; returns the tensors the kernels read (dense
+    copies where those given are not) and the argument struct without
+    pointers."""
+    index = _call.cuda_index("query", query)
+    if query.dim() != 4:
+        raise ValueError(f"query must be (B, Hq, T, D), got {tuple(query.shape)}")
+    B, Hq, T, D = query.shape
+    if D not in (32, 64, 128):
+        raise ValueError(f"head_dim must be 32, 64 or 128, got {D}")
+    if query.numel() == 0:
+        raise ValueError("query must not be empty")
+    query = _call.dense_d(query)
     a = _lib.AiHeadNormArgs()
-    a.batch, a.num_q_heads, a.seq_len, a.head_dim = B, _, T, D = q.shape
-    a.dtype = a.weight_dtype = _call.dtype_code(q, "query")
+    a.batch, a.num_q_heads, a.seq_len, a.head_dim = B, Hq, T, D
+    a.dtype = a.weight_dtype = _call.dtype_code(query, "query")
     a.eps = eps
-    a.q = _call.t4(q)
+    a.q, a.q_out = _call.strides4(query), _call.strides4(torch.empty_like(query, device="meta"))
+    if key is not None:
+        if key.dim() != 4 or key.shape[0] != B or key.shape[2:] != query.shape[2:] or key.shape[1] == 0:
+            raise ValueError(f"key must be ({B}, Hkv, {T}, {D}) and not empty, got {tuple(key.shape)}")
+        if key.dtype is not query.dtype:
+            raise TypeError(f"key is {key.dtype}, query {query.dtype}")
+        _call.on_device("key", key, index)
+        key = _call.dense_d(key)
+        a.num_kv_heads = key.shape[1]
+        a.k, a.k_out = _call.strides4(key), _call.strides4(torch.empty_like(key, device="meta"))
+    elif k_weight is not None:
+        raise ValueError("k_weight without a key")
+    q_weight = _call.head_weight("q_weight", q_weight, query, index)
+    k_weight = _call.head_weight("k_weight", k_weight, query, index)
+    if q_weight is not None and k_weight is not None and q_weight.dtype is not k_weight.dtype:
+        raise TypeError(f"q_weight is {q_weight.dtype}, k_weight {k_weight.dtype}")
+    w = q_weight if q_weight is not None else k_weight
+    if w is not None:
+        a.weight_dtype = _call.dtype_code(w, "weight")
+    cos, sin, positions = _call.check_rope(a, None if cos is None else (cos, sin), positions, B, T, D, index)
+    a.status = _call.status_ptr(index)
+    return (query, key, q_weight, k_weight, cos, sin, positions), a
+
+
+def _point(a, q, k, wq, wk, cos, sin, positions):
+    a.q.ptr = q.data_ptr()
     if k is not None:
-        a.num_kv_heads = k.shape[1]
-        a.k = _call.t4(k)
+        a.k.ptr = k.data_ptr()
     if wq is not None:
         a.q_weight = wq.data_ptr()
-        a.weight_dtype = _call.dtype_code(wq, "q_weight")
     if wk is not None:
         a.k_weight = wk.data_ptr()
-        a.weight_dtype = _call.dtype_code(wk, "k_weight")
-    table = _call.fill_rope(a, rope, positions, B, T, D, index)
-    a.status = _call.status_ptr(index)
-    return a, table
+    _call.point_rope(a, cos, sin, positions)
 
 
-def _run(a, q, k, index):
+def _run(plan, tensors):
+    a = _call.copy(plan)
+    _point(a, *tensors)
+    q, k = tensors[0], tensors[1]
     q_out = torch.empty_like(q)
-    a.q_out = _call.t4(q_out)
+    a.q_out.ptr = q_out.data_ptr()
     k_out = None
     if k is not None:
         k_out = torch.empty_like(k)
-        a.k_out = _call.t4(k_out)
-    _call.launch(_lib.lib().ai_head_norm_fwd, a, index, "ai_head_norm_fwd")
+        a.k_out.ptr = k_out.data_ptr()
+    _call.launch(_lib.lib().ai_head_norm_fwd, a, q.get_device(), "ai_head_norm_fwd")
     return q_out, k_out
 
 
@@ -59,44 +95,41 @@ class HeadNormFn(torch.autograd.Function):
     with the forward's checked arguments."""
 
     @staticmethod
-    def forward(ctx, q, k, wq, wk, table, args, index):
-        ctx.save_for_backward(q, k, wq, wk, *table)
-        ctx.args, ctx.index = args, index
-        return _run(args, q, k, index)
+    def forward(ctx, q, k, wq, wk, cos, sin, positions, plan):
+        tensors = (q, k, wq, wk, cos, sin, positions)
+        ctx.save_for_backward(*tensors)
+        ctx.plan = plan
+        return _run(plan, tensors)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dq_out, dk_out):
-        q, k, wq, wk, cos, sin, positions = ctx.saved_tensors
+        tensors = q, k, wq, wk, _, _, _ = ctx.saved_tensors
         g = _lib.AiHeadNormBwdArgs()
-        g.fwd = ctx.args
-        f = g.fwd
+        g.fwd = ctx.plan
         # (saved tensors may have been moved and brought back)
-        f.q = _call.t4(q)
+        g.fwd.q = _call.t4(q)
         dq_out = _call.dense_d(dq_out)
         dq = torch.empty_like(q)
         g.dq_out, g.dq = _call.t4(dq_out), _call.t4(dq)
         dk = dwq = dwk = None
         if k is not None:
-            f.k = _call.t4(k)
+            g.fwd.k = _call.t4(k)
             dk_out = _call.dense_d(dk_out)
             dk = torch.empty_like(k)
             g.dk_out, g.dk = _call.t4(dk_out), _call.t4(dk)
         if wq is not None:
-            f.q_weight = wq.data_ptr()
             dwq = torch.empty_like(wq)
             g.dq_weight = dwq.data_ptr()
         if wk is not None:
-            f.k_weight = wk.data_ptr()
             dwk = torch.empty_like(wk)
             g.dk_weight = dwk.data_ptr()
-        if cos is not None:
-            f.rope_cos, f.rope_sin, f.pos.ptr = cos.data_ptr(), sin.data_ptr(), positions.data_ptr()
+        _point(g.fwd, *tensors)
         lib = _lib.lib()
         ws = _call.workspace(lib.ai_head_norm_bwd_workspace, g, q.device, "ai_head_norm_bwd_workspace")
-        _call.launch(lib.ai_head_norm_bwd, g, ctx.index, "ai_head_norm_bwd")
+        _call.launch(lib.ai_head_norm_bwd, g, q.get_device(), "ai_head_norm_bwd")
         del ws
-        return dq, dk, dwq, dwk, None, None, None
+        return dq, dk, dwq, dwk, None, None, None, None
 
 
 def qk_norm_rope(query: Tensor, key: Optional[Tensor], q_weight: Optional[Tensor] = None,
@@ -114,30 +147,17 @@ def qk_norm_rope(query: Tensor, key: Optional[Tensor], q_weight: Optional[Tensor
     rotated.  CUDA tensors, bfloat16, float16 or float32, head_dim 32, 64 or
     128, any strides with the last dimension contiguous.  Arithmetic is
     float32, rounded once.  Differentiable in query, key and the weights."""
-    index = _call.cuda_index("query", query)
-    if query.dim() != 4:
-        raise ValueError(f"query must be (B, Hq, T, D), got {tuple(query.shape)}")
-    B, _, T, D = query.shape
-    if D not in (32, 64, 128):
-        raise ValueError(f"head_dim must be 32, 64 or 128, got {D}")
-    if query.numel() == 0:
-        raise ValueError("query must not be empty")
-    if key is not None:
-        if key.dim() != 4 or key.shape[0] != B or key.shape[2:] != query.shape[2:] or key.shape[1] == 0:
-            raise ValueError(f"key must be ({B}, Hkv, {T}, {D}) and not empty, got {tuple(key.shape)}")
-        if key.dtype is not query.dtype:
-            raise TypeError(f"key is {key.dtype}, query {query.dtype}")
-        _call.on_device("key", key, index)
-        key = _call.dense_d(key)
-    elif k_weight is not None:
-        raise ValueError("k_weight without a key")
-    query = _call.dense_d(query)
-    wq = _call.head_weight("q_weight", q_weight, query, index)
-    wk = _call.head_weight("k_weight", k_weight, query, index)
-    if wq is not None and wk is not None and wq.dtype is not wk.dtype:
-        raise TypeError(f"q_weight is {wq.dtype}, k_weight {wk.dtype}")
-    args, table = _args(query, key, wq, wk, rope, positions, eps, index)
-    if torch.is_grad_enabled() and (query.requires_grad or (key is not None and key.requires_grad) or
-                                    (wq is not None and wq.requires_grad) or (wk is not None and wk.requires_grad)):
-        return HeadNormFn.apply(query, key, wq, wk, table, args, index)
-    return _run(args, query, key, index)
+    cos, sin = (None, None) if rope is None else rope
+    tensors = (query, key, q_weight, k_weight, cos, sin, positions)
+    eps = float(eps)
+    at = (*map(_call.sig, tensors), eps)
+    plan = _PLANS.get(at)
+    if plan is None:
+        given = tensors
+        tensors, plan = _plan(*given, eps)
+        _PLANS.keep(at, given, tensors, plan)
+    if torch.is_grad_enabled():
+        for x in tensors[:4]:
+            if x is not None and x.requires_grad:
+                return HeadNormFn.apply(*tensors, plan)
+    return _run(plan, tensors)

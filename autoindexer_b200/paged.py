@@ -43,6 +43,45 @@ def _table(page_table: Tensor, batch: int, index: int) -> Tensor:
     return _call.ints("page_table", page_table, (batch, page_table.shape[1]), index)
 
 
+_APPEND_PLANS, _ATTEND_PLANS = _call.Plans(), _call.Plans()
+
+
+def _append_plan(key, value, k_pages, v_pages, page_table, lens, new_lens, key_weight, cos, sin, positions, eps):
+    """Checks the arguments; returns the tensors the kernel reads and the
+    argument struct without pointers."""
+    index = _call.cuda_index("key", key)
+    if key.dim() != 4 or key.shape != value.shape:
+        raise ValueError(f"key and value must be (B, Hkv, T, D), got {tuple(key.shape)} and {tuple(value.shape)}")
+    B, H, T, D = key.shape
+    if key.numel() == 0:
+        raise ValueError("key and value must not be empty")
+    if D not in (32, 64, 128):
+        raise ValueError(f"head_dim must be 32, 64 or 128, got {D}")
+    if value.dtype is not key.dtype:
+        raise TypeError(f"value is {value.dtype}, key {key.dtype}")
+    _call.on_device("value", value, index)
+    _pools(k_pages, v_pages, H, D, key.dtype, index)
+    page_table = _table(page_table, B, index)
+    if page_table.shape[1] == 0:
+        raise ValueError("page_table has no columns")
+    lens = _call.ints("lens", lens, (B,), index)
+    if new_lens is not None:
+        new_lens = _call.ints("new_lens", new_lens, (B,), index)
+    w = _call.head_weight("key_weight", key_weight, key, index)
+    k, v = _call.dense_d(key), _call.dense_d(value)
+    a = _lib.AiPagedAppendArgs()
+    a.batch, a.num_kv_heads, a.seq_len, a.head_dim = B, H, T, D
+    a.dtype = _call.dtype_code(key, "key")
+    a.weight_dtype = a.dtype if w is None else _call.dtype_code(w, "key_weight")
+    a.eps = eps
+    a.k, a.v, a.k_pages, a.v_pages = map(_call.strides4, (k, v, k_pages, v_pages))
+    a.n_pages, a.page_size = k_pages.shape[0], k_pages.shape[2]
+    a.page_table_stride, a.max_pages = page_table.stride(0), page_table.shape[1]
+    cos, sin, positions = _call.check_rope(a, None if cos is None else (cos, sin), positions, B, T, D, index)
+    a.status = _call.status_ptr(index)
+    return (k, v, k_pages, v_pages, page_table, lens, new_lens, w, cos, sin, positions), a
+
+
 def paged_append(key: Tensor, value: Tensor, k_pages: Tensor, v_pages: Tensor, page_table: Tensor, lens: Tensor,
                  rope: Optional[Tuple[Tensor, Tensor]] = None, positions: Optional[Tensor] = None,
                  new_lens: Optional[Tensor] = None, key_weight: Optional[Tensor] = None, eps: float = 1e-6) -> None:
@@ -59,42 +98,67 @@ def paged_append(key: Tensor, value: Tensor, k_pages: Tensor, v_pages: Tensor, p
     of one dtype (bfloat16, float16, float32), head_dim 32, 64 or 128, any
     page size, any strides with the last dimension contiguous.  Two tokens
     given the same slot race; no gradient flows through the cache."""
-    index = _call.cuda_index("key", key)
-    if key.dim() != 4 or key.shape != value.shape:
-        raise ValueError(f"key and value must be (B, Hkv, T, D), got {tuple(key.shape)} and {tuple(value.shape)}")
-    B, H, T, D = key.shape
-    if key.numel() == 0:
-        raise ValueError("key and value must not be empty")
-    if D not in (32, 64, 128):
-        raise ValueError(f"head_dim must be 32, 64 or 128, got {D}")
-    if value.dtype != key.dtype:
-        raise TypeError(f"value is {value.dtype}, key {key.dtype}")
-    _call.on_device("value", value, index)
-    _pools(k_pages, v_pages, H, D, key.dtype, index)
-    page_table = _table(page_table, B, index)
-    if page_table.shape[1] == 0:
-        raise ValueError("page_table has no columns")
-    lens = _call.ints("lens", lens, (B,), index)
-    w = _call.head_weight("key_weight", key_weight, key, index)
-    k, v = _call.dense_d(key), _call.dense_d(value)
-    a = _lib.AiPagedAppendArgs()
-    a.batch, a.num_kv_heads, a.seq_len, a.head_dim = B, H, T, D
-    a.dtype = _call.dtype_code(key, "key")
-    a.weight_dtype = a.dtype if w is None else _call.dtype_code(w, "key_weight")
-    a.eps = float(eps)
-    a.k, a.v, a.k_pages, a.v_pages = _call.t4(k), _call.t4(v), _call.t4(k_pages), _call.t4(v_pages)
-    a.n_pages, a.page_size = k_pages.shape[0], k_pages.shape[2]
-    a.page_table, a.page_table_stride, a.max_pages = page_table.data_ptr(), page_table.stride(0), page_table.shape[1]
-    a.lens = lens.data_ptr()
+    cos, sin = (None, None) if rope is None else rope
+    tensors = (key, value, k_pages, v_pages, page_table, lens, new_lens, key_weight, cos, sin, positions)
+    eps = float(eps)
+    at = (*map(_call.sig, tensors), eps)
+    plan = _APPEND_PLANS.get(at)
+    if plan is None:
+        given = tensors
+        tensors, plan = _append_plan(*given, eps)
+        _APPEND_PLANS.keep(at, given, tensors, plan)
+    k, v, k_pages, v_pages, page_table, lens, new_lens, w, cos, sin, positions = tensors
+    a = _call.copy(plan)
+    a.k.ptr, a.v.ptr = k.data_ptr(), v.data_ptr()
+    a.k_pages.ptr, a.v_pages.ptr = k_pages.data_ptr(), v_pages.data_ptr()
+    a.page_table, a.lens = page_table.data_ptr(), lens.data_ptr()
     if new_lens is not None:
-        new_lens = _call.ints("new_lens", new_lens, (B,), index)
         a.new_lens = new_lens.data_ptr()
     if w is not None:
         a.k_weight = w.data_ptr()
-    keep = _call.fill_rope(a, rope, positions, B, T, D, index)
+    _call.point_rope(a, cos, sin, positions)
+    _call.launch(_lib.lib().ai_paged_append, a, k.get_device(), "ai_paged_append")
+
+
+def _attend_plan(query, k_pages, v_pages, prefix_pages, page_table, lens, query_lens, prefix_len, scaling):
+    """Checks the arguments; returns the tensors the kernels read and the
+    argument struct without pointers."""
+    index = _call.cuda_index("query", query)
+    if query.dim() != 4 or query.numel() == 0:
+        raise ValueError(f"query must be (B, Hq, T, D) and not empty, got {tuple(query.shape)}")
+    B, Hq, T, D = query.shape
+    if D not in (32, 64, 128):
+        raise ValueError(f"head_dim must be 32, 64 or 128, got {D}")
+    heads = k_pages.shape[1] if k_pages.dim() == 4 else 0
+    if heads == 0 or Hq % heads != 0:
+        raise ValueError(f"num_q_heads {Hq} is not a multiple of num_kv_heads {heads}")
+    _pools(k_pages, v_pages, heads, D, query.dtype, index)
+    S = k_pages.shape[2]
+    page_table = _table(page_table, B, index)
+    lens = _call.ints("lens", lens, (B,), index)
+    if query_lens is not None:
+        query_lens = _call.ints("query_lens", query_lens, (B,), index)
+    if prefix_len < 0:
+        raise ValueError(f"prefix_len {prefix_len} is negative")
+    if prefix_len:
+        if prefix_pages is None or prefix_pages.dim() != 1 or prefix_pages.shape[0] * S < prefix_len:
+            raise ValueError(f"prefix_pages must list the pages of {prefix_len} keys ({S} a page)")
+        prefix_pages = _call.ints("prefix_pages", prefix_pages, (prefix_pages.shape[0],), index)
+    q = _call.dense_d(query)
+    st = q.stride()
+    if q.data_ptr() % 16 or (st[0] | st[1] | st[2]) * q.element_size() % 16:
+        q = q.clone(memory_format=torch.contiguous_format)  # the kernels read 16-byte pieces of its rows
+    a = _lib.AiPrefixAttnArgs()
+    a.batch, a.num_q_heads, a.seq_len, a.head_dim = B, Hq, T, D
+    a.num_kv_heads = heads
+    a.dtype = _call.dtype_code(query, "query")
+    a.scale = scaling if scaling is not None else D ** -0.5
+    a.q, a.k_pages, a.v_pages = map(_call.strides4, (q, k_pages, v_pages))
+    a.out = _lib.AiTensor4(None, T * Hq * D, D, Hq * D)
+    a.n_pages, a.page_size, a.prefix_len = k_pages.shape[0], S, prefix_len
+    a.page_table_stride, a.max_pages = page_table.stride(0), page_table.shape[1]
     a.status = _call.status_ptr(index)
-    _call.launch(_lib.lib().ai_paged_append, a, index, "ai_paged_append")
-    del keep
+    return (q, k_pages, v_pages, prefix_pages, page_table, lens, query_lens), a
 
 
 def shared_prefix_attention(query: Tensor, k_pages: Tensor, v_pages: Tensor, prefix_pages: Optional[Tensor],
@@ -117,56 +181,35 @@ def shared_prefix_attention(query: Tensor, k_pages: Tensor, v_pages: Tensor, pre
     the sequence sees must hold finite values; the slots past them may hold
     anything.  A length or page out of range is clamped and sets the status
     word."""
-    index = _call.cuda_index("query", query)
-    if query.dim() != 4 or query.numel() == 0:
-        raise ValueError(f"query must be (B, Hq, T, D) and not empty, got {tuple(query.shape)}")
-    B, Hq, T, D = query.shape
-    if D not in (32, 64, 128):
-        raise ValueError(f"head_dim must be 32, 64 or 128, got {D}")
-    heads = k_pages.shape[1] if k_pages.dim() == 4 else 0
-    if heads == 0 or Hq % heads != 0:
-        raise ValueError(f"num_q_heads {Hq} is not a multiple of num_kv_heads {heads}")
-    _pools(k_pages, v_pages, heads, D, query.dtype, index)
-    S = k_pages.shape[2]
-    page_table = _table(page_table, B, index)
-    lens = _call.ints("lens", lens, (B,), index)
     prefix_len = int(prefix_len)
-    if prefix_len < 0:
-        raise ValueError(f"prefix_len {prefix_len} is negative")
-    device = query.device
-    q = _call.dense_d(query)
-    st = q.stride()
-    if q.data_ptr() % 16 or (st[0] | st[1] | st[2]) * q.element_size() % 16:
-        q = q.contiguous()  # the kernels read 16-byte pieces of its rows
-        if q.data_ptr() % 16:
-            q = q.clone()
-    out = torch.empty((B, T, Hq, D), dtype=query.dtype, device=device)
-    a = _lib.AiPrefixAttnArgs()
-    a.batch, a.num_q_heads, a.seq_len, a.head_dim = B, Hq, T, D
-    a.num_kv_heads = heads
-    a.dtype = _call.dtype_code(query, "query")
-    a.scale = float(scaling) if scaling is not None else D ** -0.5
-    a.q, a.k_pages, a.v_pages = _call.t4(q), _call.t4(k_pages), _call.t4(v_pages)
-    a.out = _lib.AiTensor4(out.data_ptr(), T * Hq * D, D, Hq * D)
-    a.n_pages, a.page_size = k_pages.shape[0], S
-    if prefix_len:
-        if prefix_pages is None or prefix_pages.dim() != 1 or prefix_pages.shape[0] * S < prefix_len:
-            raise ValueError(f"prefix_pages must list the pages of {prefix_len} keys ({S} a page)")
-        prefix_pages = _call.ints("prefix_pages", prefix_pages, tuple(prefix_pages.shape), index)
+    if prefix_len == 0:
+        prefix_pages = None
+    tensors = (query, k_pages, v_pages, prefix_pages, page_table, lens, query_lens)
+    scaling = None if scaling is None else float(scaling)
+    at = (*map(_call.sig, tensors), prefix_len, scaling, query.data_ptr() % 16)
+    plan = _ATTEND_PLANS.get(at)
+    if plan is None:
+        given = tensors
+        tensors, plan = _attend_plan(*given, prefix_len, scaling)
+        _ATTEND_PLANS.keep(at, given, tensors, plan)
+    q, k_pages, v_pages, prefix_pages, page_table, lens, query_lens = tensors
+    B, Hq, T, D = q.shape
+    device = q.device
+    out = torch.empty((B, T, Hq, D), dtype=q.dtype, device=device)
+    a = _call.copy(plan)
+    a.q.ptr, a.out.ptr = q.data_ptr(), out.data_ptr()
+    a.k_pages.ptr, a.v_pages.ptr = k_pages.data_ptr(), v_pages.data_ptr()
+    if prefix_pages is not None:
         a.prefix_pages = prefix_pages.data_ptr()
-    a.prefix_len = prefix_len
-    a.page_table, a.page_table_stride, a.max_pages = page_table.data_ptr(), page_table.stride(0), page_table.shape[1]
-    a.lens = lens.data_ptr()
+    a.page_table, a.lens = page_table.data_ptr(), lens.data_ptr()
     if query_lens is not None:
-        query_lens = _call.ints("query_lens", query_lens, (B,), index)
         a.query_lens = query_lens.data_ptr()
     lse = None
     if return_lse:
         lse = torch.empty((B, Hq, T), dtype=torch.float32, device=device)
         a.lse = lse.data_ptr()
-    a.status = _call.status_ptr(index)
     lib = _lib.lib()
     ws = _call.workspace(lib.ai_prefix_attn_workspace, a, device, "ai_prefix_attn_workspace")
-    _call.launch(lib.ai_prefix_attn, a, index, "ai_prefix_attn")
+    _call.launch(lib.ai_prefix_attn, a, q.get_device(), "ai_prefix_attn")
     del ws
     return (out, lse) if return_lse else out

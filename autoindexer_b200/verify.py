@@ -20,6 +20,49 @@ __all__ = ["verify_draft"]
 MAX_DRAFT = 64
 
 
+_PLANS = _call.Plans()
+
+
+def _plan(target, draft_tokens, uniforms, noise, draft_logits, draft_lens, temperature):
+    """Checks the arguments; returns the tensors the kernels read and the
+    argument struct without pointers."""
+    index = _call.cuda_index("target_logits", target)
+    if target.dim() != 3 or target.numel() == 0:
+        raise ValueError(f"target_logits must be (B, L + 1, V) and not empty, got {tuple(target.shape)}")
+    B, rows, V = target.shape
+    L = rows - 1
+    if L > MAX_DRAFT:
+        raise ValueError(f"at most {MAX_DRAFT} drafted tokens, got {L}")
+    if draft_tokens.dtype is not torch.int64:
+        raise TypeError(f"draft_tokens must be int64, got {draft_tokens.dtype}")
+    if draft_tokens.shape != (B, L):
+        raise ValueError(f"draft_tokens must have shape {(B, L)}, got {tuple(draft_tokens.shape)}")
+    _call.on_device("draft_tokens", draft_tokens, index)
+    draft_tokens = draft_tokens.contiguous()
+    uniforms = _call.floats("uniforms", uniforms, (B, L), index)
+    noise = _call.floats("noise", noise, (B, V), index)
+    a = _lib.AiVerifyArgs()
+    a.batch, a.n_draft, a.vocab = B, L, V
+    a.dtype = _call.dtype_code(target, "target_logits")
+    dtype = target.dtype
+    target = _call.dense_d(target)
+    a.target_stride_b, a.target_stride_t = target.stride(0), target.stride(1)
+    if draft_logits is not None:
+        if draft_logits.shape != (B, L, V):
+            raise ValueError(f"draft_logits must have shape {(B, L, V)}, got {tuple(draft_logits.shape)}")
+        if draft_logits.dtype is not dtype:
+            raise TypeError(f"draft_logits is {draft_logits.dtype}, target_logits {dtype}")
+        _call.on_device("draft_logits", draft_logits, index)
+        draft_logits = _call.dense_d(draft_logits)
+        a.draft_stride_b, a.draft_stride_t = draft_logits.stride(0), draft_logits.stride(1)
+    if draft_lens is not None:
+        draft_lens = _call.ints("draft_lens", draft_lens, (B,), index)
+    if temperature is not None:
+        temperature = _call.floats("temperature", temperature, (B,), index)
+    a.status = _call.status_ptr(index)
+    return (target, draft_tokens, uniforms, noise, draft_logits, draft_lens, temperature), a
+
+
 def verify_draft(target_logits: Tensor, draft_tokens: Tensor, uniforms: Tensor, noise: Tensor,
                  draft_logits: Optional[Tensor] = None, draft_lens: Optional[Tensor] = None,
                  temperature: Optional[Tensor] = None) -> Tuple[Tensor, Tensor, Tensor]:
@@ -43,51 +86,32 @@ def verify_draft(target_logits: Tensor, draft_tokens: Tensor, uniforms: Tensor, 
     Logits are CUDA bfloat16, float16 or float32, finite or ``-inf``, with a
     contiguous vocabulary; up to 64 drafted tokens.  A token outside the
     vocabulary is refused and sets the status word."""
-    index, device = _call.cuda_index("target_logits", target_logits), target_logits.device
-    if target_logits.dim() != 3 or target_logits.numel() == 0:
-        raise ValueError(f"target_logits must be (B, L + 1, V) and not empty, got {tuple(target_logits.shape)}")
-    B, rows, V = target_logits.shape
-    L = rows - 1
-    if L > MAX_DRAFT:
-        raise ValueError(f"at most {MAX_DRAFT} drafted tokens, got {L}")
-    if draft_tokens.dtype != torch.int64:
-        raise TypeError(f"draft_tokens must be int64, got {draft_tokens.dtype}")
-    if tuple(draft_tokens.shape) != (B, L):
-        raise ValueError(f"draft_tokens must have shape {(B, L)}, got {tuple(draft_tokens.shape)}")
-    _call.on_device("draft_tokens", draft_tokens, index)
-    draft_tokens = draft_tokens.contiguous()
-    uniforms = _call.floats("uniforms", uniforms, (B, L), index)
-    noise = _call.floats("noise", noise, (B, V), index)
-    target = _call.dense_d(target_logits)
-    a = _lib.AiVerifyArgs()
-    a.batch, a.n_draft, a.vocab = B, L, V
-    a.dtype = _call.dtype_code(target, "target_logits")
-    a.target = target.data_ptr()
-    a.target_stride_b, a.target_stride_t = target.stride(0), target.stride(1)
-    if draft_logits is not None:
-        if tuple(draft_logits.shape) != (B, L, V):
-            raise ValueError(f"draft_logits must have shape {(B, L, V)}, got {tuple(draft_logits.shape)}")
-        if draft_logits.dtype != target.dtype:
-            raise TypeError(f"draft_logits is {draft_logits.dtype}, target_logits {target.dtype}")
-        _call.on_device("draft_logits", draft_logits, index)
-        draft_logits = _call.dense_d(draft_logits)
-        if L:
-            a.draft = draft_logits.data_ptr()
-            a.draft_stride_b, a.draft_stride_t = draft_logits.stride(0), draft_logits.stride(1)
-    if draft_lens is not None:
-        draft_lens = _call.ints("draft_lens", draft_lens, (B,), index)
-        a.draft_lens = draft_lens.data_ptr()
-    if temperature is not None:
-        temperature = _call.floats("temperature", temperature, (B,), index)
-        a.temperature = temperature.data_ptr()
+    tensors = (target_logits, draft_tokens, uniforms, noise, draft_logits, draft_lens, temperature)
+    at = tuple(map(_call.sig, tensors))
+    plan = _PLANS.get(at)
+    if plan is None:
+        given = tensors
+        tensors, plan = _plan(*given)
+        _PLANS.keep(at, given, tensors, plan)
+    target, draft_tokens, uniforms, noise, draft_logits, draft_lens, temperature = tensors
+    B, rows, _ = target.shape
+    device = target.device
+    a = _call.copy(plan)
     accepted = torch.empty(B, dtype=torch.int32, device=device)
     tokens = torch.empty((B, rows), dtype=torch.int64, device=device)
     logprobs = torch.empty((B, rows), dtype=torch.float32, device=device)
-    a.tokens, a.uniforms, a.noise = draft_tokens.data_ptr(), uniforms.data_ptr(), noise.data_ptr()
+    a.target, a.noise = target.data_ptr(), noise.data_ptr()
+    if rows > 1:
+        a.tokens, a.uniforms = draft_tokens.data_ptr(), uniforms.data_ptr()
+        if draft_logits is not None:
+            a.draft = draft_logits.data_ptr()
+    if draft_lens is not None:
+        a.draft_lens = draft_lens.data_ptr()
+    if temperature is not None:
+        a.temperature = temperature.data_ptr()
     a.accepted, a.out_tokens, a.logprobs = accepted.data_ptr(), tokens.data_ptr(), logprobs.data_ptr()
-    a.status = _call.status_ptr(index)
     lib = _lib.lib()
     ws = _call.workspace(lib.ai_verify_draft_workspace, a, device, "ai_verify_draft_workspace")
-    _call.launch(lib.ai_verify_draft, a, index, "ai_verify_draft")
+    _call.launch(lib.ai_verify_draft, a, target.get_device(), "ai_verify_draft")
     del ws
     return accepted, tokens, logprobs
