@@ -12,8 +12,8 @@
 // joins with the other list's.
 //
 // Two kernels, by the rows that meet each key:
-//   tile kernel   many rows, long lists: 128 rows x 64 keys a step on
-//                 tcgen05 (worker: a CTA);
+//   tile kernel   many rows, long lists: 128 rows x 64 keys or 256 rows x
+//                 128 keys a step on tcgen05 (worker: a CTA);
 //   warp kernel   few rows, short lists: 16 rows x 32 keys a step on
 //                 mma.sync, K and V by TMA (worker: one to four warps).
 //                 HBM-bound with few rows; a worker has no barrier of the CTA
@@ -39,7 +39,7 @@ namespace ai {
 namespace prefix {
 namespace tc {
 
-constexpr int BM = 128, BN = 64;
+constexpr int BM = 128;
 constexpr int kMaxBatch = 1024;  // two scans of the sequences sit in shared memory
 constexpr long long kWait = 1000000000LL;
 
@@ -62,26 +62,34 @@ struct Line {
 
 // Threads of a tile-kernel CTA with NT row tiles: a softmax warpgroup each, a
 // TMA and an MMA warp.
-__host__ __device__ constexpr int tile_threads(int NT) { return 128 * NT + 64; }
+// (NT = 2: whole warpgroups, for the register split.)
+__host__ __device__ constexpr int tile_threads(int NT) { return NT == 1 ? 192 : 384; }
+// Keys of its tiles.
+__host__ __device__ constexpr int tile_keys(int NT) { return NT == 1 ? 64 : 128; }
+// NT = 2: launched at 168 registers a thread; a row's 128 scores stay in the
+// softmax warpgroups', the third warpgroup (TMA and MMA warps) gives its up.
+constexpr uint32_t kRegLaunch = 168, kRegSoftmax = 208, kRegOther = 88;
+static_assert(256 * kRegSoftmax + 128 * kRegOther <= 384 * kRegLaunch, "register split");
 
 template <int D, int NT>
 struct Smem {
-  static constexpr uint32_t kTile = BN * D * 2;    // one K or V tile: D / 64 column blocks of 64 rows x 128 bytes
+  static constexpr int BN = tile_keys(NT), kBufs = 128 / BN;  // S buffers of a row tile
+  static constexpr uint32_t kTile = BN * D * 2;    // one K or V tile: D / 64 column blocks of BN rows x 128 bytes
   static constexpr uint32_t kQBlock = BM * 128;    // one column block of a Q tile
   static constexpr uint32_t kQ = BM * D * 2;
-  static constexpr int kSlots = NT * (D == 128 ? 4 : 8);  // ring of tiles, K and V alternating (64 KB per row tile)
+  static constexpr int kSlots = D == 128 ? 4 : 8;  // ring of tiles, K and V alternating (64 KB per row tile)
   static constexpr uint32_t Q = 0;
   static constexpr uint32_t RING = Q + NT * kQ;
   static constexpr uint32_t BARS = RING + kSlots * kTile;
-  // (two of each per row tile, for the two S buffers)
-  static constexpr int FULL = 0, EMPTY = kSlots, S_FULL = 2 * kSlots, P_READY = S_FULL + 2 * NT,
-                       O_DONE = P_READY + 2 * NT, Q_READY = O_DONE + 2 * NT, FINAL = Q_READY + NT, N_BARS = FINAL + 1;
+  // (kBufs of each per row tile)
+  static constexpr int FULL = 0, EMPTY = kSlots, S_FULL = 2 * kSlots, P_READY = S_FULL + kBufs * NT,
+                       O_DONE = P_READY + kBufs * NT, Q_READY = O_DONE + kBufs * NT, FINAL = Q_READY + NT, N_BARS = FINAL + 1;
   static constexpr uint32_t LINE = BARS + 8 * N_BARS;  // the line with the rows that there are
   static constexpr uint32_t TMEM_SLOT = LINE + sizeof(Line);
   static constexpr uint32_t ABORT = TMEM_SLOT + 4;
   static constexpr uint32_t SCAN = ABORT + 4;  // int [2][B + 1]
   static size_t bytes(int batch) { return SCAN + 8 * ((size_t)batch + 1) + 1024; }
-  // TMEM: two S buffers of 64 columns per row tile (P over their first 32), then O of D columns each.
+  // TMEM: 128 columns per row tile for its S buffers (P over a buffer's first half), then O of D columns each.
   static constexpr uint32_t kTmemCols = 256 * NT;
   static constexpr uint32_t C_S = 0, C_O = 128 * NT;
 };
@@ -284,14 +292,23 @@ __host__ __device__ constexpr uint32_t idesc(uint32_t fmt, int M, int N, bool b_
 }
 
 // NT = 1: up to 128 rows a unit, two CTAs per SM whose phases fill each
-// other's gaps; NT = 2: up to 256, halved over two row tiles that share every
-// K and V tile (each is read from L2 once, not twice), one CTA per SM.
+// other's gaps, 64 keys a tile and two S buffers (S of the tile after next
+// runs during a tile's softmax).  NT = 2: up to 256 rows, halved over two row
+// tiles that share every K and V tile (each is read from L2 once, not twice),
+// one CTA per SM; one row tile's MMAs run during the other's softmax, so one S
+// buffer each is enough and a tile has 128 keys: an S MMA of 64 keys reads as
+// much of Q from shared memory for half the work (172 us with 64-key tiles,
+// 158 us so, 64 sequences x 5 tokens x 32 heads on 32,768 keys, bf16, D 128).
+// Bound by the softmax: a row is one thread's, its exponentials a chain of
+// multiply-add, ex2, pack and store of about 600 instructions a tile (tensor
+// pipe and ex2 unit are each busy half of the time).
 template <typename T, int D, int NT>
 __global__ void __launch_bounds__(tile_threads(NT), NT == 1 ? 2 : 1)
     tile_kernel(const AiPrefixAttnArgs a, const Plan p, const __grid_constant__ CUtensorMap tm_k,
                 const __grid_constant__ CUtensorMap tm_v) {
   using L = Smem<D, NT>;
   constexpr int CB = D / 64, kTma = 4 * NT, kMma = kTma + 1;
+  constexpr int BN = L::BN, kBufs = L::kBufs;
   constexpr uint32_t C_S = L::C_S, C_O = L::C_O;
   // (the warp kernel reads nothing this one writes)
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -337,6 +354,13 @@ __global__ void __launch_bounds__(tile_threads(NT), NT == 1 ? 2 : 1)
     }
   auto head = [&](const Seg& s) { return s.b < 0 ? s.sub / ln.groups : s.sub % a.num_kv_heads; };
 
+  if constexpr (NT == 2) {
+    if (warp < kTma)
+      ptx::setmaxnreg_inc<kRegSoftmax>();
+    else
+      ptx::setmaxnreg_dec<kRegOther>();
+  }
+
   // Bounded wait of a whole warp: true in every lane or false in every lane
   // (a warp leaves its loops together).
   auto wait = [&](int i, uint32_t parity) -> bool {
@@ -355,7 +379,7 @@ __global__ void __launch_bounds__(tile_threads(NT), NT == 1 ? 2 : 1)
     const int wg = warp / 4, r = tid % 128;  // row tile, row of it
     const uint32_t lane_base = (uint32_t)((warp % 4) * 32) << 16;
     const uint32_t c_o = tmem + lane_base + C_O + (uint32_t)(wg * D);
-    const int S_FULL = L::S_FULL + 2 * wg, P_READY = L::P_READY + 2 * wg, O_DONE = L::O_DONE + 2 * wg;
+    const int S_FULL = L::S_FULL + kBufs * wg, P_READY = L::P_READY + kBufs * wg, O_DONE = L::O_DONE + kBufs * wg;
     const float sl2 = a.scale * kLog2e;
     // The rows of a segment: the thread's visible keys of its list, and Q into
     // shared memory (once no MMA reads the Q before it).  A thread finds its
@@ -406,7 +430,7 @@ __global__ void __launch_bounds__(tile_threads(NT), NT == 1 ? 2 : 1)
       for (int o = 16; o > 0; o >>= 1) least = min(least, __shfl_xor_sync(0xffffffffu, least, o));
       in_unit = wg * half + r;
     };
-    int g = 0;
+    int g = 0, seg = 0;
     bool ok = true;
     int w = w0;
     Seg s = next_seg(a, ln, scan, w, w1);
@@ -414,30 +438,34 @@ __global__ void __launch_bounds__(tile_threads(NT), NT == 1 ? 2 : 1)
     while (s.n > 0) {
       float m = -CUDART_INF_F, l = 0.f;
       for (int j = 0; j < s.n; ++j, ++g) {
-        const int k0 = (s.j0 + j) * BN, x = g & 1;
-        const uint32_t c_s = tmem + lane_base + C_S + (uint32_t)(wg * 128 + x * 64);
-        if (!(ok = wait(S_FULL + x, (g >> 1) & 1))) break;
+        const int k0 = (s.j0 + j) * BN, x = g % kBufs;
+        const uint32_t c_s = tmem + lane_base + C_S + (uint32_t)(wg * 128 + x * BN);
+        if (!(ok = wait(S_FULL + x, (g / kBufs) & 1))) break;
         ptx::tc_fence_after();
         if (active) {
-          uint32_t s0[32], s1[32];
-          ptx::tmem_ld32(c_s, s0);
-          ptx::tmem_ld32(c_s + 32, s1);
+          uint32_t sc[BN / 32][32];
+#pragma unroll
+          for (int c = 0; c < BN / 32; ++c) ptx::tmem_ld32(c_s + 32 * c, sc[c]);
           ptx::tmem_wait_ld();
           if (k0 + BN > least) {
             const int lim = limit - k0;
 #pragma unroll
-            for (int i = 0; i < 32; ++i) {
-              if (i >= lim) s0[i] = 0xff800000u;  // -inf
-              if (i + 32 >= lim) s1[i] = 0xff800000u;
-            }
-          }
-          float ma = -CUDART_INF_F, mb = -CUDART_INF_F;
+            for (int c = 0; c < BN / 32; ++c)
 #pragma unroll
-          for (int i = 0; i < 32; i += 2) {
-            ma = ptx::fmax3(ma, __uint_as_float(s0[i]), __uint_as_float(s0[i + 1]));
-            mb = ptx::fmax3(mb, __uint_as_float(s1[i]), __uint_as_float(s1[i + 1]));
+              for (int i = 0; i < 32; ++i)
+                if (i + 32 * c >= lim) sc[c][i] = 0xff800000u;  // -inf
           }
-          const float m_new = fmaxf(m, fmaxf(ma, mb) * sl2);
+          float mx[BN / 32];
+#pragma unroll
+          for (int c = 0; c < BN / 32; ++c) mx[c] = fmaxf(__uint_as_float(sc[c][0]), __uint_as_float(sc[c][1]));
+#pragma unroll
+          for (int i = 2; i < 32; i += 2)
+#pragma unroll
+            for (int c = 0; c < BN / 32; ++c)
+              mx[c] = ptx::fmax3(mx[c], __uint_as_float(sc[c][i]), __uint_as_float(sc[c][i + 1]));
+#pragma unroll
+          for (int c = 1; c < BN / 32; ++c) mx[0] = fmaxf(mx[0], mx[c]);
+          const float m_new = fmaxf(m, mx[0] * sl2);
           float alpha = 1.f;
           bool rescale = false;
           if (m_new > m + 8.f) {
@@ -448,8 +476,9 @@ __global__ void __launch_bounds__(tile_threads(NT), NT == 1 ? 2 : 1)
             m = m_new;
           }
           if (__any_sync(0xffffffffu, rescale)) {
-            // O holds the tiles before this one once their last P V is done.
-            if (!(ok = wait(O_DONE + (x ^ 1), ((g - 1) >> 1) & 1))) break;
+            // O holds the tiles before this one once their last P V is done
+            // (with one S buffer, this tile's S came after it).
+            if (kBufs > 1 && !(ok = wait(O_DONE + (x ^ 1), ((g - 1) / kBufs) & 1))) break;
             ptx::tc_fence_after();
 #pragma unroll
             for (int c = 0; c < D / 16; ++c) {
@@ -463,26 +492,21 @@ __global__ void __launch_bounds__(tile_threads(NT), NT == 1 ? 2 : 1)
             l *= alpha;
           }
           const float base = m == -CUDART_INF_F ? 0.f : m;
-          const float2 nm = make_float2(-base, -base), sc = make_float2(sl2, sl2);
-          float2 suma = make_float2(0.f, 0.f), sumb = make_float2(0.f, 0.f);
-          uint32_t pk[16];
+          const float2 nm = make_float2(-base, -base), sc2 = make_float2(sl2, sl2);
+          float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const float2 e = __ffma2_rn(make_float2(__uint_as_float(s0[2 * i]), __uint_as_float(s0[2 * i + 1])), sc, nm);
-            const float2 pr = make_float2(ptx::ex2(e.x), ptx::ex2(e.y));
-            suma = __fadd2_rn(suma, pr);
-            pk[i] = Pair<T>::pack(pr.x, pr.y);
-          }
-          ptx::tmem_st16(c_s, pk);
+          for (int c = 0; c < BN / 32; ++c) {
+            uint32_t pk[16];
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const float2 e = __ffma2_rn(make_float2(__uint_as_float(s1[2 * i]), __uint_as_float(s1[2 * i + 1])), sc, nm);
-            const float2 pr = make_float2(ptx::ex2(e.x), ptx::ex2(e.y));
-            sumb = __fadd2_rn(sumb, pr);
-            pk[i] = Pair<T>::pack(pr.x, pr.y);
+            for (int i = 0; i < 16; ++i) {
+              const float2 e = __ffma2_rn(make_float2(__uint_as_float(sc[c][2 * i]), __uint_as_float(sc[c][2 * i + 1])), sc2, nm);
+              const float2 pr = make_float2(ptx::ex2(e.x), ptx::ex2(e.y));
+              sum[c % 2] = __fadd2_rn(sum[c % 2], pr);
+              pk[i] = Pair<T>::pack(pr.x, pr.y);
+            }
+            ptx::tmem_st16(c_s + 16 * c, pk);
           }
-          ptx::tmem_st16(c_s + 16, pk);
-          l += (suma.x + suma.y) + (sumb.x + sumb.y);
+          l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
           ptx::tmem_wait_st();
         }
         ptx::tc_fence_before();
@@ -511,7 +535,8 @@ __global__ void __launch_bounds__(tile_threads(NT), NT == 1 ? 2 : 1)
       s = next_seg(a, ln, scan, w, w1);
       if (s.n > 0) load_rows(s);
       // The rows' partial results.
-      if (!(ok = wait(O_DONE + ((g - 1) & 1), ((g - 1) >> 1) & 1))) break;
+      if (!(ok = kBufs > 1 ? wait(O_DONE + (g - 1) % kBufs, ((g - 1) / kBufs) & 1) : wait(O_DONE, seg & 1))) break;
+      ++seg;
       ptx::tc_fence_after();
       if (cur_active) {
         const int64_t slot = cur.unit + (int)blockIdx.x;
@@ -575,7 +600,7 @@ __global__ void __launch_bounds__(tile_threads(NT), NT == 1 ? 2 : 1)
     if (!ok || *s_abort)
       for (int i = max(0, item - L::kSlots); i < item; ++i)
         ptx::mbar_wait(bar(L::FULL + i % L::kSlots), (i / L::kSlots) & 1, kWait);
-  } else {
+  } else if (warp == kMma) {
     // ------------------------------------------------------------ MMA
     constexpr uint32_t i_qk = idesc(Pair<T>::kFmt, BM, BN, false), i_pv = idesc(Pair<T>::kFmt, BM, D, true);
     const uint64_t d_q = ptx::sdesc_sw128(sbase + L::Q, 16, 1024);
@@ -593,10 +618,10 @@ __global__ void __launch_bounds__(tile_threads(NT), NT == 1 ? 2 : 1)
       const int slot = (2 * g) % L::kSlots;
 #pragma unroll
       for (int kk = 0; kk < D / 16; ++kk)
-        ptx::mma_ss_w(tmem + C_S + (uint32_t)(t * 128 + (g & 1) * 64),
+        ptx::mma_ss_w(tmem + C_S + (uint32_t)(t * 128 + (g % kBufs) * BN),
                       d_q + (uint64_t)((t * L::kQ + (kk >> 2) * L::kQBlock + (kk & 3) * 32) >> 4),
                       d_k + kT * (uint64_t)slot + (uint64_t)(((kk >> 2) * (BN * 128) + (kk & 3) * 32) >> 4), i_qk, kk > 0);
-      ptx::mma_commit_w(bar(L::S_FULL + 2 * t + (g & 1)));
+      ptx::mma_commit_w(bar(L::S_FULL + kBufs * t + g % kBufs));
       if (t == NT - 1) ptx::mma_commit_w(bar(L::EMPTY + slot));
     };
     int g = 0, seg = 0;
@@ -605,29 +630,30 @@ __global__ void __launch_bounds__(tile_threads(NT), NT == 1 ? 2 : 1)
       const Seg s = next_seg(a, ln, scan, w, w1);
       if (s.n == 0) break;
       for (int t = 0; t < NT && ok; ++t) ok = wait(L::Q_READY + t, seg & 1);
-      for (int j = 0; j < 2 && j < s.n && ok; ++j) {
+      for (int j = 0; j < kBufs && j < s.n && ok; ++j) {
         if (!(ok = wait_k(g + j))) break;
 #pragma unroll
         for (int t = 0; t < NT; ++t) issue_s(t, g + j);
       }
       for (int j = 0; j < s.n && ok; ++j) {
         const int gj = g + j, item = 2 * gj + 1, slot = item % L::kSlots;
-        const bool more = j + 2 < s.n;
+        const bool more = j + kBufs < s.n;
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
-          ok = wait(L::P_READY + 2 * t + (gj & 1), (gj >> 1) & 1) &&
+          ok = wait(L::P_READY + kBufs * t + gj % kBufs, (gj / kBufs) & 1) &&
                (t > 0 || wait(L::FULL + slot, (item / L::kSlots) & 1));
           if (!ok) break;
           ptx::tc_fence_after();
 #pragma unroll
           for (int kk = 0; kk < BN / 16; ++kk)
-            ptx::mma_ts_w(tmem + C_O + (uint32_t)(t * D), tmem + C_S + (uint32_t)(t * 128 + (gj & 1) * 64 + 8 * kk),
+            ptx::mma_ts_w(tmem + C_O + (uint32_t)(t * D), tmem + C_S + (uint32_t)(t * 128 + (gj % kBufs) * BN + 8 * kk),
                           d_v + kT * (uint64_t)slot + (uint64_t)((kk * 2048) >> 4), i_pv, (j > 0 || kk > 0) ? 1u : 0u);
-          ptx::mma_commit_w(bar(L::O_DONE + 2 * t + (gj & 1)));
+          // (one S buffer: nobody waits for another than a segment's last)
+          if (kBufs > 1 || j + 1 == s.n) ptx::mma_commit_w(bar(L::O_DONE + kBufs * t + gj % kBufs));
           if (t == NT - 1) ptx::mma_commit_w(bar(L::EMPTY + slot));
           if (more) {
-            if (t == 0 && !(ok = wait_k(gj + 2))) break;
-            issue_s(t, gj + 2);
+            if (t == 0 && !(ok = wait_k(gj + kBufs))) break;
+            issue_s(t, gj + kBufs);
           }
         }
       }
@@ -1140,6 +1166,7 @@ bool make_plan(const AiPrefixAttnArgs& a, Plan* p, size_t* bytes) {
   const int64_t most_unit = BM * p->nt, tt = (rows + most_unit - 1) / most_unit;
   // Own keys join the tile kernel's line when there is room for few of them
   // and the kernel runs anyway: a launch less.
+  const int BN = tile_keys(p->nt);
   if (!p->prefix_warp && a.batch * H * tt * (kStartTile + (capacity + BN - 1) / BN) <=
                              (int64_t)kFewOwn * (p->nt == 1 ? 2 * sms : sms))
     p->own_warp = false;
@@ -1183,7 +1210,7 @@ int launch_t(const AiPrefixAttnArgs& a, const Plan& p, cudaStream_t st) {
     return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) == cudaSuccess;
   };
   if (p.tile.workers > 0) {
-    if (!maps(BN)) return AI_ERR_TMA;
+    if (!maps(tile_keys(p.nt))) return AI_ERR_TMA;
     cfg.gridDim = dim3(p.tile.workers);
     cfg.blockDim = dim3(tile_threads(p.nt));
     const bool ok = p.nt == 1 ? smem_of(tile_kernel<T, D, 1>, Smem<D, 1>::bytes(a.batch)) &&
