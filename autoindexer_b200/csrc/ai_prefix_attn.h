@@ -2,6 +2,7 @@
 #pragma once
 
 #include <cuda_runtime.h>
+#include <math_constants.h>
 #include <stdint.h>
 
 #include "../../include/ai_attn.h"
@@ -42,6 +43,13 @@ __device__ __forceinline__ int page_of(const AiPrefixAttnArgs& a, const int32_t*
     return 0;
   }
   return p;
+}
+
+// The log-sum `lse` of a partial result with exponentials' sum l: -inf without
+// keys, +inf where l is NaN (a NaN among the row's scores), which makes the
+// joined row NaN.
+__device__ __forceinline__ float part_lse(float l, float lse) {
+  return l > 0.f ? lse : l == 0.f ? -CUDART_INF_F : CUDART_INF_F;
 }
 
 }  // namespace prefix

@@ -542,7 +542,7 @@ __global__ void __launch_bounds__(tile_threads(NT), NT == 1 ? 2 : 1)
         const int64_t slot = cur.unit + (int)blockIdx.x;
         const int64_t row = (cur.b < 0 ? ln.base_prefix + slot * ln.slot_prefix
                                        : ln.base_own + slot * ln.rows_own) + cur_row;
-        const float inv = l > 0.f ? 1.f / l : 0.f;
+        const float inv = 1.f / l;
 #pragma unroll
         for (int c = 0; c < D / 32; ++c) {
           uint32_t o[32];
@@ -553,12 +553,12 @@ __global__ void __launch_bounds__(tile_threads(NT), NT == 1 ? 2 : 1)
             for (int i = 0; i < 32; i += 8) {
               uint32_t v8[8];
 #pragma unroll
-              for (int e = 0; e < 8; ++e) v8[e] = l > 0.f ? __float_as_uint(__uint_as_float(o[i + e]) * inv) : 0u;
+              for (int e = 0; e < 8; ++e) v8[e] = l == 0.f ? 0u : __float_as_uint(__uint_as_float(o[i + e]) * inv);
               ptx::st_global_v8(p.part_o + row * D + 32 * c + i, v8);
             }
           }
         }
-        if (cur_valid) p.part_lse[row] = l > 0.f ? m + log2f(l) : -CUDART_INF_F;
+        if (cur_valid) p.part_lse[row] = part_lse(l, m + log2f(l));
       }
       ptx::tc_fence_before();
     }
@@ -1004,11 +1004,11 @@ __global__ void __launch_bounds__(warpk::kMaxThreads, 1)
       const int64_t slot = s.unit + worker;
       const int64_t row = (s.b < 0 ? ln.base_prefix + slot * ln.slot_prefix
                                    : ln.base_own + slot * ln.rows_own) + in_unit + r + 8 * h;
-      const float inv = sum > 0.f ? 1.f / sum : 0.f;
+      const float inv = sum == 0.f ? 0.f : 1.f / sum;
 #pragma unroll
       for (int i = 0; i < NB; ++i)
         *reinterpret_cast<float2*>(p.part_o + row * D + 8 * i + 2 * c) = make_float2(o[i][2 * h] * inv, o[i][2 * h + 1] * inv);
-      if (c == 0) p.part_lse[row] = sum > 0.f ? m[h] + log2f(sum) : -CUDART_INF_F;
+      if (c == 0) p.part_lse[row] = part_lse(sum, m[h] + log2f(sum));
     }
   }
   // The combine launch waits for this one; it must not end before the tile kernel's.
@@ -1101,10 +1101,10 @@ __global__ void __launch_bounds__(256) combine_kernel(const AiPrefixAttnArgs a, 
   if (!has) return;
   T* o = static_cast<T*>(a.out.ptr) + b * a.out.stride_b + h * a.out.stride_h + t * a.out.stride_t + E * lane;
 #pragma unroll
-  for (int e = 0; e < E; ++e) o[e] = from_f32<T>(sum > 0.f ? acc[e] / sum : 0.f);
+  for (int e = 0; e < E; ++e) o[e] = from_f32<T>(sum == 0.f ? 0.f : acc[e] / sum);
   if (lane == 0 && a.lse)
     a.lse[((int64_t)b * a.num_q_heads + h) * a.seq_len + t] =
-        sum > 0.f ? (M + log2f(sum)) * kLn2 : -CUDART_INF_F;
+        sum == 0.f ? -CUDART_INF_F : (M + log2f(sum)) * kLn2;
 }
 
 // ---------------------------------------------------------------- host

@@ -198,6 +198,54 @@ def test_attention_extreme_scores(cuda_device):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("T,P,dtype", [(1, 200, torch.bfloat16), (1, 5000, torch.bfloat16), (20, 200, torch.float16),
+                                       (70, 200, torch.bfloat16), (1, 200, torch.float32), (3, 5000, torch.float32)])
+def test_attention_nan_stays_with_the_rows_that_see_it(T, P, dtype, cuda_device):
+    """A NaN among a sequence's keys makes its rows of that KV head NaN, and no other."""
+    from autoindexer_b200 import shared_prefix_attention
+
+    lens = [T + 70, T + 5, T + 64]
+    q, kp, vp, prefix, table = _cache(3, T, 8, 2, 128, 64, P, lens, dtype, 12, cuda_device)
+    held = torch.tensor(lens, dtype=torch.int32, device=cuda_device)
+    want, wlse = shared_prefix_attention(q, kp, vp, prefix, P, table, held, return_lse=True)
+    kp[int(table[1, 0]), 0, 2, 5] = float("nan")
+    got, lse = shared_prefix_attention(q, kp, vp, prefix, P, table, held, return_lse=True)
+    assert got[1, :, :4].isnan().all() and lse[1, :4].isnan().all()
+    for b, heads in ((0, slice(0, 8)), (1, slice(4, 8)), (2, slice(0, 8))):
+        assert torch.equal(got[b, :, heads], want[b, :, heads]) and torch.equal(lse[b, heads], wlse[b, heads])
+
+
+MORE = [
+    # as ATTEND: the kernels for other types and layouts, and more sequences than a scan holds
+    (16, 1, 32, 8, 128, 64, 1000, list(range(3, 99, 6)), None, torch.float32),
+    (3, 7, 24, 8, 128, 48, 333, [7, 130, 64], [7, 2, 0], torch.bfloat16),
+    (2, 5, 8, 1, 64, 64, 4099, [500, 5], [5, 4], torch.float32),
+    (1, 1, 2, 2, 32, 32, 0, [0], None, torch.float16),
+    (4, 2, 4, 2, 32, 128, 129, [2, 128, 129, 400], [1, 2, 2, 2], torch.float32),
+    (1030, 1, 4, 2, 64, 16, 40, [1 + i % 7 for i in range(1030)], None, torch.bfloat16),
+    (30, 5, 32, 8, 128, 64, 900, [5 + 3 * i for i in range(30)], [1 + i % 5 for i in range(30)], torch.float16),
+    (3, 90, 16, 4, 128, 32, 600, [90, 160, 91], [90, 17, 1], torch.bfloat16),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("B,T,Hq,Hkv,D,S,P,lens,n,dtype", MORE)
+def test_attention_more(B, T, Hq, Hkv, D, S, P, lens, n, dtype, cuda_device):
+    test_attention(B, T, Hq, Hkv, D, S, P, lens, n, dtype, cuda_device)
+
+
+@pytest.mark.gpu
+def test_attention_negative_scale(cuda_device):
+    from autoindexer_b200 import shared_prefix_attention
+
+    lens = [70, 3]
+    q, kp, vp, prefix, table = _cache(2, 2, 8, 2, 128, 32, 75, lens, torch.bfloat16, 5, cuda_device)
+    out, lse = shared_prefix_attention(q, kp, vp, prefix, 75, table, torch.tensor(lens, dtype=torch.int32, device=cuda_device),
+                                       scaling=-0.05, return_lse=True)
+    _check(q, kp, vp, prefix, 75, table, lens, [2, 2], out, lse, -0.05, torch.bfloat16)
+
+
+@pytest.mark.gpu
 def test_attention_bad_lengths_and_pages_are_reported(cuda_device):
     from autoindexer_b200 import read_status, shared_prefix_attention
 
