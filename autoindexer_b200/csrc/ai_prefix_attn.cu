@@ -9,10 +9,12 @@
 // per key forms four rows' scores, the rows' running maximum and sum stay in
 // the warp, and a lane per D / 32 dims adds four rows' weighted values, so a
 // value from shared memory meets four rows.  The chunks' partial results (O / l
-// and the log-sum, fp32) are joined by a second launch.  Bound by shared
-// memory reads (fp32: eight 128-byte wavefronts per 16 warp multiply-adds).
+// and the log-sum, fp32) are joined by a second launch.  Bound by the chain of
+// a step (page, K and V rows, shared memory) at four CTAs per SM, then by
+// shared memory: eight 128-byte wavefronts per 16 warp multiply-adds.
 // Measured on 16 sequences x 32 heads (8 KV heads, D 128), one token each, on
-// a prefix of 4096 keys and up to 512 own: @MEASURED@
+// a prefix of 4096 keys and up to 512 own: 104 us in fp32, 100 us in bf16 with
+// 48-slot pages (a CTA per query row: 1453 and 1526 us).
 
 #include <cuda_runtime.h>
 #include <math_constants.h>
@@ -36,7 +38,7 @@ struct Plan {
   int splits_prefix, splits_own;     // chunks of a list (own: of what the table can hold)
   int chunk_prefix, chunk_own;       // keys of a chunk
   int items_prefix, items;           // CTAs
-  bool vec;                          // K and V rows start on 16-byte boundaries
+  bool vec_q, vec;                   // Q rows, K and V rows start on 16-byte boundaries
   float *part_o, *part_lse;          // [B Hq T][splits_prefix + splits_own] rows
 };
 
@@ -70,8 +72,9 @@ __global__ void __launch_bounds__(kThreads) rows_kernel(const AiPrefixAttnArgs a
   constexpr int E = D / 32, C = D / 4;
   const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
   __shared__ __align__(16) float s_q[kRows][D], s_k[kKeys][D + 4], s_v[kKeys][D], s_p[kRows][kKeys];
-  __shared__ int64_t s_at[2][kKeys];  // offsets of the keys' K and V rows, -1: none
+  __shared__ int64_t s_at[2][kKeys];  // offsets of the keys' K and V rows
   __shared__ int64_t s_row[kRows];    // partial-result row, -1: none
+  __shared__ int64_t s_src[kRows];    // offset of its query
   __shared__ int s_limit[kRows];      // keys of the list that the row sees
 
   // The chunk and its rows.
@@ -90,28 +93,40 @@ __global__ void __launch_bounds__(kThreads) rows_kernel(const AiPrefixAttnArgs a
   if (k_begin >= k_end) return;
   const int32_t* table = pre ? a.prefix_pages : a.page_table + b * a.page_table_stride;
 
-  for (int i = tid; i < kRows * C; i += kThreads) {
-    const int r = i / C, c = i % C;
-    const int64_t n = row0 + r;
-    float4 q = make_float4(0.f, 0.f, 0.f, 0.f);
-    int64_t part = -1;
+  // Offset of key k's row in K (threads below kKeys) or V.
+  const AiTensor4& pool = tid < kKeys ? a.k_pages : a.v_pages;
+  auto key_at = [&](int k) -> int64_t {
+    if (tid >= 2 * kKeys || k >= k_end) return -1;
+    const int page = k / a.page_size;
+    return page_of(a, table, page) * pool.stride_b + hk * pool.stride_h + (k - page * a.page_size) * pool.stride_t;
+  };
+  int64_t next_at = key_at((int)k_begin + tid % kKeys);
+  if (tid < kRows) {
+    int64_t part = -1, src = -1;
     int limit = 0;
-    if (n < (pre ? (int64_t)a.batch * p.rows_seq : p.rows_seq)) {
-      const int64_t rb = pre ? n / p.rows_seq : b;
-      const int rem = (int)(pre ? n % p.rows_seq : n), t = rem / p.group, h = hk * p.group + rem % p.group;
+    if (row0 + tid < (pre ? a.batch * p.rows_seq : p.rows_seq)) {
+      const int n = row0 + tid, rb = pre ? n / p.rows_seq : (int)b, rem = pre ? n - rb * p.rows_seq : n;
+      const int t = rem / p.group, h = hk * p.group + rem - t * p.group;
       const Lens len = seq_lens(a, rb);
       if (t < len.n) {
-        q = load4(static_cast<const T*>(a.q.ptr) + rb * a.q.stride_b + h * a.q.stride_h + t * a.q.stride_t + 4 * c, false);
+        src = rb * a.q.stride_b + h * a.q.stride_h + t * a.q.stride_t;
         limit = pre ? keys : max(0, keys - len.n + t + 1);
-        part = ((rb * a.num_q_heads + h) * a.seq_len + t) * (p.splits_prefix + p.splits_own) +
+        part = (((int64_t)rb * a.num_q_heads + h) * a.seq_len + t) * (p.splits_prefix + p.splits_own) +
                (pre ? split : p.splits_prefix + split);
       }
     }
-    q.x *= a.scale, q.y *= a.scale, q.z *= a.scale, q.w *= a.scale;
-    *reinterpret_cast<float4*>(&s_q[r][4 * c]) = q;
-    if (c == 0) s_row[r] = part, s_limit[r] = limit;
+    s_row[tid] = part, s_limit[tid] = limit, s_src[tid] = src;
   }
   __syncthreads();
+#pragma unroll
+  for (int i = tid; i < kRows * C; i += kThreads) {
+    const int r = i / C, c = i % C;
+    const int64_t src = s_src[r];
+    float4 q = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (src >= 0) q = load4(static_cast<const T*>(a.q.ptr) + src + 4 * c, p.vec_q);
+    q.x *= a.scale, q.y *= a.scale, q.z *= a.scale, q.w *= a.scale;
+    *reinterpret_cast<float4*>(&s_q[r][4 * c]) = q;
+  }
   int limit[kWarpRows], least = 0x7fffffff;
   float m[kWarpRows], l[kWarpRows], acc[kWarpRows][E];
 #pragma unroll
@@ -124,26 +139,25 @@ __global__ void __launch_bounds__(kThreads) rows_kernel(const AiPrefixAttnArgs a
     for (int e = 0; e < E; ++e) acc[r][e] = 0.f;
   }
   for (int k0 = (int)k_begin; k0 < k_end; k0 += kKeys) {
-    if (tid < 2 * kKeys) {
-      const int k = k0 + tid % kKeys;
-      const AiTensor4& pool = tid < kKeys ? a.k_pages : a.v_pages;
-      s_at[tid / kKeys][tid % kKeys] =
-          k < k_end ? page_of(a, table, k / a.page_size) * pool.stride_b + hk * pool.stride_h +
-                          (k % a.page_size) * pool.stride_t
-                    : -1;
-    }
+    if (tid < 2 * kKeys) s_at[tid / kKeys][tid % kKeys] = next_at;
     __syncthreads();
-#pragma unroll 8
-    for (int i = tid; i < kKeys * C; i += kThreads) {
-      const int k = i / C, c = i % C;
-      const int64_t ka = s_at[0][k], va = s_at[1][k];
-      float4 kv = make_float4(0.f, 0.f, 0.f, 0.f), vv = kv;
-      if (ka >= 0) {
-        kv = load4(static_cast<const T*>(a.k_pages.ptr) + ka + 4 * c, p.vec);
-        vv = load4(static_cast<const T*>(a.v_pages.ptr) + va + 4 * c, p.vec);
-      }
-      *reinterpret_cast<float4*>(&s_k[k][4 * c]) = kv;
-      *reinterpret_cast<float4*>(&s_v[k][4 * c]) = vv;
+    next_at = key_at(k0 + kKeys + tid % kKeys);
+    // (past the list: the step's first key's row, as zeros)
+    constexpr int kLoads = kKeys * C / kThreads;
+    float4 kv[kLoads], vv[kLoads];
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      const int x = tid + i * kThreads, k = k0 + x / C < k_end ? x / C : 0;
+      kv[i] = load4(static_cast<const T*>(a.k_pages.ptr) + s_at[0][k] + 4 * (x % C), p.vec);
+      vv[i] = load4(static_cast<const T*>(a.v_pages.ptr) + s_at[1][k] + 4 * (x % C), p.vec);
+    }
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      const int x = tid + i * kThreads;
+      const bool in = k0 + x / C < k_end;
+      const float4 zero = make_float4(0.f, 0.f, 0.f, 0.f);
+      *reinterpret_cast<float4*>(&s_k[x / C][4 * (x % C)]) = in ? kv[i] : zero;
+      *reinterpret_cast<float4*>(&s_v[x / C][4 * (x % C)]) = in ? vv[i] : zero;
     }
     __syncthreads();
     // Scores of key `lane` with the warp's rows.
@@ -231,16 +245,24 @@ __global__ void __launch_bounds__(kThreads) join_kernel(const AiPrefixAttnArgs a
   if (t < len.n) {
     const int pre = p.splits_prefix, all = pre + p.splits_own;
     const int n = pre + (len.keys > 0 ? (len.keys - 1) / p.chunk_own + 1 : 0);
-    for (int i = 0; i < n; ++i) {
-      const float lse = p.part_lse[row * all + i];
-      if (lse == -CUDART_INF_F) continue;
-      const float m_new = fmaxf(m, lse), alpha = expf(m - m_new), w = expf(lse - m_new);
-      float o[E];
-      read<E>(p.part_o + (row * all + i) * D + E * lane, o);
-      m = m_new;
-      l = l * alpha + w;
+    const float* lse = p.part_lse + row * all;
+    for (int i = lane; i < n; i += 32) m = fmaxf(m, lse[i]);
 #pragma unroll
-      for (int e = 0; e < E; ++e) acc[e] = acc[e] * alpha + w * o[e];
+    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    if (m != -CUDART_INF_F) {
+      for (int i0 = 0; i0 < n; i0 += 32) {
+        const float mine = i0 + lane < n ? expf(lse[i0 + lane] - m) : 0.f;
+        const int cnt = min(32, n - i0);
+#pragma unroll 4
+        for (int k = 0; k < cnt; ++k) {
+          const float w = __shfl_sync(0xffffffffu, mine, k);
+          float o[E];
+          read<E>(p.part_o + (row * all + i0 + k) * D + E * lane, o);
+          l += w;
+#pragma unroll
+          for (int e = 0; e < E; ++e) acc[e] = fmaf(w, o[e], acc[e]);
+        }
+      }
     }
   }
   T* o = static_cast<T*>(a.out.ptr) + b * a.out.stride_b + h * a.out.stride_h + t * a.out.stride_t + E * lane;
@@ -297,10 +319,11 @@ bool make_plan(const AiPrefixAttnArgs& a, Plan* p, size_t* bytes) {
   p->items_prefix = (int)items_prefix;
   p->items = (int)items;
   const int64_t es = a.dtype == AI_DTYPE_F32 ? 4 : 2;
-  p->vec = true;
-  for (const AiTensor4* t : {&a.k_pages, &a.v_pages})
-    if ((reinterpret_cast<uintptr_t>(t->ptr) | (t->stride_b * es) | (t->stride_h * es) | (t->stride_t * es)) & 15)
-      p->vec = false;
+  auto aligned = [&](const AiTensor4& t) {
+    return ((reinterpret_cast<uintptr_t>(t.ptr) | (t.stride_b * es) | (t.stride_h * es) | (t.stride_t * es)) & 15) == 0;
+  };
+  p->vec_q = aligned(a.q);
+  p->vec = aligned(a.k_pages) && aligned(a.v_pages);
   const size_t slots = (size_t)all * H * (p->splits_prefix + p->splits_own);
   const size_t o_bytes = (slots * a.head_dim * 4 + 255) & ~size_t(255);
   p->part_o = static_cast<float*>(a.workspace);
