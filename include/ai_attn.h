@@ -544,8 +544,15 @@ int ai_paged_append(const AiPagedAppendArgs* args, void* stream);
  * of prefix_pages and the first lens[b] - n_b + t + 1 keys of its own pages
  * (lens counts the new tokens).  Padding tokens (t >= n_b) and tokens without
  * a key give 0 (lse -inf).  K and V hold the keys as the scores use them
- * (already rotated).  The prefix's K and V are read once per 128 query rows
- * of a KV head over the whole batch, not once per sequence. */
+ * (already rotated).  The prefix's K and V are read for the batch, not for
+ * each sequence: once per up to 256 query rows of a KV head (a short prefix:
+ * once per 16 to 64).  A key that a row does not see still meets the row with
+ * weight 0 where other rows of its sequence see it, so held values are finite.
+ *
+ * bf16 and fp16 with head_dim 64 or 128, page_size a power of two from 16,
+ * q, k_pages and v_pages with 16-byte aligned rows, scale > 0 and at most
+ * 1024 sequences run on the tensor cores; everything else on fp32 arithmetic
+ * (several times slower). */
 typedef struct AiPrefixAttnArgs {
   int32_t batch;
   int32_t seq_len;            /* T: query tokens per sequence */
