@@ -98,10 +98,17 @@ static_assert(Smem<128, 2>::SCAN + 8 * (kMaxBatch + 1) + 1024 <= 227 * 1024, "on
 
 constexpr int kWarpRows = 64;   // most rows of a sequence on the warp kernel
 constexpr int kWarpKeys = 32;   // keys of its tile
-constexpr int kShortPrefix = 6;  // positions of a prefix per worker of the warp kernel, at most
-constexpr int kFewOwn = 6;       // positions of own keys per worker of the tile kernel, at most
-// What starting a unit costs, in tiles of its kernel (chosen by the spread of
-// the CTAs' times over prefixes and sequences of 1 to 32768 keys).
+// Cuts, with both sides measured (bf16, 32 + 8 heads, D 128, one token; us;
+// "64 on 2048 + 256": 64 sequences, prefix, most own keys).  kShortPrefix:
+// positions of a prefix per worker of the warp kernel, at most (3 / 6 / 12: 36 /
+// 24 / 23 on 64 on 1024 + 64; 45 / 44 / 34 on 64 on 2048 + 256, but 29 / 29 / 34
+// on 16 on 8192 + 512).  kFewOwn: positions of own keys per worker of the tile
+// kernel, at most (0 / 6 / 12: 34 / 29 / 27 on 16 on 8192 + 512, 47 / 39 / 39 on
+// 4 on 32,768 + 1; larger cuts send lists there that the warp kernel streams).
+constexpr int kShortPrefix = 6, kFewOwn = 6;
+// What starting a unit costs, in tiles of its kernel (kStartTile 2 / 4 / 8: 112 /
+// 108 / 107 on 64 on 32,768 + 2048, 27 / 28 / 36 on 16 on 8192 + 512; kStartWarp
+// 1 / 2 / 4: 68 / 59 / 57 on 64 on 64 + 2048, 24 / 24 / 25 on 64 on 1024 + 64).
 constexpr int kStartTile = 4, kStartWarp = 2;
 
 // What the host knows of the work.
@@ -1170,8 +1177,11 @@ bool make_plan(const AiPrefixAttnArgs& a, Plan* p, size_t* bytes) {
   if (!p->prefix_warp && a.batch * H * tt * (kStartTile + (capacity + BN - 1) / BN) <=
                              (int64_t)kFewOwn * (p->nt == 1 ? 2 * sms : sms))
     p->own_warp = false;
+  // (256 rows x 128 keys outweigh a start, so a short line spreads over all
+  // SMs: 39 us with one position a CTA at least, 44 with five, 64 sequences on
+  // 2048 + 256 keys.  64-key tiles: no difference beyond 1 us.)
   if (!line(p->tile, !p->prefix_warp, !p->own_warp, BN, most_unit, tt * H, (rows + tt - 1) / tt,
-            p->nt == 1 ? 2 * sms : sms, kStartTile, kStartTile + 1))
+            p->nt == 1 ? 2 * sms : sms, kStartTile, p->nt == 1 ? kStartTile + 1 : 1))
     return false;
   if (!line(p->warp, p->prefix_warp, p->own_warp, kWarpKeys, group_rows, H, rows, workers, kStartWarp, 2)) return false;
   char* ws = static_cast<char*>(a.workspace);

@@ -4,7 +4,10 @@
 //
 // HBM-bound: every logit is read once for its row's normaliser, and of each
 // sequence one target row, one draft row and the noise row once more for the
-// race (mostly from L2).  Two launches, the second started by programmatic
+// race (mostly from L2).  Measured with a vocabulary of 151,936: 64 sequences of
+// four drafts, bf16: 51 us (4.2 TB/s of what is read once; the stats pass
+// alone 35 us, 5.0 TB/s); 16 of seven, fp32, no draft logits: 22.5 us; one of
+// three: 8.4 us, two launches' latency.  Two launches, the second started by programmatic
 // dependent launch:
 //   stats  a CTA per (row, vocabulary slice): the sum of 2^(c x - o),
 //          c = log2(e) / tau and o = c max, four 16-byte loads per
@@ -32,6 +35,11 @@ namespace verify {
 
 constexpr int kThreads = 256, kWarps = kThreads / 32;
 constexpr int kMaxDraft = 64;
+// Logits of a slice, at least: a round of 16-byte loads of all the CTA's threads
+// (stats, 16-bit logits; half for fp32), one round of the race.  One sequence of
+// three drafts, vocabulary 151,936, bf16: stats 9.1 / 8.4 / 8.8 us with 4096 /
+// 8192 / 16384, race 8.4 / 8.4 / 9.7 with 1024 / 2048 / 8192.
+constexpr int kLeastStats = 8192, kLeastPick = 2048;
 
 // The exponent of a logit is fma(x, c, -o), rounded once, with o the rounded
 // c max: every pass over a row uses the same o, so its own rounding is a
@@ -490,11 +498,11 @@ int sm_count() {
   return sms;
 }
 
-// Slices of the vocabulary for `rows` rows: enough CTAs for four per SM (what the registers
-// of both kernels admit at once),
-// but at least 2048 logits each.
-int slices(const AiVerifyArgs& a, int64_t rows) {
-  const int64_t want = (4 * (int64_t)sm_count() + rows - 1) / rows, most = (a.vocab + 2047) / 2048;
+// Slices of the vocabulary for `rows` rows: enough CTAs for four per SM (what
+// the registers of both kernels admit at once; 64 sequences of four drafts: 59 /
+// 51 / 54 us with 2 / 4 / 8), but at least `least` logits each.
+int slices(const AiVerifyArgs& a, int64_t rows, int least) {
+  const int64_t want = (4 * (int64_t)sm_count() + rows - 1) / rows, most = (a.vocab + least - 1) / least;
   return (int)(want < most ? want : most);
 }
 
@@ -504,7 +512,7 @@ int64_t row_count(const AiVerifyArgs& a) {
 
 size_t layout(const AiVerifyArgs& a, Ws* w) {
   const int64_t rows = row_count(a);
-  w->splits = slices(a, rows);
+  w->splits = slices(a, rows, a.dtype == AI_DTYPE_F32 ? kLeastStats / 2 : kLeastStats);
   const size_t stat = ((size_t)rows * w->splits * sizeof(Stat) + 255) & ~size_t(255);
   const size_t key = ((size_t)a.batch * sizeof(unsigned long long) + 255) & ~size_t(255);
   char* p = static_cast<char*>(a.workspace);
@@ -519,7 +527,7 @@ int launch(const AiVerifyArgs& a, const Ws& w, cudaStream_t st) {
   ProfScope ps(AI_PROF_VERIFY, st);
   stats_kernel<T><<<dim3(w.splits, (unsigned)row_count(a)), kThreads, 0, st>>>(a, w);
   if (cudaGetLastError() != cudaSuccess) return AI_ERR_LAUNCH;
-  const int n = slices(a, a.batch), slice = ((a.vocab + n - 1) / n + 7) / 8 * 8;
+  const int n = slices(a, a.batch, kLeastPick), slice = ((a.vocab + n - 1) / n + 7) / 8 * 8;
   // Every row the race reads starts on a 16-byte boundary.
   uintptr_t at = reinterpret_cast<uintptr_t>(a.target) | reinterpret_cast<uintptr_t>(a.noise);
   int64_t step = (a.target_stride_b | a.target_stride_t) * (int64_t)sizeof(T) | a.vocab * (int64_t)sizeof(float);
