@@ -81,9 +81,10 @@ struct Smem {
   static constexpr uint32_t Q = 0;
   static constexpr uint32_t RING = Q + NT * kQ;
   static constexpr uint32_t BARS = RING + kSlots * kTile;
-  // (kBufs of each per row tile)
+  // (kBufs of each per row tile; P_HALF: the first half of P, with one S buffer)
   static constexpr int FULL = 0, EMPTY = kSlots, S_FULL = 2 * kSlots, P_READY = S_FULL + kBufs * NT,
-                       O_DONE = P_READY + kBufs * NT, Q_READY = O_DONE + kBufs * NT, FINAL = Q_READY + NT, N_BARS = FINAL + 1;
+                       O_DONE = P_READY + kBufs * NT, Q_READY = O_DONE + kBufs * NT, P_HALF = Q_READY + NT,
+                       FINAL = P_HALF + NT, N_BARS = FINAL + 1;
   static constexpr uint32_t LINE = BARS + 8 * N_BARS;  // the line with the rows that there are
   static constexpr uint32_t TMEM_SLOT = LINE + sizeof(Line);
   static constexpr uint32_t ABORT = TMEM_SLOT + 4;
@@ -306,6 +307,9 @@ __host__ __device__ constexpr uint32_t idesc(uint32_t fmt, int M, int N, bool b_
 // buffer each is enough and a tile has 128 keys: an S MMA of 64 keys reads as
 // much of Q from shared memory for half the work (172 us with 64-key tiles,
 // 158 us so, 64 sequences x 5 tokens x 32 heads on 32,768 keys, bf16, D 128).
+// P goes out in two halves, so that only half of P V and the next S stand
+// between a row tile's last exponential and its next scores (with own keys of
+// up to 2048: 196 us whole, 192 so).
 // Bound by the softmax: a row is one thread's, its exponentials a chain of
 // multiply-add, ex2, pack and store of about 600 instructions a tile (tensor
 // pipe and ex2 unit are each busy half of the time).
@@ -449,6 +453,20 @@ __global__ void __launch_bounds__(tile_threads(NT), NT == 1 ? 2 : 1)
         const uint32_t c_s = tmem + lane_base + C_S + (uint32_t)(wg * 128 + x * BN);
         if (!(ok = wait(S_FULL + x, (g / kBufs) & 1))) break;
         ptx::tc_fence_after();
+        if (wg == 0 && k0 + BN > s.keys) {
+          // Slots past the list hold anything, NaN included, and meet P = 0:
+          // clear their V rows (before the first row tile's P V, which the
+          // second's follows).
+          const int item = 2 * g + 1;
+          if (!(ok = wait(L::FULL + item % L::kSlots, (item / L::kSlots) & 1))) break;
+          uint8_t* v = sm + L::RING + (item % L::kSlots) * L::kTile;
+          const int first = s.keys - k0;
+          for (int i = tid; i < (BN - first) * CB * 8; i += 128) {
+            const int row = first + i / (CB * 8), c = i % (CB * 8);
+            *reinterpret_cast<uint4*>(v + (c / 8) * (BN * 128) + row * 128 + (c % 8) * 16) = make_uint4(0, 0, 0, 0);
+          }
+          ptx::fence_proxy_async_smem();
+        }
         if (active) {
           uint32_t sc[BN / 32][32];
 #pragma unroll
@@ -512,25 +530,18 @@ __global__ void __launch_bounds__(tile_threads(NT), NT == 1 ? 2 : 1)
               pk[i] = Pair<T>::pack(pr.x, pr.y);
             }
             ptx::tmem_st16(c_s + 16 * c, pk);
+            if (kBufs == 1 && c == BN / 64 - 1) {
+              ptx::tmem_wait_st();
+              ptx::tc_fence_before();
+              ptx::mbar_arrive(bar(L::P_HALF + wg));
+            }
           }
           l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
           ptx::tmem_wait_st();
+        } else if (kBufs == 1) {
+          ptx::mbar_arrive(bar(L::P_HALF + wg));
         }
         ptx::tc_fence_before();
-        if (wg == 0 && k0 + BN > s.keys) {
-          // Slots past the list hold anything, NaN included, and meet P = 0:
-          // clear their V rows (before the first row tile's P V, which the
-          // second's follows).
-          const int item = 2 * g + 1;
-          if (!(ok = wait(L::FULL + item % L::kSlots, (item / L::kSlots) & 1))) break;
-          uint8_t* v = sm + L::RING + (item % L::kSlots) * L::kTile;
-          const int first = s.keys - k0;
-          for (int i = tid; i < (BN - first) * CB * 8; i += 128) {
-            const int row = first + i / (CB * 8), c = i % (CB * 8);
-            *reinterpret_cast<uint4*>(v + (c / 8) * (BN * 128) + row * 128 + (c % 8) * 16) = make_uint4(0, 0, 0, 0);
-          }
-          ptx::fence_proxy_async_smem();
-        }
         ptx::mbar_arrive(bar(P_READY + x));
       }
       if (!ok) break;
@@ -624,10 +635,10 @@ __global__ void __launch_bounds__(tile_threads(NT), NT == 1 ? 2 : 1)
     auto issue_s = [&](int t, int g) {
       const int slot = (2 * g) % L::kSlots;
 #pragma unroll
-      for (int kk = 0; kk < D / 16; ++kk)
-        ptx::mma_ss_w(tmem + C_S + (uint32_t)(t * 128 + (g % kBufs) * BN),
-                      d_q + (uint64_t)((t * L::kQ + (kk >> 2) * L::kQBlock + (kk & 3) * 32) >> 4),
-                      d_k + kT * (uint64_t)slot + (uint64_t)(((kk >> 2) * (BN * 128) + (kk & 3) * 32) >> 4), i_qk, kk > 0);
+      for (int c = 0; c < CB; ++c)
+        ptx::mma_ss4_w(tmem + C_S + (uint32_t)(t * 128 + (g % kBufs) * BN),
+                       d_q + (uint64_t)((t * L::kQ + c * L::kQBlock) >> 4),
+                       d_k + kT * (uint64_t)slot + (uint64_t)((c * (BN * 128)) >> 4), i_qk, c > 0);
       ptx::mma_commit_w(bar(L::S_FULL + kBufs * t + g % kBufs));
       if (t == NT - 1) ptx::mma_commit_w(bar(L::EMPTY + slot));
     };
@@ -647,19 +658,27 @@ __global__ void __launch_bounds__(tile_threads(NT), NT == 1 ? 2 : 1)
         const bool more = j + kBufs < s.n;
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
-          ok = wait(L::P_READY + kBufs * t + gj % kBufs, (gj / kBufs) & 1) &&
-               (t > 0 || wait(L::FULL + slot, (item / L::kSlots) & 1));
-          if (!ok) break;
-          ptx::tc_fence_after();
+          if (t == 0 && !(ok = wait(L::FULL + slot, (item / L::kSlots) & 1))) break;
+          // P V of k-steps [k0, k1)
+          auto pv = [&](int k0, int k1) {
+            ptx::tc_fence_after();
 #pragma unroll
-          for (int kk = 0; kk < BN / 16; ++kk)
-            ptx::mma_ts_w(tmem + C_O + (uint32_t)(t * D), tmem + C_S + (uint32_t)(t * 128 + (gj % kBufs) * BN + 8 * kk),
-                          d_v + kT * (uint64_t)slot + (uint64_t)((kk * 2048) >> 4), i_pv, (j > 0 || kk > 0) ? 1u : 0u);
+            for (int kk = k0; kk < k1; kk += 4)
+              ptx::mma_ts4_w(tmem + C_O + (uint32_t)(t * D), tmem + C_S + (uint32_t)(t * 128 + (gj % kBufs) * BN + 8 * kk),
+                             d_v + kT * (uint64_t)slot + (uint64_t)((kk * 2048) >> 4), i_pv, (j > 0 || kk > 0) ? 1u : 0u);
+          };
+          if constexpr (kBufs == 1) {
+            if (!(ok = wait(L::P_HALF + t, gj & 1))) break;
+            pv(0, BN / 32);
+            if (t == 0 && more && !(ok = wait_k(gj + 1))) break;
+          }
+          if (!(ok = wait(L::P_READY + kBufs * t + gj % kBufs, (gj / kBufs) & 1))) break;
+          pv(kBufs == 1 ? BN / 32 : 0, BN / 16);
           // (one S buffer: nobody waits for another than a segment's last)
           if (kBufs > 1 || j + 1 == s.n) ptx::mma_commit_w(bar(L::O_DONE + kBufs * t + gj % kBufs));
           if (t == NT - 1) ptx::mma_commit_w(bar(L::EMPTY + slot));
           if (more) {
-            if (t == 0 && !(ok = wait_k(gj + kBufs))) break;
+            if (kBufs > 1 && t == 0 && !(ok = wait_k(gj + kBufs))) break;
             issue_s(t, gj + kBufs);
           }
         }
