@@ -19,9 +19,14 @@
 //                 HBM-bound with few rows; a worker has no barrier of the CTA
 //                 in its loop and a short list costs a few loads, where the
 //                 tile kernel pays a chain of TMA, MMA and TMEM latencies per
-//                 unit (measured: 4.8 us per unit of one 64-key tile).
-// They run one after the other by programmatic dependent launch, so that the
-// second fills the SMs the first leaves.
+//                 unit (4.8 us per unit of one 64-key tile).  Own lists of 64
+//                 sequences of up to 2048 keys: 48 us, 5.6 TB/s.
+// The second is launched by programmatic dependent launch: it fills the SMs the
+// first leaves, or takes its share of them from the start (make_plan).
+//
+// Measured (bf16, 32 + 8 heads, D 128, up to 2048 own keys): 64 sequences of
+// one token on a prefix of 32,768 keys 95 us, of up to five tokens 183 us; 16
+// on 4096 + 512 keys 24 us; four on 257 + 65 keys 14 us (two launches' latency).
 
 #include <cuda.h>
 #include <cuda_bf16.h>
@@ -112,6 +117,10 @@ constexpr int kShortPrefix = 6, kFewOwn = 6;
 // 1 / 2 / 4: 68 / 59 / 57 on 64 on 64 + 2048, 24 / 24 / 25 on 64 on 1024 + 64).
 constexpr int kStartTile = 4, kStartWarp = 2;
 
+namespace warpk {
+__host__ __device__ constexpr int workers(int split) { return split == 4 ? 2 : split == 2 ? 5 : 6; }  // per CTA (one per SM)
+}
+
 // What the host knows of the work.
 struct Plan {
   int group;        // G: query heads per KV head
@@ -119,11 +128,13 @@ struct Plan {
   int nt;           // row tiles of a tile-kernel CTA
   int split;        // warps of a warp-kernel worker
   bool prefix_warp, own_warp;  // which kernel has the list
+  int tile_cost;    // of a position of the tile kernel, in positions of the warp kernel
+  int share;        // SMs that the two kernels divide between them; 0: each has all
   Line tile, warp;
   float* part_o;    // [rows][D]
   float* part_lse;  // [rows]
   int* scan;        // [B + 1] positions before each sequence's own units, per unit
-  int* tokens;      // [B + 1] real query tokens before each sequence
+  int* tokens;      // [B + 1] real query tokens before each sequence, then the tile kernel's SMs
 };
 
 // The line with the rows that there are: the prefix's units have the real
@@ -143,6 +154,24 @@ __device__ __forceinline__ Line live_line(const AiPrefixAttnArgs& a, const Line&
 // has checked that they fit in an int).
 __device__ __forceinline__ int line_total(const Line& l, int own) {
   return l.units_prefix * (l.start + l.tiles_prefix) + own * l.per_seq;
+}
+
+// SMs of the tile kernel where the two run side by side: in proportion to what
+// the lines cost (own: positions per unit of the sequences' own lists).
+__device__ __forceinline__ int tile_sms(const AiPrefixAttnArgs& a, const Plan& p, int rows, int own) {
+  if (p.share == 0) return 0;
+  const int64_t tile = (int64_t)line_total(live_line(a, p.tile, rows), 0) * p.tile_cost, warp = line_total(p.warp, own);
+  if (warp == 0) return p.share;
+  const int64_t x = (p.share * tile + tile + warp - 1) / (tile + warp);
+  return (int)(x < 1 ? 1 : x > p.share - 1 ? p.share - 1 : x);
+}
+
+// The tile kernel's line (or the warp kernel's) with the rows and the workers
+// that there are, x SMs being the tile kernel's.
+__device__ __forceinline__ Line active_line(const AiPrefixAttnArgs& a, const Plan& p, bool tile, int rows, int x) {
+  Line l = live_line(a, tile ? p.tile : p.warp, rows);
+  if (p.share > 0) l.workers = min(l.workers, tile ? x : (p.share - x) * warpk::workers(p.split));
+  return l;
 }
 
 // The line's stretches: n workers have work, none less than `least` positions
@@ -345,9 +374,14 @@ __global__ void __launch_bounds__(tile_threads(NT), NT == 1 ? 2 : 1)
     ptx::tmem_relinquish();
   }
   if (warp == 0) {
-    scan_seqs(a, p.tile, BN, scan, tokens);
+    // (side by side with the warp kernel: that one's scan, this line has no own lists)
+    scan_seqs(a, p.share > 0 ? p.warp : p.tile, p.share > 0 ? kWarpKeys : BN, scan, tokens);
     __syncwarp();
-    if (lane == 0) *reinterpret_cast<Line*>(sm + L::LINE) = live_line(a, p.tile, tokens[a.batch] * p.group);
+    if (lane == 0) {
+      const int rows = tokens[a.batch] * p.group, x = tile_sms(a, p, rows, scan[a.batch]);
+      *reinterpret_cast<Line*>(sm + L::LINE) = active_line(a, p, true, rows, x);
+      if (blockIdx.x == 0) p.tokens[a.batch + 1] = x;
+    }
   }
   ptx::tc_fence_before();
   __syncthreads();
@@ -734,7 +768,6 @@ __device__ __forceinline__ void ldsm4_t(uint32_t (&r)[4], uint32_t addr) {
 // instructions, so loads and look-ups are kept out of it.
 namespace warpk {
 constexpr int kMaxThreads = 384;
-__host__ __device__ constexpr int workers(int split) { return split == 4 ? 2 : split == 2 ? 5 : 6; }  // per CTA (one per SM)
 template <int D>
 struct Ring {
   static constexpr uint32_t kHalf = kWarpKeys * 128;  // 64 dims of a tile's keys
@@ -775,6 +808,7 @@ __global__ void __launch_bounds__(warpk::kMaxThreads, 1)
       ptx::mbar_init(bars + 16u * i + 8, split);
     }
     *s_abort = 0;
+    s_abort[1] = p.share == 0 || blockIdx.x == 0;
     ptx::fence_mbar_init();
     ptx::prefetch_tmap(&tm_k);
     ptx::prefetch_tmap(&tm_v);
@@ -782,7 +816,7 @@ __global__ void __launch_bounds__(warpk::kMaxThreads, 1)
   if (warp == 0) {
     scan_seqs(a, p.warp, kWarpKeys, scan, tokens);
     __syncwarp();
-    if (lane == 0) *s_line = live_line(a, p.warp, tokens[a.batch] * p.group);
+    if (lane == 0) *s_line = active_line(a, p, false, tokens[a.batch] * p.group, tile_sms(a, p, tokens[a.batch] * p.group, scan[a.batch]));
   }
   __syncthreads();
   const int all_rows = tokens[a.batch] * p.group;
@@ -808,6 +842,12 @@ __global__ void __launch_bounds__(warpk::kMaxThreads, 1)
       ok = false;
     }
     return __all_sync(0xffffffffu, ok);
+  };
+
+  // The combine launch waits for this one, which must not end before the tile
+  // kernel (one CTA sees to that, the others make room).
+  auto finish = [&]() {
+    if (s_abort[1]) asm volatile("griddepcontrol.wait;" ::: "memory");
   };
 
   if (warp == n_warps) {
@@ -866,7 +906,7 @@ __global__ void __launch_bounds__(warpk::kMaxThreads, 1)
         const int turns = turn + (i < st);  // loads of stage i
         if (turns > 0) ptx::mbar_wait(full(i), (turns - 1) & 1, kWait);
       }
-    asm volatile("griddepcontrol.wait;" ::: "memory");
+    finish();
     return;
   }
 
@@ -1037,8 +1077,7 @@ __global__ void __launch_bounds__(warpk::kMaxThreads, 1)
       if (c == 0) p.part_lse[row] = part_lse(sum, m[h] + log2f(sum));
     }
   }
-  // The combine launch waits for this one; it must not end before the tile kernel's.
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+  finish();
 }
 
 // ---------------------------------------------------------------- combine
@@ -1062,11 +1101,11 @@ __global__ void __launch_bounds__(256) combine_kernel(const AiPrefixAttnArgs a, 
     // (without room for own keys neither kernel has written the scan)
     const bool own = a.max_pages > 0, pre = a.prefix_len > 0;
     const int s0 = own ? p.scan[b] : 0, size = own ? p.scan[b + 1] - s0 : 0, own_all = own ? p.scan[a.batch] : 0;
-    const int all_rows = pre ? p.tokens[a.batch] * p.group : 0;
+    const int all_rows = pre ? p.tokens[a.batch] * p.group : 0, sms = p.share > 0 ? p.tokens[a.batch + 1] : 0;
     int64_t row[2] = {0, 0}, step[2] = {0, 0};
     int n[2] = {0, 0};
     if (pre) {
-      const Line l = live_line(a, p.prefix_warp ? p.warp : p.tile, all_rows);
+      const Line l = active_line(a, p, !p.prefix_warp, all_rows, sms);
       const int all = p.tokens[b] * p.group + rem, grp = all / l.rows_prefix, unit = hk * l.groups + grp;
       const Split line = split_line(l, line_total(l, own_all));
       const int x = unit * (l.start + l.tiles_prefix) + l.start, first = line.worker(x);
@@ -1075,7 +1114,7 @@ __global__ void __launch_bounds__(256) combine_kernel(const AiPrefixAttnArgs a, 
       row[0] = l.base_prefix + (unit + first) * step[0] + all - grp * l.rows_prefix;
     }
     if (size > 0) {
-      const Line l = live_line(a, p.own_warp ? p.warp : p.tile, all_rows);
+      const Line l = active_line(a, p, !p.own_warp, all_rows, sms);
       const int grp = rem / l.rows_own, sub = grp * a.num_kv_heads + hk, unit = b * l.per_seq + sub;
       const Split line = split_line(l, line_total(l, own_all));
       const int x = l.units_prefix * (l.start + l.tiles_prefix) + s0 * l.per_seq + sub * size + l.start;
@@ -1203,6 +1242,18 @@ bool make_plan(const AiPrefixAttnArgs& a, Plan* p, size_t* bytes) {
             p->nt == 1 ? 2 * sms : sms, kStartTile, p->nt == 1 ? kStartTile + 1 : 1))
     return false;
   if (!line(p->warp, p->prefix_warp, p->own_warp, kWarpKeys, group_rows, H, rows, workers, kStartWarp, 2)) return false;
+  // A 256-row tile CTA fills its SM and leaves HBM idle; the warp kernel streams
+  // as fast from three quarters of the SMs as from all.  So they run side by
+  // side (one after the other / so, bf16, 64 sequences of one token: 110 / 95 us
+  // on 32,768 + 2048 keys, 38 / 32 on 2048 + 256; five tokens: 193 / 183 and
+  // 51 / 48 on 4096 + 5).  A tile position costs about 8 positions of the warp
+  // kernel, 11 with head_dim 64 (its CTA is bound by exponentials, theirs by
+  // bytes), fewer where a warp kernel position has several warps' rows (at 6 /
+  // 8 / 11: 109 / 96 / 100 us and 184 / 213 / 262 on the two largest above).
+  if (p->nt == 2 && p->tile.workers > 0 && p->tile.per_seq == 0 && p->warp.workers > 0) {
+    p->share = sms;
+    p->tile_cost = (a.head_dim == 128 ? 8 : 11) * (p->split == 1 ? 4 : 3) / 4;
+  }
   char* ws = static_cast<char*>(a.workspace);
   size_t off = 0;
   auto take = [&](size_t want) {
@@ -1213,7 +1264,7 @@ bool make_plan(const AiPrefixAttnArgs& a, Plan* p, size_t* bytes) {
   p->part_o = reinterpret_cast<float*>(take((size_t)at * a.head_dim * 4));
   p->part_lse = reinterpret_cast<float*>(take((size_t)at * 4));
   p->scan = reinterpret_cast<int*>(take(((size_t)a.batch + 1) * 4));
-  p->tokens = reinterpret_cast<int*>(take(((size_t)a.batch + 1) * 4));
+  p->tokens = reinterpret_cast<int*>(take(((size_t)a.batch + 2) * 4));
   *bytes = off;
   return true;
 }

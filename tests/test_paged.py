@@ -234,6 +234,22 @@ def test_attention_more(B, T, Hq, Hkv, D, S, P, lens, n, dtype, cuda_device):
     test_attention(B, T, Hq, Hkv, D, S, P, lens, n, dtype, cuda_device)
 
 
+SIDE = [
+    # as ATTEND: more than 128 rows on the prefix, own lists from none to far more work than the prefix
+    (40, 1, 8, 1, 128, 64, 700, [0] * 40, None, torch.bfloat16),
+    (40, 1, 8, 1, 128, 64, 5000, [0] * 39 + [700], None, torch.float16),
+    (33, 2, 16, 2, 64, 16, 2900, [2 + 61 * (i % 5) for i in range(33)], [i % 3 for i in range(33)], torch.bfloat16),
+    (24, 5, 32, 4, 128, 128, 2500, [5 + 37 * i for i in range(24)], [5 - i % 4 for i in range(24)], torch.bfloat16),
+    (20, 1, 16, 1, 64, 64, 9000, [100] * 20, [0] * 20, torch.bfloat16),  # no query at all
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("B,T,Hq,Hkv,D,S,P,lens,n,dtype", SIDE)
+def test_attention_side_by_side(B, T, Hq, Hkv, D, S, P, lens, n, dtype, cuda_device):
+    test_attention(B, T, Hq, Hkv, D, S, P, lens, n, dtype, cuda_device)
+
+
 @pytest.mark.gpu
 def test_attention_negative_scale(cuda_device):
     from autoindexer_b200 import shared_prefix_attention
