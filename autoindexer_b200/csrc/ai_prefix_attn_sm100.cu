@@ -21,6 +21,9 @@
 //                 tile kernel pays a chain of TMA, MMA and TMEM latencies per
 //                 unit (4.8 us per unit of one 64-key tile).  Own lists of 64
 //                 sequences of up to 2048 keys: 48 us, 5.6 TB/s.
+// P is rounded to the values' type for its product (the MMAs take one type), the
+// sums take it unrounded: about the error of the output's own rounding (1.3 to
+// 1.4 times a single-rounded result's; none for up to 8 rows a warp).
 // The second is launched by programmatic dependent launch: it fills the SMs the
 // first leaves, or takes its share of them from the start (make_plan).
 //
@@ -313,6 +316,7 @@ template <> struct Pair<__nv_bfloat16> {
     const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&h);
   }
+  __device__ static float2 unpack(uint32_t p) { return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&p)); }
 };
 template <> struct Pair<__half> {
   static constexpr uint32_t kFmt = 0;
@@ -320,6 +324,7 @@ template <> struct Pair<__half> {
     const __half2 h = __floats2half2_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&h);
   }
+  __device__ static float2 unpack(uint32_t p) { return __half22float2(*reinterpret_cast<const __half2*>(&p)); }
 };
 
 // kind::f16 instruction descriptor with fp32 accumulation (fields as in sm100_ptx.cuh).
@@ -1014,6 +1019,11 @@ __global__ void __launch_bounds__(warpk::kMaxThreads, 1)
           }
           base[h] = m[h] == -CUDART_INF_F ? 0.f : m[h];
         }
+        // Without a query among rows 8 to 15 these take what rounding P leaves of
+        // rows 0 to 7, so the output is rounded once, at no cost (a second MMA
+        // for it took 3 % to 6 % where rows 8 to 15 are in use).
+        const bool few = !__any_sync(0xffffffffu, seen[1] >= 0);
+        if (few) alpha[1] = alpha[0];
         if (__any_sync(0xffffffffu, rescale)) {
           l[0] *= alpha[0], l[1] *= alpha[1];
 #pragma unroll
@@ -1022,16 +1032,23 @@ __global__ void __launch_bounds__(warpk::kMaxThreads, 1)
             o[i][2] *= alpha[1], o[i][3] *= alpha[1];
           }
         }
-        uint32_t pa[2][4];  // P's fragments of keys 0..15 and 16..31
+        // P's fragments of keys 0..15 and 16..31, rounded to the values' type.
+        uint32_t pa[2][4];
 #pragma unroll
-        for (int nt = 0; nt < 4; ++nt)
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const float p0 = ptx::ex2(fmaf(sc[nt][2 * h], sl2, -base[h]));
-            const float p1 = ptx::ex2(fmaf(sc[nt][2 * h + 1], sl2, -base[h]));
-            l[h] += p0 + p1;
-            pa[nt >> 1][(nt & 1) * 2 + h] = Pair<T>::pack(p0, p1);
+        for (int nt = 0; nt < 4; ++nt) {
+          uint32_t* frag = &pa[nt >> 1][(nt & 1) * 2];
+          float p0 = ptx::ex2(fmaf(sc[nt][0], sl2, -base[0])), p1 = ptx::ex2(fmaf(sc[nt][1], sl2, -base[0]));
+          l[0] += p0 + p1;
+          frag[0] = Pair<T>::pack(p0, p1);
+          if (few) {
+            const float2 rounded = Pair<T>::unpack(frag[0]);
+            p0 -= rounded.x, p1 -= rounded.y;
+          } else {
+            p0 = ptx::ex2(fmaf(sc[nt][2], sl2, -base[1])), p1 = ptx::ex2(fmaf(sc[nt][3], sl2, -base[1]));
+            l[1] += p0 + p1;
           }
+          frag[1] = Pair<T>::pack(p0, p1);
+        }
         const bool ragged = k0 + kWarpKeys > s.keys;
 #pragma unroll
         for (int kk = 0; kk < 2; ++kk) {
@@ -1060,6 +1077,10 @@ __global__ void __launch_bounds__(warpk::kMaxThreads, 1)
       if (++st == stages) st = 0, turn ^= 1;
     }
     if (!ok) break;
+    if (!__any_sync(0xffffffffu, seen[1] >= 0)) {
+#pragma unroll
+      for (int i = 0; i < NB; ++i) o[i][0] += o[i][2], o[i][1] += o[i][3];
+    }
     // Partial rows: the lane's dims 8 i + 2 c + {0, 1} of rows r and r + 8.
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
