@@ -1107,7 +1107,6 @@ __global__ void __launch_bounds__(warpk::kMaxThreads, 1)
 // them, and the first adds up the warps' sums in order.
 template <typename T, int D>
 __global__ void __launch_bounds__(256) combine_kernel(const AiPrefixAttnArgs a, const Plan p, const int wide) {
-  asm volatile("griddepcontrol.wait;" ::: "memory");
   constexpr int E = D / 32;
   __shared__ float s_acc[8][D + 2];
   const int b = blockIdx.y, lane = threadIdx.x % 32, warp = threadIdx.x / 32, part = warp % wide;
@@ -1115,10 +1114,12 @@ __global__ void __launch_bounds__(256) combine_kernel(const AiPrefixAttnArgs a, 
   const bool has = item < a.seq_len * a.num_q_heads;
   const int t = has ? item / a.num_q_heads : 0, h = has ? item % a.num_q_heads : 0, hk = h / p.group;
   const int rem = t * p.group + h % p.group;
+  const bool real = has && t < seq_lens(a, b).n;  // (the caller's lengths: read before the wait)
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   float M = -CUDART_INF_F, sum = 0.f, acc[E];
 #pragma unroll
   for (int e = 0; e < E; ++e) acc[e] = 0.f;
-  if (has && t < seq_lens(a, b).n) {
+  if (real) {
     // (without room for own keys neither kernel has written the scan)
     const bool own = a.max_pages > 0, pre = a.prefix_len > 0;
     const int s0 = own ? p.scan[b] : 0, size = own ? p.scan[b + 1] - s0 : 0, own_all = own ? p.scan[a.batch] : 0;
