@@ -442,7 +442,8 @@ __global__ void __launch_bounds__(tile_threads(NT), NT == 1 ? 2 : 1)
     auto load_rows = [&](const Seg& s) {
       constexpr int kLanes = D / 8, kPer = 32 / kLanes, kFly = 8;  // lanes a row, rows a load, loads in flight
       const bool pre = s.b < 0;
-      const int per = pre ? ln.rows_prefix : ln.rows_own, half = (per + NT - 1) / NT, hk = head(s);
+      // (a row tile's rows in whole warps: a warp without rows does nothing)
+      const int per = pre ? ln.rows_prefix : ln.rows_own, half = NT == 1 ? per : (per + 63) / 64 * 32, hk = head(s);
       const int row0 = (pre ? s.sub % ln.groups : s.sub / a.num_kv_heads) * per + wg * half;
       const int n_rows = min(min(half, per - wg * half), (pre ? all_rows : p.rows_seq) - row0);
       int seen = -1;

@@ -251,6 +251,13 @@ def test_attention_side_by_side(B, T, Hq, Hkv, D, S, P, lens, n, dtype, cuda_dev
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("rows", [129, 161, 191, 193, 255, 257])
+def test_attention_row_counts(rows, cuda_device):
+    """Numbers of rows on one prefix that no tile, warp or half of one divides."""
+    test_attention(rows, 1, 2, 2, 64, 32, 700, [1 + i % 70 for i in range(rows)], None, torch.bfloat16, cuda_device)
+
+
+@pytest.mark.gpu
 def test_attention_negative_scale(cuda_device):
     from autoindexer_b200 import shared_prefix_attention
 
