@@ -28,8 +28,8 @@
 // first leaves, or takes its share of them from the start (make_plan).
 //
 // Measured (bf16, 32 + 8 heads, D 128, up to 2048 own keys): 64 sequences of
-// one token on a prefix of 32,768 keys 95 us, of up to five tokens 183 us; 16
-// on 4096 + 512 keys 24 us; four on 257 + 65 keys 14 us (two launches' latency).
+// one token on a prefix of 32,768 keys 95 us, of up to five tokens 183 us (217
+// at the power limit); 16 on 4096 + 512 keys 23 us; four on 257 + 65 keys 14 us (two launches' latency).
 
 #include <cuda.h>
 #include <cuda_bf16.h>
