@@ -108,6 +108,15 @@ def floats(name: str, x: Tensor, shape: Tuple[int, ...], index: int) -> Tensor:
     return x.contiguous()
 
 
+def dense_positions(positions: Tensor) -> Tensor:
+    return positions if positions.stride(-1) == 1 else positions.contiguous()
+
+
+def positions_stride(positions: Tensor) -> int:
+    """Elements from a batch row's ids to the next one's; 0: one row for all."""
+    return positions.stride(0) if positions.dim() == 2 and positions.shape[0] > 1 else 0
+
+
 def check_rope(a, rope, positions: Optional[Tensor], batch: int, seq_len: int, head_dim: int, index: int):
     """Sets what ``a`` says of the rotary table and the position ids; returns
     (cos, sin, positions) as the kernels read them, whose pointers
@@ -132,10 +141,9 @@ def check_rope(a, rope, positions: Optional[Tensor], batch: int, seq_len: int, h
     if len(dims) > 2 or rows not in (1, batch) or dims[-1] != seq_len:
         raise ValueError(f"positions must be ({seq_len},) or ({batch}, {seq_len}), got {tuple(dims)}")
     on_device("positions", positions, index)
-    if positions.stride(-1) != 1:
-        positions = positions.contiguous()
+    positions = dense_positions(positions)
     a.n_pos = n
-    a.pos = _lib.AiPositions(None, positions.stride(0) if rows > 1 else 0, is_int64)
+    a.pos = _lib.AiPositions(None, positions_stride(positions), is_int64)
     return cos, sin, positions
 
 

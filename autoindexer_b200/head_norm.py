@@ -104,27 +104,35 @@ class HeadNormFn(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dq_out, dk_out):
-        tensors = q, k, wq, wk, _, _, _ = ctx.saved_tensors
+        q, k, wq, wk, cos, sin, positions = ctx.saved_tensors
         g = _lib.AiHeadNormBwdArgs()
         g.fwd = ctx.plan
-        # (saved tensors may have been moved and brought back)
+        # (hooks on saved tensors may have moved them and brought back copies of
+        # other strides: all that the struct says of a layout is taken anew)
+        q = _call.dense_d(q)
         g.fwd.q = _call.t4(q)
         dq_out = _call.dense_d(dq_out)
         dq = torch.empty_like(q)
         g.dq_out, g.dq = _call.t4(dq_out), _call.t4(dq)
         dk = dwq = dwk = None
         if k is not None:
+            k = _call.dense_d(k)
             g.fwd.k = _call.t4(k)
             dk_out = _call.dense_d(dk_out)
             dk = torch.empty_like(k)
             g.dk_out, g.dk = _call.t4(dk_out), _call.t4(dk)
         if wq is not None:
+            wq = wq.contiguous()
             dwq = torch.empty_like(wq)
             g.dq_weight = dwq.data_ptr()
         if wk is not None:
+            wk = wk.contiguous()
             dwk = torch.empty_like(wk)
             g.dk_weight = dwk.data_ptr()
-        _point(g.fwd, *tensors)
+        if cos is not None:
+            cos, sin, positions = cos.contiguous(), sin.contiguous(), _call.dense_positions(positions)
+            g.fwd.pos.stride_b = _call.positions_stride(positions)
+        _point(g.fwd, q, k, wq, wk, cos, sin, positions)
         lib = _lib.lib()
         ws = _call.workspace(lib.ai_head_norm_bwd_workspace, g, q.device, "ai_head_norm_bwd_workspace")
         _call.launch(lib.ai_head_norm_bwd, g, q.get_device(), "ai_head_norm_bwd")
