@@ -9,8 +9,8 @@
 // alone 35 us, 5.0 TB/s); 16 of seven, fp32, no draft logits: 22.5 us; one of
 // three: 8.4 us, two launches' latency.  Two launches, the second started by programmatic
 // dependent launch:
-//   stats  a CTA per (row, vocabulary slice): the sum of 2^(c x - o),
-//          c = log2(e) / tau and o = c max, four 16-byte loads per
+//   stats  a CTA per (row, vocabulary slice): the largest logit m and the
+//          sum of 2^((x - m) c), c = log2(e) / tau, four 16-byte loads per
 //          thread in flight from the row's first 16-byte boundary (the ragged
 //          ends one by one); in greedy rows the maximum's lowest index
 //          instead of the sum;
@@ -24,6 +24,7 @@
 #include <cuda_runtime.h>
 #include <math_constants.h>
 
+#include <cfloat>
 #include <cstring>
 
 #include "ai_common.cuh"
@@ -41,12 +42,13 @@ constexpr int kMaxDraft = 64;
 // 8192 / 16384, race 8.4 / 8.4 / 9.7 with 1024 / 2048 / 8192.
 constexpr int kLeastStats = 8192, kLeastPick = 2048;
 
-// The exponent of a logit is fma(x, c, -o), rounded once, with o the rounded
-// c max: every pass over a row uses the same o, so its own rounding is a
-// common factor of p's numerator and sum.
+// The exponent of a logit is (x - m) c: the difference first, so that the
+// largest logit's weight is 1 at every temperature.  (As x c - m c the rounding
+// of m c is a factor of every weight, which leaves fp32's range once c m passes
+// 2^31: temperatures below 1e-7.)
 struct Stat {
-  float o;  // c times the largest logit (greedy rows: the logit); -inf for an empty or fully masked slice
-  float s;  // sum of 2^(c x - o)
+  float m;  // the largest logit; -inf for an empty or fully masked slice
+  float s;  // sum of 2^((x - m) c)
   int at;   // greedy rows: lowest index of the largest logit
 };
 
@@ -109,33 +111,34 @@ template <> struct Vec<__half> {
   }
 };
 
-// Slope c of a row's exponent; 0 for a greedy row.
-__device__ __forceinline__ float slope(float tau) { return tau > 0.f ? kLog2e / tau : 0.f; }
-
-// 2^(c x - o), 0 for a masked logit (o may be -inf then).
-__device__ __forceinline__ float weight(float x, float c, float o) {
-  return x == -CUDART_INF_F ? 0.f : ptx::ex2(fmaf(x, c, -o));
+// Slope c of a row's exponent (1 for a greedy row, which has no use for it),
+// finite and above zero: a logit at the maximum keeps the exponent 0 and a
+// masked one -inf at any temperature, subnormal or infinite ones included.
+__device__ __forceinline__ float slope(float tau) {
+  return tau > 0.f ? fminf(fmaxf(kLog2e / tau, FLT_MIN), FLT_MAX) : 1.f;
 }
 
-// 2^(a - o), 0 for a = -inf.
-__device__ __forceinline__ float shift(float a, float o) { return a == -CUDART_INF_F ? 0.f : ptx::ex2(a - o); }
+// 2^((x - m) c), 0 for a masked logit (m may be -inf then).
+__device__ __forceinline__ float weight(float x, float c, float m) {
+  return x == -CUDART_INF_F ? 0.f : ptx::ex2((x - m) * c);
+}
 
-__device__ __forceinline__ Stat merge(const Stat& a, const Stat& b) {
+__device__ __forceinline__ Stat merge(const Stat& a, const Stat& b, float c) {
   Stat r;
-  r.o = fmaxf(a.o, b.o);
-  r.at = a.o > b.o ? a.at : b.o > a.o ? b.at : min(a.at, b.at);
-  r.s = a.s * shift(a.o, r.o) + b.s * shift(b.o, r.o);
+  r.m = fmaxf(a.m, b.m);
+  r.at = a.m > b.m ? a.at : b.m > a.m ? b.at : min(a.at, b.at);
+  r.s = a.s * weight(a.m, c, r.m) + b.s * weight(b.m, c, r.m);
   return r;
 }
 
-__device__ __forceinline__ Stat merge_lanes(Stat st) {
+__device__ __forceinline__ Stat merge_lanes(Stat st, float c) {
 #pragma unroll
   for (int d = 16; d > 0; d >>= 1) {
     Stat t;
-    t.o = __shfl_xor_sync(0xffffffffu, st.o, d);
+    t.m = __shfl_xor_sync(0xffffffffu, st.m, d);
     t.s = __shfl_xor_sync(0xffffffffu, st.s, d);
     t.at = __shfl_xor_sync(0xffffffffu, st.at, d);
-    st = merge(st, t);
+    st = merge(st, t, c);
   }
   return st;
 }
@@ -186,10 +189,7 @@ __global__ void __launch_bounds__(kThreads, 4) stats_kernel(const AiVerifyArgs a
   Stat st{-CUDART_INF_F, 0.f, 0x7fffffff};
   auto one = [&](int v) {
     const float f = at(x, v);
-    Stat t{greedy ? f : f * c, 1.f, v};
-    if (f == -CUDART_INF_F) t.o = f, t.s = 0.f;
-    if (!greedy) t.s = weight(f, c, t.o);
-    st = merge(st, t);
+    st = merge(st, Stat{f, f == -CUDART_INF_F ? 0.f : 1.f, v}, c);
   };
   if (split == 0 && tid < head) one(tid);
   const uint4* xv = reinterpret_cast<const uint4*>(x + head);
@@ -223,8 +223,8 @@ __global__ void __launch_bounds__(kThreads, 4) stats_kernel(const AiVerifyArgs a
     }
     const float m = Vec<T>::top(big);
     if (greedy) {
-      if (m > st.o || st.at == 0x7fffffff) {
-        st.o = m;
+      if (m > st.m || st.at == 0x7fffffff) {
+        st.m = m;
         bool found = false;
 #pragma unroll
         for (int u = 0; u < U; ++u) {
@@ -239,8 +239,8 @@ __global__ void __launch_bounds__(kThreads, 4) stats_kernel(const AiVerifyArgs a
         }
       }
     } else {
-      // (c > 0; without a finite logit o stays -inf and nothing is added)
-      const float top = m == -CUDART_INF_F ? st.o : fmaxf(st.o, m * c), o = top == -CUDART_INF_F ? 0.f : top;
+      // (without a finite logit the maximum stays -inf and nothing is added)
+      const float top = fmaxf(st.m, m), o = top == -CUDART_INF_F ? 0.f : top;
       const float2 no = make_float2(-o, -o), cc = make_float2(c, c);
       float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
@@ -249,21 +249,21 @@ __global__ void __launch_bounds__(kThreads, 4) stats_kernel(const AiVerifyArgs a
         Vec<T>::get(raw[u], f);
 #pragma unroll
         for (int k = 0; k < E / 2; ++k) {
-          const float2 z = __ffma2_rn(f[k], cc, no);
+          const float2 z = __fmul2_rn(__fadd2_rn(f[k], no), cc);
           sum = __fadd2_rn(sum, make_float2(ptx::ex2(z.x), ptx::ex2(z.y)));
         }
       }
-      st.s = st.s * shift(st.o, top) + (sum.x + sum.y);
-      st.o = top;
+      st.s = st.s * weight(st.m, c, top) + (sum.x + sum.y);
+      st.m = top;
     }
   }
   if (split == w.splits - 1 && tail + tid < a.vocab) one(tail + tid);  // (fewer than E)
-  st = merge_lanes(st);
+  st = merge_lanes(st, c);
   __shared__ Stat sm[kWarps];
   if (lane == 0) sm[warp] = st;
   __syncthreads();
   if (tid == 0) {
-    for (int k = 1; k < kWarps; ++k) st = merge(st, sm[k]);
+    for (int k = 1; k < kWarps; ++k) st = merge(st, sm[k], c);
     w.stat[(int64_t)blockIdx.y * w.splits + split] = st;
   }
 }
@@ -279,12 +279,12 @@ struct Race {
   const T* xp;
   const T* xq;      // nullptr: no draft distribution
   const float* e;   // noise
-  float op, ip, oq, iq, c;  // offsets and reciprocal sums
+  float mp, ip, mq, iq, c;  // largest logits and reciprocal sums
   int drop;         // word that has no residual (drafted with certainty and refused), or -1
 
-  // (finite offsets: a masked logit's weight is 2^-inf = 0)
-  __device__ __forceinline__ float p(float x) const { return ptx::ex2(fmaf(x, c, -op)) * ip; }
-  __device__ __forceinline__ float q(float x) const { return ptx::ex2(fmaf(x, c, -oq)) * iq; }
+  // (finite mp, mq: a masked logit's weight is 2^-inf = 0)
+  __device__ __forceinline__ float p(float x) const { return ptx::ex2((x - mp) * c) * ip; }
+  __device__ __forceinline__ float q(float x) const { return ptx::ex2((x - mq) * c) * iq; }
 };
 
 // The thread's best of words [v0, v1): its index is the lowest of equal
@@ -387,8 +387,8 @@ __global__ void __launch_bounds__(kThreads) pick_kernel(const AiVerifyArgs a, co
     if (!needed(a, r, n)) continue;
     const Stat* p = w.stat + ((int64_t)b * rows + r) * w.splits;
     Stat s{-CUDART_INF_F, 0.f, 0x7fffffff};
-    for (int k = lane; k < w.splits; k += 32) s = merge(s, p[k]);
-    s = merge_lanes(s);
+    for (int k = lane; k < w.splits; k += 32) s = merge(s, p[k], c);
+    s = merge_lanes(s, c);
     if (lane == 0) st[r] = s;
   }
   __syncthreads();
@@ -398,11 +398,11 @@ __global__ void __launch_bounds__(kThreads) pick_kernel(const AiVerifyArgs a, co
       ok = tok == st[tid].at;
     } else if (tok >= 0) {
       const Stat& sp = st[tid];
-      const float p = sp.s > 0.f ? weight(x_p, c, sp.o) / sp.s : 0.f;
+      const float p = sp.s > 0.f ? weight(x_p, c, sp.m) / sp.s : 0.f;
       float q = 1.f;
       if (a.draft) {
         const Stat& sq = st[a.n_draft + 1 + tid];
-        q = sq.s > 0.f ? weight(x_q, c, sq.o) / sq.s : 0.f;
+        q = sq.s > 0.f ? weight(x_q, c, sq.m) / sq.s : 0.f;
       }
       ok = u * q < p;
     }
@@ -419,12 +419,12 @@ __global__ void __launch_bounds__(kThreads) pick_kernel(const AiVerifyArgs a, co
     d.xq = stop < n && a.draft ? row_ptr<T>(a, b, a.n_draft + 1 + stop) : nullptr;
     d.e = a.noise + (int64_t)b * a.vocab;
     d.c = c;
-    d.op = sp.o == -CUDART_INF_F ? 0.f : sp.o;
+    d.mp = sp.m == -CUDART_INF_F ? 0.f : sp.m;
     d.ip = sp.s > 0.f ? 1.f / sp.s : 0.f;
     d.drop = -1;
     if (d.xq) {
       const Stat sq = st[a.n_draft + 1 + stop];
-      d.oq = sq.o == -CUDART_INF_F ? 0.f : sq.o;
+      d.mq = sq.m == -CUDART_INF_F ? 0.f : sq.m;
       d.iq = sq.s > 0.f ? 1.f / sq.s : 0.f;
     } else if (stop < n) {
       const long long refused = a.tokens[(int64_t)b * a.n_draft + stop];
@@ -472,7 +472,7 @@ __global__ void __launch_bounds__(kThreads) pick_kernel(const AiVerifyArgs a, co
     float lp = 0.f;
     if (i <= stop) {
       word = i < stop ? a.tokens[(int64_t)b * a.n_draft + i] : s_next;
-      if (tau > 0.f) lp = (fmaf(at(row_ptr<T>(a, b, i), word), c, -st[i].o) - log2f(st[i].s)) * kLn2;
+      if (tau > 0.f) lp = ((at(row_ptr<T>(a, b, i), word) - st[i].m) * c - log2f(st[i].s)) * kLn2;
     }
     a.out_tokens[o] = word;
     a.logprobs[o] = lp;

@@ -73,7 +73,7 @@ def verify_draft(target_logits: Tensor, draft_tokens: Tensor, uniforms: Tensor, 
     ``draft_logits`` ``(B, L, V)`` the logits they were sampled from (``None``:
     proposed with certainty, as by a lookup); ``draft_lens`` ``(B,)`` int32 how
     many are real; ``temperature`` ``(B,)`` float32 divides both (``None``: 1;
-    0 decodes greedily).  ``uniforms`` ``(B, L)`` float32 in ``[0, 1)`` decide
+    0 decodes greedily; any positive value, however small, is a temperature).  ``uniforms`` ``(B, L)`` float32 in ``[0, 1)`` decide
     acceptance: ``u * q(x) < p(x)``; ``noise`` ``(B, V)`` float32 exponential
     variates (> 0) choose the next token: the largest ``r / noise`` with ``r``
     the residual ``max(p - q, 0)`` after a refusal, else ``p``; equal values
