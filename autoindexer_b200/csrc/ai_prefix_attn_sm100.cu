@@ -968,6 +968,11 @@ __global__ void __launch_bounds__(warpk::kMaxThreads, 1)
 #pragma unroll
       for (int e = 0; e < 4; ++e) o[i][e] = 0.f;
     float m[2] = {-CUDART_INF_F, -CUDART_INF_F}, l[2] = {0.f, 0.f};
+    // l takes the exponentials of one turn of the ring, l_before the turns'
+    // sums: one running sum of a long list would round away its small weights
+    // beside a large one (the fp32 sum's error then goes by keys / (32 stages)
+    // additions, not by keys / 8).
+    float l_before[2] = {0.f, 0.f};
 
     for (int j = s.j0; j < s.j0 + s.n; ++j) {
       const int k0 = j * kWarpKeys;
@@ -1027,6 +1032,7 @@ __global__ void __launch_bounds__(warpk::kMaxThreads, 1)
         if (few) alpha[1] = alpha[0];
         if (__any_sync(0xffffffffu, rescale)) {
           l[0] *= alpha[0], l[1] *= alpha[1];
+          l_before[0] *= alpha[0], l_before[1] *= alpha[1];
 #pragma unroll
           for (int i = 0; i < NB; ++i) {
             o[i][0] *= alpha[0], o[i][1] *= alpha[0];
@@ -1075,7 +1081,11 @@ __global__ void __launch_bounds__(warpk::kMaxThreads, 1)
       }
       __syncwarp();
       if (lane == 0) ptx::mbar_arrive(empty(st));
-      if (++st == stages) st = 0, turn ^= 1;
+      if (++st == stages) {
+        st = 0, turn ^= 1;
+        l_before[0] += l[0], l_before[1] += l[1];
+        l[0] = l[1] = 0.f;
+      }
     }
     if (!ok) break;
     if (!__any_sync(0xffffffffu, seen[1] >= 0)) {
@@ -1085,7 +1095,7 @@ __global__ void __launch_bounds__(warpk::kMaxThreads, 1)
     // Partial rows: the lane's dims 8 i + 2 c + {0, 1} of rows r and r + 8.
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      float sum = l[h];
+      float sum = l_before[h] + l[h];
       sum += __shfl_xor_sync(0xffffffffu, sum, 1);
       sum += __shfl_xor_sync(0xffffffffu, sum, 2);
       if (seen[h] < 0) continue;
