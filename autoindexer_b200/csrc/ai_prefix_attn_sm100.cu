@@ -773,7 +773,10 @@ __device__ __forceinline__ void ldsm4_t(uint32_t (&r)[4], uint32_t addr) {
 // With a few warps per scheduler the step is bound by its own chain of
 // instructions, so loads and look-ups are kept out of it.
 namespace warpk {
-constexpr int kMaxThreads = 384;
+// The largest CTA, five workers of two warps and the loading one.  (Two registers
+// more for the sums than before; at 384 the fp16 kernel spilled: 61 us for 58 on own
+// lists of 64 sequences of up to 2048 keys.)
+constexpr int kMaxThreads = 352;
 template <int D>
 struct Ring {
   static constexpr uint32_t kHalf = kWarpKeys * 128;  // 64 dims of a tile's keys
