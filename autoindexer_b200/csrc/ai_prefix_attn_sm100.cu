@@ -23,7 +23,11 @@
 //                 sequences of up to 2048 keys: 48 us, 5.6 TB/s.
 // P is rounded to the values' type for its product (the MMAs take one type), the
 // sums take it unrounded: about the error of the output's own rounding (1.3 to
-// 1.4 times a single-rounded result's; none for up to 8 rows a warp).
+// 1.4 times a single-rounded result's in either type; none for up to 8 rows a
+// warp).  fp16 holds small weights to 2^-32 of the largest (see Pair), bf16 to
+// its 8 bits at any size.  The MMAs cut a product 25 bits below its accumulator,
+// so n weights of under 2^-25 of what a stretch has gathered may add n 2^-25 to
+// the relative error, in either type.
 // The second is launched by programmatic dependent launch: it fills the SMs the
 // first leaves, or takes its share of them from the start (make_plan).
 //
@@ -309,9 +313,15 @@ __device__ __forceinline__ int visible(const AiPrefixAttnArgs& a, const Row& r, 
   return prefix ? keys : max(0, keys - len.n + r.t + 1);
 }
 
+// Two values of a type.  top: a maximum as the softmax takes it, for fp16 lower
+// by 7, so that P = 2^(s - m) and the sums are 2^7 times the weights (m plus the
+// sum's logarithm stays what it is).  The lazy maximum lets P reach 2^8; fp16
+// has room for 2^15, and each bit used above is one kept below, where weights
+// under 2^-25 of the maximum were lost and those under 2^-14 lost bits.
 template <typename T> struct Pair;
 template <> struct Pair<__nv_bfloat16> {
   static constexpr uint32_t kFmt = 1;
+  __device__ static float top(float score, float sl2) { return score * sl2; }
   __device__ static uint32_t pack(float lo, float hi) {
     const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&h);
@@ -320,6 +330,7 @@ template <> struct Pair<__nv_bfloat16> {
 };
 template <> struct Pair<__half> {
   static constexpr uint32_t kFmt = 0;
+  __device__ static float top(float score, float sl2) { return fmaf(score, sl2, -7.f); }
   __device__ static uint32_t pack(float lo, float hi) {
     const __half2 h = __floats2half2_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&h);
@@ -530,7 +541,7 @@ __global__ void __launch_bounds__(tile_threads(NT), NT == 1 ? 2 : 1)
               mx[c] = ptx::fmax3(mx[c], __uint_as_float(sc[c][i]), __uint_as_float(sc[c][i + 1]));
 #pragma unroll
           for (int c = 1; c < BN / 32; ++c) mx[0] = fmaxf(mx[0], mx[c]);
-          const float m_new = fmaxf(m, mx[0] * sl2);
+          const float m_new = fmaxf(m, Pair<T>::top(mx[0], sl2));
           float alpha = 1.f;
           bool rescale = false;
           if (m_new > m + 8.f) {
@@ -1017,7 +1028,7 @@ __global__ void __launch_bounds__(warpk::kMaxThreads, 1)
 #pragma unroll
           for (int nt = 1; nt < 4; ++nt) mx = ptx::fmax3(mx, sc[nt][2 * h], sc[nt][2 * h + 1]);
           mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2)) * sl2;
+          mx = Pair<T>::top(fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2)), sl2);
           // (O is rescaled only when the maximum grows by more than 2^8)
           if (mx > m[h] + 8.f) {
             if (m[h] != -CUDART_INF_F) {
