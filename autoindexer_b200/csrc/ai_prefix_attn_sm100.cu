@@ -317,11 +317,15 @@ __device__ __forceinline__ int visible(const AiPrefixAttnArgs& a, const Row& r, 
 // by 7, so that P = 2^(s - m) and the sums are 2^7 times the weights (m plus the
 // sum's logarithm stays what it is).  The lazy maximum lets P reach 2^8; fp16
 // has room for 2^15, and each bit used above is one kept below, where weights
-// under 2^-25 of the maximum were lost and those under 2^-14 lost bits.
+// under 2^-25 of the maximum were lost and those under 2^-14 lost bits.  limit:
+// the maximum moves when a score's top passes it.  In fp16 the one is rounded up
+// and the other down, so that P stays at 2^15 however large the scores are (a
+// maximum of 2^26 is a multiple of 8).
 template <typename T> struct Pair;
 template <> struct Pair<__nv_bfloat16> {
   static constexpr uint32_t kFmt = 1;
   __device__ static float top(float score, float sl2) { return score * sl2; }
+  __device__ static float limit(float m) { return m + 8.f; }
   __device__ static uint32_t pack(float lo, float hi) {
     const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&h);
@@ -330,7 +334,8 @@ template <> struct Pair<__nv_bfloat16> {
 };
 template <> struct Pair<__half> {
   static constexpr uint32_t kFmt = 0;
-  __device__ static float top(float score, float sl2) { return fmaf(score, sl2, -7.f); }
+  __device__ static float top(float score, float sl2) { return __fmaf_ru(score, sl2, -7.f); }
+  __device__ static float limit(float m) { return __fadd_rd(m, 8.f); }
   __device__ static uint32_t pack(float lo, float hi) {
     const __half2 h = __floats2half2_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&h);
@@ -544,7 +549,7 @@ __global__ void __launch_bounds__(tile_threads(NT), NT == 1 ? 2 : 1)
           const float m_new = fmaxf(m, Pair<T>::top(mx[0], sl2));
           float alpha = 1.f;
           bool rescale = false;
-          if (m_new > m + 8.f) {
+          if (m_new > Pair<T>::limit(m)) {
             if (l > 0.f) {
               alpha = ptx::ex2(m - m_new);
               rescale = true;
@@ -1030,7 +1035,7 @@ __global__ void __launch_bounds__(warpk::kMaxThreads, 1)
           mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
           mx = Pair<T>::top(fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2)), sl2);
           // (O is rescaled only when the maximum grows by more than 2^8)
-          if (mx > m[h] + 8.f) {
+          if (mx > Pair<T>::limit(m[h])) {
             if (m[h] != -CUDART_INF_F) {
               alpha[h] = ptx::ex2(m[h] - mx);
               rescale = true;
