@@ -13,6 +13,7 @@ from typing import Optional, Tuple
 
 import torch
 from torch import Tensor
+from torch.autograd import forward_ad
 
 from . import _lib
 from .attention import status_word
@@ -55,6 +56,19 @@ class Plans(dict):
 def copy(args):
     """A struct of one call's own."""
     return type(args).from_buffer_copy(args)
+
+
+def tracked(*tensors: Optional[Tensor]) -> bool:
+    """Whether autograd may want something of a call: an input that requires a
+    gradient with the gradients on, or any call within a forward-mode level
+    (its tensors may carry tangents whatever they require)."""
+    if forward_ad._current_level >= 0:
+        return True
+    if torch.is_grad_enabled():
+        for x in tensors:
+            if x is not None and x.requires_grad:
+                return True
+    return False
 
 
 def dtype_code(x: Tensor, name: str) -> int:

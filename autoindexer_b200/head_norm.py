@@ -154,7 +154,8 @@ def qk_norm_rope(query: Tensor, key: Optional[Tensor], q_weight: Optional[Tensor
     and sets the status word that ``read_status`` reads); without them nothing is
     rotated.  CUDA tensors, bfloat16, float16 or float32, head_dim 32, 64 or
     128, any strides with the last dimension contiguous.  Arithmetic is
-    float32, rounded once.  Differentiable in query, key and the weights."""
+    float32, rounded once.  Differentiable in query, key and the weights (in
+    reverse mode; inputs with forward-mode tangents raise)."""
     cos, sin = (None, None) if rope is None else rope
     tensors = (query, key, q_weight, k_weight, cos, sin, positions)
     eps = float(eps)
@@ -164,8 +165,6 @@ def qk_norm_rope(query: Tensor, key: Optional[Tensor], q_weight: Optional[Tensor
         given = tensors
         tensors, plan = _plan(*given, eps)
         _PLANS.keep(at, given, tensors, plan)
-    if torch.is_grad_enabled():
-        for x in tensors[:4]:
-            if x is not None and x.requires_grad:
-                return HeadNormFn.apply(*tensors, plan)
+    if _call.tracked(*tensors[:4]):
+        return HeadNormFn.apply(*tensors, plan)  # (which refuses tangents)
     return _run(plan, tensors)
