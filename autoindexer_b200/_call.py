@@ -82,8 +82,13 @@ def dense_d(x: Tensor) -> Tensor:
     return x if x.stride(-1) == 1 else x.contiguous()
 
 
-def t4(x: Tensor) -> "_lib.AiTensor4":
-    return _lib.AiTensor4(x.data_ptr(), *x.stride()[:3])
+def dense4(x: Tensor) -> Tuple[Tensor, "_lib.AiTensor4"]:
+    """``x`` with its last dimension contiguous, and what the library is told of it."""
+    b, h, t, d = x.stride()
+    if d != 1:
+        x = x.contiguous()
+        b, h, t, _ = x.stride()
+    return x, _lib.AiTensor4(x.data_ptr(), b, h, t)
 
 
 def strides4(x: Tensor) -> "_lib.AiTensor4":
@@ -128,7 +133,8 @@ def dense_positions(positions: Tensor) -> Tensor:
 
 def positions_stride(positions: Tensor) -> int:
     """Elements from a batch row's ids to the next one's; 0: one row for all."""
-    return positions.stride(0) if positions.dim() == 2 and positions.shape[0] > 1 else 0
+    strides = positions.stride()
+    return strides[0] if len(strides) == 2 and positions.size(0) > 1 else 0
 
 
 def check_rope(a, rope, positions: Optional[Tensor], batch: int, seq_len: int, head_dim: int, index: int):

@@ -109,18 +109,14 @@ class HeadNormFn(torch.autograd.Function):
         g.fwd = ctx.plan
         # (hooks on saved tensors may have moved them and brought back copies of
         # other strides: all that the struct says of a layout is taken anew)
-        q = _call.dense_d(q)
-        g.fwd.q = _call.t4(q)
-        dq_out = _call.dense_d(dq_out)
-        dq = torch.empty_like(q)
-        g.dq_out, g.dq = _call.t4(dq_out), _call.t4(dq)
+        q, g.fwd.q = _call.dense4(q)
+        dq_out, g.dq_out = _call.dense4(dq_out)
+        dq, g.dq = _call.dense4(torch.empty_like(q))
         dk = dwq = dwk = None
         if k is not None:
-            k = _call.dense_d(k)
-            g.fwd.k = _call.t4(k)
-            dk_out = _call.dense_d(dk_out)
-            dk = torch.empty_like(k)
-            g.dk_out, g.dk = _call.t4(dk_out), _call.t4(dk)
+            k, g.fwd.k = _call.dense4(k)
+            dk_out, g.dk_out = _call.dense4(dk_out)
+            dk, g.dk = _call.dense4(torch.empty_like(k))
         if wq is not None:
             wq = wq.contiguous()
             dwq = torch.empty_like(wq)
