@@ -71,6 +71,27 @@ def tracked(*tensors: Optional[Tensor]) -> bool:
     return False
 
 
+class _NoBackward(torch.autograd.Function):
+    """A call whose results carry no gradient: a backward that reaches it
+    raises, as forward-mode tangents do, where detached results would lose
+    them silently."""
+
+    @staticmethod
+    def forward(ctx, what, run, *inputs):
+        ctx.what = what
+        return run()
+
+    @staticmethod
+    def backward(ctx, *grads):
+        raise RuntimeError(f"{ctx.what} has no backward: call it under torch.no_grad() or on detached tensors")
+
+
+def no_backward(what: str, run, *inputs: Optional[Tensor]):
+    """``run()`` (the results of a call on ``inputs``, some of them ``tracked``)
+    with that mark."""
+    return _NoBackward.apply(what, run, *inputs)
+
+
 def dtype_code(x: Tensor, name: str) -> int:
     code = _DTYPES.get(x.dtype)
     if code is None:

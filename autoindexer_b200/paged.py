@@ -180,7 +180,7 @@ def shared_prefix_attention(query: Tensor, k_pages: Tensor, v_pages: Tensor, pre
     strides with the last dimension contiguous.  The keys that some query of
     the sequence sees must hold finite values; the slots past them may hold
     anything.  A length or page out of range is clamped and sets the status
-    word."""
+    word.  There is no gradient: a backward through the results raises."""
     prefix_len = int(prefix_len)
     if prefix_len == 0:
         prefix_pages = None
@@ -192,6 +192,12 @@ def shared_prefix_attention(query: Tensor, k_pages: Tensor, v_pages: Tensor, pre
         given = tensors
         tensors, plan = _attend_plan(*given, prefix_len, scaling)
         _ATTEND_PLANS.keep(at, given, tensors, plan)
+    if _call.tracked(query, k_pages, v_pages):
+        return _call.no_backward("shared_prefix_attention", lambda: _attend(plan, tensors, return_lse), query, k_pages, v_pages)
+    return _attend(plan, tensors, return_lse)
+
+
+def _attend(plan, tensors, return_lse):
     q, k_pages, v_pages, prefix_pages, page_table, lens, query_lens = tensors
     B, Hq, T, D = q.shape
     device = q.device

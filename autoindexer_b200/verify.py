@@ -85,7 +85,8 @@ def verify_draft(target_logits: Tensor, draft_tokens: Tensor, uniforms: Tensor, 
 
     Logits are CUDA bfloat16, float16 or float32, finite or ``-inf``, with a
     contiguous vocabulary; up to 64 drafted tokens.  A token outside the
-    vocabulary is refused and sets the status word."""
+    vocabulary is refused and sets the status word.  There is no gradient: a
+    backward through the log-probabilities raises."""
     tensors = (target_logits, draft_tokens, uniforms, noise, draft_logits, draft_lens, temperature)
     at = tuple(map(_call.sig, tensors))
     plan = _PLANS.get(at)
@@ -93,6 +94,12 @@ def verify_draft(target_logits: Tensor, draft_tokens: Tensor, uniforms: Tensor, 
         given = tensors
         tensors, plan = _plan(*given)
         _PLANS.keep(at, given, tensors, plan)
+    if _call.tracked(target_logits, draft_logits, temperature):
+        return _call.no_backward("verify_draft", lambda: _run(plan, tensors), target_logits, draft_logits, temperature)
+    return _run(plan, tensors)
+
+
+def _run(plan, tensors):
     target, draft_tokens, uniforms, noise, draft_logits, draft_lens, temperature = tensors
     B, rows, _ = target.shape
     device = target.device
