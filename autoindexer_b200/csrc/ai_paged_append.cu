@@ -37,7 +37,9 @@ __global__ void __launch_bounds__(kThreads, 6) append_kernel(const AiPagedAppend
   const uint32_t tok = it / (uint32_t)chunks, seq = tok / (uint32_t)a.seq_len;
   const int64_t b = seq;
   const int t = (int)(tok - seq * (uint32_t)a.seq_len);
-  if (t >= (a.new_lens ? min(__ldg(a.new_lens + b), a.seq_len) : a.seq_len)) return;
+  const int n_new = a.new_lens ? __ldg(a.new_lens + b) : a.seq_len;
+  if (n_new < 0 || n_new > a.seq_len) report(a.status, AI_ERR_DEV_BOUNDS);  // (taken as the nearest in range)
+  if (t >= n_new) return;
   const int64_t n = (int64_t)__ldg(a.lens + b) + t;
   // (the rows' loads below wait for neither the page nor its check)
   const int col = n >= 0 && n <= 0x7fffffff ? (int)n / a.page_size : -1;

@@ -149,6 +149,7 @@ __device__ __forceinline__ float tau_of(const AiVerifyArgs& a, int b) {
 
 __device__ __forceinline__ int drafted(const AiVerifyArgs& a, int b) {
   const int n = a.draft_lens ? __ldg(a.draft_lens + b) : a.n_draft;
+  if (n < 0 || n > a.n_draft) report(a.status, AI_ERR_DEV_BOUNDS);  // (taken as the nearest in range)
   return max(0, min(n, a.n_draft));
 }
 

@@ -94,7 +94,8 @@ def paged_append(key: Tensor, value: Tensor, k_pages: Tensor, v_pages: Tensor, p
     changed.  ``key_weight`` (``(D,)``) normalises each key row as
     ``qk_norm_rope`` does, ``rope`` / ``positions`` rotate it (as there).
     ``page_table`` ``(B, max_pages)`` int32; a token whose page lies outside
-    it or outside the pool is dropped and sets the status word.  CUDA tensors
+    it or outside the pool is dropped and sets the status word (so does a
+    ``new_lens`` below 0 or above ``T``, taken as 0 or ``T``).  CUDA tensors
     of one dtype (bfloat16, float16, float32), head_dim 32, 64 or 128, any
     page size, any strides with the last dimension contiguous.  Two tokens
     given the same slot race; no gradient flows through the cache."""

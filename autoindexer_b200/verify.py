@@ -85,7 +85,8 @@ def verify_draft(target_logits: Tensor, draft_tokens: Tensor, uniforms: Tensor, 
 
     Logits are CUDA bfloat16, float16 or float32, finite or ``-inf``, with a
     contiguous vocabulary; up to 64 drafted tokens.  A token outside the
-    vocabulary is refused and sets the status word.  There is no gradient: a
+    vocabulary is refused and sets the status word (so does a ``draft_lens``
+    below 0 or above ``L``, taken as 0 or ``L``).  There is no gradient: a
     backward through the log-probabilities raises."""
     tensors = (target_logits, draft_tokens, uniforms, noise, draft_logits, draft_lens, temperature)
     at = tuple(map(_call.sig, tensors))

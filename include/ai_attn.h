@@ -511,7 +511,9 @@ int ai_head_norm_bwd(const AiHeadNormBwdArgs* args, void* stream);
  * becomes its token n = lens[b] + t, stored in slot n % page_size of page
  * page_table[b][n / page_size].  Keys are normalised (k_weight not NULL) and
  * rotated (tables not NULL) on the way, values copied.  A token whose page
- * is outside the table or the pool is skipped with AI_ERR_DEV_BOUNDS. */
+ * is outside the table or the pool is skipped with AI_ERR_DEV_BOUNDS.  A
+ * new_lens outside [0, seq_len] is AI_ERR_DEV_BOUNDS too and counts as the nearest
+ * length within. */
 typedef struct AiPagedAppendArgs {
   int32_t batch;
   int32_t seq_len;            /* T: new tokens given per sequence */
@@ -591,7 +593,9 @@ int ai_prefix_attn(const AiPrefixAttnArgs* args, void* stream);
  * r = p_a after none (noise: exponential variates, so the token is a sample
  * of r); where r is zero everywhere, r = p_a.  tau_b = 0 decodes greedily:
  * p_i is one-hot at the largest logit.  Equal values go to the lowest index.
- * Logits are finite or -inf. */
+ * Logits are finite or -inf.  A draft_lens outside [0, n_draft] or a token outside
+ * the vocabulary is AI_ERR_DEV_BOUNDS; the length counts as the nearest within,
+ * the token is refused. */
 typedef struct AiVerifyArgs {
   int32_t batch;
   int32_t n_draft;            /* L: drafted tokens given per sequence, 0 .. 64 */
