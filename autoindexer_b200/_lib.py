@@ -30,9 +30,9 @@ __all__ = [
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "_ai_attn.so")
 
 DTYPE_BF16, DTYPE_F16, DTYPE_F32 = 0, 1, 2
-# AiProfKind, in order.
-PROF_KINDS = ("prerot", "fwd", "fwd_fill", "delta", "dq", "dkdv", "bwd_fill", "simt", "decode", "head_norm",
-              "append", "prefix", "verify")
+# AiProfKind, in order: those that ai_attn_profile_read writes, and all.
+PROF_KINDS = ("prerot", "fwd", "fwd_fill", "delta", "dq", "dkdv", "bwd_fill", "simt", "decode")
+ALL_PROF_KINDS = PROF_KINDS + ("head_norm", "append", "prefix", "verify")
 ABI_VERSION = 9
 BWD_DQ, BWD_DKDV = 1, 2
 
@@ -50,6 +50,7 @@ EXPORTED_SYMBOLS = (
     "ai_attn_decode",
     "ai_attn_profile_enable",
     "ai_attn_profile_read",
+    "ai_attn_profile_read_all",
     "ai_attn_read_status",
     "ai_attn_selftest_wait",
     "ai_attn_strerror",
@@ -447,6 +448,8 @@ def _bind(handle):
     handle.ai_attn_profile_enable.argtypes = [ctypes.c_int]
     handle.ai_attn_profile_read.restype = ctypes.c_int
     handle.ai_attn_profile_read.argtypes = [P(ctypes.c_float), P(ctypes.c_int32)]
+    handle.ai_attn_profile_read_all.restype = ctypes.c_int
+    handle.ai_attn_profile_read_all.argtypes = [P(ctypes.c_float), P(ctypes.c_int32), ctypes.c_int32]
     handle.ai_attn_selftest_wait.restype = ctypes.c_int
     handle.ai_attn_selftest_wait.argtypes = [ctypes.c_void_p, ctypes.c_longlong, ctypes.c_void_p]
     vp, i32, i64 = ctypes.c_void_p, ctypes.c_int32, ctypes.c_int64

@@ -190,7 +190,7 @@ def attn_bwd(q, k, v, out, lse, dout, layout: CompiledLayout, scale: float, rota
 
 class KernelTimes:
     """Per-kernel device times of this library's launches (CUDA events on the
-    launch streams; ``ai_attn_profile_enable`` / ``ai_attn_profile_read``)::
+    launch streams; ``ai_attn_profile_enable`` / ``ai_attn_profile_read_all``)::
 
         with KernelTimes() as kt:
             ...  # calls into the library
@@ -203,14 +203,14 @@ class KernelTimes:
 
     def __exit__(self, *exc):
         lib = _lib.lib()
-        n = len(_lib.PROF_KINDS)
+        n = len(_lib.ALL_PROF_KINDS)
         ms = (ctypes.c_float * n)()
         cnt = (ctypes.c_int32 * n)()
-        rc = lib.ai_attn_profile_read(ms, cnt)
+        rc = lib.ai_attn_profile_read_all(ms, cnt, n)
         lib.ai_attn_profile_enable(0)
-        _lib.check(rc, "ai_attn_profile_read")
-        self.ms = {k: float(ms[i]) for i, k in enumerate(_lib.PROF_KINDS)}
-        self.launches = {k: int(cnt[i]) for i, k in enumerate(_lib.PROF_KINDS)}
+        _lib.check(rc, "ai_attn_profile_read_all")
+        self.ms = {k: float(ms[i]) for i, k in enumerate(_lib.ALL_PROF_KINDS)}
+        self.launches = {k: int(cnt[i]) for i, k in enumerate(_lib.ALL_PROF_KINDS)}
         return False
 
 

@@ -1,5 +1,5 @@
 // Optional per-kernel timing with CUDA events (ai_attn_profile_enable /
-// ai_attn_profile_read).  When enabled, every launch of this library is
+// ai_attn_profile_read and _read_all).  When enabled, every launch of this library is
 // bracketed by two events recorded on the launch's own stream; reading
 // synchronizes them and returns the summed elapsed time and the launch count
 // per kernel kind.  Nothing is skipped or reordered; when disabled (the
@@ -63,9 +63,15 @@ int ai_attn_profile_enable(int on) {
 }
 
 int ai_attn_profile_read(float* ms_by_kind, int32_t* launches_by_kind) {
+  return ai_attn_profile_read_all(ms_by_kind, launches_by_kind, AI_PROF_KINDS);
+}
+
+int ai_attn_profile_read_all(float* ms_by_kind, int32_t* launches_by_kind, int32_t n) {
   if (!ms_by_kind || !launches_by_kind) return AI_ERR_NULL;
+  if (n < 0) return AI_ERR_SHAPE;
+  if (n > AI_PROF_ALL_KINDS) n = AI_PROF_ALL_KINDS;
   std::lock_guard<std::mutex> lock(ai::g_mu);
-  for (int k = 0; k < AI_PROF_KINDS; ++k) {
+  for (int k = 0; k < n; ++k) {
     ms_by_kind[k] = 0.f;
     launches_by_kind[k] = 0;
   }
@@ -77,7 +83,7 @@ int ai_attn_profile_read(float* ms_by_kind, int32_t* launches_by_kind) {
       rc = AI_ERR_LAUNCH;
       continue;
     }
-    if (p.kind >= 0 && p.kind < AI_PROF_KINDS) {
+    if (p.kind >= 0 && p.kind < n) {
       ms_by_kind[p.kind] += ms;
       launches_by_kind[p.kind] += 1;
     }

@@ -643,7 +643,9 @@ const char* ai_attn_strerror(int code);
  * is skipped or reordered).  ai_attn_profile_enable(1) starts a fresh
  * collection, (0) stops it.  ai_attn_profile_read synchronises the recorded
  * events and writes, per kind, the summed elapsed milliseconds and the launch
- * count (arrays of AI_PROF_KINDS entries), then clears the collection.  At
+ * count (arrays of AI_PROF_KINDS entries: the kinds that ABI 9 began with), then
+ * clears the collection.  ai_attn_profile_read_all does the same for all kinds
+ * and writes at most n entries to each array (AI_PROF_ALL_KINDS of them exist).  At
  * most 4096 launches are recorded per collection.  Not for concurrent use
  * from several host threads. */
 typedef enum AiProfKind {
@@ -656,14 +658,16 @@ typedef enum AiProfKind {
   AI_PROF_BWD_FILL = 6, /* backward rows no block owns */
   AI_PROF_SIMT = 7,     /* fp32 / fp16 / other head_dim path */
   AI_PROF_DECODE = 8,   /* decode step (split-K + combine) */
+  AI_PROF_KINDS = 9,    /* what ai_attn_profile_read writes: never more under ABI 9 */
   AI_PROF_HEAD_NORM = 9, /* per-head norms with the rotation, forward and backward */
   AI_PROF_APPEND = 10,  /* paged cache append */
   AI_PROF_PREFIX = 11,  /* shared-prefix attention (split + combine) */
   AI_PROF_VERIFY = 12,  /* draft verification */
-  AI_PROF_KINDS = 13
+  AI_PROF_ALL_KINDS = 13
 } AiProfKind;
 int ai_attn_profile_enable(int on);
 int ai_attn_profile_read(float* ms_by_kind, int32_t* launches_by_kind);
+int ai_attn_profile_read_all(float* ms_by_kind, int32_t* launches_by_kind, int32_t n);
 
 #ifdef __cplusplus
 }
