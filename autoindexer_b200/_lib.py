@@ -420,8 +420,6 @@ _lib = None
 
 def _bind(handle):
     P = ctypes.POINTER
-    handle.ai_attn_abi_version.restype = ctypes.c_int
-    handle.ai_attn_abi_version.argtypes = []
     for name in ("ai_attn_fwd_tile_rows", "ai_attn_kv_tile_rows"):
         fn = getattr(handle, name)
         fn.restype = ctypes.c_int
@@ -494,11 +492,16 @@ def lib():
                     raise RuntimeError(
                         f"autoindexer_b200: CUDA library {LIB_PATH} is not built; "
                         "run `python -m autoindexer_b200.build` (nvcc, sm_100a)")
-                handle = _bind(ctypes.CDLL(LIB_PATH))
+                handle = ctypes.CDLL(LIB_PATH)
+                handle.ai_attn_abi_version.restype = ctypes.c_int
+                handle.ai_attn_abi_version.argtypes = []
                 ver = handle.ai_attn_abi_version()
                 if ver != ABI_VERSION:
                     raise RuntimeError(f"autoindexer_b200: library ABI {ver} != expected {ABI_VERSION}; rebuild it")
-                _lib = handle
+                try:
+                    _lib = _bind(handle)
+                except AttributeError as e:  # (functions are added within an ABI)
+                    raise RuntimeError(f"autoindexer_b200: the library lacks a function ({e}); rebuild it") from e
     return _lib
 
 
