@@ -21,6 +21,8 @@ from . import _call, _lib
 
 __all__ = ["paged_append", "shared_prefix_attention"]
 
+MAX_BATCH = 65535  # sequences of an attention call
+
 
 def _pools(k_pages: Tensor, v_pages: Tensor, heads: int, head_dim: int, dtype, index: int) -> None:
     s = k_pages.shape
@@ -130,6 +132,8 @@ def _attend_plan(query, k_pages, v_pages, prefix_pages, page_table, lens, query_
     B, Hq, T, D = query.shape
     if D not in (32, 64, 128):
         raise ValueError(f"head_dim must be 32, 64 or 128, got {D}")
+    if B > MAX_BATCH:
+        raise ValueError(f"at most {MAX_BATCH} sequences, got {B}: split the batch")
     heads = k_pages.shape[1] if k_pages.dim() == 4 else 0
     if heads == 0 or Hq % heads != 0:
         raise ValueError(f"num_q_heads {Hq} is not a multiple of num_kv_heads {heads}")
@@ -178,7 +182,7 @@ def shared_prefix_attention(query: Tensor, k_pages: Tensor, v_pages: Tensor, pre
     decoding.
 
     CUDA tensors of one dtype, head_dim 32, 64 or 128, any page size, any
-    strides with the last dimension contiguous.  The keys that some query of
+    strides with the last dimension contiguous, up to 65535 sequences.  The keys that some query of
     the sequence sees must hold finite values; the slots past them may hold
     anything.  A length or page out of range is clamped and sets the status
     word.  There is no gradient: a backward through the results raises."""

@@ -18,6 +18,7 @@ from . import _call, _lib
 __all__ = ["verify_draft"]
 
 MAX_DRAFT = 64
+MAX_ROWS = 65535  # (sequences times 2 L + 1)
 
 
 _PLANS = _call.Plans()
@@ -33,6 +34,8 @@ def _plan(target, draft_tokens, uniforms, noise, draft_logits, draft_lens, tempe
     L = rows - 1
     if L > MAX_DRAFT:
         raise ValueError(f"at most {MAX_DRAFT} drafted tokens, got {L}")
+    if B * (2 * L + 1) > MAX_ROWS:
+        raise ValueError(f"B (2 L + 1) may be {MAX_ROWS} at most, got {B} sequences of {L} drafted tokens: split the batch")
     if draft_tokens.dtype is not torch.int64:
         raise TypeError(f"draft_tokens must be int64, got {draft_tokens.dtype}")
     if draft_tokens.shape != (B, L):
@@ -84,7 +87,7 @@ def verify_draft(target_logits: Tensor, draft_tokens: Tensor, uniforms: Tensor, 
     one's log-probability under the target (0 past them, and in greedy rows).
 
     Logits are CUDA bfloat16, float16 or float32, finite or ``-inf``, with a
-    contiguous vocabulary; up to 64 drafted tokens.  A token outside the
+    contiguous vocabulary; up to 64 drafted tokens, ``B (2 L + 1)`` up to 65535.  A token outside the
     vocabulary is refused and sets the status word (so does a ``draft_lens``
     below 0 or above ``L``, taken as 0 or ``L``).  There is no gradient: a
     backward through the log-probabilities raises."""

@@ -554,7 +554,7 @@ int ai_paged_append(const AiPagedAppendArgs* args, void* stream);
  * bf16 and fp16 with head_dim 64 or 128, page_size a power of two from 16,
  * q, k_pages and v_pages with 16-byte aligned rows, scale > 0 and at most
  * 1024 sequences run on the tensor cores; everything else on fp32 arithmetic
- * (several times slower). */
+ * (several times slower), for up to 65535 sequences. */
 typedef struct AiPrefixAttnArgs {
   int32_t batch;
   int32_t seq_len;            /* T: query tokens per sequence */
@@ -593,9 +593,9 @@ int ai_prefix_attn(const AiPrefixAttnArgs* args, void* stream);
  * r = p_a after none (noise: exponential variates, so the token is a sample
  * of r); where r is zero everywhere, r = p_a.  tau_b = 0 decodes greedily:
  * p_i is one-hot at the largest logit.  Equal values go to the lowest index.
- * Logits are finite or -inf.  A draft_lens outside [0, n_draft] or a token outside
- * the vocabulary is AI_ERR_DEV_BOUNDS; the length counts as the nearest within,
- * the token is refused. */
+ * Logits are finite or -inf; batch (2 n_draft + 1) is 65535 at most.  A draft_lens
+ * outside [0, n_draft] or a token outside the vocabulary is AI_ERR_DEV_BOUNDS; the
+ * length counts as the nearest within, the token is refused. */
 typedef struct AiVerifyArgs {
   int32_t batch;
   int32_t n_draft;            /* L: drafted tokens given per sequence, 0 .. 64 */
