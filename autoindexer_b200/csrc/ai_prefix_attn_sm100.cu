@@ -33,7 +33,7 @@
 //
 // Measured (bf16, 32 + 8 heads, D 128, up to 2048 own keys): 64 sequences of
 // one token on a prefix of 32,768 keys 95 us, of up to five tokens 183 us (217
-// at the power limit); 16 on 4096 + 512 keys 23 us; four on 257 + 65 keys 14 us (two launches' latency).
+// at the power limit); 16 on 4096 + 512 keys 24 us; four on 257 + 65 keys 14 us (two launches' latency).
 
 #include <cuda.h>
 #include <cuda_bf16.h>
@@ -789,9 +789,10 @@ __device__ __forceinline__ void ldsm4_t(uint32_t (&r)[4], uint32_t addr) {
 // With a few warps per scheduler the step is bound by its own chain of
 // instructions, so loads and look-ups are kept out of it.
 namespace warpk {
-// The largest CTA, five workers of two warps and the loading one.  (Two registers
-// more for the sums than before; at 384 the fp16 kernel spilled: 61 us for 58 on own
-// lists of 64 sequences of up to 2048 keys.)
+// The largest CTA, five workers of two warps and the loading one.  (With a bound of
+// 384 the fp16 kernel spills: 61 us for 58 on own lists of 64 sequences of up to
+// 2048 keys.  bf16: 56 either way, 16 sequences on 4096 + 512 keys 24.8 with 384
+// and 25.0 so.)
 constexpr int kMaxThreads = 352;
 template <int D>
 struct Ring {
@@ -1301,7 +1302,10 @@ bool make_plan(const AiPrefixAttnArgs& a, Plan* p, size_t* bytes) {
   // 51 / 48 on 4096 + 5).  A tile position costs about 8 positions of the warp
   // kernel, 11 with head_dim 64 (its CTA is bound by exponentials, theirs by
   // bytes), fewer where a warp kernel position has several warps' rows (at 6 /
-  // 8 / 11: 109 / 96 / 100 us and 184 / 213 / 262 on the two largest above).
+  // 8 / 11: 109 / 96 / 100 us and 184 / 213 / 262 on the two largest above;
+  // head_dim 64 at 8 / 11 / 14: 73 / 66 / 72 us on 32,768 + 2048, 153 / 146 / 158
+  // with five tokens, 26.0 / 25.5 / 25.9 on 2048 + 256, but three tokens on 30,000
+  // + 300 99 / 101 / 128).
   if (p->nt == 2 && p->tile.workers > 0 && p->tile.per_seq == 0 && p->warp.workers > 0) {
     p->share = sms;
     p->tile_cost = (a.head_dim == 128 ? 8 : 11) * (p->split == 1 ? 4 : 3) / 4;
