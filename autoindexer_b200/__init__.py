@@ -19,11 +19,14 @@ from .meta import CompiledLayout, RowLayouts, compile_layout
 from .positions import (BlockType, PositionBlock, PositionBlockList, blocks_from_concat, cursor_stream,
                         document_blocks, positions_from_operations)
 from .decode import decode_attention
+from .distill import distill_loss, distill_loss_and_grad
 from .head_norm import qk_norm_rope
 from .index_head import compute_index_losses_b200
 from .paged import paged_append, shared_prefix_attention
+from .paged4 import paged_append_4bit, paged_attention_4bit, paged_read_4bit
 from .prefill import plain_causal_attn_b200, prefill_attention_interface, prefill_layout
 from .rope import SectionedRope, default_inv_freq, rope_table
+from .scoring import TokenScores, token_logprobs
 from .verify import verify_draft
 
 __all__ = [
@@ -56,4 +59,11 @@ __all__ = [
     "paged_append",
     "shared_prefix_attention",
     "verify_draft",
+    "TokenScores",
+    "token_logprobs",
+    "distill_loss",
+    "distill_loss_and_grad",
+    "paged_append_4bit",
+    "paged_read_4bit",
+    "paged_attention_4bit",
 ]

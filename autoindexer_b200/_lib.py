@@ -32,9 +32,11 @@ LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "_ai_attn.so
 DTYPE_BF16, DTYPE_F16, DTYPE_F32 = 0, 1, 2
 # AiProfKind, in order: those that ai_attn_profile_read writes, and all.
 PROF_KINDS = ("prerot", "fwd", "fwd_fill", "delta", "dq", "dkdv", "bwd_fill", "simt", "decode")
-ALL_PROF_KINDS = PROF_KINDS + ("head_norm", "append", "prefix", "verify")
+ALL_PROF_KINDS = PROF_KINDS + ("head_norm", "append", "prefix", "verify", "score", "distill", "paged4", "attn4")
 ABI_VERSION = 9
 BWD_DQ, BWD_DKDV = 1, 2
+TAILS = {"bucket": 0, "renormalize": 1}  # AiTail
+MAX_TOP = 128  # AI_SCORE_MAX_TOP, AI_DISTILL_MAX_TOP
 
 # Every function include/ai_attn.h declares.
 EXPORTED_SYMBOLS = (
@@ -70,6 +72,13 @@ EXPORTED_SYMBOLS = (
     "ai_prefix_attn",
     "ai_verify_draft_workspace",
     "ai_verify_draft",
+    "ai_token_logprobs",
+    "ai_token_logprobs_bwd",
+    "ai_distill",
+    "ai_paged_append_4bit",
+    "ai_paged_read_4bit",
+    "ai_paged_attn_4bit_workspace",
+    "ai_paged_attn_4bit",
 )
 
 _i32p = ctypes.POINTER(ctypes.c_int32)
@@ -414,6 +423,113 @@ class AiVerifyArgs(ctypes.Structure):
     ]
 
 
+class AiScoreArgs(ctypes.Structure):
+    _fields_ = [
+        ("batch", ctypes.c_int32),
+        ("seq_len", ctypes.c_int32),
+        ("vocab", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("logits", ctypes.c_void_p),
+        ("stride_b", ctypes.c_int64),
+        ("stride_t", ctypes.c_int64),
+        ("tokens", ctypes.c_void_p),
+        ("temperature", ctypes.c_void_p),
+        ("top_k", ctypes.c_int32),
+        ("logprobs", ctypes.c_void_p),
+        ("entropy", ctypes.c_void_p),
+        ("top_logprobs", ctypes.c_void_p),
+        ("top_tokens", ctypes.c_void_p),
+        ("row_stats", ctypes.c_void_p),
+        ("status", ctypes.c_void_p),
+    ]
+
+
+class AiScoreBwdArgs(ctypes.Structure):
+    _fields_ = [
+        ("fwd", AiScoreArgs),
+        ("g_logprobs", ctypes.c_void_p),
+        ("g_entropy", ctypes.c_void_p),
+        ("g_top", ctypes.c_void_p),
+        ("dlogits", ctypes.c_void_p),
+        ("dstride_b", ctypes.c_int64),
+        ("dstride_t", ctypes.c_int64),
+    ]
+
+
+class AiDistillArgs(ctypes.Structure):
+    _fields_ = [
+        ("batch", ctypes.c_int32),
+        ("seq_len", ctypes.c_int32),
+        ("vocab", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("logits", ctypes.c_void_p),
+        ("stride_b", ctypes.c_int64),
+        ("stride_t", ctypes.c_int64),
+        ("n_top", ctypes.c_int32),
+        ("tail", ctypes.c_int32),
+        ("top_tokens", ctypes.c_void_p),
+        ("top_logprobs", ctypes.c_void_p),
+        ("weights", ctypes.c_void_p),
+        ("temperature", ctypes.c_void_p),
+        ("losses", ctypes.c_void_p),
+        ("dlogits", ctypes.c_void_p),
+        ("dstride_b", ctypes.c_int64),
+        ("dstride_t", ctypes.c_int64),
+        ("status", ctypes.c_void_p),
+    ]
+
+
+class AiPool4(ctypes.Structure):
+    _fields_ = [
+        ("k_codes", AiTensor4),
+        ("v_codes", AiTensor4),
+        ("k_scales", AiTensor4),
+        ("v_scales", AiTensor4),
+        ("n_pages", ctypes.c_int32),
+        ("page_size", ctypes.c_int32),
+        ("page_table", ctypes.c_void_p),
+        ("page_table_stride", ctypes.c_int64),
+        ("max_pages", ctypes.c_int32),
+    ]
+
+
+class AiPaged4Args(ctypes.Structure):
+    _fields_ = [
+        ("batch", ctypes.c_int32),
+        ("seq_len", ctypes.c_int32),
+        ("num_kv_heads", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("k", AiTensor4),
+        ("v", AiTensor4),
+        ("pool", AiPool4),
+        ("lens", ctypes.c_void_p),
+        ("n", ctypes.c_void_p),
+        ("status", ctypes.c_void_p),
+    ]
+
+
+class AiPagedAttn4Args(ctypes.Structure):
+    _fields_ = [
+        ("batch", ctypes.c_int32),
+        ("seq_len", ctypes.c_int32),
+        ("num_q_heads", ctypes.c_int32),
+        ("num_kv_heads", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("scale", ctypes.c_float),
+        ("q", AiTensor4),
+        ("out", AiTensor4),
+        ("lse", ctypes.c_void_p),
+        ("pool", AiPool4),
+        ("lens", ctypes.c_void_p),
+        ("query_lens", ctypes.c_void_p),
+        ("status", ctypes.c_void_p),
+        ("workspace", ctypes.c_void_p),
+        ("workspace_bytes", ctypes.c_size_t),
+    ]
+
+
 _lock = threading.Lock()
 _lib = None
 
@@ -469,13 +585,17 @@ def _bind(handle):
     handle.ai_index_rows.argtypes = [P(AiPrepList), vp, i64, P(AiIndexRowsOut)]
     for name, args in (("ai_head_norm_fwd", AiHeadNormArgs), ("ai_head_norm_bwd", AiHeadNormBwdArgs),
                        ("ai_paged_append", AiPagedAppendArgs), ("ai_prefix_attn", AiPrefixAttnArgs),
-                       ("ai_verify_draft", AiVerifyArgs)):
+                       ("ai_verify_draft", AiVerifyArgs), ("ai_token_logprobs", AiScoreArgs),
+                       ("ai_token_logprobs_bwd", AiScoreBwdArgs), ("ai_distill", AiDistillArgs),
+                       ("ai_paged_append_4bit", AiPaged4Args), ("ai_paged_read_4bit", AiPaged4Args),
+                       ("ai_paged_attn_4bit", AiPagedAttn4Args)):
         fn = getattr(handle, name)
         fn.restype = ctypes.c_int
         fn.argtypes = [P(args), vp]
     for name, args in (("ai_head_norm_bwd_workspace", AiHeadNormBwdArgs),
                        ("ai_prefix_attn_workspace", AiPrefixAttnArgs),
-                       ("ai_verify_draft_workspace", AiVerifyArgs)):
+                       ("ai_verify_draft_workspace", AiVerifyArgs),
+                       ("ai_paged_attn_4bit_workspace", AiPagedAttn4Args)):
         fn = getattr(handle, name)
         fn.restype = ctypes.c_int
         fn.argtypes = [P(args), P(ctypes.c_size_t)]

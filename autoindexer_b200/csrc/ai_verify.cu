@@ -24,15 +24,17 @@
 #include <cuda_runtime.h>
 #include <math_constants.h>
 
-#include <cfloat>
 #include <cstring>
 
 #include "ai_common.cuh"
 #include "ai_kernels.h"
+#include "ai_logits.cuh"
 #include "sm100_ptx.cuh"
 
 namespace ai {
 namespace verify {
+
+using namespace logits;
 
 constexpr int kThreads = 256, kWarps = kThreads / 32;
 constexpr int kMaxDraft = 64;
@@ -60,68 +62,6 @@ struct Ws {
   unsigned int* arrived;
   int splits;  // of the stats pass
 };
-
-template <typename T>
-__device__ __forceinline__ float at(const T* p, int64_t i) {
-  return to_f32(p[i]);
-}
-
-// 16 bytes of logits: all -inf, the larger of each pair of places, the largest.
-template <typename T> struct Vec;
-template <> struct Vec<float> {
-  static constexpr uint32_t kNone = 0xff800000u;
-  __device__ static uint32_t larger(uint32_t a, uint32_t b) {
-    return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b)));
-  }
-  __device__ static float top(uint32_t a) { return __uint_as_float(a); }
-  __device__ static void get(const uint4& r, float2 (&f)[2]) {
-    f[0] = make_float2(__uint_as_float(r.x), __uint_as_float(r.y));
-    f[1] = make_float2(__uint_as_float(r.z), __uint_as_float(r.w));
-  }
-};
-template <> struct Vec<__nv_bfloat16> {
-  static constexpr uint32_t kNone = 0xff80ff80u;
-  __device__ static uint32_t larger(uint32_t a, uint32_t b) {
-    const __nv_bfloat162 m = __hmax2(*reinterpret_cast<__nv_bfloat162*>(&a), *reinterpret_cast<__nv_bfloat162*>(&b));
-    return *reinterpret_cast<const uint32_t*>(&m);
-  }
-  __device__ static float top(uint32_t a) {
-    return fmaxf(__uint_as_float(a << 16), __uint_as_float(a & 0xffff0000u));
-  }
-  __device__ static void get(const uint4& r, float2 (&f)[4]) {
-    const uint32_t w[4] = {r.x, r.y, r.z, r.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) f[i] = make_float2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
-  }
-};
-template <> struct Vec<__half> {
-  static constexpr uint32_t kNone = 0xfc00fc00u;
-  __device__ static uint32_t larger(uint32_t a, uint32_t b) {
-    const __half2 m = __hmax2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
-    return *reinterpret_cast<const uint32_t*>(&m);
-  }
-  __device__ static float top(uint32_t a) {
-    const float2 f = __half22float2(*reinterpret_cast<__half2*>(&a));
-    return fmaxf(f.x, f.y);
-  }
-  __device__ static void get(const uint4& r, float2 (&f)[4]) {
-    const uint32_t w[4] = {r.x, r.y, r.z, r.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) f[i] = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
-  }
-};
-
-// Slope c of a row's exponent (1 for a greedy row, which has no use for it),
-// finite and above zero: a logit at the maximum keeps the exponent 0 and a
-// masked one -inf at any temperature, subnormal or infinite ones included.
-__device__ __forceinline__ float slope(float tau) {
-  return tau > 0.f ? fminf(fmaxf(kLog2e / tau, FLT_MIN), FLT_MAX) : 1.f;
-}
-
-// 2^((x - m) c), 0 for a masked logit (m may be -inf then).
-__device__ __forceinline__ float weight(float x, float c, float m) {
-  return x == -CUDART_INF_F ? 0.f : ptx::ex2((x - m) * c);
-}
 
 __device__ __forceinline__ Stat merge(const Stat& a, const Stat& b, float c) {
   Stat r;

@@ -1,0 +1,241 @@
+"""The paged key / value cache in 4 bits: appending to it, reading it back and
+attending over it.
+
+Of a head row, 32 dims share a float16 scale ``d``, minus an eighth of their
+value of largest magnitude; a dim's code ``c`` in 0..15 stands for ``(c - 8)
+d``.  A token takes 144 bytes per KV head at head_dim 128 (keys and values
+together) where bfloat16 takes 512.  Codes live in pools ``(n_pages, Hkv,
+page_size, D / 2)`` of bytes (dim ``32 c + 4 g + j``, ``g < 8``, ``j < 4``, in
+byte ``g D / 16 + 2 c + j // 2``, the low half for even ``j``), scales in pools
+``(n_pages, Hkv, page_size, D / 32)``.  Page tables, lengths and graph capture
+are as in the 16-bit cache (``paged_append``, ``shared_prefix_attention``);
+sequences that share a prompt list the same pages.
+"""
+
+from __future__ import annotations
+
+from typing import Optional, Tuple
+
+import torch
+from torch import Tensor
+
+from . import _call, _lib
+from .paged import _table
+
+__all__ = ["paged_append_4bit", "paged_read_4bit", "paged_attention_4bit"]
+
+MAX_BATCH = 4096  # sequences of an attention call
+GROUP = 32
+
+
+def _pool(p, k_pages, v_pages, k_scales, v_scales, page_table, batch: int, heads: int, head_dim: int, index: int) -> Tensor:
+    """Sets what ``p`` says of the pools, without pointers; returns the page table."""
+    s = k_pages.shape
+    if len(s) != 4 or s != v_pages.shape or s[1] != heads or s[3] != head_dim // 2:
+        raise ValueError(f"k_pages and v_pages must be (n_pages, {heads}, page_size, {head_dim // 2}), got "
+                         f"{tuple(s)} and {tuple(v_pages.shape)}")
+    if s[0] == 0 or s[2] < 16 or s[2] & (s[2] - 1):
+        raise ValueError(f"page_size must be a power of two from 16 and the pools not empty, got {tuple(s)}")
+    size = head_dim // GROUP
+    for name, x, dtype, last, unit in (("k_pages", k_pages, torch.uint8, s[3], 16), ("v_pages", v_pages, torch.uint8, s[3], 16),
+                                       ("k_scales", k_scales, torch.float16, size, size),
+                                       ("v_scales", v_scales, torch.float16, size, size)):
+        if x.dtype is not dtype:
+            raise TypeError(f"{name} must be {dtype}, got {x.dtype}")
+        if x.shape != (*s[:3], last):
+            raise ValueError(f"{name} must have shape {(*s[:3], last)}, got {tuple(x.shape)}")
+        if x.stride(3) != 1 and last > 1:
+            raise ValueError(f"{name} must have a contiguous last dimension")
+        st = x.stride()
+        if (st[0] | st[1] | st[2]) % unit or x.data_ptr() % (unit * x.element_size()):
+            raise ValueError(f"the rows of {name} must start on {unit * x.element_size()}-byte boundaries")
+        _call.on_device(name, x, index)
+    page_table = _table(page_table, batch, index)
+    if page_table.shape[1] == 0:
+        raise ValueError("page_table has no columns")
+    p.k_codes, p.v_codes, p.k_scales, p.v_scales = map(_call.strides4, (k_pages, v_pages, k_scales, v_scales))
+    p.n_pages, p.page_size = s[0], s[2]
+    p.page_table_stride, p.max_pages = page_table.stride(0), page_table.shape[1]
+    return page_table
+
+
+def _point(p, k_pages, v_pages, k_scales, v_scales, page_table) -> None:
+    p.k_codes.ptr, p.v_codes.ptr = k_pages.data_ptr(), v_pages.data_ptr()
+    p.k_scales.ptr, p.v_scales.ptr = k_scales.data_ptr(), v_scales.data_ptr()
+    p.page_table = page_table.data_ptr()
+
+
+def _aligned(*pools: Tensor) -> Tuple[int, ...]:
+    return tuple(x.data_ptr() % 16 for x in pools)
+
+
+def _head_dim(D: int) -> None:
+    if D not in (32, 64, 128):
+        raise ValueError(f"head_dim must be 32, 64 or 128, got {D}")
+
+
+_PLANS, _ATTEND_PLANS = _call.Plans(), _call.Plans()
+
+
+def _paged_plan(key, value, k_pages, v_pages, k_scales, v_scales, page_table, lens, n, name):
+    """Checks the arguments of an append (or a read, with ``key`` and ``value`` for
+    its results); returns the tensors the kernel reads and the argument struct
+    without pointers."""
+    index = _call.cuda_index("key", key)
+    if key.dim() != 4 or key.shape != value.shape:
+        raise ValueError(f"key and value must be (B, Hkv, T, D), got {tuple(key.shape)} and {tuple(value.shape)}")
+    B, H, T, D = key.shape
+    if key.numel() == 0:
+        raise ValueError("key and value must not be empty")
+    _head_dim(D)
+    if value.dtype is not key.dtype:
+        raise TypeError(f"value is {value.dtype}, key {key.dtype}")
+    _call.on_device("value", value, index)
+    a = _lib.AiPaged4Args()
+    a.batch, a.num_kv_heads, a.seq_len, a.head_dim = B, H, T, D
+    a.dtype = _call.dtype_code(key, "key")
+    page_table = _pool(a.pool, k_pages, v_pages, k_scales, v_scales, page_table, B, H, D, index)
+    lens = _call.ints("lens", lens, (B,), index)
+    if n is not None:
+        n = _call.ints(name, n, (B,), index)
+    key, value = _call.dense_d(key), _call.dense_d(value)
+    a.k, a.v = _call.strides4(key), _call.strides4(value)
+    a.status = _call.status_ptr(index)
+    return (key, value, k_pages, v_pages, k_scales, v_scales, page_table, lens, n), a
+
+
+def _paged(fn, what, tensors, name) -> None:
+    at = (*map(_call.sig, tensors), name, _aligned(*tensors[2:6]))
+    plan = _PLANS.get(at)
+    if plan is None:
+        given = tensors
+        tensors, plan = _paged_plan(*given, name)
+        _PLANS.keep(at, given, tensors, plan)
+    k, v, *pools, lens, n = tensors
+    a = _call.copy(plan)
+    a.k.ptr, a.v.ptr, a.lens = k.data_ptr(), v.data_ptr(), lens.data_ptr()
+    _point(a.pool, *pools)
+    if n is not None:
+        a.n = n.data_ptr()
+    _call.launch(fn, a, k.get_device(), what)
+
+
+def paged_append_4bit(key: Tensor, value: Tensor, k_pages: Tensor, v_pages: Tensor, k_scales: Tensor, v_scales: Tensor,
+                      page_table: Tensor, lens: Tensor, new_lens: Optional[Tensor] = None) -> None:
+    """Writes new tokens into the cache, in place.
+
+    ``key`` (normalised and rotated: ``qk_norm_rope`` returns them so) and
+    ``value`` ``(B, Hkv, T, D)``: token ``t < new_lens[b]`` (all ``T`` without
+    it) becomes sequence ``b``'s token ``lens[b] + t``, in slot ``n %
+    page_size`` of page ``page_table[b, n // page_size]``; ``lens`` ``(B,)``
+    int32 is not changed.  A token whose page lies outside the table or the
+    pool is dropped and sets the status word (so does a ``new_lens`` below 0
+    or above ``T``, taken as 0 or ``T``).  32 dims with a NaN or an infinity
+    among them read back as NaN; scales are limited to 65504.  ``key`` and
+    ``value`` are CUDA tensors of one dtype (bfloat16, float16, float32),
+    head_dim 32, 64 or 128, any strides; page sizes are powers of two from 16,
+    the rows of codes lie on 16-byte boundaries.  Two tokens given the same
+    slot race; no gradient flows through the cache."""
+    _paged(_lib.lib().ai_paged_append_4bit, "ai_paged_append_4bit",
+           (key, value, k_pages, v_pages, k_scales, v_scales, page_table, lens, new_lens), "new_lens")
+
+
+def paged_read_4bit(k_pages: Tensor, v_pages: Tensor, k_scales: Tensor, v_scales: Tensor, page_table: Tensor, lens: Tensor,
+                    n_tokens: int, dtype: torch.dtype, read_lens: Optional[Tensor] = None) -> Tuple[Tensor, Tensor]:
+    """What the cache holds of each sequence's tokens ``lens[b] + t``, ``t <
+    n_tokens``: keys and values ``(B, Hkv, n_tokens, D)``, rounded to ``dtype``
+    (0 past ``read_lens[b]``, int32, and where there is no page).  The call that
+    mirrors ``paged_append_4bit``, with its arguments: what a prefill that wrote
+    to the cache attends to, or a sequence on its way to another cache."""
+    if page_table.dim() != 2 or k_pages.dim() != 4 or n_tokens < 1:
+        raise ValueError(f"page_table must be (B, max_pages), k_pages (n_pages, Hkv, page_size, D / 2), n_tokens 1 or more, "
+                         f"got {tuple(page_table.shape)}, {tuple(k_pages.shape)}, {n_tokens}")
+    shape = (page_table.shape[0], k_pages.shape[1], int(n_tokens), 2 * k_pages.shape[3])
+    k = torch.empty(shape, dtype=dtype, device=k_pages.device)
+    v = torch.empty(shape, dtype=dtype, device=k_pages.device)
+    _paged(_lib.lib().ai_paged_read_4bit, "ai_paged_read_4bit",
+           (k, v, k_pages, v_pages, k_scales, v_scales, page_table, lens, read_lens), "read_lens")
+    return k, v
+
+
+def _attend_plan(query, k_pages, v_pages, k_scales, v_scales, page_table, lens, query_lens, scaling):
+    """Checks the arguments; returns the tensors the kernels read and the
+    argument struct without pointers."""
+    index = _call.cuda_index("query", query)
+    if query.dim() != 4 or query.numel() == 0:
+        raise ValueError(f"query must be (B, Hq, T, D) and not empty, got {tuple(query.shape)}")
+    B, Hq, T, D = query.shape
+    _head_dim(D)
+    if query.dtype not in (torch.bfloat16, torch.float16):
+        raise TypeError(f"query must be bfloat16 or float16, got {query.dtype}")
+    if B > MAX_BATCH:
+        raise ValueError(f"at most {MAX_BATCH} sequences, got {B}: split the batch")
+    heads = k_pages.shape[1] if k_pages.dim() == 4 else 0
+    if heads == 0 or Hq % heads != 0:
+        raise ValueError(f"num_q_heads {Hq} is not a multiple of num_kv_heads {heads}")
+    a = _lib.AiPagedAttn4Args()
+    a.batch, a.num_q_heads, a.num_kv_heads, a.seq_len, a.head_dim = B, Hq, heads, T, D
+    a.dtype = _call.dtype_code(query, "query")
+    a.scale = scaling if scaling is not None else D ** -0.5
+    page_table = _pool(a.pool, k_pages, v_pages, k_scales, v_scales, page_table, B, heads, D, index)
+    lens = _call.ints("lens", lens, (B,), index)
+    if query_lens is not None:
+        query_lens = _call.ints("query_lens", query_lens, (B,), index)
+    q = _call.dense_d(query)
+    a.q = _call.strides4(q)
+    a.out = _lib.AiTensor4(None, T * Hq * D, D, Hq * D)
+    a.status = _call.status_ptr(index)
+    return (q, k_pages, v_pages, k_scales, v_scales, page_table, lens, query_lens), a
+
+
+def paged_attention_4bit(query: Tensor, k_pages: Tensor, v_pages: Tensor, k_scales: Tensor, v_scales: Tensor,
+                         page_table: Tensor, lens: Tensor, scaling: Optional[float] = None,
+                         query_lens: Optional[Tensor] = None, return_lse: bool = False):
+    """Attention of each sequence's new tokens over its cache in 4 bits.
+
+    ``query`` ``(B, Hq, T, D)`` (normalised and rotated, bfloat16 or float16):
+    query token ``t < query_lens[b]`` (all ``T`` without it) sees the first
+    ``lens[b] - query_lens[b] + t + 1`` keys of the pages in row ``b`` of
+    ``page_table``, so ``lens`` ``(B,)`` int32 counts the new tokens, already
+    appended.  Returns ``(B, T, Hq, D)`` (and the float32 log-sum-exp ``(B, Hq,
+    T)`` with ``return_lse``); a padding token, or one without a key, gives
+    zeros and ``-inf``.  ``scaling`` defaults to ``D ** -0.5``.
+
+    Keys and values are taken as the cache stands for them, exactly; sums and
+    the softmax are float32.  Slots that no query of the sequence sees may hold
+    anything.  Up to 4096 sequences, head_dim 32, 64 or 128, any strides of the
+    query; the pools as ``paged_append_4bit`` takes them.  A length or page out
+    of range is clamped and sets the status word.  There is no gradient: a
+    backward through the results raises."""
+    tensors = (query, k_pages, v_pages, k_scales, v_scales, page_table, lens, query_lens)
+    scaling = None if scaling is None else float(scaling)
+    at = (*map(_call.sig, tensors), scaling, _aligned(*tensors[1:5]))
+    plan = _ATTEND_PLANS.get(at)
+    if plan is None:
+        given = tensors
+        tensors, plan = _attend_plan(*given, scaling)
+        _ATTEND_PLANS.keep(at, given, tensors, plan)
+    if _call.tracked(query):
+        return _call.no_backward("paged_attention_4bit", lambda: _attend(plan, tensors, return_lse), query)
+    return _attend(plan, tensors, return_lse)
+
+
+def _attend(plan, tensors, return_lse):
+    q, *pools, lens, query_lens = tensors
+    B, Hq, T, D = q.shape
+    device = q.device
+    out = torch.empty((B, T, Hq, D), dtype=q.dtype, device=device)
+    a = _call.copy(plan)
+    a.q.ptr, a.out.ptr, a.lens = q.data_ptr(), out.data_ptr(), lens.data_ptr()
+    _point(a.pool, *pools)
+    if query_lens is not None:
+        a.query_lens = query_lens.data_ptr()
+    lse = None
+    if return_lse:
+        lse = torch.empty((B, Hq, T), dtype=torch.float32, device=device)
+        a.lse = lse.data_ptr()
+    lib = _lib.lib()
+    ws = _call.workspace(lib.ai_paged_attn_4bit_workspace, a, device, "ai_paged_attn_4bit_workspace")
+    _call.launch(lib.ai_paged_attn_4bit, a, q.get_device(), "ai_paged_attn_4bit")
+    del ws
+    return (out, lse) if return_lse else out

@@ -621,6 +621,176 @@ typedef struct AiVerifyArgs {
 int ai_verify_draft_workspace(const AiVerifyArgs* args, size_t* bytes);
 int ai_verify_draft(const AiVerifyArgs* args, void* stream);
 
+/* ------------------------------------------------------------------------
+ * Operators for rollouts and what is learnt from them: log-probabilities of
+ * given tokens, distillation from a teacher's likeliest tokens, and a paged
+ * cache held in 4 bits with the attention that reads it.
+ *
+ * Rows of logits are (b, t) of a (B, T, V) tensor with v contiguous; every row
+ * has its temperature, z = x / tau with tau = temperature[b] (NULL: 1).  A
+ * temperature that is not above zero counts as 1 and is AI_ERR_DEV_BOUNDS in
+ * the status word.  Logits are finite or -inf (masked); a row with a NaN or a
+ * +inf gives NaN.
+ * ------------------------------------------------------------------------ */
+
+/* Log-probability of a given token per row, the row's entropy and its top_k
+ * likeliest words:
+ *   logprob = z[token] - lse(z),  entropy = -sum_v p_v ln p_v,  p = softmax(z),
+ *   top: the words with the largest logits, best first, equal ones by index,
+ *   and their log-probabilities; -1 and -inf past the unmasked words.
+ * A row whose token is negative is padding: it is not read, its log-probability
+ * and entropy are 0, its list is empty; so is one whose token lies outside the
+ * vocabulary, which is AI_ERR_DEV_BOUNDS too.  A row without an unmasked word
+ * has the log-probability -inf, entropy 0 and an empty list; a row with a NaN
+ * has an empty list (its log-probabilities NaN). */
+#define AI_SCORE_MAX_TOP 128
+typedef struct AiScoreArgs {
+  int32_t batch;
+  int32_t seq_len;            /* T */
+  int32_t vocab;
+  int32_t dtype;              /* AiDtype of the logits */
+  const void* logits;         /* (B, T, V), v contiguous */
+  int64_t stride_b, stride_t;
+  const int64_t* tokens;      /* [B][T] */
+  const float* temperature;   /* [B], or NULL */
+  int32_t top_k;              /* 0 .. AI_SCORE_MAX_TOP */
+  float* logprobs;            /* [B][T] */
+  float* entropy;             /* [B][T], or NULL */
+  float* top_logprobs;        /* [B][T][top_k] */
+  int64_t* top_tokens;        /* [B][T][top_k] */
+  float* row_stats;           /* [B][T][4], 16-B aligned: what the backward needs; or NULL */
+  int32_t* status;
+} AiScoreArgs;
+
+/* Gradient of the logits for upstream gradients of logprobs, entropy and
+ * top_logprobs (each may be NULL: zero):
+ *   dx_v = (1 / tau) (g_l [v = token] + sum_k g_k [v = top_k]
+ *                     - p_v (g_l + sum_k g_k) - g_h p_v (ln p_v + entropy)),
+ * rounded once.  fwd.row_stats and fwd.top_tokens hold what the forward wrote
+ * (row_stats of a forward with `entropy`, where g_entropy is given); its other
+ * outputs are not read.  A padding row, one without an unmasked word and one
+ * whose upstream gradients are all zero has the gradient 0. */
+typedef struct AiScoreBwdArgs {
+  AiScoreArgs fwd;
+  const float* g_logprobs;    /* [B][T], or NULL */
+  const float* g_entropy;     /* [B][T], or NULL */
+  const float* g_top;         /* [B][T][top_k], or NULL */
+  void* dlogits;              /* (B, T, V) of the logits' type */
+  int64_t dstride_b, dstride_t;
+} AiScoreBwdArgs;
+
+int ai_token_logprobs(const AiScoreArgs* args, void* stream);
+int ai_token_logprobs_bwd(const AiScoreBwdArgs* args, void* stream);
+
+/* Kullback-Leibler divergence of a student's rows from a teacher whose n_top
+ * likeliest words are known per row (ids and their log-probabilities t_k), with
+ * q = softmax(z) over the whole vocabulary:
+ *   AI_TAIL_BUCKET       p_k = exp(t_k), and the other words as one: p_r = 1 - sum p_k (0 where that is
+ *                        below 2^-20, which rounding the t_k leaves),
+ *                        q_r = sum of q over them;
+ *                        L = sum_k p_k (t_k - ln q_k) + p_r (ln p_r - ln q_r);
+ *   AI_TAIL_RENORMALIZE  p = softmax(t), p_r = 0; L = sum_k p_k (ln p_k - ln q_k);
+ *   dx_v = (weight / tau) (M q_v - p_v) for a listed word, M = sum_k p_k + p_r,
+ *          (weight / tau) (M q_v - p_r q_v / q_r) for another.
+ * (The bucket is left out where no other word is unmasked.)  Entries with a
+ * negative id or t_k = -inf are left out, so lists may be shorter than n_top;
+ * ids outside the vocabulary and repeated ones (all but the first) are left out
+ * too, with AI_ERR_DEV_BOUNDS.  A row without an entry, and one of weight 0, is
+ * not read: loss and gradient 0.  A row without an unmasked word has the loss
+ * +inf and the gradient 0.  dlogits may be the logits' own memory (same
+ * strides). */
+#define AI_DISTILL_MAX_TOP 128
+enum AiTail { AI_TAIL_BUCKET = 0, AI_TAIL_RENORMALIZE = 1 };
+typedef struct AiDistillArgs {
+  int32_t batch;
+  int32_t seq_len;            /* T */
+  int32_t vocab;
+  int32_t dtype;              /* AiDtype of the logits */
+  const void* logits;         /* (B, T, V), v contiguous */
+  int64_t stride_b, stride_t;
+  int32_t n_top;              /* 1 .. AI_DISTILL_MAX_TOP */
+  int32_t tail;               /* AiTail */
+  const int64_t* top_tokens;  /* [B][T][n_top] */
+  const float* top_logprobs;  /* [B][T][n_top] */
+  const float* weights;       /* [B][T], or NULL: 1 */
+  const float* temperature;   /* [B], or NULL */
+  float* losses;              /* [B][T], without the weight; or NULL */
+  void* dlogits;              /* (B, T, V) of the logits' type, or NULL: losses alone */
+  int64_t dstride_b, dstride_t;
+  int32_t* status;
+} AiDistillArgs;
+
+int ai_distill(const AiDistillArgs* args, void* stream);
+
+/* A paged cache held in 4 bits.  Of a head row of D dims, the 32 dims of a
+ * group share an fp16 scale d, minus an eighth of their value of largest
+ * magnitude (the negative one of two; limited to fp16's range), and dim i has
+ * the code c = round(x_i / d) + 8 within 0 .. 15 (halves to even), which stands
+ * for (c - 8) d.  Where d is 0 every code is 8.  A group with a NaN or an
+ * infinity has the scale NaN.  Pools: codes (n_pages, Hkv, page_size, D / 2)
+ * bytes, scales (n_pages, Hkv, page_size, D / 32) fp16.  Dim 32 c + 4 g + j (g <
+ * 8, j < 4) of a row lies in its byte g D / 16 + 2 c + j / 2, in the low half
+ * for even j.  Strides of the pools are in elements (bytes, halfs); code rows
+ * start on 16-byte boundaries, scale rows on boundaries of their size. */
+typedef struct AiPool4 {
+  AiTensor4 k_codes, v_codes;   /* (n_pages, Hkv, page_size, D / 2) uint8 */
+  AiTensor4 k_scales, v_scales; /* (n_pages, Hkv, page_size, D / 32) fp16 */
+  int32_t n_pages;
+  int32_t page_size;            /* a power of two from 16 */
+  const int32_t* page_table;    /* [B][max_pages] */
+  int64_t page_table_stride;
+  int32_t max_pages;
+} AiPool4;
+
+/* ai_paged_append_4bit: token t < n[b] (n NULL: all T) of sequence b becomes its token
+ * lens[b] + t.  ai_paged_read_4bit: the same tokens' values come back, rounded
+ * to dtype; tokens past n[b], or whose page is out of range, read as 0.  A token
+ * whose page is outside the table or the pool is skipped with
+ * AI_ERR_DEV_BOUNDS; n outside [0, T] is AI_ERR_DEV_BOUNDS too and counts as
+ * the nearest within. */
+typedef struct AiPaged4Args {
+  int32_t batch;
+  int32_t seq_len;            /* T */
+  int32_t num_kv_heads;
+  int32_t head_dim;           /* 32, 64 or 128 */
+  int32_t dtype;              /* AiDtype of k and v */
+  AiTensor4 k, v;             /* (B, Hkv, T, D) */
+  AiPool4 pool;
+  const int32_t* lens;        /* [B] */
+  const int32_t* n;           /* [B], or NULL */
+  int32_t* status;
+} AiPaged4Args;
+
+int ai_paged_append_4bit(const AiPaged4Args* args, void* stream);
+int ai_paged_read_4bit(const AiPaged4Args* args, void* stream);
+
+/* Attention over such a cache: query token t < n_b = query_lens[b] of sequence
+ * b sees the first lens[b] - n_b + t + 1 keys of its pages (lens counts the new
+ * tokens, already appended).  Padding tokens (t >= n_b) and tokens without a
+ * key give 0 (lse -inf).  Slots that no query of the sequence sees may hold
+ * anything, also within a page. */
+typedef struct AiPagedAttn4Args {
+  int32_t batch;              /* up to 4096 */
+  int32_t seq_len;            /* T: query tokens per sequence */
+  int32_t num_q_heads;
+  int32_t num_kv_heads;
+  int32_t head_dim;           /* 32, 64 or 128 */
+  int32_t dtype;              /* AI_DTYPE_BF16 or AI_DTYPE_F16 */
+  float scale;
+  AiTensor4 q;                /* (B, Hq, T, D) */
+  AiTensor4 out;              /* (B, Hq, T, D) view */
+  float* lse;                 /* (B, Hq, T) natural log, or NULL */
+  AiPool4 pool;
+  const int32_t* lens;        /* [B] */
+  const int32_t* query_lens;  /* [B], or NULL: T for every sequence */
+  int32_t* status;
+  void* workspace;            /* ai_paged_attn_4bit_workspace bytes, 256-B aligned */
+  size_t workspace_bytes;
+} AiPagedAttn4Args;
+
+int ai_paged_attn_4bit_workspace(const AiPagedAttn4Args* args, size_t* bytes);
+int ai_paged_attn_4bit(const AiPagedAttn4Args* args, void* stream);
+
 /* Synchronises the stream, copies the device status word to *host_out and
  * resets it to AI_OK.  For tests and debugging; not needed on the hot path. */
 int ai_attn_read_status(int32_t* dev_status, void* stream, int32_t* host_out);
@@ -663,7 +833,11 @@ typedef enum AiProfKind {
   AI_PROF_APPEND = 10,  /* paged cache append */
   AI_PROF_PREFIX = 11,  /* shared-prefix attention (split + combine) */
   AI_PROF_VERIFY = 12,  /* draft verification */
-  AI_PROF_ALL_KINDS = 13
+  AI_PROF_SCORE = 13,   /* token log-probabilities, forward and backward */
+  AI_PROF_DISTILL = 14, /* distillation */
+  AI_PROF_PAGED4 = 15,  /* append to and read from the cache in 4 bits */
+  AI_PROF_ATTN4 = 16,   /* attention over it (split + combine) */
+  AI_PROF_ALL_KINDS = 17
 } AiProfKind;
 int ai_attn_profile_enable(int on);
 int ai_attn_profile_read(float* ms_by_kind, int32_t* launches_by_kind);
