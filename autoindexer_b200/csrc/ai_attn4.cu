@@ -1,10 +1,33 @@
-// Attention over the paged cache in 4 bits (declared in include/ai_attn.h).
+// Attention over the paged cache in 4 bits (declared in include/ai_attn.h; the
+// format at AiPool4).
 //
-// A warp per query row, fp32 arithmetic: a lane per key forms its score, a lane
-// per D / 32 dims adds the weighted values.
+// A unit is a (sequence, KV head, group of up to 32 query rows); its keys are
+// cut into tiles of 32, the tiles of all units stand in one line, and each worker,
+// a warp, takes an equal stretch of the line, whatever the lengths are (they
+// are read on the device).  The rows of a unit that a worker touched leave
+// partial results (O / l in fp32 and the log2-sum), which a second launch joins.
+//
+// A warp's tile, on 16 x 8 x 16 fp16 matrix instructions with fp32 sums:
+//   S^T = K Q^T   K's codes are exact in fp16 as 64 + c (one logical operation a
+//                 pair of codes); the sums of a group of 32 dims start at -72
+//                 sum(q), which makes them those of c - 8, and meet the group's
+//                 scale in fp32.  bf16 queries are scaled per row by a power of
+//                 two into fp16's range.
+//   O^T += V^T P  V's codes as c - 8; P takes each key's V scale in fp32, per group
+//                 of 32 dims, and is rounded once, to fp16.  P is held 2^7 above
+//                 1 for the largest |scale| met so far, so that it fits fp16 and
+//                 weights down to 2^-31 of the largest count.
+// Both products have the tile's keys on the instruction's long side, so up to 8
+// query rows of a KV head cost one column block.
+//
+// HBM-bound when few rows meet each key: 144 bytes per token and KV head at D 128.
 
+#include <cuda_fp16.h>
 #include <cuda_runtime.h>
 #include <math_constants.h>
+
+#include <cstring>
+#include <type_traits>
 
 #include "ai_common.cuh"
 #include "ai_kernels.h"
@@ -15,77 +38,629 @@ namespace ai {
 namespace attn4 {
 
 using namespace kv4;
-constexpr int kWarps = 4, kThreads = 32 * kWarps;
 
-template <typename T, int D>
-__global__ void __launch_bounds__(kThreads) rows_kernel(const AiPagedAttn4Args a) {
-  constexpr int C = D / kGroup;
-  __shared__ float s_q[kWarps][D];
-  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
-  const int64_t row = (int64_t)blockIdx.x * kWarps + warp;
-  if (row >= (int64_t)a.batch * a.num_q_heads * a.seq_len) return;
-  const int t = (int)(row % a.seq_len), h = (int)(row / a.seq_len % a.num_q_heads);
-  const int64_t b = row / a.seq_len / a.num_q_heads;
-  const int64_t hk = h / (a.num_q_heads / a.num_kv_heads);
-  T* out = static_cast<T*>(const_cast<void*>(a.out.ptr)) + b * a.out.stride_b + h * a.out.stride_h + t * a.out.stride_t;
-  const int n = new_tokens(a.query_lens, b, a.seq_len, a.status);
-  int keys = __ldg(a.lens + b);
-  const int64_t most = (int64_t)a.pool.max_pages * a.pool.page_size;
-  if (keys < 0 || keys > most) report(a.status, AI_ERR_DEV_BOUNDS);
-  keys = max(0, (int)min((int64_t)keys, most));
-  const int seen = t < n ? max(0, keys - n + t + 1) : 0;
-  const T* q = static_cast<const T*>(a.q.ptr) + b * a.q.stride_b + h * a.q.stride_h + t * a.q.stride_t;
-  for (int i = lane; i < D; i += 32) s_q[warp][i] = to_f32(q[i]);
-  __syncwarp();
-  float m = -CUDART_INF_F, l = 0.f, o[C] = {};
-  for (int k0 = 0; k0 < seen; k0 += 32) {
-    const int key = k0 + lane;
-    float s = -CUDART_INF_F;
-    Place p{0, 0};
-    if (key < seen) {
-      p = place(a.pool, b, key);
-      if (p.page < 0) report(a.status, AI_ERR_DEV_BOUNDS), p.page = 0;
-      const AiTensor4 &cd = a.pool.k_codes, &sc = a.pool.k_scales;
-      const uint8_t* co = static_cast<const uint8_t*>(cd.ptr) + p.page * cd.stride_b + hk * cd.stride_h + p.slot * cd.stride_t;
-      const __half* so = static_cast<const __half*>(sc.ptr) + p.page * sc.stride_b + hk * sc.stride_h + p.slot * sc.stride_t;
-      s = 0.f;
-      for (int c = 0; c < C; ++c) {
-        float part = 0.f;
-        for (int g = 0; g < 8; ++g)
-          for (int j = 0; j < 4; ++j)
-            part += (float)((co[g * 2 * C + 2 * c + j / 2] >> (4 * (j % 2)) & 15) - 8) * s_q[warp][32 * c + 4 * g + j];
-        s += part * __half2float(so[c]);
-      }
-      s *= a.scale;
+constexpr int kMaxBatch = 2048;  // a scan of the sequences sits in shared memory
+constexpr int kKeys = 32;      // keys of a tile
+constexpr int kStart = 2;      // what starting a unit costs, in tiles
+constexpr int kLeast = 4;      // positions a worker takes, at least
+constexpr int kMaxBlocks = 4;  // column blocks (of 8 query rows) of a unit, at most
+constexpr float kLift = 7.f;   // P at a weight of 1 and the largest |scale|: 2^7
+constexpr float kSlack = 8.f;  // the running maximum moves when a score passes it by 2^8
+
+// Warps of a CTA (one per SM) and tiles of a warp's ring.
+__host__ __device__ constexpr int warps_of(int blocks) { return blocks <= 2 ? 12 : 8; }
+constexpr int kStages = 4;
+
+// A tile in shared memory: codes of K and V, scales of K and V.
+template <int D>
+struct Tile {
+  static constexpr int C = D / kGroup, kRow = D / 2, kCodes = kKeys * kRow, kScales = kKeys * C * 2;
+  static constexpr int K = 0, V = kCodes, KS = 2 * kCodes, VS = KS + kScales, kBytes = VS + kScales;
+  // V's rows stand so that the four keys which a quarter of a warp reads
+  // together are neighbours (keys 2 t of eight, then 2 t + 1), and at D 128 their
+  // 16-byte pieces in halves of the row that do not share banks.
+  __device__ static int v_row(int key) { return (key & 24) | ((key & 1) << 2) | ((key >> 1) & 3); }
+  __device__ static int v_piece(int row, int piece) { return D == 128 ? piece ^ (row & 2) : piece; }
+};
+
+static_assert(warps_of(1) * kStages * Tile<128>::kBytes + 4 * (kMaxBatch + 1) <= 227 * 1024, "a CTA's shared memory");
+
+struct Plan {
+  int group;       // G: query heads per KV head
+  int rows;        // T G
+  int groups;      // groups of query rows per (sequence, KV head)
+  int unit_rows;   // rows of a unit (the last group may have fewer)
+  int blocks;      // column blocks of a unit
+  int workers;
+  float* part_o;   // [units + workers][unit_rows][D]
+  float* part_lse;
+  int* scan;       // [B + 1] positions before each sequence, per unit
+};
+
+struct Lens {
+  int keys, n;
+};
+
+// Keys of a sequence (clamped to what its page table can hold) and its real
+// query tokens.
+__device__ __forceinline__ Lens seq_lens(const AiPagedAttn4Args& a, int64_t b) {
+  Lens r;
+  r.keys = __ldg(a.lens + b);
+  r.n = new_tokens(a.query_lens, b, a.seq_len, a.status);
+  const int64_t most = min((int64_t)a.pool.max_pages * a.pool.page_size, (int64_t)0x7fffffff);
+  if (r.keys < 0 || r.keys > most) report(a.status, AI_ERR_DEV_BOUNDS);
+  r.keys = max(0, (int)min((int64_t)r.keys, most));
+  return r;
+}
+
+// Positions of a sequence's unit: its tiles behind `kStart` idle positions; none
+// without a key or a query.
+__device__ __forceinline__ int unit_size(const Lens& l) { return l.keys > 0 && l.n > 0 ? kStart + (l.keys - 1) / kKeys + 1 : 0; }
+
+// The line's stretches: n workers, none less than kLeast positions unless the
+// line is shorter; the first `more` take one position more.
+struct Split {
+  int n, len, more;
+  __device__ __forceinline__ int begin(int w) const { return w * len + min(w, more); }
+  __device__ __forceinline__ int worker(int x) const {
+    const int head = more * (len + 1);
+    return x < head ? x / (len + 1) : more + (x - head) / len;
+  }
+};
+
+__device__ __forceinline__ Split split_line(int workers, int total) {
+  Split s{0, 1, 0};
+  if (total > 0) {
+    s.n = min(workers, (total + kLeast - 1) / kLeast);
+    s.len = total / s.n;
+    s.more = total - s.len * s.n;
+  }
+  return s;
+}
+
+// A worker's stretch within one unit: tiles [tile, end) of it.
+struct Seg {
+  int unit, b, hk, grp;
+  int tile, end;
+  int keys, n;
+};
+
+// The next stretch with tiles from position w on; false: there is none.
+__device__ __forceinline__ bool next_seg(const AiPagedAttn4Args& a, const Plan& p, const int* scan, int& w, int w1, Seg& s) {
+  const int per = a.num_kv_heads * p.groups;
+  while (w < w1) {
+    int lo = 0, hi = a.batch - 1;  // the last sequence that starts by w (it has positions)
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) / 2;
+      if (scan[mid] * per <= w)
+        lo = mid;
+      else
+        hi = mid - 1;
     }
-    float top = s;
-    for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-    top = fmaxf(top, m);
-    const float base = top == -CUDART_INF_F ? 0.f : top, e = key < seen ? expf(s - base) : 0.f;
-    const float down = m == -CUDART_INF_F ? 0.f : expf(m - base);
-    float sum = e;
-    for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-    l = l * down + sum;
-    m = top;
-    for (int c = 0; c < C; ++c) o[c] *= down;
-    for (int j = 0; j < min(32, seen - k0); ++j) {
-      const float w = __shfl_sync(0xffffffffu, e, j);
-      const int64_t page = __shfl_sync(0xffffffffu, p.page, j), slot = __shfl_sync(0xffffffffu, p.slot, j);
-      const AiTensor4 &cd = a.pool.v_codes, &sc = a.pool.v_scales;
-      const uint8_t* co = static_cast<const uint8_t*>(cd.ptr) + page * cd.stride_b + hk * cd.stride_h + slot * cd.stride_t;
-      const __half* so = static_cast<const __half*>(sc.ptr) + page * sc.stride_b + hk * sc.stride_h + slot * sc.stride_t;
-      for (int c = 0; c < C; ++c)  // (dim 32 c + lane)
-        o[c] += w * ((float)((co[lane / 4 * 2 * C + 2 * c + lane % 4 / 2] >> (4 * (lane % 2)) & 15) - 8) * __half2float(so[c]));
+    const int size = scan[lo + 1] - scan[lo], rem = w - scan[lo] * per, sub = rem / size, at = rem - sub * size;
+    const int end = min(size, at + (w1 - w));
+    w += end - at;
+    s.tile = max(0, at - kStart);
+    s.end = end - kStart;
+    if (s.tile >= s.end) continue;
+    s.b = lo;
+    s.hk = sub / p.groups;
+    s.grp = sub - s.hk * p.groups;
+    s.unit = lo * per + sub;
+    const Lens l = seq_lens(a, lo);
+    s.keys = l.keys;
+    s.n = l.n;
+    return true;
+  }
+  return false;
+}
+
+__device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// An 8 x 8 matrix of 16-bit elements, a row of pairs per four lanes, transposed.
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+  uint32_t y;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+
+// Copies `N` bytes to shared memory, zeros where there is nothing to copy.
+template <int N>
+__device__ __forceinline__ void copy_async(uint32_t dst, const void* src, bool some) {
+  if constexpr (N == 16)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(some ? 16 : 0) : "memory");
+  else
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(N), "r"(some ? N : 0) : "memory");
+}
+
+// Lower (or upper) halves of two words, side by side.
+__device__ __forceinline__ uint32_t halves(uint32_t a, uint32_t b, bool upper) { return __byte_perm(a, b, upper ? 0x7632 : 0x5410); }
+
+// Words of a lane's codes by N bytes from shared memory.
+template <int N>
+__device__ __forceinline__ void lds(uint32_t (&w)[(N + 3) / 4], const uint8_t* p) {
+  if constexpr (N == 16) {
+    const uint4 r = *reinterpret_cast<const uint4*>(p);
+    w[0] = r.x, w[1] = r.y, w[2] = r.z, w[3] = r.w;
+  } else if constexpr (N == 8) {
+    const uint2 r = *reinterpret_cast<const uint2*>(p);
+    w[0] = r.x, w[1] = r.y;
+  } else if constexpr (N == 4) {
+    w[0] = *reinterpret_cast<const uint32_t*>(p);
+  } else {
+    w[0] = *reinterpret_cast<const uint16_t*>(p);
+  }
+}
+
+// Four pairs of codes (at bits 4 j and 16 + 4 j) as fp16 64 + c ...
+__device__ __forceinline__ uint32_t biased(uint32_t x, int j) {
+  const uint32_t s = j == 0 ? x << 4 : x >> (4 * (j - 1));
+  return (s & 0x00f000f0u) | 0x54005400u;
+}
+// ... and as c - 8.
+__device__ __forceinline__ uint32_t centred(uint32_t x, int j) {
+  const uint32_t s = j < 2 ? x : x >> 8;
+  const uint32_t f = j % 2 == 0 ? (s & 0x000f000fu) | 0x64006400u : (s & 0x00f000f0u) | 0x54005400u;
+  const __half2 off = j % 2 == 0 ? __half2half2(__ushort_as_half(0x6408)) : __half2half2(__ushort_as_half(0x5480));
+  const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&f), off);
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// Eight elements of a query row, any strides of the rows.
+template <typename T>
+__device__ __forceinline__ void load_q(const T* p, float (&f)[8]) {
+  if ((reinterpret_cast<uintptr_t>(p) & 15) == 0) {
+    const uint4 r = __ldg(reinterpret_cast<const uint4*>(p));
+    T e[8];
+    memcpy(e, &r, 16);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] = to_f32(e[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] = to_f32(p[i]);
+  }
+}
+
+template <typename T, int D, int NT>
+__global__ void __launch_bounds__(32 * warps_of(NT), 1) split_kernel(const AiPagedAttn4Args a, const Plan p) {
+  using L = Tile<D>;
+  constexpr int C = L::C, W = warps_of(NT);
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  extern __shared__ __align__(128) uint8_t smem[];
+  int* scan = reinterpret_cast<int*>(smem + W * kStages * L::kBytes);
+  const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, g = lane / 4, t = lane % 4;
+  if (warp == 0) {
+    int base = 0;
+    for (int b0 = 0; b0 < a.batch; b0 += 32) {
+      const int b = b0 + lane;
+      int v = b < a.batch ? unit_size(seq_lens(a, b)) : 0;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int u = __shfl_up_sync(0xffffffffu, v, o);
+        if (lane >= o) v += u;
+      }
+      if (b < a.batch) scan[b + 1] = base + v;
+      base += __shfl_sync(0xffffffffu, v, 31);
+    }
+    if (lane == 0) scan[0] = 0;
+  }
+  __syncthreads();
+  if (blockIdx.x == 0)
+    for (int b = tid; b <= a.batch; b += blockDim.x) p.scan[b] = scan[b];
+  const Split line = split_line(p.workers, scan[a.batch] * a.num_kv_heads * p.groups);
+  const int worker = warp * gridDim.x + blockIdx.x;  // (few workers: on as many SMs)
+  if (worker >= line.n) return;
+  const int w0 = line.begin(worker), w1 = line.begin(worker + 1);
+  uint8_t* ring = smem + warp * kStages * L::kBytes;
+
+  // ---- loads, `kStages - 1` tiles ahead of what is computed
+  const int page_bits = 31 - __clz(a.pool.page_size), page_mask = a.pool.page_size - 1;
+  Seg ld;
+  int wl = w0, page[2] = {0, 0};
+  auto look_up = [&]() {  // pages of the tile's halves
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int key = ld.tile * kKeys + 16 * h;
+      page[h] = 0;
+      if (key < ld.keys) {
+        page[h] = __ldg(a.pool.page_table + ld.b * a.pool.page_table_stride + (key >> page_bits));
+        if (page[h] < 0 || page[h] >= a.pool.n_pages) report(a.status, AI_ERR_DEV_BOUNDS), page[h] = 0;
+      }
+    }
+  };
+  bool loads = next_seg(a, p, scan, wl, w1, ld);
+  if (loads) look_up();
+  uint16_t held[2] = {0, 0};  // D 32: scales on their way (two bytes are no copy)
+  int held_at = -1;
+  auto issue = [&](int stage) {
+    if constexpr (D == 32) {
+      if (held_at >= 0) {
+        uint8_t* dst = ring + held_at * L::kBytes;
+        reinterpret_cast<uint16_t*>(dst + L::KS)[lane] = held[0];
+        reinterpret_cast<uint16_t*>(dst + L::VS)[lane] = held[1];
+        held_at = -1;
+      }
+    }
+    if (loads) {
+      uint8_t* dst = ring + stage * L::kBytes;
+      const uint32_t to = ptx::smem_u32(dst);
+      const int k0 = ld.tile * kKeys, left = ld.keys - k0;
+      constexpr int P = L::kRow / 16;  // 16-byte pieces of a row
+#pragma unroll
+      for (int i = 0; i < P; ++i) {
+        const int at = i * 32 + lane, key = at / P, piece = at % P, h = key / 16;
+        const int64_t pg = h ? page[1] : page[0], slot = (k0 + key) & page_mask;
+        const bool some = key < left;
+        const uint8_t* k = static_cast<const uint8_t*>(a.pool.k_codes.ptr) + pg * a.pool.k_codes.stride_b +
+                           ld.hk * a.pool.k_codes.stride_h + slot * a.pool.k_codes.stride_t + 16 * piece;
+        const uint8_t* v = static_cast<const uint8_t*>(a.pool.v_codes.ptr) + pg * a.pool.v_codes.stride_b +
+                           ld.hk * a.pool.v_codes.stride_h + slot * a.pool.v_codes.stride_t + 16 * piece;
+        const int row = L::v_row(key);
+        copy_async<16>(to + L::K + key * L::kRow + 16 * piece, k, some);
+        copy_async<16>(to + L::V + row * L::kRow + 16 * L::v_piece(row, piece), v, some);
+      }
+      {
+        const int64_t pg = lane < 16 ? page[0] : page[1], slot = (k0 + lane) & page_mask;
+        const bool some = lane < left;
+        const __half* k = static_cast<const __half*>(a.pool.k_scales.ptr) + pg * a.pool.k_scales.stride_b +
+                          ld.hk * a.pool.k_scales.stride_h + slot * a.pool.k_scales.stride_t;
+        const __half* v = static_cast<const __half*>(a.pool.v_scales.ptr) + pg * a.pool.v_scales.stride_b +
+                          ld.hk * a.pool.v_scales.stride_h + slot * a.pool.v_scales.stride_t;
+        if constexpr (D == 32) {
+          held[0] = some ? __ldg(reinterpret_cast<const uint16_t*>(k)) : (uint16_t)0;
+          held[1] = some ? __ldg(reinterpret_cast<const uint16_t*>(v)) : (uint16_t)0;
+          held_at = stage;
+        } else {
+          copy_async<2 * C>(to + L::KS + lane * 2 * C, k, some);
+          copy_async<2 * C>(to + L::VS + lane * 2 * C, v, some);
+        }
+      }
+      if (++ld.tile == ld.end) loads = next_seg(a, p, scan, wl, w1, ld);
+      if (loads) look_up();
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+#pragma unroll
+  for (int s = 0; s < kStages - 1; ++s) issue(s);
+
+  // ---- products
+  int wc = w0, st = 0;
+  Seg s;
+  while (next_seg(a, p, scan, wc, w1, s)) {
+    const int row0 = s.grp * p.unit_rows, n_rows = min(p.rows - row0, p.unit_rows);
+    // Query fragments: lane (g, t) has dims 32 c + 8 t + {0 .. 7} of row 8 nt + g.
+    uint32_t q[NT][C][4];
+    float q_off[NT][C][2];            // -72 sum(q) of rows 2 t and 2 t + 1, per group
+    float slope[NT][2];               // of the scores, in units of log 2
+    int seen[NT][2];                  // keys that those rows see; -1: no query
+    int least = 0x7fffffff;           // tiles that end by it are seen whole
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const int i = 8 * nt + g;
+      const bool has = i < n_rows;
+      const int r = has ? row0 + i : row0, tok = r / p.group, head = s.hk * p.group + r - tok * p.group;
+      const T* src = static_cast<const T*>(a.q.ptr) + s.b * a.q.stride_b + head * a.q.stride_h + tok * a.q.stride_t + 8 * t;
+      float f[C][8], top = 0.f;
+#pragma unroll
+      for (int c = 0; c < C; ++c) {
+        load_q(src + kGroup * c, f[c]);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          if (!has) f[c][e] = 0.f;
+          top = fmaxf(top, fabsf(f[c][e]));
+        }
+      }
+      int up = 0;
+      if constexpr (sizeof(T) == 2 && !std::is_same<T, __half>::value) {
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        if (top > 0.f && top < CUDART_INF_F) up = 14 - ilogbf(top);
+      }
+      const float slope_g = ldexpf(a.scale * kLog2e, -up);
+#pragma unroll
+      for (int c = 0; c < C; ++c) {
+        __half2 h[4];
+        float sum = 0.f;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {  // (dims 8 t + e and 8 t + 4 + e are a pair)
+          h[e] = __floats2half2_rn(ldexpf(f[c][e], up), ldexpf(f[c][4 + e], up));
+          const float2 back = __half22float2(h[e]);
+          sum += back.x + back.y;
+        }
+        memcpy(q[nt][c], h, 16);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+#pragma unroll
+        for (int e = 0; e < 2; ++e) q_off[nt][c][e] = -72.f * __shfl_sync(0xffffffffu, sum, 4 * (2 * t + e));
+      }
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        slope[nt][e] = __shfl_sync(0xffffffffu, slope_g, 4 * (2 * t + e));
+        const int i2 = 8 * nt + 2 * t + e, tok2 = (row0 + i2) / p.group;
+        seen[nt][e] = i2 < n_rows && tok2 < s.n ? max(0, s.keys - s.n + tok2 + 1) : -1;
+        if (seen[nt][e] >= 0) least = min(least, seen[nt][e]);
+      }
+    }
+    least = min(least, __shfl_xor_sync(0xffffffffu, least, 1));
+    least = min(least, __shfl_xor_sync(0xffffffffu, least, 2));
+
+    float o[NT][2 * C][4];
+    float m[NT][2], ref[NT][2], l[NT][2], l_before[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+      for (int i = 0; i < 2 * C; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[nt][i][e] = 0.f;
+#pragma unroll
+      for (int e = 0; e < 2; ++e) m[nt][e] = -CUDART_INF_F, ref[nt][e] = l[nt][e] = l_before[nt][e] = 0.f;
+    }
+    // The largest |V scale| so far is at most 2^v_exp (v_lim in both halves; the
+    // first one above 0 sets them).
+    int v_exp = -24;
+    uint32_t v_lim = 0;
+
+    for (int tile = s.tile; tile < s.end; ++tile) {
+      asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
+      __syncwarp();
+      issue((st + kStages - 1) % kStages);
+      const uint8_t* sm = ring + st * L::kBytes;
+      st = st + 1 == kStages ? 0 : st + 1;
+      const int k0 = tile * kKeys;
+      const bool ragged = k0 + kKeys > least;
+
+      // Scores: keys 16 mt + g (e = 0, 1) and 16 mt + g + 8 (2, 3), rows 2 t + e % 2.
+      float sc[2][NT][4];
+      uint32_t vs[2][2][(C + 1) / 2];
+#pragma unroll
+      for (int mt = 0; mt < 2; ++mt) {
+        uint32_t kw[2][C];
+        float ks[2][C];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int key = 16 * mt + 8 * h + g;
+          lds<4 * C>(kw[h], sm + L::K + key * L::kRow + 4 * C * t);
+          uint32_t raw[(C + 1) / 2];
+          lds<2 * C>(raw, sm + L::KS + key * 2 * C);
+#pragma unroll
+          for (int c = 0; c < C; ++c)
+            ks[h][c] = __half2float(__ushort_as_half((unsigned short)(raw[c / 2] >> (16 * (c % 2)))));
+          lds<2 * C>(vs[mt][h], sm + L::VS + key * 2 * C);
+        }
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) sc[mt][nt][e] = 0.f;
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+          uint32_t x[2];
+#pragma unroll
+          for (int h = 0; h < 2; ++h) x[h] = C == 1 ? kw[h][0] : halves(kw[h][c / 2], kw[h][(C + c) / 2], c % 2);
+          uint32_t f[2][4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) f[0][j] = biased(x[0], j), f[1][j] = biased(x[1], j);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            float acc[4] = {q_off[nt][c][0], q_off[nt][c][1], q_off[nt][c][0], q_off[nt][c][1]};
+            mma(acc, f[0][0], f[1][0], f[0][1], f[1][1], q[nt][c][0], q[nt][c][1]);
+            mma(acc, f[0][2], f[1][2], f[0][3], f[1][3], q[nt][c][2], q[nt][c][3]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) sc[mt][nt][e] = fmaf(ks[e / 2][c], acc[e], sc[mt][nt][e]);
+          }
+        }
+      }
+      // The running maximum of each row, lazily.
+      bool move = false;
+      float top[NT][2];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+        for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            sc[mt][nt][e] *= slope[nt][e % 2];
+            if (ragged && k0 + 16 * mt + 8 * (e / 2) + g >= seen[nt][e % 2]) sc[mt][nt][e] = -CUDART_INF_F;
+          }
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          top[nt][e] = fmaxf(ptx::fmax3(sc[0][nt][e], sc[0][nt][2 + e], sc[1][nt][e]), sc[1][nt][2 + e]);
+          move |= top[nt][e] > m[nt][e] + kSlack;
+        }
+      }
+      __half2 big = __half2half2(__ushort_as_half(0));
+#pragma unroll
+      for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int i = 0; i < (C + 1) / 2; ++i) big = __hmax2(big, __habs2(*reinterpret_cast<const __half2*>(&vs[mt][h][i])));
+      move |= !__hble2(big, *reinterpret_cast<const __half2*>(&v_lim));
+      if (__any_sync(0xffffffffu, move)) {
+        // (an infinite scale makes what it meets infinite; it has no part in the bound)
+        float mine = 0.f;
+#pragma unroll
+        for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int c = 0; c < C; ++c) {
+              const float d = fabsf(__half2float(__ushort_as_half((unsigned short)(vs[mt][h][c / 2] >> (16 * (c % 2))))));
+              if (d < CUDART_INF_F) mine = fmaxf(mine, d);
+            }
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) mine = fmaxf(mine, __shfl_xor_sync(0xffffffffu, mine, d));
+        float down = 1.f;
+        if (mine > 0.f) {
+          const int e = ilogbf(mine) + 1;
+          if (e > v_exp) {
+            down = ptx::ex2((float)(v_exp - e));
+            v_exp = e;
+            const uint32_t h = e > 15 ? 0x7bffu : __half_as_ushort(__float2half_rn(ptx::ex2((float)e)));
+            v_lim = h | h << 16;
+          }
+        }
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float x = top[nt][e], alpha = down;
+#pragma unroll
+            for (int d = 4; d < 32; d <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, d));
+            if (x > m[nt][e] + kSlack) {
+              if (m[nt][e] != -CUDART_INF_F) alpha *= ptx::ex2(m[nt][e] - x);
+              m[nt][e] = x;
+            }
+            ref[nt][e] = (m[nt][e] == -CUDART_INF_F ? 0.f : m[nt][e]) + ((float)v_exp - kLift);
+            l[nt][e] *= alpha;
+            l_before[nt][e] *= alpha;
+#pragma unroll
+            for (int i = 0; i < 2 * C; ++i) o[nt][i][e] *= alpha, o[nt][i][2 + e] *= alpha;
+          }
+      }
+      // Weights, and per group of dims the weights times the V scales as the
+      // second product takes them: lane (g, t) keys 2 t, 2 t + 1 (and + 8) of row g.
+#pragma unroll
+      for (int mt = 0; mt < 2; ++mt) {
+        uint32_t pv[NT][C][2];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          float w[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) w[e] = ptx::ex2(sc[mt][nt][e] - ref[nt][e % 2]);
+#pragma unroll
+          for (int e = 0; e < 2; ++e) l[nt][e] += w[e] + w[2 + e];
+#pragma unroll
+          for (int c = 0; c < C; ++c)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const float d = __half2float(__ushort_as_half((unsigned short)(vs[mt][h][c / 2] >> (16 * (c % 2)))));
+              float2 x = __fmul2_rn(make_float2(w[2 * h], w[2 * h + 1]), make_float2(d, d));
+              if (ragged) {  // (a key that the row does not see may have any scale)
+                if (sc[mt][nt][2 * h] == -CUDART_INF_F) x.x = 0.f;
+                if (sc[mt][nt][2 * h + 1] == -CUDART_INF_F) x.y = 0.f;
+              }
+              pv[nt][c][h] = transpose8(pack2(x.x, x.y));
+            }
+        }
+        uint32_t vw[4][(C + 1) / 2];  // keys 2 t, 2 t + 1, 2 t + 8, 2 t + 9
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int row = 16 * mt + 4 * i + t;
+          if constexpr (D == 128)
+            lds<8>(vw[i], sm + L::V + row * L::kRow + 16 * L::v_piece(row, g / 2) + 8 * (g % 2));
+          else
+            lds<2 * C>(vw[i], sm + L::V + row * L::kRow + 2 * C * g);
+        }
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+          const uint32_t z0 = halves(vw[0][c / 2], vw[1][c / 2], c % 2), z1 = halves(vw[2][c / 2], vw[3][c / 2], c % 2);
+          uint32_t f[2][4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) f[0][j] = centred(z0, j), f[1][j] = centred(z1, j);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            mma(o[nt][2 * c], f[0][0], f[0][1], f[1][0], f[1][1], pv[nt][c][0], pv[nt][c][1]);
+            mma(o[nt][2 * c + 1], f[0][2], f[0][3], f[1][2], f[1][3], pv[nt][c][0], pv[nt][c][1]);
+          }
+        }
+      }
+      // (a sum of sums: one running sum of a long list would round its small weights away)
+      if (tile % 16 == 15) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) l_before[nt][e] += l[nt][e], l[nt][e] = 0.f;
+      }
+    }
+    // Partial rows: dims 32 c + 4 g + {0 .. 3} of rows 2 t and 2 t + 1.
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        float sum = l_before[nt][e] + l[nt][e];
+#pragma unroll
+        for (int d = 4; d < 32; d <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+        if (seen[nt][e] <= 0) continue;
+        const int64_t row = (int64_t)(s.unit + worker) * p.unit_rows + 8 * nt + 2 * t + e;
+        const float inv = sum == 0.f ? 0.f : 1.f / sum;
+#pragma unroll
+        for (int c = 0; c < C; ++c)
+          *reinterpret_cast<float4*>(p.part_o + row * D + kGroup * c + 4 * g) =
+              make_float4(o[nt][2 * c][e] * inv, o[nt][2 * c][2 + e] * inv, o[nt][2 * c + 1][e] * inv, o[nt][2 * c + 1][2 + e] * inv);
+        // (NaN among the scores: +inf, which makes the joined row NaN)
+        if (g == 0) p.part_lse[row] = sum > 0.f ? ref[nt][e] + log2f(sum) : sum == 0.f ? -CUDART_INF_F : CUDART_INF_F;
+      }
+  }
+  asm volatile("cp.async.wait_all;" ::: "memory");
+}
+
+// A warp per (sequence, query token, query head) joins the row's partial results.
+template <typename T, int D>
+__global__ void __launch_bounds__(256) combine_kernel(const AiPagedAttn4Args a, const Plan p) {
+  constexpr int E = D / 32;
+  const int b = blockIdx.y, lane = threadIdx.x % 32, item = blockIdx.x * 8 + threadIdx.x / 32;
+  const bool has = item < a.seq_len * a.num_q_heads;
+  const int t = has ? item / a.num_q_heads : 0, h = has ? item % a.num_q_heads : 0, hk = h / p.group;
+  const Lens len = seq_lens(a, b);  // (the caller's lengths: read before the wait)
+  const int seen = has && t < len.n ? len.keys - len.n + t + 1 : 0;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (!has) return;
+  float M = -CUDART_INF_F, sum = 0.f, acc[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) acc[e] = 0.f;
+  if (seen > 0) {
+    const int per = a.num_kv_heads * p.groups, s0 = p.scan[b], size = p.scan[b + 1] - s0;
+    const Split line = split_line(p.workers, p.scan[a.batch] * per);
+    const int i = t * p.group + h - hk * p.group, grp = i / p.unit_rows, sub = hk * p.groups + grp;
+    const int x = s0 * per + sub * size + kStart, tiles = min((seen - 1) / kKeys + 1, size - kStart);
+    const int first = line.worker(x), n = line.worker(x + tiles - 1) - first + 1;
+    const int64_t row = (int64_t)(b * per + sub + first) * p.unit_rows + i - grp * p.unit_rows;
+    auto row_at = [&](int k) { return row + (int64_t)k * p.unit_rows; };
+    for (int k = lane; k < n; k += 32) M = fmaxf(M, p.part_lse[row_at(k)]);
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, d));
+    if (M != -CUDART_INF_F) {
+      for (int k0 = 0; k0 < n; k0 += 32) {
+        const float mine = k0 + lane < n ? exp2f(p.part_lse[row_at(k0 + lane)] - M) : 0.f;
+        const int cnt = min(32, n - k0);
+#pragma unroll 4
+        for (int k = 0; k < cnt; ++k) {
+          const float w = __shfl_sync(0xffffffffu, mine, k);
+          const float* src = p.part_o + row_at(k0 + k) * D + E * lane;
+          float o[E];
+          if constexpr (E == 4)
+            *reinterpret_cast<float4*>(o) = *reinterpret_cast<const float4*>(src);
+          else if constexpr (E == 2)
+            *reinterpret_cast<float2*>(o) = *reinterpret_cast<const float2*>(src);
+          else
+            o[0] = *src;
+          sum += w;
+#pragma unroll
+          for (int e = 0; e < E; ++e) acc[e] = fmaf(w, o[e], acc[e]);
+        }
+      }
     }
   }
-  const float inv = l == 0.f ? 0.f : 1.f / l;
-  for (int c = 0; c < C; ++c) out[32 * c + lane] = from_f32<T>(o[c] * inv);
-  if (a.lse && lane == 0) a.lse[row] = l == 0.f ? -CUDART_INF_F : m + logf(l);
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  T* out = static_cast<T*>(const_cast<void*>(a.out.ptr)) + b * a.out.stride_b + h * a.out.stride_h + t * a.out.stride_t + E * lane;
+#pragma unroll
+  for (int e = 0; e < E; ++e) out[e] = from_f32<T>(acc[e] * inv);
+  if (a.lse && lane == 0)
+    a.lse[((int64_t)b * a.num_q_heads + h) * a.seq_len + t] = sum == 0.f ? -CUDART_INF_F : (M + log2f(sum)) * kLn2;
 }
 
 int check(const AiPagedAttn4Args* a) {
   if (!a) return AI_ERR_NULL;
-  if (a->batch <= 0 || a->batch > 4096 || a->seq_len <= 0 || a->num_q_heads <= 0 || a->num_kv_heads <= 0 ||
+  if (a->batch <= 0 || a->batch > kMaxBatch || a->seq_len <= 0 || a->num_q_heads <= 0 || a->num_kv_heads <= 0 ||
       a->num_q_heads % a->num_kv_heads)
     return AI_ERR_SHAPE;
   if (a->head_dim != 32 && a->head_dim != 64 && a->head_dim != 128) return AI_ERR_HEAD_DIM;
@@ -95,23 +670,72 @@ int check(const AiPagedAttn4Args* a) {
     if (t->stride_b < 0 || t->stride_h < 0 || t->stride_t < 0) return AI_ERR_STRIDE;
   }
   if (!a->lens) return AI_ERR_NULL;
-  return check_pool(a->pool, a->head_dim);
+  const int rc = check_pool(a->pool, a->head_dim);
+  if (rc != AI_OK) return rc;
+  // The line's positions and the combine launch's grid fit in 31 bits.
+  const int64_t rows = (int64_t)a->num_q_heads * a->seq_len, groups = rows / a->num_kv_heads / (8 * kMaxBlocks) + 1;
+  const int64_t tiles = (int64_t)a->pool.max_pages * a->pool.page_size / kKeys + kStart + 1;
+  if (rows > 0x7fffffff || tiles > 0x7fffffff || a->batch * a->num_kv_heads * groups > 0x7fffffff / tiles) return AI_ERR_SHAPE;
+  return AI_OK;
+}
+
+int sm_count() {
+  int dev = 0, sms = 148;
+  if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  return sms;
+}
+
+size_t layout(const AiPagedAttn4Args& a, Plan* p) {
+  p->group = a.num_q_heads / a.num_kv_heads;
+  p->rows = p->group * a.seq_len;
+  p->groups = (p->rows + 8 * kMaxBlocks - 1) / (8 * kMaxBlocks);
+  p->unit_rows = (p->rows + p->groups - 1) / p->groups;
+  p->blocks = (p->unit_rows + 7) / 8;
+  p->workers = sm_count() * warps_of(p->blocks);
+  const size_t rows = ((size_t)a.batch * a.num_kv_heads * p->groups + p->workers) * p->unit_rows;
+  const size_t o = (rows * a.head_dim * sizeof(float) + 255) & ~size_t(255), l = (rows * sizeof(float) + 255) & ~size_t(255);
+  char* w = static_cast<char*>(a.workspace);
+  p->part_o = reinterpret_cast<float*>(w);
+  p->part_lse = reinterpret_cast<float*>(w + o);
+  p->scan = reinterpret_cast<int*>(w + o + l);
+  return o + l + (((size_t)a.batch + 1) * sizeof(int) + 255) / 256 * 256;
+}
+
+template <typename T, int D, int NT>
+int launch(const AiPagedAttn4Args& a, const Plan& p, cudaStream_t st) {
+  const size_t smem = warps_of(NT) * kStages * Tile<D>::kBytes + (a.batch + 1) * sizeof(int);
+  if (cudaFuncSetAttribute(split_kernel<T, D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
+    return AI_ERR_LAUNCH;
+  split_kernel<T, D, NT><<<p.workers / warps_of(NT), 32 * warps_of(NT), smem, st>>>(a, p);
+  return cudaGetLastError() == cudaSuccess ? AI_OK : AI_ERR_LAUNCH;
 }
 
 template <typename T, int D>
-int launch(const AiPagedAttn4Args& a, cudaStream_t st) {
-  const int64_t rows = (int64_t)a.batch * a.num_q_heads * a.seq_len, blocks = (rows + kWarps - 1) / kWarps;
-  if (blocks > 0x7fffffff) return AI_ERR_SHAPE;
+int run(const AiPagedAttn4Args& a, const Plan& p, cudaStream_t st) {
   ProfScope ps(AI_PROF_ATTN4, st);
-  rows_kernel<T, D><<<(unsigned)blocks, kThreads, 0, st>>>(a);
+  const int rc = p.blocks == 1   ? launch<T, D, 1>(a, p, st)
+                 : p.blocks == 2 ? launch<T, D, 2>(a, p, st)
+                 : p.blocks == 3 ? launch<T, D, 3>(a, p, st)
+                                 : launch<T, D, 4>(a, p, st);
+  if (rc != AI_OK) return rc;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)((a.seq_len * (int64_t)a.num_q_heads + 7) / 8), a.batch);
+  cfg.blockDim = dim3(256);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (cudaLaunchKernelEx(&cfg, combine_kernel<T, D>, a, p) != cudaSuccess) return AI_ERR_LAUNCH;
   return cudaGetLastError() == cudaSuccess ? AI_OK : AI_ERR_LAUNCH;
 }
 
 template <typename T>
-int dispatch(const AiPagedAttn4Args& a, cudaStream_t st) {
-  if (a.head_dim == 128) return launch<T, 128>(a, st);
-  if (a.head_dim == 64) return launch<T, 64>(a, st);
-  return launch<T, 32>(a, st);
+int dispatch(const AiPagedAttn4Args& a, const Plan& p, cudaStream_t st) {
+  if (a.head_dim == 128) return run<T, 128>(a, p, st);
+  if (a.head_dim == 64) return run<T, 64>(a, p, st);
+  return run<T, 32>(a, p, st);
 }
 
 }  // namespace attn4
@@ -121,14 +745,19 @@ extern "C" int ai_paged_attn_4bit_workspace(const AiPagedAttn4Args* args, size_t
   const int rc = ai::attn4::check(args);
   if (rc != AI_OK) return rc;
   if (!bytes) return AI_ERR_NULL;
-  *bytes = 0;
+  ai::attn4::Plan p;
+  *bytes = ai::attn4::layout(*args, &p);
   return AI_OK;
 }
 
 extern "C" int ai_paged_attn_4bit(const AiPagedAttn4Args* args, void* stream) {
   const int rc = ai::attn4::check(args);
   if (rc != AI_OK) return rc;
+  ai::attn4::Plan p;
+  const size_t need = ai::attn4::layout(*args, &p);
+  if (!args->workspace || args->workspace_bytes < need) return AI_ERR_WORKSPACE;
+  if (reinterpret_cast<uintptr_t>(args->workspace) & 255) return AI_ERR_ALIGN;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (args->dtype == AI_DTYPE_BF16) return ai::attn4::dispatch<__nv_bfloat16>(*args, st);
-  return ai::attn4::dispatch<__half>(*args, st);
+  if (args->dtype == AI_DTYPE_BF16) return ai::attn4::dispatch<__nv_bfloat16>(*args, p, st);
+  return ai::attn4::dispatch<__half>(*args, p, st);
 }
