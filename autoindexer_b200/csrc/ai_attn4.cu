@@ -26,6 +26,7 @@
 #include <cuda_runtime.h>
 #include <math_constants.h>
 
+#include <cfloat>
 #include <cstring>
 #include <type_traits>
 
@@ -45,25 +46,36 @@ constexpr int kStart = 2;      // what starting a unit costs, in tiles
 constexpr int kLeast = 4;      // positions a worker takes, at least
 constexpr int kMaxBlocks = 4;  // column blocks (of 8 query rows) of a unit, at most
 constexpr float kLift = 7.f;   // P at a weight of 1 and the largest |scale|: 2^7
+constexpr long long kWait = 1000000000LL;
 constexpr float kSlack = 8.f;  // the running maximum moves when a score passes it by 2^8
 
-// Warps of a CTA (one per SM) and tiles of a warp's ring.
-__host__ __device__ constexpr int warps_of(int blocks) { return blocks <= 2 ? 12 : 8; }
-constexpr int kStages = 4;
+// Warps of a CTA (one per SM) and tiles of a warp's ring, by column blocks.
+__host__ __device__ constexpr int warps_of(int blocks) { return blocks == 1 ? 16 : blocks == 2 ? 12 : 8; }
+__host__ __device__ constexpr int stages_of(int blocks) { return blocks <= 2 ? 3 : 4; }
 
-// A tile in shared memory: codes of K and V, scales of K and V.
+// A tile in shared memory: codes of K and V, scales of K and V, as they lie in
+// the pools.  Row i of a product's 16 keys is key place(i): the rows that a
+// quarter of a warp reads together are then neighbours (K's even and odd ones,
+// V's four of a pair's first or second key).
 template <int D>
 struct Tile {
   static constexpr int C = D / kGroup, kRow = D / 2, kCodes = kKeys * kRow, kScales = kKeys * C * 2;
   static constexpr int K = 0, V = kCodes, KS = 2 * kCodes, VS = KS + kScales, kBytes = VS + kScales;
-  // V's rows stand so that the four keys which a quarter of a warp reads
-  // together are neighbours (keys 2 t of eight, then 2 t + 1), and at D 128 their
-  // 16-byte pieces in halves of the row that do not share banks.
-  __device__ static int v_row(int key) { return (key & 24) | ((key & 1) << 2) | ((key >> 1) & 3); }
-  __device__ static int v_piece(int row, int piece) { return D == 128 ? piece ^ (row & 2) : piece; }
+  __device__ static int place(int i) { return (i & 8) | (i & 1 ? 4 + (i >> 1 & 3 ^ 1) : i >> 1 & 3); }
 };
 
-static_assert(warps_of(1) * kStages * Tile<128>::kBytes + 4 * (kMaxBatch + 1) <= 227 * 1024, "a CTA's shared memory");
+// A CTA's shared memory: rings, the query fragments of its warps (kept there
+// from two column blocks on), barriers, the scan.
+template <int D, int NT>
+struct Smem {
+  static constexpr int W = warps_of(NT), S = stages_of(NT);
+  static constexpr int kQ = NT == 1 ? 0 : NT * (D / kGroup) * 512;
+  static constexpr int RING = 0, Q = W * S * Tile<D>::kBytes, BARS = Q + W * kQ, SCAN = BARS + W * S * 8;
+  static size_t bytes(int batch) { return SCAN + ((size_t)batch + 1) * sizeof(int); }
+};
+static_assert(Smem<128, 1>::SCAN + 4 * (kMaxBatch + 1) <= 227 * 1024, "a CTA's shared memory");
+static_assert(Smem<128, 2>::SCAN + 4 * (kMaxBatch + 1) <= 227 * 1024, "a CTA's shared memory");
+static_assert(Smem<128, 4>::SCAN + 4 * (kMaxBatch + 1) <= 227 * 1024, "a CTA's shared memory");
 
 struct Plan {
   int group;       // G: query heads per KV head
@@ -155,10 +167,14 @@ __device__ __forceinline__ bool next_seg(const AiPagedAttn4Args& a, const Plan& 
   return false;
 }
 
-__device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+__device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1,
+                                    float c0, float c1, float c2, float c3) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %12, %13};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2), "f"(c3));
+}
+__device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  mma(d, a0, a1, a2, a3, b0, b1, d[0], d[1], d[2], d[3]);
 }
 
 // An 8 x 8 matrix of 16-bit elements, a row of pairs per four lanes, transposed.
@@ -168,13 +184,11 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
   return y;
 }
 
-// Copies `N` bytes to shared memory, zeros where there is nothing to copy.
-template <int N>
-__device__ __forceinline__ void copy_async(uint32_t dst, const void* src, bool some) {
-  if constexpr (N == 16)
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(some ? 16 : 0) : "memory");
-  else
-    asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(N), "r"(some ? N : 0) : "memory");
+// Bulk copy of a contiguous piece to shared memory (16-byte boundaries and size).
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src),
+               "r"(bytes), "r"(bar)
+               : "memory");
 }
 
 // Lower (or upper) halves of two words, side by side.
@@ -196,18 +210,27 @@ __device__ __forceinline__ void lds(uint32_t (&w)[(N + 3) / 4], const uint8_t* p
   }
 }
 
-// Four pairs of codes (at bits 4 j and 16 + 4 j) as fp16 64 + c ...
-__device__ __forceinline__ uint32_t biased(uint32_t x, int j) {
-  const uint32_t s = j == 0 ? x << 4 : x >> (4 * (j - 1));
-  return (s & 0x00f000f0u) | 0x54005400u;
-}
-// ... and as c - 8.
-__device__ __forceinline__ uint32_t centred(uint32_t x, int j) {
-  const uint32_t s = j < 2 ? x : x >> 8;
-  const uint32_t f = j % 2 == 0 ? (s & 0x000f000fu) | 0x64006400u : (s & 0x00f000f0u) | 0x54005400u;
-  const __half2 off = j % 2 == 0 ? __half2half2(__ushort_as_half(0x6408)) : __half2half2(__ushort_as_half(0x5480));
-  const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&f), off);
+// Four pairs of codes (at bits 4 j and 16 + 4 j of x) as fp16: the bits of a
+// code at the bottom of 1024's mantissa, or above its four lowest in 64's, are
+// 1024 + c and 64 + c.  `off` taken away from the first leaves 64 + c or c - 8,
+// exactly (the logic unit is the busier one, so no shift for it).
+__device__ __forceinline__ uint32_t sub2(uint32_t x, uint16_t off) {
+  const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&x), __half2half2(__ushort_as_half(off)));
   return *reinterpret_cast<const uint32_t*>(&r);
+}
+__device__ __forceinline__ void biased(uint32_t x, uint32_t (&f)[4]) {  // 64 + c
+  const uint32_t y = x >> 8;
+  f[0] = sub2((x & 0x000f000fu) | 0x64006400u, 0x6380);
+  f[1] = (x & 0x00f000f0u) | 0x54005400u;
+  f[2] = sub2((y & 0x000f000fu) | 0x64006400u, 0x6380);
+  f[3] = (y & 0x00f000f0u) | 0x54005400u;
+}
+__device__ __forceinline__ void centred(uint32_t x, uint32_t (&f)[4]) {  // c - 8
+  const uint32_t y = x >> 8;
+  f[0] = sub2((x & 0x000f000fu) | 0x64006400u, 0x6408);
+  f[1] = sub2((x & 0x00f000f0u) | 0x54005400u, 0x5480);
+  f[2] = sub2((y & 0x000f000fu) | 0x64006400u, 0x6408);
+  f[3] = sub2((y & 0x00f000f0u) | 0x54005400u, 0x5480);
 }
 
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
@@ -230,13 +253,18 @@ __device__ __forceinline__ void load_q(const T* p, float (&f)[8]) {
   }
 }
 
+__device__ __forceinline__ float half_of(uint32_t w, int i) {
+  return __half2float(__ushort_as_half((unsigned short)(i ? w >> 16 : w)));
+}
+
 template <typename T, int D, int NT>
 __global__ void __launch_bounds__(32 * warps_of(NT), 1) split_kernel(const AiPagedAttn4Args a, const Plan p) {
   using L = Tile<D>;
-  constexpr int C = L::C, W = warps_of(NT);
+  using M = Smem<D, NT>;
+  constexpr int C = L::C, H = (C + 1) / 2, S = M::S;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   extern __shared__ __align__(128) uint8_t smem[];
-  int* scan = reinterpret_cast<int*>(smem + W * kStages * L::kBytes);
+  int* scan = reinterpret_cast<int*>(smem + M::SCAN);
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, g = lane / 4, t = lane % 4;
   if (warp == 0) {
     int base = 0;
@@ -253,6 +281,9 @@ __global__ void __launch_bounds__(32 * warps_of(NT), 1) split_kernel(const AiPag
     }
     if (lane == 0) scan[0] = 0;
   }
+  const uint32_t bars = ptx::smem_u32(smem + M::BARS) + warp * S * 8;
+  if (lane < S) ptx::mbar_init(bars + 8 * lane, 1);
+  if (lane == 0) ptx::fence_mbar_init();
   __syncthreads();
   if (blockIdx.x == 0)
     for (int b = tid; b <= a.batch; b += blockDim.x) p.scan[b] = scan[b];
@@ -260,89 +291,69 @@ __global__ void __launch_bounds__(32 * warps_of(NT), 1) split_kernel(const AiPag
   const int worker = warp * gridDim.x + blockIdx.x;  // (few workers: on as many SMs)
   if (worker >= line.n) return;
   const int w0 = line.begin(worker), w1 = line.begin(worker + 1);
-  uint8_t* ring = smem + warp * kStages * L::kBytes;
+  const uint8_t* ring = smem + warp * S * L::kBytes;
+  const uint32_t ring_at = ptx::smem_u32(ring);
 
-  // ---- loads, `kStages - 1` tiles ahead of what is computed
+  // ---- loads: lane 4 h + i copies piece i (codes of K and V, scales of K and V)
+  // of the half h of a tile, whose 16 keys lie in one page.
   const int page_bits = 31 - __clz(a.pool.page_size), page_mask = a.pool.page_size - 1;
+  const int half = lane / 4 & 1;
+  const AiTensor4& mine = t == 0 ? a.pool.k_codes : t == 1 ? a.pool.v_codes : t == 2 ? a.pool.k_scales : a.pool.v_scales;
+  const int unit_bytes = t < 2 ? 1 : 2, key_bytes = t < 2 ? L::kRow : 2 * C;
+  const uint32_t piece_at = (t == 0 ? L::K : t == 1 ? L::V : t == 2 ? L::KS : L::VS) + half * 16 * key_bytes;
+  const char* pool = static_cast<const char*>(mine.ptr);
+  const int64_t page_step = mine.stride_b * unit_bytes, head_step = mine.stride_h * unit_bytes;
   Seg ld;
-  int wl = w0, page[2] = {0, 0};
-  auto look_up = [&]() {  // pages of the tile's halves
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int key = ld.tile * kKeys + 16 * h;
-      page[h] = 0;
-      if (key < ld.keys) {
-        page[h] = __ldg(a.pool.page_table + ld.b * a.pool.page_table_stride + (key >> page_bits));
-        if (page[h] < 0 || page[h] >= a.pool.n_pages) report(a.status, AI_ERR_DEV_BOUNDS), page[h] = 0;
-      }
+  int wl = w0, page = 0, in_flight = 0, at_stage = 0;
+  auto look_up = [&]() {  // the page of the lane's half
+    const int key = ld.tile * kKeys + 16 * half;
+    page = 0;
+    if (lane < 8 && key < ld.keys) {
+      page = __ldg(a.pool.page_table + ld.b * a.pool.page_table_stride + (key >> page_bits));
+      if (page < 0 || page >= a.pool.n_pages) report(a.status, AI_ERR_DEV_BOUNDS), page = 0;
     }
   };
   bool loads = next_seg(a, p, scan, wl, w1, ld);
   if (loads) look_up();
-  uint16_t held[2] = {0, 0};  // D 32: scales on their way (two bytes are no copy)
-  int held_at = -1;
-  auto issue = [&](int stage) {
-    if constexpr (D == 32) {
-      if (held_at >= 0) {
-        uint8_t* dst = ring + held_at * L::kBytes;
-        reinterpret_cast<uint16_t*>(dst + L::KS)[lane] = held[0];
-        reinterpret_cast<uint16_t*>(dst + L::VS)[lane] = held[1];
-        held_at = -1;
-      }
-    }
-    if (loads) {
-      uint8_t* dst = ring + stage * L::kBytes;
-      const uint32_t to = ptx::smem_u32(dst);
-      const int k0 = ld.tile * kKeys, left = ld.keys - k0;
-      constexpr int P = L::kRow / 16;  // 16-byte pieces of a row
-#pragma unroll
-      for (int i = 0; i < P; ++i) {
-        const int at = i * 32 + lane, key = at / P, piece = at % P, h = key / 16;
-        const int64_t pg = h ? page[1] : page[0], slot = (k0 + key) & page_mask;
-        const bool some = key < left;
-        const uint8_t* k = static_cast<const uint8_t*>(a.pool.k_codes.ptr) + pg * a.pool.k_codes.stride_b +
-                           ld.hk * a.pool.k_codes.stride_h + slot * a.pool.k_codes.stride_t + 16 * piece;
-        const uint8_t* v = static_cast<const uint8_t*>(a.pool.v_codes.ptr) + pg * a.pool.v_codes.stride_b +
-                           ld.hk * a.pool.v_codes.stride_h + slot * a.pool.v_codes.stride_t + 16 * piece;
-        const int row = L::v_row(key);
-        copy_async<16>(to + L::K + key * L::kRow + 16 * piece, k, some);
-        copy_async<16>(to + L::V + row * L::kRow + 16 * L::v_piece(row, piece), v, some);
-      }
-      {
-        const int64_t pg = lane < 16 ? page[0] : page[1], slot = (k0 + lane) & page_mask;
-        const bool some = lane < left;
-        const __half* k = static_cast<const __half*>(a.pool.k_scales.ptr) + pg * a.pool.k_scales.stride_b +
-                          ld.hk * a.pool.k_scales.stride_h + slot * a.pool.k_scales.stride_t;
-        const __half* v = static_cast<const __half*>(a.pool.v_scales.ptr) + pg * a.pool.v_scales.stride_b +
-                          ld.hk * a.pool.v_scales.stride_h + slot * a.pool.v_scales.stride_t;
-        if constexpr (D == 32) {
-          held[0] = some ? __ldg(reinterpret_cast<const uint16_t*>(k)) : (uint16_t)0;
-          held[1] = some ? __ldg(reinterpret_cast<const uint16_t*>(v)) : (uint16_t)0;
-          held_at = stage;
-        } else {
-          copy_async<2 * C>(to + L::KS + lane * 2 * C, k, some);
-          copy_async<2 * C>(to + L::VS + lane * 2 * C, v, some);
-        }
-      }
-      if (++ld.tile == ld.end) loads = next_seg(a, p, scan, wl, w1, ld);
-      if (loads) look_up();
-    }
-    asm volatile("cp.async.commit_group;" ::: "memory");
+  auto issue = [&]() {
+    if (!loads) return;
+    const uint32_t bar = bars + 8 * at_stage;
+    const int key = ld.tile * kKeys + 16 * half;
+    const bool both = ld.tile * kKeys + 16 < ld.keys;
+    if (lane == 0) ptx::mbar_arrive_expect_tx(bar, (both ? 2 : 1) * 16 * (2 * L::kRow + 4 * C));
+    __syncwarp();
+    if (lane < 4 || (lane < 8 && both))
+      bulk_load(ring_at + at_stage * L::kBytes + piece_at, pool + page * page_step + ld.hk * head_step + (key & page_mask) * key_bytes,
+                16 * key_bytes, bar);
+    ++in_flight;
+    at_stage = at_stage + 1 == S ? 0 : at_stage + 1;
+    if (++ld.tile == ld.end) loads = next_seg(a, p, scan, wl, w1, ld);
+    if (loads) look_up();
+  };
+  int st = 0;
+  uint32_t phase = 0;
+  auto arrived = [&]() -> bool {
+    if (__all_sync(0xffffffffu, ptx::mbar_try_wait(bars + 8 * st, phase))) return true;
+    return __all_sync(0xffffffffu, ptx::mbar_wait(bars + 8 * st, phase, kWait));
   };
 #pragma unroll
-  for (int s = 0; s < kStages - 1; ++s) issue(s);
+  for (int i = 0; i < S - 1; ++i) issue();
 
   // ---- products
-  int wc = w0, st = 0;
+  int wc = w0;
+  bool ok = true;
   Seg s;
-  while (next_seg(a, p, scan, wc, w1, s)) {
+  const int row_g = L::place(g);  // the lane's key of a product's first eight, as they lie
+  uint4* q_smem = reinterpret_cast<uint4*>(smem + M::Q + warp * M::kQ) + lane;
+  while (ok && next_seg(a, p, scan, wc, w1, s)) {
     const int row0 = s.grp * p.unit_rows, n_rows = min(p.rows - row0, p.unit_rows);
     // Query fragments: lane (g, t) has dims 32 c + 8 t + {0 .. 7} of row 8 nt + g.
-    uint32_t q[NT][C][4];
+    uint4 q_reg[C];
     float q_off[NT][C][2];            // -72 sum(q) of rows 2 t and 2 t + 1, per group
-    float slope[NT][2];               // of the scores, in units of log 2
+    float slope[NT][2];               // of the scores, in units of log 2, above zero (its sign is the fragments')
     int seen[NT][2];                  // keys that those rows see; -1: no query
     int least = 0x7fffffff;           // tiles that end by it are seen whole
+    const float unit = fabsf(a.scale) * kLog2e, sign = a.scale < 0.f ? -1.f : 1.f;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       const int i = 8 * nt + g;
@@ -355,28 +366,35 @@ __global__ void __launch_bounds__(32 * warps_of(NT), 1) split_kernel(const AiPag
         load_q(src + kGroup * c, f[c]);
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          if (!has) f[c][e] = 0.f;
+          f[c][e] = has ? f[c][e] * sign : 0.f;
           top = fmaxf(top, fabsf(f[c][e]));
         }
       }
-      int up = 0;
-      if constexpr (sizeof(T) == 2 && !std::is_same<T, __half>::value) {
+      float slope_g = unit;
+      if constexpr (!std::is_same<T, __half>::value) {  // (fp16 holds its own)
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        if (top > 0.f && top < CUDART_INF_F) up = 14 - ilogbf(top);
+        const int up = top > 0.f && top < CUDART_INF_F ? 14 - ilogbf(top) : 0;
+        slope_g = ldexpf(unit, -up);
+#pragma unroll
+        for (int c = 0; c < C; ++c)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) f[c][e] = ldexpf(f[c][e], up);
       }
-      const float slope_g = ldexpf(a.scale * kLog2e, -up);
 #pragma unroll
       for (int c = 0; c < C; ++c) {
-        __half2 h[4];
+        uint32_t h[4];
         float sum = 0.f;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {  // (dims 8 t + e and 8 t + 4 + e are a pair)
-          h[e] = __floats2half2_rn(ldexpf(f[c][e], up), ldexpf(f[c][4 + e], up));
-          const float2 back = __half22float2(h[e]);
-          sum += back.x + back.y;
+          h[e] = pack2(f[c][e], f[c][4 + e]);
+          sum += half_of(h[e], 0) + half_of(h[e], 1);
         }
-        memcpy(q[nt][c], h, 16);
+        const uint4 frag = make_uint4(h[0], h[1], h[2], h[3]);
+        if constexpr (NT == 1)
+          q_reg[c] = frag;
+        else
+          q_smem[(nt * C + c) * 32] = frag;  // (its own lane's alone)
         sum += __shfl_xor_sync(0xffffffffu, sum, 1);
         sum += __shfl_xor_sync(0xffffffffu, sum, 2);
 #pragma unroll
@@ -384,7 +402,7 @@ __global__ void __launch_bounds__(32 * warps_of(NT), 1) split_kernel(const AiPag
       }
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        slope[nt][e] = __shfl_sync(0xffffffffu, slope_g, 4 * (2 * t + e));
+        slope[nt][e] = fmaxf(__shfl_sync(0xffffffffu, slope_g, 4 * (2 * t + e)), FLT_MIN);  // (a masked score stays -inf)
         const int i2 = 8 * nt + 2 * t + e, tok2 = (row0 + i2) / p.group;
         seen[nt][e] = i2 < n_rows && tok2 < s.n ? max(0, s.keys - s.n + tok2 + 1) : -1;
         if (seen[nt][e] >= 0) least = min(least, seen[nt][e]);
@@ -392,17 +410,21 @@ __global__ void __launch_bounds__(32 * warps_of(NT), 1) split_kernel(const AiPag
     }
     least = min(least, __shfl_xor_sync(0xffffffffu, least, 1));
     least = min(least, __shfl_xor_sync(0xffffffffu, least, 2));
+    least = min(least, s.keys);
 
     float o[NT][2 * C][4];
-    float m[NT][2], ref[NT][2], l[NT][2], l_before[NT][2];
+    float m[NT][2];                    // running maximum, in units of log 2
+    float ref[NT][2];                  // what the exponents are taken from: the maximum and P's place in fp16
+    float2 l[NT], l_before[NT];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
       for (int i = 0; i < 2 * C; ++i)
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[nt][i][e] = 0.f;
-#pragma unroll
-      for (int e = 0; e < 2; ++e) m[nt][e] = -CUDART_INF_F, ref[nt][e] = l[nt][e] = l_before[nt][e] = 0.f;
+      m[nt][0] = m[nt][1] = -CUDART_INF_F;
+      ref[nt][0] = ref[nt][1] = 0.f;
+      l[nt] = l_before[nt] = make_float2(0.f, 0.f);
     }
     // The largest |V scale| so far is at most 2^v_exp (v_lim in both halves; the
     // first one above 0 sets them).
@@ -410,71 +432,75 @@ __global__ void __launch_bounds__(32 * warps_of(NT), 1) split_kernel(const AiPag
     uint32_t v_lim = 0;
 
     for (int tile = s.tile; tile < s.end; ++tile) {
-      asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
-      __syncwarp();
-      issue((st + kStages - 1) % kStages);
+      if (!(ok = arrived())) break;
+      issue();  // (into the stage of the tile before: every lane has read it)
       const uint8_t* sm = ring + st * L::kBytes;
-      st = st + 1 == kStages ? 0 : st + 1;
+      if (++st == S) st = 0, phase ^= 1;
+      --in_flight;
       const int k0 = tile * kKeys;
-      const bool ragged = k0 + kKeys > least;
 
-      // Scores: keys 16 mt + g (e = 0, 1) and 16 mt + g + 8 (2, 3), rows 2 t + e % 2.
-      float sc[2][NT][4];
-      uint32_t vs[2][2][(C + 1) / 2];
+      // Scores: keys place(g) (e = 0, 1) and 8 behind (2, 3) of half mt, rows 2 t + e % 2.
+      float2 sc[2][NT][2];
+      uint32_t vs[2][2][H];
 #pragma unroll
       for (int mt = 0; mt < 2; ++mt) {
-        uint32_t kw[2][C];
-        float ks[2][C];
+        uint32_t kw[2][C], ks[2][H];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const int key = 16 * mt + 8 * h + g;
+          const int key = 16 * mt + 8 * h + row_g;
           lds<4 * C>(kw[h], sm + L::K + key * L::kRow + 4 * C * t);
-          uint32_t raw[(C + 1) / 2];
-          lds<2 * C>(raw, sm + L::KS + key * 2 * C);
-#pragma unroll
-          for (int c = 0; c < C; ++c)
-            ks[h][c] = __half2float(__ushort_as_half((unsigned short)(raw[c / 2] >> (16 * (c % 2)))));
+          lds<2 * C>(ks[h], sm + L::KS + key * 2 * C);
           lds<2 * C>(vs[mt][h], sm + L::VS + key * 2 * C);
         }
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) sc[mt][nt][e] = 0.f;
+        for (int nt = 0; nt < NT; ++nt) sc[mt][nt][0] = sc[mt][nt][1] = make_float2(0.f, 0.f);
 #pragma unroll
         for (int c = 0; c < C; ++c) {
-          uint32_t x[2];
-#pragma unroll
-          for (int h = 0; h < 2; ++h) x[h] = C == 1 ? kw[h][0] : halves(kw[h][c / 2], kw[h][(C + c) / 2], c % 2);
           uint32_t f[2][4];
 #pragma unroll
-          for (int j = 0; j < 4; ++j) f[0][j] = biased(x[0], j), f[1][j] = biased(x[1], j);
+          for (int h = 0; h < 2; ++h) biased(C == 1 ? kw[h][0] : halves(kw[h][c / 2], kw[h][(C + c) / 2], c % 2), f[h]);
+          const float k_lo = half_of(ks[0][c / 2], c % 2), k_hi = half_of(ks[1][c / 2], c % 2);
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
-            float acc[4] = {q_off[nt][c][0], q_off[nt][c][1], q_off[nt][c][0], q_off[nt][c][1]};
-            mma(acc, f[0][0], f[1][0], f[0][1], f[1][1], q[nt][c][0], q[nt][c][1]);
-            mma(acc, f[0][2], f[1][2], f[0][3], f[1][3], q[nt][c][2], q[nt][c][3]);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) sc[mt][nt][e] = fmaf(ks[e / 2][c], acc[e], sc[mt][nt][e]);
+            uint4 q;
+            if constexpr (NT == 1)
+              q = q_reg[c];
+            else
+              q = q_smem[(nt * C + c) * 32];
+            float acc[4];
+            mma(acc, f[0][0], f[1][0], f[0][1], f[1][1], q.x, q.y, q_off[nt][c][0], q_off[nt][c][1], q_off[nt][c][0], q_off[nt][c][1]);
+            mma(acc, f[0][2], f[1][2], f[0][3], f[1][3], q.z, q.w);
+            sc[mt][nt][0] = __ffma2_rn(make_float2(k_lo, k_lo), make_float2(acc[0], acc[1]), sc[mt][nt][0]);
+            sc[mt][nt][1] = __ffma2_rn(make_float2(k_hi, k_hi), make_float2(acc[2], acc[3]), sc[mt][nt][1]);
           }
         }
       }
-      // The running maximum of each row, lazily.
+      const bool ragged = k0 + kKeys > least;
+      if (ragged) {
+#pragma unroll
+        for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int key = k0 + 16 * mt + 8 * h + row_g;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+              if (key >= seen[nt][0]) sc[mt][nt][h].x = -CUDART_INF_F;
+              if (key >= seen[nt][1]) sc[mt][nt][h].y = -CUDART_INF_F;
+            }
+            if (key >= s.keys) {  // (a slot that no one wrote)
+#pragma unroll
+              for (int i = 0; i < H; ++i) vs[mt][h][i] = 0;
+            }
+          }
+      }
+      // The running maximum of each row, and of the V scales, lazily.
       bool move = false;
       float top[NT][2];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-        for (int mt = 0; mt < 2; ++mt)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            sc[mt][nt][e] *= slope[nt][e % 2];
-            if (ragged && k0 + 16 * mt + 8 * (e / 2) + g >= seen[nt][e % 2]) sc[mt][nt][e] = -CUDART_INF_F;
-          }
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          top[nt][e] = fmaxf(ptx::fmax3(sc[0][nt][e], sc[0][nt][2 + e], sc[1][nt][e]), sc[1][nt][2 + e]);
-          move |= top[nt][e] > m[nt][e] + kSlack;
-        }
+        top[nt][0] = fmaxf(ptx::fmax3(sc[0][nt][0].x, sc[0][nt][1].x, sc[1][nt][0].x), sc[1][nt][1].x) * slope[nt][0];
+        top[nt][1] = fmaxf(ptx::fmax3(sc[0][nt][0].y, sc[0][nt][1].y, sc[1][nt][0].y), sc[1][nt][1].y) * slope[nt][1];
+        move |= top[nt][0] > m[nt][0] + kSlack || top[nt][1] > m[nt][1] + kSlack;
       }
       __half2 big = __half2half2(__ushort_as_half(0));
 #pragma unroll
@@ -482,25 +508,25 @@ __global__ void __launch_bounds__(32 * warps_of(NT), 1) split_kernel(const AiPag
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
-          for (int i = 0; i < (C + 1) / 2; ++i) big = __hmax2(big, __habs2(*reinterpret_cast<const __half2*>(&vs[mt][h][i])));
+          for (int i = 0; i < H; ++i) big = __hmax2(big, __habs2(*reinterpret_cast<const __half2*>(&vs[mt][h][i])));
       move |= !__hble2(big, *reinterpret_cast<const __half2*>(&v_lim));
       if (__any_sync(0xffffffffu, move)) {
         // (an infinite scale makes what it meets infinite; it has no part in the bound)
-        float mine = 0.f;
+        float size = 0.f;
 #pragma unroll
         for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
           for (int h = 0; h < 2; ++h)
 #pragma unroll
             for (int c = 0; c < C; ++c) {
-              const float d = fabsf(__half2float(__ushort_as_half((unsigned short)(vs[mt][h][c / 2] >> (16 * (c % 2))))));
-              if (d < CUDART_INF_F) mine = fmaxf(mine, d);
+              const float d = fabsf(half_of(vs[mt][h][c / 2], c % 2));
+              if (d < CUDART_INF_F) size = fmaxf(size, d);
             }
 #pragma unroll
-        for (int d = 1; d < 32; d <<= 1) mine = fmaxf(mine, __shfl_xor_sync(0xffffffffu, mine, d));
+        for (int d = 1; d < 32; d <<= 1) size = fmaxf(size, __shfl_xor_sync(0xffffffffu, size, d));
         float down = 1.f;
-        if (mine > 0.f) {
-          const int e = ilogbf(mine) + 1;
+        if (size > 0.f) {
+          const int e = ilogbf(size) + 1;
           if (e > v_exp) {
             down = ptx::ex2((float)(v_exp - e));
             v_exp = e;
@@ -509,63 +535,59 @@ __global__ void __launch_bounds__(32 * warps_of(NT), 1) split_kernel(const AiPag
           }
         }
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
+        for (int nt = 0; nt < NT; ++nt) {
+          float alpha[2] = {down, down};
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            float x = top[nt][e], alpha = down;
+            float x = top[nt][e];
 #pragma unroll
             for (int d = 4; d < 32; d <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, d));
             if (x > m[nt][e] + kSlack) {
-              if (m[nt][e] != -CUDART_INF_F) alpha *= ptx::ex2(m[nt][e] - x);
+              if (m[nt][e] != -CUDART_INF_F) alpha[e] *= ptx::ex2(m[nt][e] - x);
               m[nt][e] = x;
             }
             ref[nt][e] = (m[nt][e] == -CUDART_INF_F ? 0.f : m[nt][e]) + ((float)v_exp - kLift);
-            l[nt][e] *= alpha;
-            l_before[nt][e] *= alpha;
 #pragma unroll
-            for (int i = 0; i < 2 * C; ++i) o[nt][i][e] *= alpha, o[nt][i][2 + e] *= alpha;
+            for (int i = 0; i < 2 * C; ++i) o[nt][i][e] *= alpha[e], o[nt][i][2 + e] *= alpha[e];
           }
+          l[nt] = __fmul2_rn(l[nt], make_float2(alpha[0], alpha[1]));
+          l_before[nt] = __fmul2_rn(l_before[nt], make_float2(alpha[0], alpha[1]));
+        }
       }
       // Weights, and per group of dims the weights times the V scales as the
-      // second product takes them: lane (g, t) keys 2 t, 2 t + 1 (and + 8) of row g.
+      // second product takes them.
 #pragma unroll
       for (int mt = 0; mt < 2; ++mt) {
         uint32_t pv[NT][C][2];
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          float w[4];
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) w[e] = ptx::ex2(sc[mt][nt][e] - ref[nt][e % 2]);
+          for (int h = 0; h < 2; ++h) {
+            const float2 y = __ffma2_rn(sc[mt][nt][h], make_float2(slope[nt][0], slope[nt][1]), make_float2(-ref[nt][0], -ref[nt][1]));
+            const float2 w = make_float2(ptx::ex2(y.x), ptx::ex2(y.y));
+            l[nt] = __fadd2_rn(l[nt], w);
 #pragma unroll
-          for (int e = 0; e < 2; ++e) l[nt][e] += w[e] + w[2 + e];
-#pragma unroll
-          for (int c = 0; c < C; ++c)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              const float d = __half2float(__ushort_as_half((unsigned short)(vs[mt][h][c / 2] >> (16 * (c % 2)))));
-              float2 x = __fmul2_rn(make_float2(w[2 * h], w[2 * h + 1]), make_float2(d, d));
-              if (ragged) {  // (a key that the row does not see may have any scale)
-                if (sc[mt][nt][2 * h] == -CUDART_INF_F) x.x = 0.f;
-                if (sc[mt][nt][2 * h + 1] == -CUDART_INF_F) x.y = 0.f;
-              }
-              pv[nt][c][h] = transpose8(pack2(x.x, x.y));
+            for (int c = 0; c < C; ++c) {
+              const float d = half_of(vs[mt][h][c / 2], c % 2);
+              const float2 x = __fmul2_rn(w, make_float2(d, d));
+              pv[nt][c][h] = pack2(x.x, x.y);
             }
-        }
-        uint32_t vw[4][(C + 1) / 2];  // keys 2 t, 2 t + 1, 2 t + 8, 2 t + 9
+            if (ragged) {  // (a key that a row does not see may have any scale)
+              const uint32_t keep = (sc[mt][nt][h].x == -CUDART_INF_F ? 0u : 0xffffu) | (sc[mt][nt][h].y == -CUDART_INF_F ? 0u : 0xffff0000u);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int row = 16 * mt + 4 * i + t;
-          if constexpr (D == 128)
-            lds<8>(vw[i], sm + L::V + row * L::kRow + 16 * L::v_piece(row, g / 2) + 8 * (g % 2));
-          else
-            lds<2 * C>(vw[i], sm + L::V + row * L::kRow + 2 * C * g);
-        }
+              for (int c = 0; c < C; ++c) pv[nt][c][h] &= keep;
+            }
+#pragma unroll
+            for (int c = 0; c < C; ++c) pv[nt][c][h] = transpose8(pv[nt][c][h]);
+          }
+        uint32_t vw[4][H];  // the keys of rows 2 t, 2 t + 1, 2 t + 8, 2 t + 9
+#pragma unroll
+        for (int i = 0; i < 4; ++i) lds<2 * C>(vw[i], sm + L::V + (16 * mt + L::place(8 * (i / 2) + 2 * t + i % 2)) * L::kRow + 2 * C * g);
 #pragma unroll
         for (int c = 0; c < C; ++c) {
-          const uint32_t z0 = halves(vw[0][c / 2], vw[1][c / 2], c % 2), z1 = halves(vw[2][c / 2], vw[3][c / 2], c % 2);
           uint32_t f[2][4];
-#pragma unroll
-          for (int j = 0; j < 4; ++j) f[0][j] = centred(z0, j), f[1][j] = centred(z1, j);
+          centred(halves(vw[0][c / 2], vw[1][c / 2], c % 2), f[0]);
+          centred(halves(vw[2][c / 2], vw[3][c / 2], c % 2), f[1]);
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
             mma(o[nt][2 * c], f[0][0], f[0][1], f[1][0], f[1][1], pv[nt][c][0], pv[nt][c][1]);
@@ -576,17 +598,16 @@ __global__ void __launch_bounds__(32 * warps_of(NT), 1) split_kernel(const AiPag
       // (a sum of sums: one running sum of a long list would round its small weights away)
       if (tile % 16 == 15) {
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int e = 0; e < 2; ++e) l_before[nt][e] += l[nt][e], l[nt][e] = 0.f;
+        for (int nt = 0; nt < NT; ++nt) l_before[nt] = __fadd2_rn(l_before[nt], l[nt]), l[nt] = make_float2(0.f, 0.f);
       }
     }
+    if (!ok) break;
     // Partial rows: dims 32 c + 4 g + {0 .. 3} of rows 2 t and 2 t + 1.
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        float sum = l_before[nt][e] + l[nt][e];
+        float sum = e ? l_before[nt].y + l[nt].y : l_before[nt].x + l[nt].x;
 #pragma unroll
         for (int d = 4; d < 32; d <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
         if (seen[nt][e] <= 0) continue;
@@ -600,7 +621,14 @@ __global__ void __launch_bounds__(32 * warps_of(NT), 1) split_kernel(const AiPag
         if (g == 0) p.part_lse[row] = sum > 0.f ? ref[nt][e] + log2f(sum) : sum == 0.f ? -CUDART_INF_F : CUDART_INF_F;
       }
   }
-  asm volatile("cp.async.wait_all;" ::: "memory");
+  if (!ok) {
+    // A wait gave up: the copies in flight land before the warp ends.
+    if (lane == 0) report(a.status, AI_ERR_DEV_TIMEOUT);
+    for (; in_flight > 0; --in_flight) {
+      ptx::mbar_wait(bars + 8 * st, phase, kWait);
+      if (++st == S) st = 0, phase ^= 1;
+    }
+  }
 }
 
 // A warp per (sequence, query token, query head) joins the row's partial results.
@@ -703,7 +731,7 @@ size_t layout(const AiPagedAttn4Args& a, Plan* p) {
 
 template <typename T, int D, int NT>
 int launch(const AiPagedAttn4Args& a, const Plan& p, cudaStream_t st) {
-  const size_t smem = warps_of(NT) * kStages * Tile<D>::kBytes + (a.batch + 1) * sizeof(int);
+  const size_t smem = Smem<D, NT>::bytes(a.batch);
   if (cudaFuncSetAttribute(split_kernel<T, D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
     return AI_ERR_LAUNCH;
   split_kernel<T, D, NT><<<p.workers / warps_of(NT), 32 * warps_of(NT), smem, st>>>(a, p);

@@ -47,10 +47,10 @@ inline int check_pool(const AiPool4& p, int head_dim) {
     const AiTensor4& t = i == 0 ? p.k_codes : i == 1 ? p.v_codes : i == 2 ? p.k_scales : p.v_scales;
     if (!t.ptr) return AI_ERR_NULL;
     if (t.stride_b < 0 || t.stride_h < 0 || t.stride_t < 0) return AI_ERR_STRIDE;
-    // (code rows on 16 bytes, scale rows on their size)
-    const int64_t unit = i < 2 ? 16 : head_dim / kGroup * 2, size = i < 2 ? 1 : 2;
-    if (((t.stride_b | t.stride_h | t.stride_t) * size) % unit) return AI_ERR_STRIDE;
-    if (reinterpret_cast<uintptr_t>(t.ptr) % unit) return AI_ERR_ALIGN;
+    // (the slots of a page and head follow one another, from a 16-byte boundary)
+    if (t.stride_t != (i < 2 ? head_dim / 2 : head_dim / kGroup)) return AI_ERR_STRIDE;
+    if ((t.stride_b | t.stride_h) % (i < 2 ? 16 : 8)) return AI_ERR_STRIDE;
+    if (reinterpret_cast<uintptr_t>(t.ptr) & 15) return AI_ERR_ALIGN;
   }
   return AI_OK;
 }

@@ -37,18 +37,17 @@ def _pool(p, k_pages, v_pages, k_scales, v_scales, page_table, batch: int, heads
     if s[0] == 0 or s[2] < 16 or s[2] & (s[2] - 1):
         raise ValueError(f"page_size must be a power of two from 16 and the pools not empty, got {tuple(s)}")
     size = head_dim // GROUP
-    for name, x, dtype, last, unit in (("k_pages", k_pages, torch.uint8, s[3], 16), ("v_pages", v_pages, torch.uint8, s[3], 16),
-                                       ("k_scales", k_scales, torch.float16, size, size),
-                                       ("v_scales", v_scales, torch.float16, size, size)):
+    for name, x, dtype, last in (("k_pages", k_pages, torch.uint8, s[3]), ("v_pages", v_pages, torch.uint8, s[3]),
+                                 ("k_scales", k_scales, torch.float16, size), ("v_scales", v_scales, torch.float16, size)):
         if x.dtype is not dtype:
             raise TypeError(f"{name} must be {dtype}, got {x.dtype}")
         if x.shape != (*s[:3], last):
             raise ValueError(f"{name} must have shape {(*s[:3], last)}, got {tuple(x.shape)}")
-        if x.stride(3) != 1 and last > 1:
-            raise ValueError(f"{name} must have a contiguous last dimension")
         st = x.stride()
-        if (st[0] | st[1] | st[2]) % unit or x.data_ptr() % (unit * x.element_size()):
-            raise ValueError(f"the rows of {name} must start on {unit * x.element_size()}-byte boundaries")
+        if st[2] != last or (st[3] != 1 and last > 1):
+            raise ValueError(f"the slots of a page and head of {name} must follow one another")
+        if x.data_ptr() % 16 or (st[0] | st[1]) * x.element_size() % 16:
+            raise ValueError(f"the pages and heads of {name} must start on 16-byte boundaries")
         _call.on_device(name, x, index)
     page_table = _table(page_table, batch, index)
     if page_table.shape[1] == 0:
@@ -134,7 +133,8 @@ def paged_append_4bit(key: Tensor, value: Tensor, k_pages: Tensor, v_pages: Tens
     among them read back as NaN; scales are limited to 65504.  ``key`` and
     ``value`` are CUDA tensors of one dtype (bfloat16, float16, float32),
     head_dim 32, 64 or 128, any strides; page sizes are powers of two from 16,
-    the rows of codes lie on 16-byte boundaries.  Two tokens given the same
+    and the slots of a page and head follow one another in the pools, from a
+    16-byte boundary (pages and heads may be strided).  Two tokens given the same
     slot race; no gradient flows through the cache."""
     _paged(_lib.lib().ai_paged_append_4bit, "ai_paged_append_4bit",
            (key, value, k_pages, v_pages, k_scales, v_scales, page_table, lens, new_lens), "new_lens")

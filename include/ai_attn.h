@@ -730,8 +730,8 @@ int ai_distill(const AiDistillArgs* args, void* stream);
  * infinity has the scale NaN.  Pools: codes (n_pages, Hkv, page_size, D / 2)
  * bytes, scales (n_pages, Hkv, page_size, D / 32) fp16.  Dim 32 c + 4 g + j (g <
  * 8, j < 4) of a row lies in its byte g D / 16 + 2 c + j / 2, in the low half
- * for even j.  Strides of the pools are in elements (bytes, halfs); code rows
- * start on 16-byte boundaries, scale rows on boundaries of their size. */
+ * for even j.  Strides of the pools are in elements (bytes, halfs); the slots
+ * of a page and head follow one another, from a 16-byte boundary. */
 typedef struct AiPool4 {
   AiTensor4 k_codes, v_codes;   /* (n_pages, Hkv, page_size, D / 2) uint8 */
   AiTensor4 k_scales, v_scales; /* (n_pages, Hkv, page_size, D / 32) fp16 */
