@@ -8,15 +8,14 @@
 // partial results (O / l in fp32 and the log2-sum), which a second launch joins.
 //
 // A warp's tile, on 16 x 8 x 16 fp16 matrix instructions with fp32 sums:
-//   S^T = K Q^T   K's codes are exact in fp16 as 64 + c (one logical operation a
-//                 pair of codes); the sums of a group of 32 dims start at -72
-//                 sum(q), which makes them those of c - 8, and meet the group's
-//                 scale in fp32.  bf16 queries are scaled per row by a power of
-//                 two into fp16's range.
-//   O^T += V^T P  V's codes as c - 8; P takes each key's V scale in fp32, per group
-//                 of 32 dims, and is rounded once, to fp16.  P is held 2^7 above
-//                 1 for the largest |scale| met so far, so that it fits fp16 and
-//                 weights down to 2^-31 of the largest count.
+//   S^T = K Q^T   the sums of a group of 32 dims, less 8 sum(q), meet the group's
+//                 scale in fp32;
+//   O^T += V^T P  P takes each key's V scale in fp32, per group of 32 dims, and is
+//                 rounded once, to fp16.  P is held 2^7 above 1 for the largest
+//                 |scale| met so far, so that it fits fp16 and weights down to
+//                 2^-31 of the largest count.
+// The codes are fp16's subnormal numbers as they lie, 2^-24 c: one logical operation
+// a pair.  (Their 8 comes off K's after a group's sums, off V's before the product.)
 // Both products have the tile's keys on the instruction's long side, so up to 8
 // query rows of a KV head cost one column block.
 //
@@ -28,7 +27,6 @@
 
 #include <cfloat>
 #include <cstring>
-#include <type_traits>
 
 #include "ai_common.cuh"
 #include "ai_kernels.h"
@@ -46,12 +44,12 @@ constexpr int kStart = 2;      // what starting a unit costs, in tiles
 constexpr int kLeast = 4;      // positions a worker takes, at least
 constexpr int kMaxBlocks = 4;  // column blocks (of 8 query rows) of a unit, at most
 constexpr float kLift = 7.f;   // P at a weight of 1 and the largest |scale|: 2^7
-constexpr long long kWait = 1000000000LL;
 constexpr float kSlack = 8.f;  // the running maximum moves when a score passes it by 2^8
+constexpr float kNoRef = -1e30f;  // before the first score
 
-// Warps of a CTA (one per SM) and tiles of a warp's ring, by column blocks.
+// Warps of a CTA (one per SM), by column blocks.
 __host__ __device__ constexpr int warps_of(int blocks) { return blocks == 1 ? 16 : blocks == 2 ? 12 : 8; }
-__host__ __device__ constexpr int stages_of(int blocks) { return blocks <= 2 ? 3 : 4; }
+constexpr int kStages = 2;     // tiles of a warp's ring: one is loaded while one is multiplied
 
 // A tile in shared memory: codes of K and V, scales of K and V, as they lie in
 // the pools.  Row i of a product's 16 keys is key place(i): the rows that a
@@ -64,18 +62,18 @@ struct Tile {
   __device__ static int place(int i) { return (i & 8) | (i & 1 ? 4 + (i >> 1 & 3 ^ 1) : i >> 1 & 3); }
 };
 
-// A CTA's shared memory: rings, the query fragments of its warps (kept there
-// from two column blocks on), barriers, the scan.
+// A CTA's shared memory: rings, the query fragments of its warps with the
+// groups' offsets, the sequences' places on the line and lengths.
 template <int D, int NT>
 struct Smem {
-  static constexpr int W = warps_of(NT), S = stages_of(NT);
-  static constexpr int kQ = NT == 1 ? 0 : NT * (D / kGroup) * 512;
-  static constexpr int RING = 0, Q = W * S * Tile<D>::kBytes, BARS = Q + W * kQ, SCAN = BARS + W * S * 8;
-  static size_t bytes(int batch) { return SCAN + ((size_t)batch + 1) * sizeof(int); }
+  static constexpr int W = warps_of(NT), C = D / kGroup;
+  static constexpr int kQ = NT * C * 512, kOff = NT * C * 256;
+  static constexpr int RING = 0, Q = W * kStages * Tile<D>::kBytes, OFF = Q + W * kQ, SCAN = OFF + W * kOff;
+  static constexpr size_t bytes(int batch) { return SCAN + (3 * (size_t)batch + 1) * sizeof(int); }
 };
-static_assert(Smem<128, 1>::SCAN + 4 * (kMaxBatch + 1) <= 227 * 1024, "a CTA's shared memory");
-static_assert(Smem<128, 2>::SCAN + 4 * (kMaxBatch + 1) <= 227 * 1024, "a CTA's shared memory");
-static_assert(Smem<128, 4>::SCAN + 4 * (kMaxBatch + 1) <= 227 * 1024, "a CTA's shared memory");
+static_assert(Smem<128, 1>::bytes(kMaxBatch) <= 227 * 1024 && Smem<128, 2>::bytes(kMaxBatch) <= 227 * 1024 &&
+                  Smem<128, 4>::bytes(kMaxBatch) <= 227 * 1024,
+              "a CTA's shared memory");
 
 struct Plan {
   int group;       // G: query heads per KV head
@@ -137,7 +135,8 @@ struct Seg {
   int keys, n;
 };
 
-// The next stretch with tiles from position w on; false: there is none.
+// The next stretch with tiles from position w on; false: there is none.  `scan`
+// is followed by the sequences' keys and query tokens.
 __device__ __forceinline__ bool next_seg(const AiPagedAttn4Args& a, const Plan& p, const int* scan, int& w, int w1, Seg& s) {
   const int per = a.num_kv_heads * p.groups;
   while (w < w1) {
@@ -159,9 +158,8 @@ __device__ __forceinline__ bool next_seg(const AiPagedAttn4Args& a, const Plan& 
     s.hk = sub / p.groups;
     s.grp = sub - s.hk * p.groups;
     s.unit = lo * per + sub;
-    const Lens l = seq_lens(a, lo);
-    s.keys = l.keys;
-    s.n = l.n;
+    s.keys = scan[a.batch + 1 + lo];
+    s.n = scan[2 * a.batch + 1 + lo];
     return true;
   }
   return false;
@@ -184,11 +182,8 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
   return y;
 }
 
-// Bulk copy of a contiguous piece to shared memory (16-byte boundaries and size).
-__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
-  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src),
-               "r"(bytes), "r"(bar)
-               : "memory");
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
 
 // Lower (or upper) halves of two words, side by side.
@@ -210,29 +205,21 @@ __device__ __forceinline__ void lds(uint32_t (&w)[(N + 3) / 4], const uint8_t* p
   }
 }
 
-// Four pairs of codes (at bits 4 j and 16 + 4 j of x) as fp16: the bits of a
-// code at the bottom of 1024's mantissa, or above its four lowest in 64's, are
-// 1024 + c and 64 + c.  `off` taken away from the first leaves 64 + c or c - 8,
-// exactly (the logic unit is the busier one, so no shift for it).
-__device__ __forceinline__ uint32_t sub2(uint32_t x, uint16_t off) {
-  const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&x), __half2half2(__ushort_as_half(off)));
+// Four pairs of codes (at bits 4 j and 16 + 4 j of x) as fp16's subnormal numbers
+// 2^-24 c and, for odd j, 2^-20 c: the bits as they lie.
+__device__ __forceinline__ void numbers(uint32_t x, uint32_t (&f)[4]) {
+  const uint32_t y = x >> 8;
+  f[0] = x & 0x000f000fu;
+  f[1] = x & 0x00f000f0u;
+  f[2] = y & 0x000f000fu;
+  f[3] = y & 0x00f000f0u;
+}
+// Less 8 in either measure, exactly.  (A second product with a constant -8, and the
+// sums' rounding of it, costs more: 85 us for 82 on 64 sequences of up to 8192 tokens.)
+__device__ __forceinline__ uint32_t less8(uint32_t x, uint32_t off) {
+  const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&x), *reinterpret_cast<const __half2*>(&off));
   return *reinterpret_cast<const uint32_t*>(&r);
 }
-__device__ __forceinline__ void biased(uint32_t x, uint32_t (&f)[4]) {  // 64 + c
-  const uint32_t y = x >> 8;
-  f[0] = sub2((x & 0x000f000fu) | 0x64006400u, 0x6380);
-  f[1] = (x & 0x00f000f0u) | 0x54005400u;
-  f[2] = sub2((y & 0x000f000fu) | 0x64006400u, 0x6380);
-  f[3] = (y & 0x00f000f0u) | 0x54005400u;
-}
-__device__ __forceinline__ void centred(uint32_t x, uint32_t (&f)[4]) {  // c - 8
-  const uint32_t y = x >> 8;
-  f[0] = sub2((x & 0x000f000fu) | 0x64006400u, 0x6408);
-  f[1] = sub2((x & 0x00f000f0u) | 0x54005400u, 0x5480);
-  f[2] = sub2((y & 0x000f000fu) | 0x64006400u, 0x6408);
-  f[3] = sub2((y & 0x00f000f0u) | 0x54005400u, 0x5480);
-}
-
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   const __half2 h = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&h);
@@ -261,7 +248,7 @@ template <typename T, int D, int NT>
 __global__ void __launch_bounds__(32 * warps_of(NT), 1) split_kernel(const AiPagedAttn4Args a, const Plan p) {
   using L = Tile<D>;
   using M = Smem<D, NT>;
-  constexpr int C = L::C, H = (C + 1) / 2, S = M::S;
+  constexpr int C = L::C, H = (C + 1) / 2, S = kStages;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   extern __shared__ __align__(128) uint8_t smem[];
   int* scan = reinterpret_cast<int*>(smem + M::SCAN);
@@ -270,7 +257,13 @@ __global__ void __launch_bounds__(32 * warps_of(NT), 1) split_kernel(const AiPag
     int base = 0;
     for (int b0 = 0; b0 < a.batch; b0 += 32) {
       const int b = b0 + lane;
-      int v = b < a.batch ? unit_size(seq_lens(a, b)) : 0;
+      int v = 0;
+      if (b < a.batch) {
+        const Lens l = seq_lens(a, b);
+        v = unit_size(l);
+        scan[a.batch + 1 + b] = l.keys;
+        scan[2 * a.batch + 1 + b] = l.n;
+      }
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
         const int u = __shfl_up_sync(0xffffffffu, v, o);
@@ -281,9 +274,6 @@ __global__ void __launch_bounds__(32 * warps_of(NT), 1) split_kernel(const AiPag
     }
     if (lane == 0) scan[0] = 0;
   }
-  const uint32_t bars = ptx::smem_u32(smem + M::BARS) + warp * S * 8;
-  if (lane < S) ptx::mbar_init(bars + 8 * lane, 1);
-  if (lane == 0) ptx::fence_mbar_init();
   __syncthreads();
   if (blockIdx.x == 0)
     for (int b = tid; b <= a.batch; b += blockDim.x) p.scan[b] = scan[b];
@@ -294,127 +284,159 @@ __global__ void __launch_bounds__(32 * warps_of(NT), 1) split_kernel(const AiPag
   const uint8_t* ring = smem + warp * S * L::kBytes;
   const uint32_t ring_at = ptx::smem_u32(ring);
 
-  // ---- loads: lane 4 h + i copies piece i (codes of K and V, scales of K and V)
-  // of the half h of a tile, whose 16 keys lie in one page.
+  // ---- loads, S - 1 tiles ahead of the products: a half of a tile, 16 keys, lies
+  // in one page, its pieces in one stretch each.  (Bulk copies of the pieces, eight
+  // a tile, take more instructions: they are issued one by one.)
   const int page_bits = 31 - __clz(a.pool.page_size), page_mask = a.pool.page_size - 1;
-  const int half = lane / 4 & 1;
-  const AiTensor4& mine = t == 0 ? a.pool.k_codes : t == 1 ? a.pool.v_codes : t == 2 ? a.pool.k_scales : a.pool.v_scales;
-  const int unit_bytes = t < 2 ? 1 : 2, key_bytes = t < 2 ? L::kRow : 2 * C;
-  const uint32_t piece_at = (t == 0 ? L::K : t == 1 ? L::V : t == 2 ? L::KS : L::VS) + half * 16 * key_bytes;
-  const char* pool = static_cast<const char*>(mine.ptr);
-  const int64_t page_step = mine.stride_b * unit_bytes, head_step = mine.stride_h * unit_bytes;
+  constexpr int kHalfCodes = 16 * L::kRow, kHalfScales = 16 * 2 * C, kPer = kHalfScales / 16;
+  const int s_half = lane / kPer & 1;               // of the scales this lane copies, if any
+  const bool s_has = lane < 4 * kPer, s_v = lane >= 2 * kPer;
+  const AiTensor4 &kc = a.pool.k_codes, &vc = a.pool.v_codes;
+  const uint32_t s_step = (uint32_t)((s_v ? a.pool.v_scales.stride_b : a.pool.k_scales.stride_b) >> 3);  // (16-byte units)
+  const uint32_t k_step = (uint32_t)(kc.stride_b >> 4), v_step = (uint32_t)(vc.stride_b >> 4);
+  const int s_at = (s_v ? L::VS : L::KS) + s_half * kHalfScales + lane % kPer * 16;
   Seg ld;
-  int wl = w0, page = 0, in_flight = 0, at_stage = 0;
-  auto look_up = [&]() {  // the page of the lane's half
-    const int key = ld.tile * kKeys + 16 * half;
-    page = 0;
-    if (lane < 8 && key < ld.keys) {
-      page = __ldg(a.pool.page_table + ld.b * a.pool.page_table_stride + (key >> page_bits));
-      if (page < 0 || page >= a.pool.n_pages) report(a.status, AI_ERR_DEV_BOUNDS), page = 0;
-    }
+  int wl = w0, at_stage = 0, page[2] = {0, 0};
+  const uint8_t *k_from = nullptr, *v_from = nullptr, *s_from = nullptr;  // the head's, in page 0
+  auto look_up = [&]() {  // pages of the tile's halves
+    const int key = ld.tile * kKeys;
+    const int32_t* table = a.pool.page_table + ld.b * a.pool.page_table_stride + (key >> page_bits);
+    page[0] = __ldg(table);
+    page[1] = page[0];
+    if (page_bits == 4) page[1] = key + 16 < ld.keys ? __ldg(table + 1) : 0;
   };
-  bool loads = next_seg(a, p, scan, wl, w1, ld);
+  auto enter = [&]() -> bool {  // the next stretch to load
+    if (!next_seg(a, p, scan, wl, w1, ld)) return false;
+    k_from = static_cast<const uint8_t*>(kc.ptr) + ld.hk * kc.stride_h + 16 * lane;
+    v_from = static_cast<const uint8_t*>(vc.ptr) + ld.hk * vc.stride_h + 16 * lane;
+    s_from = s_v ? static_cast<const uint8_t*>(a.pool.v_scales.ptr) + 2 * ld.hk * a.pool.v_scales.stride_h
+                 : static_cast<const uint8_t*>(a.pool.k_scales.ptr) + 2 * ld.hk * a.pool.k_scales.stride_h;
+    s_from += lane % kPer * 16;
+    // (its queries on their way to L2 meanwhile)
+    const int i = ld.grp * p.unit_rows + lane, tok = i / p.group;
+    if (lane < p.unit_rows && i < p.rows)
+      asm volatile("prefetch.global.L2 [%0];" ::"l"(static_cast<const T*>(a.q.ptr) + ld.b * a.q.stride_b +
+                                                    (ld.hk * p.group + i - tok * p.group) * a.q.stride_h + tok * a.q.stride_t));
+    return true;
+  };
+  bool loads = enter();
   if (loads) look_up();
   auto issue = [&]() {
-    if (!loads) return;
-    const uint32_t bar = bars + 8 * at_stage;
-    const int key = ld.tile * kKeys + 16 * half;
-    const bool both = ld.tile * kKeys + 16 < ld.keys;
-    if (lane == 0) ptx::mbar_arrive_expect_tx(bar, (both ? 2 : 1) * 16 * (2 * L::kRow + 4 * C));
-    __syncwarp();
-    if (lane < 4 || (lane < 8 && both))
-      bulk_load(ring_at + at_stage * L::kBytes + piece_at, pool + page * page_step + ld.hk * head_step + (key & page_mask) * key_bytes,
-                16 * key_bytes, bar);
-    ++in_flight;
-    at_stage = at_stage + 1 == S ? 0 : at_stage + 1;
-    if (++ld.tile == ld.end) loads = next_seg(a, p, scan, wl, w1, ld);
-    if (loads) look_up();
+    if (loads) {
+      const int key = ld.tile * kKeys;
+      const bool both = key + 16 < ld.keys;
+      const uint32_t to = ring_at + at_stage * L::kBytes;
+      // (here, not at the look-up: the ids have had a tile's time to arrive)
+      if ((uint32_t)page[0] >= (uint32_t)a.pool.n_pages) report(a.status, AI_ERR_DEV_BOUNDS), page[0] = 0;
+      if ((uint32_t)page[1] >= (uint32_t)a.pool.n_pages) report(a.status, AI_ERR_DEV_BOUNDS), page[1] = 0;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int slot = (key + 16 * h) & page_mask;
+        const uint8_t* k = k_from + ((uint64_t)page[h] * k_step << 4) + slot * L::kRow;
+        const uint8_t* v = v_from + ((uint64_t)page[h] * v_step << 4) + slot * L::kRow;
+        const uint32_t dst = to + h * kHalfCodes + 16 * lane;
+        if ((h == 0 || both) && 16 * lane < kHalfCodes) {
+#pragma unroll
+          for (int i = 0; i < kHalfCodes; i += 512) {
+            copy16(dst + L::K + i, k + i);
+            copy16(dst + L::V + i, v + i);
+          }
+        }
+      }
+      if (s_has && (s_half == 0 || both)) {
+        const int slot = (key + 16 * s_half) & page_mask;
+        copy16(to + s_at, s_from + ((uint64_t)(s_half ? page[1] : page[0]) * s_step << 4) + slot * 2 * C);
+      }
+      at_stage = at_stage + 1 == S ? 0 : at_stage + 1;
+      if (++ld.tile == ld.end) loads = enter();
+      if (loads) look_up();
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
   };
   int st = 0;
-  uint32_t phase = 0;
-  auto arrived = [&]() -> bool {
-    if (__all_sync(0xffffffffu, ptx::mbar_try_wait(bars + 8 * st, phase))) return true;
-    return __all_sync(0xffffffffu, ptx::mbar_wait(bars + 8 * st, phase, kWait));
-  };
 #pragma unroll
   for (int i = 0; i < S - 1; ++i) issue();
 
   // ---- products
   int wc = w0;
-  bool ok = true;
   Seg s;
   const int row_g = L::place(g);  // the lane's key of a product's first eight, as they lie
+  // (a lane reads its own fragments alone)
   uint4* q_smem = reinterpret_cast<uint4*>(smem + M::Q + warp * M::kQ) + lane;
-  while (ok && next_seg(a, p, scan, wc, w1, s)) {
+  float2* off_smem = reinterpret_cast<float2*>(smem + M::OFF + warp * M::kOff) + lane;
+  while (next_seg(a, p, scan, wc, w1, s)) {
     const int row0 = s.grp * p.unit_rows, n_rows = min(p.rows - row0, p.unit_rows);
-    // Query fragments: lane (g, t) has dims 32 c + 8 t + {0 .. 7} of row 8 nt + g.
-    uint4 q_reg[C];
-    float q_off[NT][C][2];            // -72 sum(q) of rows 2 t and 2 t + 1, per group
-    float slope[NT][2];               // of the scores, in units of log 2, above zero (its sign is the fragments')
-    int seen[NT][2];                  // keys that those rows see; -1: no query
-    int least = 0x7fffffff;           // tiles that end by it are seen whole
-    const float unit = fabsf(a.scale) * kLog2e, sign = a.scale < 0.f ? -1.f : 1.f;
+    // Query fragments: lane (g, t) has dims 32 c + 8 t + {0 .. 7} of row 8 nt + g,
+    // all rows scaled by the power of two that brings the unit's largest element
+    // to the top of fp16's range (and odd dims by 2^-4, for their codes).
+    int seen[NT][2];                  // keys that rows 2 t and 2 t + 1 see; -1: no query
+    int least = s.keys;               // tiles that end by it are seen whole
+    float slope;                      // of the scores, in units of log 2, above zero (its sign is the fragments')
+    {
+      const float sign = a.scale < 0.f ? -1.f : 1.f;
+      float top = 0.f;
+      auto row_at = [&](int nt) -> const T* {
+        const int i = 8 * nt + g, r = i < n_rows ? row0 + i : row0, tok = r / p.group, head = s.hk * p.group + r - tok * p.group;
+        return static_cast<const T*>(a.q.ptr) + s.b * a.q.stride_b + head * a.q.stride_h + tok * a.q.stride_t + 8 * t;
+      };
+      float f[C][8];
+      auto load_row = [&](int nt) {
+        const T* src = row_at(nt);
+        const float keep = 8 * nt + g < n_rows ? sign : 0.f;
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      const int i = 8 * nt + g;
-      const bool has = i < n_rows;
-      const int r = has ? row0 + i : row0, tok = r / p.group, head = s.hk * p.group + r - tok * p.group;
-      const T* src = static_cast<const T*>(a.q.ptr) + s.b * a.q.stride_b + head * a.q.stride_h + tok * a.q.stride_t + 8 * t;
-      float f[C][8], top = 0.f;
+        for (int c = 0; c < C; ++c) {
+          load_q(src + kGroup * c, f[c]);
 #pragma unroll
-      for (int c = 0; c < C; ++c) {
-        load_q(src + kGroup * c, f[c]);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          f[c][e] = has ? f[c][e] * sign : 0.f;
-          top = fmaxf(top, fabsf(f[c][e]));
+          for (int e = 0; e < 8; ++e) f[c][e] = keep == 0.f ? 0.f : f[c][e] * keep;
         }
-      }
-      float slope_g = unit;
-      if constexpr (!std::is_same<T, __half>::value) {  // (fp16 holds its own)
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        const int up = top > 0.f && top < CUDART_INF_F ? 14 - ilogbf(top) : 0;
-        slope_g = ldexpf(unit, -up);
+      };
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        load_row(nt);
 #pragma unroll
         for (int c = 0; c < C; ++c)
 #pragma unroll
-          for (int e = 0; e < 8; ++e) f[c][e] = ldexpf(f[c][e], up);
+          for (int e = 0; e < 8; ++e)
+            if (fabsf(f[c][e]) < CUDART_INF_F) top = fmaxf(top, fabsf(f[c][e]));
       }
 #pragma unroll
-      for (int c = 0; c < C; ++c) {
-        uint32_t h[4];
-        float sum = 0.f;
+      for (int d = 1; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+      const int up = top > 0.f ? 14 - ilogbf(top) : 0;
+      slope = fmaxf(ldexpf(fabsf(a.scale) * kLog2e, 24 - up), FLT_MIN);  // (above 0, so that a masked score stays -inf)
+      // (in two factors: up reaches 163)
+      const float up1 = ldexpf(1.f, up / 2), up2 = ldexpf(1.f, up - up / 2);
+      __syncwarp();  // (the last unit's fragments have been read)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {  // (dims 8 t + e and 8 t + 4 + e are a pair)
-          h[e] = pack2(f[c][e], f[c][4 + e]);
-          sum += half_of(h[e], 0) + half_of(h[e], 1);
+      for (int nt = 0; nt < NT; ++nt) {
+        if (NT > 1) load_row(nt);
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+          uint32_t h[4];
+          float sum = 0.f;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {  // (dims 8 t + e and 8 t + 4 + e are a pair)
+            const float odd = e % 2 ? 0x1p-4f : 1.f;
+            h[e] = pack2(f[c][e] * up1 * up2 * odd, f[c][4 + e] * up1 * up2 * odd);
+            sum += (half_of(h[e], 0) + half_of(h[e], 1)) * (e % 2 ? 0x1p-20f : 0x1p-24f);
+          }
+          q_smem[(nt * C + c) * 32] = make_uint4(h[0], h[1], h[2], h[3]);
+          sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+          sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+          off_smem[(nt * C + c) * 32] = make_float2(-8.f * __shfl_sync(0xffffffffu, sum, 8 * t), -8.f * __shfl_sync(0xffffffffu, sum, 8 * t + 4));
         }
-        const uint4 frag = make_uint4(h[0], h[1], h[2], h[3]);
-        if constexpr (NT == 1)
-          q_reg[c] = frag;
-        else
-          q_smem[(nt * C + c) * 32] = frag;  // (its own lane's alone)
-        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
 #pragma unroll
-        for (int e = 0; e < 2; ++e) q_off[nt][c][e] = -72.f * __shfl_sync(0xffffffffu, sum, 4 * (2 * t + e));
+        for (int e = 0; e < 2; ++e) {
+          const int i2 = 8 * nt + 2 * t + e, tok2 = (row0 + i2) / p.group;
+          seen[nt][e] = i2 < n_rows && tok2 < s.n ? max(0, s.keys - s.n + tok2 + 1) : -1;
+          if (seen[nt][e] >= 0) least = min(least, seen[nt][e]);
+        }
       }
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        slope[nt][e] = fmaxf(__shfl_sync(0xffffffffu, slope_g, 4 * (2 * t + e)), FLT_MIN);  // (a masked score stays -inf)
-        const int i2 = 8 * nt + 2 * t + e, tok2 = (row0 + i2) / p.group;
-        seen[nt][e] = i2 < n_rows && tok2 < s.n ? max(0, s.keys - s.n + tok2 + 1) : -1;
-        if (seen[nt][e] >= 0) least = min(least, seen[nt][e]);
-      }
+      least = min(least, __shfl_xor_sync(0xffffffffu, least, 1));
+      least = min(least, __shfl_xor_sync(0xffffffffu, least, 2));
     }
-    least = min(least, __shfl_xor_sync(0xffffffffu, least, 1));
-    least = min(least, __shfl_xor_sync(0xffffffffu, least, 2));
-    least = min(least, s.keys);
 
-    float o[NT][2 * C][4];
-    float m[NT][2];                    // running maximum, in units of log 2
-    float ref[NT][2];                  // what the exponents are taken from: the maximum and P's place in fp16
+    float o[NT][2 * C][4];             // (odd rows of a block, of odd dims, are 2^4 times the even ones)
+    float ref[NT][2];                  // what the exponents are taken from: the running maximum and P's place in fp16
     float2 l[NT], l_before[NT];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
@@ -422,21 +444,21 @@ __global__ void __launch_bounds__(32 * warps_of(NT), 1) split_kernel(const AiPag
       for (int i = 0; i < 2 * C; ++i)
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[nt][i][e] = 0.f;
-      m[nt][0] = m[nt][1] = -CUDART_INF_F;
-      ref[nt][0] = ref[nt][1] = 0.f;
+      ref[nt][0] = ref[nt][1] = kNoRef;
       l[nt] = l_before[nt] = make_float2(0.f, 0.f);
     }
     // The largest |V scale| so far is at most 2^v_exp (v_lim in both halves; the
     // first one above 0 sets them).
     int v_exp = -24;
     uint32_t v_lim = 0;
+    float room = kSlack + kLift + 24.f;  // how far above ref a score may be: kSlack + kLift - v_exp
 
     for (int tile = s.tile; tile < s.end; ++tile) {
-      if (!(ok = arrived())) break;
+      asm volatile("cp.async.wait_group %0;" ::"n"(S - 2) : "memory");
+      __syncwarp();
       issue();  // (into the stage of the tile before: every lane has read it)
       const uint8_t* sm = ring + st * L::kBytes;
-      if (++st == S) st = 0, phase ^= 1;
-      --in_flight;
+      st = st + 1 == S ? 0 : st + 1;
       const int k0 = tile * kKeys;
 
       // Scores: keys place(g) (e = 0, 1) and 8 behind (2, 3) of half mt, rows 2 t + e % 2.
@@ -458,20 +480,17 @@ __global__ void __launch_bounds__(32 * warps_of(NT), 1) split_kernel(const AiPag
         for (int c = 0; c < C; ++c) {
           uint32_t f[2][4];
 #pragma unroll
-          for (int h = 0; h < 2; ++h) biased(C == 1 ? kw[h][0] : halves(kw[h][c / 2], kw[h][(C + c) / 2], c % 2), f[h]);
+          for (int h = 0; h < 2; ++h) numbers(C == 1 ? kw[h][0] : halves(kw[h][c / 2], kw[h][(C + c) / 2], c % 2), f[h]);
           const float k_lo = half_of(ks[0][c / 2], c % 2), k_hi = half_of(ks[1][c / 2], c % 2);
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
-            uint4 q;
-            if constexpr (NT == 1)
-              q = q_reg[c];
-            else
-              q = q_smem[(nt * C + c) * 32];
+            const uint4 q = q_smem[(nt * C + c) * 32];
+            const float2 off = off_smem[(nt * C + c) * 32];
             float acc[4];
-            mma(acc, f[0][0], f[1][0], f[0][1], f[1][1], q.x, q.y, q_off[nt][c][0], q_off[nt][c][1], q_off[nt][c][0], q_off[nt][c][1]);
+            mma(acc, f[0][0], f[1][0], f[0][1], f[1][1], q.x, q.y, 0.f, 0.f, 0.f, 0.f);
             mma(acc, f[0][2], f[1][2], f[0][3], f[1][3], q.z, q.w);
-            sc[mt][nt][0] = __ffma2_rn(make_float2(k_lo, k_lo), make_float2(acc[0], acc[1]), sc[mt][nt][0]);
-            sc[mt][nt][1] = __ffma2_rn(make_float2(k_hi, k_hi), make_float2(acc[2], acc[3]), sc[mt][nt][1]);
+            sc[mt][nt][0] = __ffma2_rn(make_float2(k_lo, k_lo), __fadd2_rn(make_float2(acc[0], acc[1]), off), sc[mt][nt][0]);
+            sc[mt][nt][1] = __ffma2_rn(make_float2(k_hi, k_hi), __fadd2_rn(make_float2(acc[2], acc[3]), off), sc[mt][nt][1]);
           }
         }
       }
@@ -498,9 +517,9 @@ __global__ void __launch_bounds__(32 * warps_of(NT), 1) split_kernel(const AiPag
       float top[NT][2];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        top[nt][0] = fmaxf(ptx::fmax3(sc[0][nt][0].x, sc[0][nt][1].x, sc[1][nt][0].x), sc[1][nt][1].x) * slope[nt][0];
-        top[nt][1] = fmaxf(ptx::fmax3(sc[0][nt][0].y, sc[0][nt][1].y, sc[1][nt][0].y), sc[1][nt][1].y) * slope[nt][1];
-        move |= top[nt][0] > m[nt][0] + kSlack || top[nt][1] > m[nt][1] + kSlack;
+        top[nt][0] = fmaxf(ptx::fmax3(sc[0][nt][0].x, sc[0][nt][1].x, sc[1][nt][0].x), sc[1][nt][1].x) * slope;
+        top[nt][1] = fmaxf(ptx::fmax3(sc[0][nt][0].y, sc[0][nt][1].y, sc[1][nt][0].y), sc[1][nt][1].y) * slope;
+        move |= top[nt][0] > ref[nt][0] + room || top[nt][1] > ref[nt][1] + room;
       }
       __half2 big = __half2half2(__ushort_as_half(0));
 #pragma unroll
@@ -524,29 +543,27 @@ __global__ void __launch_bounds__(32 * warps_of(NT), 1) split_kernel(const AiPag
             }
 #pragma unroll
         for (int d = 1; d < 32; d <<= 1) size = fmaxf(size, __shfl_xor_sync(0xffffffffu, size, d));
-        float down = 1.f;
         if (size > 0.f) {
           const int e = ilogbf(size) + 1;
           if (e > v_exp) {
-            down = ptx::ex2((float)(v_exp - e));
-            v_exp = e;
             const uint32_t h = e > 15 ? 0x7bffu : __half_as_ushort(__float2half_rn(ptx::ex2((float)e)));
+            v_exp = e;
             v_lim = h | h << 16;
           }
         }
+        const float lift = kSlack + kLift - (float)v_exp - room;  // (0 or less)
+        room += lift;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-          float alpha[2] = {down, down};
+          float alpha[2];
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            float x = top[nt][e];
+            float x = top[nt][e], to = ref[nt][e] - lift;
 #pragma unroll
             for (int d = 4; d < 32; d <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, d));
-            if (x > m[nt][e] + kSlack) {
-              if (m[nt][e] != -CUDART_INF_F) alpha[e] *= ptx::ex2(m[nt][e] - x);
-              m[nt][e] = x;
-            }
-            ref[nt][e] = (m[nt][e] == -CUDART_INF_F ? 0.f : m[nt][e]) + ((float)v_exp - kLift);
+            if (x > to + room) to = x - (room - kSlack);
+            alpha[e] = ptx::ex2(ref[nt][e] - to);
+            ref[nt][e] = to;
 #pragma unroll
             for (int i = 0; i < 2 * C; ++i) o[nt][i][e] *= alpha[e], o[nt][i][2 + e] *= alpha[e];
           }
@@ -563,7 +580,7 @@ __global__ void __launch_bounds__(32 * warps_of(NT), 1) split_kernel(const AiPag
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            const float2 y = __ffma2_rn(sc[mt][nt][h], make_float2(slope[nt][0], slope[nt][1]), make_float2(-ref[nt][0], -ref[nt][1]));
+            const float2 y = __ffma2_rn(sc[mt][nt][h], make_float2(slope, slope), make_float2(-ref[nt][0], -ref[nt][1]));
             const float2 w = make_float2(ptx::ex2(y.x), ptx::ex2(y.y));
             l[nt] = __fadd2_rn(l[nt], w);
 #pragma unroll
@@ -586,13 +603,17 @@ __global__ void __launch_bounds__(32 * warps_of(NT), 1) split_kernel(const AiPag
 #pragma unroll
         for (int c = 0; c < C; ++c) {
           uint32_t f[2][4];
-          centred(halves(vw[0][c / 2], vw[1][c / 2], c % 2), f[0]);
-          centred(halves(vw[2][c / 2], vw[3][c / 2], c % 2), f[1]);
+          numbers(halves(vw[0][c / 2], vw[1][c / 2], c % 2), f[0]);
+          numbers(halves(vw[2][c / 2], vw[3][c / 2], c % 2), f[1]);
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            mma(o[nt][2 * c], f[0][0], f[0][1], f[1][0], f[1][1], pv[nt][c][0], pv[nt][c][1]);
-            mma(o[nt][2 * c + 1], f[0][2], f[0][3], f[1][2], f[1][3], pv[nt][c][0], pv[nt][c][1]);
-          }
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) f[h][j] = less8(f[h][j], j % 2 ? 0x00800080u : 0x00080008u);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+              mma(o[nt][2 * c + i], f[0][2 * i], f[0][2 * i + 1], f[1][2 * i], f[1][2 * i + 1], pv[nt][c][0], pv[nt][c][1]);
         }
       }
       // (a sum of sums: one running sum of a long list would round its small weights away)
@@ -601,7 +622,6 @@ __global__ void __launch_bounds__(32 * warps_of(NT), 1) split_kernel(const AiPag
         for (int nt = 0; nt < NT; ++nt) l_before[nt] = __fadd2_rn(l_before[nt], l[nt]), l[nt] = make_float2(0.f, 0.f);
       }
     }
-    if (!ok) break;
     // Partial rows: dims 32 c + 4 g + {0 .. 3} of rows 2 t and 2 t + 1.
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
@@ -616,19 +636,13 @@ __global__ void __launch_bounds__(32 * warps_of(NT), 1) split_kernel(const AiPag
 #pragma unroll
         for (int c = 0; c < C; ++c)
           *reinterpret_cast<float4*>(p.part_o + row * D + kGroup * c + 4 * g) =
-              make_float4(o[nt][2 * c][e] * inv, o[nt][2 * c][2 + e] * inv, o[nt][2 * c + 1][e] * inv, o[nt][2 * c + 1][2 + e] * inv);
+              make_float4(o[nt][2 * c][e] * 0x1p24f * inv, o[nt][2 * c][2 + e] * 0x1p20f * inv, o[nt][2 * c + 1][e] * 0x1p24f * inv,
+                          o[nt][2 * c + 1][2 + e] * 0x1p20f * inv);
         // (NaN among the scores: +inf, which makes the joined row NaN)
         if (g == 0) p.part_lse[row] = sum > 0.f ? ref[nt][e] + log2f(sum) : sum == 0.f ? -CUDART_INF_F : CUDART_INF_F;
       }
   }
-  if (!ok) {
-    // A wait gave up: the copies in flight land before the warp ends.
-    if (lane == 0) report(a.status, AI_ERR_DEV_TIMEOUT);
-    for (; in_flight > 0; --in_flight) {
-      ptx::mbar_wait(bars + 8 * st, phase, kWait);
-      if (++st == S) st = 0, phase ^= 1;
-    }
-  }
+  asm volatile("cp.async.wait_all;" ::: "memory");
 }
 
 // A warp per (sequence, query token, query head) joins the row's partial results.

@@ -50,6 +50,7 @@ inline int check_pool(const AiPool4& p, int head_dim) {
     // (the slots of a page and head follow one another, from a 16-byte boundary)
     if (t.stride_t != (i < 2 ? head_dim / 2 : head_dim / kGroup)) return AI_ERR_STRIDE;
     if ((t.stride_b | t.stride_h) % (i < 2 ? 16 : 8)) return AI_ERR_STRIDE;
+    if (t.stride_b / (i < 2 ? 16 : 8) > 0xffffffffLL) return AI_ERR_STRIDE;  // (kernels count 16-byte units in 32 bits)
     if (reinterpret_cast<uintptr_t>(t.ptr) & 15) return AI_ERR_ALIGN;
   }
   return AI_OK;
