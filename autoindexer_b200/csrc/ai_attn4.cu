@@ -10,12 +10,13 @@
 // A warp's tile, on 16 x 8 x 16 fp16 matrix instructions with fp32 sums:
 //   S^T = K Q^T   the sums of a group of 32 dims, less 8 sum(q), meet the group's
 //                 scale in fp32;
-//   O^T += V^T P  P takes each key's V scale in fp32, per group of 32 dims, and is
-//                 rounded once, to fp16.  P is held 2^7 above 1 for the largest
-//                 |scale| met so far, so that it fits fp16 and weights down to
-//                 2^-31 of the largest count.
+//   O^T += V^T P  P takes each key's V scale, per group of 32 dims: weights, held 2^7
+//                 above 1 at the running maximum, and scales, divided by the power
+//                 of two above the largest |scale| met so far, are fp16, and so is
+//                 their product (two roundings of 2^-12; weights down to 2^-31 of
+//                 the largest count).
 // The codes are fp16's subnormal numbers as they lie, 2^-24 c: one logical operation
-// a pair.  (Their 8 comes off K's after a group's sums, off V's before the product.)
+// a pair.  (Their 8 comes off K's as the sums start, off V's before the product.)
 // Both products have the tile's keys on the instruction's long side, so up to 8
 // query rows of a KV head cost one column block.
 //
@@ -38,13 +39,14 @@ namespace attn4 {
 
 using namespace kv4;
 
-constexpr int kMaxBatch = 2048;  // a scan of the sequences sits in shared memory
+constexpr int kMaxBatch = 1024;  // a scan of the sequences sits in shared memory
 constexpr int kKeys = 32;      // keys of a tile
 constexpr int kStart = 2;      // what starting a unit costs, in tiles
 constexpr int kLeast = 4;      // positions a worker takes, at least
 constexpr int kMaxBlocks = 4;  // column blocks (of 8 query rows) of a unit, at most
-constexpr float kLift = 7.f;   // P at a weight of 1 and the largest |scale|: 2^7
+constexpr float kLift = 7.f;   // a weight of 1 is held as 2^7
 constexpr float kSlack = 8.f;  // the running maximum moves when a score passes it by 2^8
+constexpr int kLeastExp = -14;  // V scales below 2^-14 are divided by no less
 constexpr float kNoRef = -1e30f;  // before the first score
 
 // Warps of a CTA (one per SM), by column blocks.
@@ -67,7 +69,7 @@ struct Tile {
 template <int D, int NT>
 struct Smem {
   static constexpr int W = warps_of(NT), C = D / kGroup;
-  static constexpr int kQ = NT * C * 512, kOff = NT * C * 256;
+  static constexpr int kQ = NT * C * 512, kOff = NT * C * 512;
   static constexpr int RING = 0, Q = W * kStages * Tile<D>::kBytes, OFF = Q + W * kQ, SCAN = OFF + W * kOff;
   static constexpr size_t bytes(int batch) { return SCAN + (3 * (size_t)batch + 1) * sizeof(int); }
 };
@@ -84,7 +86,6 @@ struct Plan {
   int workers;
   float* part_o;   // [units + workers][unit_rows][D]
   float* part_lse;
-  int* scan;       // [B + 1] positions before each sequence, per unit
 };
 
 struct Lens {
@@ -240,6 +241,17 @@ __device__ __forceinline__ void load_q(const T* p, float (&f)[8]) {
   }
 }
 
+__device__ __forceinline__ __half2 as_half2(uint32_t w) { return *reinterpret_cast<const __half2*>(&w); }
+__device__ __forceinline__ uint32_t mul2(uint32_t a, uint32_t b) {
+  const __half2 r = __hmul2(as_half2(a), as_half2(b));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+// A half in both halves.
+__device__ __forceinline__ uint32_t twice(uint32_t h) { return h | h << 16; }
+__device__ __forceinline__ uint32_t twice_of(uint32_t w, int i) {
+  const __half2 r = i ? __high2half2(as_half2(w)) : __low2half2(as_half2(w));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
 __device__ __forceinline__ float half_of(uint32_t w, int i) {
   return __half2float(__ushort_as_half((unsigned short)(i ? w >> 16 : w)));
 }
@@ -275,8 +287,6 @@ __global__ void __launch_bounds__(32 * warps_of(NT), 1) split_kernel(const AiPag
     if (lane == 0) scan[0] = 0;
   }
   __syncthreads();
-  if (blockIdx.x == 0)
-    for (int b = tid; b <= a.batch; b += blockDim.x) p.scan[b] = scan[b];
   const Split line = split_line(p.workers, scan[a.batch] * a.num_kv_heads * p.groups);
   const int worker = warp * gridDim.x + blockIdx.x;  // (few workers: on as many SMs)
   if (worker >= line.n) return;
@@ -328,24 +338,38 @@ __global__ void __launch_bounds__(32 * warps_of(NT), 1) split_kernel(const AiPag
       const uint32_t to = ring_at + at_stage * L::kBytes;
       // (here, not at the look-up: the ids have had a tile's time to arrive)
       if ((uint32_t)page[0] >= (uint32_t)a.pool.n_pages) report(a.status, AI_ERR_DEV_BOUNDS), page[0] = 0;
-      if ((uint32_t)page[1] >= (uint32_t)a.pool.n_pages) report(a.status, AI_ERR_DEV_BOUNDS), page[1] = 0;
+      const int slot = key & page_mask;
+      const uint8_t* k = k_from + ((uint64_t)page[0] * k_step << 4) + slot * L::kRow;
+      const uint8_t* v = v_from + ((uint64_t)page[0] * v_step << 4) + slot * L::kRow;
+      const uint8_t* c = s_from + ((uint64_t)page[0] * s_step << 4) + slot * 2 * C;
+      const uint32_t dst = to + 16 * lane;
+      if (page_bits > 4 && both) {  // (a whole tile in one page)
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int slot = (key + 16 * h) & page_mask;
-        const uint8_t* k = k_from + ((uint64_t)page[h] * k_step << 4) + slot * L::kRow;
-        const uint8_t* v = v_from + ((uint64_t)page[h] * v_step << 4) + slot * L::kRow;
-        const uint32_t dst = to + h * kHalfCodes + 16 * lane;
-        if ((h == 0 || both) && 16 * lane < kHalfCodes) {
-#pragma unroll
-          for (int i = 0; i < kHalfCodes; i += 512) {
+        for (int i = 0; i < 2 * kHalfCodes; i += 512)
+          if (i + 16 * lane < 2 * kHalfCodes) {
             copy16(dst + L::K + i, k + i);
             copy16(dst + L::V + i, v + i);
           }
+        if (s_has) copy16(to + s_at, c + s_half * kHalfScales);
+      } else {
+        if ((uint32_t)page[1] >= (uint32_t)a.pool.n_pages) report(a.status, AI_ERR_DEV_BOUNDS), page[1] = 0;
+        const int slot1 = (key + 16) & page_mask;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          if (h == 1) {
+            k = k_from + ((uint64_t)page[1] * k_step << 4) + slot1 * L::kRow;
+            v = v_from + ((uint64_t)page[1] * v_step << 4) + slot1 * L::kRow;
+          }
+          if ((h == 0 || both) && 16 * lane < kHalfCodes) {
+#pragma unroll
+            for (int i = 0; i < kHalfCodes; i += 512) {
+              copy16(dst + L::K + h * kHalfCodes + i, k + i);
+              copy16(dst + L::V + h * kHalfCodes + i, v + i);
+            }
+          }
         }
-      }
-      if (s_has && (s_half == 0 || both)) {
-        const int slot = (key + 16 * s_half) & page_mask;
-        copy16(to + s_at, s_from + ((uint64_t)(s_half ? page[1] : page[0]) * s_step << 4) + slot * 2 * C);
+        if (s_half) c = s_from + ((uint64_t)page[1] * s_step << 4) + slot1 * 2 * C;
+        if (s_has && (s_half == 0 || both)) copy16(to + s_at, c);
       }
       at_stage = at_stage + 1 == S ? 0 : at_stage + 1;
       if (++ld.tile == ld.end) loads = enter();
@@ -363,7 +387,7 @@ __global__ void __launch_bounds__(32 * warps_of(NT), 1) split_kernel(const AiPag
   const int row_g = L::place(g);  // the lane's key of a product's first eight, as they lie
   // (a lane reads its own fragments alone)
   uint4* q_smem = reinterpret_cast<uint4*>(smem + M::Q + warp * M::kQ) + lane;
-  float2* off_smem = reinterpret_cast<float2*>(smem + M::OFF + warp * M::kOff) + lane;
+  float4* off_smem = reinterpret_cast<float4*>(smem + M::OFF + warp * M::kOff) + lane;
   while (next_seg(a, p, scan, wc, w1, s)) {
     const int row0 = s.grp * p.unit_rows, n_rows = min(p.rows - row0, p.unit_rows);
     // Query fragments: lane (g, t) has dims 32 c + 8 t + {0 .. 7} of row 8 nt + g,
@@ -422,7 +446,8 @@ __global__ void __launch_bounds__(32 * warps_of(NT), 1) split_kernel(const AiPag
           q_smem[(nt * C + c) * 32] = make_uint4(h[0], h[1], h[2], h[3]);
           sum += __shfl_xor_sync(0xffffffffu, sum, 1);
           sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-          off_smem[(nt * C + c) * 32] = make_float2(-8.f * __shfl_sync(0xffffffffu, sum, 8 * t), -8.f * __shfl_sync(0xffffffffu, sum, 8 * t + 4));
+          const float2 off = make_float2(-8.f * __shfl_sync(0xffffffffu, sum, 8 * t), -8.f * __shfl_sync(0xffffffffu, sum, 8 * t + 4));
+          off_smem[(nt * C + c) * 32] = make_float4(off.x, off.y, off.x, off.y);
         }
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
@@ -436,7 +461,7 @@ __global__ void __launch_bounds__(32 * warps_of(NT), 1) split_kernel(const AiPag
     }
 
     float o[NT][2 * C][4];             // (odd rows of a block, of odd dims, are 2^4 times the even ones)
-    float ref[NT][2];                  // what the exponents are taken from: the running maximum and P's place in fp16
+    float ref[NT][2];                  // what the exponents are taken from: the running maximum less kLift
     float2 l[NT], l_before[NT];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
@@ -447,11 +472,11 @@ __global__ void __launch_bounds__(32 * warps_of(NT), 1) split_kernel(const AiPag
       ref[nt][0] = ref[nt][1] = kNoRef;
       l[nt] = l_before[nt] = make_float2(0.f, 0.f);
     }
-    // The largest |V scale| so far is at most 2^v_exp (v_lim in both halves; the
-    // first one above 0 sets them).
-    int v_exp = -24;
-    uint32_t v_lim = 0;
-    float room = kSlack + kLift + 24.f;  // how far above ref a score may be: kSlack + kLift - v_exp
+    // The largest |V scale| so far is at most 2^v_exp (v_lim, before the first one
+    // 0; v_unit divides by it).
+    int v_exp = kLeastExp;
+    uint32_t v_lim = 0, v_unit = twice(0x7400u);
+    static_assert(kLeastExp == -14, "v_unit: 2^14");
 
     for (int tile = s.tile; tile < s.end; ++tile) {
       asm volatile("cp.async.wait_group %0;" ::"n"(S - 2) : "memory");
@@ -463,114 +488,132 @@ __global__ void __launch_bounds__(32 * warps_of(NT), 1) split_kernel(const AiPag
 
       // Scores: keys place(g) (e = 0, 1) and 8 behind (2, 3) of half mt, rows 2 t + e % 2.
       float2 sc[2][NT][2];
-      uint32_t vs[2][2][H];
-#pragma unroll
-      for (int mt = 0; mt < 2; ++mt) {
-        uint32_t kw[2][C], ks[2][H];
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int key = 16 * mt + 8 * h + row_g;
-          lds<4 * C>(kw[h], sm + L::K + key * L::kRow + 4 * C * t);
-          lds<2 * C>(ks[h], sm + L::KS + key * 2 * C);
-          lds<2 * C>(vs[mt][h], sm + L::VS + key * 2 * C);
-        }
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) sc[mt][nt][0] = sc[mt][nt][1] = make_float2(0.f, 0.f);
-#pragma unroll
-        for (int c = 0; c < C; ++c) {
-          uint32_t f[2][4];
-#pragma unroll
-          for (int h = 0; h < 2; ++h) numbers(C == 1 ? kw[h][0] : halves(kw[h][c / 2], kw[h][(C + c) / 2], c % 2), f[h]);
-          const float k_lo = half_of(ks[0][c / 2], c % 2), k_hi = half_of(ks[1][c / 2], c % 2);
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            const uint4 q = q_smem[(nt * C + c) * 32];
-            const float2 off = off_smem[(nt * C + c) * 32];
-            float acc[4];
-            mma(acc, f[0][0], f[1][0], f[0][1], f[1][1], q.x, q.y, 0.f, 0.f, 0.f, 0.f);
-            mma(acc, f[0][2], f[1][2], f[0][3], f[1][3], q.z, q.w);
-            sc[mt][nt][0] = __ffma2_rn(make_float2(k_lo, k_lo), __fadd2_rn(make_float2(acc[0], acc[1]), off), sc[mt][nt][0]);
-            sc[mt][nt][1] = __ffma2_rn(make_float2(k_hi, k_hi), __fadd2_rn(make_float2(acc[2], acc[3]), off), sc[mt][nt][1]);
-          }
-        }
-      }
-      const bool ragged = k0 + kKeys > least;
-      if (ragged) {
-#pragma unroll
-        for (int mt = 0; mt < 2; ++mt)
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const int key = k0 + 16 * mt + 8 * h + row_g;
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-              if (key >= seen[nt][0]) sc[mt][nt][h].x = -CUDART_INF_F;
-              if (key >= seen[nt][1]) sc[mt][nt][h].y = -CUDART_INF_F;
-            }
-            if (key >= s.keys) {  // (a slot that no one wrote)
-#pragma unroll
-              for (int i = 0; i < H; ++i) vs[mt][h][i] = 0;
-            }
-          }
-      }
-      // The running maximum of each row, and of the V scales, lazily.
-      bool move = false;
-      float top[NT][2];
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        top[nt][0] = fmaxf(ptx::fmax3(sc[0][nt][0].x, sc[0][nt][1].x, sc[1][nt][0].x), sc[1][nt][1].x) * slope;
-        top[nt][1] = fmaxf(ptx::fmax3(sc[0][nt][0].y, sc[0][nt][1].y, sc[1][nt][0].y), sc[1][nt][1].y) * slope;
-        move |= top[nt][0] > ref[nt][0] + room || top[nt][1] > ref[nt][1] + room;
-      }
-      __half2 big = __half2half2(__ushort_as_half(0));
+      uint32_t kw[2][2][C], ks[2][2][H], vs[2][2][H];
 #pragma unroll
       for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
+        for (int h = 0; h < 2; ++h) {
+          const int key = 16 * mt + 8 * h + row_g;
+          lds<4 * C>(kw[mt][h], sm + L::K + key * L::kRow + 4 * C * t);
+          lds<2 * C>(ks[mt][h], sm + L::KS + key * 2 * C);
+          lds<2 * C>(vs[mt][h], sm + L::VS + key * 2 * C);
 #pragma unroll
-          for (int i = 0; i < H; ++i) big = __hmax2(big, __habs2(*reinterpret_cast<const __half2*>(&vs[mt][h][i])));
-      move |= !__hble2(big, *reinterpret_cast<const __half2*>(&v_lim));
-      if (__any_sync(0xffffffffu, move)) {
-        // (an infinite scale makes what it meets infinite; it has no part in the bound)
-        float size = 0.f;
+          for (int nt = 0; nt < NT; ++nt) sc[mt][nt][h] = make_float2(0.f, 0.f);
+        }
+#pragma unroll
+      for (int c = 0; c < C; ++c) {
+        uint32_t f[2][2][4];
+#pragma unroll
+        for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) numbers(C == 1 ? kw[mt][h][0] : halves(kw[mt][h][c / 2], kw[mt][h][(C + c) / 2], c % 2), f[mt][h]);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          const uint4 q = q_smem[(nt * C + c) * 32];
+          const float4 off = off_smem[(nt * C + c) * 32];
+#pragma unroll
+          for (int mt = 0; mt < 2; ++mt) {
+            float acc[4];
+            mma(acc, f[mt][0][0], f[mt][1][0], f[mt][0][1], f[mt][1][1], q.x, q.y, off.x, off.y, off.z, off.w);
+            mma(acc, f[mt][0][2], f[mt][1][2], f[mt][0][3], f[mt][1][3], q.z, q.w);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const float d = half_of(ks[mt][h][c / 2], c % 2);
+              sc[mt][nt][h] = __ffma2_rn(make_float2(d, d), make_float2(acc[2 * h], acc[2 * h + 1]), sc[mt][nt][h]);
+            }
+          }
+        }
+      }
+      // The running maximum of each row, and of the V scales, lazily; masks where a
+      // row does not see the whole tile.
+      const bool ragged = k0 + kKeys > least;
+      float top[NT][2];
+      auto tops = [&]() -> bool {
+        bool move = false;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          top[nt][0] = fmaxf(ptx::fmax3(sc[0][nt][0].x, sc[0][nt][1].x, sc[1][nt][0].x), sc[1][nt][1].x) * slope;
+          top[nt][1] = fmaxf(ptx::fmax3(sc[0][nt][0].y, sc[0][nt][1].y, sc[1][nt][0].y), sc[1][nt][1].y) * slope;
+          move |= top[nt][0] > ref[nt][0] + (kSlack + kLift) || top[nt][1] > ref[nt][1] + (kSlack + kLift);
+        }
+        __half2 big = __half2half2(__ushort_as_half(0));
 #pragma unroll
         for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
           for (int h = 0; h < 2; ++h)
 #pragma unroll
-            for (int c = 0; c < C; ++c) {
-              const float d = fabsf(half_of(vs[mt][h][c / 2], c % 2));
-              if (d < CUDART_INF_F) size = fmaxf(size, d);
+            for (int i = 0; i < H; ++i) big = __hmax2(big, __habs2(as_half2(vs[mt][h][i])));
+        return move || !__hble2(big, as_half2(v_lim));
+      };
+      bool guard = false;  // some row must not meet an infinite or NaN scale that another sees
+      if (__any_sync(0xffffffffu, tops() || ragged)) {
+        if (ragged) {
+          bool odd = false;
+#pragma unroll
+          for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const int key = k0 + 16 * mt + 8 * h + row_g;
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt) {
+                if (key >= seen[nt][0]) sc[mt][nt][h].x = -CUDART_INF_F;
+                if (key >= seen[nt][1]) sc[mt][nt][h].y = -CUDART_INF_F;
+              }
+#pragma unroll
+              for (int i = 0; i < H; ++i) {
+                if (key >= s.keys) vs[mt][h][i] = 0;  // (a slot that no one wrote)
+                odd |= !__hble2(__habs2(as_half2(vs[mt][h][i])), as_half2(0x7bff7bffu));
+              }
             }
-#pragma unroll
-        for (int d = 1; d < 32; d <<= 1) size = fmaxf(size, __shfl_xor_sync(0xffffffffu, size, d));
-        if (size > 0.f) {
-          const int e = ilogbf(size) + 1;
-          if (e > v_exp) {
-            const uint32_t h = e > 15 ? 0x7bffu : __half_as_ushort(__float2half_rn(ptx::ex2((float)e)));
-            v_exp = e;
-            v_lim = h | h << 16;
-          }
+          guard = __any_sync(0xffffffffu, odd);
         }
-        const float lift = kSlack + kLift - (float)v_exp - room;  // (0 or less)
-        room += lift;
+        if (__any_sync(0xffffffffu, tops())) {
+          // (an infinite scale makes what it meets infinite; it has no part in the bound)
+          float size = 0.f;
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          float alpha[2];
+          for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            float x = top[nt][e], to = ref[nt][e] - lift;
+            for (int h = 0; h < 2; ++h)
 #pragma unroll
-            for (int d = 4; d < 32; d <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, d));
-            if (x > to + room) to = x - (room - kSlack);
-            alpha[e] = ptx::ex2(ref[nt][e] - to);
-            ref[nt][e] = to;
+              for (int c = 0; c < C; ++c) {
+                const float d = fabsf(half_of(vs[mt][h][c / 2], c % 2));
+                if (d < CUDART_INF_F) size = fmaxf(size, d);
+              }
 #pragma unroll
-            for (int i = 0; i < 2 * C; ++i) o[nt][i][e] *= alpha[e], o[nt][i][2 + e] *= alpha[e];
+          for (int d = 1; d < 32; d <<= 1) size = fmaxf(size, __shfl_xor_sync(0xffffffffu, size, d));
+          float down = 1.f;
+          const int e = size > 0.f ? max(ilogbf(size) + 1, kLeastExp) : kLeastExp;
+          if (e > v_exp) {
+            down = ptx::ex2((float)(v_exp - e));
+            v_exp = e;
+            v_lim = twice(e > 15 ? 0x7bffu : __half_as_ushort(__float2half_rn(ptx::ex2((float)e))));
+            v_unit = twice(__half_as_ushort(__float2half_rn(ptx::ex2((float)-e))));
           }
-          l[nt] = __fmul2_rn(l[nt], make_float2(alpha[0], alpha[1]));
-          l_before[nt] = __fmul2_rn(l_before[nt], make_float2(alpha[0], alpha[1]));
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            float alpha[2];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              float x = top[nt][e], to = ref[nt][e];
+#pragma unroll
+              for (int d = 4; d < 32; d <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, d));
+              if (x > to + (kSlack + kLift)) to = x - kLift;
+              alpha[e] = ptx::ex2(ref[nt][e] - to);
+              ref[nt][e] = to;
+#pragma unroll
+              for (int i = 0; i < 2 * C; ++i) o[nt][i][e] *= alpha[e] * down, o[nt][i][2 + e] *= alpha[e] * down;
+            }
+            l[nt] = __fmul2_rn(l[nt], make_float2(alpha[0], alpha[1]));
+            l_before[nt] = __fmul2_rn(l_before[nt], make_float2(alpha[0], alpha[1]));
+          }
         }
       }
+#pragma unroll
+      for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int i = 0; i < H; ++i) vs[mt][h][i] = mul2(vs[mt][h][i], v_unit);
       // Weights, and per group of dims the weights times the V scales as the
       // second product takes them.
 #pragma unroll
@@ -583,13 +626,10 @@ __global__ void __launch_bounds__(32 * warps_of(NT), 1) split_kernel(const AiPag
             const float2 y = __ffma2_rn(sc[mt][nt][h], make_float2(slope, slope), make_float2(-ref[nt][0], -ref[nt][1]));
             const float2 w = make_float2(ptx::ex2(y.x), ptx::ex2(y.y));
             l[nt] = __fadd2_rn(l[nt], w);
+            const uint32_t w2 = pack2(w.x, w.y);
 #pragma unroll
-            for (int c = 0; c < C; ++c) {
-              const float d = half_of(vs[mt][h][c / 2], c % 2);
-              const float2 x = __fmul2_rn(w, make_float2(d, d));
-              pv[nt][c][h] = pack2(x.x, x.y);
-            }
-            if (ragged) {  // (a key that a row does not see may have any scale)
+            for (int c = 0; c < C; ++c) pv[nt][c][h] = mul2(w2, twice_of(vs[mt][h][c / 2], c % 2));
+            if (guard) {
               const uint32_t keep = (sc[mt][nt][h].x == -CUDART_INF_F ? 0u : 0xffffu) | (sc[mt][nt][h].y == -CUDART_INF_F ? 0u : 0xffff0000u);
 #pragma unroll
               for (int c = 0; c < C; ++c) pv[nt][c][h] &= keep;
@@ -632,7 +672,7 @@ __global__ void __launch_bounds__(32 * warps_of(NT), 1) split_kernel(const AiPag
         for (int d = 4; d < 32; d <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
         if (seen[nt][e] <= 0) continue;
         const int64_t row = (int64_t)(s.unit + worker) * p.unit_rows + 8 * nt + 2 * t + e;
-        const float inv = sum == 0.f ? 0.f : 1.f / sum;
+        const float inv = sum == 0.f ? 0.f : ptx::ex2((float)v_exp) / sum;
 #pragma unroll
         for (int c = 0; c < C; ++c)
           *reinterpret_cast<float4*>(p.part_o + row * D + kGroup * c + 4 * g) =
@@ -645,53 +685,105 @@ __global__ void __launch_bounds__(32 * warps_of(NT), 1) split_kernel(const AiPag
   asm volatile("cp.async.wait_all;" ::: "memory");
 }
 
-// A warp per (sequence, query token, query head) joins the row's partial results.
+// `wide` warps per (sequence, query token, query head) join the row's partial
+// results: each takes every wide-th of them, the first adds up the warps' in order.
+// Where they lie follows from the lengths alone, which are the caller's: all of it
+// is worked out before the first launch has ended.
 template <typename T, int D>
-__global__ void __launch_bounds__(256) combine_kernel(const AiPagedAttn4Args a, const Plan p) {
-  constexpr int E = D / 32;
-  const int b = blockIdx.y, lane = threadIdx.x % 32, item = blockIdx.x * 8 + threadIdx.x / 32;
+__global__ void __launch_bounds__(256) combine_kernel(const AiPagedAttn4Args a, const Plan p, const int wide) {
+  constexpr int E = D / 32, kAhead = 4;
+  __shared__ int s_sum[2][8];
+  __shared__ float s_acc[8][D + 2];
+  const int b = blockIdx.y, tid = threadIdx.x, lane = tid % 32, warp = tid / 32, part = warp % wide;
+  // Positions before sequence b, and all.
+  int before = 0, all = 0;
+  for (int i = tid; i < a.batch; i += 256) {
+    const int v = unit_size(seq_lens(a, i));
+    all += v;
+    if (i < b) before += v;
+  }
+  before = __reduce_add_sync(0xffffffffu, before);
+  all = __reduce_add_sync(0xffffffffu, all);
+  if (lane == 0) s_sum[0][warp] = before, s_sum[1][warp] = all;
+  __syncthreads();
+  before = all = 0;
+  for (int w = 0; w < 8; ++w) before += s_sum[0][w], all += s_sum[1][w];
+  const Lens len = seq_lens(a, b);
+  const int item = blockIdx.x * (8 / wide) + warp / wide;
   const bool has = item < a.seq_len * a.num_q_heads;
-  const int t = has ? item / a.num_q_heads : 0, h = has ? item % a.num_q_heads : 0, hk = h / p.group;
-  const Lens len = seq_lens(a, b);  // (the caller's lengths: read before the wait)
+  const int t = has ? item / a.num_q_heads : 0, h = has ? item - t * a.num_q_heads : 0, hk = h / p.group;
   const int seen = has && t < len.n ? len.keys - len.n + t + 1 : 0;
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  if (!has) return;
+  int n = 0;
+  int64_t row = 0;
+  if (seen > 0) {
+    const int per = a.num_kv_heads * p.groups, size = unit_size(len);
+    const Split line = split_line(p.workers, all * per);
+    const int i = t * p.group + h - hk * p.group, grp = i / p.unit_rows, sub = hk * p.groups + grp;
+    const int x = before * per + sub * size + kStart, tiles = (seen - 1) / kKeys + 1;
+    const int first = line.worker(x);
+    n = line.worker(x + tiles - 1) - first + 1;
+    row = (int64_t)(b * per + sub + first) * p.unit_rows + i - grp * p.unit_rows;
+  }
+  auto row_at = [&](int k) { return row + (int64_t)k * p.unit_rows; };
+  auto load = [&](int k, float (&o)[E]) {
+    const float* src = p.part_o + row_at(k) * D + E * lane;
+    if constexpr (E == 4)
+      *reinterpret_cast<float4*>(o) = *reinterpret_cast<const float4*>(src);
+    else if constexpr (E == 2)
+      *reinterpret_cast<float2*>(o) = *reinterpret_cast<const float2*>(src);
+    else
+      o[0] = *src;
+  };
   float M = -CUDART_INF_F, sum = 0.f, acc[E];
 #pragma unroll
   for (int e = 0; e < E; ++e) acc[e] = 0.f;
-  if (seen > 0) {
-    const int per = a.num_kv_heads * p.groups, s0 = p.scan[b], size = p.scan[b + 1] - s0;
-    const Split line = split_line(p.workers, p.scan[a.batch] * per);
-    const int i = t * p.group + h - hk * p.group, grp = i / p.unit_rows, sub = hk * p.groups + grp;
-    const int x = s0 * per + sub * size + kStart, tiles = min((seen - 1) / kKeys + 1, size - kStart);
-    const int first = line.worker(x), n = line.worker(x + tiles - 1) - first + 1;
-    const int64_t row = (int64_t)(b * per + sub + first) * p.unit_rows + i - grp * p.unit_rows;
-    auto row_at = [&](int k) { return row + (int64_t)k * p.unit_rows; };
-    for (int k = lane; k < n; k += 32) M = fmaxf(M, p.part_lse[row_at(k)]);
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  // (the first rows are on their way beside the sums' logarithms)
+  float ahead[kAhead][E];
 #pragma unroll
-    for (int d = 16; d > 0; d >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, d));
-    if (M != -CUDART_INF_F) {
-      for (int k0 = 0; k0 < n; k0 += 32) {
-        const float mine = k0 + lane < n ? exp2f(p.part_lse[row_at(k0 + lane)] - M) : 0.f;
-        const int cnt = min(32, n - k0);
+  for (int k = 0; k < kAhead; ++k)
+    if (part + k * wide < n) load(part + k * wide, ahead[k]);
+  for (int k = lane; k < n; k += 32) M = fmaxf(M, p.part_lse[row_at(k)]);
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, d));
+  if (M != -CUDART_INF_F) {
+    for (int k0 = part; k0 < n; k0 += 32 * wide) {
+      const int mine = k0 + lane * wide;
+      const float my_w = mine < n ? exp2f(p.part_lse[row_at(mine)] - M) : 0.f;
+      const int cnt = min(32, (n - k0 + wide - 1) / wide);
+      auto add = [&](int k, const float (&o)[E]) {
+        const float w = __shfl_sync(0xffffffffu, my_w, k);
+        sum += w;
+#pragma unroll
+        for (int e = 0; e < E; ++e) acc[e] = fmaf(w, o[e], acc[e]);
+      };
+      int k = 0;
+      if (k0 == part) {
+#pragma unroll
+        for (; k < kAhead; ++k)
+          if (k < cnt) add(k, ahead[k]);
+      }
 #pragma unroll 4
-        for (int k = 0; k < cnt; ++k) {
-          const float w = __shfl_sync(0xffffffffu, mine, k);
-          const float* src = p.part_o + row_at(k0 + k) * D + E * lane;
-          float o[E];
-          if constexpr (E == 4)
-            *reinterpret_cast<float4*>(o) = *reinterpret_cast<const float4*>(src);
-          else if constexpr (E == 2)
-            *reinterpret_cast<float2*>(o) = *reinterpret_cast<const float2*>(src);
-          else
-            o[0] = *src;
-          sum += w;
-#pragma unroll
-          for (int e = 0; e < E; ++e) acc[e] = fmaf(w, o[e], acc[e]);
-        }
+      for (; k < cnt; ++k) {
+        float o[E];
+        load(k0 + k * wide, o);
+        add(k, o);
       }
     }
   }
+  if (wide > 1) {
+#pragma unroll
+    for (int e = 0; e < E; ++e) s_acc[warp][E * lane + e] = acc[e];
+    if (lane == 0) s_acc[warp][D] = sum;
+    __syncthreads();
+    if (part > 0) return;
+    for (int w = 1; w < wide; ++w) {
+      sum += s_acc[warp + w][D];
+#pragma unroll
+      for (int e = 0; e < E; ++e) acc[e] += s_acc[warp + w][E * lane + e];
+    }
+  }
+  if (!has) return;
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
   T* out = static_cast<T*>(const_cast<void*>(a.out.ptr)) + b * a.out.stride_b + h * a.out.stride_h + t * a.out.stride_t + E * lane;
 #pragma unroll
@@ -739,8 +831,7 @@ size_t layout(const AiPagedAttn4Args& a, Plan* p) {
   char* w = static_cast<char*>(a.workspace);
   p->part_o = reinterpret_cast<float*>(w);
   p->part_lse = reinterpret_cast<float*>(w + o);
-  p->scan = reinterpret_cast<int*>(w + o + l);
-  return o + l + (((size_t)a.batch + 1) * sizeof(int) + 255) / 256 * 256;
+  return o + l;
 }
 
 template <typename T, int D, int NT>
@@ -760,8 +851,11 @@ int run(const AiPagedAttn4Args& a, const Plan& p, cudaStream_t st) {
                  : p.blocks == 3 ? launch<T, D, 3>(a, p, st)
                                  : launch<T, D, 4>(a, p, st);
   if (rc != AI_OK) return rc;
+  // Warps that join a row: by the partial results it has, where the lists are alike.
+  const int64_t parts = p.workers / ((int64_t)a.batch * a.num_kv_heads * p.groups);
+  const int wide = parts >= 32 ? 8 : parts >= 16 ? 4 : parts >= 8 ? 2 : 1;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)((a.seq_len * (int64_t)a.num_q_heads + 7) / 8), a.batch);
+  cfg.gridDim = dim3((unsigned)((a.seq_len * (int64_t)a.num_q_heads * wide + 7) / 8), a.batch);
   cfg.blockDim = dim3(256);
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
@@ -769,7 +863,7 @@ int run(const AiPagedAttn4Args& a, const Plan& p, cudaStream_t st) {
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  if (cudaLaunchKernelEx(&cfg, combine_kernel<T, D>, a, p) != cudaSuccess) return AI_ERR_LAUNCH;
+  if (cudaLaunchKernelEx(&cfg, combine_kernel<T, D>, a, p, wide) != cudaSuccess) return AI_ERR_LAUNCH;
   return cudaGetLastError() == cudaSuccess ? AI_OK : AI_ERR_LAUNCH;
 }
 

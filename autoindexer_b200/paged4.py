@@ -24,7 +24,7 @@ from .paged import _table
 
 __all__ = ["paged_append_4bit", "paged_read_4bit", "paged_attention_4bit"]
 
-MAX_BATCH = 2048  # sequences of an attention call
+MAX_BATCH = 1024  # sequences of an attention call
 GROUP = 32
 
 
@@ -203,7 +203,7 @@ def paged_attention_4bit(query: Tensor, k_pages: Tensor, v_pages: Tensor, k_scal
 
     Keys and values are taken as the cache stands for them, exactly; sums and
     the softmax are float32.  Slots that no query of the sequence sees may hold
-    anything.  Up to 2048 sequences, head_dim 32, 64 or 128, any strides of the
+    anything.  Up to 1024 sequences, head_dim 32, 64 or 128, any strides of the
     query; the pools as ``paged_append_4bit`` takes them.  A length or page out
     of range is clamped and sets the status word.  There is no gradient: a
     backward through the results raises."""

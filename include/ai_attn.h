@@ -770,7 +770,7 @@ int ai_paged_read_4bit(const AiPaged4Args* args, void* stream);
  * key give 0 (lse -inf).  Slots that no query of the sequence sees may hold
  * anything, also within a page. */
 typedef struct AiPagedAttn4Args {
-  int32_t batch;              /* up to 2048 */
+  int32_t batch;              /* up to 1024 */
   int32_t seq_len;            /* T: query tokens per sequence */
   int32_t num_q_heads;
   int32_t num_kv_heads;

@@ -552,7 +552,7 @@ def test_refusals(cuda_device):
         (ValueError, (q, *cache, table[0], n)), (ValueError, (q, *cache, table[:, :0], n)), (ValueError, (q, *cache, table, n[:1])),
         (ValueError, (q.expand(2, 4, 1, 64)[:, :, :0], *cache, table, n)), (TypeError, (q.float(), *cache, table, n)),
         (TypeError, (q, *cache, table.long(), n)), (TypeError, (q, *cache, table, n.long())), (RuntimeError, (q, *cache, table, n.cpu())),
-        (ValueError, (q[:1].expand(2049, 4, 1, 64), *cache, table[:1].expand(2049, -1), n[:1].expand(2049))),
+        (ValueError, (q[:1].expand(1025, 4, 1, 64), *cache, table[:1].expand(1025, -1), n[:1].expand(1025))),
     ]:
         with pytest.raises(error):
             paged_attention_4bit(*args)
@@ -629,7 +629,7 @@ def test_c_abi_refusals():
             assert fn(paged(**{field: value}), None) == code, field
     assert L.ai_paged_attn_4bit(None, None) == 1 and L.ai_paged_attn_4bit_workspace(None, ctypes.byref(n)) == 1
     assert L.ai_paged_attn_4bit_workspace(attn(), None) == 1
-    for field, value, code in pool + (("batch", 2049, 2), ("seq_len", 0, 2), ("num_q_heads", 5, 2), ("head_dim", 16, 3),
+    for field, value, code in pool + (("batch", 1025, 2), ("seq_len", 0, 2), ("num_q_heads", 5, 2), ("head_dim", 16, 3),
                                       ("dtype", _lib.DTYPE_F32, 4), ("q__ptr", None, 1), ("out__stride_h", -1, 5)):
         assert L.ai_paged_attn_4bit(attn(**{field: value}), None) == code, field
         assert L.ai_paged_attn_4bit_workspace(attn(**{field: value}), ctypes.byref(n)) == code, field
