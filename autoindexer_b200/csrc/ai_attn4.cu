@@ -1,7 +1,7 @@
 // Attention over the paged cache in 4 bits (declared in include/ai_attn.h; the
 // format at AiPool4).
 //
-// A unit is a (sequence, KV head, group of up to 32 query rows); its keys are
+// A unit is a (sequence, KV head, group of up to 24 query rows); its keys are
 // cut into tiles of 32, the tiles of all units stand in one line, and each worker,
 // a warp, takes an equal stretch of the line, whatever the lengths are (they
 // are read on the device).  The rows of a unit that a worker touched leave
@@ -41,16 +41,16 @@ using namespace kv4;
 
 constexpr int kMaxBatch = 1024;  // a scan of the sequences sits in shared memory
 constexpr int kKeys = 32;      // keys of a tile
-constexpr int kStart = 2;      // what starting a unit costs, in tiles
+constexpr int kStart = 4;      // what starting a unit costs, in tiles
 constexpr int kLeast = 4;      // positions a worker takes, at least
-constexpr int kMaxBlocks = 4;  // column blocks (of 8 query rows) of a unit, at most
+constexpr int kMaxBlocks = 3;  // column blocks (of 8 query rows) of a unit, at most (four do not fit the registers)
 constexpr float kLift = 7.f;   // a weight of 1 is held as 2^7
 constexpr float kSlack = 8.f;  // the running maximum moves when a score passes it by 2^8
 constexpr int kLeastExp = -14;  // V scales below 2^-14 are divided by no less
 constexpr float kNoRef = -1e30f;  // before the first score
 
 // Warps of a CTA (one per SM), by column blocks.
-__host__ __device__ constexpr int warps_of(int blocks) { return blocks == 1 ? 16 : blocks == 2 ? 12 : 8; }
+__host__ __device__ constexpr int warps_of(int blocks) { return blocks == 1 ? 16 : 8; }
 constexpr int kStages = 2;     // tiles of a warp's ring: one is loaded while one is multiplied
 
 // A tile in shared memory: codes of K and V, scales of K and V, as they lie in
@@ -74,7 +74,7 @@ struct Smem {
   static constexpr size_t bytes(int batch) { return SCAN + (3 * (size_t)batch + 1) * sizeof(int); }
 };
 static_assert(Smem<128, 1>::bytes(kMaxBatch) <= 227 * 1024 && Smem<128, 2>::bytes(kMaxBatch) <= 227 * 1024 &&
-                  Smem<128, 4>::bytes(kMaxBatch) <= 227 * 1024,
+                  Smem<128, 3>::bytes(kMaxBatch) <= 227 * 1024,
               "a CTA's shared memory");
 
 struct Plan {
@@ -226,19 +226,24 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-// Eight elements of a query row, any strides of the rows.
+// Eight elements of a query row, any strides of the rows; and one of them.
 template <typename T>
-__device__ __forceinline__ void load_q(const T* p, float (&f)[8]) {
-  if ((reinterpret_cast<uintptr_t>(p) & 15) == 0) {
-    const uint4 r = __ldg(reinterpret_cast<const uint4*>(p));
-    T e[8];
-    memcpy(e, &r, 16);
+__device__ __forceinline__ uint4 load_q(const T* p) {
+  if ((reinterpret_cast<uintptr_t>(p) & 15) == 0) return __ldg(reinterpret_cast<const uint4*>(p));
+  T e[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = to_f32(e[i]);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = to_f32(p[i]);
-  }
+  for (int i = 0; i < 8; ++i) e[i] = p[i];
+  uint4 r;
+  memcpy(&r, e, 16);
+  return r;
+}
+template <typename T>
+__device__ __forceinline__ float element(const uint4& r, int i) {
+  const uint32_t w = i < 2 ? r.x : i < 4 ? r.y : i < 6 ? r.z : r.w;
+  const uint16_t h = (uint16_t)(i % 2 ? w >> 16 : w);
+  T x;
+  memcpy(&x, &h, 2);
+  return to_f32(x);
 }
 
 __device__ __forceinline__ __half2 as_half2(uint32_t w) { return *reinterpret_cast<const __half2*>(&w); }
@@ -393,46 +398,47 @@ __global__ void __launch_bounds__(32 * warps_of(NT), 1) split_kernel(const AiPag
     // Query fragments: lane (g, t) has dims 32 c + 8 t + {0 .. 7} of row 8 nt + g,
     // all rows scaled by the power of two that brings the unit's largest element
     // to the top of fp16's range (and odd dims by 2^-4, for their codes).
-    int seen[NT][2];                  // keys that rows 2 t and 2 t + 1 see; -1: no query
+    // Keys that row 8 nt + 2 t + e sees; -1: no query.  (Looked up where it is
+    // wanted when registers are short.)
+    auto count = [&](int nt, int e) -> int {
+      const int i = 8 * nt + 2 * t + e, tok = (row0 + i) / p.group;
+      return i < n_rows && tok < s.n ? max(0, s.keys - s.n + tok + 1) : -1;
+    };
+    const int first[2] = {count(0, 0), count(0, 1)};
+    auto seen = [&](int nt, int e) -> int { return NT == 1 ? first[e] : count(nt, e); };
     int least = s.keys;               // tiles that end by it are seen whole
     float slope;                      // of the scores, in units of log 2, above zero (its sign is the fragments')
     {
       const float sign = a.scale < 0.f ? -1.f : 1.f;
-      float top = 0.f;
-      auto row_at = [&](int nt) -> const T* {
-        const int i = 8 * nt + g, r = i < n_rows ? row0 + i : row0, tok = r / p.group, head = s.hk * p.group + r - tok * p.group;
-        return static_cast<const T*>(a.q.ptr) + s.b * a.q.stride_b + head * a.q.stride_h + tok * a.q.stride_t + 8 * t;
-      };
-      float f[C][8];
-      auto load_row = [&](int nt) {
-        const T* src = row_at(nt);
-        const float keep = 8 * nt + g < n_rows ? sign : 0.f;
-#pragma unroll
-        for (int c = 0; c < C; ++c) {
-          load_q(src + kGroup * c, f[c]);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) f[c][e] = keep == 0.f ? 0.f : f[c][e] * keep;
-        }
-      };
+      uint4 raw[NT][C];  // (all of them in flight at once)
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        load_row(nt);
+        const int i = 8 * nt + g, r = i < n_rows ? row0 + i : row0, tok = r / p.group, head = s.hk * p.group + r - tok * p.group;
+        const T* src = static_cast<const T*>(a.q.ptr) + s.b * a.q.stride_b + head * a.q.stride_h + tok * a.q.stride_t + 8 * t;
 #pragma unroll
-        for (int c = 0; c < C; ++c)
-#pragma unroll
-          for (int e = 0; e < 8; ++e)
-            if (fabsf(f[c][e]) < CUDART_INF_F) top = fmaxf(top, fabsf(f[c][e]));
+        for (int c = 0; c < C; ++c) raw[nt][c] = load_q(src + kGroup * c);
       }
+      float top = 0.f;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+          if (8 * nt + g >= n_rows) raw[nt][c] = make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const float f = fabsf(element<T>(raw[nt][c], e));
+            if (f < CUDART_INF_F) top = fmaxf(top, f);
+          }
+        }
 #pragma unroll
       for (int d = 1; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
       const int up = top > 0.f ? 14 - ilogbf(top) : 0;
       slope = fmaxf(ldexpf(fabsf(a.scale) * kLog2e, 24 - up), FLT_MIN);  // (above 0, so that a masked score stays -inf)
       // (in two factors: up reaches 163)
-      const float up1 = ldexpf(1.f, up / 2), up2 = ldexpf(1.f, up - up / 2);
+      const float up1 = sign * ldexpf(1.f, up / 2), up2 = ldexpf(1.f, up - up / 2);
       __syncwarp();  // (the last unit's fragments have been read)
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        if (NT > 1) load_row(nt);
 #pragma unroll
         for (int c = 0; c < C; ++c) {
           uint32_t h[4];
@@ -440,7 +446,7 @@ __global__ void __launch_bounds__(32 * warps_of(NT), 1) split_kernel(const AiPag
 #pragma unroll
           for (int e = 0; e < 4; ++e) {  // (dims 8 t + e and 8 t + 4 + e are a pair)
             const float odd = e % 2 ? 0x1p-4f : 1.f;
-            h[e] = pack2(f[c][e] * up1 * up2 * odd, f[c][4 + e] * up1 * up2 * odd);
+            h[e] = pack2(element<T>(raw[nt][c], e) * up1 * up2 * odd, element<T>(raw[nt][c], 4 + e) * up1 * up2 * odd);
             sum += (half_of(h[e], 0) + half_of(h[e], 1)) * (e % 2 ? 0x1p-20f : 0x1p-24f);
           }
           q_smem[(nt * C + c) * 32] = make_uint4(h[0], h[1], h[2], h[3]);
@@ -451,9 +457,8 @@ __global__ void __launch_bounds__(32 * warps_of(NT), 1) split_kernel(const AiPag
         }
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const int i2 = 8 * nt + 2 * t + e, tok2 = (row0 + i2) / p.group;
-          seen[nt][e] = i2 < n_rows && tok2 < s.n ? max(0, s.keys - s.n + tok2 + 1) : -1;
-          if (seen[nt][e] >= 0) least = min(least, seen[nt][e]);
+          const int n = seen(nt, e);
+          if (n >= 0) least = min(least, n);
         }
       }
       least = min(least, __shfl_xor_sync(0xffffffffu, least, 1));
@@ -488,38 +493,45 @@ __global__ void __launch_bounds__(32 * warps_of(NT), 1) split_kernel(const AiPag
 
       // Scores: keys place(g) (e = 0, 1) and 8 behind (2, 3) of half mt, rows 2 t + e % 2.
       float2 sc[2][NT][2];
-      uint32_t kw[2][2][C], ks[2][2][H], vs[2][2][H];
+      uint32_t vs[2][2][H];
+      // (both halves at once share their query fragments; with more column blocks
+      // the registers are the blocks')
+      constexpr int kAtOnce = NT == 1 ? 2 : 1;
 #pragma unroll
-      for (int mt = 0; mt < 2; ++mt)
+      for (int m0 = 0; m0 < 2; m0 += kAtOnce) {
+        uint32_t kw[kAtOnce][2][C], ks[kAtOnce][2][H];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int key = 16 * mt + 8 * h + row_g;
-          lds<4 * C>(kw[mt][h], sm + L::K + key * L::kRow + 4 * C * t);
-          lds<2 * C>(ks[mt][h], sm + L::KS + key * 2 * C);
-          lds<2 * C>(vs[mt][h], sm + L::VS + key * 2 * C);
+        for (int i = 0; i < kAtOnce; ++i)
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) sc[mt][nt][h] = make_float2(0.f, 0.f);
-        }
+          for (int h = 0; h < 2; ++h) {
+            const int key = 16 * (m0 + i) + 8 * h + row_g;
+            lds<4 * C>(kw[i][h], sm + L::K + key * L::kRow + 4 * C * t);
+            lds<2 * C>(ks[i][h], sm + L::KS + key * 2 * C);
+            lds<2 * C>(vs[m0 + i][h], sm + L::VS + key * 2 * C);
 #pragma unroll
-      for (int c = 0; c < C; ++c) {
-        uint32_t f[2][2][4];
+            for (int nt = 0; nt < NT; ++nt) sc[m0 + i][nt][h] = make_float2(0.f, 0.f);
+          }
 #pragma unroll
-        for (int mt = 0; mt < 2; ++mt)
+        for (int c = 0; c < C; ++c) {
+          uint32_t f[kAtOnce][2][4];
 #pragma unroll
-          for (int h = 0; h < 2; ++h) numbers(C == 1 ? kw[mt][h][0] : halves(kw[mt][h][c / 2], kw[mt][h][(C + c) / 2], c % 2), f[mt][h]);
+          for (int i = 0; i < kAtOnce; ++i)
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          const uint4 q = q_smem[(nt * C + c) * 32];
-          const float4 off = off_smem[(nt * C + c) * 32];
+            for (int h = 0; h < 2; ++h) numbers(C == 1 ? kw[i][h][0] : halves(kw[i][h][c / 2], kw[i][h][(C + c) / 2], c % 2), f[i][h]);
 #pragma unroll
-          for (int mt = 0; mt < 2; ++mt) {
-            float acc[4];
-            mma(acc, f[mt][0][0], f[mt][1][0], f[mt][0][1], f[mt][1][1], q.x, q.y, off.x, off.y, off.z, off.w);
-            mma(acc, f[mt][0][2], f[mt][1][2], f[mt][0][3], f[mt][1][3], q.z, q.w);
+          for (int nt = 0; nt < NT; ++nt) {
+            const uint4 q = q_smem[(nt * C + c) * 32];
+            const float4 off = off_smem[(nt * C + c) * 32];
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              const float d = half_of(ks[mt][h][c / 2], c % 2);
-              sc[mt][nt][h] = __ffma2_rn(make_float2(d, d), make_float2(acc[2 * h], acc[2 * h + 1]), sc[mt][nt][h]);
+            for (int i = 0; i < kAtOnce; ++i) {
+              float acc[4];
+              mma(acc, f[i][0][0], f[i][1][0], f[i][0][1], f[i][1][1], q.x, q.y, off.x, off.y, off.z, off.w);
+              mma(acc, f[i][0][2], f[i][1][2], f[i][0][3], f[i][1][3], q.z, q.w);
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                const float d = half_of(ks[i][h][c / 2], c % 2);
+                sc[m0 + i][nt][h] = __ffma2_rn(make_float2(d, d), make_float2(acc[2 * h], acc[2 * h + 1]), sc[m0 + i][nt][h]);
+              }
             }
           }
         }
@@ -550,15 +562,21 @@ __global__ void __launch_bounds__(32 * warps_of(NT), 1) split_kernel(const AiPag
         if (ragged) {
           bool odd = false;
 #pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            const int s0 = seen(nt, 0) - k0 - row_g, s1 = seen(nt, 1) - k0 - row_g;
+#pragma unroll
+            for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                if (16 * mt + 8 * h >= s0) sc[mt][nt][h].x = -CUDART_INF_F;
+                if (16 * mt + 8 * h >= s1) sc[mt][nt][h].y = -CUDART_INF_F;
+              }
+          }
+#pragma unroll
           for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
               const int key = k0 + 16 * mt + 8 * h + row_g;
-#pragma unroll
-              for (int nt = 0; nt < NT; ++nt) {
-                if (key >= seen[nt][0]) sc[mt][nt][h].x = -CUDART_INF_F;
-                if (key >= seen[nt][1]) sc[mt][nt][h].y = -CUDART_INF_F;
-              }
 #pragma unroll
               for (int i = 0; i < H; ++i) {
                 if (key >= s.keys) vs[mt][h][i] = 0;  // (a slot that no one wrote)
@@ -670,7 +688,7 @@ __global__ void __launch_bounds__(32 * warps_of(NT), 1) split_kernel(const AiPag
         float sum = e ? l_before[nt].y + l[nt].y : l_before[nt].x + l[nt].x;
 #pragma unroll
         for (int d = 4; d < 32; d <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-        if (seen[nt][e] <= 0) continue;
+        if (seen(nt, e) <= 0) continue;
         const int64_t row = (int64_t)(s.unit + worker) * p.unit_rows + 8 * nt + 2 * t + e;
         const float inv = sum == 0.f ? 0.f : ptx::ex2((float)v_exp) / sum;
 #pragma unroll
@@ -848,8 +866,7 @@ int run(const AiPagedAttn4Args& a, const Plan& p, cudaStream_t st) {
   ProfScope ps(AI_PROF_ATTN4, st);
   const int rc = p.blocks == 1   ? launch<T, D, 1>(a, p, st)
                  : p.blocks == 2 ? launch<T, D, 2>(a, p, st)
-                 : p.blocks == 3 ? launch<T, D, 3>(a, p, st)
-                                 : launch<T, D, 4>(a, p, st);
+                                 : launch<T, D, 3>(a, p, st);
   if (rc != AI_OK) return rc;
   // Warps that join a row: by the partial results it has, where the lists are alike.
   const int64_t parts = p.workers / ((int64_t)a.batch * a.num_kv_heads * p.groups);
