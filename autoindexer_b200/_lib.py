@@ -37,6 +37,7 @@ ABI_VERSION = 9
 BWD_DQ, BWD_DKDV = 1, 2
 TAILS = {"bucket": 0, "renormalize": 1}  # AiTail
 MAX_TOP = 128  # AI_SCORE_MAX_TOP, AI_DISTILL_MAX_TOP
+MAX_ROW_BYTES = 3145728  # AI_DISTILL_MAX_ROW_BYTES
 
 # Every function include/ai_attn.h declares.
 EXPORTED_SYMBOLS = (

@@ -177,7 +177,7 @@ __device__ __forceinline__ float row_tau(const float* temperature, int64_t b, in
   return 1.f;
 }
 
-// A row cut for `splits` CTAs of `threads`: whole 16-byte vectors [i0, i1) of
+// A row cut for `splits` CTAs, in units of `unit` vectors: whole 16-byte vectors [i0, i1) of
 // the row from its first boundary (element `head`), in the CTA's slice, and the
 // elements [e0, e1) that the slice covers with the row's ragged ends, which the
 // first and the last slice have.
@@ -188,14 +188,14 @@ struct Slice {
 };
 
 template <typename T>
-__device__ __forceinline__ Slice slice_of(const T* row, int vocab, int split, int splits, int threads) {
+__device__ __forceinline__ Slice slice_of(const T* row, int vocab, int split, int splits, int unit) {
   constexpr int E = 16 / sizeof(T);
   Slice r;
   const int mis = (int)((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(T));
   r.head = min(vocab, (E - mis) % E);
   const int vecs = (vocab - r.head) / E;
   r.tail = r.head + vecs * E;
-  const int per = ((vecs + splits - 1) / splits + threads - 1) / threads * threads;
+  const int per = ((vecs + splits - 1) / splits + unit - 1) / unit * unit;
   r.i0 = min(vecs, split * per);
   r.i1 = min(vecs, r.i0 + per);
   r.e0 = split == 0 ? 0 : r.head + r.i0 * E;

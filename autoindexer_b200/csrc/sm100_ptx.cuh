@@ -89,6 +89,14 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map
       : "memory");
 }
 
+// Bulk copy of a contiguous piece to shared memory (16-byte boundaries and size),
+// completing on `bar`.
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src),
+               "r"(bytes), "r"(bar)
+               : "memory");
+}
+
 // Tiled TMA store of a shared-memory box to global memory (bulk-group
 // completion, this CTA's box only).  The writing threads must have made their smem
 // stores visible to the async proxy (fence_proxy_async_smem + a barrier).

@@ -28,6 +28,8 @@ def _plan(logits, ids, logprobs, weights, temperature, tail):
     argument struct without pointers."""
     a = _lib.AiDistillArgs()
     logits, rows, index = check_rows(a, "student_logits", logits)
+    if logits.shape[-1] * logits.element_size() > _lib.MAX_ROW_BYTES:
+        raise ValueError(f"a row of student_logits may have {_lib.MAX_ROW_BYTES} bytes at most, got {tuple(logits.shape)} of {logits.dtype}")
     if tail not in _lib.TAILS:
         raise ValueError(f"tail must be one of {', '.join(map(repr, _lib.TAILS))}, got {tail!r}")
     a.tail = _lib.TAILS[tail]
@@ -120,7 +122,7 @@ def distill_loss(student_logits: Tensor, teacher_tokens: Tensor, teacher_logprob
     entry, which is not read; ``inf`` where a listed word is masked).  A token
     outside the vocabulary, or one that an earlier entry of its row has, is left
     out and sets the status word.  Types, strides and masked logits as in
-    ``token_logprobs``.  Differentiable in the student's logits (reverse mode,
+    ``token_logprobs``; rows of up to 3,145,728 bytes.  Differentiable in the student's logits (reverse mode,
     once; rounded once to their type)."""
     tensors, plan = _planned(student_logits, teacher_tokens, teacher_logprobs, None, temperature, tail)
     logits, ids, logprobs, _, temperature = tensors

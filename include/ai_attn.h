@@ -700,6 +700,7 @@ int ai_token_logprobs_bwd(const AiScoreBwdArgs* args, void* stream);
  * +inf and the gradient 0.  dlogits may be the logits' own memory (same
  * strides). */
 #define AI_DISTILL_MAX_TOP 128
+#define AI_DISTILL_MAX_ROW_BYTES 3145728 /* of a row of logits: 16 CTAs hold one */
 enum AiTail { AI_TAIL_BUCKET = 0, AI_TAIL_RENORMALIZE = 1 };
 typedef struct AiDistillArgs {
   int32_t batch;

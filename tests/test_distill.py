@@ -68,6 +68,7 @@ CASES = [
     ((5, 33), 4099, 1, torch.float32),
     ((2, 2), 140001, 40, torch.float32),
     ((650,), 3000, 8, torch.bfloat16),
+    ((3,), 786431, 16, torch.float32),
 ]
 
 
@@ -317,6 +318,7 @@ def test_refusals(cuda_device):
         (ValueError, (x, ids, t[..., :3])),
         (ValueError, (x, ids, t, tau[:1])),
         (ValueError, (x, ids, t, None, "drop")),
+        (ValueError, (x[:, :1].expand(2, 3, 200)[..., :1].expand(2, 3, 2 ** 21), ids, t)),
         (TypeError, (x, ids.int(), t)),
         (TypeError, (x, ids, t.double())),
         (TypeError, (x.double(), ids, t)),
@@ -356,7 +358,7 @@ def test_c_abi_refusals():
 
     assert L.ai_distill(None, None) == 1
     for field, value, code in (("batch", 0, 2), ("vocab", 0, 2), ("n_top", 0, 2), ("n_top", 129, 2), ("tail", 2, 2), ("dtype", 5, 4),
-                               ("batch", 2 ** 30, 2), ("logits", None, 1), ("top_tokens", None, 1), ("top_logprobs", None, 1),
+                               ("batch", 2 ** 30, 2), ("vocab", 2 ** 21, 2), ("logits", None, 1), ("top_tokens", None, 1), ("top_logprobs", None, 1),
                                ("losses", None, 1), ("stride_b", -1, 5), ("dstride_t", -1, 5), ("logits", 257, 6), ("dlogits", 255, 6)):
         assert L.ai_distill(args(**{field: value}), None) == code, field
 
