@@ -101,6 +101,7 @@ __global__ void __launch_bounds__(kThreads, 5) distill_kernel(const AiDistillArg
       const int k = 32 * i + lane;
       word[i] = -1;
       logp[i] = -CUDART_INF_F;
+      if (32 * i >= K) continue;  // (here and below: sets past the list take no instruction of the warp)
       if (k < K) {
         const long long w = a.top_tokens[row * K + k];
         logp[i] = a.top_logprobs[row * K + k];
@@ -142,16 +143,17 @@ __global__ void __launch_bounds__(kThreads, 5) distill_kernel(const AiDistillArg
     for (int i = 0; i < kSets; ++i) xk[i] = word[i] >= 0 ? at(x, word[i]) : -CUDART_INF_F;
     // A word that an earlier entry has is left out.
     bool again[kSets] = {};
-#pragma unroll 4
-    for (int j = 0; j < K; ++j) {
-      const int w = list.word[j];
 #pragma unroll
-      for (int i = 0; i < kSets; ++i) again[i] |= j < 32 * i + lane && w == word[i];
+    for (int i = 0; i < kSets; ++i) {
+      if (32 * i >= K) continue;
+      again[i] = (__match_any_sync(0xffffffffu, word[i]) & ((1u << lane) - 1)) != 0;
+      for (int j = 0; j < 32 * i; ++j) again[i] |= list.word[j] == word[i];
     }
     __syncwarp();
     float top = -CUDART_INF_F, m = -CUDART_INF_F;
 #pragma unroll
     for (int i = 0; i < kSets; ++i) {
+      if (32 * i >= K) continue;
       if (again[i] && word[i] >= 0) {
         if (split == 0) report(a.status, AI_ERR_DEV_BOUNDS);
         word[i] = list.word[32 * i + lane] = -1;
@@ -165,7 +167,8 @@ __global__ void __launch_bounds__(kThreads, 5) distill_kernel(const AiDistillArg
       top = warp_max(top);
       float sum = 0.f;
 #pragma unroll
-      for (int i = 0; i < kSets; ++i) sum += word[i] >= 0 ? expf(logp[i] - top) : 0.f;
+      for (int i = 0; i < kSets; ++i)
+        if (32 * i < K) sum += word[i] >= 0 ? expf(logp[i] - top) : 0.f;
       const float norm = top + logf(warp_sum(sum));
 #pragma unroll
       for (int i = 0; i < kSets; ++i) logp[i] -= norm;
@@ -175,6 +178,7 @@ __global__ void __launch_bounds__(kThreads, 5) distill_kernel(const AiDistillArg
     float p_top = 0.f, sum = 0.f, term = 0.f;
 #pragma unroll
     for (int i = 0; i < kSets; ++i) {
+      if (32 * i >= K) continue;
       p[i] = word[i] >= 0 ? expf(logp[i]) : 0.f;
       p_top += p[i];
       sum += share(xk[i], c, o);
