@@ -136,17 +136,24 @@ __device__ __forceinline__ Part merge_lanes(Part p, float c) {
   return p;
 }
 
-// Adds U vectors of logits to a thread's part (vectors past the row's end are
-// all -inf, which adds nothing).  kT: with t.
-template <typename T, int U, bool kT>
-__device__ __forceinline__ void accumulate(Part& p, const uint4 (&raw)[U], float c) {
-  constexpr int E = 16 / sizeof(T);
+// The largest of vectors [u0, u1) (NaN counts as -inf).
+template <typename T, int U>
+__device__ __forceinline__ float largest(const uint4 (&raw)[U], int u0, int u1) {
   uint32_t big = Vec<T>::kNone;
 #pragma unroll
   for (int u = 0; u < U; ++u)
-    big = Vec<T>::larger(big, Vec<T>::larger(Vec<T>::larger(raw[u].x, raw[u].y), Vec<T>::larger(raw[u].z, raw[u].w)));
+    if (u >= u0 && u < u1)
+      big = Vec<T>::larger(big, Vec<T>::larger(Vec<T>::larger(raw[u].x, raw[u].y), Vec<T>::larger(raw[u].z, raw[u].w)));
+  return Vec<T>::top(big);
+}
+
+// Adds U vectors of logits, `largest` among them, to a thread's part (vectors past
+// the row's end are all -inf, which adds nothing).  kT: with t.
+template <typename T, int U, bool kT>
+__device__ __forceinline__ void accumulate(Part& p, const uint4 (&raw)[U], float c, float largest) {
+  constexpr int E = 16 / sizeof(T);
   // (without an unmasked logit the maximum stays -inf and nothing is added)
-  const float top = fmaxf(p.m, Vec<T>::top(big)), o = top == -CUDART_INF_F ? 0.f : top;
+  const float top = fmaxf(p.m, largest), o = top == -CUDART_INF_F ? 0.f : top;
   const float2 no = make_float2(-o, -o), cc = make_float2(c, c);
   float2 s = make_float2(0.f, 0.f), t = make_float2(0.f, 0.f);
 #pragma unroll
@@ -165,6 +172,11 @@ __device__ __forceinline__ void accumulate(Part& p, const uint4 (&raw)[U], float
   if constexpr (kT) p.t = f * fmaf(fmaxf(y, kNoWeight), p.s, p.t) + (t.x + t.y);
   p.s = p.s * f + (s.x + s.y);
   p.m = top;
+}
+
+template <typename T, int U, bool kT>
+__device__ __forceinline__ void accumulate(Part& p, const uint4 (&raw)[U], float c) {
+  accumulate<T, U, kT>(p, raw, c, largest<T, U>(raw, 0, U));
 }
 
 // The temperature of a batch row; one that is not above zero is reported and

@@ -12,13 +12,13 @@
 // so no row can stay on the chip between the two).
 //
 // A row is cut for a cluster of CTAs (one where there are rows enough), whose
-// first CTA joins the parts through distributed shared memory: one launch, no
-// workspace.  The list of the largest logits needs no second pass over the row:
-// k threads' own maxima, the k-th largest of all threads', are k logits, so no
-// logit below the smallest of them can be in the list, and only those k threads
-// can have met one above it; what these k of 256 threads read is looked at again.
-// A part whose logits crowd above that bound (ties, sorted rows) is gone
-// through in order instead, keeping the best so far.
+// first CTA joins what the others send it through distributed shared memory: one
+// launch, no workspace.  The list of the largest logits needs no second pass over
+// the row: k threads' own maxima, the k-th largest of all threads', are k logits,
+// so no logit below the smallest of them can be in the list, and the maxima of
+// 1 KB pieces, kept on the way, say where the others are (about k pieces).  A part
+// whose logits crowd above that bound (ties, sorted rows) is gone through in order
+// instead, keeping the best so far.
 
 #include <cooperative_groups.h>
 #include <cuda_runtime.h>
@@ -47,24 +47,42 @@ using Key = unsigned long long;
 
 // Larger logit first, then the lower index; 0 stands for no entry, which is
 // below every key.
-__device__ __forceinline__ Key key_of(float x, int v) {
-  const uint32_t b = __float_as_uint(x + 0.f);  // (-0 equals 0)
-  const uint32_t o = b & 0x80000000u ? ~b : b | 0x80000000u;
-  return ((Key)o << 32) | (uint32_t)(~v);
-}
+__device__ __forceinline__ Key key_of(uint32_t order, int v) { return ((Key)order << 32) | (uint32_t)(~v); }
 __device__ __forceinline__ int key_index(Key k) { return (int)~(uint32_t)k; }
 __device__ __forceinline__ float key_value(Key k) {
   const uint32_t o = (uint32_t)(k >> 32);
   return __uint_as_float(o & 0x80000000u ? o & 0x7fffffffu : ~o);
 }
 
+// Order of float values as whole numbers (-0 equals 0), above `kMasked` for what is
+// not masked.
+__device__ __forceinline__ uint32_t order(float x) {
+  const uint32_t b = __float_as_uint(x + 0.f);
+  return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+constexpr uint32_t kMasked = 0x007fffffu;  // order(-inf)
+
+constexpr int kPieces = 2048;
+
 struct TopSmem {
-  Key room[kRoom];        // candidates
-  Key best[kMaxTop];      // the slice's list
-  float top[kThreads];    // each thread's largest logit
-  int hot[kThreads];      // threads whose logits are looked at again
-  float bound;
-  int n_hot, n;
+  Key room[kRoom];            // candidates
+  Key best[kMaxTop];          // the slice's list
+  uint32_t pieces[kPieces];   // order of the largest logit of each piece
+  int n;
+};
+
+// Pieces of a slice: what a warp reads as two vectors a lane in one round (the
+// first or the second two of its four), in so many rounds that they fit.
+struct Pieces {
+  int rounds;  // of the slice
+  int bits;    // a piece is of 2^bits rounds
+  __device__ __forceinline__ Pieces(const Slice& sl) {
+    rounds = (sl.i1 - sl.i0 + kThreads * U - 1) / (kThreads * U);
+    bits = 0;
+    while ((((rounds - 1) >> bits) + 1) * 2 * kWarps > kPieces) ++bits;
+  }
+  __device__ __forceinline__ int count() const { return rounds > 0 ? (((rounds - 1) >> bits) + 1) * 2 * kWarps : 0; }
+  __device__ __forceinline__ int at(int round, int warp, int pair) const { return ((round >> bits) * kWarps + warp) * 2 + pair; }
 };
 
 // The k largest of room[0 .. n) to best[], sorted, 0 past the last one.
@@ -99,30 +117,25 @@ __device__ void select(TopSmem& sm, int n, int k) {
 }
 
 // The slice's k largest logits.  `top`: the thread's largest one among its
-// vectors (i0 + tid + kThreads n).
+// vectors; sm.pieces holds the pieces', n 0.
 template <typename T>
-__device__ void top_of_slice(TopSmem& sm, const T* x, int vocab, const Slice& sl, float top, int k) {
+__device__ void top_of_slice(TopSmem& sm, const T* x, int vocab, const Slice& sl, const Pieces& pieces, float top, int k) {
   constexpr int E = 16 / sizeof(T);
-  const int tid = threadIdx.x;
-  if (tid == 0) sm.n = sm.n_hot = 0, sm.bound = -CUDART_INF_F;
-  sm.top[tid] = top;
-  __syncthreads();
-  int rank = 0;
-#pragma unroll 8
-  for (int j = 0; j < kThreads; j += 4) {
-    const float4 t = *reinterpret_cast<const float4*>(sm.top + j);
-    rank += (t.x > top || (t.x == top && j < tid)) + (t.y > top || (t.y == top && j + 1 < tid)) +
-            (t.z > top || (t.z == top && j + 2 < tid)) + (t.w > top || (t.w == top && j + 3 < tid));
+  const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
+  // A bound that k threads' maxima reach, from its first bit down.
+  const uint32_t mine = order(top);
+  uint32_t bound = 0;
+  for (int bit = 31; bit >= 8; --bit) {
+    const uint32_t next = bound | 1u << bit;
+    const int reach = __syncthreads_count(mine >= next);  // (also: the pieces are written)
+    if (reach >= k) bound = next;
+    if (reach == k) break;
   }
-  if (rank == k - 1) sm.bound = top;
-  __syncthreads();
-  const float bound = sm.bound;
-  if (top >= bound && top != -CUDART_INF_F) sm.hot[atomicAdd(&sm.n_hot, 1)] = tid;
-  __syncthreads();
   auto offer = [&](float f, int v) {
-    if (f >= bound && f != -CUDART_INF_F) {
+    const uint32_t o = order(f);
+    if (o >= bound && o > kMasked && f == f) {
       const int n = atomicAdd(&sm.n, 1);
-      if (n < kRoom) sm.room[n] = key_of(f, v);
+      if (n < kRoom) sm.room[n] = key_of(o, v);
     }
   };
   // (the row's ragged ends are in no thread's maximum)
@@ -131,15 +144,26 @@ __device__ void top_of_slice(TopSmem& sm, const T* x, int vocab, const Slice& sl
     if (sl.e1 > sl.tail && sl.tail + tid < vocab) offer(at(x, sl.tail + tid), sl.tail + tid);
   }
   const uint4* xv = reinterpret_cast<const uint4*>(x + sl.head);
-  const int per = (sl.i1 - sl.i0 + kThreads - 1) / kThreads, all = sm.n_hot * per;
-  for (int w = tid; w < all; w += kThreads) {
-    const int j = w / per, i = sl.i0 + sm.hot[j] + (w - j * per) * kThreads;
-    if (i >= sl.i1) continue;
-    const uint4 raw = __ldg(xv + i);
-    T e[E];
-    memcpy(e, &raw, 16);
+  const int count = pieces.count();
+  for (int p0 = 32 * warp; p0 < count; p0 += kThreads) {
+    const uint32_t o = p0 + lane < count ? sm.pieces[p0 + lane] : 0u;
+    uint32_t hot = __ballot_sync(0xffffffffu, o >= bound && o > kMasked);
+    while (hot) {
+      const int p = p0 + __ffs(hot) - 1;
+      hot &= hot - 1;
+      const int r0 = p / (2 * kWarps) << pieces.bits, of = p / 2 % kWarps, r1 = min(pieces.rounds, r0 + (1 << pieces.bits));
+      for (int r = r0; r < r1; ++r)
 #pragma unroll
-    for (int q = 0; q < E; ++q) offer(to_f32(e[q]), sl.head + i * E + q);
+        for (int u = 0; u < 2; ++u) {
+          const int i = sl.i0 + (r * U + 2 * (p % 2) + u) * kThreads + 32 * of + lane;
+          if (i >= sl.i1) continue;
+          const uint4 raw = __ldg(xv + i);
+          T e[E];
+          memcpy(e, &raw, 16);
+#pragma unroll
+          for (int q = 0; q < E; ++q) offer(to_f32(e[q]), sl.head + i * E + q);
+        }
+    }
   }
   __syncthreads();
   const int n = sm.n;
@@ -161,7 +185,7 @@ __device__ void top_of_slice(TopSmem& sm, const T* x, int vocab, const Slice& sl
       const int v = v0 + q * kThreads + tid;
       if (v >= sl.e1) continue;
       const float f = at(x, v);
-      const Key key = key_of(f, v);
+      const Key key = key_of(order(f), v);
       if (f > -CUDART_INF_F && key > least) sm.room[atomicAdd(&sm.n, 1)] = key;  // (at most kRoom: held is half of it)
     }
     __syncthreads();
@@ -180,10 +204,11 @@ template <typename T, bool kEntropy, bool kTop>
 __global__ void __launch_bounds__(kThreads, 4) score_kernel(const AiScoreArgs a, const int splits) {
   constexpr int E = 16 / sizeof(T);
   __shared__ Part s_part[kWarps];
-  __shared__ Part s_slice;
+  __shared__ Part s_slices[kMaxSplit];  // of the cluster, in its first CTA
   __shared__ float s_row[2];
   extern __shared__ __align__(16) uint8_t smem[];
   TopSmem& top = *reinterpret_cast<TopSmem*>(smem);
+  Key* lists = reinterpret_cast<Key*>(smem + sizeof(TopSmem));  // the cluster's, in its first CTA
   const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
   const int64_t row = blockIdx.x / (uint32_t)splits;
   const int split = (int)(blockIdx.x - row * splits);
@@ -203,6 +228,8 @@ __global__ void __launch_bounds__(kThreads, 4) score_kernel(const AiScoreArgs a,
     }
     return;
   }
+  // (a CTA of the cluster must run before its shared memory is written to)
+  if (splits > 1) asm volatile("barrier.cluster.arrive;" ::: "memory");
   const float tau = row_tau(a.temperature, b, split == 0 && tid == 0 ? a.status : nullptr);
   const float c = slope(tau), inv = inverse(tau);
   const T* x = static_cast<const T*>(a.logits) + b * a.stride_b + t * a.stride_t;
@@ -218,12 +245,26 @@ __global__ void __launch_bounds__(kThreads, 4) score_kernel(const AiScoreArgs a,
     for (int u = 0; u < U; ++u) next[u] = i + u * kThreads < sl.i1 ? __ldg(xv + i + u * kThreads) : none;
   };
   load(sl.i0 + tid);
-  for (int i = sl.i0 + tid; i < sl.i1; i += kThreads * U) {
+  const Pieces pieces(sl);
+  if (kTop && tid == 0) top.n = 0;
+  // (whole rounds of the CTA, for the pieces' sake)
+  for (int i0 = sl.i0, r = 0; i0 < sl.i1; i0 += kThreads * U, ++r) {
     uint4 raw[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) raw[u] = next[u];
-    load(i + kThreads * U);
-    accumulate<T, U, kEntropy>(p, raw, c);
+    load(i0 + tid + kThreads * U);
+    if constexpr (kTop) {
+      const float a0 = largest<T, U>(raw, 0, 2), a1 = largest<T, U>(raw, 2, 4);
+      const uint32_t o0 = __reduce_max_sync(0xffffffffu, order(a0)), o1 = __reduce_max_sync(0xffffffffu, order(a1));
+      if (lane < 2) {
+        uint32_t& to = top.pieces[pieces.at(r, warp, lane)];
+        const uint32_t o = lane ? o1 : o0;
+        to = (r & ((1 << pieces.bits) - 1)) == 0 || o > to ? o : to;
+      }
+      accumulate<T, U, kEntropy>(p, raw, c, fmaxf(a0, a1));
+    } else {
+      accumulate<T, U, kEntropy>(p, raw, c);
+    }
   }
   const float mine = p.m;
   if (tid < E) {
@@ -237,48 +278,34 @@ __global__ void __launch_bounds__(kThreads, 4) score_kernel(const AiScoreArgs a,
   p = merge_lanes(p, c);
   if (lane == 0) s_part[warp] = p;
   if constexpr (kTop) {
-    top_of_slice(top, x, a.vocab, sl, mine, k);
+    top_of_slice(top, x, a.vocab, sl, pieces, mine, k);
   } else {
     __syncthreads();
   }
-  if (tid == 0) {
+  if (tid == 0)
     for (int w = 1; w < kWarps; ++w) p = merge(p, s_part[w], c);
-    s_slice = p;
-  }
   if (splits > 1) {
     const cg::cluster_group cluster = cg::this_cluster();
+    asm volatile("barrier.cluster.wait;" ::: "memory");
+    if (tid == 0) cluster.map_shared_rank(s_slices, 0)[split] = p;
+    if (tid < k) cluster.map_shared_rank(lists, 0)[split * k + tid] = top.best[tid];
     cluster.sync();
-    if (split == 0) {
-      if (tid == 0)
-        for (int r = 1; r < splits; ++r) p = merge(p, *cluster.map_shared_rank(&s_slice, r), c);
-      if constexpr (kTop) {
-        // Sorted lists: an entry's place is the number of larger ones in each.
-        const int all = splits * k;
-        for (int j = tid; j < all; j += kThreads) top.room[j] = cluster.map_shared_rank(&top, j / k)->best[j % k];
-        __syncthreads();
-        if (tid < k) top.best[tid] = 0;
-        __syncthreads();
-        for (int j = tid; j < all; j += kThreads) {
-          const Key key = top.room[j];
-          if (key == 0) continue;
-          int rank = 0;
-          for (int r = 0; r < splits && rank < k; ++r) {
-            int lo = 0, hi = k;
-            while (lo < hi) {
-              const int mid = (lo + hi) / 2;
-              if (top.room[r * k + mid] > key)
-                lo = mid + 1;
-              else
-                hi = mid;
-            }
-            rank += lo;
-          }
-          if (rank < k) top.best[rank] = key;
-        }
-      }
-    }
-    cluster.sync();  // (the parts have been read)
     if (split > 0) return;
+    if (tid == 0)
+      for (int r = 1; r < splits; ++r) p = merge(p, s_slices[r], c);
+    if constexpr (kTop) {
+      // An entry below some slice's k-th one is in no list of k.
+      Key least = 0;
+      for (int r = 0; r < splits; ++r) least = max(least, lists[r * k + k - 1]);
+      if (tid == 0) top.n = 0;
+      __syncthreads();
+      for (int j = tid; j < splits * k; j += kThreads) {
+        const Key key = lists[j];
+        if (key != 0 && key >= least) top.room[atomicAdd(&top.n, 1)] = key;
+      }
+      __syncthreads();
+      select(top, top.n, k);
+    }
   }
   if (tid == 0) {
     const bool empty = p.s == 0.f;
@@ -451,7 +478,7 @@ int launch(const AiScoreArgs& a, cudaStream_t st) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)((int64_t)a.batch * a.seq_len * splits));
   cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = kTop ? sizeof(TopSmem) : 0;
+  cfg.dynamicSmemBytes = kTop ? sizeof(TopSmem) + (splits > 1 ? splits * a.top_k * sizeof(Key) : 0) : 0;
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
