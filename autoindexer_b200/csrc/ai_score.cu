@@ -94,6 +94,7 @@ __device__ void select(TopSmem& sm, int n, int k) {
     if (tid < n) {
       const Key mine = sm.room[tid];
       int rank = 0;
+#pragma unroll 8
       for (int j = 0; j < n; ++j) rank += sm.room[j] > mine;
       if (rank < k) sm.best[rank] = mine;
     }
@@ -145,11 +146,11 @@ __device__ void top_of_slice(TopSmem& sm, const T* x, int vocab, const Slice& sl
   }
   const uint4* xv = reinterpret_cast<const uint4*>(x + sl.head);
   const int count = pieces.count();
-  for (int p0 = 32 * warp; p0 < count; p0 += kThreads) {
-    const uint32_t o = p0 + lane < count ? sm.pieces[p0 + lane] : 0u;
+  for (int p0 = warp; p0 < count; p0 += kThreads) {  // (a warp's pieces are the CTA's warps apart)
+    const uint32_t o = p0 + kWarps * lane < count ? sm.pieces[p0 + kWarps * lane] : 0u;
     uint32_t hot = __ballot_sync(0xffffffffu, o >= bound && o > kMasked);
     while (hot) {
-      const int p = p0 + __ffs(hot) - 1;
+      const int p = p0 + kWarps * (__ffs(hot) - 1);
       hot &= hot - 1;
       const int r0 = p / (2 * kWarps) << pieces.bits, of = p / 2 % kWarps, r1 = min(pieces.rounds, r0 + (1 << pieces.bits));
       for (int r = r0; r < r1; ++r)
@@ -215,6 +216,17 @@ __global__ void __launch_bounds__(kThreads, 4) score_kernel(const AiScoreArgs a,
   const int64_t b = row / a.seq_len, t = row - b * a.seq_len;
   const int k = kTop ? a.top_k : 0;
   const long long token = a.tokens[row];
+  const T* x = static_cast<const T*>(a.logits) + b * a.stride_b + t * a.stride_t;
+  const Slice sl = slice_of(x, a.vocab, split, splits, kThreads);
+  const uint4* xv = reinterpret_cast<const uint4*>(x + sl.head);
+  const uint4 none = make_uint4(Vec<T>::kNone, Vec<T>::kNone, Vec<T>::kNone, Vec<T>::kNone);
+  // (the next round's loads are in flight while this one's are summed)
+  uint4 next[U];
+  auto load = [&](int i) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) next[u] = i + u * kThreads < sl.i1 ? __ldg(xv + i + u * kThreads) : none;
+  };
+  if (splits > 1) load(sl.i0 + tid);  // (few rows: they do not wait for the token)
   if (token < 0 || token >= a.vocab) {
     if (split > 0) return;
     if (tid == 0) {
@@ -232,19 +244,9 @@ __global__ void __launch_bounds__(kThreads, 4) score_kernel(const AiScoreArgs a,
   if (splits > 1) asm volatile("barrier.cluster.arrive;" ::: "memory");
   const float tau = row_tau(a.temperature, b, split == 0 && tid == 0 ? a.status : nullptr);
   const float c = slope(tau), inv = inverse(tau);
-  const T* x = static_cast<const T*>(a.logits) + b * a.stride_b + t * a.stride_t;
-  const Slice sl = slice_of(x, a.vocab, split, splits, kThreads);
   const float given = split == 0 && tid == 0 ? at(x, token) : 0.f;
   Part p{-CUDART_INF_F, 0.f, 0.f};
-  const uint4* xv = reinterpret_cast<const uint4*>(x + sl.head);
-  const uint4 none = make_uint4(Vec<T>::kNone, Vec<T>::kNone, Vec<T>::kNone, Vec<T>::kNone);
-  // (the next round's loads are in flight while this one's are summed)
-  uint4 next[U];
-  auto load = [&](int i) {
-#pragma unroll
-    for (int u = 0; u < U; ++u) next[u] = i + u * kThreads < sl.i1 ? __ldg(xv + i + u * kThreads) : none;
-  };
-  load(sl.i0 + tid);
+  if (splits == 1) load(sl.i0 + tid);
   const Pieces pieces(sl);
   if (kTop && tid == 0) top.n = 0;
   // (whole rounds of the CTA, for the pieces' sake)
@@ -292,10 +294,12 @@ __global__ void __launch_bounds__(kThreads, 4) score_kernel(const AiScoreArgs a,
     cluster.sync();
     if (split > 0) return;
     if (tid == 0)
+#pragma unroll 4
       for (int r = 1; r < splits; ++r) p = merge(p, s_slices[r], c);
     if constexpr (kTop) {
       // An entry below some slice's k-th one is in no list of k.
       Key least = 0;
+#pragma unroll 4
       for (int r = 0; r < splits; ++r) least = max(least, lists[r * k + k - 1]);
       if (tid == 0) top.n = 0;
       __syncthreads();
