@@ -1,16 +1,17 @@
 // New keys and values into the paged cache in 4 bits, and the values back from
 // it (declared in include/ai_attn.h, the format at AiPool4).
 //
-// A head row sits in eight lanes: lane g has dims 32 c + 4 g + {0 .. 3} of every
-// group c, whose codes are its D / 16 consecutive bytes of the row, so a row's
-// bytes leave in one piece and a group's extremes are three shuffles.  A warp
-// takes four heads of a token at a time, K rows and V rows alike.
+// Sixteen consecutive dims of a head row, half a group, sit in a lane, so a
+// group's extremes are one shuffle; their codes are four pairs of bytes of the row.
+// A warp takes a token's K and V rows 512 dims at a time, two such turns' loads in
+// flight together.
 //
 // A code is the whole number nearest to x / d, halves to even, as the quotient's
-// exact value has it: x times the reciprocal gives a candidate c, the remainder
-// x - c d is exact in fp32 (c is off by less than one, so it has no more bits
-// than x and d together leave), and where it is not below half of d the candidate
-// moves.
+// exact value has it.  16-bit values: x times the reciprocal of d is good to 2^-20,
+// and a quotient that is not a half exactly is at least 2^-13 from one (x has 8 or
+// 11 bits, d 11), so it is rounded to 2^-16 first, which makes exact halves exact.
+// fp32: the remainder x - c d of a candidate c is exact, and where it is not below
+// half of d the candidate moves.
 
 #include <cuda_runtime.h>
 
@@ -24,83 +25,113 @@ namespace ai {
 namespace kv4 {
 
 constexpr int kWarps = 4, kThreads = 32 * kWarps;
-constexpr int kRows = 4;  // head rows of a warp
+constexpr int kDims = 16;  // of a lane
 
-// Four consecutive elements.
-template <typename T, bool kVec>
-__device__ __forceinline__ float4 load4(const T* p) {
-  if constexpr (kVec && sizeof(T) == 4) {
-    return __ldg(reinterpret_cast<const float4*>(p));
-  } else if constexpr (kVec) {
-    const uint2 r = __ldg(reinterpret_cast<const uint2*>(p));
-    T e[4];
-    memcpy(e, &r, 8);
-    return make_float4(to_f32(e[0]), to_f32(e[1]), to_f32(e[2]), to_f32(e[3]));
-  } else {
-    return make_float4(to_f32(p[0]), to_f32(p[1]), to_f32(p[2]), to_f32(p[3]));
-  }
-}
+// Sixteen consecutive elements as they lie in memory.
+template <typename T>
+struct Raw {
+  uint4 v[sizeof(T)];
+};
 
 template <typename T, bool kVec>
-__device__ __forceinline__ void store4(T* p, float4 f) {
-  T e[4] = {from_f32<T>(f.x), from_f32<T>(f.y), from_f32<T>(f.z), from_f32<T>(f.w)};
-  if constexpr (kVec && sizeof(T) == 4) {
-    *reinterpret_cast<float4*>(p) = f;
-  } else if constexpr (kVec) {
-    uint2 r;
-    memcpy(&r, e, 8);
-    *reinterpret_cast<uint2*>(p) = r;
+__device__ __forceinline__ Raw<T> load(const T* p) {
+  Raw<T> r;
+  if constexpr (kVec) {
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T); ++i) r.v[i] = __ldg(reinterpret_cast<const uint4*>(p) + i);
   } else {
+    T e[kDims];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) p[i] = e[i];
+    for (int i = 0; i < kDims; ++i) e[i] = p[i];
+    memcpy(&r, e, sizeof(r));
+  }
+  return r;
+}
+
+template <typename T, bool kVec>
+__device__ __forceinline__ void store(T* p, const Raw<T>& r) {
+  if constexpr (kVec) {
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T); ++i) reinterpret_cast<uint4*>(p)[i] = r.v[i];
+  } else {
+    T e[kDims];
+    memcpy(e, &r, sizeof(r));
+#pragma unroll
+    for (int i = 0; i < kDims; ++i) p[i] = e[i];
   }
 }
 
-__device__ __forceinline__ int code(float x, float d, float inv) {
-  constexpr float kShift = 12582912.f;  // 1.5 2^23: the sum's last bit counts ones
-  float c = fmaf(x, inv, kShift) - kShift;
-  const float rest = fmaf(-c, d, x), half = 0.5f * fabsf(d);
-  if (!(fabsf(rest) < half)) {
-    // Past the half: on to the neighbour; on it: to the even one.
-    const float step = (rest < 0.f) == (d < 0.f) ? 1.f : -1.f;
-    if (fabsf(rest) > half || (fabsf(rest) == half && ((int)c & 1))) c += step;
-  }
-  return (int)fminf(fmaxf(c, -8.f), 7.f) + 8;
-}
+// Sums with 2^23 + 2^22 keep whole numbers in their last bits, sums with 192 keep
+// 2^-16.
+constexpr float kWhole = 12582912.f, kSixteenth = 192.f;
 
-// The lane's codes and the scales of a row of which it has f[c] (eight lanes).
-template <int C>
-__device__ __forceinline__ void quantize(const float4 (&f)[C], uint16_t (&codes)[C], __half (&scales)[C]) {
-#pragma unroll
-  for (int c = 0; c < C; ++c) {
-    float top = fmaxf(fmaxf(f[c].x, f[c].y), fmaxf(f[c].z, f[c].w));
-    float low = fminf(fminf(f[c].x, f[c].y), fminf(f[c].z, f[c].w));
-    // (0 times a NaN or an infinity is NaN)
-    float bad = f[c].x * 0.f + f[c].y * 0.f + (f[c].z * 0.f + f[c].w * 0.f);
-#pragma unroll
-    for (int o = 1; o < 8; o <<= 1) {
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-      low = fminf(low, __shfl_xor_sync(0xffffffffu, low, o));
-      bad += __shfl_xor_sync(0xffffffffu, bad, o);
+// The bits of 2^23 + 2^22 + code.
+template <typename T>
+__device__ __forceinline__ uint32_t code(float x, float d, float inv) {
+  float t;
+  if constexpr (sizeof(T) == 2) {
+    t = fmaf(x, inv, kSixteenth) - kSixteenth + (kWhole + 8.f);
+  } else {
+    float c = fmaf(x, inv, kWhole) - kWhole;
+    const float rest = fmaf(-c, d, x), half = 0.5f * fabsf(d);
+    if (!(fabsf(rest) < half)) {
+      // Past the half: on to the neighbour; on it: to the even one.
+      const float step = (rest < 0.f) == (d < 0.f) ? 1.f : -1.f;
+      if (fabsf(rest) > half || (fabsf(rest) == half && ((int)c & 1))) c += step;
     }
-    const float want = fminf(fmaxf((top > -low ? top : low) * -0.125f, -65504.f), 65504.f);
-    __half h = __float2half_rn(want);
-    const float d = __half2float(h), inv = 1.f / d;
-    uint32_t q = 0x8888u;
-    if (bad != 0.f) {
-      h = __ushort_as_half((unsigned short)0x7fffu);
-    } else if (d != 0.f) {
-      q = code(f[c].x, d, inv) | code(f[c].y, d, inv) << 4 | code(f[c].z, d, inv) << 8 | code(f[c].w, d, inv) << 12;
-    }
-    codes[c] = (uint16_t)q;
-    scales[c] = h;
+    t = c + (kWhole + 8.f);
+  }
+  return __float_as_uint(fminf(fmaxf(t, kWhole), kWhole + 15.f));
+}
+
+// The lane's codes, a word of four per four dims, and its group's scale.
+template <typename T>
+__device__ __forceinline__ void quantize(const Raw<T>& raw, uint16_t (&codes)[4], __half& scale) {
+  T e[kDims];
+  memcpy(e, &raw, sizeof(raw));
+  float f[kDims], top = -CUDART_INF_F, low = CUDART_INF_F, bad = 0.f;
+#pragma unroll
+  for (int i = 0; i < kDims; ++i) {
+    f[i] = to_f32(e[i]);
+    top = fmaxf(top, f[i]);
+    low = fminf(low, f[i]);
+    bad = fmaf(f[i], 0.f, bad);  // (0 times a NaN or an infinity is NaN)
+  }
+  top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+  low = fminf(low, __shfl_xor_sync(0xffffffffu, low, 1));
+  bad += __shfl_xor_sync(0xffffffffu, bad, 1);
+  scale = __float2half_rn(fminf(fmaxf((top > -low ? top : low) * -0.125f, -65504.f), 65504.f));
+  const float d = __half2float(scale), inv = 1.f / d;
+  if (bad != 0.f) scale = __ushort_as_half((unsigned short)0x7fffu);
+  const bool plain = bad == 0.f && d != 0.f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t c0 = code<T>(f[4 * i], d, inv), c1 = code<T>(f[4 * i + 1], d, inv), c2 = code<T>(f[4 * i + 2], d, inv),
+                   c3 = code<T>(f[4 * i + 3], d, inv);
+    const uint32_t w = (c0 + (c1 << 4)) + ((c2 + (c3 << 4)) << 8);
+    codes[i] = plain ? (uint16_t)w : (uint16_t)0x8888u;
   }
 }
 
-// Which token and heads an item is about.
+// The values of a lane's codes.
+template <typename T>
+__device__ __forceinline__ Raw<T> values(const uint16_t (&codes)[4], __half scale) {
+  const float d = __half2float(scale);
+  T e[kDims];
+#pragma unroll
+  for (int i = 0; i < kDims; ++i) {
+    const uint32_t c = codes[i / 4] >> (4 * (i % 4)) & 15u;
+    e[i] = from_f32<T>((__uint_as_float(0x4b400000u | c) - (kWhole + 8.f)) * d);
+  }
+  Raw<T> r;
+  memcpy(&r, e, sizeof(r));
+  return r;
+}
+
+// Which token and rows (K rows, then V rows) an item is about.
 struct Item {
   int64_t b;
-  int t, h0, h1;
+  int t, r0, r1;
 };
 
 __device__ __forceinline__ Item item_of(const AiPaged4Args& a, uint32_t it, int per, int chunks) {
@@ -108,16 +139,38 @@ __device__ __forceinline__ Item item_of(const AiPaged4Args& a, uint32_t it, int 
   Item r;
   r.b = seq;
   r.t = (int)(tok - seq * (uint32_t)a.seq_len);
-  r.h0 = (int)(it - tok * (uint32_t)chunks) * per;
-  r.h1 = min(a.num_kv_heads, r.h0 + per);
+  r.r0 = (int)(it - tok * (uint32_t)chunks) * per;
+  r.r1 = min(2 * a.num_kv_heads, r.r0 + per);
+  return r;
+}
+
+// A lane's sixteen dims of a row: of the tensor, of the codes, of the scales.
+template <typename T>
+struct Spot {
+  T* x;
+  uint8_t* codes;
+  __half* scale;
+};
+
+template <typename T, int D>
+__device__ __forceinline__ Spot<T> spot_of(const AiPaged4Args& a, const Item& i, const Place& p, int row, int l) {
+  constexpr int C = D / kGroup;
+  const bool v = row >= a.num_kv_heads;
+  const int64_t h = v ? row - a.num_kv_heads : row;
+  const AiTensor4 &x = v ? a.v : a.k, &cd = v ? a.pool.v_codes : a.pool.k_codes, &sc = v ? a.pool.v_scales : a.pool.k_scales;
+  Spot<T> r;
+  r.x = static_cast<T*>(const_cast<void*>(x.ptr)) + i.b * x.stride_b + h * x.stride_h + i.t * x.stride_t + kDims * l;
+  // (dims 16 l + 4 i + j: group l / 2, byte pairs 4 (l % 2) + i)
+  r.codes = static_cast<uint8_t*>(const_cast<void*>(cd.ptr)) + p.page * cd.stride_b + h * cd.stride_h + p.slot * (D / 2) +
+            (l % 2 * 4) * 2 * C + l / 2 * 2;
+  r.scale = static_cast<__half*>(const_cast<void*>(sc.ptr)) + p.page * sc.stride_b + h * sc.stride_h + p.slot * C + l / 2;
   return r;
 }
 
 template <typename T, int D, bool kVec>
-__global__ void __launch_bounds__(kThreads, 6) append_kernel(const AiPaged4Args a, const int per, const int chunks,
-                                                             const uint32_t items) {
-  constexpr int C = D / kGroup;
-  const int lane = threadIdx.x % 32, sub = lane / 8, g = lane % 8;
+__global__ void __launch_bounds__(kThreads) append_kernel(const AiPaged4Args a, const int per, const int chunks, const uint32_t items) {
+  constexpr int L = D / kDims, R = 32 / L, C = D / kGroup;  // lanes of a row, rows of a turn
+  const int lane = threadIdx.x % 32, sub = lane / L, l = lane % L;
   const uint32_t it = blockIdx.x * kWarps + threadIdx.x / 32;
   if (it >= items) return;
   const Item i = item_of(a, it, per, chunks);
@@ -127,101 +180,54 @@ __global__ void __launch_bounds__(kThreads, 6) append_kernel(const AiPaged4Args 
     report(a.status, AI_ERR_DEV_BOUNDS);
     return;
   }
-  for (int hb = i.h0; hb < i.h1; hb += kRows) {
-    const int64_t h = min(hb + sub, i.h1 - 1);  // (rows past the last head repeat it, unstored)
+  for (int r0 = i.r0; r0 < i.r1; r0 += 2 * R) {
+    Spot<T> at[2];
+    Raw<T> raw[2];
 #pragma unroll
-    for (int kv = 0; kv < 2; ++kv) {
-      const AiTensor4 &src = kv ? a.v : a.k, &cd = kv ? a.pool.v_codes : a.pool.k_codes,
-                      &sc = kv ? a.pool.v_scales : a.pool.k_scales;
-      const T* x = static_cast<const T*>(src.ptr) + i.b * src.stride_b + h * src.stride_h + i.t * src.stride_t + 4 * g;
-      float4 f[C];
+    for (int u = 0; u < 2; ++u) {
+      at[u] = spot_of<T, D>(a, i, p, min(r0 + u * R + sub, i.r1 - 1), l);  // (rows past the last repeat it, unstored)
+      if (u == 0 || r0 + R < i.r1) raw[u] = load<T, kVec>(at[u].x);
+    }
 #pragma unroll
-      for (int c = 0; c < C; ++c) f[c] = load4<T, kVec>(x + kGroup * c);
-      uint16_t codes[C];
-      __half scales[C];
-      quantize<C>(f, codes, scales);
-      if (hb + sub < i.h1) {
-        uint8_t* co = static_cast<uint8_t*>(const_cast<void*>(cd.ptr)) + p.page * cd.stride_b + h * cd.stride_h +
-                      p.slot * cd.stride_t + g * 2 * C;
-        __half* so = static_cast<__half*>(const_cast<void*>(sc.ptr)) + p.page * sc.stride_b + h * sc.stride_h +
-                     p.slot * sc.stride_t;
-        if constexpr (C == 4) {
-          uint2 r;
-          memcpy(&r, codes, 8);
-          *reinterpret_cast<uint2*>(co) = r;
-          if (g == 0) {
-            memcpy(&r, scales, 8);
-            *reinterpret_cast<uint2*>(so) = r;
-          }
-        } else if constexpr (C == 2) {
-          uint32_t r;
-          memcpy(&r, codes, 4);
-          *reinterpret_cast<uint32_t*>(co) = r;
-          if (g == 0) {
-            memcpy(&r, scales, 4);
-            *reinterpret_cast<uint32_t*>(so) = r;
-          }
-        } else {
-          *reinterpret_cast<uint16_t*>(co) = codes[0];
-          if (g == 0) *so = scales[0];
-        }
-      }
+    for (int u = 0; u < 2; ++u) {
+      if (u == 1 && r0 + R >= i.r1) break;
+      uint16_t codes[4];
+      __half scale;
+      quantize<T>(raw[u], codes, scale);
+      if (r0 + u * R + sub >= i.r1) continue;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) *reinterpret_cast<uint16_t*>(at[u].codes + k * 2 * C) = codes[k];
+      if (l % 2 == 0) *at[u].scale = scale;
     }
   }
 }
 
 template <typename T, int D, bool kVec>
-__global__ void __launch_bounds__(kThreads, 6) read_kernel(const AiPaged4Args a, const int per, const int chunks,
-                                                           const uint32_t items) {
-  constexpr int C = D / kGroup;
-  const int lane = threadIdx.x % 32, sub = lane / 8, g = lane % 8;
+__global__ void __launch_bounds__(kThreads) read_kernel(const AiPaged4Args a, const int per, const int chunks, const uint32_t items) {
+  constexpr int L = D / kDims, R = 32 / L, C = D / kGroup;
+  const int lane = threadIdx.x % 32, sub = lane / L, l = lane % L;
   const uint32_t it = blockIdx.x * kWarps + threadIdx.x / 32;
   if (it >= items) return;
   const Item i = item_of(a, it, per, chunks);
-  const bool wanted = i.t < new_tokens(a.n, i.b, a.seq_len, a.status);
   Place p{-1, 0};
-  if (wanted) {
+  if (i.t < new_tokens(a.n, i.b, a.seq_len, a.status)) {
     p = place(a.pool, i.b, (int64_t)__ldg(a.lens + i.b) + i.t);
     if (p.page < 0) report(a.status, AI_ERR_DEV_BOUNDS);
   }
-  for (int hb = i.h0; hb < i.h1; hb += kRows) {
-    const int64_t h = hb + sub;
-    if (h >= i.h1) continue;
+  for (int r0 = i.r0; r0 < i.r1; r0 += 2 * R) {
+    Spot<T> at[2];
+    uint16_t codes[2][4];
+    __half scale[2];
 #pragma unroll
-    for (int kv = 0; kv < 2; ++kv) {
-      const AiTensor4 &dst = kv ? a.v : a.k, &cd = kv ? a.pool.v_codes : a.pool.k_codes,
-                      &sc = kv ? a.pool.v_scales : a.pool.k_scales;
-      uint16_t codes[C] = {};
-      __half scales[C] = {};
-      if (p.page >= 0) {
-        const uint8_t* co = static_cast<const uint8_t*>(cd.ptr) + p.page * cd.stride_b + h * cd.stride_h +
-                            p.slot * cd.stride_t + g * 2 * C;
-        const __half* so = static_cast<const __half*>(sc.ptr) + p.page * sc.stride_b + h * sc.stride_h +
-                           p.slot * sc.stride_t;
-        if constexpr (C == 4) {
-          uint2 r = *reinterpret_cast<const uint2*>(co);
-          memcpy(codes, &r, 8);
-          r = *reinterpret_cast<const uint2*>(so);
-          memcpy(scales, &r, 8);
-        } else if constexpr (C == 2) {
-          uint32_t r = *reinterpret_cast<const uint32_t*>(co);
-          memcpy(codes, &r, 4);
-          r = *reinterpret_cast<const uint32_t*>(so);
-          memcpy(scales, &r, 4);
-        } else {
-          codes[0] = *reinterpret_cast<const uint16_t*>(co);
-          scales[0] = *so;
-        }
-      }
-      T* x = static_cast<T*>(const_cast<void*>(dst.ptr)) + i.b * dst.stride_b + h * dst.stride_h + i.t * dst.stride_t + 4 * g;
+    for (int u = 0; u < 2; ++u) {
+      at[u] = spot_of<T, D>(a, i, p, min(r0 + u * R + sub, i.r1 - 1), l);
 #pragma unroll
-      for (int c = 0; c < C; ++c) {
-        const float d = __half2float(scales[c]);
-        const int q = codes[c];
-        auto value = [&](int j) { return (float)((q >> (4 * j) & 15) - 8) * d; };
-        store4<T, kVec>(x + kGroup * c, p.page >= 0 ? make_float4(value(0), value(1), value(2), value(3)) : make_float4(0.f, 0.f, 0.f, 0.f));
-      }
+      for (int k = 0; k < 4; ++k) codes[u][k] = p.page < 0 ? (uint16_t)0x8888u : *reinterpret_cast<const uint16_t*>(at[u].codes + k * 2 * C);
+      scale[u] = p.page < 0 ? __ushort_as_half((unsigned short)0) : *at[u].scale;
     }
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+      if (r0 + u * R + sub < i.r1) store<T, kVec>(at[u].x, values<T>(codes[u], scale[u]));
   }
 }
 
@@ -240,11 +246,12 @@ int check(const AiPaged4Args* a) {
 
 template <typename T, int D>
 int launch(const AiPaged4Args& a, bool read, cudaStream_t st) {
-  // One row group per item while that gives every SM at most a few warps; then
-  // a token's heads stay together, so its page is looked up once.
+  // Two turns of rows per item while that gives every SM at most a few warps; then
+  // a token's rows stay together, so its page is looked up once.
+  constexpr int kTurns = 2 * 32 / (D / kDims);
   const int64_t tokens = (int64_t)a.batch * a.seq_len;
-  const int per = tokens <= 4096 ? (kRows < a.num_kv_heads ? kRows : a.num_kv_heads) : a.num_kv_heads;
-  const int chunks = (a.num_kv_heads + per - 1) / per;
+  const int rows = 2 * a.num_kv_heads, per = tokens <= 4096 && kTurns < rows ? kTurns : rows;
+  const int chunks = (rows + per - 1) / per;
   const int64_t items = tokens * chunks, blocks = (items + kWarps - 1) / kWarps;
   if (items > 0x7fffffff) return AI_ERR_SHAPE;
   const bool vec = headrow::rows_aligned(a.k, a.dtype) && headrow::rows_aligned(a.v, a.dtype);
