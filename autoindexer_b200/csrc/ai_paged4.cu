@@ -3,8 +3,7 @@
 //
 // Sixteen consecutive dims of a head row, half a group, sit in a lane, so a
 // group's extremes are one shuffle; their codes are four pairs of bytes of the row.
-// A warp takes a token's K and V rows 512 dims at a time, two such turns' loads in
-// flight together.
+// A warp takes K and V of 512 dims of a token at a time.
 //
 // A code is the whole number nearest to x / d, halves to even, as the quotient's
 // exact value has it.  16-bit values: x times the reciprocal of d is good to 2^-20,
@@ -17,9 +16,10 @@
 
 #include <cstring>
 
-#include "ai_head_row.cuh"
+#include "ai_common.cuh"
 #include "ai_kernels.h"
 #include "ai_kv4.cuh"
+#include "sm100_ptx.cuh"
 
 namespace ai {
 namespace kv4 {
@@ -27,18 +27,30 @@ namespace kv4 {
 constexpr int kWarps = 4, kThreads = 32 * kWarps;
 constexpr int kDims = 16;  // of a lane
 
-// Sixteen consecutive elements as they lie in memory.
+// Sixteen consecutive elements as they lie in memory: words of 32 bits.
 template <typename T>
 struct Raw {
-  uint4 v[sizeof(T)];
+  uint32_t w[4 * sizeof(T)];
 };
 
-template <typename T, bool kVec>
+// kAlign: the boundaries that rows start on, 32 or 16 bytes (wide accesses; with 32
+// whole sectors each), or 0: element by element.
+template <typename T, int kAlign>
 __device__ __forceinline__ Raw<T> load(const T* p) {
   Raw<T> r;
-  if constexpr (kVec) {
+  if constexpr (kAlign == 32) {
 #pragma unroll
-    for (int i = 0; i < (int)sizeof(T); ++i) r.v[i] = __ldg(reinterpret_cast<const uint4*>(p) + i);
+    for (int i = 0; i < (int)(4 * sizeof(T)); i += 8)
+      asm volatile("ld.global.nc.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                   : "=r"(r.w[i]), "=r"(r.w[i + 1]), "=r"(r.w[i + 2]), "=r"(r.w[i + 3]), "=r"(r.w[i + 4]), "=r"(r.w[i + 5]),
+                     "=r"(r.w[i + 6]), "=r"(r.w[i + 7])
+                   : "l"(reinterpret_cast<const uint32_t*>(p) + i));
+  } else if constexpr (kAlign == 16) {
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T); ++i) {
+      const uint4 v = __ldg(reinterpret_cast<const uint4*>(p) + i);
+      r.w[4 * i] = v.x, r.w[4 * i + 1] = v.y, r.w[4 * i + 2] = v.z, r.w[4 * i + 3] = v.w;
+    }
   } else {
     T e[kDims];
 #pragma unroll
@@ -48,11 +60,20 @@ __device__ __forceinline__ Raw<T> load(const T* p) {
   return r;
 }
 
-template <typename T, bool kVec>
+template <typename T, int kAlign>
 __device__ __forceinline__ void store(T* p, const Raw<T>& r) {
-  if constexpr (kVec) {
+  if constexpr (kAlign == 32) {
 #pragma unroll
-    for (int i = 0; i < (int)sizeof(T); ++i) reinterpret_cast<uint4*>(p)[i] = r.v[i];
+    for (int i = 0; i < (int)(4 * sizeof(T)); i += 8) {
+      uint32_t w[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) w[k] = r.w[i + k];
+      ptx::st_global_v8(reinterpret_cast<uint32_t*>(p) + i, w);
+    }
+  } else if constexpr (kAlign == 16) {
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T); ++i)
+      reinterpret_cast<uint4*>(p)[i] = make_uint4(r.w[4 * i], r.w[4 * i + 1], r.w[4 * i + 2], r.w[4 * i + 3]);
   } else {
     T e[kDims];
     memcpy(e, &r, sizeof(r));
@@ -128,10 +149,10 @@ __device__ __forceinline__ Raw<T> values(const uint16_t (&codes)[4], __half scal
   return r;
 }
 
-// Which token and rows (K rows, then V rows) an item is about.
+// Which token and heads an item is about.
 struct Item {
   int64_t b;
-  int t, r0, r1;
+  int t, h0, h1;
 };
 
 __device__ __forceinline__ Item item_of(const AiPaged4Args& a, uint32_t it, int per, int chunks) {
@@ -139,37 +160,34 @@ __device__ __forceinline__ Item item_of(const AiPaged4Args& a, uint32_t it, int 
   Item r;
   r.b = seq;
   r.t = (int)(tok - seq * (uint32_t)a.seq_len);
-  r.r0 = (int)(it - tok * (uint32_t)chunks) * per;
-  r.r1 = min(2 * a.num_kv_heads, r.r0 + per);
+  r.h0 = (int)(it - tok * (uint32_t)chunks) * per;
+  r.h1 = min(a.num_kv_heads, r.h0 + per);
   return r;
 }
 
-// A lane's sixteen dims of a row: of the tensor, of the codes, of the scales.
-template <typename T>
+// A lane's sixteen dims of head h of K or V: in the tensor, its codes, its scale.
+// (Dims 16 l + 4 i + j: group l / 2, byte pairs 4 (l % 2) + i.)
+template <typename T, int D>
 struct Spot {
+  static constexpr int C = D / kGroup;
   T* x;
   uint8_t* codes;
   __half* scale;
+  __device__ __forceinline__ Spot(const AiTensor4& tx, const AiTensor4& tc, const AiTensor4& ts, const Item& i, const Place& p, int64_t h, int l) {
+    x = static_cast<T*>(const_cast<void*>(tx.ptr)) + i.b * tx.stride_b + h * tx.stride_h + i.t * tx.stride_t + kDims * l;
+    codes = static_cast<uint8_t*>(const_cast<void*>(tc.ptr)) + p.page * tc.stride_b + h * tc.stride_h + p.slot * (D / 2) +
+            (l % 2 * 4) * 2 * C + l / 2 * 2;
+    scale = static_cast<__half*>(const_cast<void*>(ts.ptr)) + p.page * ts.stride_b + h * ts.stride_h + p.slot * C + l / 2;
+  }
+  __device__ __forceinline__ void advance(const AiTensor4& tx, const AiTensor4& tc, const AiTensor4& ts, int heads) {
+    x += heads * tx.stride_h, codes += heads * tc.stride_h, scale += heads * ts.stride_h;
+  }
 };
 
-template <typename T, int D>
-__device__ __forceinline__ Spot<T> spot_of(const AiPaged4Args& a, const Item& i, const Place& p, int row, int l) {
-  constexpr int C = D / kGroup;
-  const bool v = row >= a.num_kv_heads;
-  const int64_t h = v ? row - a.num_kv_heads : row;
-  const AiTensor4 &x = v ? a.v : a.k, &cd = v ? a.pool.v_codes : a.pool.k_codes, &sc = v ? a.pool.v_scales : a.pool.k_scales;
-  Spot<T> r;
-  r.x = static_cast<T*>(const_cast<void*>(x.ptr)) + i.b * x.stride_b + h * x.stride_h + i.t * x.stride_t + kDims * l;
-  // (dims 16 l + 4 i + j: group l / 2, byte pairs 4 (l % 2) + i)
-  r.codes = static_cast<uint8_t*>(const_cast<void*>(cd.ptr)) + p.page * cd.stride_b + h * cd.stride_h + p.slot * (D / 2) +
-            (l % 2 * 4) * 2 * C + l / 2 * 2;
-  r.scale = static_cast<__half*>(const_cast<void*>(sc.ptr)) + p.page * sc.stride_b + h * sc.stride_h + p.slot * C + l / 2;
-  return r;
-}
-
-template <typename T, int D, bool kVec>
+// (a turn: K and V of as many heads as 512 dims are, R)
+template <typename T, int D, int kAlign>
 __global__ void __launch_bounds__(kThreads) append_kernel(const AiPaged4Args a, const int per, const int chunks, const uint32_t items) {
-  constexpr int L = D / kDims, R = 32 / L, C = D / kGroup;  // lanes of a row, rows of a turn
+  constexpr int L = D / kDims, R = 32 / L, C = D / kGroup;  // lanes of a row
   const int lane = threadIdx.x % 32, sub = lane / L, l = lane % L;
   const uint32_t it = blockIdx.x * kWarps + threadIdx.x / 32;
   if (it >= items) return;
@@ -180,29 +198,30 @@ __global__ void __launch_bounds__(kThreads) append_kernel(const AiPaged4Args a, 
     report(a.status, AI_ERR_DEV_BOUNDS);
     return;
   }
-  for (int r0 = i.r0; r0 < i.r1; r0 += 2 * R) {
-    Spot<T> at[2];
-    Raw<T> raw[2];
+  int h = i.h0 + sub;
+  Spot<T, D> at[2] = {{a.k, a.pool.k_codes, a.pool.k_scales, i, p, h, l}, {a.v, a.pool.v_codes, a.pool.v_scales, i, p, h, l}};
+  for (int h0 = i.h0; h0 < i.h1; h0 += R, h += R) {
+    Raw<T> raw[2] = {};
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+      if (h < i.h1) raw[u] = load<T, kAlign>(at[u].x);
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-      at[u] = spot_of<T, D>(a, i, p, min(r0 + u * R + sub, i.r1 - 1), l);  // (rows past the last repeat it, unstored)
-      if (u == 0 || r0 + R < i.r1) raw[u] = load<T, kVec>(at[u].x);
-    }
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      if (u == 1 && r0 + R >= i.r1) break;
       uint16_t codes[4];
       __half scale;
       quantize<T>(raw[u], codes, scale);
-      if (r0 + u * R + sub >= i.r1) continue;
+      if (h < i.h1) {
 #pragma unroll
-      for (int k = 0; k < 4; ++k) *reinterpret_cast<uint16_t*>(at[u].codes + k * 2 * C) = codes[k];
-      if (l % 2 == 0) *at[u].scale = scale;
+        for (int k = 0; k < 4; ++k) *reinterpret_cast<uint16_t*>(at[u].codes + k * 2 * C) = codes[k];
+        if (l % 2 == 0) *at[u].scale = scale;
+      }
     }
+    at[0].advance(a.k, a.pool.k_codes, a.pool.k_scales, R);
+    at[1].advance(a.v, a.pool.v_codes, a.pool.v_scales, R);
   }
 }
 
-template <typename T, int D, bool kVec>
+template <typename T, int D, int kAlign>
 __global__ void __launch_bounds__(kThreads) read_kernel(const AiPaged4Args a, const int per, const int chunks, const uint32_t items) {
   constexpr int L = D / kDims, R = 32 / L, C = D / kGroup;
   const int lane = threadIdx.x % 32, sub = lane / L, l = lane % L;
@@ -214,20 +233,27 @@ __global__ void __launch_bounds__(kThreads) read_kernel(const AiPaged4Args a, co
     p = place(a.pool, i.b, (int64_t)__ldg(a.lens + i.b) + i.t);
     if (p.page < 0) report(a.status, AI_ERR_DEV_BOUNDS);
   }
-  for (int r0 = i.r0; r0 < i.r1; r0 += 2 * R) {
-    Spot<T> at[2];
-    uint16_t codes[2][4];
-    __half scale[2];
+  const bool held = p.page >= 0;
+  p.page = max(p.page, 0);
+  Spot<T, D> at[2] = {{a.k, a.pool.k_codes, a.pool.k_scales, i, p, i.h0 + sub, l}, {a.v, a.pool.v_codes, a.pool.v_scales, i, p, i.h0 + sub, l}};
+  for (int h = i.h0 + sub; h < i.h1; h += R) {
+    if (held) {
+      uint16_t codes[2][4];
+      __half scale[2];
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      at[u] = spot_of<T, D>(a, i, p, min(r0 + u * R + sub, i.r1 - 1), l);
+      for (int u = 0; u < 2; ++u) {
 #pragma unroll
-      for (int k = 0; k < 4; ++k) codes[u][k] = p.page < 0 ? (uint16_t)0x8888u : *reinterpret_cast<const uint16_t*>(at[u].codes + k * 2 * C);
-      scale[u] = p.page < 0 ? __ushort_as_half((unsigned short)0) : *at[u].scale;
+        for (int k = 0; k < 4; ++k) codes[u][k] = *reinterpret_cast<const uint16_t*>(at[u].codes + k * 2 * C);
+        scale[u] = *at[u].scale;
+      }
+#pragma unroll
+      for (int u = 0; u < 2; ++u) store<T, kAlign>(at[u].x, values<T>(codes[u], scale[u]));
+    } else {
+      store<T, kAlign>(at[0].x, Raw<T>{});
+      store<T, kAlign>(at[1].x, Raw<T>{});
     }
-#pragma unroll
-    for (int u = 0; u < 2; ++u)
-      if (r0 + u * R + sub < i.r1) store<T, kVec>(at[u].x, values<T>(codes[u], scale[u]));
+    at[0].advance(a.k, a.pool.k_codes, a.pool.k_scales, R);
+    at[1].advance(a.v, a.pool.v_codes, a.pool.v_scales, R);
   }
 }
 
@@ -246,17 +272,24 @@ int check(const AiPaged4Args* a) {
 
 template <typename T, int D>
 int launch(const AiPaged4Args& a, bool read, cudaStream_t st) {
-  // Two turns of rows per item while that gives every SM at most a few warps; then
-  // a token's rows stay together, so its page is looked up once.
-  constexpr int kTurns = 2 * 32 / (D / kDims);
+  // One turn per item while that gives every SM at most a few warps; then a
+  // token's heads stay together, so its page is looked up once.
+  constexpr int kTurn = 32 / (D / kDims);
   const int64_t tokens = (int64_t)a.batch * a.seq_len;
-  const int rows = 2 * a.num_kv_heads, per = tokens <= 4096 && kTurns < rows ? kTurns : rows;
-  const int chunks = (rows + per - 1) / per;
+  const int per = tokens <= 4096 && kTurn < a.num_kv_heads ? kTurn : a.num_kv_heads;
+  const int chunks = (a.num_kv_heads + per - 1) / per;
   const int64_t items = tokens * chunks, blocks = (items + kWarps - 1) / kWarps;
   if (items > 0x7fffffff) return AI_ERR_SHAPE;
-  const bool vec = headrow::rows_aligned(a.k, a.dtype) && headrow::rows_aligned(a.v, a.dtype);
-  const auto kernel = read ? (vec ? read_kernel<T, D, true> : read_kernel<T, D, false>)
-                           : (vec ? append_kernel<T, D, true> : append_kernel<T, D, false>);
+  int align = 32;
+  for (const AiTensor4* t : {&a.k, &a.v})
+    while (align >= 16 && ((reinterpret_cast<uintptr_t>(t->ptr) | (uintptr_t)((t->stride_b | t->stride_h | t->stride_t) * (int64_t)sizeof(T))) & (align - 1)))
+      align /= 2;
+  const auto kernel = read ? (align == 32   ? read_kernel<T, D, 32>
+                              : align == 16 ? read_kernel<T, D, 16>
+                                            : read_kernel<T, D, 0>)
+                           : (align == 32   ? append_kernel<T, D, 32>
+                              : align == 16 ? append_kernel<T, D, 16>
+                                            : append_kernel<T, D, 0>);
   ProfScope ps(AI_PROF_PAGED4, st);
   kernel<<<(unsigned)blocks, kThreads, 0, st>>>(a, per, chunks, (uint32_t)items);
   return cudaGetLastError() == cudaSuccess ? AI_OK : AI_ERR_LAUNCH;
