@@ -42,6 +42,11 @@ def sig(x: Optional[Tensor]):
     return None if x is None else (x.shape, x.stride(), x.dtype, x.get_device())
 
 
+def sigs(tensors) -> list:
+    """``sig`` of each (in one go: a decode step's calls are made of these)."""
+    return [None if x is None else (x.shape, x.stride(), x.dtype, x.get_device()) for x in tensors]
+
+
 class Plans(dict):
     """Checked argument structs by signature, at most a few hundred."""
 

@@ -50,7 +50,7 @@ def _plan(logits, ids, logprobs, weights, temperature, tail):
 
 def _planned(logits, ids, logprobs, weights, temperature, tail):
     tensors = (logits, ids, logprobs, weights, temperature)
-    at = (*map(_call.sig, tensors), tail)
+    at = (*_call.sigs(tensors), tail)
     plan = _PLANS.get(at)
     if plan is None:
         given = tensors

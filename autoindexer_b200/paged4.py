@@ -14,6 +14,7 @@ sequences that share a prompt list the same pages.
 
 from __future__ import annotations
 
+import ctypes
 from typing import Optional, Tuple
 
 import torch
@@ -46,7 +47,7 @@ def _pool(p, k_pages, v_pages, k_scales, v_scales, page_table, batch: int, heads
         st = x.stride()
         if st[2] != last or (st[3] != 1 and last > 1):
             raise ValueError(f"the slots of a page and head of {name} must follow one another")
-        if x.data_ptr() % 16 or (st[0] | st[1]) * x.element_size() % 16:
+        if (st[0] | st[1]) * x.element_size() % 16:
             raise ValueError(f"the pages and heads of {name} must start on 16-byte boundaries")
         _call.on_device(name, x, index)
     page_table = _table(page_table, batch, index)
@@ -59,13 +60,11 @@ def _pool(p, k_pages, v_pages, k_scales, v_scales, page_table, batch: int, heads
 
 
 def _point(p, k_pages, v_pages, k_scales, v_scales, page_table) -> None:
-    p.k_codes.ptr, p.v_codes.ptr = k_pages.data_ptr(), v_pages.data_ptr()
-    p.k_scales.ptr, p.v_scales.ptr = k_scales.data_ptr(), v_scales.data_ptr()
+    k, v, ks, vs = k_pages.data_ptr(), v_pages.data_ptr(), k_scales.data_ptr(), v_scales.data_ptr()
+    if (k | v | ks | vs) & 15:
+        raise ValueError("the pools must start on 16-byte boundaries")
+    p.k_codes.ptr, p.v_codes.ptr, p.k_scales.ptr, p.v_scales.ptr = k, v, ks, vs
     p.page_table = page_table.data_ptr()
-
-
-def _aligned(*pools: Tensor) -> Tuple[int, ...]:
-    return tuple(x.data_ptr() % 16 for x in pools)
 
 
 def _head_dim(D: int) -> None:
@@ -73,7 +72,7 @@ def _head_dim(D: int) -> None:
         raise ValueError(f"head_dim must be 32, 64 or 128, got {D}")
 
 
-_PLANS, _ATTEND_PLANS = _call.Plans(), _call.Plans()
+_PLANS, _READ_PLANS, _ATTEND_PLANS = _call.Plans(), _call.Plans(), _call.Plans()
 
 
 def _paged_plan(key, value, k_pages, v_pages, k_scales, v_scales, page_table, lens, n, name):
@@ -103,17 +102,11 @@ def _paged_plan(key, value, k_pages, v_pages, k_scales, v_scales, page_table, le
     return (key, value, k_pages, v_pages, k_scales, v_scales, page_table, lens, n), a
 
 
-def _paged(fn, what, tensors, name) -> None:
-    at = (*map(_call.sig, tensors), name, _aligned(*tensors[2:6]))
-    plan = _PLANS.get(at)
-    if plan is None:
-        given = tensors
-        tensors, plan = _paged_plan(*given, name)
-        _PLANS.keep(at, given, tensors, plan)
-    k, v, *pools, lens, n = tensors
+def _paged(fn, what, plan, tensors) -> None:
+    k, v, k_pages, v_pages, k_scales, v_scales, page_table, lens, n = tensors
     a = _call.copy(plan)
     a.k.ptr, a.v.ptr, a.lens = k.data_ptr(), v.data_ptr(), lens.data_ptr()
-    _point(a.pool, *pools)
+    _point(a.pool, k_pages, v_pages, k_scales, v_scales, page_table)
     if n is not None:
         a.n = n.data_ptr()
     _call.launch(fn, a, k.get_device(), what)
@@ -136,8 +129,14 @@ def paged_append_4bit(key: Tensor, value: Tensor, k_pages: Tensor, v_pages: Tens
     and the slots of a page and head follow one another in the pools, from a
     16-byte boundary (pages and heads may be strided).  Two tokens given the same
     slot race; no gradient flows through the cache."""
-    _paged(_lib.lib().ai_paged_append_4bit, "ai_paged_append_4bit",
-           (key, value, k_pages, v_pages, k_scales, v_scales, page_table, lens, new_lens), "new_lens")
+    tensors = (key, value, k_pages, v_pages, k_scales, v_scales, page_table, lens, new_lens)
+    at = tuple(_call.sigs(tensors))
+    plan = _PLANS.get(at)
+    if plan is None:
+        given = tensors
+        tensors, plan = _paged_plan(*given, "new_lens")
+        _PLANS.keep(at, given, tensors, plan)
+    _paged(_lib.lib().ai_paged_append_4bit, "ai_paged_append_4bit", plan, tensors)
 
 
 def paged_read_4bit(k_pages: Tensor, v_pages: Tensor, k_scales: Tensor, v_scales: Tensor, page_table: Tensor, lens: Tensor,
@@ -147,14 +146,22 @@ def paged_read_4bit(k_pages: Tensor, v_pages: Tensor, k_scales: Tensor, v_scales
     (0 past ``read_lens[b]``, int32, and where there is no page).  The call that
     mirrors ``paged_append_4bit``, with its arguments: what a prefill that wrote
     to the cache attends to, or a sequence on its way to another cache."""
-    if page_table.dim() != 2 or k_pages.dim() != 4 or n_tokens < 1:
-        raise ValueError(f"page_table must be (B, max_pages), k_pages (n_pages, Hkv, page_size, D / 2), n_tokens 1 or more, "
-                         f"got {tuple(page_table.shape)}, {tuple(k_pages.shape)}, {n_tokens}")
-    shape = (page_table.shape[0], k_pages.shape[1], int(n_tokens), 2 * k_pages.shape[3])
+    tensors = (k_pages, v_pages, k_scales, v_scales, page_table, lens, read_lens)
+    at = (*_call.sigs(tensors), n_tokens, dtype)
+    known = _READ_PLANS.get(at)
+    if known is None:
+        if page_table.dim() != 2 or k_pages.dim() != 4 or n_tokens < 1:
+            raise ValueError(f"page_table must be (B, max_pages), k_pages (n_pages, Hkv, page_size, D / 2), n_tokens 1 or more, "
+                             f"got {tuple(page_table.shape)}, {tuple(k_pages.shape)}, {n_tokens}")
+        shape = (page_table.shape[0], k_pages.shape[1], int(n_tokens), 2 * k_pages.shape[3])
+        given, like = tensors, torch.empty(shape, dtype=dtype, device=k_pages.device)
+        (_, _, *tensors), plan = _paged_plan(like, like, *given, "read_lens")
+        known = (shape, plan)
+        _READ_PLANS.keep(at, given, tensors, known)
+    shape, plan = known
     k = torch.empty(shape, dtype=dtype, device=k_pages.device)
-    v = torch.empty(shape, dtype=dtype, device=k_pages.device)
-    _paged(_lib.lib().ai_paged_read_4bit, "ai_paged_read_4bit",
-           (k, v, k_pages, v_pages, k_scales, v_scales, page_table, lens, read_lens), "read_lens")
+    v = torch.empty_like(k)
+    _paged(_lib.lib().ai_paged_read_4bit, "ai_paged_read_4bit", plan, (k, v, *tensors))
     return k, v
 
 
@@ -185,6 +192,15 @@ def _attend_plan(query, k_pages, v_pages, k_scales, v_scales, page_table, lens, 
     a.q = _call.strides4(q)
     a.out = _lib.AiTensor4(None, T * Hq * D, D, Hq * D)
     a.status = _call.status_ptr(index)
+    # (the workspace's size goes by the signature too; it is asked for with the pointers set)
+    asked = _call.copy(a)
+    asked.q.ptr = asked.out.ptr = q.data_ptr()
+    asked.lens = lens.data_ptr()
+    _point(asked.pool, k_pages, v_pages, k_scales, v_scales, page_table)
+    n = ctypes.c_size_t(0)
+    with torch.cuda.device(index):  # (by the device's SMs)
+        _lib.check(_lib.lib().ai_paged_attn_4bit_workspace(asked, n), "ai_paged_attn_4bit_workspace")
+    a.workspace_bytes = n.value
     return (q, k_pages, v_pages, k_scales, v_scales, page_table, lens, query_lens), a
 
 
@@ -209,7 +225,7 @@ def paged_attention_4bit(query: Tensor, k_pages: Tensor, v_pages: Tensor, k_scal
     backward through the results raises."""
     tensors = (query, k_pages, v_pages, k_scales, v_scales, page_table, lens, query_lens)
     scaling = None if scaling is None else float(scaling)
-    at = (*map(_call.sig, tensors), scaling, _aligned(*tensors[1:5]))
+    at = (*_call.sigs(tensors), scaling)
     plan = _ATTEND_PLANS.get(at)
     if plan is None:
         given = tensors
@@ -221,21 +237,21 @@ def paged_attention_4bit(query: Tensor, k_pages: Tensor, v_pages: Tensor, k_scal
 
 
 def _attend(plan, tensors, return_lse):
-    q, *pools, lens, query_lens = tensors
+    q, k_pages, v_pages, k_scales, v_scales, page_table, lens, query_lens = tensors
     B, Hq, T, D = q.shape
     device = q.device
     out = torch.empty((B, T, Hq, D), dtype=q.dtype, device=device)
     a = _call.copy(plan)
     a.q.ptr, a.out.ptr, a.lens = q.data_ptr(), out.data_ptr(), lens.data_ptr()
-    _point(a.pool, *pools)
+    _point(a.pool, k_pages, v_pages, k_scales, v_scales, page_table)
     if query_lens is not None:
         a.query_lens = query_lens.data_ptr()
     lse = None
     if return_lse:
         lse = torch.empty((B, Hq, T), dtype=torch.float32, device=device)
         a.lse = lse.data_ptr()
-    lib = _lib.lib()
-    ws = _call.workspace(lib.ai_paged_attn_4bit_workspace, a, device, "ai_paged_attn_4bit_workspace")
-    _call.launch(lib.ai_paged_attn_4bit, a, q.get_device(), "ai_paged_attn_4bit")
+    ws = torch.empty(a.workspace_bytes, dtype=torch.uint8, device=device)
+    a.workspace = ws.data_ptr()
+    _call.launch(_lib.lib().ai_paged_attn_4bit, a, q.get_device(), "ai_paged_attn_4bit")
     del ws
     return (out, lse) if return_lse else out

@@ -192,7 +192,7 @@ def token_logprobs(logits: Tensor, tokens: Tensor, temperature: Optional[Tensor]
     the logits' type), by one more read of them."""
     top_k = int(top_k)
     tensors = (logits, tokens, temperature)
-    at = (*map(_call.sig, tensors), top_k)
+    at = (*_call.sigs(tensors), top_k)
     plan = _PLANS.get(at)
     if plan is None:
         given = tensors
