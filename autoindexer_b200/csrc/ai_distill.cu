@@ -15,6 +15,16 @@
 // and the gradient: one bulk copy a slice, the listed words masked there (the sums
 // then need no look at the list), the sums exchanged through distributed shared
 // memory.
+//
+// Measured: 4096 rows of 151,936 bf16 with lists of 32, losses and gradients, 537 us
+// (4.4 TB/s); 1023 of 32,003 fp16 with lists of 64, the losses in one call and the
+// gradients in another, 72 us; 16 of 151,936 8.3 us.  What
+// keeps it from the memory's 365 us are the exponentials (two a logit: 250 us of the
+// SFU) and each slice's list, join and exchange (half of a CTA's 25,000 cycles), of
+// which the CTAs of an SM overlap as much as their shared memory holds.  Slices of 20
+// or 80 KB take 640 and 650 us; rows that pass through an SM as a pipeline (warps that
+// sum a row beside others that write the one before) 529, but twice the time where
+// there are few rows for an SM.
 
 #include <cooperative_groups.h>
 #include <cuda_runtime.h>
@@ -33,28 +43,32 @@ namespace distill {
 using namespace logits;
 namespace cg = cooperative_groups;
 
-constexpr int kThreads = 256, kWarps = kThreads / 32, U = 4;
+constexpr int kThreads = 256, kWarps = kThreads / 32;
+constexpr int U = 2;                   // vectors of a thread in flight
 constexpr int kMaxTop = AI_DISTILL_MAX_TOP;
+constexpr int kSets = kMaxTop / 32;    // entries of a lane
 constexpr int kMaxSplit = 16;
 constexpr int kLeast = 16 * 1024;      // bytes of a slice, at least (for more CTAs than the memory asks for)
-constexpr int kSlice = 40 * 1024;      // bytes of a slice where there are rows enough: five CTAs per SM
+constexpr int kSlice = 38 * 1024;      // bytes of a slice where there are rows enough: five CTAs per SM
 constexpr int kWidth = 32;             // slices are whole vectors of so many lanes
 static_assert(AI_DISTILL_MAX_ROW_BYTES / kMaxSplit + 16 * kWidth <= 200 * 1024, "a slice in shared memory");
-constexpr long long kWait = 1000000000LL;
 static_assert(kMaxTop <= kThreads, "a thread per entry");
+constexpr long long kWait = 1000000000LL;
 // A remainder of the teacher's probability below 2^-20 is what the rounding of
 // its fp32 log-probabilities may leave.
 constexpr float kLeastRest = 0x1p-20f;
 
-constexpr int kSets = kMaxTop / 32;  // entries of a lane
-
-// What the first warp finds out of a row's list while the slice is on its way.
+// What one warp finds out of a row's list.
 struct List {
   int live;            // whether the row has an entry (and a weight)
-  int word[kMaxTop];   // -1: left out
+  float up;            // weight / tau
+  float c, inv;        // log2(e) / tau, 1 / tau
   float p_top, p_rest; // the teacher's probability on the listed words, and beside them
   float m, s;          // the student's logits there: the largest, and the sum of 2^((x - m) c)
   float term;          // sum p (ln p - (x - m) / tau)
+  int word[kMaxTop];   // -1: left out
+  float x[kMaxTop];    // the student's logits
+  float p[kMaxTop];    // the teacher's probabilities
 };
 
 __device__ __forceinline__ float warp_sum(float v) {
@@ -73,143 +87,270 @@ __device__ __forceinline__ float share(float x, float c, float m) {
   return x == -CUDART_INF_F ? 0.f : ptx::ex2((x - m) * c);
 }
 
+// A row of the call.
 template <typename T>
-__global__ void __launch_bounds__(kThreads, 5) distill_kernel(const AiDistillArgs a, const int splits) {
+struct Row {
+  const T* x;
+  T* d;  // nullptr: losses alone
+  uint32_t b;
+  __device__ __forceinline__ Row(const AiDistillArgs& a, uint32_t row) {
+    b = row / (uint32_t)a.seq_len;
+    const int64_t t = row - b * (uint32_t)a.seq_len;
+    x = static_cast<const T*>(a.logits) + b * a.stride_b + t * a.stride_t;
+    d = a.dlogits ? static_cast<T*>(a.dlogits) + b * a.dstride_b + t * a.dstride_t : nullptr;
+  }
+};
+
+// A row's list, by one warp.  `known` is called as soon as it is known whether the
+// row is live.
+template <typename T, typename F>
+__device__ __forceinline__ void read_list(const AiDistillArgs& a, List& list, uint32_t row, bool reports, F known) {
+  const int lane = threadIdx.x % 32, K = a.n_top;
+  const Row<T> r(a, row);
+  int32_t* status = reports ? a.status : nullptr;
+  const float wgt = a.weights ? __ldg(a.weights + row) : 1.f;
+  const float tau = row_tau(a.temperature, r.b, nullptr);
+  int word[kSets];
+  float logp[kSets], p[kSets], xk[kSets];
+  bool any = false;
+#pragma unroll
+  for (int i = 0; i < kSets; ++i) {
+    const int k = 32 * i + lane;
+    word[i] = -1;
+    logp[i] = xk[i] = -CUDART_INF_F;
+    p[i] = 0.f;
+    if (32 * i >= K) continue;  // (here and below: sets past the list take no instruction of the warp)
+    if (k < K) {
+      const long long w = a.top_tokens[(int64_t)row * K + k];
+      logp[i] = a.top_logprobs[(int64_t)row * K + k];
+      if (wgt != 0.f && w >= a.vocab) report(status, AI_ERR_DEV_BOUNDS);
+      if (wgt != 0.f && w >= 0 && w < a.vocab && logp[i] != -CUDART_INF_F) {
+        word[i] = (int)w;
+        xk[i] = at(r.x, word[i]);
+      }
+    }
+    list.word[k] = word[i];
+    any |= word[i] >= 0;
+  }
+  any = __any_sync(0xffffffffu, any);
+  if (lane == 0) list.live = any;
+  known(any);
+  if (!any) return;
+  if (lane == 0) row_tau(a.temperature, r.b, status);
+  const float c = slope(tau), inv = inverse(tau);
+  // A word that an earlier entry has is left out.
+  bool again[kSets] = {};
+#pragma unroll
+  for (int i = 0; i < kSets; ++i) {
+    if (32 * i >= K) continue;
+    again[i] = (__match_any_sync(0xffffffffu, word[i]) & ((1u << lane) - 1)) != 0;
+    for (int j = 0; j < 32 * i; ++j) again[i] |= list.word[j] == word[i];
+  }
+  __syncwarp();
+  float top = -CUDART_INF_F, m = -CUDART_INF_F;
+#pragma unroll
+  for (int i = 0; i < kSets; ++i) {
+    if (32 * i >= K) continue;
+    if (again[i] && word[i] >= 0) {
+      report(status, AI_ERR_DEV_BOUNDS);
+      word[i] = list.word[32 * i + lane] = -1;
+      xk[i] = -CUDART_INF_F;
+    }
+    if (word[i] >= 0) top = fmaxf(top, logp[i]);
+    m = fmaxf(m, xk[i]);
+  }
+  const bool renorm = a.tail == AI_TAIL_RENORMALIZE;
+  if (renorm) {
+    top = warp_max(top);
+    float sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < kSets; ++i)
+      if (32 * i < K) sum += word[i] >= 0 ? expf(logp[i] - top) : 0.f;
+    const float norm = top + logf(warp_sum(sum));
+#pragma unroll
+    for (int i = 0; i < kSets; ++i) logp[i] -= norm;
+  }
+  m = warp_max(m);
+  const float o = m == -CUDART_INF_F ? 0.f : m;
+  float p_top = 0.f, sum = 0.f, term = 0.f;
+#pragma unroll
+  for (int i = 0; i < kSets; ++i) {
+    if (32 * i >= K) continue;
+    if (word[i] >= 0) p[i] = expf(logp[i]);
+    p_top += p[i];
+    sum += share(xk[i], c, o);
+    if (p[i] != 0.f) term += p[i] * logp[i] - p[i] * inv * (xk[i] - o);  // (p / tau first: logits may be as far apart as fp32 goes)
+    list.x[32 * i + lane] = xk[i];
+    list.p[32 * i + lane] = p[i];
+  }
+  p_top = warp_sum(p_top);
+  sum = warp_sum(sum);
+  term = warp_sum(term);
+  if (lane == 0) {
+    list.up = wgt * inv;
+    list.c = c;
+    list.inv = inv;
+    list.p_top = p_top;
+    list.p_rest = p_top != p_top ? p_top : renorm || 1.f - p_top < kLeastRest ? 0.f : 1.f - p_top;
+    list.m = m;
+    list.s = sum;
+    list.term = term;
+  }
+}
+
+// A warp's sum of the parts (m, s) of its lanes, with respect to their largest m.
+__device__ __forceinline__ float2 join_lanes(float2 q, float c) {
+  const float m = warp_max(q.x);
+  return make_float2(m, warp_sum(q.x == -CUDART_INF_F ? q.y : q.y * ptx::ex2((q.x - m) * c)));
+}
+
+// The row's ragged ends (elements before the first vector and behind the last one):
+// f(element) for those of a slice, one per thread.
+template <int E, typename F>
+__device__ __forceinline__ void ends(const Slice& sl, int vocab, int tid, F f) {
+  if (tid >= E) return;
+  if (sl.e0 + tid < sl.head) f(tid);
+  if (sl.e1 > sl.tail && sl.tail + tid < vocab) f(sl.tail + tid);
+}
+
+// An element of the ragged ends joins a thread's sum.
+__device__ __forceinline__ void add_end(Part& part, float f, float c) {
+  part = merge(part, Part{f, f == -CUDART_INF_F ? 0.f : f - f + 1.f, 0.f}, c);  // (NaN for +inf and NaN)
+}
+
+// All words of a row: the listed ones beside the others (m, s).
+struct Totals {
+  float m, s;          // of the others
+  float m_all, s_all;  // of all
+  float p_rest, mass;
+  bool empty;
+  __device__ __forceinline__ Totals(const List& list, float2 rest) {
+    m = rest.x, s = rest.y;
+    m_all = fmaxf(list.m, m);
+    const float of_top = list.m == -CUDART_INF_F ? 0.f : ptx::ex2((list.m - m_all) * list.c);
+    s_all = list.s * of_top + (m == -CUDART_INF_F ? s : s * of_rest(list));
+    p_rest = s == 0.f ? 0.f : list.p_rest;  // (no word for the bucket)
+    mass = list.p_top + p_rest;
+    empty = s_all == 0.f;
+  }
+  __device__ __forceinline__ float of_rest(const List& list) const {
+    return m == -CUDART_INF_F ? 0.f : ptx::ex2((m - m_all) * list.c);
+  }
+  // sum p (ln p - ln q), the list's part having been taken from its own largest logit.
+  __device__ __forceinline__ float loss(const List& list) const {
+    const float o = list.m == -CUDART_INF_F ? 0.f : list.m, l2 = log2f(s_all);
+    float r = list.term;
+    if (list.p_top != 0.f) r += list.p_top * list.inv * (m_all - o) + list.p_top * (l2 * kLn2);
+    if (p_rest != 0.f) r += p_rest * (logf(p_rest) - (log2f(s) - l2) * kLn2) - p_rest * list.inv * (m - m_all);
+    return empty ? CUDART_INF_F : r;
+  }
+  // Gradient of listed entry k.
+  __device__ __forceinline__ float listed(const List& list, int k) const {
+    return empty ? 0.f : list.up * (mass * (share(list.x[k], list.c, m_all) / s_all) - list.p[k]);
+  }
+};
+
+// Gradients of the words that are not listed: 2^((x - m) c) coef.  (Those of the
+// listed ones come out as anything and are written over.)
+struct Dense {
+  float m, c, coef;
+  Dense() = default;
+  __device__ __forceinline__ Dense(const List& list, const Totals& t) {
+    m = t.m == -CUDART_INF_F ? 0.f : t.m;
+    c = list.c;
+    coef = t.s == 0.f ? 0.f : list.up * (t.mass * t.of_rest(list) / t.s_all - t.p_rest / t.s);
+  }
+  __device__ __forceinline__ float one(float x) const { return ptx::ex2((x - m) * c) * coef; }
+  template <typename T>
+  __device__ __forceinline__ uint4 vector(const uint4& raw) const {
+    constexpr int E = 16 / sizeof(T);
+    const float2 nm = make_float2(-m, -m), cc = make_float2(c, c), cf = make_float2(coef, coef);
+    float2 f[E / 2];
+    Vec<T>::get(raw, f);
+#pragma unroll
+    for (int q = 0; q < E / 2; ++q) {
+      const float2 y = __fmul2_rn(__fadd2_rn(f[q], nm), cc);
+      f[q] = __fmul2_rn(make_float2(ptx::ex2(y.x), ptx::ex2(y.y)), cf);
+    }
+    return Vec<T>::put(f);
+  }
+};
+
+// Vector `out` to elements [v, v + E) of a row of the gradient; `wide`: on a 16-byte
+// boundary.
+template <typename T>
+__device__ __forceinline__ void put(T* d, int v, const uint4& out, bool wide) {
+  constexpr int E = 16 / sizeof(T);
+  if (wide) {
+    __stcs(reinterpret_cast<uint4*>(d + v), out);
+  } else {
+    T e[E];
+    memcpy(e, &out, 16);
+#pragma unroll
+    for (int q = 0; q < E; ++q) d[v + q] = e[q];
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ bool lie_alike(const T* x, const T* d) {
+  return ((reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(d)) & 15) == 0;
+}
+
+template <typename T>
+__device__ __forceinline__ void zero_row(T* d, int vocab, int split, int splits, int unit, int tid, int threads) {
+  constexpr int E = 16 / sizeof(T);
+  const Slice z = slice_of(d, vocab, split, splits, unit);
+  for (int i = z.i0 + tid; i < z.i1; i += threads) put(d, z.head + i * E, make_uint4(0u, 0u, 0u, 0u), true);
+  ends<E>(z, vocab, tid, [&](int v) { d[v] = from_f32<T>(0.f); });
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads, 6) distill_kernel(const AiDistillArgs a, const int splits) {
   constexpr int E = 16 / sizeof(T);
   __shared__ List list;
   __shared__ float2 s_parts[kMaxSplit * kWarps];  // (m, s) of each warp of the cluster
   __shared__ __align__(8) uint64_t s_bar;
   extern __shared__ __align__(128) uint8_t smem[];
   const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32, K = a.n_top;
-  const int64_t row = blockIdx.x / (uint32_t)splits;
+  const uint32_t row = blockIdx.x / (uint32_t)splits, bar = ptx::smem_u32(&s_bar);
   const int split = (int)(blockIdx.x - row * splits);
-  const int64_t b = row / a.seq_len, t = row - b * a.seq_len;
-  const T* x = static_cast<const T*>(a.logits) + b * a.stride_b + t * a.stride_t;
-  T* d = a.dlogits ? static_cast<T*>(a.dlogits) + b * a.dstride_b + t * a.dstride_t : nullptr;
-  const Slice sl = slice_of(x, a.vocab, split, splits, kWidth);
+  const Row<T> r(a, row);
+  const Slice sl = slice_of(r.x, a.vocab, split, splits, kWidth);
   const int vecs = sl.i1 - sl.i0;
-  const uint32_t bar = ptx::smem_u32(&s_bar);
   // (a CTA of the cluster must run before its shared memory is written to)
   if (splits > 1) asm volatile("barrier.cluster.arrive;" ::: "memory");
-  int word[kSets];
-  float logp[kSets], wgt = 1.f;
   if (warp == 0) {
-    if (a.weights) wgt = __ldg(a.weights + row);
-    bool any = false;
-#pragma unroll
-    for (int i = 0; i < kSets; ++i) {
-      const int k = 32 * i + lane;
-      word[i] = -1;
-      logp[i] = -CUDART_INF_F;
-      if (32 * i >= K) continue;  // (here and below: sets past the list take no instruction of the warp)
-      if (k < K) {
-        const long long w = a.top_tokens[row * K + k];
-        logp[i] = a.top_logprobs[row * K + k];
-        if (wgt != 0.f && w >= a.vocab && split == 0) report(a.status, AI_ERR_DEV_BOUNDS);
-        if (wgt != 0.f && w >= 0 && w < a.vocab && logp[i] != -CUDART_INF_F) word[i] = (int)w;
-      }
-      list.word[k] = word[i];
-      any |= word[i] >= 0;
-    }
-    any = __any_sync(0xffffffffu, any);
     if (lane == 0) {
       ptx::mbar_init(bar, 1);
       ptx::fence_mbar_init();
-      list.live = any;
-      if (any && vecs > 0) {
-        ptx::mbar_arrive_expect_tx(bar, 16u * vecs);
-        ptx::bulk_load(ptx::smem_u32(smem), x + sl.head + (int64_t)sl.i0 * E, 16u * vecs, bar);
-      }
     }
+    read_list<T>(a, list, row, split == 0, [&](bool live) {
+      if (lane == 0 && live && vecs > 0) {
+        ptx::mbar_arrive_expect_tx(bar, 16u * vecs);
+        ptx::bulk_load(ptx::smem_u32(smem), r.x + sl.head + (int64_t)sl.i0 * E, 16u * vecs, bar);
+      }
+    });
   }
   __syncthreads();
   if (!list.live) {
     if (split == 0 && tid == 0 && a.losses) a.losses[row] = 0.f;
-    if (d) {
-      const Slice z = slice_of(d, a.vocab, split, splits, kWidth);
-      uint4* dv = reinterpret_cast<uint4*>(d + z.head);
-      for (int i = z.i0 + tid; i < z.i1; i += kThreads) __stcs(dv + i, make_uint4(0u, 0u, 0u, 0u));
-      if (tid < E) {
-        if (z.e0 + tid < z.head) d[tid] = from_f32<T>(0.f);
-        if (z.e1 > z.tail && z.tail + tid < a.vocab) d[z.tail + tid] = from_f32<T>(0.f);
-      }
-    }
+    if (r.d) zero_row(r.d, a.vocab, split, splits, kWidth, tid, kThreads);
     return;
-  }
-  const float tau = row_tau(a.temperature, b, split == 0 && tid == 0 ? a.status : nullptr), c = slope(tau), inv = inverse(tau);
-  float p[kSets], xk[kSets];
-  if (warp == 0) {
-#pragma unroll
-    for (int i = 0; i < kSets; ++i) xk[i] = word[i] >= 0 ? at(x, word[i]) : -CUDART_INF_F;
-    // A word that an earlier entry has is left out.
-    bool again[kSets] = {};
-#pragma unroll
-    for (int i = 0; i < kSets; ++i) {
-      if (32 * i >= K) continue;
-      again[i] = (__match_any_sync(0xffffffffu, word[i]) & ((1u << lane) - 1)) != 0;
-      for (int j = 0; j < 32 * i; ++j) again[i] |= list.word[j] == word[i];
-    }
-    __syncwarp();
-    float top = -CUDART_INF_F, m = -CUDART_INF_F;
-#pragma unroll
-    for (int i = 0; i < kSets; ++i) {
-      if (32 * i >= K) continue;
-      if (again[i] && word[i] >= 0) {
-        if (split == 0) report(a.status, AI_ERR_DEV_BOUNDS);
-        word[i] = list.word[32 * i + lane] = -1;
-        xk[i] = -CUDART_INF_F;
-      }
-      if (word[i] >= 0) top = fmaxf(top, logp[i]);
-      m = fmaxf(m, xk[i]);
-    }
-    const bool renorm = a.tail == AI_TAIL_RENORMALIZE;
-    if (renorm) {
-      top = warp_max(top);
-      float sum = 0.f;
-#pragma unroll
-      for (int i = 0; i < kSets; ++i)
-        if (32 * i < K) sum += word[i] >= 0 ? expf(logp[i] - top) : 0.f;
-      const float norm = top + logf(warp_sum(sum));
-#pragma unroll
-      for (int i = 0; i < kSets; ++i) logp[i] -= norm;
-    }
-    m = warp_max(m);
-    const float o = m == -CUDART_INF_F ? 0.f : m;
-    float p_top = 0.f, sum = 0.f, term = 0.f;
-#pragma unroll
-    for (int i = 0; i < kSets; ++i) {
-      if (32 * i >= K) continue;
-      p[i] = word[i] >= 0 ? expf(logp[i]) : 0.f;
-      p_top += p[i];
-      sum += share(xk[i], c, o);
-      if (p[i] != 0.f) term += p[i] * (logp[i] - (xk[i] - o) * inv);
-    }
-    p_top = warp_sum(p_top);
-    sum = warp_sum(sum);
-    term = warp_sum(term);
-    if (lane == 0) {
-      list.p_top = p_top;
-      list.p_rest = p_top != p_top ? p_top : renorm || 1.f - p_top < kLeastRest ? 0.f : 1.f - p_top;
-      list.m = m;
-      list.s = sum;
-      list.term = term;
-    }
   }
   if (vecs > 0 && !ptx::mbar_wait(bar, 0, kWait)) {
     report(a.status, AI_ERR_DEV_TIMEOUT);
     ptx::mbar_wait(bar, 0, kWait);  // (the copy lands before the CTA ends)
   }
   // The listed words' places become -inf, which adds nothing to the others' sum.
-  if (warp == 0) {
-#pragma unroll
-    for (int i = 0; i < kSets; ++i) {
-      const int at_ = word[i] - sl.head - sl.i0 * E;
-      if (word[i] >= 0 && at_ >= 0 && at_ < vecs * E) reinterpret_cast<T*>(smem)[at_] = from_f32<T>(-CUDART_INF_F);
+  if (warp == 0)
+    for (int k = lane; k < K; k += 32) {
+      const int w = list.word[k], at_ = w - sl.head - sl.i0 * E;
+      if (w >= 0 && at_ >= 0 && at_ < vecs * E) reinterpret_cast<T*>(smem)[at_] = from_f32<T>(-CUDART_INF_F);
     }
-  }
   __syncthreads();
   const uint4* held = reinterpret_cast<const uint4*>(smem);
   const uint4 none = make_uint4(Vec<T>::kNone, Vec<T>::kNone, Vec<T>::kNone, Vec<T>::kNone);
+  const float c = list.c;
   Part part{-CUDART_INF_F, 0.f, 0.f};
   for (int i = tid; i < vecs; i += kThreads * U) {
     uint4 raw[U];
@@ -217,92 +358,39 @@ __global__ void __launch_bounds__(kThreads, 5) distill_kernel(const AiDistillArg
     for (int u = 0; u < U; ++u) raw[u] = i + u * kThreads < vecs ? held[i + u * kThreads] : none;
     accumulate<T, U, false>(part, raw, c);
   }
-  if (tid < E) {
-    auto one = [&](int v) {
-      for (int j = 0; j < K; ++j)
-        if (list.word[j] == v) return;
-      const float f = at(x, v);
-      part = merge(part, Part{f, f == -CUDART_INF_F ? 0.f : f - f + 1.f, 0.f}, c);
-    };
-    if (sl.e0 + tid < sl.head) one(tid);
-    if (sl.e1 > sl.tail && sl.tail + tid < a.vocab) one(sl.tail + tid);
-  }
+  ends<E>(sl, a.vocab, tid, [&](int v) {
+    for (int j = 0; j < K; ++j)
+      if (list.word[j] == v) return;
+    add_end(part, at(r.x, v), c);
+  });
   // The warps' sums go to every CTA of the cluster; each joins them in the same order.
-  {
-    const float m = warp_max(part.m), s = warp_sum(part.m == -CUDART_INF_F ? part.s : part.s * ptx::ex2((part.m - m) * c));
-    if (splits > 1) {
-      const cg::cluster_group cluster = cg::this_cluster();
-      asm volatile("barrier.cluster.wait;" ::: "memory");
-      if (lane < splits) cluster.map_shared_rank(s_parts, lane)[split * kWarps + warp] = make_float2(m, s);
-      cluster.sync();
-    } else {
-      if (lane == 0) s_parts[warp] = make_float2(m, s);
-      __syncthreads();
-    }
+  const float2 mine = join_lanes(make_float2(part.m, part.s), c);
+  if (splits > 1) {
+    const cg::cluster_group cluster = cg::this_cluster();
+    asm volatile("barrier.cluster.wait;" ::: "memory");
+    if (lane < splits) cluster.map_shared_rank(s_parts, lane)[split * kWarps + warp] = mine;
+    cluster.sync();
+  } else {
+    if (lane == 0) s_parts[warp] = mine;
+    __syncthreads();
   }
-  float m_rest = -CUDART_INF_F, s_rest = 0.f;
-  for (int i = lane; i < splits * kWarps; i += 32) m_rest = fmaxf(m_rest, s_parts[i].x);
-  m_rest = warp_max(m_rest);
+  float2 rest = make_float2(-CUDART_INF_F, 0.f);
   for (int i = lane; i < splits * kWarps; i += 32) {
-    const float2 q = s_parts[i];
-    s_rest += q.x == -CUDART_INF_F ? q.y : q.y * ptx::ex2((q.x - m_rest) * c);
+    const Part q = merge(Part{rest.x, rest.y, 0.f}, Part{s_parts[i].x, s_parts[i].y, 0.f}, c);
+    rest = make_float2(q.m, q.s);
   }
-  s_rest = warp_sum(s_rest);
-  // All words: the listed ones beside the others.
-  const float p_top = list.p_top, m_all = fmaxf(list.m, m_rest);
-  const float of_top = list.m == -CUDART_INF_F ? 0.f : ptx::ex2((list.m - m_all) * c);
-  const float of_rest = m_rest == -CUDART_INF_F ? 0.f : ptx::ex2((m_rest - m_all) * c);
-  const float s_all = list.s * of_top + (m_rest == -CUDART_INF_F ? s_rest : s_rest * of_rest);
-  const float p_rest = s_rest == 0.f ? 0.f : list.p_rest;  // (no word for the bucket)
-  const bool empty = s_all == 0.f;
-  const float l2 = log2f(s_all);
-  if (split == 0 && tid == 0 && a.losses) {
-    // sum p (ln p - ln q), the list's part having been taken from its own largest logit
-    const float o = list.m == -CUDART_INF_F ? 0.f : list.m;
-    float loss = list.term;
-    if (p_top != 0.f) loss += p_top * ((m_all - o) * inv + l2 * kLn2);
-    if (p_rest != 0.f) loss += p_rest * (logf(p_rest) - (m_rest - m_all) * inv - (log2f(s_rest) - l2) * kLn2);
-    a.losses[row] = empty ? CUDART_INF_F : loss;
-  }
-  if (!d) return;
-  const float weight = a.weights ? __ldg(a.weights + row) : 1.f;
-  const float up = weight * inv, mass = p_top + p_rest, m = m_rest == -CUDART_INF_F ? 0.f : m_rest;
-  const float coef = s_rest == 0.f ? 0.f : up * (mass * of_rest / s_all - p_rest / s_rest);
-  const float2 nm = make_float2(-m, -m), cc = make_float2(c, c), cf = make_float2(coef, coef);
-  const bool alike = ((reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(d)) & 15) == 0;
-  uint4* dv = reinterpret_cast<uint4*>(d + sl.head) + sl.i0;
+  const Totals all(list, join_lanes(rest, c));
+  if (split == 0 && tid == 0 && a.losses) a.losses[row] = all.loss(list);
+  if (!r.d) return;
+  const Dense dense(list, all);
+  const bool alike = lie_alike(r.x, r.d);
 #pragma unroll 2
-  for (int i = tid; i < vecs; i += kThreads) {
-    float2 f[E / 2];
-    Vec<T>::get(held[i], f);
-#pragma unroll
-    for (int q = 0; q < E / 2; ++q) {
-      const float2 y = __fmul2_rn(__fadd2_rn(f[q], nm), cc);
-      f[q] = __fmul2_rn(make_float2(ptx::ex2(y.x), ptx::ex2(y.y)), cf);
-    }
-    const uint4 out = Vec<T>::put(f);
-    if (alike) {
-      __stcs(dv + i, out);
-    } else {
-      T el[E];
-      memcpy(el, &out, 16);
-#pragma unroll
-      for (int q = 0; q < E; ++q) d[sl.head + (sl.i0 + i) * E + q] = el[q];
-    }
-  }
-  if (tid < E) {
-    auto one = [&](int v) { d[v] = from_f32<T>(ptx::ex2((at(x, v) - m) * c) * coef); };
-    if (sl.e0 + tid < sl.head) one(tid);
-    if (sl.e1 > sl.tail && sl.tail + tid < a.vocab) one(sl.tail + tid);
-  }
+  for (int i = tid; i < vecs; i += kThreads) put(r.d, sl.head + (sl.i0 + i) * E, dense.template vector<T>(held[i]), alike);
+  ends<E>(sl, a.vocab, tid, [&](int v) { r.d[v] = from_f32<T>(dense.one(at(r.x, v))); });
   __syncthreads();
-  if (warp == 0) {
-#pragma unroll
-    for (int i = 0; i < kSets; ++i) {
-      if (word[i] < sl.e0 || word[i] >= sl.e1) continue;
-      const float q = share(xk[i], c, m_all) / s_all;
-      d[word[i]] = from_f32<T>(empty ? 0.f : up * (mass * q - p[i]));
-    }
+  if (tid < K) {
+    const int w = list.word[tid];
+    if (w >= sl.e0 && w < sl.e1) r.d[w] = from_f32<T>(all.listed(list, tid));
   }
 }
 
@@ -345,6 +433,7 @@ int64_t slice_bytes(const AiDistillArgs& a, int splits) {
 
 template <typename T>
 int launch(const AiDistillArgs& a, cudaStream_t st) {
+  ProfScope ps(AI_PROF_DISTILL, st);
   const int splits = slices(a);
   const int64_t smem = slice_bytes(a, splits);
   if (splits > 8 &&
@@ -363,7 +452,6 @@ int launch(const AiDistillArgs& a, cudaStream_t st) {
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = splits > 1 ? 1 : 0;
-  ProfScope ps(AI_PROF_DISTILL, st);
   if (cudaLaunchKernelEx(&cfg, distill_kernel<T>, a, splits) != cudaSuccess) return AI_ERR_LAUNCH;
   return cudaGetLastError() == cudaSuccess ? AI_OK : AI_ERR_LAUNCH;
 }

@@ -50,6 +50,8 @@ def check(x, ids, t, w, tau, tail, losses, grad):
         weight = 1.0 if w is None else w.reshape(-1)[i].double().item()
         loss, d, mag, big = O.distill_row(row, ids[i], t[i], 1.0 if tau is None else float(tau[i // per]), tail, weight)
         if losses is not None:
+            if loss > torch.finfo(torch.float32).max:  # rounds to inf: logits at the type's lowest value, divided by tau < 1
+                loss = INF
             close(losses.reshape(-1)[i].item(), loss, REL * (1 + big), f"loss of row {i}")
         if grad is not None:
             fin = torch.finfo(dtype)
@@ -137,6 +139,33 @@ def test_awkward_rows(V, tail, cuda_device):
     t[:, 2] = -INF
     check(x, ids, t, None, None, tail, *distill_loss_and_grad(x, ids, t, tail=tail))
     assert read_status(cuda_device) == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("tail", TAILS)
+@pytest.mark.parametrize("V,K,dtype", [(7, 3, torch.bfloat16), (1003, 40, torch.float16), (3077, 128, torch.bfloat16), (9001, 64, torch.float32),
+                                       (30011, 100, torch.bfloat16)])
+def test_many_rows(V, K, dtype, tail, cuda_device):
+    """More rows than run at once, awkward ones among them: copies of a row come out alike,
+    in place too, and losses do not depend on whether the gradient is written."""
+    from autoindexer_b200 import distill_loss, distill_loss_and_grad, read_status
+
+    x, ids, t, w, tau = make((24,), V, K, dtype, K)
+    for i, row in enumerate(list(odd_rows(V).values())[:12] if V > 20 else []):
+        x[3 + i] = row.to(dtype)
+    ids[20, 0], ids[20, -1] = 0, V - 1
+    few = [x, ids, t, w, tau]
+    many = [y.repeat(50, *[1] * (y.dim() - 1)).to(cuda_device) for y in few]
+    losses, grad = distill_loss_and_grad(*many, tail=tail)
+    check(*few[:3], w, tau, tail, losses[:24].cpu(), grad[:24].cpu())
+    for y in (losses, grad):
+        assert all(torch.equal(y[24 * i:24 * i + 24].nan_to_num(9), y[:24].nan_to_num(9)) for i in range(50))
+    alone = distill_loss(*many[:3], many[4], tail=tail)
+    here = distill_loss_and_grad(*many, tail=tail, out=many[0])
+    assert torch.equal(here[1].nan_to_num(9), grad.nan_to_num(9))
+    live = many[3] != 0
+    assert torch.equal(alone[live].nan_to_num(9), losses[live].nan_to_num(9))
+    read_status(cuda_device)  # (word 0 is also word V - 1 where a list has one twice)
 
 
 @pytest.mark.gpu
