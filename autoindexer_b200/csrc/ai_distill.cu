@@ -16,7 +16,7 @@
 // then need no look at the list), the sums exchanged through distributed shared
 // memory.
 //
-// Measured: 4096 rows of 151,936 bf16 with lists of 32, losses and gradients, 537 us
+// Measured: 4096 rows of 151,936 bf16, most with lists of 32, losses and gradients, 537 us
 // (4.4 TB/s); 1023 of 32,003 fp16 with lists of 64, the losses in one call and the
 // gradients in another, 72 us; 16 of 151,936 8.3 us.  What
 // keeps it from the memory's 365 us are the exponentials (two a logit: 250 us of the

@@ -19,6 +19,12 @@
 // 1 KB pieces, kept on the way, say where the others are (about k pieces).  A part
 // whose logits crowd above that bound (ties, sorted rows) is gone through in order
 // instead, keeping the best so far.
+//
+// Measured: 4096 rows of 151,936 bf16 with entropies, 3592 of them with a token,
+// forward 188 us (5.8 TB/s), backward 366 us (6.4 TB/s): at the memory's rate.  509
+// rows of fp32 with the 32 likeliest 66 us (4.6 TB/s; less than four CTAs per SM, the
+// last of which find the memory idle).  8 rows of bf16 with the 20 likeliest 14 us:
+// latency, of which the list is 6 us.
 
 #include <cooperative_groups.h>
 #include <cuda_runtime.h>

@@ -638,8 +638,9 @@ int ai_verify_draft(const AiVerifyArgs* args, void* stream);
  *   logprob = z[token] - lse(z),  entropy = -sum_v p_v ln p_v,  p = softmax(z),
  *   top: the words with the largest logits, best first, equal ones by index,
  *   and their log-probabilities; -1 and -inf past the unmasked words.
- * A row whose token is negative is padding: it is not read, its log-probability
- * and entropy are 0, its list is empty; so is one whose token lies outside the
+ * A row whose token is negative is padding: what it holds does not matter (it is
+ * not read, but for a first part where rows are few), its log-probability and
+ * entropy are 0, its list is empty; so is one whose token lies outside the
  * vocabulary, which is AI_ERR_DEV_BOUNDS too.  A row without an unmasked word
  * has the log-probability -inf, entropy 0 and an empty list; a row with a NaN
  * has an empty list (its log-probabilities NaN). */
