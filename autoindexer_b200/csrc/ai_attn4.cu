@@ -12,9 +12,12 @@
 //                 scale in fp32;
 //   O^T += V^T P  P takes each key's V scale, per group of 32 dims: weights, held 2^7
 //                 above 1 at the running maximum, and scales, divided by the power
-//                 of two above the largest |scale| met so far, are fp16, and so is
-//                 their product (two roundings of 2^-12; weights down to 2^-31 of
-//                 the largest count).
+//                 of two above the largest |scale| met so far, have an fp16 product
+//                 (weights down to 2^-31 of the largest count).  For bf16 queries the
+//                 weights are fp16 before it, two roundings of 2^-12 beside the output's
+//                 2^-9; for fp16 ones the product is rounded alone: the error against 64
+//                 bits is then 1.33 times that of the output's rounding, not 1.6 times, and
+//                 the drafted case below takes 152 us, not 145.
 // The codes are fp16's subnormal numbers as they lie, 2^-24 c: one logical operation
 // a pair.  (Their 8 comes off K's as the sums start, off V's before the product.)
 // Both products have the tile's keys on the instruction's long side, so up to 8
@@ -25,7 +28,7 @@
 // query token each, 73 us (4.1 TB/s); 32 of up to 32,768 125 us (4.7 TB/s): the 684
 // instructions a warp spends on a tile of 32 keys, issued in 72% of the cycles, bound
 // it together with the loads.  With up to five query tokens (20 rows to a KV head,
-// three column blocks) 144 us: eight warps an SM, as their sums fill the registers, do
+// three column blocks) 152 us: eight warps an SM, as their sums fill the registers, do
 // not cover the latencies of 980 instructions a tile.  4 sequences of 322 tokens 12.8
 // us: one tile's latency, a launch, and the second one's joining.
 
@@ -35,6 +38,7 @@
 
 #include <cfloat>
 #include <cstring>
+#include <type_traits>
 
 #include "ai_common.cuh"
 #include "ai_kernels.h"
@@ -273,6 +277,7 @@ __global__ void __launch_bounds__(32 * warps_of(NT), 1) split_kernel(const AiPag
   using L = Tile<D>;
   using M = Smem<D, NT>;
   constexpr int C = L::C, H = (C + 1) / 2, S = kStages;
+  constexpr bool kOnce = std::is_same<T, __half>::value;  // weights times scales are rounded once
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   extern __shared__ __align__(128) uint8_t smem[];
   int* scan = reinterpret_cast<int*>(smem + M::SCAN);
@@ -651,9 +656,17 @@ __global__ void __launch_bounds__(32 * warps_of(NT), 1) split_kernel(const AiPag
             const float2 y = __ffma2_rn(sc[mt][nt][h], make_float2(slope, slope), make_float2(-ref[nt][0], -ref[nt][1]));
             const float2 w = make_float2(ptx::ex2(y.x), ptx::ex2(y.y));
             l[nt] = __fadd2_rn(l[nt], w);
-            const uint32_t w2 = pack2(w.x, w.y);
+            if constexpr (kOnce) {
 #pragma unroll
-            for (int c = 0; c < C; ++c) pv[nt][c][h] = mul2(w2, twice_of(vs[mt][h][c / 2], c % 2));
+              for (int c = 0; c < C; ++c) {
+                const float d = half_of(vs[mt][h][c / 2], c % 2);
+                pv[nt][c][h] = pack2(w.x * d, w.y * d);
+              }
+            } else {
+              const uint32_t w2 = pack2(w.x, w.y);
+#pragma unroll
+              for (int c = 0; c < C; ++c) pv[nt][c][h] = mul2(w2, twice_of(vs[mt][h][c / 2], c % 2));
+            }
             if (guard) {
               const uint32_t keep = (sc[mt][nt][h].x == -CUDART_INF_F ? 0u : 0xffffu) | (sc[mt][nt][h].y == -CUDART_INF_F ? 0u : 0xffff0000u);
 #pragma unroll
