@@ -13,15 +13,15 @@
 // HBM-bound: a row is read once and its gradient written.  A row is cut for a
 // cluster of CTAs, so that its slices stay in their shared memory between the sums
 // and the gradient: one bulk copy a slice, the listed words masked there (the sums
-// then need no look at the list), the sums exchanged through distributed shared
-// memory.
+// then need no look at the list; one warp gathers the list's own sums meanwhile), the
+// sums exchanged through distributed shared memory.
 //
 // Measured: 4096 rows of 151,936 bf16, most with lists of 32, losses and gradients, 537 us
 // (4.4 TB/s); 1023 of 32,003 fp16 with lists of 64, the losses in one call and the
-// gradients in another, 72 us; 16 of 151,936 8.3 us.  What
-// keeps it from the memory's 365 us are the exponentials (two a logit: 250 us of the
-// SFU) and each slice's list, join and exchange (half of a CTA's 25,000 cycles), of
-// which the CTAs of an SM overlap as much as their shared memory holds.  Slices of 20
+// gradients in another, 70 us; 16 of 151,936 8.0 us.  Between
+// it and the memory's 365 us stand the instructions (issued in 56% of the cycles; two
+// exponentials a logit keep the SFU busy for 58%) and the phases of a slice, which
+// the CTAs of an SM overlap as much as their shared memory holds.  Slices of 20
 // or 80 KB take 640 and 650 us; rows that pass through an SM as a pipeline (warps that
 // sum a row beside others that write the one before) 529, but twice the time where
 // there are few rows for an SM.
@@ -52,7 +52,7 @@ constexpr int kLeast = 16 * 1024;      // bytes of a slice, at least (for more C
 constexpr int kSlice = 38 * 1024;      // bytes of a slice where there are rows enough: five CTAs per SM
 constexpr int kWidth = 32;             // slices are whole vectors of so many lanes
 static_assert(AI_DISTILL_MAX_ROW_BYTES / kMaxSplit + 16 * kWidth <= 200 * 1024, "a slice in shared memory");
-static_assert(kMaxTop <= kThreads, "a thread per entry");
+static_assert(kMaxTop <= kThreads - 32, "a thread per entry");
 constexpr long long kWait = 1000000000LL;
 // A remainder of the teacher's probability below 2^-20 is what the rounding of
 // its fp32 log-probabilities may leave.
@@ -101,24 +101,30 @@ struct Row {
   }
 };
 
-// A row's list, by one warp.  `known` is called as soon as it is known whether the
-// row is live.
+// A lane's entries of a row's list.
+struct Entries {
+  int word[kSets];
+  float logp[kSets], x[kSets];
+  float wgt, inv;
+};
+
+// A row's list, by one warp: its words, which the others wait for (`known` is called as
+// soon as it is known whether the row is live) ...
 template <typename T, typename F>
-__device__ __forceinline__ void read_list(const AiDistillArgs& a, List& list, uint32_t row, bool reports, F known) {
+__device__ __forceinline__ void read_words(const AiDistillArgs& a, List& list, Entries& mine, uint32_t row, bool reports, F known) {
   const int lane = threadIdx.x % 32, K = a.n_top;
   const Row<T> r(a, row);
   int32_t* status = reports ? a.status : nullptr;
   const float wgt = a.weights ? __ldg(a.weights + row) : 1.f;
   const float tau = row_tau(a.temperature, r.b, nullptr);
-  int word[kSets];
-  float logp[kSets], p[kSets], xk[kSets];
+  int(&word)[kSets] = mine.word;
+  float(&logp)[kSets] = mine.logp, (&xk)[kSets] = mine.x;
   bool any = false;
 #pragma unroll
   for (int i = 0; i < kSets; ++i) {
     const int k = 32 * i + lane;
     word[i] = -1;
     logp[i] = xk[i] = -CUDART_INF_F;
-    p[i] = 0.f;
     if (32 * i >= K) continue;  // (here and below: sets past the list take no instruction of the warp)
     if (k < K) {
       const long long w = a.top_tokens[(int64_t)row * K + k];
@@ -137,7 +143,9 @@ __device__ __forceinline__ void read_list(const AiDistillArgs& a, List& list, ui
   known(any);
   if (!any) return;
   if (lane == 0) row_tau(a.temperature, r.b, status);
-  const float c = slope(tau), inv = inverse(tau);
+  mine.wgt = wgt;
+  mine.inv = inverse(tau);
+  if (lane == 0) list.c = slope(tau);
   // A word that an earlier entry has is left out.
   bool again[kSets] = {};
 #pragma unroll
@@ -147,7 +155,6 @@ __device__ __forceinline__ void read_list(const AiDistillArgs& a, List& list, ui
     for (int j = 0; j < 32 * i; ++j) again[i] |= list.word[j] == word[i];
   }
   __syncwarp();
-  float top = -CUDART_INF_F, m = -CUDART_INF_F;
 #pragma unroll
   for (int i = 0; i < kSets; ++i) {
     if (32 * i >= K) continue;
@@ -156,6 +163,21 @@ __device__ __forceinline__ void read_list(const AiDistillArgs& a, List& list, ui
       word[i] = list.word[32 * i + lane] = -1;
       xk[i] = -CUDART_INF_F;
     }
+  }
+  __syncwarp();  // (list.c)
+}
+
+// ... and the sums over them, while the others go through the slice.
+__device__ __forceinline__ void weigh(const AiDistillArgs& a, List& list, Entries& mine) {
+  const int lane = threadIdx.x % 32, K = a.n_top;
+  const int(&word)[kSets] = mine.word;
+  float(&logp)[kSets] = mine.logp, (&xk)[kSets] = mine.x;
+  const float c = list.c, inv = mine.inv;
+  float p[kSets], top = -CUDART_INF_F, m = -CUDART_INF_F;
+#pragma unroll
+  for (int i = 0; i < kSets; ++i) {
+    p[i] = 0.f;
+    if (32 * i >= K) continue;
     if (word[i] >= 0) top = fmaxf(top, logp[i]);
     m = fmaxf(m, xk[i]);
   }
@@ -187,8 +209,7 @@ __device__ __forceinline__ void read_list(const AiDistillArgs& a, List& list, ui
   sum = warp_sum(sum);
   term = warp_sum(term);
   if (lane == 0) {
-    list.up = wgt * inv;
-    list.c = c;
+    list.up = mine.wgt * inv;
     list.inv = inv;
     list.p_top = p_top;
     list.p_rest = p_top != p_top ? p_top : renorm || 1.f - p_top < kLeastRest ? 0.f : 1.f - p_top;
@@ -319,12 +340,13 @@ __global__ void __launch_bounds__(kThreads, 6) distill_kernel(const AiDistillArg
   const int vecs = sl.i1 - sl.i0;
   // (a CTA of the cluster must run before its shared memory is written to)
   if (splits > 1) asm volatile("barrier.cluster.arrive;" ::: "memory");
+  Entries entries;  // (the first warp's)
   if (warp == 0) {
     if (lane == 0) {
       ptx::mbar_init(bar, 1);
       ptx::fence_mbar_init();
     }
-    read_list<T>(a, list, row, split == 0, [&](bool live) {
+    read_words<T>(a, list, entries, row, split == 0, [&](bool live) {
       if (lane == 0 && live && vecs > 0) {
         ptx::mbar_arrive_expect_tx(bar, 16u * vecs);
         ptx::bulk_load(ptx::smem_u32(smem), r.x + sl.head + (int64_t)sl.i0 * E, 16u * vecs, bar);
@@ -337,34 +359,40 @@ __global__ void __launch_bounds__(kThreads, 6) distill_kernel(const AiDistillArg
     if (r.d) zero_row(r.d, a.vocab, split, splits, kWidth, tid, kThreads);
     return;
   }
-  if (vecs > 0 && !ptx::mbar_wait(bar, 0, kWait)) {
-    report(a.status, AI_ERR_DEV_TIMEOUT);
-    ptx::mbar_wait(bar, 0, kWait);  // (the copy lands before the CTA ends)
-  }
-  // The listed words' places become -inf, which adds nothing to the others' sum.
-  if (warp == 0)
-    for (int k = lane; k < K; k += 32) {
-      const int w = list.word[k], at_ = w - sl.head - sl.i0 * E;
+  const uint4* held = reinterpret_cast<const uint4*>(smem);
+  const float c = list.c;
+  float2 mine = make_float2(-CUDART_INF_F, 0.f);
+  if (warp == 0) {
+    weigh(a, list, entries);
+  } else {
+    if (vecs > 0 && !ptx::mbar_wait(bar, 0, kWait)) {
+      report(a.status, AI_ERR_DEV_TIMEOUT);
+      ptx::mbar_wait(bar, 0, kWait);  // (the copy lands before the CTA ends)
+    }
+    // The listed words' places become -inf, which adds nothing to the others' sum.
+    constexpr int kSum = kThreads - 32;
+    const int id = tid - 32;
+    if (id < K) {
+      const int w = list.word[id], at_ = w - sl.head - sl.i0 * E;
       if (w >= 0 && at_ >= 0 && at_ < vecs * E) reinterpret_cast<T*>(smem)[at_] = from_f32<T>(-CUDART_INF_F);
     }
-  __syncthreads();
-  const uint4* held = reinterpret_cast<const uint4*>(smem);
-  const uint4 none = make_uint4(Vec<T>::kNone, Vec<T>::kNone, Vec<T>::kNone, Vec<T>::kNone);
-  const float c = list.c;
-  Part part{-CUDART_INF_F, 0.f, 0.f};
-  for (int i = tid; i < vecs; i += kThreads * U) {
-    uint4 raw[U];
+    asm volatile("bar.sync 1, %0;" ::"n"(kSum) : "memory");
+    const uint4 none = make_uint4(Vec<T>::kNone, Vec<T>::kNone, Vec<T>::kNone, Vec<T>::kNone);
+    Part part{-CUDART_INF_F, 0.f, 0.f};
+    for (int i = id; i < vecs; i += kSum * U) {
+      uint4 raw[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) raw[u] = i + u * kThreads < vecs ? held[i + u * kThreads] : none;
-    accumulate<T, U, false>(part, raw, c);
+      for (int u = 0; u < U; ++u) raw[u] = i + u * kSum < vecs ? held[i + u * kSum] : none;
+      accumulate<T, U, false>(part, raw, c);
+    }
+    ends<E>(sl, a.vocab, id, [&](int v) {
+      for (int j = 0; j < K; ++j)
+        if (list.word[j] == v) return;
+      add_end(part, at(r.x, v), c);
+    });
+    mine = join_lanes(make_float2(part.m, part.s), c);
   }
-  ends<E>(sl, a.vocab, tid, [&](int v) {
-    for (int j = 0; j < K; ++j)
-      if (list.word[j] == v) return;
-    add_end(part, at(r.x, v), c);
-  });
   // The warps' sums go to every CTA of the cluster; each joins them in the same order.
-  const float2 mine = join_lanes(make_float2(part.m, part.s), c);
   if (splits > 1) {
     const cg::cluster_group cluster = cg::this_cluster();
     asm volatile("barrier.cluster.wait;" ::: "memory");
