@@ -76,6 +76,7 @@ EXPORTED_SYMBOLS = (
     "ai_token_logprobs",
     "ai_token_logprobs_bwd",
     "ai_distill",
+    "ai_distill_bwd",
     "ai_paged_append_4bit",
     "ai_paged_read_4bit",
     "ai_paged_attn_4bit_workspace",
@@ -476,7 +477,18 @@ class AiDistillArgs(ctypes.Structure):
         ("dlogits", ctypes.c_void_p),
         ("dstride_b", ctypes.c_int64),
         ("dstride_t", ctypes.c_int64),
+        ("row_stats", ctypes.c_void_p),
         ("status", ctypes.c_void_p),
+    ]
+
+
+class AiDistillBwdArgs(ctypes.Structure):
+    _fields_ = [
+        ("fwd", AiDistillArgs),
+        ("g_losses", ctypes.c_void_p),
+        ("dlogits", ctypes.c_void_p),
+        ("dstride_b", ctypes.c_int64),
+        ("dstride_t", ctypes.c_int64),
     ]
 
 
@@ -588,6 +600,7 @@ def _bind(handle):
                        ("ai_paged_append", AiPagedAppendArgs), ("ai_prefix_attn", AiPrefixAttnArgs),
                        ("ai_verify_draft", AiVerifyArgs), ("ai_token_logprobs", AiScoreArgs),
                        ("ai_token_logprobs_bwd", AiScoreBwdArgs), ("ai_distill", AiDistillArgs),
+                       ("ai_distill_bwd", AiDistillBwdArgs),
                        ("ai_paged_append_4bit", AiPaged4Args), ("ai_paged_read_4bit", AiPaged4Args),
                        ("ai_paged_attn_4bit", AiPagedAttn4Args)):
         fn = getattr(handle, name)

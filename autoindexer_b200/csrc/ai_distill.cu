@@ -16,9 +16,10 @@
 // then need no look at the list; one warp gathers the list's own sums meanwhile), the
 // sums exchanged through distributed shared memory.
 //
-// Measured: 4096 rows of 151,936 bf16, most with lists of 32, losses and gradients, 537 us
-// (4.4 TB/s); 1023 of 32,003 fp16 with lists of 64, the losses in one call and the
-// gradients in another, 70 us; 16 of 151,936 8.0 us.  Between
+// Measured: 4096 rows of 151,936 bf16, most with lists of 32, losses and gradients, 542 us
+// (4.3 TB/s); 16 of 151,936 8.0 us; 1023 of 32,003 fp16 with lists of 64, the losses
+// in one launch and the gradients, from the rows' totals, in another, 55 us (70 when
+// the second one summed again).  Between
 // it and the memory's 365 us stand the instructions (issued in 56% of the cycles; two
 // exponentials a logit keep the SFU busy for 58%) and the phases of a slice, which
 // the CTAs of an SM overlap as much as their shared memory holds.  Slices of 20
@@ -65,6 +66,7 @@ struct List {
   float c, inv;        // log2(e) / tau, 1 / tau
   float p_top, p_rest; // the teacher's probability on the listed words, and beside them
   float m, s;          // the student's logits there: the largest, and the sum of 2^((x - m) c)
+  float norm;          // what the teacher's log-probabilities are taken less
   float term;          // sum p (ln p - (x - m) / tau)
   int word[kMaxTop];   // -1: left out
   float x[kMaxTop];    // the student's logits
@@ -86,6 +88,14 @@ __device__ __forceinline__ float warp_max(float v) {
 __device__ __forceinline__ float share(float x, float c, float m) {
   return x == -CUDART_INF_F ? 0.f : ptx::ex2((x - m) * c);
 }
+
+// What a backward of its own needs of a row.
+struct __align__(16) RowStats {
+  float m, base;       // of the words that are not listed
+  float m_all, s_all;  // of all
+  float mass, norm;
+  float live, unused;
+};
 
 // A row of the call.
 template <typename T>
@@ -182,13 +192,14 @@ __device__ __forceinline__ void weigh(const AiDistillArgs& a, List& list, Entrie
     m = fmaxf(m, xk[i]);
   }
   const bool renorm = a.tail == AI_TAIL_RENORMALIZE;
+  float norm = 0.f;
   if (renorm) {
     top = warp_max(top);
     float sum = 0.f;
 #pragma unroll
     for (int i = 0; i < kSets; ++i)
       if (32 * i < K) sum += word[i] >= 0 ? expf(logp[i] - top) : 0.f;
-    const float norm = top + logf(warp_sum(sum));
+    norm = top + logf(warp_sum(sum));
 #pragma unroll
     for (int i = 0; i < kSets; ++i) logp[i] -= norm;
   }
@@ -215,9 +226,13 @@ __device__ __forceinline__ void weigh(const AiDistillArgs& a, List& list, Entrie
     list.p_rest = p_top != p_top ? p_top : renorm || 1.f - p_top < kLeastRest ? 0.f : 1.f - p_top;
     list.m = m;
     list.s = sum;
+    list.norm = norm;
     list.term = term;
   }
 }
+
+// Gradient of a listed word with the student's share q and the teacher's p.
+__device__ __forceinline__ float listed_gradient(float up, float mass, float q, float p) { return up * (mass * q - p); }
 
 // A warp's sum of the parts (m, s) of its lanes, with respect to their largest m.
 __device__ __forceinline__ float2 join_lanes(float2 q, float c) {
@@ -265,9 +280,11 @@ struct Totals {
     if (p_rest != 0.f) r += p_rest * (logf(p_rest) - (log2f(s) - l2) * kLn2) - p_rest * list.inv * (m - m_all);
     return empty ? CUDART_INF_F : r;
   }
+  // What the gradients of the others have in common, but for the weight.
+  __device__ __forceinline__ float base(const List& list) const { return s == 0.f ? 0.f : mass * of_rest(list) / s_all - p_rest / s; }
   // Gradient of listed entry k.
   __device__ __forceinline__ float listed(const List& list, int k) const {
-    return empty ? 0.f : list.up * (mass * (share(list.x[k], list.c, m_all) / s_all) - list.p[k]);
+    return empty ? 0.f : listed_gradient(list.up, mass, share(list.x[k], list.c, m_all) / s_all, list.p[k]);
   }
 };
 
@@ -275,11 +292,10 @@ struct Totals {
 // listed ones come out as anything and are written over.)
 struct Dense {
   float m, c, coef;
-  Dense() = default;
-  __device__ __forceinline__ Dense(const List& list, const Totals& t) {
-    m = t.m == -CUDART_INF_F ? 0.f : t.m;
-    c = list.c;
-    coef = t.s == 0.f ? 0.f : list.up * (t.mass * t.of_rest(list) / t.s_all - t.p_rest / t.s);
+  __device__ __forceinline__ Dense(float largest, float slope, float up, float base) {
+    m = largest == -CUDART_INF_F ? 0.f : largest;
+    c = slope;
+    coef = base == 0.f ? 0.f : up * base;
   }
   __device__ __forceinline__ float one(float x) const { return ptx::ex2((x - m) * c) * coef; }
   template <typename T>
@@ -355,7 +371,10 @@ __global__ void __launch_bounds__(kThreads, 6) distill_kernel(const AiDistillArg
   }
   __syncthreads();
   if (!list.live) {
-    if (split == 0 && tid == 0 && a.losses) a.losses[row] = 0.f;
+    if (split == 0 && tid == 0) {
+      if (a.losses) a.losses[row] = 0.f;
+      if (a.row_stats) *reinterpret_cast<RowStats*>(a.row_stats + 8 * (int64_t)row) = RowStats{};
+    }
     if (r.d) zero_row(r.d, a.vocab, split, splits, kWidth, tid, kThreads);
     return;
   }
@@ -408,9 +427,14 @@ __global__ void __launch_bounds__(kThreads, 6) distill_kernel(const AiDistillArg
     rest = make_float2(q.m, q.s);
   }
   const Totals all(list, join_lanes(rest, c));
-  if (split == 0 && tid == 0 && a.losses) a.losses[row] = all.loss(list);
+  if (split == 0 && tid == 0) {
+    if (a.losses) a.losses[row] = all.loss(list);
+    if (a.row_stats)
+      *reinterpret_cast<RowStats*>(a.row_stats + 8 * (int64_t)row) =
+          RowStats{all.m, all.base(list), all.m_all, all.s_all, all.mass, list.norm, 1.f, 0.f};
+  }
   if (!r.d) return;
-  const Dense dense(list, all);
+  const Dense dense(all.m, c, list.up, all.base(list));
   const bool alike = lie_alike(r.x, r.d);
 #pragma unroll 2
   for (int i = tid; i < vecs; i += kThreads) put(r.d, sl.head + (sl.i0 + i) * E, dense.template vector<T>(held[i]), alike);
@@ -422,6 +446,69 @@ __global__ void __launch_bounds__(kThreads, 6) distill_kernel(const AiDistillArg
   }
 }
 
+// The gradient alone, from the rows' totals: a CTA per (row, slice).  One read and one
+// write of the row, bound by them.
+template <typename T>
+__global__ void __launch_bounds__(kThreads, 4) distill_bwd_kernel(const AiDistillBwdArgs g, const int splits) {
+  constexpr int E = 16 / sizeof(T), N = 4;  // vectors of a thread in flight
+  const AiDistillArgs& a = g.fwd;
+  __shared__ int s_word[kMaxTop];
+  const int tid = threadIdx.x, K = a.n_top;
+  const uint32_t row = blockIdx.x / (uint32_t)splits;
+  const int split = (int)(blockIdx.x - row * splits);
+  const Row<T> r(a, row);
+  const int64_t t = row - r.b * (uint32_t)a.seq_len;
+  T* d = static_cast<T*>(g.dlogits) + r.b * g.dstride_b + t * g.dstride_t;
+  const float wgt = __ldg(g.g_losses + row);
+  const RowStats st = *reinterpret_cast<const RowStats*>(a.row_stats + 8 * (int64_t)row);
+  const float tau = row_tau(a.temperature, r.b, nullptr);
+  if (wgt == 0.f || st.live == 0.f) {
+    zero_row(d, a.vocab, split, splits, kThreads, tid, kThreads);
+    return;
+  }
+  const Slice sl = slice_of(r.x, a.vocab, split, splits, kThreads);
+  const uint4* xv = reinterpret_cast<const uint4*>(r.x + sl.head);
+  uint4 next[N];
+  auto load = [&](int i) {
+#pragma unroll
+    for (int u = 0; u < N; ++u)
+      if (i + u * kThreads < sl.i1) next[u] = __ldcs(xv + i + u * kThreads);
+  };
+  load(sl.i0 + tid);
+  // The thread's entry of the list: of its words in the slice the first.
+  int word = -1;
+  float p = 0.f, x = 0.f;
+  if (tid < K) {
+    const long long w = a.top_tokens[(int64_t)row * K + tid];
+    const float logp = a.top_logprobs[(int64_t)row * K + tid];
+    if (w >= sl.e0 && w < sl.e1 && logp != -CUDART_INF_F) {
+      word = (int)w;
+      x = at(r.x, word);
+      p = expf(logp - st.norm);
+    }
+    s_word[tid] = word;
+  }
+  const float c = slope(tau), up = wgt * inverse(tau);
+  const Dense dense(st.m, c, up, st.base);
+  const bool alike = lie_alike(r.x, d);
+  for (int i = sl.i0 + tid; i < sl.i1; i += kThreads * N) {
+    uint4 raw[N];
+#pragma unroll
+    for (int u = 0; u < N; ++u) raw[u] = next[u];
+    load(i + kThreads * N);
+#pragma unroll
+    for (int u = 0; u < N; ++u)
+      if (i + u * kThreads < sl.i1) put(d, sl.head + (i + u * kThreads) * E, dense.template vector<T>(raw[u]), alike);
+  }
+  ends<E>(sl, a.vocab, tid, [&](int v) { d[v] = from_f32<T>(dense.one(at(r.x, v))); });
+  __syncthreads();
+  if (word >= 0) {
+    for (int j = 0; j < tid; ++j)
+      if (s_word[j] == word) return;
+    d[word] = from_f32<T>(st.s_all == 0.f ? 0.f : listed_gradient(up, st.mass, share(x, c, st.m_all) / st.s_all, p));
+  }
+}
+
 int check(const AiDistillArgs* a) {
   if (!a) return AI_ERR_NULL;
   if (a->batch <= 0 || a->seq_len <= 0 || a->vocab <= 0 || a->vocab > 0x40000000 || a->n_top <= 0 || a->n_top > kMaxTop)
@@ -429,12 +516,13 @@ int check(const AiDistillArgs* a) {
   if ((int64_t)a->batch * a->seq_len > 0x7fffffff / kMaxSplit) return AI_ERR_SHAPE;
   if (a->tail != AI_TAIL_BUCKET && a->tail != AI_TAIL_RENORMALIZE) return AI_ERR_SHAPE;
   if (a->dtype != AI_DTYPE_BF16 && a->dtype != AI_DTYPE_F16 && a->dtype != AI_DTYPE_F32) return AI_ERR_DTYPE;
-  if (!a->logits || !a->top_tokens || !a->top_logprobs || (!a->losses && !a->dlogits)) return AI_ERR_NULL;
+  if (!a->logits || !a->top_tokens || !a->top_logprobs) return AI_ERR_NULL;
   if (a->stride_b < 0 || a->stride_t < 0 || a->dstride_b < 0 || a->dstride_t < 0) return AI_ERR_STRIDE;
   if ((int64_t)a->vocab * (a->dtype == AI_DTYPE_F32 ? 4 : 2) > AI_DISTILL_MAX_ROW_BYTES) return AI_ERR_SHAPE;
   if ((reinterpret_cast<uintptr_t>(a->logits) | reinterpret_cast<uintptr_t>(a->dlogits)) &
       (a->dtype == AI_DTYPE_F32 ? 3 : 1))
     return AI_ERR_ALIGN;
+  if (reinterpret_cast<uintptr_t>(a->row_stats) & 15) return AI_ERR_ALIGN;
   return AI_OK;
 }
 
@@ -484,14 +572,40 @@ int launch(const AiDistillArgs& a, cudaStream_t st) {
   return cudaGetLastError() == cudaSuccess ? AI_OK : AI_ERR_LAUNCH;
 }
 
+template <typename T>
+int launch_bwd(const AiDistillBwdArgs& g, cudaStream_t st) {
+  // Slices of a row: CTAs for four per SM, at least 16 KB each.
+  const int64_t rows = (int64_t)g.fwd.batch * g.fwd.seq_len, bytes = (int64_t)g.fwd.vocab * (int)sizeof(T);
+  int splits = 1;
+  while (2 * splits <= kMaxSplit && 2 * splits * rows <= 4 * (int64_t)sm_count() && splits * (int64_t)kLeast < bytes) splits *= 2;
+  ProfScope ps(AI_PROF_DISTILL, st);
+  distill_bwd_kernel<T><<<(unsigned)(rows * splits), kThreads, 0, st>>>(g, splits);
+  return cudaGetLastError() == cudaSuccess ? AI_OK : AI_ERR_LAUNCH;
+}
+
 }  // namespace distill
 }  // namespace ai
 
 extern "C" int ai_distill(const AiDistillArgs* args, void* stream) {
   const int rc = ai::distill::check(args);
   if (rc != AI_OK) return rc;
+  if (!args->losses && !args->dlogits) return AI_ERR_NULL;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (args->dtype == AI_DTYPE_BF16) return ai::distill::launch<__nv_bfloat16>(*args, st);
   if (args->dtype == AI_DTYPE_F16) return ai::distill::launch<__half>(*args, st);
   return ai::distill::launch<float>(*args, st);
+}
+
+extern "C" int ai_distill_bwd(const AiDistillBwdArgs* args, void* stream) {
+  if (!args) return AI_ERR_NULL;
+  const AiDistillArgs& a = args->fwd;
+  const int rc = ai::distill::check(&a);
+  if (rc != AI_OK) return rc;
+  if (!args->dlogits || !args->g_losses || !a.row_stats) return AI_ERR_NULL;
+  if (args->dstride_b < 0 || args->dstride_t < 0) return AI_ERR_STRIDE;
+  if (reinterpret_cast<uintptr_t>(args->dlogits) & (a.dtype == AI_DTYPE_F32 ? 3 : 1)) return AI_ERR_ALIGN;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (a.dtype == AI_DTYPE_BF16) return ai::distill::launch_bwd<__nv_bfloat16>(*args, st);
+  if (a.dtype == AI_DTYPE_F16) return ai::distill::launch_bwd<__half>(*args, st);
+  return ai::distill::launch_bwd<float>(*args, st);
 }

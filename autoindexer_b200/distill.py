@@ -80,27 +80,36 @@ def _losses(logits: Tensor) -> Tensor:
 
 
 class DistillFn(torch.autograd.Function):
-    """Autograd wrapper: saves the inputs; the backward is the same launch with
-    the upstream gradients as weights."""
+    """Autograd wrapper: saves the inputs and eight numbers a row; backward is
+    ``ai_distill_bwd``."""
 
     @staticmethod
     def forward(ctx, logits, ids, logprobs, temperature, plan):
-        ctx.save_for_backward(logits, ids, logprobs, temperature)
+        a, losses = _call.copy(plan), _losses(logits)
+        stats = torch.empty((losses.numel(), 8), dtype=torch.float32, device=logits.device)
+        a.row_stats = stats.data_ptr()
+        _run(a, (logits, ids, logprobs, None, temperature), losses, None)
+        ctx.save_for_backward(logits, ids, logprobs, temperature, stats)
         ctx.plan = plan
-        losses = _losses(logits)
-        _run(_call.copy(plan), (logits, ids, logprobs, None, temperature), losses, None)
         return losses
 
     @staticmethod
     @once_differentiable
     def backward(ctx, g):
         # (hooks on saved tensors may have brought back copies of other strides)
-        logits, ids, logprobs, temperature = ctx.saved_tensors
-        logits = _call.dense_d(logits)
+        logits, ids, logprobs, temperature, stats = ctx.saved_tensors
+        logits, ids, logprobs, stats, g = _call.dense_d(logits), ids.contiguous(), logprobs.contiguous(), stats.contiguous(), g.contiguous()
+        a = _lib.AiDistillBwdArgs()
+        a.fwd = ctx.plan
+        point_rows(a.fwd, logits)
+        a.fwd.top_tokens, a.fwd.top_logprobs, a.fwd.row_stats = ids.data_ptr(), logprobs.data_ptr(), stats.data_ptr()
         if temperature is not None:
             temperature = temperature.contiguous()
+            a.fwd.temperature = temperature.data_ptr()
         grad = empty_rows(logits)
-        _run(_call.copy(ctx.plan), (logits, ids.contiguous(), logprobs.contiguous(), g.contiguous(), temperature), None, grad)
+        sd = grad.stride()
+        a.g_losses, a.dlogits, a.dstride_b, a.dstride_t = g.data_ptr(), grad.data_ptr(), sd[0], sd[1] if len(sd) == 3 else 0
+        _call.launch(_lib.lib().ai_distill_bwd, a, logits.get_device(), "ai_distill_bwd")
         return grad, None, None, None, None
 
 

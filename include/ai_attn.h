@@ -719,10 +719,23 @@ typedef struct AiDistillArgs {
   float* losses;              /* [B][T], without the weight; or NULL */
   void* dlogits;              /* (B, T, V) of the logits' type, or NULL: losses alone */
   int64_t dstride_b, dstride_t;
+  float* row_stats;           /* [B][T][8], 16-B aligned: what ai_distill_bwd needs; or NULL */
   int32_t* status;
 } AiDistillArgs;
 
+/* The gradient alone, with the losses' upstream gradients as weights: what ai_distill
+ * with `weights` gives.  fwd has the inputs of an ai_distill call without weights,
+ * whose row_stats are read; its outputs and weights are not, and dlogits may not be
+ * the logits' memory. */
+typedef struct AiDistillBwdArgs {
+  AiDistillArgs fwd;
+  const float* g_losses;      /* [B][T] */
+  void* dlogits;              /* (B, T, V) of the logits' type */
+  int64_t dstride_b, dstride_t;
+} AiDistillBwdArgs;
+
 int ai_distill(const AiDistillArgs* args, void* stream);
+int ai_distill_bwd(const AiDistillBwdArgs* args, void* stream);
 
 /* A paged cache held in 4 bits.  Of a head row of D dims, the 32 dims of a
  * group share an fp16 scale d, minus an eighth of their value of largest

@@ -313,6 +313,36 @@ def test_captured_graph_and_another_stream(shape, V, cuda_device):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("tail", TAILS)
+@pytest.mark.parametrize("shape,V,dtype", [((5,), 7, torch.float32), ((3, 2), 1003, torch.float16), ((2,), 150001, torch.bfloat16),
+                                           ((700,), 515, torch.float32)])
+def test_backward_of_its_own(shape, V, dtype, tail, cuda_device):
+    """Upstream gradients of either sign, zero and NaN; saved tensors that hooks bring
+    back with other strides; lists with a word twice and words that are masked."""
+    from autoindexer_b200 import distill_loss, distill_loss_and_grad, read_status
+
+    x, ids, t, w, tau = (y.to(cuda_device) for y in make(shape, V, 5, dtype, 21))
+    ids.view(-1, 5)[0, 3] = ids.view(-1, 5)[0, 1]
+    x.view(-1, V)[-2, int(ids.view(-1, 5)[-2, 0].clamp_min(0))] = -INF
+    x.view(-1, V)[0, V // 2:] = -INF
+    w.view(-1)[0] *= -1
+    want = distill_loss_and_grad(x, ids, t, w, tau, tail)
+    check(x, ids, t, w, tau, tail, None, want[1])
+    y = x.clone().requires_grad_()
+    wide = lambda z: torch.stack((z, z), -1)[..., 0]  # noqa: E731
+    with torch.autograd.graph.saved_tensors_hooks(lambda z: z, wide):
+        loss = distill_loss(y, ids, t, tau, tail)
+    assert torch.equal(torch.autograd.grad(loss, y, wide(w), retain_graph=True)[0], want[1])
+    plain = distill_loss(y, ids, t, tau, tail)
+    assert torch.equal(torch.autograd.grad(plain, y, w)[0], want[1])
+    read_status(cuda_device)  # (the word twice)
+    nan = torch.full(shape, float("nan"), device=cuda_device)
+    d = torch.autograd.grad(loss, y, nan)[0].reshape(-1, V)
+    live = (ids.view(-1, 5) >= 0).any(1)
+    assert bool(d[live].isnan().any(1).all()) and not bool(d[~live].any())
+
+
+@pytest.mark.gpu
 def test_gradients_that_do_not_exist(cuda_device):
     from autoindexer_b200 import distill_loss, distill_loss_and_grad
 
@@ -390,6 +420,26 @@ def test_c_abi_refusals():
                                ("batch", 2 ** 30, 2), ("vocab", 2 ** 21, 2), ("logits", None, 1), ("top_tokens", None, 1), ("top_logprobs", None, 1),
                                ("losses", None, 1), ("stride_b", -1, 5), ("dstride_t", -1, 5), ("logits", 257, 6), ("dlogits", 255, 6)):
         assert L.ai_distill(args(**{field: value}), None) == code, field
+
+
+def test_c_abi_refusals_of_the_backward():
+    from autoindexer_b200 import _lib
+
+    L = _lib.lib()
+    assert L.ai_distill_bwd(None, None) == 1
+
+    def args(**over):
+        g = _lib.AiDistillBwdArgs()
+        a = g.fwd
+        a.batch, a.seq_len, a.vocab, a.dtype, a.n_top = 2, 3, 100, _lib.DTYPE_BF16, 4
+        a.logits = a.top_tokens = a.top_logprobs = a.row_stats = g.g_losses = g.dlogits = 256
+        for n, v in over.items():
+            setattr(a if n in ("vocab", "row_stats", "top_tokens") else g, n, v)
+        return ctypes.byref(g)
+
+    for field, value, code in (("vocab", 0, 2), ("row_stats", None, 1), ("row_stats", 264, 6), ("top_tokens", None, 1), ("g_losses", None, 1),
+                               ("dlogits", None, 1), ("dlogits", 255, 6), ("dstride_b", -1, 5), ("dstride_t", -1, 5)):
+        assert L.ai_distill_bwd(args(**{field: value}), None) == code, field
 
 
 @pytest.mark.parametrize("tail", TAILS)
