@@ -13,7 +13,7 @@
 // half of d the candidate moves.
 //
 // Measured, for an append and a read of what it wrote (8 KV heads of 128): 64
-// sequences by a token 5.5 us, two launches' latency; 8 by up to 2047 tokens of fp16
+// sequences by a token 5.3 us, two launches' latency; 8 by up to 2047 tokens of fp16
 // 29 us for 115 MB (4 TB/s): about 200 instructions per lane and 32 dims, the two
 // extremes and the checks for what is no number before all, share the time with memory.
 
@@ -170,22 +170,26 @@ __device__ __forceinline__ Item item_of(const AiPaged4Args& a, uint32_t it, int 
   return r;
 }
 
-// A lane's sixteen dims of head h of K or V: in the tensor, its codes, its scale.
+// Head h of an item's token in K or V.
+template <typename T>
+__device__ __forceinline__ T* row(const AiTensor4& x, const Item& i, int64_t h) {
+  return static_cast<T*>(const_cast<void*>(x.ptr)) + i.b * x.stride_b + h * x.stride_h + i.t * x.stride_t;
+}
+
+// Where a lane's sixteen dims of head h lie in a pool: their codes, their scale.
 // (Dims 16 l + 4 i + j: group l / 2, byte pairs 4 (l % 2) + i.)
-template <typename T, int D>
+template <int D>
 struct Spot {
   static constexpr int C = D / kGroup;
-  T* x;
   uint8_t* codes;
   __half* scale;
-  __device__ __forceinline__ Spot(const AiTensor4& tx, const AiTensor4& tc, const AiTensor4& ts, const Item& i, const Place& p, int64_t h, int l) {
-    x = static_cast<T*>(const_cast<void*>(tx.ptr)) + i.b * tx.stride_b + h * tx.stride_h + i.t * tx.stride_t + kDims * l;
+  __device__ __forceinline__ Spot(const AiTensor4& tc, const AiTensor4& ts, const Place& p, int64_t h, int l) {
     codes = static_cast<uint8_t*>(const_cast<void*>(tc.ptr)) + p.page * tc.stride_b + h * tc.stride_h + p.slot * (D / 2) +
             (l % 2 * 4) * 2 * C + l / 2 * 2;
     scale = static_cast<__half*>(const_cast<void*>(ts.ptr)) + p.page * ts.stride_b + h * ts.stride_h + p.slot * C + l / 2;
   }
-  __device__ __forceinline__ void advance(const AiTensor4& tx, const AiTensor4& tc, const AiTensor4& ts, int heads) {
-    x += heads * tx.stride_h, codes += heads * tc.stride_h, scale += heads * ts.stride_h;
+  __device__ __forceinline__ void advance(const AiTensor4& tc, const AiTensor4& ts, int heads) {
+    codes += heads * tc.stride_h, scale += heads * ts.stride_h;
   }
 };
 
@@ -197,19 +201,27 @@ __global__ void __launch_bounds__(kThreads) append_kernel(const AiPaged4Args a, 
   const uint32_t it = blockIdx.x * kWarps + threadIdx.x / 32;
   if (it >= items) return;
   const Item i = item_of(a, it, per, chunks);
+  const int len = __ldg(a.lens + i.b);
   if (i.t >= new_tokens(a.n, i.b, a.seq_len, a.status)) return;
-  const Place p = place(a.pool, i.b, (int64_t)__ldg(a.lens + i.b) + i.t);
+  // (the first turn's loads do not wait for the page, nor a turn's for the one before)
+  int h = i.h0 + sub;
+  const T* x[2] = {row<T>(a.k, i, h) + kDims * l, row<T>(a.v, i, h) + kDims * l};
+  Raw<T> next[2] = {};
+#pragma unroll
+  for (int u = 0; u < 2; ++u)
+    if (h < i.h1) next[u] = load<T, kAlign>(x[u]);
+  const Place p = place(a.pool, i.b, (int64_t)len + i.t);
   if (p.page < 0) {
     report(a.status, AI_ERR_DEV_BOUNDS);
     return;
   }
-  int h = i.h0 + sub;
-  Spot<T, D> at[2] = {{a.k, a.pool.k_codes, a.pool.k_scales, i, p, h, l}, {a.v, a.pool.v_codes, a.pool.v_scales, i, p, h, l}};
+  Spot<D> at[2] = {{a.pool.k_codes, a.pool.k_scales, p, h, l}, {a.pool.v_codes, a.pool.v_scales, p, h, l}};
   for (int h0 = i.h0; h0 < i.h1; h0 += R, h += R) {
-    Raw<T> raw[2] = {};
+    Raw<T> raw[2] = {next[0], next[1]};
+    x[0] += R * a.k.stride_h, x[1] += R * a.v.stride_h;
 #pragma unroll
     for (int u = 0; u < 2; ++u)
-      if (h < i.h1) raw[u] = load<T, kAlign>(at[u].x);
+      if (h + R < i.h1) next[u] = load<T, kAlign>(x[u]);
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       uint16_t codes[4];
@@ -221,8 +233,8 @@ __global__ void __launch_bounds__(kThreads) append_kernel(const AiPaged4Args a, 
         if (l % 2 == 0) *at[u].scale = scale;
       }
     }
-    at[0].advance(a.k, a.pool.k_codes, a.pool.k_scales, R);
-    at[1].advance(a.v, a.pool.v_codes, a.pool.v_scales, R);
+    at[0].advance(a.pool.k_codes, a.pool.k_scales, R);
+    at[1].advance(a.pool.v_codes, a.pool.v_scales, R);
   }
 }
 
@@ -234,13 +246,15 @@ __global__ void __launch_bounds__(kThreads) read_kernel(const AiPaged4Args a, co
   if (it >= items) return;
   const Item i = item_of(a, it, per, chunks);
   Place p{-1, 0};
+  const int len = __ldg(a.lens + i.b);
   if (i.t < new_tokens(a.n, i.b, a.seq_len, a.status)) {
-    p = place(a.pool, i.b, (int64_t)__ldg(a.lens + i.b) + i.t);
+    p = place(a.pool, i.b, (int64_t)len + i.t);
     if (p.page < 0) report(a.status, AI_ERR_DEV_BOUNDS);
   }
   const bool held = p.page >= 0;
   p.page = max(p.page, 0);
-  Spot<T, D> at[2] = {{a.k, a.pool.k_codes, a.pool.k_scales, i, p, i.h0 + sub, l}, {a.v, a.pool.v_codes, a.pool.v_scales, i, p, i.h0 + sub, l}};
+  T* x[2] = {row<T>(a.k, i, i.h0 + sub) + kDims * l, row<T>(a.v, i, i.h0 + sub) + kDims * l};
+  Spot<D> at[2] = {{a.pool.k_codes, a.pool.k_scales, p, i.h0 + sub, l}, {a.pool.v_codes, a.pool.v_scales, p, i.h0 + sub, l}};
   for (int h = i.h0 + sub; h < i.h1; h += R) {
     if (held) {
       uint16_t codes[2][4];
@@ -252,13 +266,14 @@ __global__ void __launch_bounds__(kThreads) read_kernel(const AiPaged4Args a, co
         scale[u] = *at[u].scale;
       }
 #pragma unroll
-      for (int u = 0; u < 2; ++u) store<T, kAlign>(at[u].x, values<T>(codes[u], scale[u]));
+      for (int u = 0; u < 2; ++u) store<T, kAlign>(x[u], values<T>(codes[u], scale[u]));
     } else {
-      store<T, kAlign>(at[0].x, Raw<T>{});
-      store<T, kAlign>(at[1].x, Raw<T>{});
+      store<T, kAlign>(x[0], Raw<T>{});
+      store<T, kAlign>(x[1], Raw<T>{});
     }
-    at[0].advance(a.k, a.pool.k_codes, a.pool.k_scales, R);
-    at[1].advance(a.v, a.pool.v_codes, a.pool.v_scales, R);
+    x[0] += R * a.k.stride_h, x[1] += R * a.v.stride_h;
+    at[0].advance(a.pool.k_codes, a.pool.k_scales, R);
+    at[1].advance(a.pool.v_codes, a.pool.v_scales, R);
   }
 }
 

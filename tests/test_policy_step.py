@@ -137,3 +137,46 @@ def test_gradient_of_the_objective(cuda_device):
 
     slope = (f(x.double() + step * way) - f(x.double() - step * way)) / (2 * step)
     assert abs(slope - float((got * way).sum())) <= 1e-4 * (1 + abs(slope))
+
+
+@pytest.mark.gpu
+def test_streams_at_once_and_graphs_that_share_memory(cuda_device):
+    """The same calls on two streams that overlap, and in two graphs of one memory pool
+    replayed in turns, give what they give alone."""
+    import autoindexer_b200 as ab
+
+    def inputs(seed, lens):
+        cache, table = test_paged4.filled(len(lens), 2, 64, 16, lens, torch.bfloat16, seed, cuda_device)
+        q = test_paged4.heads(len(lens), 8, 1, 64, torch.bfloat16, seed, cuda_device)
+        x, ids, t, w, tau = (y.to(cuda_device) for y in test_distill.make((40,), 5003, 6, torch.bfloat16, seed))
+        return q, cache, table, test_paged4.ints(lens, cuda_device), x, ids, t, w, tau
+
+    def step(q, cache, table, lens, x, ids, t, w, tau):
+        score = ab.token_logprobs(x, ids[:, 0].clamp_min(0), tau, top_k=6, entropy=True)
+        return [ab.paged_attention_4bit(q, *cache, table, lens), *score, *ab.distill_loss_and_grad(x, ids, t, w, tau)]
+
+    both = [inputs(1, [700, 33, 1500]), inputs(2, [5, 2049, 64, 900])]
+    want = [step(*given) for given in both]
+    torch.cuda.synchronize(cuda_device)
+    streams = [torch.cuda.Stream(cuda_device) for _ in both]
+    got = [[], []]
+    for _ in range(20):
+        for i, stream in enumerate(streams):
+            with torch.cuda.stream(stream):
+                got[i].append(step(*both[i]))
+    torch.cuda.synchronize(cuda_device)
+    for i in range(2):
+        assert all(torch.equal(a, b) for out in got[i] for a, b in zip(out, want[i]))
+    del got
+    graphs, outs = [torch.cuda.CUDAGraph() for _ in both], []
+    for i, graph in enumerate(graphs):
+        with torch.cuda.graph(graph, pool=graphs[0].pool() if i else None):
+            outs.append(step(*both[i]))
+    for i in (0, 1, 1, 0):
+        graphs[i].replay()
+        torch.cuda.synchronize(cuda_device)
+        assert all(torch.equal(a, b) for a, b in zip(outs[i], want[i]))
+    del outs
+    for graph in graphs:
+        graph.reset()
+    assert ab.read_status(cuda_device) == 0
