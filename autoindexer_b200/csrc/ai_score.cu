@@ -23,8 +23,9 @@
 // Measured: 4096 rows of 151,936 bf16 with entropies, 3592 of them with a token,
 // forward 188 us (5.8 TB/s), backward 366 us (6.4 TB/s): at the memory's rate.  509
 // rows of fp32 with the 32 likeliest 66 us (4.6 TB/s; less than four CTAs per SM, the
-// last of which find the memory idle).  8 rows of bf16 with the 20 likeliest 14 us:
-// latency, of which the list is 6 us.
+// last of which find the memory idle).  8 rows of bf16 5.1 us, with the 20 likeliest
+// 12.5 us, with 128 21 us: latency of the list's steps (its bound 1.5 us, the pieces
+// above it 2 to 4, the slices' lists into one 3 to 5).
 
 #include <cooperative_groups.h>
 #include <cuda_runtime.h>
@@ -47,6 +48,7 @@ constexpr int kThreads = 256, kWarps = kThreads / 32, U = 4;
 constexpr int kMaxTop = AI_SCORE_MAX_TOP, kRoom = 2048;
 constexpr int kMaxSplit = 16;  // CTAs of a cluster
 constexpr int kLeast = 8192;   // logits of a slice, at least (half for fp32)
+constexpr int kWidth = 8;      // slices are whole groups of so many vectors
 static_assert(kMaxSplit * kMaxTop <= kRoom && kMaxTop <= kThreads, "the parts' lists fit the buffer");
 
 using Key = unsigned long long;
@@ -74,6 +76,7 @@ struct TopSmem {
   Key room[kRoom];            // candidates
   Key best[kMaxTop];          // the slice's list
   uint32_t pieces[kPieces];   // order of the largest logit of each piece
+  int counts[2][kWarps];
   int n;
 };
 
@@ -105,20 +108,39 @@ __device__ void select(TopSmem& sm, int n, int k) {
       if (rank < k) sm.best[rank] = mine;
     }
   } else {
-    int size = 2 * kThreads;
-    while (size < n) size *= 2;
-    for (int j = n + tid; j < size; j += kThreads) sm.room[j] = 0;
+    // The k-th largest, bit by bit (keys differ), then the k entries that reach it.
+    constexpr int N = kRoom / kThreads;
+    Key held[N];
+#pragma unroll
+    for (int q = 0; q < N; ++q) held[q] = q * kThreads + tid < n ? sm.room[q * kThreads + tid] : 0;
+    Key bound = 0;
+    for (int bit = 63, turn = 0; bit >= 0; --bit, turn ^= 1) {
+      const Key next = bound | (Key)1 << bit;
+      int c = 0;
+#pragma unroll
+      for (int q = 0; q < N; ++q) c += held[q] >= next;
+      c = __reduce_add_sync(0xffffffffu, c);
+      if (tid % 32 == 0) sm.counts[turn][tid / 32] = c;
+      __syncthreads();
+      c = 0;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) c += sm.counts[turn][w];
+      if (c >= k) bound = next;
+      if (c == k) break;
+    }
+    if (tid == 0) sm.n = 0;
     __syncthreads();
-    for (int run = 2; run <= size; run *= 2)
-      for (int gap = run / 2; gap > 0; gap /= 2) {
-        for (int i = tid; i < size / 2; i += kThreads) {
-          const int lo = 2 * i - (i & (gap - 1)), hi = lo + gap;
-          const Key a = sm.room[lo], b = sm.room[hi];
-          if ((a < b) == ((lo & run) == 0)) sm.room[lo] = b, sm.room[hi] = a;
-        }
-        __syncthreads();
-      }
-    for (int j = tid; j < k; j += kThreads) sm.best[j] = sm.room[j];
+#pragma unroll
+    for (int q = 0; q < N; ++q)
+      if (held[q] >= bound) sm.room[atomicAdd(&sm.n, 1)] = held[q];
+    __syncthreads();
+    if (tid < k) {
+      const Key mine = sm.room[tid];
+      int rank = 0;
+#pragma unroll 8
+      for (int j = 0; j < k; ++j) rank += sm.room[j] > mine;
+      sm.best[rank] = mine;
+    }
   }
   __syncthreads();
 }
@@ -223,7 +245,7 @@ __global__ void __launch_bounds__(kThreads, 4) score_kernel(const AiScoreArgs a,
   const int k = kTop ? a.top_k : 0;
   const long long token = a.tokens[row];
   const T* x = static_cast<const T*>(a.logits) + b * a.stride_b + t * a.stride_t;
-  const Slice sl = slice_of(x, a.vocab, split, splits, kThreads);
+  const Slice sl = slice_of(x, a.vocab, split, splits, kWidth);
   const uint4* xv = reinterpret_cast<const uint4*>(x + sl.head);
   const uint4 none = make_uint4(Vec<T>::kNone, Vec<T>::kNone, Vec<T>::kNone, Vec<T>::kNone);
   // (the next round's loads are in flight while this one's are summed)
@@ -303,10 +325,16 @@ __global__ void __launch_bounds__(kThreads, 4) score_kernel(const AiScoreArgs a,
 #pragma unroll 4
       for (int r = 1; r < splits; ++r) p = merge(p, s_slices[r], c);
     if constexpr (kTop) {
-      // An entry below some slice's k-th one is in no list of k.
-      Key least = 0;
+      // An entry below some slice's k-th one, or below the (k / splits)-th ones of all
+      // slices, is in no list of k.
+      const int share = (k - 1) / splits;
+      Key least = 0, all = ~(Key)0;
 #pragma unroll 4
-      for (int r = 0; r < splits; ++r) least = max(least, lists[r * k + k - 1]);
+      for (int r = 0; r < splits; ++r) {
+        least = max(least, lists[r * k + k - 1]);
+        all = min(all, lists[r * k + share]);
+      }
+      least = max(least, all);
       if (tid == 0) top.n = 0;
       __syncthreads();
       for (int j = tid; j < splits * k; j += kThreads) {

@@ -72,7 +72,7 @@ def empty_rows(logits: Tensor) -> Tensor:
     *rows, V = logits.shape
     pitch = logits.stride(-2)
     if not V < pitch <= V + 1024:
-        pitch = V
+        return torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
     return torch.empty((*rows, pitch), dtype=logits.dtype, device=logits.device)[..., :V]
 
 
