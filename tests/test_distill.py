@@ -335,6 +335,11 @@ def test_backward_of_its_own(shape, V, dtype, tail, cuda_device):
     assert torch.equal(torch.autograd.grad(loss, y, wide(w), retain_graph=True)[0], want[1])
     plain = distill_loss(y, ids, t, tau, tail)
     assert torch.equal(torch.autograd.grad(plain, y, w)[0], want[1])
+    base = torch.zeros(*shape, 2 * V, dtype=dtype, device=cuda_device)
+    base[..., ::2] = x
+    base.requires_grad_()
+    d = torch.autograd.grad(distill_loss(base[..., ::2], ids, t, tau, tail), base, w)[0]
+    assert torch.equal(d[..., ::2], want[1]) and not bool(d[..., 1::2].any())
     read_status(cuda_device)  # (the word twice)
     nan = torch.full(shape, float("nan"), device=cuda_device)
     d = torch.autograd.grad(loss, y, nan)[0].reshape(-1, V)
