@@ -101,13 +101,13 @@ struct __align__(16) RowStats {
 template <typename T>
 struct Row {
   const T* x;
-  T* d;  // nullptr: losses alone
+  T* d;  // (no meaning for losses alone)
   uint32_t b;
   __device__ __forceinline__ Row(const AiDistillArgs& a, uint32_t row) {
     b = row / (uint32_t)a.seq_len;
     const int64_t t = row - b * (uint32_t)a.seq_len;
     x = static_cast<const T*>(a.logits) + b * a.stride_b + t * a.stride_t;
-    d = a.dlogits ? static_cast<T*>(a.dlogits) + b * a.dstride_b + t * a.dstride_t : nullptr;
+    d = static_cast<T*>(a.dlogits) + b * a.dstride_b + t * a.dstride_t;
   }
 };
 
@@ -341,6 +341,143 @@ __device__ __forceinline__ void zero_row(T* d, int vocab, int split, int splits,
   ends<E>(z, vocab, tid, [&](int v) { d[v] = from_f32<T>(0.f); });
 }
 
+__device__ __forceinline__ void finish(const AiDistillArgs& a, uint32_t row, const List& list, const Totals& all) {
+  if (a.losses) a.losses[row] = all.loss(list);
+  if (a.row_stats)
+    *reinterpret_cast<RowStats*>(a.row_stats + 8 * (int64_t)row) =
+        RowStats{all.m, all.base(list), all.m_all, all.s_all, all.mass, list.norm, 1.f, 0.f};
+}
+__device__ __forceinline__ void finish_dead(const AiDistillArgs& a, uint32_t row) {
+  if (a.losses) a.losses[row] = 0.f;
+  if (a.row_stats) *reinterpret_cast<RowStats*>(a.row_stats + 8 * (int64_t)row) = RowStats{};
+}
+
+// Losses alone, of rows enough and long ones: nothing has to stay, so a slice is streamed
+// through the registers, by as many CTAs a row as there are rows too few for; the first
+// of them joins the sums.  4096 rows of 151,936 bf16 252 us (4.4 TB/s), where slices held
+// in shared memory take 371; 1023 rows of 65,536 words 50 (49), of 32,003 45 (33: more
+// CTAs to hide the lists behind), 16 of 151,936 6.9 (6.2).
+// Listed words are looked for where a bit says that a warp's vectors of a round hold
+// one, and hidden there.
+constexpr int kStreamed = 128 * 1024;  // bytes of a row from which losses alone are streamed
+constexpr int kSum = kThreads - 32;  // threads that sum (the first warp reads and weighs the list)
+constexpr int kAtOnce = 4;           // vectors of a thread in flight
+constexpr int kRound = kSum * kAtOnce;
+constexpr int kMaxRounds = AI_DISTILL_MAX_ROW_BYTES / 16 / kRound + 1;
+
+// Sets element q of vector v, counted from the warp's first one of a round, to -inf.
+template <typename T>
+__device__ __forceinline__ void hide(uint4 (&raw)[kAtOnce], int v, int q) {
+  constexpr int P = 4 / sizeof(T);  // elements of a word
+  const uint32_t keep = P == 1 ? 0u : q % P ? 0xffffu : 0xffff0000u;
+#pragma unroll
+  for (int u = 0; u < kAtOnce; ++u) {
+    if (v - u * kSum != (int)(threadIdx.x % 32)) continue;
+    uint32_t w[4] = {raw[u].x, raw[u].y, raw[u].z, raw[u].w};
+#pragma unroll
+    for (int h = 0; h < 4; ++h)
+      if (q / P == h) w[h] = (w[h] & keep) | (Vec<T>::kNone & ~keep);
+    raw[u] = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads, 4) losses_kernel(const AiDistillArgs a, const int splits) {
+  constexpr int E = 16 / sizeof(T);
+  __shared__ List list;
+  __shared__ float2 s_parts[kMaxSplit * kWarps];  // (m, s) of each warp of the cluster, in its first CTA
+  __shared__ uint32_t s_flags[kMaxRounds];        // per round: bit kAtOnce warp + u
+  const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32, K = a.n_top, id = tid - 32;
+  const uint32_t row = blockIdx.x / (uint32_t)splits;
+  const int split = (int)(blockIdx.x - row * splits);
+  const Row<T> r(a, row);
+  const Slice sl = slice_of(r.x, a.vocab, split, splits, kWidth);
+  const uint4* xv = reinterpret_cast<const uint4*>(r.x + sl.head);
+  const uint4 none = make_uint4(Vec<T>::kNone, Vec<T>::kNone, Vec<T>::kNone, Vec<T>::kNone);
+  // (a CTA of the cluster must run before its shared memory is written to)
+  if (splits > 1) asm volatile("barrier.cluster.arrive;" ::: "memory");
+  uint4 next[kAtOnce];
+  auto load = [&](int i) {
+#pragma unroll
+    for (int u = 0; u < kAtOnce; ++u) next[u] = i + u * kSum < sl.i1 ? __ldg(xv + i + u * kSum) : none;
+  };
+  Entries entries;  // (the first warp's)
+  if (warp == 0) {
+    for (int i = lane; i < kMaxRounds; i += 32) s_flags[i] = 0;
+    read_words<T>(a, list, entries, row, split == 0, [](bool) {});
+    __syncwarp();
+    if (list.live) {
+#pragma unroll
+      for (int i = 0; i < kSets; ++i) {
+        const int w = entries.word[i];
+        if (32 * i >= K || w < sl.head || w >= sl.tail) continue;
+        const int v = (w - sl.head) / E - sl.i0;
+        if (v >= 0 && v < sl.i1 - sl.i0) atomicOr(s_flags + v / kRound, 1u << (kAtOnce * (v % kSum / 32) + v % kRound / kSum));
+      }
+    }
+  } else if (splits > 1) {
+    load(sl.i0 + id);  // (few rows: they do not wait for the list)
+  }
+  __syncthreads();
+  if (!list.live) {
+    if (split == 0 && tid == 0) finish_dead(a, row);
+    return;
+  }
+  const float c = list.c;
+  if (warp == 0) {
+    weigh(a, list, entries);
+  } else {
+    if (splits == 1) load(sl.i0 + id);
+    Part part{-CUDART_INF_F, 0.f, 0.f};
+    for (int i = sl.i0, round = 0; i < sl.i1; i += kRound, ++round) {
+      uint4 raw[kAtOnce];
+#pragma unroll
+      for (int u = 0; u < kAtOnce; ++u) raw[u] = next[u];
+      load(i + kRound + id);
+      if (s_flags[round] >> (kAtOnce * (warp - 1)) & ((1u << kAtOnce) - 1)) {
+        const int v0 = sl.head + (i + id - lane) * E;
+        for (int k0 = 0; k0 < K; k0 += 32) {
+          const int el = list.word[k0 + lane] - v0;
+          uint32_t in = __ballot_sync(0xffffffffu, el >= 0 && el < kRound * E && el / E % kSum < 32);
+          while (in) {
+            const int e = __shfl_sync(0xffffffffu, el, __ffs(in) - 1);
+            in &= in - 1;
+            hide<T>(raw, e / E, e % E);
+          }
+        }
+      }
+      accumulate<T, kAtOnce, false>(part, raw, c);
+    }
+    ends<E>(sl, a.vocab, id, [&](int v) {
+      for (int j = 0; j < K; ++j)
+        if (list.word[j] == v) return;
+      add_end(part, at(r.x, v), c);
+    });
+    const float2 mine = join_lanes(make_float2(part.m, part.s), c);
+    if (splits > 1) {
+      asm volatile("barrier.cluster.wait;" ::: "memory");
+      if (lane == 0) cg::this_cluster().map_shared_rank(s_parts, 0)[split * kWarps + warp] = mine;
+    } else if (lane == 0) {
+      s_parts[warp] = mine;
+    }
+  }
+  if (splits > 1) {
+    if (warp == 0) asm volatile("barrier.cluster.wait;" ::: "memory");
+    cg::this_cluster().sync();
+  } else {
+    __syncthreads();
+  }
+  if (split > 0 || warp > 0) return;
+  float2 rest = make_float2(-CUDART_INF_F, 0.f);
+  for (int i = lane; i < splits * kWarps; i += 32) {
+    if (i % kWarps == 0) continue;
+    const Part q = merge(Part{rest.x, rest.y, 0.f}, Part{s_parts[i].x, s_parts[i].y, 0.f}, c);
+    rest = make_float2(q.m, q.s);
+  }
+  const Totals all(list, join_lanes(rest, c));
+  if (lane == 0) finish(a, row, list, all);
+}
+
 template <typename T>
 __global__ void __launch_bounds__(kThreads, 6) distill_kernel(const AiDistillArgs a, const int splits) {
   constexpr int E = 16 / sizeof(T);
@@ -371,11 +508,8 @@ __global__ void __launch_bounds__(kThreads, 6) distill_kernel(const AiDistillArg
   }
   __syncthreads();
   if (!list.live) {
-    if (split == 0 && tid == 0) {
-      if (a.losses) a.losses[row] = 0.f;
-      if (a.row_stats) *reinterpret_cast<RowStats*>(a.row_stats + 8 * (int64_t)row) = RowStats{};
-    }
-    if (r.d) zero_row(r.d, a.vocab, split, splits, kWidth, tid, kThreads);
+    if (split == 0 && tid == 0) finish_dead(a, row);
+    if (a.dlogits) zero_row(r.d, a.vocab, split, splits, kWidth, tid, kThreads);
     return;
   }
   const uint4* held = reinterpret_cast<const uint4*>(smem);
@@ -389,7 +523,6 @@ __global__ void __launch_bounds__(kThreads, 6) distill_kernel(const AiDistillArg
       ptx::mbar_wait(bar, 0, kWait);  // (the copy lands before the CTA ends)
     }
     // The listed words' places become -inf, which adds nothing to the others' sum.
-    constexpr int kSum = kThreads - 32;
     const int id = tid - 32;
     if (id < K) {
       const int w = list.word[id], at_ = w - sl.head - sl.i0 * E;
@@ -427,13 +560,8 @@ __global__ void __launch_bounds__(kThreads, 6) distill_kernel(const AiDistillArg
     rest = make_float2(q.m, q.s);
   }
   const Totals all(list, join_lanes(rest, c));
-  if (split == 0 && tid == 0) {
-    if (a.losses) a.losses[row] = all.loss(list);
-    if (a.row_stats)
-      *reinterpret_cast<RowStats*>(a.row_stats + 8 * (int64_t)row) =
-          RowStats{all.m, all.base(list), all.m_all, all.s_all, all.mass, list.norm, 1.f, 0.f};
-  }
-  if (!r.d) return;
+  if (split == 0 && tid == 0) finish(a, row, list, all);
+  if (!a.dlogits) return;
   const Dense dense(all.m, c, list.up, all.base(list));
   const bool alike = lie_alike(r.x, r.d);
 #pragma unroll 2
@@ -547,15 +675,19 @@ int64_t slice_bytes(const AiDistillArgs& a, int splits) {
   return ((vecs + splits - 1) / splits + kWidth - 1) / kWidth * kWidth * 16;
 }
 
-template <typename T>
-int launch(const AiDistillArgs& a, cudaStream_t st) {
-  ProfScope ps(AI_PROF_DISTILL, st);
-  const int splits = slices(a);
-  const int64_t smem = slice_bytes(a, splits);
-  if (splits > 8 &&
-      cudaFuncSetAttribute(distill_kernel<T>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess)
+// CTAs of a row where they are streamed: for four per SM, at least kLeast bytes each.
+int stream_slices(const AiDistillArgs& a) {
+  const int64_t rows = (int64_t)a.batch * a.seq_len, bytes = (int64_t)a.vocab * (a.dtype == AI_DTYPE_F32 ? 4 : 2);
+  int s = 1;
+  while (2 * s <= kMaxSplit && 2 * s * rows <= 4 * (int64_t)sm_count() && s * (int64_t)kLeast < bytes) s *= 2;
+  return s;
+}
+
+// `kernel` on clusters of `splits` CTAs, one per row.
+int launch_rows(void (*kernel)(AiDistillArgs, int), const AiDistillArgs& a, int splits, int64_t smem, cudaStream_t st) {
+  if (splits > 8 && cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess)
     return AI_ERR_LAUNCH;
-  if (cudaFuncSetAttribute(distill_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
+  if (smem > 0 && cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
     return AI_ERR_LAUNCH;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)((int64_t)a.batch * a.seq_len * splits));
@@ -568,16 +700,23 @@ int launch(const AiDistillArgs& a, cudaStream_t st) {
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = splits > 1 ? 1 : 0;
-  if (cudaLaunchKernelEx(&cfg, distill_kernel<T>, a, splits) != cudaSuccess) return AI_ERR_LAUNCH;
+  if (cudaLaunchKernelEx(&cfg, kernel, a, splits) != cudaSuccess) return AI_ERR_LAUNCH;
   return cudaGetLastError() == cudaSuccess ? AI_OK : AI_ERR_LAUNCH;
 }
 
 template <typename T>
+int launch(const AiDistillArgs& a, cudaStream_t st) {
+  ProfScope ps(AI_PROF_DISTILL, st);
+  if (!a.dlogits && (int64_t)a.batch * a.seq_len >= sm_count() && (int64_t)a.vocab * (int64_t)sizeof(T) >= kStreamed)
+    return launch_rows(losses_kernel<T>, a, stream_slices(a), 0, st);
+  const int splits = slices(a);
+  return launch_rows(distill_kernel<T>, a, splits, slice_bytes(a, splits), st);
+}
+
+template <typename T>
 int launch_bwd(const AiDistillBwdArgs& g, cudaStream_t st) {
-  // Slices of a row: CTAs for four per SM, at least 16 KB each.
-  const int64_t rows = (int64_t)g.fwd.batch * g.fwd.seq_len, bytes = (int64_t)g.fwd.vocab * (int)sizeof(T);
-  int splits = 1;
-  while (2 * splits <= kMaxSplit && 2 * splits * rows <= 4 * (int64_t)sm_count() && splits * (int64_t)kLeast < bytes) splits *= 2;
+  const int64_t rows = (int64_t)g.fwd.batch * g.fwd.seq_len;
+  const int splits = stream_slices(g.fwd);
   ProfScope ps(AI_PROF_DISTILL, st);
   distill_bwd_kernel<T><<<(unsigned)(rows * splits), kThreads, 0, st>>>(g, splits);
   return cudaGetLastError() == cudaSuccess ? AI_OK : AI_ERR_LAUNCH;

@@ -90,8 +90,7 @@ def test_against_definition(shape, V, K, dtype, tail, cuda_device):
         y = x.clone().requires_grad_()
         loss = distill_loss(y, ids, t, temperature=temp, tail=tail)
         check(x, ids, t, None, temp, tail, loss.detach(), None)
-        d = torch.autograd.grad(loss, y, w)[0]
-        assert torch.equal(d, grad)
+        check(x, ids, t, w, temp, tail, None, torch.autograd.grad(loss, y, w)[0])
         assert torch.equal(distill_loss(x, ids, t, temperature=temp, tail=tail), loss.detach())
     check(x, ids, t, None, None, tail, *distill_loss_and_grad(x, ids, t, tail=tail))
     assert read_status(cuda_device) == 0
@@ -143,11 +142,12 @@ def test_awkward_rows(V, tail, cuda_device):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("tail", TAILS)
-@pytest.mark.parametrize("V,K,dtype", [(7, 3, torch.bfloat16), (1003, 40, torch.float16), (3077, 128, torch.bfloat16), (9001, 64, torch.float32),
-                                       (30011, 100, torch.bfloat16)])
-def test_many_rows(V, K, dtype, tail, cuda_device):
+@pytest.mark.parametrize("V,K,dtype,n", [(7, 3, torch.bfloat16, 50), (1003, 40, torch.float16, 50), (3077, 128, torch.bfloat16, 50),
+                                         (9001, 64, torch.float32, 50), (30011, 100, torch.bfloat16, 50), (65541, 128, torch.float16, 7),
+                                         (32800, 33, torch.float32, 13), (70003, 5, torch.bfloat16, 40)])
+def test_many_rows(V, K, dtype, n, tail, cuda_device):
     """More rows than run at once, awkward ones among them: copies of a row come out alike,
-    in place too, and losses do not depend on whether the gradient is written."""
+    in place too, and through autograd."""
     from autoindexer_b200 import distill_loss, distill_loss_and_grad, read_status
 
     x, ids, t, w, tau = make((24,), V, K, dtype, K)
@@ -155,16 +155,19 @@ def test_many_rows(V, K, dtype, tail, cuda_device):
         x[3 + i] = row.to(dtype)
     ids[20, 0], ids[20, -1] = 0, V - 1
     few = [x, ids, t, w, tau]
-    many = [y.repeat(50, *[1] * (y.dim() - 1)).to(cuda_device) for y in few]
+    many = [y.to(cuda_device).repeat(n, *[1] * (y.dim() - 1)) for y in few]
     losses, grad = distill_loss_and_grad(*many, tail=tail)
     check(*few[:3], w, tau, tail, losses[:24].cpu(), grad[:24].cpu())
-    for y in (losses, grad):
-        assert all(torch.equal(y[24 * i:24 * i + 24].nan_to_num(9), y[:24].nan_to_num(9)) for i in range(50))
-    alone = distill_loss(*many[:3], many[4], tail=tail)
+    leaf = many[0].clone().requires_grad_()
+    alone = distill_loss(leaf, *many[1:3], many[4], tail=tail)
+    through = torch.autograd.grad(alone, leaf, many[3])[0]
+    live = w != 0
+    check(x[live], ids[live], t[live], w[live], tau[live], tail, alone.detach()[:24][live.to(cuda_device)].cpu(),
+          through[:24][live.to(cuda_device)].cpu())
+    for y in (losses, grad, alone.detach(), through):
+        assert all(torch.equal(y[24 * i:24 * i + 24].nan_to_num(9), y[:24].nan_to_num(9)) for i in range(n))
     here = distill_loss_and_grad(*many, tail=tail, out=many[0])
     assert torch.equal(here[1].nan_to_num(9), grad.nan_to_num(9))
-    live = many[3] != 0
-    assert torch.equal(alone[live].nan_to_num(9), losses[live].nan_to_num(9))
     read_status(cuda_device)  # (word 0 is also word V - 1 where a list has one twice)
 
 
@@ -326,20 +329,20 @@ def test_backward_of_its_own(shape, V, dtype, tail, cuda_device):
     x.view(-1, V)[-2, int(ids.view(-1, 5)[-2, 0].clamp_min(0))] = -INF
     x.view(-1, V)[0, V // 2:] = -INF
     w.view(-1)[0] *= -1
-    want = distill_loss_and_grad(x, ids, t, w, tau, tail)
-    check(x, ids, t, w, tau, tail, None, want[1])
+    check(x, ids, t, w, tau, tail, *distill_loss_and_grad(x, ids, t, w, tau, tail))
     y = x.clone().requires_grad_()
+    plain = distill_loss(y, ids, t, tau, tail)
+    want = torch.autograd.grad(plain, y, w)[0]
+    check(x, ids, t, w, tau, tail, None, want)
     wide = lambda z: torch.stack((z, z), -1)[..., 0]  # noqa: E731
     with torch.autograd.graph.saved_tensors_hooks(lambda z: z, wide):
         loss = distill_loss(y, ids, t, tau, tail)
-    assert torch.equal(torch.autograd.grad(loss, y, wide(w), retain_graph=True)[0], want[1])
-    plain = distill_loss(y, ids, t, tau, tail)
-    assert torch.equal(torch.autograd.grad(plain, y, w)[0], want[1])
+    assert torch.equal(torch.autograd.grad(loss, y, wide(w), retain_graph=True)[0], want)
     base = torch.zeros(*shape, 2 * V, dtype=dtype, device=cuda_device)
     base[..., ::2] = x
     base.requires_grad_()
     d = torch.autograd.grad(distill_loss(base[..., ::2], ids, t, tau, tail), base, w)[0]
-    assert torch.equal(d[..., ::2], want[1]) and not bool(d[..., 1::2].any())
+    assert torch.equal(d[..., ::2], want) and not bool(d[..., 1::2].any())
     read_status(cuda_device)  # (the word twice)
     nan = torch.full(shape, float("nan"), device=cuda_device)
     d = torch.autograd.grad(loss, y, nan)[0].reshape(-1, V)
