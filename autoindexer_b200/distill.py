@@ -154,7 +154,8 @@ def distill_loss_and_grad(student_logits: Tensor, teacher_tokens: Tensor, teache
     gradient are 0.  Returns ``(losses, gradient)``, the losses without the
     weights; the gradient, of the logits' shape and type, goes on by
     ``student_logits.backward(gradient)``.  ``out`` receives it (same shape and
-    type; ``student_logits`` itself is allowed, which needs no memory for it).
+    type; ``student_logits`` itself is allowed, which needs no memory for it, but
+    no other tensor that overlaps it).
     A backward through the losses raises."""
     tensors, plan = _planned(student_logits, teacher_tokens, teacher_logprobs, weights, temperature, tail)
     logits = tensors[0]
@@ -166,6 +167,8 @@ def distill_loss_and_grad(student_logits: Tensor, teacher_tokens: Tensor, teache
             raise ValueError(f"out must be {logits.dtype} of shape {tuple(logits.shape)}, got {out.dtype} {tuple(out.shape)}")
         if grad.stride(-1) != 1:
             raise ValueError("out must have a contiguous last dimension")
+        if any(st == 0 and n > 1 for n, st in zip(grad.shape, grad.stride())):
+            raise ValueError("the rows of out must not share memory")
         _call.on_device("out", grad, logits.get_device())
     losses = _losses(logits)
 

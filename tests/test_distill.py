@@ -396,6 +396,7 @@ def test_refusals(cuda_device):
             distill_loss(*args)
     for error, more in [(ValueError, dict(weights=w[:, :1])), (TypeError, dict(weights=w.double())),
                         (ValueError, dict(out=x[:1])), (ValueError, dict(out=x.float())), (RuntimeError, dict(out=x.cpu())),
+                        (ValueError, dict(out=x[:, :1].expand(2, 3, 200))),
                         (ValueError, dict(out=torch.empty(2, 200, 3, dtype=x.dtype, device=cuda_device).transpose(1, 2)))]:
         with pytest.raises(error):
             distill_loss_and_grad(x, ids, t, **more)
