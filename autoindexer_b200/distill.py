@@ -76,7 +76,7 @@ def _run(a, tensors, losses: Optional[Tensor], grad: Optional[Tensor]) -> None:
 
 
 def _losses(logits: Tensor) -> Tensor:
-    return torch.empty(logits.shape[:-1], dtype=torch.float32, device=logits.device)
+    return logits.new_empty(logits.shape[:-1], dtype=torch.float32)
 
 
 class DistillFn(torch.autograd.Function):
@@ -86,7 +86,7 @@ class DistillFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, ids, logprobs, temperature, plan):
         a, losses = _call.copy(plan), _losses(logits)
-        stats = torch.empty((losses.numel(), 8), dtype=torch.float32, device=logits.device)
+        stats = losses.new_empty((losses.numel(), 8))
         a.row_stats = stats.data_ptr()
         _run(a, (logits, ids, logprobs, None, temperature), losses, None)
         ctx.save_for_backward(logits, ids, logprobs, temperature, stats)

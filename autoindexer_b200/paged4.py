@@ -159,8 +159,8 @@ def paged_read_4bit(k_pages: Tensor, v_pages: Tensor, k_scales: Tensor, v_scales
         known = (shape, plan)
         _READ_PLANS.keep(at, given, tensors, known)
     shape, plan = known
-    k = torch.empty(shape, dtype=dtype, device=k_pages.device)
-    v = torch.empty_like(k)
+    k = k_pages.new_empty(shape, dtype=dtype)
+    v = k.new_empty(shape)
     _paged(_lib.lib().ai_paged_read_4bit, "ai_paged_read_4bit", plan, (k, v, *tensors))
     return k, v
 
@@ -240,8 +240,7 @@ def paged_attention_4bit(query: Tensor, k_pages: Tensor, v_pages: Tensor, k_scal
 def _attend(plan, tensors, return_lse):
     q, k_pages, v_pages, k_scales, v_scales, page_table, lens, query_lens = tensors
     B, Hq, T, D = q.shape
-    device = q.device
-    out = torch.empty((B, T, Hq, D), dtype=q.dtype, device=device)
+    out = q.new_empty((B, T, Hq, D))
     a = _call.copy(plan)
     a.q.ptr, a.out.ptr, a.lens = q.data_ptr(), out.data_ptr(), lens.data_ptr()
     _point(a.pool, k_pages, v_pages, k_scales, v_scales, page_table)
@@ -249,9 +248,9 @@ def _attend(plan, tensors, return_lse):
         a.query_lens = query_lens.data_ptr()
     lse = None
     if return_lse:
-        lse = torch.empty((B, Hq, T), dtype=torch.float32, device=device)
+        lse = q.new_empty((B, Hq, T), dtype=torch.float32)
         a.lse = lse.data_ptr()
-    ws = torch.empty(a.workspace_bytes, dtype=torch.uint8, device=device)
+    ws = k_pages.new_empty(a.workspace_bytes)
     a.workspace = ws.data_ptr()
     _call.launch(_lib.lib().ai_paged_attn_4bit, a, q.get_device(), "ai_paged_attn_4bit")
     del ws

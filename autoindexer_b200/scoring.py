@@ -72,8 +72,8 @@ def empty_rows(logits: Tensor) -> Tensor:
     *rows, V = logits.shape
     pitch = logits.stride(-2)
     if not V < pitch <= V + 1024:
-        return torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
-    return torch.empty((*rows, pitch), dtype=logits.dtype, device=logits.device)[..., :V]
+        return logits.new_empty(logits.shape)
+    return logits.new_empty((*rows, pitch))[..., :V]
 
 
 _PLANS = _call.Plans()
@@ -104,19 +104,18 @@ def _run(plan, tensors, entropy: bool, stats: bool):
     a.logits, a.tokens = logits.data_ptr(), tokens.data_ptr()
     if temperature is not None:
         a.temperature = temperature.data_ptr()
-    rows, device, k = tokens.shape, logits.device, a.top_k
-    logprobs = torch.empty(rows, dtype=torch.float32, device=device)
+    rows, k = tokens.shape, a.top_k
+    logprobs = logits.new_empty(rows, dtype=torch.float32)  # (cheaper than torch.empty)
     a.logprobs = logprobs.data_ptr()
     h = top = ids = st = None
     if entropy:
-        h = torch.empty(rows, dtype=torch.float32, device=device)
+        h = logprobs.new_empty(rows)
         a.entropy = h.data_ptr()
     if k:
-        top = torch.empty((*rows, k), dtype=torch.float32, device=device)
-        ids = torch.empty((*rows, k), dtype=torch.int64, device=device)
+        top, ids = logprobs.new_empty((*rows, k)), tokens.new_empty((*rows, k))
         a.top_logprobs, a.top_tokens = top.data_ptr(), ids.data_ptr()
     if stats:
-        st = torch.empty((rows.numel(), 4), dtype=torch.float32, device=device)
+        st = logprobs.new_empty((rows.numel(), 4))
         a.row_stats = st.data_ptr()
     _call.launch(_lib.lib().ai_token_logprobs, a, logits.get_device(), "ai_token_logprobs")
     return logprobs, h, top, ids, st
