@@ -408,8 +408,9 @@ __global__ void __launch_bounds__(32 * warps_of(NT), 1) split_kernel(const AiPag
   while (next_seg(a, p, scan, wc, w1, s)) {
     const int row0 = s.grp * p.unit_rows, n_rows = min(p.rows - row0, p.unit_rows);
     // Query fragments: lane (g, t) has dims 32 c + 8 t + {0 .. 7} of row 8 nt + g,
-    // all rows scaled by the power of two that brings the unit's largest element
-    // to the top of fp16's range (and odd dims by 2^-4, for their codes).
+    // scaled by the power of two that brings the row's largest element to the top of
+    // fp16's range (and odd dims by 2^-4, for their codes).  Rows without a query
+    // are zeros, whatever the padding holds.
     // Keys that row 8 nt + 2 t + e sees; -1: no query.  (Looked up where it is
     // wanted when registers are short.)
     auto count = [&](int nt, int e) -> int {
@@ -419,7 +420,7 @@ __global__ void __launch_bounds__(32 * warps_of(NT), 1) split_kernel(const AiPag
     const int first[2] = {count(0, 0), count(0, 1)};
     auto seen = [&](int nt, int e) -> int { return NT == 1 ? first[e] : count(nt, e); };
     int least = s.keys;               // tiles that end by it are seen whole
-    float slope;                      // of the scores, in units of log 2, above zero (its sign is the fragments')
+    float2 slope[NT];                 // of rows 2 t and 2 t + 1's scores, in units of log 2, above zero (its sign is the fragments')
     {
       const float sign = a.scale < 0.f ? -1.f : 1.f;
       uint4 raw[NT][C];  // (all of them in flight at once)
@@ -427,30 +428,29 @@ __global__ void __launch_bounds__(32 * warps_of(NT), 1) split_kernel(const AiPag
       for (int nt = 0; nt < NT; ++nt) {
         const int i = 8 * nt + g, r = i < n_rows ? row0 + i : row0, tok = r / p.group, head = s.hk * p.group + r - tok * p.group;
         const T* src = static_cast<const T*>(a.q.ptr) + s.b * a.q.stride_b + head * a.q.stride_h + tok * a.q.stride_t + 8 * t;
+        const bool real = i < n_rows && tok < s.n;
 #pragma unroll
-        for (int c = 0; c < C; ++c) raw[nt][c] = load_q(src + kGroup * c);
+        for (int c = 0; c < C; ++c) raw[nt][c] = real ? load_q(src + kGroup * c) : make_uint4(0u, 0u, 0u, 0u);
       }
-      float top = 0.f;
+      __syncwarp();  // (the last unit's fragments have been read)
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
+      for (int nt = 0; nt < NT; ++nt) {
+        float top = 0.f;
 #pragma unroll
-        for (int c = 0; c < C; ++c) {
-          if (8 * nt + g >= n_rows) raw[nt][c] = make_uint4(0u, 0u, 0u, 0u);
+        for (int c = 0; c < C; ++c)
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
             const float f = fabsf(element<T>(raw[nt][c], e));
             if (f < CUDART_INF_F) top = fmaxf(top, f);
           }
-        }
-#pragma unroll
-      for (int d = 1; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-      const int up = top > 0.f ? 14 - ilogbf(top) : 0;
-      slope = fmaxf(ldexpf(fabsf(a.scale) * kLog2e, 24 - up), FLT_MIN);  // (above 0, so that a masked score stays -inf)
-      // (in two factors: up reaches 163)
-      const float up1 = sign * ldexpf(1.f, up / 2), up2 = ldexpf(1.f, up - up / 2);
-      __syncwarp();  // (the last unit's fragments have been read)
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        const int up = top > 0.f ? 14 - ilogbf(top) : 0;
+        // (in two factors: up reaches 163)
+        const float up1 = sign * ldexpf(1.f, up / 2), up2 = ldexpf(1.f, up - up / 2);
+        // (above 0, so that a masked score stays -inf, and finite)
+        const float mine = fminf(fmaxf(ldexpf(fabsf(a.scale) * kLog2e, 24 - up), FLT_MIN), FLT_MAX);
+        slope[nt] = make_float2(__shfl_sync(0xffffffffu, mine, 8 * t), __shfl_sync(0xffffffffu, mine, 8 * t + 4));
 #pragma unroll
         for (int c = 0; c < C; ++c) {
           uint32_t h[4];
@@ -556,8 +556,8 @@ __global__ void __launch_bounds__(32 * warps_of(NT), 1) split_kernel(const AiPag
         bool move = false;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-          top[nt][0] = fmaxf(ptx::fmax3(sc[0][nt][0].x, sc[0][nt][1].x, sc[1][nt][0].x), sc[1][nt][1].x) * slope;
-          top[nt][1] = fmaxf(ptx::fmax3(sc[0][nt][0].y, sc[0][nt][1].y, sc[1][nt][0].y), sc[1][nt][1].y) * slope;
+          top[nt][0] = fmaxf(ptx::fmax3(sc[0][nt][0].x, sc[0][nt][1].x, sc[1][nt][0].x), sc[1][nt][1].x) * slope[nt].x;
+          top[nt][1] = fmaxf(ptx::fmax3(sc[0][nt][0].y, sc[0][nt][1].y, sc[1][nt][0].y), sc[1][nt][1].y) * slope[nt].y;
           move |= top[nt][0] > ref[nt][0] + (kSlack + kLift) || top[nt][1] > ref[nt][1] + (kSlack + kLift);
         }
         __half2 big = __half2half2(__ushort_as_half(0));
@@ -653,7 +653,7 @@ __global__ void __launch_bounds__(32 * warps_of(NT), 1) split_kernel(const AiPag
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            const float2 y = __ffma2_rn(sc[mt][nt][h], make_float2(slope, slope), make_float2(-ref[nt][0], -ref[nt][1]));
+            const float2 y = __ffma2_rn(sc[mt][nt][h], slope[nt], make_float2(-ref[nt][0], -ref[nt][1]));
             const float2 w = make_float2(ptx::ex2(y.x), ptx::ex2(y.y));
             l[nt] = __fadd2_rn(l[nt], w);
             if constexpr (kOnce) {
