@@ -58,7 +58,9 @@ constexpr int kMaxBlocks = 3;  // column blocks (of 8 query rows) of a unit, at 
 constexpr float kLift = 7.f;   // a weight of 1 is held as 2^7
 constexpr float kSlack = 8.f;  // the running maximum moves when a score passes it by 2^8
 constexpr int kLeastExp = -14;  // V scales below 2^-14 are divided by no less
-constexpr float kNoRef = -1e30f;  // before the first score
+// Before the first score: below any (of a row scaled to fp16's top, 2^-9 a dim and
+// step of a code, with |scale| <= 2^16: 2^17 at most), near enough for a difference.
+constexpr float kNoRef = -0x1p20f;
 
 // Warps of a CTA (one per SM), by column blocks.
 __host__ __device__ constexpr int warps_of(int blocks) { return blocks == 1 ? 16 : 8; }
@@ -478,7 +480,7 @@ __global__ void __launch_bounds__(32 * warps_of(NT), 1) split_kernel(const AiPag
     }
 
     float o[NT][2 * C][4];             // (odd rows of a block, of odd dims, are 2^4 times the even ones)
-    float ref[NT][2];                  // what the exponents are taken from: the running maximum less kLift
+    float ref[NT][2];                  // what the scores are taken less: their running maximum
     float2 l[NT], l_before[NT];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
@@ -556,9 +558,9 @@ __global__ void __launch_bounds__(32 * warps_of(NT), 1) split_kernel(const AiPag
         bool move = false;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-          top[nt][0] = fmaxf(ptx::fmax3(sc[0][nt][0].x, sc[0][nt][1].x, sc[1][nt][0].x), sc[1][nt][1].x) * slope[nt].x;
-          top[nt][1] = fmaxf(ptx::fmax3(sc[0][nt][0].y, sc[0][nt][1].y, sc[1][nt][0].y), sc[1][nt][1].y) * slope[nt].y;
-          move |= top[nt][0] > ref[nt][0] + (kSlack + kLift) || top[nt][1] > ref[nt][1] + (kSlack + kLift);
+          top[nt][0] = fmaxf(ptx::fmax3(sc[0][nt][0].x, sc[0][nt][1].x, sc[1][nt][0].x), sc[1][nt][1].x);
+          top[nt][1] = fmaxf(ptx::fmax3(sc[0][nt][0].y, sc[0][nt][1].y, sc[1][nt][0].y), sc[1][nt][1].y);
+          move |= (top[nt][0] - ref[nt][0]) * slope[nt].x > kSlack || (top[nt][1] - ref[nt][1]) * slope[nt].y > kSlack;
         }
         __half2 big = __half2half2(__ushort_as_half(0));
 #pragma unroll
@@ -627,8 +629,9 @@ __global__ void __launch_bounds__(32 * warps_of(NT), 1) split_kernel(const AiPag
               float x = top[nt][e], to = ref[nt][e];
 #pragma unroll
               for (int d = 4; d < 32; d <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, d));
-              if (x > to + (kSlack + kLift)) to = x - kLift;
-              alpha[e] = ptx::ex2(ref[nt][e] - to);
+              const float per = e ? slope[nt].y : slope[nt].x;
+              if ((x - to) * per > kSlack) to = x;
+              alpha[e] = ptx::ex2((ref[nt][e] - to) * per);
               ref[nt][e] = to;
 #pragma unroll
               for (int i = 0; i < 2 * C; ++i) o[nt][i][e] *= alpha[e] * down, o[nt][i][2 + e] *= alpha[e] * down;
@@ -653,7 +656,8 @@ __global__ void __launch_bounds__(32 * warps_of(NT), 1) split_kernel(const AiPag
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            const float2 y = __ffma2_rn(sc[mt][nt][h], slope[nt], make_float2(-ref[nt][0], -ref[nt][1]));
+            // (the difference first: scores of any size then have the largest one's weight exact)
+            const float2 y = __ffma2_rn(__fadd2_rn(sc[mt][nt][h], make_float2(-ref[nt][0], -ref[nt][1])), slope[nt], make_float2(kLift, kLift));
             const float2 w = make_float2(ptx::ex2(y.x), ptx::ex2(y.y));
             l[nt] = __fadd2_rn(l[nt], w);
             if constexpr (kOnce) {
@@ -717,7 +721,7 @@ __global__ void __launch_bounds__(32 * warps_of(NT), 1) split_kernel(const AiPag
               make_float4(o[nt][2 * c][e] * 0x1p24f * inv, o[nt][2 * c][2 + e] * 0x1p20f * inv, o[nt][2 * c + 1][e] * 0x1p24f * inv,
                           o[nt][2 * c + 1][2 + e] * 0x1p20f * inv);
         // (NaN among the scores: +inf, which makes the joined row NaN)
-        if (g == 0) p.part_lse[row] = sum > 0.f ? ref[nt][e] + log2f(sum) : sum == 0.f ? -CUDART_INF_F : CUDART_INF_F;
+        if (g == 0) p.part_lse[row] = sum > 0.f ? fmaf(ref[nt][e], e ? slope[nt].y : slope[nt].x, log2f(sum) - kLift) : sum == 0.f ? -CUDART_INF_F : CUDART_INF_F;
       }
   }
   asm volatile("cp.async.wait_all;" ::: "memory");

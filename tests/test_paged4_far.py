@@ -1,10 +1,11 @@
 """``paged_attention_4bit`` where parts of one call are far apart in size: what
 padding rows hold, query heads and tokens.  Tolerances as in ``test_paged4``."""
 
+import numpy as np
 import pytest
 import torch
 
-from test_paged4 import check_attention, filled, heads, ints
+from test_paged4 import check_attention, dense, filled, heads, ints
 
 HALVES = [torch.bfloat16, torch.float16]
 
@@ -73,3 +74,40 @@ def test_tokens_far_apart(cuda_device):
     got, l2 = paged_attention_4bit(q, *args, return_lse=True)
     for t in (0, 1, 3, 4):
         assert torch.equal(got[:, t], want[:, t]) and torch.equal(l2[:, :, t], lse[:, :, t])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,of_q,of_k,scaling", [
+    (torch.bfloat16, 2.0 ** 20, 1.0, None), (torch.bfloat16, 2.0 ** 30, 1.0, None), (torch.bfloat16, 2.0 ** 60, 1.0, -0.1),
+    (torch.bfloat16, 2.0 ** 100, 1.0, None), (torch.float16, 2.0 ** 12, 2.0 ** 12, 8.0), (torch.float16, 2.0 ** 10, 2.0 ** 10, 1.0)])
+@pytest.mark.parametrize("T,D", [(1, 128), (3, 64), (5, 128)])
+def test_large_scores(T, D, dtype, of_q, of_k, scaling, cuda_device):
+    """Scores of 2^20 and more, whose steps in fp32 are many powers of e: a row is the
+    value of its best key where that is best by more than a score's rounding."""
+    from autoindexer_b200 import paged_attention_4bit, read_status
+
+    lens = [65, 1300]
+    cache, table = filled(2, 2, D, 32, lens, torch.float32, 5, cuda_device)
+    cache[2].mul_(of_k)
+    q = (heads(2, 8, T, D, dtype, 6, cuda_device) * of_q).contiguous()
+    out, lse = paged_attention_4bit(q, *cache, table, ints(lens, cuda_device), scaling=scaling, return_lse=True)
+    assert read_status(cuda_device) == 0
+    scale = scaling or D ** -0.5
+    qn, got, l = q.double().cpu().numpy(), out.double().cpu().numpy(), lse.double().cpu().numpy()
+    sure = 0
+    for b in range(2):
+        k, v = dense(cache, table, b, lens[b])
+        for h in range(8):
+            for t in range(T):
+                n = lens[b] - T + t + 1
+                s = k[h // 4, :n] @ qn[b, h, t] * scale
+                most = (np.abs(k[h // 4, :n]) @ np.abs(qn[b, h, t])).max() * abs(scale)
+                best, second = np.sort(s)[::-1][:2]
+                assert abs(l[b, h, t] - best) <= 2.0 ** -19 * most + 1e-5 * (1 + abs(best)) + np.log(n)
+                assert (np.abs(got[b, t, h]) <= np.abs(v[h // 4, :n]).max(0) * (1 + 2.0 ** -8)).all()
+                if best - second > 2.0 ** -18 * most + 40:
+                    sure += 1
+                    want = v[h // 4, int(np.argmax(s))]
+                    tol = (2.0 ** -10 + torch.finfo(dtype).eps / 2) * np.abs(want) + 2.0 ** -24
+                    assert (np.abs(got[b, t, h] - want) <= tol).all(), (b, h, t)
+    assert sure >= 8 * T
