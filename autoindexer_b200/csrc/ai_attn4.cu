@@ -11,13 +11,13 @@
 //   S^T = K Q^T   the sums of a group of 32 dims, less 8 sum(q), meet the group's
 //                 scale in fp32;
 //   O^T += V^T P  P takes each key's V scale, per group of 32 dims: weights, held 2^7
-//                 above 1 at the running maximum, and scales, divided by the power
-//                 of two above the largest |scale| met so far, have an fp16 product
-//                 (weights down to 2^-31 of the largest count).  For bf16 queries the
-//                 weights are fp16 before it, two roundings of 2^-12 beside the output's
-//                 2^-9; for fp16 ones the product is rounded alone: the error against 64
-//                 bits is then 1.33 times that of the output's rounding, not 1.6 times, and
-//                 the drafted case below takes 152 us, not 145.
+//                 above 1 at the running maximum, times scales, divided by a power of two
+//                 of the group's own (two to four times the largest |scale| met so far), in
+//                 fp32 and rounded to fp16 once.  A product of 2^-19 of the largest weight's
+//                 with the group's largest scale begins to lose digits, one of 2^-30 does
+//                 not count.  (Scales divided, and bf16 queries' weights rounded, in fp16
+//                 before that: 73 us for 76 on the first case below, but scales of 2^-14 of
+//                 the group's largest lose digits whatever their weight.)
 // The codes are fp16's subnormal numbers as they lie, 2^-24 c: one logical operation
 // a pair.  (Their 8 comes off K's as the sums start, off V's before the product.)
 // Both products have the tile's keys on the instruction's long side, so up to 8
@@ -38,7 +38,6 @@
 
 #include <cfloat>
 #include <cstring>
-#include <type_traits>
 
 #include "ai_common.cuh"
 #include "ai_kernels.h"
@@ -260,16 +259,8 @@ __device__ __forceinline__ float element(const uint4& r, int i) {
 }
 
 __device__ __forceinline__ __half2 as_half2(uint32_t w) { return *reinterpret_cast<const __half2*>(&w); }
-__device__ __forceinline__ uint32_t mul2(uint32_t a, uint32_t b) {
-  const __half2 r = __hmul2(as_half2(a), as_half2(b));
-  return *reinterpret_cast<const uint32_t*>(&r);
-}
 // A half in both halves.
 __device__ __forceinline__ uint32_t twice(uint32_t h) { return h | h << 16; }
-__device__ __forceinline__ uint32_t twice_of(uint32_t w, int i) {
-  const __half2 r = i ? __high2half2(as_half2(w)) : __low2half2(as_half2(w));
-  return *reinterpret_cast<const uint32_t*>(&r);
-}
 __device__ __forceinline__ float half_of(uint32_t w, int i) {
   return __half2float(__ushort_as_half((unsigned short)(i ? w >> 16 : w)));
 }
@@ -279,7 +270,6 @@ __global__ void __launch_bounds__(32 * warps_of(NT), 1) split_kernel(const AiPag
   using L = Tile<D>;
   using M = Smem<D, NT>;
   constexpr int C = L::C, H = (C + 1) / 2, S = kStages;
-  constexpr bool kOnce = std::is_same<T, __half>::value;  // weights times scales are rounded once
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   extern __shared__ __align__(128) uint8_t smem[];
   int* scan = reinterpret_cast<int*>(smem + M::SCAN);
@@ -491,11 +481,13 @@ __global__ void __launch_bounds__(32 * warps_of(NT), 1) split_kernel(const AiPag
       ref[nt][0] = ref[nt][1] = kNoRef;
       l[nt] = l_before[nt] = make_float2(0.f, 0.f);
     }
-    // The largest |V scale| so far is at most 2^v_exp (v_lim, before the first one
-    // 0; v_unit divides by it).
-    int v_exp = kLeastExp;
-    uint32_t v_lim = 0, v_unit = twice(0x7400u);
-    static_assert(kLeastExp == -14, "v_unit: 2^14");
+    // Per group of dims: |V scales| so far are at most a power of two (v_lim, two
+    // groups a word), and v_unit divides by it.
+    float2 v_unit[H];
+    uint32_t v_lim[H];
+#pragma unroll
+    for (int i = 0; i < H; ++i) v_unit[i] = make_float2(0x1p14f, 0x1p14f), v_lim[i] = twice(0x0400u);
+    static_assert(kLeastExp == -14, "v_unit and v_lim");
 
     for (int tile = s.tile; tile < s.end; ++tile) {
       asm volatile("cp.async.wait_group %0;" ::"n"(S - 2) : "memory");
@@ -562,14 +554,13 @@ __global__ void __launch_bounds__(32 * warps_of(NT), 1) split_kernel(const AiPag
           top[nt][1] = fmaxf(ptx::fmax3(sc[0][nt][0].y, sc[0][nt][1].y, sc[1][nt][0].y), sc[1][nt][1].y);
           move |= (top[nt][0] - ref[nt][0]) * slope[nt].x > kSlack || (top[nt][1] - ref[nt][1]) * slope[nt].y > kSlack;
         }
-        __half2 big = __half2half2(__ushort_as_half(0));
 #pragma unroll
-        for (int mt = 0; mt < 2; ++mt)
-#pragma unroll
-          for (int h = 0; h < 2; ++h)
-#pragma unroll
-            for (int i = 0; i < H; ++i) big = __hmax2(big, __habs2(as_half2(vs[mt][h][i])));
-        return move || !__hble2(big, as_half2(v_lim));
+        for (int i = 0; i < H; ++i) {
+          const __half2 big = __hmax2(__hmax2(__habs2(as_half2(vs[0][0][i])), __habs2(as_half2(vs[0][1][i]))),
+                                      __hmax2(__habs2(as_half2(vs[1][0][i])), __habs2(as_half2(vs[1][1][i]))));
+          move |= !__hble2(big, as_half2(v_lim[i]));
+        }
+        return move;
       };
       bool guard = false;  // some row must not meet an infinite or NaN scale that another sees
       if (__any_sync(0xffffffffu, tops() || ragged)) {
@@ -601,25 +592,29 @@ __global__ void __launch_bounds__(32 * warps_of(NT), 1) split_kernel(const AiPag
         }
         if (__any_sync(0xffffffffu, tops())) {
           // (an infinite scale makes what it meets infinite; it has no part in the bound)
-          float size = 0.f;
+          float down[2 * H];
 #pragma unroll
-          for (int mt = 0; mt < 2; ++mt)
+          for (int c = 0; c < 2 * H; ++c) {
+            float size = 0.f;
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
+            for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
-              for (int c = 0; c < C; ++c) {
+              for (int h = 0; h < 2; ++h) {
                 const float d = fabsf(half_of(vs[mt][h][c / 2], c % 2));
                 if (d < CUDART_INF_F) size = fmaxf(size, d);
               }
 #pragma unroll
-          for (int d = 1; d < 32; d <<= 1) size = fmaxf(size, __shfl_xor_sync(0xffffffffu, size, d));
-          float down = 1.f;
-          const int e = size > 0.f ? max(ilogbf(size) + 1, kLeastExp) : kLeastExp;
-          if (e > v_exp) {
-            down = ptx::ex2((float)(v_exp - e));
-            v_exp = e;
-            v_lim = twice(e > 15 ? 0x7bffu : __half_as_ushort(__float2half_rn(ptx::ex2((float)e))));
-            v_unit = twice(__half_as_ushort(__float2half_rn(ptx::ex2((float)-e))));
+            for (int d = 4; d < 32; d <<= 1) size = fmaxf(size, __shfl_xor_sync(0xffffffffu, size, d));
+            float& unit = c % 2 ? v_unit[c / 2].y : v_unit[c / 2].x;
+            down[c] = 1.f;
+            if (size * unit > 1.f) {
+              const int e = min(ilogbf(size) + 2, 16);  // (room for twice as much: few lists then meet a larger one)
+              const float to = ptx::ex2((float)-e);
+              down[c] = to / unit;
+              unit = to;
+              const uint32_t lim = e > 15 ? 0x7bffu : (uint32_t)(15 + e) << 10;  // 2^e
+              v_lim[c / 2] = c % 2 ? (v_lim[c / 2] & 0xffffu) | lim << 16 : (v_lim[c / 2] & 0xffff0000u) | lim;
+            }
           }
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
@@ -634,19 +629,13 @@ __global__ void __launch_bounds__(32 * warps_of(NT), 1) split_kernel(const AiPag
               alpha[e] = ptx::ex2((ref[nt][e] - to) * per);
               ref[nt][e] = to;
 #pragma unroll
-              for (int i = 0; i < 2 * C; ++i) o[nt][i][e] *= alpha[e] * down, o[nt][i][2 + e] *= alpha[e] * down;
+              for (int i = 0; i < 2 * C; ++i) o[nt][i][e] *= alpha[e] * down[i / 2], o[nt][i][2 + e] *= alpha[e] * down[i / 2];
             }
             l[nt] = __fmul2_rn(l[nt], make_float2(alpha[0], alpha[1]));
             l_before[nt] = __fmul2_rn(l_before[nt], make_float2(alpha[0], alpha[1]));
           }
         }
       }
-#pragma unroll
-      for (int mt = 0; mt < 2; ++mt)
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-          for (int i = 0; i < H; ++i) vs[mt][h][i] = mul2(vs[mt][h][i], v_unit);
       // Weights, and per group of dims the weights times the V scales as the
       // second product takes them.
 #pragma unroll
@@ -660,16 +649,11 @@ __global__ void __launch_bounds__(32 * warps_of(NT), 1) split_kernel(const AiPag
             const float2 y = __ffma2_rn(__fadd2_rn(sc[mt][nt][h], make_float2(-ref[nt][0], -ref[nt][1])), slope[nt], make_float2(kLift, kLift));
             const float2 w = make_float2(ptx::ex2(y.x), ptx::ex2(y.y));
             l[nt] = __fadd2_rn(l[nt], w);
-            if constexpr (kOnce) {
 #pragma unroll
-              for (int c = 0; c < C; ++c) {
-                const float d = half_of(vs[mt][h][c / 2], c % 2);
-                pv[nt][c][h] = pack2(w.x * d, w.y * d);
-              }
-            } else {
-              const uint32_t w2 = pack2(w.x, w.y);
-#pragma unroll
-              for (int c = 0; c < C; ++c) pv[nt][c][h] = mul2(w2, twice_of(vs[mt][h][c / 2], c % 2));
+            for (int i = 0; i < H; ++i) {
+              const float2 d = __fmul2_rn(__half22float2(as_half2(vs[mt][h][i])), v_unit[i]);
+              pv[nt][2 * i][h] = pack2(w.x * d.x, w.y * d.x);
+              if (2 * i + 1 < C) pv[nt][2 * i + 1][h] = pack2(w.x * d.y, w.y * d.y);
             }
             if (guard) {
               const uint32_t keep = (sc[mt][nt][h].x == -CUDART_INF_F ? 0u : 0xffffu) | (sc[mt][nt][h].y == -CUDART_INF_F ? 0u : 0xffff0000u);
@@ -714,12 +698,14 @@ __global__ void __launch_bounds__(32 * warps_of(NT), 1) split_kernel(const AiPag
         for (int d = 4; d < 32; d <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
         if (seen(nt, e) <= 0) continue;
         const int64_t row = (int64_t)(s.unit + worker) * p.unit_rows + 8 * nt + 2 * t + e;
-        const float inv = sum == 0.f ? 0.f : ptx::ex2((float)v_exp) / sum;
+        const float all = sum == 0.f ? 0.f : 1.f / sum;
 #pragma unroll
-        for (int c = 0; c < C; ++c)
+        for (int c = 0; c < C; ++c) {
+          const float inv = all / (c % 2 ? v_unit[c / 2].y : v_unit[c / 2].x);  // (a power of two)
           *reinterpret_cast<float4*>(p.part_o + row * D + kGroup * c + 4 * g) =
               make_float4(o[nt][2 * c][e] * 0x1p24f * inv, o[nt][2 * c][2 + e] * 0x1p20f * inv, o[nt][2 * c + 1][e] * 0x1p24f * inv,
                           o[nt][2 * c + 1][2 + e] * 0x1p20f * inv);
+        }
         // (NaN among the scores: +inf, which makes the joined row NaN)
         if (g == 0) p.part_lse[row] = sum > 0.f ? fmaf(ref[nt][e], e ? slope[nt].y : slope[nt].x, log2f(sum) - kLift) : sum == 0.f ? -CUDART_INF_F : CUDART_INF_F;
       }

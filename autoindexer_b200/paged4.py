@@ -219,8 +219,9 @@ def paged_attention_4bit(query: Tensor, k_pages: Tensor, v_pages: Tensor, k_scal
 
     Keys and values are taken as the cache stands for them; scores, sums and the
     softmax are float32, and the products of weights and the values' scales are
-    float16 (bfloat16 queries: the weights too; 2^-11 together).  Slots that no query of the sequence sees may hold
-    anything.  Up to 1024 sequences, head_dim 32, 64 or 128, any strides of the
+    rounded to float16 once: to 2^-11 of themselves and 2^-30 of the largest
+    weight times the largest scale of their 32 dims.  Padding tokens, and slots that
+    no query of the sequence sees, may hold anything.  Up to 1024 sequences, head_dim 32, 64 or 128, any strides of the
     query; the pools as ``paged_append_4bit`` takes them.  A length or page out
     of range is clamped and sets the status word.  There is no gradient: a
     backward through the results raises."""
