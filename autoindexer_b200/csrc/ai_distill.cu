@@ -157,6 +157,7 @@ __device__ __forceinline__ void read_words(const AiDistillArgs& a, List& list, E
   mine.inv = inverse(tau);
   if (lane == 0) list.c = slope(tau);
   // A word that an earlier entry has is left out.
+  __syncwarp();  // (votes do not order the lanes' words in shared memory)
   bool again[kSets] = {};
 #pragma unroll
   for (int i = 0; i < kSets; ++i) {
