@@ -55,9 +55,10 @@ constexpr int kWidth = 32;             // slices are whole vectors of so many la
 static_assert(AI_DISTILL_MAX_ROW_BYTES / kMaxSplit + 16 * kWidth <= 200 * 1024, "a slice in shared memory");
 static_assert(kMaxTop <= kThreads - 32, "a thread per entry");
 constexpr long long kWait = 1000000000LL;
-// A remainder of the teacher's probability below 2^-20 is what the rounding of
-// its fp32 log-probabilities may leave.
-constexpr float kLeastRest = 0x1p-20f;
+// A remainder of the teacher's probability within kLostSum + kLost sum p |ln p| is
+// what the rounding of its fp32 log-probabilities may leave: 2^-24 of each, and of the
+// logarithm and the sum that they were taken less.
+constexpr float kLost = 0x1p-24f, kLostSum = 0x1p-23f;
 
 // What one warp finds out of a row's list.
 struct List {
@@ -74,6 +75,11 @@ struct List {
 };
 
 __device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
+  return v;
+}
+__device__ __forceinline__ double warp_sum(double v) {
 #pragma unroll
   for (int d = 16; d > 0; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
   return v;
@@ -220,11 +226,27 @@ __device__ __forceinline__ void weigh(const AiDistillArgs& a, List& list, Entrie
   p_top = warp_sum(p_top);
   sum = warp_sum(sum);
   term = warp_sum(term);
+  // The remainder in 64 bits: a sure teacher's, 1e-5 say, is a small difference.
+  float rest = 0.f;
+  if (!renorm) {
+    double all = 0.;
+    float lost = 0.f;
+#pragma unroll
+    for (int i = 0; i < kSets; ++i) {
+      if (32 * i >= K || word[i] < 0) continue;
+      all += exp((double)logp[i]);
+      lost += p[i] * fabsf(logp[i]);
+    }
+    all = 1. - warp_sum(all);
+    lost = fmaf(kLost, warp_sum(lost), kLostSum);
+    rest = (float)all;
+    if (rest <= lost) rest = 0.f;  // (NaN stays)
+  }
   if (lane == 0) {
     list.up = mine.wgt * inv;
     list.inv = inv;
     list.p_top = p_top;
-    list.p_rest = p_top != p_top ? p_top : renorm || 1.f - p_top < kLeastRest ? 0.f : 1.f - p_top;
+    list.p_rest = rest;
     list.m = m;
     list.s = sum;
     list.norm = norm;

@@ -123,7 +123,8 @@ def distill_loss(student_logits: Tensor, teacher_tokens: Tensor, teacher_logprob
     ``token_logprobs`` gives them (taken at the same temperature); entries with
     a negative token or ``-inf`` are left out, so lists may be shorter than K.
     ``tail="bucket"``: the teacher's remaining probability is compared with the
-    student's on all other words together (a remainder below 2^-20 counts as none); ``"renormalize"``: the teacher's
+    student's on all other words together (a remainder of 2^-23 + 2^-24 sum p_k |ln p_k| or less, which the rounding of
+    ``teacher_logprobs`` may leave, counts as none); ``"renormalize"``: the teacher's
     words are all there is (any logits will do for ``teacher_logprobs``).
     ``temperature`` as in ``token_logprobs``.
 

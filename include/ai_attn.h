@@ -687,7 +687,8 @@ int ai_token_logprobs_bwd(const AiScoreBwdArgs* args, void* stream);
  * likeliest words are known per row (ids and their log-probabilities t_k), with
  * q = softmax(z) over the whole vocabulary:
  *   AI_TAIL_BUCKET       p_k = exp(t_k), and the other words as one: p_r = 1 - sum p_k (0 where that is
- *                        below 2^-20, which rounding the t_k leaves),
+ *                        at most 2^-23 + 2^-24 sum p_k |t_k|, which fp32's rounding of
+ *                        the t_k may leave),
  *                        q_r = sum of q over them;
  *                        L = sum_k p_k (t_k - ln q_k) + p_r (ln p_r - ln q_r);
  *   AI_TAIL_RENORMALIZE  p = softmax(t), p_r = 0; L = sum_k p_k (ln p_k - ln q_k);
