@@ -219,7 +219,7 @@ __device__ __forceinline__ void weigh(const AiDistillArgs& a, List& list, Entrie
     if (word[i] >= 0) p[i] = expf(logp[i]);
     p_top += p[i];
     sum += share(xk[i], c, o);
-    if (p[i] != 0.f) term += p[i] * logp[i] - p[i] * inv * (xk[i] - o);  // (p / tau first: logits may be as far apart as fp32 goes)
+    if (p[i] != 0.f) term += p[i] * logp[i] - scaled(xk[i] - o, p[i] * inv);  // (p / tau first: logits may be as far apart as fp32 goes)
     list.x[32 * i + lane] = xk[i];
     list.p[32 * i + lane] = p[i];
   }
@@ -299,8 +299,8 @@ struct Totals {
   __device__ __forceinline__ float loss(const List& list) const {
     const float o = list.m == -CUDART_INF_F ? 0.f : list.m, l2 = log2f(s_all);
     float r = list.term;
-    if (list.p_top != 0.f) r += list.p_top * list.inv * (m_all - o) + list.p_top * (l2 * kLn2);
-    if (p_rest != 0.f) r += p_rest * (logf(p_rest) - (log2f(s) - l2) * kLn2) - p_rest * list.inv * (m - m_all);
+    if (list.p_top != 0.f) r += scaled(m_all - o, list.p_top * list.inv) + list.p_top * (l2 * kLn2);
+    if (p_rest != 0.f) r += p_rest * (logf(p_rest) - (log2f(s) - l2) * kLn2) - scaled(m - m_all, p_rest * list.inv);
     return empty ? CUDART_INF_F : r;
   }
   // What the gradients of the others have in common, but for the weight.

@@ -99,6 +99,10 @@ __device__ __forceinline__ float slope(float tau) {
 // logits are (in units of log 2 it may pass it).
 __device__ __forceinline__ float inverse(float tau) { return fminf(1.f / tau, FLT_MAX); }
 
+// d (a difference of logits, -inf for a masked one) times `inv`, 1 / tau or a
+// probability over tau, which may be 0 (an infinite temperature) or infinite.
+__device__ __forceinline__ float scaled(float d, float inv) { return d == 0.f || d == -CUDART_INF_F ? d : d * inv; }
+
 // 2^((x - m) c), 0 for a masked logit (m may be -inf then).
 __device__ __forceinline__ float weight(float x, float c, float m) {
   return x == -CUDART_INF_F ? 0.f : ptx::ex2((x - m) * c);

@@ -348,7 +348,7 @@ __global__ void __launch_bounds__(kThreads, 4) score_kernel(const AiScoreArgs a,
   if (tid == 0) {
     const bool empty = p.s == 0.f;
     const float l2 = log2f(p.s), h = empty ? 0.f : (l2 - p.t / p.s) * kLn2;
-    a.logprobs[row] = empty ? -CUDART_INF_F : (given - p.m) * inv - l2 * kLn2;
+    a.logprobs[row] = empty ? -CUDART_INF_F : scaled(given - p.m, inv) - l2 * kLn2;
     if constexpr (kEntropy) a.entropy[row] = h;
     if (a.row_stats) reinterpret_cast<float4*>(a.row_stats)[row] = make_float4(p.m, l2, h, empty ? 1.f : 0.f);
     s_row[0] = p.m, s_row[1] = l2;
@@ -358,7 +358,7 @@ __global__ void __launch_bounds__(kThreads, 4) score_kernel(const AiScoreArgs a,
     if (tid < k) {
       const float m = s_row[0], l2 = s_row[1];
       const Key key = l2 == l2 ? top.best[tid] : 0;  // (a row with a NaN has no order)
-      a.top_logprobs[row * k + tid] = l2 != l2 ? l2 : key ? (key_value(key) - m) * inv - l2 * kLn2 : -CUDART_INF_F;
+      a.top_logprobs[row * k + tid] = l2 != l2 ? l2 : key ? scaled(key_value(key) - m, inv) - l2 * kLn2 : -CUDART_INF_F;
       a.top_tokens[row * k + tid] = key ? key_index(key) : -1;
     }
   }
