@@ -865,7 +865,10 @@ size_t layout(const AiPagedAttn4Args& a, Plan* p) {
 template <typename T, int D, int NT>
 int launch(const AiPagedAttn4Args& a, const Plan& p, cudaStream_t st) {
   const size_t smem = Smem<D, NT>::bytes(a.batch);
-  if (cudaFuncSetAttribute(split_kernel<T, D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
+  // (the limit is the kernel's, not the call's: always the same, so that calls of other
+  // threads never find it lower than they need)
+  if (cudaFuncSetAttribute(split_kernel<T, D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                           (int)Smem<D, NT>::bytes(kMaxBatch)) != cudaSuccess)
     return AI_ERR_LAUNCH;
   split_kernel<T, D, NT><<<p.workers / warps_of(NT), 32 * warps_of(NT), smem, st>>>(a, p);
   return cudaGetLastError() == cudaSuccess ? AI_OK : AI_ERR_LAUNCH;

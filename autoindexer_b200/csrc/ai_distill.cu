@@ -52,7 +52,8 @@ constexpr int kMaxSplit = 16;
 constexpr int kLeast = 16 * 1024;      // bytes of a slice, at least (for more CTAs than the memory asks for)
 constexpr int kSlice = 38 * 1024;      // bytes of a slice where there are rows enough: five CTAs per SM
 constexpr int kWidth = 32;             // slices are whole vectors of so many lanes
-static_assert(AI_DISTILL_MAX_ROW_BYTES / kMaxSplit + 16 * kWidth <= 200 * 1024, "a slice in shared memory");
+constexpr int kMostSlice = AI_DISTILL_MAX_ROW_BYTES / kMaxSplit + 16 * kWidth;  // bytes
+static_assert(kMostSlice <= 200 * 1024, "a slice in shared memory");
 static_assert(kMaxTop <= kThreads - 32, "a thread per entry");
 constexpr long long kWait = 1000000000LL;
 // A remainder of the teacher's probability within kLostSum + kLost sum p |ln p| is
@@ -710,7 +711,9 @@ int stream_slices(const AiDistillArgs& a) {
 int launch_rows(void (*kernel)(AiDistillArgs, int), const AiDistillArgs& a, int splits, int64_t smem, cudaStream_t st) {
   if (splits > 8 && cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess)
     return AI_ERR_LAUNCH;
-  if (smem > 0 && cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
+  // (the limit is the kernel's, not the call's: always the same, so that calls of other
+  // threads never find it lower than they need)
+  if (smem > 0 && cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostSlice) != cudaSuccess)
     return AI_ERR_LAUNCH;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)((int64_t)a.batch * a.seq_len * splits));
