@@ -1341,9 +1341,11 @@ int launch_t(const AiPrefixAttnArgs& a, const Plan& p, cudaStream_t st) {
     return sm100_make_map_of(&tk, a.k_pages, a.n_pages, a.num_kv_heads, a.page_size, box, D, a.dtype) &&
            sm100_make_map_of(&tv, a.v_pages, a.n_pages, a.num_kv_heads, a.page_size, box, D, a.dtype);
   };
+  // (the limit is the kernel's, not the call's: always all that there is, so that calls of
+  // other threads never find it lower than they need)
   auto smem_of = [&](auto kernel, size_t bytes) {
     cfg.dynamicSmemBytes = bytes;
-    return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) == cudaSuccess;
+    return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024) == cudaSuccess;
   };
   if (p.tile.workers > 0) {
     if (!maps(tile_keys(p.nt))) return AI_ERR_TMA;

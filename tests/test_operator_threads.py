@@ -64,3 +64,21 @@ def test_attention_of_two_batches(cuda_device):
         jobs.append(lambda args=(q, *cache, table, ints(lens, cuda_device)): [paged_attention_4bit(*args)])
     wants = [job() for job in jobs]
     same(together(jobs, 3000, cuda_device), wants)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("prefix_len", [0, 3000])
+def test_shared_prefix_attention_of_two_batches(prefix_len, cuda_device):
+    from autoindexer_b200 import shared_prefix_attention
+
+    H, S, D = 2, 16, 64
+    pages = [heads(200, H, S, D, torch.bfloat16, s, cuda_device).contiguous() for s in (1, 2)]
+    prefix = torch.arange(-(-prefix_len // S), dtype=torch.int32, device=cuda_device) if prefix_len else None
+    jobs = []
+    for B in (1, 700):
+        table = torch.randint(0, 200, (B, 2), dtype=torch.int32, device=cuda_device)
+        lens = ints([20 + i % 3 for i in range(B)], cuda_device)
+        q = heads(B, 4, 1, D, torch.bfloat16, 6, cuda_device)
+        jobs.append(lambda args=(q, *pages, prefix, prefix_len, table, lens): [shared_prefix_attention(*args)])
+    wants = [job() for job in jobs]
+    same(together(jobs, 3000, cuda_device), wants)
