@@ -23,6 +23,43 @@ __all__ = ["distill_loss", "distill_loss_and_grad"]
 _PLANS = _call.Plans()
 
 
+def _starts(x: Tensor):
+    """Where the rows of ``x`` start, in bytes, in order."""
+    at = torch.zeros((), dtype=torch.int64)
+    for n, st in zip(x.shape[:-1], x.stride()[:-1]):
+        at = at[..., None] + torch.arange(n) * st
+    return at.flatten().mul_(x.element_size()).add_(x.data_ptr()).sort()[0]
+
+
+def _span(x: Tensor) -> int:
+    return (sum((n - 1) * st for n, st in zip(x.shape, x.stride())) + 1) * x.element_size()
+
+
+def check_out(out: Tensor, logits: Tensor) -> None:
+    """Raises where rows of ``out`` overlap one another, or rows of ``logits`` other
+    than as the same memory in the same places."""
+    row = out.shape[-1] * out.element_size()
+    inner, least = out.shape[-1], True
+    for st, n in sorted((st, n) for n, st in zip(out.shape[:-1], out.stride()) if n > 1):
+        least &= st >= inner  # (each dimension steps past all that lies within it: rows one after the other)
+        inner = st * (n - 1) + inner
+    if not least:
+        at = _starts(out)
+        if at.numel() > 1 and int(at.diff().min()) < row:
+            raise ValueError("the rows of out must not share memory")
+    a, b = out.data_ptr(), logits.data_ptr()
+    if a + _span(out) <= b or b + _span(logits) <= a:
+        return
+    if a == b and all(n == 1 or x == y for n, x, y in zip(out.shape, out.stride(), logits.stride())):
+        return
+    mine, other = _starts(out), _starts(logits)
+    after = torch.searchsorted(mine, other)  # (mine[after - 1] < other <= mine[after])
+    before = other - mine[(after - 1).clamp_min(0)]
+    behind = mine[after.clamp_max(len(mine) - 1)] - other
+    if bool((((after > 0) & (before < row)) | ((after < len(mine)) & (behind < row))).any()):
+        raise ValueError("out overlaps student_logits: it may be the same rows or apart from them")
+
+
 def _plan(logits, ids, logprobs, weights, temperature, tail):
     """Checks the arguments; returns the tensors the kernel reads and the
     argument struct without pointers."""
@@ -155,8 +192,8 @@ def distill_loss_and_grad(student_logits: Tensor, teacher_tokens: Tensor, teache
     gradient are 0.  Returns ``(losses, gradient)``, the losses without the
     weights; the gradient, of the logits' shape and type, goes on by
     ``student_logits.backward(gradient)``.  ``out`` receives it (same shape and
-    type; ``student_logits`` itself is allowed, which needs no memory for it, but
-    no other tensor that overlaps it).
+    type; ``student_logits`` itself is allowed, which needs no memory for it; rows
+    that overlap one another, or those of ``student_logits`` in part, are refused).
     A backward through the losses raises."""
     tensors, plan = _planned(student_logits, teacher_tokens, teacher_logprobs, weights, temperature, tail)
     logits = tensors[0]
@@ -168,9 +205,8 @@ def distill_loss_and_grad(student_logits: Tensor, teacher_tokens: Tensor, teache
             raise ValueError(f"out must be {logits.dtype} of shape {tuple(logits.shape)}, got {out.dtype} {tuple(out.shape)}")
         if grad.stride(-1) != 1:
             raise ValueError("out must have a contiguous last dimension")
-        if any(st == 0 and n > 1 for n, st in zip(grad.shape, grad.stride())):
-            raise ValueError("the rows of out must not share memory")
         _call.on_device("out", grad, logits.get_device())
+        check_out(grad, logits)
     losses = _losses(logits)
 
     def run():
