@@ -56,6 +56,7 @@ constexpr int kMostSlice = AI_DISTILL_MAX_ROW_BYTES / kMaxSplit + 16 * kWidth;  
 static_assert(kMostSlice <= 200 * 1024, "a slice in shared memory");
 static_assert(kMaxTop <= kThreads - 32, "a thread per entry");
 constexpr long long kWait = 1000000000LL;
+constexpr float kLostSlice = -1.f;     // a warp's sum over a slice whose copy did not come: losses NaN, no gradient
 // A remainder of the teacher's probability within kLostSum + kLost sum p |ln p| is
 // what the rounding of its fp32 log-probabilities may leave: 2^-24 of each, and of the
 // logarithm and the sum that they were taken less.
@@ -542,9 +543,10 @@ __global__ void __launch_bounds__(kThreads, 6) distill_kernel(const AiDistillArg
   if (warp == 0) {
     weigh(a, list, entries);
   } else {
+    bool lost = false;  // the slice never came
     if (vecs > 0 && !ptx::mbar_wait(bar, 0, kWait)) {
       report(a.status, AI_ERR_DEV_TIMEOUT);
-      ptx::mbar_wait(bar, 0, kWait);  // (the copy lands before the CTA ends)
+      lost = !ptx::mbar_wait(bar, 0, kWait);  // (once more: the copy should land before the CTA ends)
     }
     // The listed words' places become -inf, which adds nothing to the others' sum.
     const int id = tid - 32;
@@ -567,6 +569,7 @@ __global__ void __launch_bounds__(kThreads, 6) distill_kernel(const AiDistillArg
       add_end(part, at(r.x, v), c);
     });
     mine = join_lanes(make_float2(part.m, part.s), c);
+    if (__any_sync(0xffffffffu, lost)) mine.y = kLostSlice;
   }
   // The warps' sums go to every CTA of the cluster; each joins them in the same order.
   if (splits > 1) {
@@ -579,11 +582,19 @@ __global__ void __launch_bounds__(kThreads, 6) distill_kernel(const AiDistillArg
     __syncthreads();
   }
   float2 rest = make_float2(-CUDART_INF_F, 0.f);
+  bool whole = true;
   for (int i = lane; i < splits * kWarps; i += 32) {
+    whole &= s_parts[i].y != kLostSlice;
     const Part q = merge(Part{rest.x, rest.y, 0.f}, Part{s_parts[i].x, s_parts[i].y, 0.f}, c);
     rest = make_float2(q.m, q.s);
   }
-  const Totals all(list, join_lanes(rest, c));
+  rest = join_lanes(rest, c);
+  if (!__all_sync(0xffffffffu, whole)) {
+    // (no gradient: it may lie over the logits)
+    if (split == 0 && tid == 0) finish(a, row, list, Totals(list, make_float2(0.f, CUDART_NAN_F)));
+    return;
+  }
+  const Totals all(list, rest);
   if (split == 0 && tid == 0) finish(a, row, list, all);
   if (!a.dlogits) return;
   const Dense dense(all.m, c, list.up, all.base(list));
