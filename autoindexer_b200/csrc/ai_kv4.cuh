@@ -40,7 +40,9 @@ __device__ __forceinline__ Place place(const AiPool4& p, int64_t b, int64_t at) 
 }
 
 inline int check_pool(const AiPool4& p, int head_dim) {
-  if (p.n_pages <= 0 || p.page_size < 16 || (p.page_size & (p.page_size - 1)) || p.max_pages <= 0) return AI_ERR_SHAPE;
+  // (a slot's bytes from its page's start are counted in 31 bits)
+  if (p.n_pages <= 0 || p.page_size < 16 || p.page_size > AI_POOL4_MAX_PAGE || (p.page_size & (p.page_size - 1)) || p.max_pages <= 0)
+    return AI_ERR_SHAPE;
   if (!p.page_table) return AI_ERR_NULL;
   if (p.page_table_stride < 0) return AI_ERR_STRIDE;
   for (int i = 0; i < 4; ++i) {

@@ -26,6 +26,7 @@ from .paged import _table
 __all__ = ["paged_append_4bit", "paged_read_4bit", "paged_attention_4bit"]
 
 MAX_BATCH = 1024  # sequences of an attention call
+MAX_PAGE = 16777216  # slots of a page (AI_POOL4_MAX_PAGE)
 GROUP = 32
 
 
@@ -35,8 +36,8 @@ def _pool(p, k_pages, v_pages, k_scales, v_scales, page_table, batch: int, heads
     if len(s) != 4 or s != v_pages.shape or s[1] != heads or s[3] != head_dim // 2:
         raise ValueError(f"k_pages and v_pages must be (n_pages, {heads}, page_size, {head_dim // 2}), got "
                          f"{tuple(s)} and {tuple(v_pages.shape)}")
-    if s[0] == 0 or s[2] < 16 or s[2] & (s[2] - 1):
-        raise ValueError(f"page_size must be a power of two from 16 and the pools not empty, got {tuple(s)}")
+    if s[0] == 0 or not 16 <= s[2] <= MAX_PAGE or s[2] & (s[2] - 1):
+        raise ValueError(f"page_size must be a power of two from 16 to {MAX_PAGE} and the pools not empty, got {tuple(s)}")
     size = head_dim // GROUP
     for name, x, dtype, last in (("k_pages", k_pages, torch.uint8, s[3]), ("v_pages", v_pages, torch.uint8, s[3]),
                                  ("k_scales", k_scales, torch.float16, size), ("v_scales", v_scales, torch.float16, size)):
@@ -125,8 +126,8 @@ def paged_append_4bit(key: Tensor, value: Tensor, k_pages: Tensor, v_pages: Tens
     or above ``T``, taken as 0 or ``T``).  32 dims with a NaN or an infinity
     among them read back as NaN; scales are limited to 65504.  ``key`` and
     ``value`` are CUDA tensors of one dtype (bfloat16, float16, float32),
-    head_dim 32, 64 or 128, any strides; page sizes are powers of two from 16,
-    and the slots of a page and head follow one another in the pools, from a
+    head_dim 32, 64 or 128, any strides; page sizes are powers of two from 16
+    (to 2^24), and the slots of a page and head follow one another in the pools, from a
     16-byte boundary (pages and heads may be strided).  Two tokens given the same
     slot race; no gradient flows through the cache."""
     tensors = (key, value, k_pages, v_pages, k_scales, v_scales, page_table, lens, new_lens)

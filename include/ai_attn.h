@@ -748,11 +748,12 @@ int ai_distill_bwd(const AiDistillBwdArgs* args, void* stream);
  * 8, j < 4) of a row lies in its byte g D / 16 + 2 c + j / 2, in the low half
  * for even j.  Strides of the pools are in elements (bytes, halfs); the slots
  * of a page and head follow one another, from a 16-byte boundary. */
+#define AI_POOL4_MAX_PAGE 16777216 /* slots of a page */
 typedef struct AiPool4 {
   AiTensor4 k_codes, v_codes;   /* (n_pages, Hkv, page_size, D / 2) uint8 */
   AiTensor4 k_scales, v_scales; /* (n_pages, Hkv, page_size, D / 32) fp16 */
   int32_t n_pages;
-  int32_t page_size;            /* a power of two from 16 */
+  int32_t page_size;            /* a power of two from 16 to AI_POOL4_MAX_PAGE */
   const int32_t* page_table;    /* [B][max_pages] */
   int64_t page_table_stride;
   int32_t max_pages;

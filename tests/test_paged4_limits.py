@@ -1,0 +1,49 @@
+"""The cache in 4 bits at the ends of what its calls take."""
+
+import ctypes
+
+import pytest
+import torch
+
+
+@pytest.mark.parametrize("D", [32, 64, 128])
+def test_the_largest_page(D):
+    """A slot lies at most 2^30 bytes behind its page's start."""
+    from autoindexer_b200 import _lib
+    from autoindexer_b200.paged4 import MAX_PAGE, _pool
+
+    def pool(size, p):
+        meta = dict(device="meta")
+        codes = torch.empty(1, 1, size, D // 2, dtype=torch.uint8, **meta)
+        scales = torch.empty(1, 1, size, D // 32, dtype=torch.float16, **meta)
+        table = torch.empty(1, 1, dtype=torch.int32, **meta)
+        return _pool(p, codes, codes, scales, scales, table, 1, 1, D, codes.get_device())
+
+    p = _lib.AiPool4()
+    pool(MAX_PAGE, p)
+    assert p.page_size == MAX_PAGE and (MAX_PAGE - 1) * D // 2 < 2 ** 30
+    with pytest.raises(ValueError, match="page_size must be a power of two from 16 to"):
+        pool(2 * MAX_PAGE, _lib.AiPool4())
+    a = _lib.AiPaged4Args()
+    a.batch = a.seq_len = a.num_kv_heads = 1
+    a.head_dim, a.dtype = D, _lib.DTYPE_BF16
+    a.k.ptr = a.v.ptr = a.lens = 256
+    for name in ("k_codes", "v_codes", "k_scales", "v_scales"):
+        t = getattr(p, name)
+        t.ptr = 256
+    p.page_table = 256
+    a.pool = p
+    a.pool.page_size = 2 * MAX_PAGE
+    L = _lib.lib()
+    for fn in (L.ai_paged_append_4bit, L.ai_paged_read_4bit):
+        assert fn(ctypes.byref(a), None) == 2
+    b = _lib.AiPagedAttn4Args()
+    b.batch = b.seq_len = b.num_q_heads = b.num_kv_heads = 1
+    b.head_dim, b.dtype, b.scale = D, _lib.DTYPE_BF16, 0.1
+    b.q.ptr = b.out.ptr = b.lens = 256
+    b.pool = p
+    n = ctypes.c_size_t(0)
+    assert L.ai_paged_attn_4bit_workspace(ctypes.byref(b), ctypes.byref(n)) == 0
+    b.pool.page_size = 2 * MAX_PAGE
+    assert L.ai_paged_attn_4bit_workspace(ctypes.byref(b), ctypes.byref(n)) == 2
+    assert L.ai_paged_attn_4bit(ctypes.byref(b), None) == 2
