@@ -322,7 +322,7 @@ __global__ void __launch_bounds__(32 * warps_of(NT), 1) split_kernel(const AiPag
     const int32_t* table = a.pool.page_table + ld.b * a.pool.page_table_stride + (key >> page_bits);
     page[0] = __ldg(table);
     page[1] = page[0];
-    if (page_bits == 4) page[1] = key + 16 < ld.keys ? __ldg(table + 1) : 0;
+    if (page_bits == 4) page[1] = ld.keys - key > 16 ? __ldg(table + 1) : 0;
   };
   auto enter = [&]() -> bool {  // the next stretch to load
     if (!next_seg(a, p, scan, wl, w1, ld)) return false;
@@ -343,7 +343,7 @@ __global__ void __launch_bounds__(32 * warps_of(NT), 1) split_kernel(const AiPag
   auto issue = [&]() {
     if (loads) {
       const int key = ld.tile * kKeys;
-      const bool both = key + 16 < ld.keys;
+      const bool both = ld.keys - key > 16;
       const uint32_t to = ring_at + at_stage * L::kBytes;
       // (here, not at the look-up: the ids have had a tile's time to arrive)
       if ((uint32_t)page[0] >= (uint32_t)a.pool.n_pages) report(a.status, AI_ERR_DEV_BOUNDS), page[0] = 0;
@@ -544,7 +544,7 @@ __global__ void __launch_bounds__(32 * warps_of(NT), 1) split_kernel(const AiPag
       }
       // The running maximum of each row, and of the V scales, lazily; masks where a
       // row does not see the whole tile.
-      const bool ragged = k0 + kKeys > least;
+      const bool ragged = least - k0 < kKeys;  // (lists end by 2^31: differences)
       float top[NT][2];
       auto tops = [&]() -> bool {
         bool move = false;
@@ -581,10 +581,9 @@ __global__ void __launch_bounds__(32 * warps_of(NT), 1) split_kernel(const AiPag
           for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-              const int key = k0 + 16 * mt + 8 * h + row_g;
 #pragma unroll
               for (int i = 0; i < H; ++i) {
-                if (key >= s.keys) vs[mt][h][i] = 0;  // (a slot that no one wrote)
+                if (16 * mt + 8 * h + row_g >= s.keys - k0) vs[mt][h][i] = 0;  // (a slot that no one wrote)
                 odd |= !__hble2(__habs2(as_half2(vs[mt][h][i])), as_half2(0x7bff7bffu));
               }
             }

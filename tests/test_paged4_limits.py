@@ -47,3 +47,34 @@ def test_the_largest_page(D):
     b.pool.page_size = 2 * MAX_PAGE
     assert L.ai_paged_attn_4bit_workspace(ctypes.byref(b), ctypes.byref(n)) == 2
     assert L.ai_paged_attn_4bit(ctypes.byref(b), None) == 2
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T", [1, 2])
+def test_the_longest_list(T, cuda_device):
+    """2^31 - 1 keys (the pages repeat): the one slot past them is not looked at."""
+    from autoindexer_b200 import paged_attention_4bit, read_status
+
+    D, S, keys = 32, 2 ** 20, 2 ** 31 - 1
+    g = torch.Generator().manual_seed(3)
+    codes = [torch.randint(0, 256, (2, 1, S, D // 2), generator=g, dtype=torch.uint8) for _ in range(2)]
+    scales = [0.05 + 0.2 * torch.rand(2, 1, S, 1, generator=g) for _ in range(2)]
+    cache = [x.to(cuda_device) for x in (*codes, *(x.half() for x in scales))]
+    for x in cache:
+        x[1] = x[0]
+    cache[2][1, 0, S - 1] = cache[3][1, 0, S - 1] = float("nan")
+    table = torch.zeros(1, keys // S + 1, dtype=torch.int32, device=cuda_device)
+    table[0, -1] = 1
+    q = (0.3 * torch.randn(1, 2, T, D, generator=g)).to(torch.bfloat16).to(cuda_device)
+    n = torch.tensor([keys], dtype=torch.int32, device=cuda_device)
+    out, lse = paged_attention_4bit(q, *cache, table, n, return_lse=True)
+    once, of_page = paged_attention_4bit(q, *cache, table[:, :1], torch.full_like(n, S), return_lse=True)
+    assert read_status(cuda_device) == 0
+    # A page 2048 times has the page's mean, and ln 2048 more; a key more or less changes 2^-20 of
+    # it.  (Two values that close, each rounded by half a step at most, are a step apart at most:
+    # bf16's step is 2^-7 of a value or less.)
+    assert bool(((out - once)[:, -1].abs() <= 2.0 ** -7 * once[:, -1].abs() + 1e-5).all())
+    more = torch.log(torch.tensor(2048.0)).item()
+    assert bool(((lse - of_page)[..., -1] - more).abs().le(1e-4).all())
+    if T > 1:
+        assert bool(out[:, 0].isfinite().all())
