@@ -15,6 +15,7 @@ sequences that share a prompt list the same pages.
 from __future__ import annotations
 
 import ctypes
+import operator
 from typing import Optional, Tuple
 
 import torch
@@ -148,13 +149,14 @@ def paged_read_4bit(k_pages: Tensor, v_pages: Tensor, k_scales: Tensor, v_scales
     mirrors ``paged_append_4bit``, with its arguments: what a prefill that wrote
     to the cache attends to, or a sequence on its way to another cache."""
     tensors = (k_pages, v_pages, k_scales, v_scales, page_table, lens, read_lens)
+    n_tokens = operator.index(n_tokens)  # (a number: a plan kept by a tensor would outlive its value)
     at = (*_call.sigs(tensors), n_tokens, dtype)
     known = _READ_PLANS.get(at)
     if known is None:
         if page_table.dim() != 2 or k_pages.dim() != 4 or n_tokens < 1:
             raise ValueError(f"page_table must be (B, max_pages), k_pages (n_pages, Hkv, page_size, D / 2), n_tokens 1 or more, "
                              f"got {tuple(page_table.shape)}, {tuple(k_pages.shape)}, {n_tokens}")
-        shape = (page_table.shape[0], k_pages.shape[1], int(n_tokens), 2 * k_pages.shape[3])
+        shape = (page_table.shape[0], k_pages.shape[1], n_tokens, 2 * k_pages.shape[3])
         given, like = tensors, torch.empty(shape, dtype=dtype, device=k_pages.device)
         (_, _, *tensors), plan = _paged_plan(like, like, *given, "read_lens")
         known = (shape, plan)

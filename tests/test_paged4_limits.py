@@ -78,3 +78,26 @@ def test_the_longest_list(T, cuda_device):
     assert bool(((lse - of_page)[..., -1] - more).abs().le(1e-4).all())
     if T > 1:
         assert bool(out[:, 0].isfinite().all())
+
+
+def test_n_tokens_is_a_whole_number():
+    from autoindexer_b200 import paged_read_4bit
+
+    cache = [torch.zeros(2, 1, 16, 16, dtype=torch.uint8)] * 2 + [torch.zeros(2, 1, 16, 1, dtype=torch.float16)] * 2
+    table, lens = torch.zeros(1, 1, dtype=torch.int32), torch.zeros(1, dtype=torch.int32)
+    for bad in (2.5, 2.0, "2", None, torch.tensor(2.0)):
+        with pytest.raises(TypeError):
+            paged_read_4bit(*cache, table, lens, bad, torch.bfloat16)
+
+
+@pytest.mark.gpu
+def test_n_tokens_of_a_tensor_that_changes(cuda_device):
+    from autoindexer_b200 import paged_read_4bit
+
+    cache = [torch.zeros(2, 1, 16, 16, dtype=torch.uint8, device=cuda_device)] * 2
+    cache += [torch.zeros(2, 1, 16, 1, dtype=torch.float16, device=cuda_device)] * 2
+    table, lens = (torch.zeros(*n, dtype=torch.int32, device=cuda_device) for n in ((1, 1), (1,)))
+    n = torch.tensor(3)
+    assert paged_read_4bit(*cache, table, lens, n, torch.bfloat16)[0].shape[2] == 3
+    n.fill_(5)
+    assert paged_read_4bit(*cache, table, lens, n, torch.bfloat16)[0].shape[2] == 5
