@@ -236,8 +236,8 @@ def paged_attention_4bit(query: Tensor, k_pages: Tensor, v_pages: Tensor, k_scal
         given = tensors
         tensors, plan = _attend_plan(*given, scaling)
         _ATTEND_PLANS.keep(at, given, tensors, plan)
-    if _call.tracked(query):
-        return _call.no_backward("paged_attention_4bit", lambda: _attend(plan, tensors, return_lse), query)
+    if _call.tracked(query, k_scales, v_scales):
+        return _call.no_backward("paged_attention_4bit", lambda: _attend(plan, tensors, return_lse), query, k_scales, v_scales)
     return _attend(plan, tensors, return_lse)
 
 

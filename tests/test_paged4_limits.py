@@ -101,3 +101,24 @@ def test_n_tokens_of_a_tensor_that_changes(cuda_device):
     assert paged_read_4bit(*cache, table, lens, n, torch.bfloat16)[0].shape[2] == 3
     n.fill_(5)
     assert paged_read_4bit(*cache, table, lens, n, torch.bfloat16)[0].shape[2] == 5
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("which", [2, 3])
+def test_scales_that_require_a_gradient(which, cuda_device):
+    """A backward that would reach them raises, as one to the query does."""
+    from autoindexer_b200 import paged_attention_4bit
+
+    cache = [torch.randint(0, 256, (2, 1, 16, 16), dtype=torch.uint8, device=cuda_device) for _ in range(2)]
+    cache += [torch.ones(2, 1, 16, 1, dtype=torch.float16, device=cuda_device) for _ in range(2)]
+    table, lens = (torch.full(n, 1, dtype=torch.int32, device=cuda_device) for n in ((1, 1), (1,)))
+    q = torch.randn(1, 2, 1, 32, device=cuda_device).bfloat16()
+    want = paged_attention_4bit(q, *cache, table, lens)
+    assert not want.requires_grad
+    cache[which].requires_grad_()
+    out = paged_attention_4bit(q, *cache, table, lens)
+    assert torch.equal(out, want)
+    with pytest.raises(RuntimeError, match="paged_attention_4bit has no backward"):
+        out.sum().backward()
+    with torch.no_grad():
+        assert not paged_attention_4bit(q, *cache, table, lens).requires_grad
