@@ -840,12 +840,6 @@ int check(const AiPagedAttn4Args* a) {
   return AI_OK;
 }
 
-int sm_count() {
-  int dev = 0, sms = 148;
-  if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-  return sms;
-}
-
 size_t layout(const AiPagedAttn4Args& a, Plan* p) {
   p->group = a.num_q_heads / a.num_kv_heads;
   p->rows = p->group * a.seq_len;

@@ -92,11 +92,6 @@ __device__ __forceinline__ float warp_max(float v) {
   return v;
 }
 
-// 2^((x - m) c), 0 for a masked logit and NaN for NaN and +inf (m may be -inf).
-__device__ __forceinline__ float share(float x, float c, float m) {
-  return x == -CUDART_INF_F ? 0.f : ptx::ex2((x - m) * c);
-}
-
 // What a backward of its own needs of a row.
 struct __align__(16) RowStats {
   float m, base;       // of the words that are not listed
@@ -220,7 +215,7 @@ __device__ __forceinline__ void weigh(const AiDistillArgs& a, List& list, Entrie
     if (32 * i >= K) continue;
     if (word[i] >= 0) p[i] = expf(logp[i]);
     p_top += p[i];
-    sum += share(xk[i], c, o);
+    sum += weight(xk[i], c, o);
     if (p[i] != 0.f) term += p[i] * logp[i] - scaled(xk[i] - o, p[i] * inv);  // (p / tau first: logits may be as far apart as fp32 goes)
     list.x[32 * i + lane] = xk[i];
     list.p[32 * i + lane] = p[i];
@@ -309,7 +304,7 @@ struct Totals {
   __device__ __forceinline__ float base(const List& list) const { return s == 0.f ? 0.f : mass * of_rest(list) / s_all - p_rest / s; }
   // Gradient of listed entry k.
   __device__ __forceinline__ float listed(const List& list, int k) const {
-    return empty ? 0.f : listed_gradient(list.up, mass, share(list.x[k], list.c, m_all) / s_all, list.p[k]);
+    return empty ? 0.f : listed_gradient(list.up, mass, weight(list.x[k], list.c, m_all) / s_all, list.p[k]);
   }
 };
 
@@ -668,7 +663,7 @@ __global__ void __launch_bounds__(kThreads, 4) distill_bwd_kernel(const AiDistil
   if (word >= 0) {
     for (int j = 0; j < tid; ++j)
       if (s_word[j] == word) return;
-    d[word] = from_f32<T>(st.s_all == 0.f ? 0.f : listed_gradient(up, st.mass, share(x, c, st.m_all) / st.s_all, p));
+    d[word] = from_f32<T>(st.s_all == 0.f ? 0.f : listed_gradient(up, st.mass, weight(x, c, st.m_all) / st.s_all, p));
   }
 }
 
@@ -687,12 +682,6 @@ int check(const AiDistillArgs* a) {
     return AI_ERR_ALIGN;
   if (reinterpret_cast<uintptr_t>(a->row_stats) & 15) return AI_ERR_ALIGN;
   return AI_OK;
-}
-
-int sm_count() {
-  int dev = 0, sms = 148;
-  if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-  return sms;
 }
 
 // CTAs of a row: what its slices ask for, and as many as give four CTAs per SM.

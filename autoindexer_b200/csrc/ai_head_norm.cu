@@ -267,12 +267,6 @@ int check_bwd(const AiHeadNormBwdArgs* g) {
   return AI_OK;
 }
 
-int sm_count() {
-  int dev = 0, sms = 148;
-  if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-  return sms;
-}
-
 // A token's heads are cut into items of whole unrolled row groups once there
 // are too few tokens for every SM to have a few warps of them; a long
 // sequence keeps a token's heads together (its angles are then read once).

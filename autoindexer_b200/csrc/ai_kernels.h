@@ -36,6 +36,13 @@ struct ProfScope {
   ~ProfScope() { prof_end(slot, st); }
 };
 
+// Multiprocessors of the current device.
+inline int sm_count() {
+  int dev = 0, sms = 148;
+  if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  return sms;
+}
+
 // Returns AI_OK or an AiStatus > 0; `cuda_err` receives the CUDA error of a failed launch.
 int sm100_fwd(const AiAttnFwdArgs& a, cudaStream_t st, cudaError_t* cuda_err);
 // Forward workspace after the rotated copies for the abs split: partial rows

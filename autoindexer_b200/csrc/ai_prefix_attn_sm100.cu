@@ -1226,12 +1226,6 @@ __global__ void __launch_bounds__(256) combine_kernel(const AiPrefixAttnArgs a, 
 }
 
 // ---------------------------------------------------------------- host
-int sm_count() {
-  int dev = 0, sms = 148;
-  if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-  return sms;
-}
-
 // Warps of a warp-kernel worker for units of `rows` rows.
 int warp_split(int64_t rows) { return rows <= 16 ? 1 : rows <= 32 ? 2 : 4; }
 

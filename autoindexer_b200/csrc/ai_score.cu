@@ -490,12 +490,6 @@ int check(const AiScoreArgs* a) {
   return AI_OK;
 }
 
-int sm_count() {
-  int dev = 0, sms = 148;
-  if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-  return sms;
-}
-
 // Slices of a row: CTAs for four per SM, at least kLeast logits each.
 int slices(const AiScoreArgs& a, int most) {
   const int64_t rows = (int64_t)a.batch * a.seq_len;

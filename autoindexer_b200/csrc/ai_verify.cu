@@ -433,12 +433,6 @@ int check(const AiVerifyArgs* a) {
   return AI_OK;
 }
 
-int sm_count() {
-  int dev = 0, sms = 148;
-  if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-  return sms;
-}
-
 // Slices of the vocabulary for `rows` rows: enough CTAs for four per SM (what
 // the registers of both kernels admit at once; 64 sequences of four drafts: 59 /
 // 51 / 54 us with 2 / 4 / 8), but at least `least` logits each.
