@@ -25,12 +25,14 @@
 //
 // HBM-bound when few rows meet each key: 144 bytes per token and KV head at D 128.
 // Measured (32 query heads, 8 KV heads of 128): 64 sequences of up to 8192 tokens, one
-// query token each, 73 us (4.1 TB/s); 32 of up to 32,768 125 us (4.7 TB/s): the 684
-// instructions a warp spends on a tile of 32 keys, issued in 65% of the cycles, bound
-// it together with the loads.  With up to five query tokens (20 rows to a KV head,
-// three column blocks) 152 us: eight warps an SM, as their sums fill the registers, do
-// not cover the latencies of 1070 instructions a tile.  4 sequences of 322 tokens 12.8
-// us: one tile's latency, a launch, and the second one's joining.
+// query token each, 76 us (4.0 TB/s); 32 of up to 32,768 130 us (4.5 TB/s).  Neither the
+// memory nor the issue slots are full (706 instructions a tile of 32 keys, issued in 67%
+// of the cycles): what is left are the waits within a warp's tile, scores, maximum, weights
+// and sums one after the other, which the 16 warps that the registers allow do not hide
+// from one another.  With up to five query tokens (20 rows to a KV head, three column
+// blocks) 153 us: eight warps an SM, as their sums take 255 registers, and 1070
+// instructions a tile, issued in 46%.  4 sequences of 322 tokens 13.5 us: one tile's
+// latency, a launch, and the second one's joining.
 
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>

@@ -784,8 +784,8 @@ int ai_paged_read_4bit(const AiPaged4Args* args, void* stream);
 /* Attention over such a cache: query token t < n_b = query_lens[b] of sequence
  * b sees the first lens[b] - n_b + t + 1 keys of its pages (lens counts the new
  * tokens, already appended).  Padding tokens (t >= n_b) and tokens without a
- * key give 0 (lse -inf).  Slots that no query of the sequence sees may hold
- * anything, also within a page. */
+ * key give 0 (lse -inf).  Padding tokens, and slots that no query of the sequence
+ * sees, may hold anything, also within a page. */
 typedef struct AiPagedAttn4Args {
   int32_t batch;              /* up to 1024 */
   int32_t seq_len;            /* T: query tokens per sequence */
