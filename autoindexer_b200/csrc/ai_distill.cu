@@ -240,7 +240,7 @@ __device__ __forceinline__ void weigh(const AiDistillArgs& a, List& list, Entrie
     if (rest <= lost) rest = 0.f;  // (NaN stays)
   }
   if (lane == 0) {
-    list.up = mine.wgt * inv;
+    list.up = over_tau(mine.wgt, inv);
     list.inv = inv;
     list.p_top = p_top;
     list.p_rest = rest;
@@ -646,7 +646,7 @@ __global__ void __launch_bounds__(kThreads, 4) distill_bwd_kernel(const AiDistil
     }
     s_word[tid] = word;
   }
-  const float c = slope(tau), up = wgt * inverse(tau);
+  const float c = slope(tau), up = over_tau(wgt, inverse(tau));
   const Dense dense(st.m, c, up, st.base);
   const bool alike = lie_alike(r.x, d);
   for (int i = sl.i0 + tid; i < sl.i1; i += kThreads * N) {

@@ -103,6 +103,14 @@ __device__ __forceinline__ float inverse(float tau) { return fminf(1.f / tau, FL
 // probability over tau, which may be 0 (an infinite temperature) or infinite.
 __device__ __forceinline__ float scaled(float d, float inv) { return d == 0.f || d == -CUDART_INF_F ? d : d * inv; }
 
+// A finite upstream gradient over tau, short of fp32's range by 2^12: what it meets,
+// weights of 0 among it, gives no NaN at the smallest temperatures.
+__device__ __forceinline__ float over_tau(float up, float inv) {
+  constexpr float kMost = FLT_MAX * 0x1p-12f;
+  const float x = up * inv;
+  return fabsf(x) > kMost && fabsf(up) < CUDART_INF_F ? copysignf(kMost, x) : x;
+}
+
 // 2^((x - m) c), 0 for a masked logit (m may be -inf then).
 __device__ __forceinline__ float weight(float x, float c, float m) {
   return x == -CUDART_INF_F ? 0.f : ptx::ex2((x - m) * c);

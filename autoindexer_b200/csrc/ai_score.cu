@@ -417,7 +417,7 @@ __global__ void __launch_bounds__(kThreads, 4) score_bwd_kernel(const AiScoreBwd
     return;
   }
   const float tau = row_tau(a.temperature, b, nullptr), c = slope(tau), inv = inverse(tau);
-  const float ca = -(up + gh * st.z) * inv, cb = -gh * kLn2 * inv;
+  const float ca = over_tau(-(up + gh * st.z), inv), cb = over_tau(-gh * kLn2, inv);
   auto dense = [&](float xv) {
     const float y = (xv - m) * c - l2;
     return ptx::ex2(y) * fmaf(cb, fmaxf(y, kNoWeight), ca);
@@ -473,7 +473,7 @@ __global__ void __launch_bounds__(kThreads, 4) score_bwd_kernel(const AiScoreBwd
         if (j < tid) first = false;
         sum += s_up[j];
       }
-    if (first) d[word] = from_f32<T>(fmaf(sum, inv, dense(at(x, word))));
+    if (first) d[word] = from_f32<T>(over_tau(sum, inv) + dense(at(x, word)));
   }
 }
 

@@ -81,3 +81,32 @@ def test_the_smallest_temperature(tail, cuda_device):
     losses, grad = distill_loss_and_grad(*(y.to(cuda_device) for y in (x, ids, t)), tail=tail,
                                          temperature=torch.full((2,), 1e-45, device=cuda_device))
     assert bool((losses.abs() <= 2.0 ** -19).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("tau", [1e-45, 1e-38, 1e-36, 1e-30])
+def test_gradients_at_small_temperatures(tau, dtype, cuda_device):
+    """Upstream gradients over tau may pass fp32's range; a row that is sure of its
+    word has the gradient 0 all the same."""
+    from autoindexer_b200 import distill_loss, distill_loss_and_grad, token_logprobs
+
+    V = 1003
+    x = torch.randn(3, V, generator=torch.Generator().manual_seed(1)).clamp(-2, 2)
+    x[0, 5], x[1, V - 1], x[2, 40] = 9.0, 8.0, 7.0
+    best = torch.tensor([5, V - 1, 40])
+    x, best = x.to(dtype).to(cuda_device), best.to(cuda_device)
+    t = torch.full((3,), tau, device=cuda_device)
+    for up in (1.0, -3.0, 1e6):
+        leaf = x.clone().requires_grad_()
+        got = token_logprobs(leaf, best, t, top_k=1, entropy=True)
+        d = torch.autograd.grad([got.logprobs, got.entropy, got.top_logprobs], leaf,
+                                [torch.full((3,), up, device=cuda_device), torch.full((3,), up, device=cuda_device),
+                                 torch.full((3, 1), up, device=cuda_device)])[0]
+        assert not bool(d.any()), (tau, up)
+        ids, lp = best[:, None], torch.zeros(3, 1, device=cuda_device)
+        w = torch.full((3,), up, device=cuda_device)
+        losses, grad = distill_loss_and_grad(x, ids, lp, w, t)
+        loss = distill_loss(leaf, ids, lp, t)
+        through = torch.autograd.grad(loss, leaf, w)[0]
+        assert not bool(grad.any()) and not bool(through.any()) and not bool(losses.any()) and torch.equal(loss, losses)
